@@ -90,9 +90,55 @@ class PostsynapticUpdateGroup(C.Structure):
                 ("rowLength", p_u32), ("ind", p_u32)]
 
 
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("rowStride", C.c_uint64), ("sequenceStride", C.c_uint64)]
+
+
+class Sequences(C.Structure):
+    _fields_ = [("count", C.c_uint32), ("length", C.c_uint32), ("offsets", p_u32), ("rows", C.c_uint64), ("slots", C.c_void_p),
+                ("numSlots", C.c_uint32), ("pad_", C.c_uint32)]
+
+
+class CausalConv(C.Structure):
+    _fields_ = [("sequences", Sequences), ("type", C.c_uint32), ("channels", C.c_uint32), ("taps", C.c_uint32), ("silu", C.c_uint32),
+                ("x", Rows), ("out", Rows), ("weight", p_f32), ("bias", p_f32), ("initialState", C.c_void_p), ("finalState", C.c_void_p)]
+
+
+class CausalConvGradient(C.Structure):
+    _fields_ = [("out", Rows), ("x", Rows), ("finalState", C.c_void_p), ("initialState", C.c_void_p), ("weight", p_f32), ("bias", p_f32)]
+
+
+class Scan(C.Structure):
+    _fields_ = [("sequences", Sequences), ("type", C.c_uint32), ("channels", C.c_uint32), ("states", C.c_uint32), ("groups", C.c_uint32),
+                ("softplus", C.c_uint32), ("pad_", C.c_uint32), ("u", Rows), ("delta", Rows), ("z", Rows), ("out", Rows), ("B", Rows), ("C", Rows),
+                ("A", p_f32), ("D", p_f32), ("deltaBias", p_f32), ("initialState", p_f32), ("finalState", p_f32)]
+
+
+class ScanGradient(C.Structure):
+    _fields_ = [("out", Rows), ("u", Rows), ("delta", Rows), ("z", Rows), ("B", Rows), ("C", Rows), ("finalState", p_f32),
+                ("initialState", p_f32), ("A", p_f32), ("D", p_f32), ("deltaBias", p_f32)]
+
+
+class AdamWSettings(C.Structure):
+    _fields_ = [("beta1", C.c_double), ("beta2", C.c_double), ("epsilon", C.c_double), ("stateBits", C.c_uint32), ("pad_", C.c_uint32)]
+
+
+class Parameter(C.Structure):
+    _fields_ = [("weight", C.c_void_p), ("gradient", C.c_void_p), ("copy", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("mScale", p_f32),
+                ("vScale", p_f32), ("count", C.c_uint64), ("weightType", C.c_uint32), ("gradientType", C.c_uint32), ("copyType", C.c_uint32),
+                ("pad_", C.c_uint32), ("weightDecay", C.c_double)]
+
+
+class AdamWStep(C.Structure):
+    _fields_ = [("rate", C.c_double), ("rateDevice", p_f32), ("gradientScale", p_f32), ("skip", p_u32)]
+
+
+OPERATOR_STRUCTS = (Rows, Sequences, CausalConv, CausalConvGradient, Scan, ScanGradient, AdamWSettings, Parameter, AdamWStep)
+
 INIT_SNIPPETS = {"Constant": 0, "Uniform": 1, "Normal": 2, "NormalClipped": 3, "NormalClippedDelay": 4, "Exponential": 5,
                  "Gamma": 6, "Binomial": 7}
 ELEMENT_TYPES = {"float32": 0, "uint32": 1, "int32": 2, "uint16": 3, "uint8": 4}
+FLOAT_TYPES = {"float32": 0, "float16": 5, "bfloat16": 6}           # element types of the operators on sequences and of the optimiser
 
 # every symbol include/genn_mi355x.h declares: (restype, argtypes)
 _ULL = C.c_ulonglong
@@ -185,6 +231,22 @@ SYMBOLS = {
     "gennmi_runner_stream_elapsed": (C.c_int, [C.c_void_p, C.POINTER(C.c_double)]),
     "gennmi_runner_get_info": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32 * 4)]),
     "gennmi_runner_event_count": (C.c_int, [C.c_void_p, C.POINTER(_ULL)]),
+    "gennmi_stream_is_capturing": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
+    "gennmi_causal_conv": (C.c_int, [C.POINTER(CausalConv), C.c_void_p]),
+    "gennmi_causal_conv_backward_workspace": (C.c_int, [C.POINTER(CausalConv), C.POINTER(C.c_size_t)]),
+    "gennmi_causal_conv_backward": (C.c_int, [C.POINTER(CausalConv), C.POINTER(CausalConvGradient), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gennmi_selective_scan_workspace": (C.c_int, [C.POINTER(Scan), C.POINTER(C.c_size_t)]),
+    "gennmi_selective_scan": (C.c_int, [C.POINTER(Scan), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gennmi_selective_scan_backward_workspace": (C.c_int, [C.POINTER(Scan), C.POINTER(C.c_size_t)]),
+    "gennmi_selective_scan_backward": (C.c_int, [C.POINTER(Scan), C.POINTER(ScanGradient), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gennmi_optimiser_create": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(AdamWSettings)]),
+    "gennmi_optimiser_destroy": (C.c_int, [C.c_void_p]),
+    "gennmi_optimiser_push": (C.c_int, [C.c_void_p, C.POINTER(Parameter), C.POINTER(C.c_uint32)]),
+    "gennmi_optimiser_finalise": (C.c_int, [C.c_void_p]),
+    "gennmi_optimiser_step": (C.c_int, [C.c_void_p, C.POINTER(AdamWStep), C.c_void_p]),
+    "gennmi_optimiser_get_step": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "gennmi_optimiser_set_step": (C.c_int, [C.c_void_p, C.c_uint64]),
+    "gennmi_abi_operator_sizes": (C.c_int, [C.POINTER(C.c_size_t * 9)]),
 }
 
 _lib = None

@@ -233,6 +233,7 @@ namespace gennmi_detail
 int fail(int code, const std::string &msg) { return ::fail(code, msg); }
 void noteDeviceWrite(const void *dev, size_t bytes) { ::noteDeviceWrite(dev, bytes); }
 int flushQueuedSteps() { return ::flushQueuedSteps(); }
+bool stepsQueued();                     // whether that would have anything to do (defined behind the programs)
 int prepareStaticScratch();             // looks up the current device's copy of the static counter array (defined with it)
 }
 
@@ -2734,3 +2735,5 @@ int gennmi_build_remap(uint32_t numSrc, uint32_t numTrg, uint32_t rowStride, uin
 
 // generated code objects behind the C ABI: gennmi_program_*
 #include "genn_mi355x_program.h"
+
+bool gennmi_detail::stepsQueued() { return g_programsPending.load(std::memory_order_relaxed) != 0 || g_queuedRunners.load(std::memory_order_relaxed) != 0; }

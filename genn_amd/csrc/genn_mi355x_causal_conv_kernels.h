@@ -1,0 +1,260 @@
+// Part of libgenn_mi355x.so: included by genn_mi355x_sequence.hip only.
+//
+// Short causal convolution of every channel by itself:  s[t] = bias + sum_k w[k] x[t - (K - 1) + k],  out = s or s sigmoid(s).
+// Bound by memory: 2 K + 6 operations for one element read and one written.  A thread owns a few neighbouring channels (VEC of
+// them, one access a row) and a chunk of rows, which it walks with the last K inputs in registers, so that a row is read once but for
+// the K - 1 rows before a chunk.
+#ifndef GENN_MI355X_CAUSAL_CONV_KERNELS_H
+#define GENN_MI355X_CAUSAL_CONV_KERNELS_H
+
+namespace
+{
+struct ConvArgs
+{
+    Sequences sequences;
+    gennmi_rows_t x, out;
+    const float *weight, *bias;
+    const void *initialState; void *finalState;
+    uint32_t channels, taps, silu, vectors;         // vectors: threads a row
+    uint32_t numbers;                               // chunk numbers
+};
+struct ConvGradientArgs
+{
+    gennmi_rows_t out, x;
+    const void *finalState; void *initialState;
+    float *partial;                 // [numbers][taps + 1][channels]: sums over a chunk for the weights and the bias; or NULL
+};
+
+__device__ inline float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f)); }
+
+template<typename T, int VEC> __device__ inline void loadRow(const T *from, float (&to)[VEC])
+{
+    const Pack<T, VEC> p = *(const Pack<T, VEC>*)from;
+    #pragma unroll
+    for(int v = 0; v < VEC; v++) { to[v] = widen(p.v[v]); }
+}
+template<typename T, int VEC> __device__ inline void storeRow(T *to, const float (&from)[VEC])
+{
+    Pack<T, VEC> p;
+    #pragma unroll
+    for(int v = 0; v < VEC; v++) { p.v[v] = narrow<T>(from[v]); }
+    *(Pack<T, VEC>*)to = p;
+}
+template<int K, int VEC> __device__ inline void loadWeights(const ConvArgs &a, uint32_t channel, float (&w)[K][VEC], float (&bias)[VEC])
+{
+    #pragma unroll
+    for(int v = 0; v < VEC; v++) {
+        bias[v] = a.bias ? a.bias[channel + v] : 0.0f;
+        #pragma unroll
+        for(int k = 0; k < K; k++) { w[k][v] = a.weight[(uint64_t)(channel + v) * K + k]; }
+    }
+}
+// The K - 1 rows before row `first` of the sequence, as window[1 ..]
+template<typename T, int K, int VEC>
+__device__ inline void loadWindow(const ConvArgs &a, const T *x, const Place &p, uint32_t first, uint32_t channel, float (&window)[K][VEC])
+{
+    const T *state = (const T*)a.initialState;
+    #pragma unroll
+    for(int j = 1; j < K; j++) {
+        #pragma unroll
+        for(int v = 0; v < VEC; v++) { window[j][v] = 0.0f; }
+        const long long t = (long long)first - (K - j);
+        if(t >= 0) { loadRow<T, VEC>(x + (uint64_t)t * a.x.rowStride + channel, window[j]); }
+        else if(state) { loadRow<T, VEC>(state + ((uint64_t)p.state * (K - 1) + (uint64_t)(K - 1 + t)) * a.channels + channel, window[j]); }
+    }
+}
+// The final state: rows length - (K - 1) .. length - 1, of which negative ones are the initial state's, still in the window of the first
+// chunk.  One thread reads what it needs of the initial state before it writes: the two may be the same array.
+template<typename T, int K, int VEC>
+__device__ inline void storeState(const ConvArgs &a, const T *x, const Place &p, uint32_t channel, const float (&window)[K][VEC])
+{
+    T *to = (T*)a.finalState + (uint64_t)p.state * (K - 1) * a.channels + channel;
+    #pragma unroll
+    for(int j = 1; j < K; j++) {
+        const long long t = (long long)p.length - (K - j);
+        float row[VEC];
+        if(t >= 0) { loadRow<T, VEC>(x + (uint64_t)t * a.x.rowStride + channel, row); }
+        else {
+            // row t lies -t rows before the first: window[K + t]
+            #pragma unroll
+            for(int i = 1; i < K; i++) {
+                #pragma unroll
+                for(int v = 0; v < VEC; v++) { row[v] = i == 1 || i == K + t ? window[i][v] : row[v]; }
+            }
+        }
+        storeRow<T, VEC>(to + (uint64_t)(j - 1) * a.channels, row);
+    }
+}
+
+template<int K, int VEC>
+__device__ inline void product(const float (&w)[K][VEC], const float (&window)[K][VEC], const float (&bias)[VEC], float (&s)[VEC])
+{
+    #pragma unroll
+    for(int v = 0; v < VEC; v++) {
+        s[v] = bias[v];
+        #pragma unroll
+        for(int k = 0; k < K; k++) { s[v] = __builtin_fmaf(w[k][v], window[k][v], s[v]); }
+    }
+}
+// One row on: what is at k + 1 moves to k
+template<int K, int VEC> __device__ inline void shift(float (&window)[K][VEC])
+{
+    #pragma unroll
+    for(int k = 0; k < K - 1; k++) {
+        #pragma unroll
+        for(int v = 0; v < VEC; v++) { window[k][v] = window[k + 1][v]; }
+    }
+}
+
+// (the chunk of a thread; lanes of a wavefront may lie in two chunks, so nothing here is uniform)
+__device__ inline bool convPlace(const ConvArgs &a, uint32_t number, Place &p)
+{
+    uint32_t sequence;
+    if(!a.sequences.offsets) {
+        sequence = number / a.sequences.perSequence;
+        p.index = number - sequence * a.sequences.perSequence;
+    }
+    else {
+        uint32_t low = 0, high = a.sequences.count;         // firstChunk(low) <= number
+        while(high - low > 1) {
+            const uint32_t middle = low + (high - low) / 2;
+            if(firstChunk(a.sequences, middle) <= number) { low = middle; } else { high = middle; }
+        }
+        sequence = low;
+        p.index = number - (uint32_t)firstChunk(a.sequences, sequence);
+    }
+    if(sequence >= a.sequences.count || !describe(a.sequences, sequence, p)) { return false; }
+    return (uint64_t)p.index * a.sequences.chunk < p.length || p.index == 0;
+}
+
+template<typename T, int K, int VEC>
+__global__ __launch_bounds__(256)
+void causalConvKernel(ConvArgs a)
+{
+    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t number = (uint32_t)(item / a.vectors);
+    if(number >= a.numbers) { return; }
+    const uint32_t channel = (uint32_t)(item - (uint64_t)number * a.vectors) * VEC;
+    Place p;
+    if(!convPlace(a, number, p)) { return; }
+    const T *x = rowsOf<const T>(a.x, a.sequences, p);
+    T *out = rowsOf<T>(a.out, a.sequences, p);
+    const uint32_t first = p.index * a.sequences.chunk, last = (uint32_t)min((uint64_t)first + a.sequences.chunk, (uint64_t)p.length);
+    float w[K][VEC], window[K][VEC], bias[VEC];
+    loadWindow<T, K, VEC>(a, x, p, first, channel, window);
+    if(K > 1 && p.index == 0 && a.finalState) { storeState<T, K, VEC>(a, x, p, channel, window); }
+    loadWeights<K, VEC>(a, channel, w, bias);
+    for(uint32_t t = first; t < last; t++) {
+        shift<K, VEC>(window);
+        loadRow<T, VEC>(x + (uint64_t)t * a.x.rowStride + channel, window[K - 1]);
+        float s[VEC];
+        product<K, VEC>(w, window, bias, s);
+        if(a.silu) {
+            #pragma unroll
+            for(int v = 0; v < VEC; v++) { s[v] *= sigmoid(s[v]); }
+        }
+        storeRow<T, VEC>(out + (uint64_t)t * a.out.rowStride + channel, s);
+    }
+}
+
+// Gradients.  With ds[t] = dout[t] f'(s[t]):  dx[p] = sum_k w[k] ds[p + (K - 1) - k], which is complete when ds[p + K - 1] is there, so a
+// thread walks K - 1 rows further than its chunk, with the last K inputs and the last K ds in registers, and writes row t - (K - 1)
+// at row t; in front of a sequence's first chunk these are the rows of the initial state.  dw[k] = sum ds[t] x[t - (K - 1) + k] and
+// dbias are summed over the chunk and then over chunks by a kernel of their own, always in the same order.
+template<typename T, int K, int VEC>
+__global__ __launch_bounds__(256)
+void causalConvBackwardKernel(ConvArgs a, ConvGradientArgs g)
+{
+    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t number = (uint32_t)(item / a.vectors);
+    if(number >= a.numbers) { return; }
+    const uint32_t channel = (uint32_t)(item - (uint64_t)number * a.vectors) * VEC;
+    float w[K][VEC], window[K][VEC], bias[VEC], ds[K][VEC], dw[K][VEC], db[VEC];
+    #pragma unroll
+    for(int v = 0; v < VEC; v++) {
+        db[v] = 0.0f;
+        #pragma unroll
+        for(int k = 0; k < K; k++) { dw[k][v] = ds[k][v] = 0.0f; }
+    }
+    Place p;
+    if(convPlace(a, number, p)) {
+        const T *x = rowsOf<const T>(a.x, a.sequences, p), *dout = rowsOf<const T>(g.out, a.sequences, p);
+        T *dx = g.x.data ? rowsOf<T>(g.x, a.sequences, p) : nullptr;
+        T *dstate = (T*)g.initialState;
+        const T *dfinal = (const T*)g.finalState;
+        const uint32_t first = p.index * a.sequences.chunk, last = (uint32_t)min((uint64_t)first + a.sequences.chunk, (uint64_t)p.length);
+        loadWindow<T, K, VEC>(a, x, p, first, channel, window);
+        loadWeights<K, VEC>(a, channel, w, bias);
+        // (dx of rows before `last`; in the first chunk of rows -(K - 1) on)
+        const long long from = p.index == 0 ? -(long long)(K - 1) : (long long)first;
+        for(uint64_t t = first; t < (uint64_t)last + (K - 1); t++) {
+            shift<K, VEC>(window);
+            shift<K, VEC>(ds);
+            if(t < p.length) {
+                loadRow<T, VEC>(x + t * a.x.rowStride + channel, window[K - 1]);
+                loadRow<T, VEC>(dout + t * g.out.rowStride + channel, ds[K - 1]);
+                if(a.silu) {
+                    float s[VEC];
+                    product<K, VEC>(w, window, bias, s);
+                    #pragma unroll
+                    for(int v = 0; v < VEC; v++) { const float q = sigmoid(s[v]); ds[K - 1][v] *= q * (1.0f + s[v] * (1.0f - q)); }
+                }
+                if(t < last) {
+                    #pragma unroll
+                    for(int v = 0; v < VEC; v++) {
+                        db[v] += ds[K - 1][v];
+                        #pragma unroll
+                        for(int k = 0; k < K; k++) { dw[k][v] = __builtin_fmaf(ds[K - 1][v], window[k][v], dw[k][v]); }
+                    }
+                }
+            }
+            else {
+                #pragma unroll
+                for(int v = 0; v < VEC; v++) { ds[K - 1][v] = 0.0f; }
+            }
+            const long long row = (long long)t - (K - 1);
+            if(row >= from) {
+                float d[VEC];
+                #pragma unroll
+                for(int v = 0; v < VEC; v++) {
+                    d[v] = 0.0f;
+                    #pragma unroll
+                    for(int k = 0; k < K; k++) { d[v] = __builtin_fmaf(w[k][v], ds[K - 1 - k][v], d[v]); }
+                }
+                const long long behind = row - ((long long)p.length - (K - 1));         // its place in the final state
+                if(dfinal && behind >= 0) {
+                    float f[VEC];
+                    loadRow<T, VEC>(dfinal + ((uint64_t)p.state * (K - 1) + (uint64_t)behind) * a.channels + channel, f);
+                    #pragma unroll
+                    for(int v = 0; v < VEC; v++) { d[v] += f[v]; }
+                }
+                if(row >= 0) { if(dx) { storeRow<T, VEC>(dx + (uint64_t)row * g.x.rowStride + channel, d); } }
+                else if(dstate) { storeRow<T, VEC>(dstate + ((uint64_t)p.state * (K - 1) + (uint64_t)(row + K - 1)) * a.channels + channel, d); }
+            }
+        }
+    }
+    if(g.partial) {
+        float *to = g.partial + (uint64_t)number * (K + 1) * a.channels + channel;
+        #pragma unroll
+        for(int v = 0; v < VEC; v++) {
+            #pragma unroll
+            for(int k = 0; k < K; k++) { to[(uint64_t)k * a.channels + v] = dw[k][v]; }
+            to[(uint64_t)K * a.channels + v] = db[v];
+        }
+    }
+}
+
+// Sums of the chunks, in 64 bits: there may be thousands, of either sign.
+__global__ __launch_bounds__(256)
+void causalConvReduceKernel(const float *partial, uint32_t numbers, uint32_t channels, uint32_t taps, float *weight, float *bias)
+{
+    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if(item >= (uint64_t)channels * (taps + 1)) { return; }
+    const uint32_t k = (uint32_t)(item / channels), c = (uint32_t)(item - (uint64_t)k * channels);
+    if(!(k < taps ? weight : bias)) { return; }
+    double sum = 0.0;
+    for(uint32_t n = 0; n < numbers; n++) { sum += partial[((uint64_t)n * (taps + 1) + k) * channels + c]; }
+    if(k < taps) { weight[(uint64_t)c * taps + k] = (float)sum; } else { bias[c] = (float)sum; }
+}
+}
+#endif

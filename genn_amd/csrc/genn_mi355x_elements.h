@@ -1,0 +1,177 @@
+// Part of libgenn_mi355x.so: element types, rows and sequences, as the operators' translation units share them.
+#ifndef GENN_MI355X_ELEMENTS_H
+#define GENN_MI355X_ELEMENTS_H
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "genn_mi355x.h"
+
+namespace gennmi_detail
+{
+// (defined beside the runner)
+int fail(int code, const std::string &msg);
+void noteDeviceWrite(const void *dev, size_t bytes);
+int flushQueuedSteps();
+bool stepsQueued();
+
+// What every operator does before it launches: steps queued in runners run first.  Under capture they cannot: their launches would
+// join the null stream's order, which a capture forbids.
+inline int beforeLaunch(hipStream_t stream)
+{
+    if(!stepsQueued()) { return GENNMI_OK; }
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if(stream && hipStreamIsCapturing(stream, &status) == hipSuccess && status != hipStreamCaptureStatusNone) {
+        return fail(GENNMI_ESTATE, "steps are queued in a runner while the stream is captured: call gennmi_flush before");
+    }
+    return flushQueuedSteps();
+}
+inline int afterLaunch(const char *what)
+{
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? GENNMI_OK : fail(GENNMI_EHIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+// An entry point's body: no C++ exception leaves the library
+template<typename F> int guarded(const char *what, F &&body)
+{
+    try { return body(); }
+    catch(const std::exception &e) { try { return fail(GENNMI_EHIP, std::string(what) + ": " + e.what()); } catch(...) { return GENNMI_EHIP; } }
+    catch(...) { return GENNMI_EHIP; }
+}
+}
+
+namespace gennmi_elements
+{
+// Types are converted by the hardware's instructions, to fewer bits with ties to even
+typedef __bf16 bf16;
+typedef _Float16 f16;
+template<typename T> __device__ inline float widen(T x) { return (float)x; }
+template<typename T> __device__ inline T narrow(float x) { return (T)x; }
+
+inline uint32_t sizeOf(uint32_t type) { return type == GENNMI_TYPE_F32 ? 4 : (type == GENNMI_TYPE_F16 || type == GENNMI_TYPE_BF16) ? 2 : 0; }
+
+// Calls f with a value of the element type, which picks the instance
+template<typename F> int withType(uint32_t type, F &&f)
+{
+    switch(type) {
+    case GENNMI_TYPE_F32: return f(float{});
+    case GENNMI_TYPE_F16: return f(f16{});
+    default: return f(bf16{});
+    }
+}
+
+// N neighbouring elements in one access
+template<typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+
+// Which rows a work-group owns.  Sequences are cut into chunks of `chunk` rows; a packed sequence's chunks are numbered from
+// offsets[s] / chunk + s, so that rows / chunk + count numbers do for any lengths, and every sequence (also one without rows) has one.
+struct Sequences
+{
+    const uint32_t *offsets;
+    const int32_t *slots;
+    uint64_t rows;
+    uint32_t count, length, numSlots, chunk, perSequence;      // perSequence: chunk numbers of a sequence that is not packed
+};
+struct Place
+{
+    uint64_t first;         // packed: the sequence's first row; else 0
+    uint32_t sequence, index, length;       // index: number of the chunk in its sequence
+    int32_t state;
+};
+__device__ inline uint64_t firstRow(const Sequences &s, uint32_t sequence)
+{
+    const uint64_t at = s.offsets[sequence];
+    return at < s.rows ? at : s.rows;
+}
+__device__ inline uint64_t firstChunk(const Sequences &s, uint32_t sequence)
+{
+    return s.offsets ? firstRow(s, sequence) / s.chunk + sequence : (uint64_t)sequence * s.perSequence;
+}
+// false: padding, nothing to do
+__device__ inline bool describe(const Sequences &s, uint32_t sequence, Place &p)
+{
+    p.sequence = sequence;
+    p.first = 0;
+    p.length = s.length;
+    if(s.offsets) {
+        p.first = firstRow(s, sequence);
+        const uint64_t end = firstRow(s, sequence + 1);
+        p.length = end > p.first ? (uint32_t)(end - p.first < s.length ? end - p.first : s.length) : 0;
+    }
+    p.state = s.slots ? s.slots[sequence] : (int32_t)sequence;
+    return !s.slots || (p.state >= 0 && (uint32_t)p.state < s.numSlots);
+}
+// The sequence that chunk number `number` belongs to (uniform over the wavefront); 64 candidates are looked at a time
+__device__ inline bool locate(const Sequences &s, uint32_t number, Place &p)
+{
+    uint32_t sequence;
+    if(!s.offsets) {
+        sequence = number / s.perSequence;
+        p.index = number - sequence * s.perSequence;
+    }
+    else {
+        const uint32_t lane = threadIdx.x & 63;
+        uint32_t low = 0, span = s.count;       // the answer is in low .. low + span - 1
+        while(span > 1) {
+            const uint32_t step = (span + 63) / 64;
+            const uint32_t candidate = low + lane * step;
+            const bool below = lane * step < span && firstChunk(s, candidate) <= number;
+            const uint64_t votes = __ballot(below);
+            const uint32_t last = votes ? 63 - __clzll((long long)votes) : 0;
+            low += last * step;
+            span = min(step, span - last * step);
+        }
+        sequence = __builtin_amdgcn_readfirstlane(low);
+        p.index = __builtin_amdgcn_readfirstlane(number - (uint32_t)firstChunk(s, sequence));
+    }
+    if(sequence >= s.count || !describe(s, sequence, p)) { return false; }
+    return (uint64_t)p.index * s.chunk < p.length || p.index == 0;
+}
+template<typename T> __device__ inline T *rowsOf(const gennmi_rows_t &r, const Sequences &s, const Place &p)
+{
+    return (T*)r.data + (s.offsets ? p.first * r.rowStride : (uint64_t)p.sequence * r.sequenceStride);
+}
+
+// host side
+inline int checkSequences(const char *what, const gennmi_sequences_t &s, bool gradients)
+{
+    using gennmi_detail::fail;
+    const std::string name(what);
+    if(s.slots && gradients) { return fail(GENNMI_EINVAL, name + ": slots are not for gradients"); }
+    if(s.count > (1u << 24) || s.length > 0x7fffffffu || (s.offsets ? s.rows : (uint64_t)s.count * s.length) > 0x7fffffffull) { return fail(GENNMI_EINVAL, name + ": more sequences or rows than the kernels number"); }
+    if(s.slots && s.numSlots == 0) { return fail(GENNMI_EINVAL, name + ": slots, but no states (numSlots is 0)"); }
+    if((uintptr_t)s.offsets % 4 || (uintptr_t)s.slots % 4) { return fail(GENNMI_EINVAL, name + ": offsets or slots not aligned"); }
+    return GENNMI_OK;
+}
+inline int checkRows(const char *what, const char *which, const gennmi_rows_t &r, const gennmi_sequences_t &s, uint32_t width, uint32_t size)
+{
+    using gennmi_detail::fail;
+    const std::string name = std::string(what) + ": " + which;
+    if(!(s.offsets ? s.rows : (uint64_t)s.count * s.length)) { return GENNMI_OK; }       // (nothing of it is touched)
+    if(!r.data) { return fail(GENNMI_EINVAL, name + " is missing"); }
+    if((uintptr_t)r.data % size) { return fail(GENNMI_EINVAL, name + " is not aligned to its elements"); }
+    if(s.length > 1 && r.rowStride < width) { return fail(GENNMI_EINVAL, name + ": rows overlap (rowStride)"); }
+    if(r.rowStride > (1ull << 40) || r.sequenceStride > (1ull << 50)) { return fail(GENNMI_EINVAL, name + ": stride out of range"); }
+    return GENNMI_OK;
+}
+// What is written: one row of a sequence and another must not share elements either
+inline int checkWrittenRows(const char *what, const char *which, const gennmi_rows_t &r, const gennmi_sequences_t &s, uint32_t width, uint32_t size)
+{
+    if(const int rc = checkRows(what, which, r, s, width, size)) { return rc; }
+    const bool overlap = s.count > 1 && (s.offsets ? r.rowStride < width : r.sequenceStride < width);
+    return overlap ? gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": " + which + ": sequences overlap") : GENNMI_OK;
+}
+inline void noteRows(const gennmi_rows_t &r, const gennmi_sequences_t &s, uint32_t width, uint32_t size)
+{
+    const uint64_t rows = s.offsets ? s.rows : s.length;
+    if(!r.data || !rows || !s.count) { return; }
+    const uint64_t last = (rows - 1) * r.rowStride + (s.offsets ? 0 : (s.count - 1) * r.sequenceStride);
+    gennmi_detail::noteDeviceWrite(r.data, (last + width) * size);
+}
+inline uint64_t statesOf(const gennmi_sequences_t &s) { return s.slots ? s.numSlots : s.count; }
+}
+
+#endif

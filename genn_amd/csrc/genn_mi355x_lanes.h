@@ -1,0 +1,34 @@
+// Part of libgenn_mi355x.so: exchanges between the lanes of a wavefront without a trip through LDS, shared by the operators' kernels.
+#ifndef GENN_MI355X_LANES_H
+#define GENN_MI355X_LANES_H
+
+#include <hip/hip_runtime.h>
+
+namespace gennmi_lanes
+{
+// The value of the lane's partner in the other half of its group of 2 WIDTH lanes.  Lane l's partner is l ^ WIDTH for WIDTH 1, 2, 16 and 32; for 4 and 8
+// it is the lane mirrored in the group: for sums and maxima one is as good as the other.
+template<int WIDTH> __device__ inline float partner(float x)
+{
+    const int v = __float_as_int(x);
+    if constexpr(WIDTH == 1) { return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, true)); }          // quad_perm [1, 0, 3, 2]
+    else if constexpr(WIDTH == 2) { return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, true)); }     // quad_perm [2, 3, 0, 1]
+    else if constexpr(WIDTH == 4) { return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true)); }    // row_half_mirror
+    else if constexpr(WIDTH == 8) { return __int_as_float(__builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true)); }    // row_mirror
+    else {
+        // (swaps the odd rows of 16 lanes, or the upper half, of its first operand with the even ones, or the lower half, of its second)
+        const auto s = [&] {
+            if constexpr(WIDTH == 16) { return __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false); }
+            else { return __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false); }
+        }();
+        return __int_as_float((int)((threadIdx.x & WIDTH) ? s[0] : s[1]));
+    }
+}
+template<int WIDTH = 32> __device__ inline float maxOfLanes(float x)
+{
+    x = fmaxf(x, partner<WIDTH>(x));
+    if constexpr(WIDTH > 1) { return maxOfLanes<WIDTH / 2>(x); }
+    return x;
+}
+}
+#endif

@@ -1,0 +1,383 @@
+// AdamW over many tensors in one launch, with states in 32 bits or in 8.
+//
+// Bound by memory: a weight is read and written with its gradient and states, 28 bytes in 32 bits with fp32 gradients, 16 in 8 bits, for some
+// 30 to 80 operations.  A work-group takes CHUNK neighbouring weights of one tensor (a table says which), four a lane in one access each.  In
+// 8 bits the 256 weights that share a scale are one wavefront's four a lane, so their maxima are found in registers and codes are written by the
+// pass that made the states.  The number of the step is the device's: the work-group that ends last counts it, so a captured step counts as well.
+#include <cmath>
+#include <new>
+#include <type_traits>
+#include <vector>
+
+#include "genn_mi355x_elements.h"
+#include "genn_mi355x_lanes.h"
+
+using namespace gennmi_elements;
+using gennmi_detail::fail;
+
+namespace
+{
+constexpr uint32_t CHUNK = 4096;        // weights of a work-group: a multiple of GENNMI_ADAMW_BLOCK * 4
+static_assert(GENNMI_ADAMW_BLOCK == 256, "a block is the four weights a lane of one wavefront");
+
+struct ParameterDev
+{
+    void *weight; const void *gradient; void *copy; void *m, *v; float *mScale, *vScale;
+    uint64_t count;
+    uint32_t weightType, gradientType, copyType, whole;         // whole: four neighbouring weights are one aligned access in every array
+    double weightDecay;
+};
+struct ChunkDev { uint32_t parameter, index; };
+// What the device knows of time: beta^t of the steps so far
+struct CounterDev { double power1, power2; unsigned long long step; uint32_t ended, pad; };
+
+struct StepArgs
+{
+    const ParameterDev *parameters; const ChunkDev *chunks; CounterDev *counter;
+    uint32_t numChunks, pad;
+    double beta1, beta2, rate;
+    float epsilon;
+    const float *rateDevice, *gradientScale; const uint32_t *skip;
+};
+
+template<typename T> __device__ inline void load4(const void *array, uint64_t at, uint32_t there, bool whole, float (&x)[4])
+{
+    const T *from = (const T*)array + at;
+    if(whole && there == 4) {
+        const Pack<T, 4> p = *(const Pack<T, 4>*)from;
+        #pragma unroll
+        for(int k = 0; k < 4; k++) { x[k] = widen(p.v[k]); }
+    }
+    else {
+        #pragma unroll
+        for(int k = 0; k < 4; k++) { x[k] = k < (int)there ? widen(from[k]) : 0.0f; }
+    }
+}
+__device__ inline void load4(const void *array, uint32_t type, uint64_t at, uint32_t there, bool whole, float (&x)[4])
+{
+    if(type == GENNMI_TYPE_F32) { load4<float>(array, at, there, whole, x); }
+    else if(type == GENNMI_TYPE_F16) { load4<f16>(array, at, there, whole, x); }
+    else { load4<bf16>(array, at, there, whole, x); }
+}
+template<typename T> __device__ inline void store4(void *array, uint64_t at, uint32_t there, bool whole, const float (&x)[4])
+{
+    T *to = (T*)array + at;
+    if(whole && there == 4) {
+        Pack<T, 4> p;
+        #pragma unroll
+        for(int k = 0; k < 4; k++) { p.v[k] = narrow<T>(x[k]); }
+        *(Pack<T, 4>*)to = p;
+    }
+    else {
+        #pragma unroll
+        for(int k = 0; k < 4; k++) { if(k < (int)there) { to[k] = narrow<T>(x[k]); } }
+    }
+}
+__device__ inline void store4(void *array, uint32_t type, uint64_t at, uint32_t there, bool whole, const float (&x)[4])
+{
+    if(type == GENNMI_TYPE_F32) { store4<float>(array, at, there, whole, x); }
+    else if(type == GENNMI_TYPE_F16) { store4<f16>(array, at, there, whole, x); }
+    else { store4<bf16>(array, at, there, whole, x); }
+}
+__device__ inline uint32_t loadCodes(const void *array, uint64_t at, uint32_t there, bool whole)
+{
+    const uint8_t *from = (const uint8_t*)array + at;
+    if(whole && there == 4) { return *(const uint32_t*)from; }
+    uint32_t codes = 0;
+    #pragma unroll
+    for(int k = 0; k < 4; k++) { if(k < (int)there) { codes |= (uint32_t)from[k] << (8 * k); } }
+    return codes;
+}
+__device__ inline void storeCodes(void *array, uint64_t at, uint32_t there, bool whole, uint32_t codes)
+{
+    uint8_t *to = (uint8_t*)array + at;
+    if(whole && there == 4) { *(uint32_t*)to = codes; }
+    else {
+        #pragma unroll
+        for(int k = 0; k < 4; k++) { if(k < (int)there) { to[k] = (uint8_t)(codes >> (8 * k)); } }
+    }
+}
+__device__ inline void decode(uint32_t codes, float (&c)[4])
+{
+    const auto low = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), high = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+    c[0] = low[0]; c[1] = low[1]; c[2] = high[0]; c[3] = high[1];
+}
+__device__ inline uint32_t encode(const float (&r)[4])
+{
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false), true);
+}
+// A 64-bit value in 24 bits such that rounding it once more, to fewer bits, gives what rounding the value itself would: the last bit is set
+// where the result is not exact (of the two neighbours the odd one)
+__device__ inline float roundToOdd(double r)
+{
+    const float f = (float)r;
+    const double off = r - (double)f;
+    const uint32_t bits = __float_as_uint(f);
+    if(off == 0.0 || off != off || (bits & 1)) { return f; }
+    return __uint_as_float((off > 0.0) == (r > 0.0) ? bits + 1 : bits - 1);
+}
+// 448 sqrt(v / V), ready to be rounded to e4m3: in 32 bits, and in 64 where that lies as near to the border between two codes as its error
+__device__ inline float scaledRoot(double v, float inverse, double V)
+{
+    const float r = 448.0f * __builtin_amdgcn_sqrtf((float)v * inverse);
+    // borders: halfway between neighbours of 4 bits' mantissa, or of multiples of 2^-9 below 2^-6
+    const uint32_t low = (__float_as_uint(r) & 0xfffffu) - 0x80000u + 16u;
+    const float t = r * 512.0f;
+    const bool near = r >= 0.015625f ? low < 32u : fabsf(t - floorf(t) - 0.5f) < 1e-4f;
+    return near && V > 0.0 ? roundToOdd(448.0 * sqrt(v / V)) : r;
+}
+
+template<bool EIGHT>
+__global__ __launch_bounds__(256)
+void adamwKernel(StepArgs a)
+{
+    if(a.skip && *a.skip) { return; }
+    const double power1 = a.counter->power1 * a.beta1, power2 = a.counter->power2 * a.beta2;
+    if(blockIdx.x < a.numChunks) {
+        const ChunkDev chunk = a.chunks[blockIdx.x];
+        const ParameterDev p = a.parameters[chunk.parameter];
+        const double rate = a.rateDevice ? (double)*a.rateDevice : a.rate;
+        const float scale = a.gradientScale ? *a.gradientScale : 1.0f;
+        const float keep = (float)(1.0 - rate * p.weightDecay), step = (float)rate;
+        const float correct1 = (float)(1.0 / (1.0 - power1)), correct2 = (float)(1.0 / (1.0 - power2));
+        const bool whole = p.whole;
+        for(uint32_t k = 0; k < CHUNK / 1024; k++) {
+            const uint64_t block = (uint64_t)chunk.index * (CHUNK / 256) + k * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            const uint64_t at = block * 256 + (threadIdx.x & 63) * 4;
+            if(block * 256 >= p.count) { break; }
+            const uint32_t there = at < p.count ? (uint32_t)(p.count - at < 4 ? p.count - at : 4) : 0;
+            float w[4], g[4], m[4], v[4];
+            load4(p.weight, p.weightType, at, there, whole, w);
+            load4(p.gradient, p.gradientType, at, there, whole, g);
+            #pragma unroll
+            for(int i = 0; i < 4; i++) { g[i] *= scale; }
+            if(!EIGHT) {
+                load4<float>(p.m, at, there, whole, m);
+                load4<float>(p.v, at, there, whole, v);
+                #pragma unroll
+                for(int i = 0; i < 4; i++) {
+                    m[i] = __builtin_fmaf((float)a.beta1, m[i], (float)(1.0 - a.beta1) * g[i]);
+                    v[i] = __builtin_fmaf((float)a.beta2, v[i], (float)(1.0 - a.beta2) * g[i] * g[i]);
+                }
+                store4<float>(p.m, at, there, whole, m);
+                store4<float>(p.v, at, there, whole, v);
+            }
+            else {
+                // In 64 bits (as fast here as 32): the codes are those of the formula, not of its rounding errors next to a border
+                decode(loadCodes(p.m, at, there, whole), m);
+                decode(loadCodes(p.v, at, there, whole), v);
+                const double unitM = (double)p.mScale[block] * (1.0 / 448.0), unitV = (double)p.vScale[block] * (1.0 / (448.0 * 448.0));
+                double m64[4], v64[4];
+                float mostM = 0.0f, mostV = 0.0f;
+                bool oddM = false, oddV = false;        // not a number somewhere: maxima pass those over
+                #pragma unroll
+                for(int i = 0; i < 4; i++) {
+                    const double gradient = g[i], c = v[i];
+                    m64[i] = __builtin_fma(a.beta1, (double)m[i] * unitM, (1.0 - a.beta1) * gradient);
+                    v64[i] = __builtin_fma(a.beta2, c * c * unitV, (1.0 - a.beta2) * gradient * gradient);
+                    m[i] = (float)m64[i];
+                    v[i] = (float)v64[i];
+                    mostM = fmaxf(mostM, fabsf(m[i]));
+                    mostV = fmaxf(mostV, v[i]);
+                    oddM = oddM || m[i] != m[i];
+                    oddV = oddV || v[i] != v[i];
+                }
+                mostM = gennmi_lanes::maxOfLanes(mostM);
+                mostV = gennmi_lanes::maxOfLanes(mostV);
+                if(__ballot(oddM)) { mostM = __builtin_nanf(""); }
+                if(__ballot(oddV)) { mostV = __builtin_nanf(""); }
+                const double inverseM = mostM > 0.0f ? 448.0 / (double)mostM : (double)mostM;
+                const float inverseV = mostV > 0.0f ? 1.0f / mostV : mostV;
+                float codesM[4], codesV[4];
+                #pragma unroll
+                for(int i = 0; i < 4; i++) {
+                    codesM[i] = roundToOdd(m64[i] * inverseM);
+                    codesV[i] = scaledRoot(v64[i], inverseV, (double)mostV);
+                    if(v64[i] > 0.0 && codesV[i] < 0.001953125f) { codesV[i] = 0.001953125f; }
+                }
+                storeCodes(p.m, at, there, whole, encode(codesM));
+                storeCodes(p.v, at, there, whole, encode(codesV));
+                if((threadIdx.x & 63) == 0) { p.mScale[block] = mostM; p.vScale[block] = mostV; }
+            }
+            #pragma unroll
+            for(int i = 0; i < 4; i++) {
+                const float change = m[i] * correct1 / (sqrtf(v[i] * correct2) + a.epsilon);
+                w[i] = __builtin_fmaf(-step, change, w[i] * keep);
+            }
+            store4(p.weight, p.weightType, at, there, whole, w);
+            if(p.copy) { store4(p.copy, p.copyType, at, there, whole, w); }
+        }
+    }
+    // (every work-group has read the powers before it is counted here)
+    __syncthreads();
+    if(threadIdx.x == 0 && atomicAdd(&a.counter->ended, 1u) == gridDim.x - 1) {
+        a.counter->ended = 0;
+        a.counter->power1 = power1;
+        a.counter->power2 = power2;
+        a.counter->step++;
+    }
+}
+
+}
+
+struct gennmi_optimiser
+{
+    gennmi_adamw_t settings{};
+    std::vector<gennmi_parameter_t> parameters;
+    std::vector<ParameterDev> table;
+    ParameterDev *dParameters = nullptr; ChunkDev *dChunks = nullptr; CounterDev *dCounter = nullptr;
+    uint32_t numChunks = 0;
+    bool finalised = false;
+    ~gennmi_optimiser() { (void)gennmi_free(dParameters); (void)gennmi_free(dChunks); (void)gennmi_free(dCounter); }
+};
+
+extern "C" {
+
+int gennmi_optimiser_create(gennmi_optimiser **optimiser, const gennmi_adamw_t *settings)
+{
+    return gennmi_detail::guarded("optimiser_create", [&] {
+        if(!optimiser || !settings) { return fail(GENNMI_EINVAL, "optimiser_create: null argument"); }
+        *optimiser = nullptr;
+        if(settings->stateBits != 8 && settings->stateBits != 32) { return fail(GENNMI_EUNSUPPORTED, "optimiser_create: states have 8 or 32 bits"); }
+        if(!(settings->beta1 >= 0.0 && settings->beta1 < 1.0 && settings->beta2 >= 0.0 && settings->beta2 < 1.0 && settings->epsilon >= 0.0 && std::isfinite(settings->epsilon))) {
+            return fail(GENNMI_EINVAL, "optimiser_create: needs 0 <= beta < 1 and epsilon >= 0");
+        }
+        gennmi_optimiser *o = new gennmi_optimiser;
+        o->settings = *settings;
+        *optimiser = o;
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_optimiser_destroy(gennmi_optimiser *optimiser)
+{
+    return gennmi_detail::guarded("optimiser_destroy", [&] { delete optimiser; return (int)GENNMI_OK; });
+}
+
+int gennmi_optimiser_push(gennmi_optimiser *optimiser, const gennmi_parameter_t *parameter, uint32_t *idx)
+{
+    return gennmi_detail::guarded("optimiser_push", [&] {
+        if(!optimiser || !parameter) { return fail(GENNMI_EINVAL, "optimiser_push: null argument"); }
+        if(optimiser->finalised) { return fail(GENNMI_ESTATE, "optimiser_push: the optimiser is finalised"); }
+        const gennmi_parameter_t &p = *parameter;
+        const bool eight = optimiser->settings.stateBits == 8;
+        const uint32_t weightSize = sizeOf(p.weightType), gradientSize = sizeOf(p.gradientType), copySize = p.copy ? sizeOf(p.copyType) : 2;
+        if(!weightSize || !gradientSize || copySize != 2) { return fail(GENNMI_EUNSUPPORTED, "optimiser_push: unknown element type"); }
+        if(p.count > (1ull << 40)) { return fail(GENNMI_EINVAL, "optimiser_push: number of weights"); }
+        if(p.count && (!p.weight || !p.gradient || !p.m || !p.v || (eight && (!p.mScale || !p.vScale)))) { return fail(GENNMI_EINVAL, "optimiser_push: an array is missing"); }
+        if((uintptr_t)p.weight % weightSize || (uintptr_t)p.gradient % gradientSize || (uintptr_t)p.copy % 2 ||
+           (!eight && ((uintptr_t)p.m % 4 || (uintptr_t)p.v % 4)) || (eight && ((uintptr_t)p.mScale % 4 || (uintptr_t)p.vScale % 4))) {
+            return fail(GENNMI_EINVAL, "optimiser_push: an array is not aligned to its elements");
+        }
+        if(!std::isfinite(p.weightDecay)) { return fail(GENNMI_EINVAL, "optimiser_push: weight decay"); }
+        // (two tensors that share weights or states would be updated twice, by work-groups that do not wait for one another)
+        const size_t stateSize = eight ? 1 : 4;
+        auto overlap = [](const void *a, size_t aBytes, const void *b, size_t bBytes) {
+            return (uintptr_t)a < (uintptr_t)b + bBytes && (uintptr_t)b < (uintptr_t)a + aBytes;
+        };
+        const struct { const void *ptr; size_t bytes; } mine[] = {{p.weight, p.count * weightSize}, {p.m, p.count * stateSize}, {p.v, p.count * stateSize},
+                                                                  {p.copy, p.copy ? p.count * 2 : 0}};
+        for(size_t i = 0; i < 4; i++) {
+            for(size_t j = 0; j < i; j++) {
+                if(overlap(mine[i].ptr, mine[i].bytes, mine[j].ptr, mine[j].bytes)) { return fail(GENNMI_EINVAL, "optimiser_push: weight, states and copy are arrays of their own"); }
+            }
+        }
+        for(const gennmi_parameter_t &q : optimiser->parameters) {
+            if(overlap(p.weight, p.count * weightSize, q.weight, q.count * sizeOf(q.weightType)) || overlap(p.m, p.count * stateSize, q.m, q.count * stateSize) ||
+               overlap(p.v, p.count * stateSize, q.v, q.count * stateSize)) {
+                return fail(GENNMI_EINVAL, "optimiser_push: overlaps a tensor that was pushed before");
+            }
+        }
+        ParameterDev d{p.weight, p.gradient, p.copy, p.m, p.v, p.mScale, p.vScale, p.count, p.weightType, p.gradientType, p.copyType, 0, p.weightDecay};
+        d.whole = (uintptr_t)p.weight % (4 * weightSize) == 0 && (uintptr_t)p.gradient % (4 * gradientSize) == 0 && (uintptr_t)p.copy % 8 == 0 &&
+                  (uintptr_t)p.m % (4 * stateSize) == 0 && (uintptr_t)p.v % (4 * stateSize) == 0;
+        optimiser->parameters.push_back(p);
+        optimiser->table.push_back(d);
+        if(idx) { *idx = (uint32_t)optimiser->parameters.size() - 1; }
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_optimiser_finalise(gennmi_optimiser *optimiser)
+{
+    return gennmi_detail::guarded("optimiser_finalise", [&] {
+        if(!optimiser) { return fail(GENNMI_EINVAL, "optimiser_finalise: null argument"); }
+        if(optimiser->finalised) { return fail(GENNMI_ESTATE, "optimiser_finalise: the optimiser is finalised"); }
+        std::vector<ChunkDev> chunks;
+        for(size_t k = 0; k < optimiser->table.size(); k++) {
+            const uint64_t of = (optimiser->table[k].count + CHUNK - 1) / CHUNK;
+            if(chunks.size() + of > 0x7fffffffull) { return fail(GENNMI_EINVAL, "optimiser_finalise: more weights than one launch covers"); }
+            for(uint64_t c = 0; c < of; c++) { chunks.push_back({(uint32_t)k, (uint32_t)c}); }
+        }
+        // (arrays of an earlier attempt that failed half-way are freed with the optimiser)
+        auto upload = [&](auto **to, const auto &from) {
+            if(const int rc = gennmi_malloc((void**)to, from.size() * sizeof(from[0]))) { return rc; }
+            return from.empty() ? (int)GENNMI_OK : gennmi_memcpy_to_device(*to, from.data(), from.size() * sizeof(from[0]));
+        };
+        if(!optimiser->dParameters) { if(const int rc = upload(&optimiser->dParameters, optimiser->table)) { return rc; } }
+        if(!optimiser->dChunks) { if(const int rc = upload(&optimiser->dChunks, chunks)) { return rc; } }
+        if(!optimiser->dCounter) { if(const int rc = upload(&optimiser->dCounter, std::vector<CounterDev>(1, CounterDev{1.0, 1.0, 0, 0, 0}))) { return rc; } }
+        optimiser->numChunks = (uint32_t)chunks.size();
+        optimiser->finalised = true;
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_optimiser_step(gennmi_optimiser *optimiser, const gennmi_adamw_step_t *step, void *stream)
+{
+    return gennmi_detail::guarded("optimiser_step", [&] {
+        if(!optimiser || !step) { return fail(GENNMI_EINVAL, "optimiser_step: null argument"); }
+        if(!optimiser->finalised) { return fail(GENNMI_ESTATE, "optimiser_step: the optimiser is not finalised"); }
+        if(!step->rateDevice && !std::isfinite(step->rate)) { return fail(GENNMI_EINVAL, "optimiser_step: learning rate"); }
+        for(const void *p : {(const void*)step->rateDevice, (const void*)step->gradientScale, (const void*)step->skip}) {
+            if((uintptr_t)p % 4) { return fail(GENNMI_EINVAL, "optimiser_step: a device value is not aligned"); }
+        }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        const gennmi_optimiser &o = *optimiser;
+        const StepArgs a{o.dParameters, o.dChunks, o.dCounter, o.numChunks, 0, o.settings.beta1, o.settings.beta2, step->rate, (float)o.settings.epsilon,
+                         step->rateDevice, step->gradientScale, step->skip};
+        const dim3 grid(o.numChunks ? o.numChunks : 1);
+        if(o.settings.stateBits == 8) { adamwKernel<true><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
+        else { adamwKernel<false><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
+        if(const int rc = gennmi_detail::afterLaunch("optimiser_step")) { return rc; }
+        for(const gennmi_parameter_t &p : o.parameters) {
+            if(p.count) { gennmi_detail::noteDeviceWrite(p.weight, p.count * sizeOf(p.weightType)); }
+        }
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_optimiser_get_step(gennmi_optimiser *optimiser, uint64_t *step)
+{
+    return gennmi_detail::guarded("optimiser_get_step", [&] {
+        if(!optimiser || !step) { return fail(GENNMI_EINVAL, "optimiser_get_step: null argument"); }
+        if(!optimiser->finalised) { return fail(GENNMI_ESTATE, "optimiser_get_step: the optimiser is not finalised"); }
+        if(const int rc = gennmi_synchronize()) { return rc; }
+        CounterDev counter;
+        if(const int rc = gennmi_memcpy_from_device(&counter, optimiser->dCounter, sizeof(counter))) { return rc; }
+        *step = counter.step;
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_optimiser_set_step(gennmi_optimiser *optimiser, uint64_t step)
+{
+    return gennmi_detail::guarded("optimiser_set_step", [&] {
+        if(!optimiser) { return fail(GENNMI_EINVAL, "optimiser_set_step: null argument"); }
+        if(!optimiser->finalised) { return fail(GENNMI_ESTATE, "optimiser_set_step: the optimiser is not finalised"); }
+        if(const int rc = gennmi_synchronize()) { return rc; }
+        const CounterDev counter{std::pow(optimiser->settings.beta1, (double)step), std::pow(optimiser->settings.beta2, (double)step), step, 0, 0};
+        return gennmi_memcpy_to_device(optimiser->dCounter, &counter, sizeof(counter));
+    });
+}
+
+int gennmi_abi_operator_sizes(size_t sizes[9])
+{
+    const size_t values[9] = {sizeof(gennmi_rows_t), sizeof(gennmi_sequences_t), sizeof(gennmi_causal_conv_t), sizeof(gennmi_causal_conv_gradient_t), sizeof(gennmi_scan_t),
+                              sizeof(gennmi_scan_gradient_t), sizeof(gennmi_adamw_t), sizeof(gennmi_parameter_t), sizeof(gennmi_adamw_step_t)};
+    if(!sizes) { return fail(GENNMI_EINVAL, "abi_operator_sizes: null result pointer"); }
+    for(int k = 0; k < 9; k++) { sizes[k] = values[k]; }
+    return GENNMI_OK;
+}
+
+}

@@ -1,0 +1,605 @@
+// Part of libgenn_mi355x.so: included by genn_mi355x_sequence.hip only.
+//
+// Selective state space scan.  A channel d drives N leaky units:
+//   h[t][n] = exp(dt A[n]) h[t - 1][n] + dt u B[t][n],   y = sum_n C[t][n] h[t][n] + D u,   out = y z sigmoid(z)
+// B and C are those of the channel's group.
+//
+// Layout: a lane is a channel, with NP of its states in registers, and walks rows one after another; a wavefront has 64 neighbouring
+// channels, so every access to a row of channels is one run of memory, sums over the states stay in a lane, and B and C are the same for all
+// lanes (staged in LDS in fp32, read as broadcasts).  More than NP states are the work of several wavefronts of a work-group, whose sums
+// over the states meet in LDS.  Where channels and sequences are too few to fill the chip, sequences are cut into chunks: one kernel
+// finds what each chunk adds to a state that comes in as zero (and the sum of dt, which says what becomes of one that does not), a second
+// walks over the chunks, and the third does the work from the right state.
+#ifndef GENN_MI355X_SCAN_KERNELS_H
+#define GENN_MI355X_SCAN_KERNELS_H
+
+namespace
+{
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+
+struct ScanArgs
+{
+    Sequences sequences;
+    gennmi_rows_t u, delta, z, out, B, C;
+    const float *A, *D, *deltaBias;
+    const float *initialState; float *finalState;
+    uint32_t channels, states, groups, softplus;
+    uint32_t groupChannels, groupTiles, tiles;      // channels of a group; tiles of 64 of them; of all groups
+    uint32_t numbers, slabs;                        // chunk numbers; wavefronts that share the states of a channel
+    float *chunkState;                              // [numbers][states][channels]: what a chunk adds, then the state it starts from; NULL: one chunk a sequence
+    float *chunkTime;                               // [numbers][channels]: sum of dt
+};
+struct ScanGradientArgs
+{
+    gennmi_rows_t out, u, delta, z, B, C;
+    const float *finalState; float *initialState;
+    float *chunkGradient;           // [numbers][states][channels]: what a chunk's rows give the state before it, then the gradient of the state behind it
+    float *sumA, *sumD, *sumBias;   // [numbers][states][channels], [numbers][slabs][channels] twice: sums over a chunk
+    float *sumBC;                   // [tiles][rows][2][states]: sums over a tile's channels, of B's gradient and of C's
+    uint64_t rows;                  // rows of sumBC
+};
+
+__device__ inline float exp2Of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float logistic(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2Of(x * -LOG2E)); }
+// log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|).  With f the rounded 1 + e, log(1 + e) = log(f) e / (f - 1) to the last bits,
+// also where e is small and f has lost most of it.
+__device__ inline float softplusOf(float x)
+{
+    const float e = exp2Of(fabsf(x) * -LOG2E), f = 1.0f + e, d = f - 1.0f;
+    const float tail = d == 0.0f ? e : __builtin_amdgcn_logf(f) * LN2 * (e * __builtin_amdgcn_rcpf(d));
+    return x != x ? x : fmaxf(x, 0.0f) + tail;
+}
+
+// Where a work-group is: a chunk and a tile of channels
+struct ScanPlace
+{
+    Place place;
+    uint32_t tile, group, channel, first, rows;     // first row of the chunk in its sequence, and how many
+    uint32_t firstState, numStates;                 // of the wavefront
+    bool valid, active;                             // there is a chunk; the lane has a channel (else it reads the last one's and writes nothing)
+};
+template<int NP> __device__ inline ScanPlace scanPlace(const ScanArgs &a, uint32_t &number)
+{
+    ScanPlace s;
+    number = blockIdx.x / a.tiles;
+    s.tile = blockIdx.x - number * a.tiles;
+    s.group = s.tile / a.groupTiles;
+    const uint32_t within = (s.tile - s.group * a.groupTiles) * 64 + (threadIdx.x & 63);
+    s.active = within < a.groupChannels;
+    s.channel = s.group * a.groupChannels + min(within, a.groupChannels - 1);
+    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    s.firstState = slab * NP;
+    s.numStates = min((uint32_t)NP, a.states - s.firstState);
+    s.valid = locate(a.sequences, number, s.place);
+    s.first = s.place.index * a.sequences.chunk;
+    s.rows = s.valid && s.place.length > s.first ? min(a.sequences.chunk, s.place.length - s.first) : 0;
+    return s;
+}
+
+// B and C of R rows, of a wavefront's states, in LDS as [row][B, C][NP], zero where there is no row or state.  A lane fetches
+// R * 2 * NP / 64 of the values, a block of rows before they are needed.
+template<typename T, int NP, int R> struct StagedBC
+{
+    static constexpr int EACH = R * 2 * NP / 64;
+    T raw[EACH];
+    __device__ inline void fetch(const T *B, const T *C, const ScanArgs &a, uint32_t row, uint32_t rows, uint32_t numStates)
+    {
+        const uint32_t lane = threadIdx.x & 63;
+        #pragma unroll
+        for(int q = 0; q < EACH; q++) {
+            const uint32_t e = q * 64 + lane, r = e / (2 * NP), n = e % NP;
+            const bool isC = (e / NP) & 1;
+            raw[q] = T(0.0f);
+            if(row + r < rows && n < numStates) { raw[q] = isC ? C[(uint64_t)(row + r) * a.C.rowStride + n] : B[(uint64_t)(row + r) * a.B.rowStride + n]; }
+        }
+    }
+    __device__ inline void store(float *lds) const
+    {
+        const uint32_t lane = threadIdx.x & 63;
+        #pragma unroll
+        for(int q = 0; q < EACH; q++) { lds[q * 64 + lane] = widen(raw[q]); }
+    }
+};
+// What one wavefront wrote to LDS is read by its other lanes: LDS accesses of a wavefront are done in order, only the compiler has to keep it
+__device__ inline void waveFence() { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); __builtin_amdgcn_wave_barrier(); }
+
+template<int NP> __device__ inline void loadA(const ScanArgs &a, const ScanPlace &s, float (&A)[NP])
+{
+    #pragma unroll
+    for(int n = 0; n < NP; n++) { A[n] = n < (int)s.numStates ? a.A[(uint64_t)s.channel * a.states + s.firstState + n] * LOG2E : 0.0f; }
+}
+template<int NP> __device__ inline void loadState(const ScanArgs &a, const ScanPlace &s, const float *state, uint64_t which, float (&h)[NP])
+{
+    #pragma unroll
+    for(int n = 0; n < NP; n++) {
+        h[n] = state && n < (int)s.numStates ? state[(which * a.channels + s.channel) * a.states + s.firstState + n] : 0.0f;
+    }
+}
+template<int NP> __device__ inline void storeState(const ScanArgs &a, const ScanPlace &s, float *state, uint64_t which, const float (&h)[NP])
+{
+    if(!state || !s.active) { return; }
+    #pragma unroll
+    for(int n = 0; n < NP; n++) {
+        if(n < (int)s.numStates) { state[(which * a.channels + s.channel) * a.states + s.firstState + n] = h[n]; }
+    }
+}
+template<int NP> __device__ inline void loadChunk(const ScanArgs &a, const ScanPlace &s, const float *chunks, uint32_t number, float (&h)[NP])
+{
+    #pragma unroll
+    for(int n = 0; n < NP; n++) { h[n] = n < (int)s.numStates ? chunks[((uint64_t)number * a.states + s.firstState + n) * a.channels + s.channel] : 0.0f; }
+}
+template<int NP> __device__ inline void storeChunk(const ScanArgs &a, const ScanPlace &s, float *chunks, uint32_t number, const float (&h)[NP])
+{
+    if(!s.active) { return; }
+    #pragma unroll
+    for(int n = 0; n < NP; n++) {
+        if(n < (int)s.numStates) { chunks[((uint64_t)number * a.states + s.firstState + n) * a.channels + s.channel] = h[n]; }
+    }
+}
+
+// First kernel of a split scan: every chunk from a state of zero.  With GRADIENT also sum_t (prod_{s <= t} exp(dt_s A)) C_t g_t, what the chunk's rows
+// give the gradient of the state before it.
+template<typename T, int NP, bool GRADIENT, bool SLABS>
+__global__ __launch_bounds__(SLABS ? 512 : 64)
+void scanChunkKernel(ScanArgs a, ScanGradientArgs g)
+{
+    constexpr int R = 8;
+    __shared__ float staged[SLABS ? 8 : 1][R * 2 * NP];
+    uint32_t number;
+    const ScanPlace s = scanPlace<NP>(a, number);
+    if(!s.valid) { return; }
+    float *const bc = staged[threadIdx.x >> 6];
+    const T *u = rowsOf<const T>(a.u, a.sequences, s.place) + s.channel, *delta = rowsOf<const T>(a.delta, a.sequences, s.place) + s.channel;
+    const uint32_t bcAt = s.group * a.states + s.firstState;
+    const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
+    const T *dout = GRADIENT ? rowsOf<const T>(g.out, a.sequences, s.place) + s.channel : nullptr;
+    const T *z = GRADIENT && a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) + s.channel : nullptr;
+    const float bias = a.deltaBias ? a.deltaBias[s.channel] : 0.0f;
+    float A[NP], h[NP], G[NP], P[NP], time = 0.0f;
+    loadA<NP>(a, s, A);
+    #pragma unroll
+    for(int n = 0; n < NP; n++) { h[n] = G[n] = 0.0f; P[n] = 1.0f; }
+    const uint32_t end = s.first + s.rows;
+    StagedBC<T, NP, R> next;
+    next.fetch(B, C, a, s.first, end, s.numStates);
+    for(uint32_t row = s.first; row < end; row += R) {
+        waveFence();
+        next.store(bc);
+        waveFence();
+        if(row + R < end) { next.fetch(B, C, a, row + R, end, s.numStates); }
+        T rawU[R], rawDelta[R], rawOut[R], rawZ[R];
+        #pragma unroll
+        for(int r = 0; r < R; r++) {
+            const uint64_t t = min(row + r, end - 1);
+            rawU[r] = u[t * a.u.rowStride];
+            rawDelta[r] = delta[t * a.delta.rowStride];
+            if(GRADIENT) {
+                rawOut[r] = dout[t * g.out.rowStride];
+                if(z) { rawZ[r] = z[t * a.z.rowStride]; }
+            }
+        }
+        #pragma unroll
+        for(int r = 0; r < R; r++) {
+            if(row + r >= end) { break; }
+            float dt = widen(rawDelta[r]) + bias;
+            if(a.softplus) { dt = softplusOf(dt); }
+            const float w = dt * widen(rawU[r]);
+            float gy = 0.0f;
+            if(GRADIENT) {
+                gy = widen(rawOut[r]);
+                if(z) { const float zr = widen(rawZ[r]); gy *= zr * logistic(zr); }
+            }
+            time += dt;
+            #pragma unroll
+            for(int n = 0; n < NP; n++) {
+                const float decay = exp2Of(dt * A[n]);
+                h[n] = __builtin_fmaf(decay, h[n], w * bc[r * 2 * NP + n]);
+                if(GRADIENT) {
+                    P[n] *= decay;
+                    G[n] = __builtin_fmaf(P[n], gy * bc[(r * 2 + 1) * NP + n], G[n]);
+                }
+            }
+        }
+    }
+    storeChunk<NP>(a, s, a.chunkState, number, h);
+    if(s.firstState == 0 && s.active) { a.chunkTime[(uint64_t)number * a.channels + s.channel] = time; }
+    if(GRADIENT) { storeChunk<NP>(a, s, g.chunkGradient, number, G); }
+}
+
+// Second kernel: a lane has one state of one channel of one sequence and walks over the chunks, leaving in each one's place the state it starts from,
+// and (GRADIENT) back again, leaving the gradient of the state behind each.
+template<bool GRADIENT>
+__global__ __launch_bounds__(64)
+void scanJoinKernel(ScanArgs a, ScanGradientArgs g)
+{
+    const uint32_t parts = (a.channels + 63) / 64;
+    const uint32_t part = blockIdx.x % parts, rest = blockIdx.x / parts;
+    const uint32_t n = rest % a.states, sequence = rest / a.states;
+    const uint32_t channel = part * 64 + threadIdx.x;
+    Place p;
+    if(!describe(a.sequences, sequence, p) || channel >= a.channels) { return; }
+    const uint64_t chunk0 = firstChunk(a.sequences, sequence);
+    const uint32_t chunks = max(1u, (uint32_t)(((uint64_t)p.length + a.sequences.chunk - 1) / a.sequences.chunk));
+    const float A = a.A[(uint64_t)channel * a.states + n] * LOG2E;
+    const uint64_t at = ((uint64_t)p.state * a.channels + channel) * a.states + n;
+    float *state = a.chunkState + (chunk0 * a.states + n) * a.channels + channel;
+    const float *time = a.chunkTime + chunk0 * a.channels + channel;
+    const uint64_t stride = (uint64_t)a.states * a.channels;
+    float h = a.initialState ? a.initialState[at] : 0.0f;
+    for(uint32_t c = 0; c < chunks; c++) {
+        const float adds = state[c * stride];
+        state[c * stride] = h;
+        h = __builtin_fmaf(exp2Of(time[(uint64_t)c * a.channels] * A), h, adds);
+    }
+    if(!GRADIENT) { if(a.finalState) { a.finalState[at] = h; } }
+    else {
+        float *gradient = g.chunkGradient + (chunk0 * a.states + n) * a.channels + channel;
+        float r = g.finalState ? g.finalState[at] : 0.0f;
+        for(uint32_t c = chunks; c-- > 0; ) {
+            const float adds = gradient[c * stride];
+            gradient[c * stride] = r;
+            r = __builtin_fmaf(exp2Of(time[(uint64_t)c * a.channels] * A), r, adds);
+        }
+        if(g.initialState) { g.initialState[at] = r; }
+    }
+}
+
+// Third kernel, or the only one: the outputs.
+template<typename T, int NP, bool SLABS>
+__global__ __launch_bounds__(SLABS ? 512 : 64)
+void scanKernel(ScanArgs a)
+{
+    constexpr int R = 8;
+    __shared__ float staged[SLABS ? 8 : 1][R * 2 * NP];
+    __shared__ float sums[SLABS ? 2 : 1][SLABS ? 8 : 1][SLABS ? R : 1][64];     // [alternating][slab][row][lane]
+    uint32_t number;
+    const ScanPlace s = scanPlace<NP>(a, number);
+    if(!s.valid) { return; }
+    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    float *const bc = staged[slab];
+    const T *u = rowsOf<const T>(a.u, a.sequences, s.place) + s.channel, *delta = rowsOf<const T>(a.delta, a.sequences, s.place) + s.channel;
+    const T *z = a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) + s.channel : nullptr;
+    T *out = rowsOf<T>(a.out, a.sequences, s.place) + s.channel;
+    const uint32_t bcAt = s.group * a.states + s.firstState;
+    const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
+    const float bias = a.deltaBias ? a.deltaBias[s.channel] : 0.0f, skip = a.D ? a.D[s.channel] : 0.0f;
+    float A[NP], h[NP];
+    loadA<NP>(a, s, A);
+    if(a.chunkState) { loadChunk<NP>(a, s, a.chunkState, number, h); } else { loadState<NP>(a, s, a.initialState, s.place.state, h); }
+    const uint32_t end = s.first + s.rows;
+    StagedBC<T, NP, R> next;
+    next.fetch(B, C, a, s.first, end, s.numStates);
+    uint32_t turn = 0;
+    for(uint32_t row = s.first; row < end; row += R, turn ^= 1) {
+        waveFence();
+        next.store(bc);
+        waveFence();
+        if(row + R < end) { next.fetch(B, C, a, row + R, end, s.numStates); }
+        T rawU[R], rawDelta[R], rawZ[R];
+        #pragma unroll
+        for(int r = 0; r < R; r++) {
+            const uint64_t t = min(row + r, end - 1);
+            rawU[r] = u[t * a.u.rowStride];
+            rawDelta[r] = delta[t * a.delta.rowStride];
+            if(z) { rawZ[r] = z[t * a.z.rowStride]; }
+        }
+        #pragma unroll
+        for(int r = 0; r < R; r++) {
+            if(row + r >= end) { break; }
+            float dt = widen(rawDelta[r]) + bias;
+            if(a.softplus) { dt = softplusOf(dt); }
+            const float w = dt * widen(rawU[r]);
+            float y = 0.0f, y1 = 0.0f;
+            #pragma unroll
+            for(int n = 0; n < NP; n++) {
+                const float decay = exp2Of(dt * A[n]);
+                h[n] = __builtin_fmaf(decay, h[n], w * bc[r * 2 * NP + n]);
+                if(n & 1) { y1 = __builtin_fmaf(h[n], bc[(r * 2 + 1) * NP + n], y1); } else { y = __builtin_fmaf(h[n], bc[(r * 2 + 1) * NP + n], y); }
+            }
+            y += y1;
+            if(SLABS) { sums[turn][slab][r][lane] = y; }
+            else if(s.active) {
+                y = __builtin_fmaf(skip, widen(rawU[r]), y);
+                if(z) { const float zr = widen(rawZ[r]); y *= zr * logistic(zr); }
+                out[(uint64_t)(row + r) * a.out.rowStride] = narrow<T>(y);
+            }
+        }
+        if(SLABS) {
+            __syncthreads();        // (the other half of `sums` is written next, so one barrier a block of rows does)
+            #pragma unroll
+            for(int r = 0; r < R; r++) {
+                if(row + r < end && r % a.slabs == slab && s.active) {
+                    float y = skip * widen(rawU[r]);
+                    for(uint32_t k = 0; k < a.slabs; k++) { y += sums[turn][k][r][lane]; }
+                    if(z) { const float zr = widen(rawZ[r]); y *= zr * logistic(zr); }
+                    out[(uint64_t)(row + r) * a.out.rowStride] = narrow<T>(y);
+                }
+            }
+        }
+    }
+    if(!a.chunkState) { storeState<NP>(a, s, a.finalState, s.place.state, h); }
+}
+
+// One row a sequence (a token): the states of a sequence's channel are neighbours in memory, and reading and writing them is all there is to it.
+// LANES lanes have four each; what they give the output is added up between them.
+template<typename T, int LANES, bool QUADS>
+__global__ __launch_bounds__(256)
+void scanTokenKernel(ScanArgs a)
+{
+    const uint64_t item = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+    const uint32_t part = threadIdx.x % LANES;
+    const uint32_t sequence = (uint32_t)(item / a.channels), channel = (uint32_t)(item - (uint64_t)sequence * a.channels);
+    Place p;
+    if(sequence >= a.sequences.count || !describe(a.sequences, sequence, p)) { return; }
+    const uint64_t at = ((uint64_t)p.state * a.channels + channel) * a.states;
+    const uint32_t n0 = part * 4;
+    float h[4];
+    #pragma unroll
+    for(int k = 0; k < 4; k++) { h[k] = 0.0f; }
+    if(a.initialState && n0 < a.states) {
+        if(QUADS) { *(float4*)h = *(const float4*)(a.initialState + at + n0); }
+        else {
+            #pragma unroll
+            for(int k = 0; k < 4; k++) { if(n0 + k < a.states) { h[k] = a.initialState[at + n0 + k]; } }
+        }
+    }
+    if(p.length) {          // (a packed sequence may have none)
+        const uint32_t group = channel / a.groupChannels;
+        const float u = widen(rowsOf<const T>(a.u, a.sequences, p)[channel]);
+        float dt = widen(rowsOf<const T>(a.delta, a.sequences, p)[channel]) + (a.deltaBias ? a.deltaBias[channel] : 0.0f);
+        if(a.softplus) { dt = softplusOf(dt); }
+        const T *B = rowsOf<const T>(a.B, a.sequences, p) + group * a.states, *C = rowsOf<const T>(a.C, a.sequences, p) + group * a.states;
+        const float *A = a.A + (uint64_t)channel * a.states;
+        float y = 0.0f;
+        #pragma unroll
+        for(int k = 0; k < 4; k++) {
+            if(n0 + k < a.states) {
+                h[k] = __builtin_fmaf(exp2Of(dt * (A[n0 + k] * LOG2E)), h[k], dt * u * widen(B[n0 + k]));
+                y = __builtin_fmaf(h[k], widen(C[n0 + k]), y);
+            }
+        }
+        #pragma unroll
+        for(int mask = 1; mask < LANES; mask *= 2) { y += __shfl_xor(y, mask); }
+        if(part == 0) {
+            if(a.D) { y = __builtin_fmaf(a.D[channel], u, y); }
+            if(a.z.data) { const float z = widen(rowsOf<const T>(a.z, a.sequences, p)[channel]); y *= z * logistic(z); }
+            rowsOf<T>(a.out, a.sequences, p)[channel] = narrow<T>(y);
+        }
+    }
+    if(a.finalState && n0 < a.states) {
+        if(QUADS) { *(float4*)(a.finalState + at + n0) = *(const float4*)h; }
+        else {
+            #pragma unroll
+            for(int k = 0; k < 4; k++) { if(n0 + k < a.states) { a.finalState[at + n0 + k] = h[k]; } }
+        }
+    }
+}
+
+// Sums over the 64 lanes of M values a lane, M = 64 / 2^k: in every step two values become one register, whose halves hold the two sums so far.
+// Afterwards lane l has the sum of value laneValue<M>(l) in v[0].
+template<int M> __device__ inline void sumLanes(float (&v)[M])
+{
+    const uint32_t lane = threadIdx.x & 63;
+    int width = 32;
+    #pragma unroll
+    for(int m = M; m > 1; m /= 2) {
+        const bool upper = lane & width;
+        #pragma unroll
+        for(int i = 0; i < m / 2; i++) {
+            const float keep = upper ? v[i + m / 2] : v[i], send = upper ? v[i] : v[i + m / 2];
+            v[i] = keep + __shfl_xor(send, width);
+        }
+        width /= 2;
+    }
+    for(; width >= 1; width /= 2) { v[0] += __shfl_xor(v[0], width); }
+}
+// which value that is: bit by bit, the highest lane bit chose between the two halves of the values
+template<int M> __device__ inline uint32_t laneValue()
+{
+    const uint32_t lane = threadIdx.x & 63;
+    return lane / (64 / M);
+}
+
+// Gradients of a chunk, from the state before it and the gradient of the state behind it.  The states in between are made again, a block of
+// R rows at a time: first one walk forward that keeps the state before every block (LDS), then from the last block to the first one walk
+// forward through a block that keeps its states in registers, and one back:
+//   dh = C gy + (what comes from the row behind);  dC = gy h, dB = dh dt u (summed over channels);  q = sum dh B, x = dh exp(dt A) h', r = sum x A
+//   du = dt q + D gy;  d(dt) = u q + r;  dA += x dt;  and exp(dt A) dh for the row before
+template<typename T, int NP, int R, int BLOCKS, bool SLABS>
+__global__ __launch_bounds__(SLABS ? 512 : 64)
+void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
+{
+    constexpr int WAVES = SLABS ? 8 : 1;
+    extern __shared__ float lds[];
+    uint32_t number;
+    const ScanPlace s = scanPlace<NP>(a, number);
+    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    float *const kept = lds + (size_t)slab * ((BLOCKS - 1) * NP * 64 + R * 2 * NP);     // [block][state][lane]
+    float *const bc = kept + (BLOCKS - 1) * NP * 64;
+    float *const sums = lds + (size_t)a.slabs * ((BLOCKS - 1) * NP * 64 + R * 2 * NP);  // SLABS: [slab][row][q, r, y][lane]
+    float A[NP], h[NP], carry[NP], dA[NP], dD = 0.0f, dBias = 0.0f;
+    #pragma unroll
+    for(int n = 0; n < NP; n++) { dA[n] = 0.0f; }
+    if(s.valid) {
+        const T *u = rowsOf<const T>(a.u, a.sequences, s.place) + s.channel, *delta = rowsOf<const T>(a.delta, a.sequences, s.place) + s.channel;
+        const T *z = a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) + s.channel : nullptr;
+        const T *dout = rowsOf<const T>(g.out, a.sequences, s.place) + s.channel;
+        const uint32_t bcAt = s.group * a.states + s.firstState;
+        const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
+        const float bias = a.deltaBias ? a.deltaBias[s.channel] : 0.0f, skip = a.D ? a.D[s.channel] : 0.0f;
+        const uint64_t sumRow = a.sequences.offsets ? s.place.first : (uint64_t)s.place.sequence * a.sequences.length;
+        loadA<NP>(a, s, A);
+        if(a.chunkState) { loadChunk<NP>(a, s, a.chunkState, number, h); loadChunk<NP>(a, s, g.chunkGradient, number, carry); }
+        else { loadState<NP>(a, s, a.initialState, s.place.state, h); loadState<NP>(a, s, g.finalState, s.place.state, carry); }
+        const uint32_t end = s.first + s.rows, blocks = (s.rows + R - 1) / R;
+        StagedBC<T, NP, R> stage;
+        for(uint32_t b = 0; b + 1 < blocks; b++) {
+            const uint32_t row = s.first + b * R;
+            #pragma unroll
+            for(int n = 0; n < NP; n++) { kept[(b * NP + n) * 64 + lane] = h[n]; }
+            stage.fetch(B, C, a, row, end, s.numStates);
+            waveFence();
+            stage.store(bc);
+            waveFence();
+            #pragma unroll
+            for(int r = 0; r < R; r++) {
+                float dt = widen(delta[(uint64_t)(row + r) * a.delta.rowStride]) + bias;
+                if(a.softplus) { dt = softplusOf(dt); }
+                const float w = dt * widen(u[(uint64_t)(row + r) * a.u.rowStride]);
+                #pragma unroll
+                for(int n = 0; n < NP; n++) { h[n] = __builtin_fmaf(exp2Of(dt * A[n]), h[n], w * bc[r * 2 * NP + n]); }
+            }
+        }
+        for(uint32_t b = blocks; b-- > 0; ) {
+            const uint32_t row = s.first + b * R;
+            if(b + 1 < blocks) {
+                #pragma unroll
+                for(int n = 0; n < NP; n++) { h[n] = kept[(b * NP + n) * 64 + lane]; }
+            }
+            stage.fetch(B, C, a, row, end, s.numStates);
+            waveFence();
+            stage.store(bc);
+            waveFence();
+            float hs[R][NP], dt[R], raw[R], uu[R], gy[R], zz[R], dd[R];
+            #pragma unroll
+            for(int r = 0; r < R; r++) {
+                // (rows behind the end, and lanes without a channel: dt, u and gradient 0 leave everything as it is)
+                const bool there = row + r < end && s.active;
+                const uint64_t t = min(row + r, end - 1);
+                raw[r] = widen(delta[t * a.delta.rowStride]) + bias;
+                dt[r] = there ? (a.softplus ? softplusOf(raw[r]) : raw[r]) : 0.0f;
+                uu[r] = there ? widen(u[t * a.u.rowStride]) : 0.0f;
+                dd[r] = there ? widen(dout[t * g.out.rowStride]) : 0.0f;
+                zz[r] = z && there ? widen(z[t * a.z.rowStride]) : 0.0f;
+                gy[r] = z ? dd[r] * zz[r] * logistic(zz[r]) : dd[r];
+                const float w = dt[r] * uu[r];
+                #pragma unroll
+                for(int n = 0; n < NP; n++) { hs[r][n] = __builtin_fmaf(exp2Of(dt[r] * A[n]), r ? hs[r - 1][n] : h[n], w * bc[r * 2 * NP + n]); }
+            }
+            #pragma unroll
+            for(int r = R - 1; r >= 0; r--) {
+                const float w = dt[r] * uu[r];
+                float q = 0.0f, rr = 0.0f, y = 0.0f, both[2 * NP];
+                #pragma unroll
+                for(int n = 0; n < NP; n++) {
+                    const float Bn = bc[r * 2 * NP + n], Cn = bc[(r * 2 + 1) * NP + n];
+                    const float decay = exp2Of(dt[r] * A[n]);
+                    const float dh = __builtin_fmaf(gy[r], Cn, carry[n]);
+                    y = __builtin_fmaf(Cn, hs[r][n], y);
+                    both[n] = dh * w;
+                    both[NP + n] = gy[r] * hs[r][n];
+                    q = __builtin_fmaf(dh, Bn, q);
+                    carry[n] = decay * dh;
+                    const float x = carry[n] * (r ? hs[r - 1][n] : h[n]);
+                    dA[n] = __builtin_fmaf(x, dt[r], dA[n]);
+                    rr = __builtin_fmaf(x, A[n], rr);
+                }
+                if(g.sumBC) {
+                    sumLanes<2 * NP>(both);
+                    const uint32_t value = laneValue<2 * NP>(), n = value % NP, which = value / NP;
+                    if(row + r < end && lane % (32 / NP) == 0 && n < s.numStates) {
+                        g.sumBC[(((uint64_t)s.tile * g.rows + sumRow + row + r) * 2 + which) * a.states + s.firstState + n] = both[0];
+                    }
+                }
+                if(SLABS) {
+                    sums[((slab * R + r) * 3) * 64 + lane] = q;
+                    sums[((slab * R + r) * 3 + 1) * 64 + lane] = rr;
+                    sums[((slab * R + r) * 3 + 2) * 64 + lane] = y;
+                }
+                else if(row + r < end && s.active) {
+                    const uint64_t t = row + r;
+                    if(g.u.data) { rowsOf<T>(g.u, a.sequences, s.place)[t * g.u.rowStride + s.channel] = narrow<T>(__builtin_fmaf(dt[r], q, skip * gy[r])); }
+                    float d = __builtin_fmaf(uu[r], q, rr * LN2);
+                    if(a.softplus) { d *= logistic(raw[r]); }
+                    if(g.delta.data) { rowsOf<T>(g.delta, a.sequences, s.place)[t * g.delta.rowStride + s.channel] = narrow<T>(d); }
+                    if(z && g.z.data) {
+                        const float sig = logistic(zz[r]);
+                        rowsOf<T>(g.z, a.sequences, s.place)[t * g.z.rowStride + s.channel] =
+                            narrow<T>(dd[r] * __builtin_fmaf(skip, uu[r], y) * (sig * (1.0f + zz[r] * (1.0f - sig))));
+                    }
+                    dBias += d;
+                    dD = __builtin_fmaf(gy[r], uu[r], dD);
+                }
+            }
+            if(SLABS) {
+                __syncthreads();
+                #pragma unroll
+                for(int r = 0; r < R; r++) {
+                    if(row + r < end && r % a.slabs == slab && s.active) {
+                        const uint64_t t = row + r;
+                        float q = 0.0f, rr = 0.0f, y = 0.0f;
+                        for(uint32_t k = 0; k < a.slabs; k++) {
+                            q += sums[((k * R + r) * 3) * 64 + lane];
+                            rr += sums[((k * R + r) * 3 + 1) * 64 + lane];
+                            y += sums[((k * R + r) * 3 + 2) * 64 + lane];
+                        }
+                        if(g.u.data) { rowsOf<T>(g.u, a.sequences, s.place)[t * g.u.rowStride + s.channel] = narrow<T>(__builtin_fmaf(dt[r], q, skip * gy[r])); }
+                        float d = __builtin_fmaf(uu[r], q, rr * LN2);
+                        if(a.softplus) { d *= logistic(raw[r]); }
+                        if(g.delta.data) { rowsOf<T>(g.delta, a.sequences, s.place)[t * g.delta.rowStride + s.channel] = narrow<T>(d); }
+                        if(z && g.z.data) {
+                            const float sig = logistic(zz[r]);
+                            rowsOf<T>(g.z, a.sequences, s.place)[t * g.z.rowStride + s.channel] =
+                                narrow<T>(dd[r] * __builtin_fmaf(skip, uu[r], y) * (sig * (1.0f + zz[r] * (1.0f - sig))));
+                        }
+                        dBias += d;
+                        dD = __builtin_fmaf(gy[r], uu[r], dD);
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        if(!a.chunkState) { storeState<NP>(a, s, g.initialState, s.place.state, carry); }
+    }
+    // (numbers without a chunk leave zeros)
+    if(g.sumA) { storeChunk<NP>(a, s, g.sumA, number, dA); }
+    if(s.active) {
+        const uint64_t at = ((uint64_t)number * a.slabs + slab) * a.channels + s.channel;
+        if(g.sumD) { g.sumD[at] = dD; }
+        if(g.sumBias) { g.sumBias[at] = dBias; }
+    }
+}
+
+// Sums over the chunks of what belongs to a channel, in 64 bits: out[channel][n] of sums[number][n][channel]
+__global__ __launch_bounds__(256)
+void scanChannelSumKernel(const float *sums, uint32_t numbers, uint32_t each, uint32_t channels, uint32_t width, float *out)
+{
+    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if(item >= (uint64_t)channels * width) { return; }
+    const uint32_t n = (uint32_t)(item / channels), c = (uint32_t)(item - (uint64_t)n * channels);
+    double sum = 0.0;
+    for(uint64_t k = 0; k < (uint64_t)numbers * each; k++) { sum += sums[(k * width + n) * channels + c]; }
+    out[(uint64_t)c * width + n] = (float)sum;
+}
+// Sums over a group's tiles of what belongs to a row
+template<typename T>
+__global__ __launch_bounds__(256)
+void scanRowSumKernel(ScanArgs a, ScanGradientArgs g)
+{
+    const uint32_t width = a.groups * a.states;
+    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t row = item / (2 * width);
+    if(row >= g.rows) { return; }
+    const uint32_t e = (uint32_t)(item - row * 2 * width), which = e / width, group = (e - which * width) / a.states, n = e % a.states;
+    uint32_t sequence = 0;
+    uint64_t t = row;
+    if(!a.sequences.offsets) { sequence = (uint32_t)(row / a.sequences.length); t = row - (uint64_t)sequence * a.sequences.length; }
+    else {
+        // rows of no sequence (in front of the first, behind one that was cut, behind the last) are left as they were
+        uint32_t low = 0, high = a.sequences.count;
+        while(high - low > 1) {
+            const uint32_t middle = low + (high - low) / 2;
+            if(firstRow(a.sequences, middle) <= row) { low = middle; } else { high = middle; }
+        }
+        Place p;
+        if(!describe(a.sequences, low, p) || row < p.first || row - p.first >= p.length) { return; }
+    }
+    float sum = 0.0f;
+    for(uint32_t k = 0; k < a.groupTiles; k++) { sum += g.sumBC[(((uint64_t)(group * a.groupTiles + k) * g.rows + row) * 2 + which) * a.states + n]; }
+    const gennmi_rows_t &to = which ? g.C : g.B;
+    if(!to.data) { return; }
+    T *at = (T*)to.data + (a.sequences.offsets ? row * to.rowStride : (uint64_t)sequence * to.sequenceStride + t * to.rowStride);
+    at[group * a.states + n] = narrow<T>(sum);
+}
+}
+#endif

@@ -1,0 +1,455 @@
+// Operators on sequences: a short causal convolution and a selective state space scan, with their gradients, for whole sequences and for
+// single tokens.  Entry points and their checks; the kernels are in the headers included below.
+#include "genn_mi355x_elements.h"
+
+using namespace gennmi_elements;
+using gennmi_detail::fail;
+
+#include "genn_mi355x_causal_conv_kernels.h"
+#include "genn_mi355x_scan_kernels.h"
+
+namespace
+{
+Sequences sequencesOf(const gennmi_sequences_t &s, uint32_t chunk)
+{
+    Sequences d{};
+    d.offsets = s.offsets;
+    d.slots = s.slots;
+    d.rows = s.rows;
+    d.count = s.count;
+    d.length = s.length;
+    d.numSlots = s.numSlots;
+    d.chunk = chunk;
+    d.perSequence = std::max(1u, (s.length + chunk - 1) / chunk);
+    return d;
+}
+// Chunk numbers: see Sequences
+uint64_t chunkNumbers(const gennmi_sequences_t &s, uint32_t chunk)
+{
+    return s.offsets ? s.rows / chunk + s.count : (uint64_t)s.count * std::max(1u, (s.length + chunk - 1) / chunk);
+}
+uint64_t totalRows(const gennmi_sequences_t &s) { return s.offsets ? s.rows : (uint64_t)s.count * s.length; }
+constexpr uint64_t MOST_BLOCKS = 0x7fffffffull;
+
+// ---- causal convolution
+constexpr uint32_t CONV_ROWS = 16;          // rows of a chunk; at least taps - 1, which only the first chunk then reads of the initial state
+
+int checkConv(const char *what, const gennmi_causal_conv_t *c, bool gradients)
+{
+    if(!c) { return fail(GENNMI_EINVAL, std::string(what) + ": null descriptor"); }
+    const std::string name(what);
+    const uint32_t size = sizeOf(c->type);
+    if(!size) { return fail(GENNMI_EUNSUPPORTED, name + ": unknown element type"); }
+    if(c->taps < 1 || c->taps > GENNMI_MAX_TAPS) { return fail(GENNMI_EUNSUPPORTED, name + ": number of taps"); }
+    if(c->channels < 1 || c->channels > (1u << 24)) { return fail(GENNMI_EINVAL, name + ": number of channels"); }
+    if(const int rc = checkSequences(what, c->sequences, gradients)) { return rc; }
+    if(const int rc = checkRows(what, "x", c->x, c->sequences, c->channels, size)) { return rc; }
+    if(!gradients) {
+        if(const int rc = checkWrittenRows(what, "out", c->out, c->sequences, c->channels, size)) { return rc; }
+        if(c->out.data && c->out.data == c->x.data) { return fail(GENNMI_EINVAL, name + ": out and x are the same array"); }
+    }
+    if(!c->weight || (uintptr_t)c->weight % 4 || (uintptr_t)c->bias % 4) { return fail(GENNMI_EINVAL, name + ": weight is missing, or weight or bias not aligned"); }
+    if((uintptr_t)c->initialState % size || (uintptr_t)c->finalState % size) { return fail(GENNMI_EINVAL, name + ": a state is not aligned to its elements"); }
+    return GENNMI_OK;
+}
+// Channels of a thread: four where every row and state of them is one aligned access, else one
+uint32_t convVector(const gennmi_causal_conv_t &c, const gennmi_causal_conv_gradient_t *g)
+{
+    const uint32_t bytes = 4 * sizeOf(c.type);
+    bool whole = c.channels % 4 == 0;
+    auto rows = [&](const gennmi_rows_t &r) { whole = whole && (uintptr_t)r.data % bytes == 0 && r.rowStride % 4 == 0 && r.sequenceStride % 4 == 0; };
+    auto array = [&](const void *p) { whole = whole && (uintptr_t)p % bytes == 0; };
+    rows(c.x);
+    array(c.initialState);
+    if(g) { rows(g->out); rows(g->x); array(g->initialState); array(g->finalState); }
+    else { rows(c.out); array(c.finalState); }
+    return whole ? 4 : 1;
+}
+// (a single row needs no chunks, and the whole of a shorter sequence is one)
+uint32_t convChunk(const gennmi_causal_conv_t &) { return CONV_ROWS; }
+ConvArgs convArgs(const gennmi_causal_conv_t &c, uint32_t vector)
+{
+    ConvArgs a{};
+    const uint32_t chunk = convChunk(c);
+    a.sequences = sequencesOf(c.sequences, chunk);
+    a.x = c.x;
+    a.out = c.out;
+    a.weight = c.weight;
+    a.bias = c.bias;
+    a.initialState = c.initialState;
+    a.finalState = c.finalState;
+    a.channels = c.channels;
+    a.taps = c.taps;
+    a.silu = c.silu;
+    a.vectors = c.channels / vector;
+    a.numbers = (uint32_t)chunkNumbers(c.sequences, chunk);
+    return a;
+}
+template<typename T, int VEC> void launchConv(const ConvArgs &a, const ConvGradientArgs *g, dim3 grid, hipStream_t stream)
+{
+    switch(a.taps) {
+#define TAPS(K) case K: if(g) { causalConvBackwardKernel<T, K, VEC><<<grid, dim3(256), 0, stream>>>(a, *g); } \
+                        else { causalConvKernel<T, K, VEC><<<grid, dim3(256), 0, stream>>>(a); } break;
+    TAPS(1) TAPS(2) TAPS(3) TAPS(4) TAPS(5) TAPS(6) TAPS(7) TAPS(8)
+#undef TAPS
+    }
+}
+int runConv(const char *what, const gennmi_causal_conv_t &c, uint32_t vector, const ConvGradientArgs *g, hipStream_t stream)
+{
+    const ConvArgs a = convArgs(c, vector);
+    const uint64_t blocks = ((uint64_t)a.numbers * a.vectors + 255) / 256;
+    if(chunkNumbers(c.sequences, convChunk(c)) > MOST_BLOCKS || blocks > MOST_BLOCKS) { return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers"); }
+    if(!blocks) { return GENNMI_OK; }
+    return withType(c.type, [&](auto t) {
+        if(vector == 4) { launchConv<decltype(t), 4>(a, g, dim3((uint32_t)blocks), stream); } else { launchConv<decltype(t), 1>(a, g, dim3((uint32_t)blocks), stream); }
+        return gennmi_detail::afterLaunch(what);
+    });
+}
+size_t convWorkspace(const gennmi_causal_conv_t &c) { return (size_t)chunkNumbers(c.sequences, convChunk(c)) * (c.taps + 1) * c.channels * sizeof(float); }
+
+// ---- selective scan
+int checkScan(const char *what, const gennmi_scan_t *c, bool gradients)
+{
+    if(!c) { return fail(GENNMI_EINVAL, std::string(what) + ": null descriptor"); }
+    const std::string name(what);
+    const uint32_t size = sizeOf(c->type);
+    if(!size) { return fail(GENNMI_EUNSUPPORTED, name + ": unknown element type"); }
+    if(c->states < 1 || c->states > GENNMI_MAX_SCAN_STATES) { return fail(GENNMI_EUNSUPPORTED, name + ": number of states"); }
+    if(c->channels < 1 || c->channels > (1u << 24) || c->groups < 1 || c->channels % c->groups) { return fail(GENNMI_EINVAL, name + ": number of channels or groups"); }
+    if(const int rc = checkSequences(what, c->sequences, gradients)) { return rc; }
+    if(const int rc = checkRows(what, "u", c->u, c->sequences, c->channels, size)) { return rc; }
+    if(const int rc = checkRows(what, "delta", c->delta, c->sequences, c->channels, size)) { return rc; }
+    if(const int rc = checkRows(what, "B", c->B, c->sequences, c->groups * c->states, size)) { return rc; }
+    if(const int rc = checkRows(what, "C", c->C, c->sequences, c->groups * c->states, size)) { return rc; }
+    if(c->z.data) { if(const int rc = checkRows(what, "z", c->z, c->sequences, c->channels, size)) { return rc; } }
+    if(!gradients) {
+        if(const int rc = checkWrittenRows(what, "out", c->out, c->sequences, c->channels, size)) { return rc; }
+        for(const void *p : {c->u.data, c->delta.data, c->z.data, c->B.data, c->C.data}) {
+            if(p && p == c->out.data) { return fail(GENNMI_EINVAL, name + ": out is an array of its own"); }
+        }
+    }
+    if(!c->A) { return fail(GENNMI_EINVAL, name + ": A is missing"); }
+    for(const void *p : {(const void*)c->A, (const void*)c->D, (const void*)c->deltaBias, (const void*)c->initialState, (const void*)c->finalState}) {
+        if((uintptr_t)p % 4) { return fail(GENNMI_EINVAL, name + ": an array of fp32 is not aligned"); }
+    }
+    return GENNMI_OK;
+}
+
+struct ScanPlan { uint32_t slab, slabs, chunk; bool split; };
+constexpr uint32_t SCAN_BLOCK_ROWS = 8, SCAN_BACKWARD_BLOCKS = 4;
+uint32_t scanTiles(const gennmi_scan_t &c) { return c.groups * ((c.channels / c.groups + 63) / 64); }
+// States of a wavefront, wavefronts of a work-group, rows of a chunk
+ScanPlan scanPlan(const gennmi_scan_t &c, bool gradients)
+{
+    ScanPlan p;
+    p.slab = c.states <= 8 ? 8 : 16;
+    p.slabs = (c.states + p.slab - 1) / p.slab;
+    if(gradients) { p.chunk = SCAN_BLOCK_ROWS * SCAN_BACKWARD_BLOCKS; }
+    else {
+        // enough chunks for a few wavefronts on each of the chip's 1024 SIMDs, of 64 rows at least
+        const uint64_t waves = (uint64_t)scanTiles(c) * p.slabs;
+        const uint64_t rows = std::max<uint64_t>(1, totalRows(c.sequences));
+        const uint64_t chunks = std::max<uint64_t>(1, 2048 / waves);
+        p.chunk = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(64, (rows + chunks - 1) / chunks + 7) / 8 * 8, 0x7ffffff8u);
+        // (a split costs every state twice: not worth it for less than twice the wavefronts)
+        if((uint64_t)p.chunk * 2 > c.sequences.length) { p.chunk = std::max(1u, c.sequences.length); }
+    }
+    p.split = c.sequences.length > p.chunk;
+    return p;
+}
+struct ScanSpace { size_t state, time, gradient, sumA, sumD, sumBias, sumBC, bytes; };
+ScanSpace scanSpace(const gennmi_scan_t &c, const ScanPlan &p, bool gradients)
+{
+    ScanSpace s{};
+    const uint64_t numbers = chunkNumbers(c.sequences, p.chunk);
+    auto take = [&](uint64_t floats) { const size_t at = s.bytes; s.bytes += (floats * sizeof(float) + 255) / 256 * 256; return at; };
+    if(p.split) {
+        s.state = take(numbers * c.states * c.channels);
+        s.time = take(numbers * c.channels);
+    }
+    if(gradients) {
+        if(p.split) { s.gradient = take(numbers * c.states * c.channels); }
+        s.sumA = take(numbers * c.states * c.channels);
+        s.sumD = take(numbers * p.slabs * c.channels);
+        s.sumBias = take(numbers * p.slabs * c.channels);
+        s.sumBC = take((uint64_t)scanTiles(c) * totalRows(c.sequences) * 2 * c.states);
+    }
+    return s;
+}
+int scanArgs(const char *what, const gennmi_scan_t &c, const ScanPlan &p, ScanArgs &a)
+{
+    a = ScanArgs{};
+    const uint64_t numbers = chunkNumbers(c.sequences, p.chunk), tiles = scanTiles(c);
+    if(numbers * tiles > MOST_BLOCKS || (uint64_t)c.sequences.count * c.states * ((c.channels + 63) / 64) > MOST_BLOCKS) {
+        return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers");
+    }
+    a.sequences = sequencesOf(c.sequences, p.chunk);
+    a.u = c.u; a.delta = c.delta; a.z = c.z; a.out = c.out; a.B = c.B; a.C = c.C;
+    a.A = c.A; a.D = c.D; a.deltaBias = c.deltaBias;
+    a.initialState = c.initialState; a.finalState = c.finalState;
+    a.channels = c.channels; a.states = c.states; a.groups = c.groups; a.softplus = c.softplus;
+    a.groupChannels = c.channels / c.groups;
+    a.groupTiles = (a.groupChannels + 63) / 64;
+    a.tiles = (uint32_t)tiles;
+    a.numbers = (uint32_t)numbers;
+    a.slabs = p.slabs;
+    return GENNMI_OK;
+}
+int checkWorkspace(const char *what, const void *workspace, size_t have, size_t need)
+{
+    if(need && (!workspace || have < need)) { return fail(GENNMI_EINVAL, std::string(what) + ": workspace is missing or too small"); }
+    return (uintptr_t)workspace % 16 ? fail(GENNMI_EINVAL, std::string(what) + ": workspace is not 16-byte aligned") : GENNMI_OK;
+}
+
+template<typename T, int NP, bool SLABS> int launchScan(const ScanArgs &a, const ScanPlan &p, hipStream_t stream)
+{
+    const dim3 grid(a.numbers * a.tiles), threads(64 * p.slabs);
+    if(p.split) {
+        scanChunkKernel<T, NP, false, SLABS><<<grid, threads, 0, stream>>>(a, ScanGradientArgs{});
+        if(const int rc = gennmi_detail::afterLaunch("selective_scan")) { return rc; }
+        scanJoinKernel<false><<<dim3(a.sequences.count * a.states * ((a.channels + 63) / 64)), dim3(64), 0, stream>>>(a, ScanGradientArgs{});
+        if(const int rc = gennmi_detail::afterLaunch("selective_scan")) { return rc; }
+    }
+    scanKernel<T, NP, SLABS><<<grid, threads, 0, stream>>>(a);
+    return gennmi_detail::afterLaunch("selective_scan");
+}
+template<typename T, int LANES> int launchToken(const ScanArgs &a, hipStream_t stream)
+{
+    const bool quads = a.states % 4 == 0 && (uintptr_t)a.initialState % 16 == 0 && (uintptr_t)a.finalState % 16 == 0;
+    const dim3 grid((uint32_t)(((uint64_t)a.sequences.count * a.channels * LANES + 255) / 256));
+    if(quads) { scanTokenKernel<T, LANES, true><<<grid, dim3(256), 0, stream>>>(a); } else { scanTokenKernel<T, LANES, false><<<grid, dim3(256), 0, stream>>>(a); }
+    return gennmi_detail::afterLaunch("selective_scan");
+}
+template<typename T, int NP, bool SLABS> int launchScanBackward(const ScanArgs &a, const ScanGradientArgs &g, const ScanPlan &p, hipStream_t stream)
+{
+    const dim3 grid(a.numbers * a.tiles), threads(64 * p.slabs);
+    if(p.split) {
+        scanChunkKernel<T, NP, true, SLABS><<<grid, threads, 0, stream>>>(a, g);
+        if(const int rc = gennmi_detail::afterLaunch("selective_scan_backward")) { return rc; }
+        scanJoinKernel<true><<<dim3(a.sequences.count * a.states * ((a.channels + 63) / 64)), dim3(64), 0, stream>>>(a, g);
+        if(const int rc = gennmi_detail::afterLaunch("selective_scan_backward")) { return rc; }
+    }
+    const size_t lds = sizeof(float) * (p.slabs * ((SCAN_BACKWARD_BLOCKS - 1) * NP * 64 + SCAN_BLOCK_ROWS * 2 * NP) + (SLABS ? p.slabs * SCAN_BLOCK_ROWS * 3 * 64 : 0));
+    auto kernel = scanBackwardKernel<T, NP, (int)SCAN_BLOCK_ROWS, (int)SCAN_BACKWARD_BLOCKS, SLABS>;
+    if(lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if(e != hipSuccess) { return fail(GENNMI_EHIP, std::string("selective_scan_backward: ") + hipGetErrorString(e)); }
+    }
+    kernel<<<grid, threads, lds, stream>>>(a, g);
+    return gennmi_detail::afterLaunch("selective_scan_backward");
+}
+// Picks the instance: states of a wavefront, and whether several wavefronts share a channel
+template<typename F> int withStates(const ScanPlan &p, F &&f)
+{
+    if(p.slabs > 1) { return f(std::integral_constant<int, 16>{}, std::true_type{}); }
+    if(p.slab == 16) { return f(std::integral_constant<int, 16>{}, std::false_type{}); }
+    return f(std::integral_constant<int, 8>{}, std::false_type{});
+}
+}
+
+extern "C" {
+
+int gennmi_stream_is_capturing(void *stream, int *capturing)
+{
+    if(!capturing) { return fail(GENNMI_EINVAL, "stream_is_capturing: null result pointer"); }
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if(stream) {
+        const hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &status);
+        if(e != hipSuccess) { return fail(GENNMI_EHIP, std::string("stream_is_capturing: ") + hipGetErrorString(e)); }
+    }
+    *capturing = status != hipStreamCaptureStatusNone;
+    return GENNMI_OK;
+}
+
+int gennmi_causal_conv(const gennmi_causal_conv_t *conv, void *stream)
+{
+    return gennmi_detail::guarded("causal_conv", [&] {
+        if(const int rc = checkConv("causal_conv", conv, false)) { return rc; }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        if(const int rc = runConv("causal_conv", *conv, convVector(*conv, nullptr), nullptr, (hipStream_t)stream)) { return rc; }
+        const uint32_t size = sizeOf(conv->type);
+        noteRows(conv->out, conv->sequences, conv->channels, size);
+        if(conv->finalState) { gennmi_detail::noteDeviceWrite(conv->finalState, statesOf(conv->sequences) * (conv->taps - 1) * conv->channels * size); }
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_causal_conv_backward_workspace(const gennmi_causal_conv_t *conv, size_t *bytes)
+{
+    return gennmi_detail::guarded("causal_conv_backward_workspace", [&] {
+        if(const int rc = checkConv("causal_conv_backward_workspace", conv, true)) { return rc; }
+        if(!bytes) { return fail(GENNMI_EINVAL, "causal_conv_backward_workspace: null result pointer"); }
+        *bytes = convWorkspace(*conv);
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_causal_conv_gradient_t *gradient, void *workspace, size_t workspaceBytes,
+                                void *stream)
+{
+    const char *what = "causal_conv_backward";
+    return gennmi_detail::guarded(what, [&] {
+        if(const int rc = checkConv(what, conv, true)) { return rc; }
+        if(!gradient) { return fail(GENNMI_EINVAL, "causal_conv_backward: null gradient"); }
+        const gennmi_causal_conv_gradient_t &g = *gradient;
+        const uint32_t size = sizeOf(conv->type);
+        if(const int rc = checkRows(what, "the gradient of out", g.out, conv->sequences, conv->channels, size)) { return rc; }
+        if(g.x.data) {
+            if(const int rc = checkWrittenRows(what, "the gradient of x", g.x, conv->sequences, conv->channels, size)) { return rc; }
+            if(g.x.data == g.out.data || g.x.data == conv->x.data) { return fail(GENNMI_EINVAL, "causal_conv_backward: the gradient of x is an array of its own"); }
+        }
+        if((uintptr_t)g.finalState % size || (uintptr_t)g.initialState % size || (uintptr_t)g.weight % 4 || (uintptr_t)g.bias % 4) {
+            return fail(GENNMI_EINVAL, "causal_conv_backward: an array is not aligned to its elements");
+        }
+        const bool sums = g.weight || g.bias;
+        if(const int rc = checkWorkspace(what, workspace, workspaceBytes, sums ? convWorkspace(*conv) : 0)) { return rc; }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        ConvGradientArgs a{};
+        a.out = g.out;
+        a.x = g.x;
+        a.finalState = g.finalState;
+        a.initialState = g.initialState;
+        a.partial = sums ? (float*)workspace : nullptr;
+        if(const int rc = runConv(what, *conv, convVector(*conv, gradient), &a, (hipStream_t)stream)) { return rc; }
+        if(sums) {
+            const uint64_t items = (uint64_t)conv->channels * (conv->taps + 1);
+            causalConvReduceKernel<<<dim3((uint32_t)((items + 255) / 256)), dim3(256), 0, (hipStream_t)stream>>>(a.partial, (uint32_t)chunkNumbers(conv->sequences, convChunk(*conv)),
+                                                                                                                conv->channels, conv->taps, g.weight, g.bias);
+            if(const int rc = gennmi_detail::afterLaunch(what)) { return rc; }
+        }
+        noteRows(g.x, conv->sequences, conv->channels, size);
+        if(g.initialState) { gennmi_detail::noteDeviceWrite(g.initialState, (uint64_t)conv->sequences.count * (conv->taps - 1) * conv->channels * size); }
+        if(g.weight) { gennmi_detail::noteDeviceWrite(g.weight, (uint64_t)conv->channels * conv->taps * sizeof(float)); }
+        if(g.bias) { gennmi_detail::noteDeviceWrite(g.bias, conv->channels * sizeof(float)); }
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_selective_scan_workspace(const gennmi_scan_t *scan, size_t *bytes)
+{
+    return gennmi_detail::guarded("selective_scan_workspace", [&] {
+        if(const int rc = checkScan("selective_scan_workspace", scan, false)) { return rc; }
+        if(!bytes) { return fail(GENNMI_EINVAL, "selective_scan_workspace: null result pointer"); }
+        *bytes = scanSpace(*scan, scanPlan(*scan, false), false).bytes;
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_selective_scan(const gennmi_scan_t *scan, void *workspace, size_t workspaceBytes, void *stream)
+{
+    const char *what = "selective_scan";
+    return gennmi_detail::guarded(what, [&] {
+        if(const int rc = checkScan(what, scan, false)) { return rc; }
+        const ScanPlan p = scanPlan(*scan, false);
+        const ScanSpace space = scanSpace(*scan, p, false);
+        if(const int rc = checkWorkspace(what, workspace, workspaceBytes, space.bytes)) { return rc; }
+        ScanArgs a;
+        if(const int rc = scanArgs(what, *scan, p, a)) { return rc; }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        if(!scan->sequences.count) { return (int)GENNMI_OK; }
+        if(p.split) {
+            a.chunkState = (float*)((char*)workspace + space.state);
+            a.chunkTime = (float*)((char*)workspace + space.time);
+        }
+        const int rc = withType(scan->type, [&](auto t) {
+            typedef decltype(t) T;
+            if(scan->sequences.length <= 1) {
+                if(a.states <= 4) { return launchToken<T, 1>(a, (hipStream_t)stream); }
+                if(a.states <= 8) { return launchToken<T, 2>(a, (hipStream_t)stream); }
+                if(a.states <= 16) { return launchToken<T, 4>(a, (hipStream_t)stream); }
+                if(a.states <= 32) { return launchToken<T, 8>(a, (hipStream_t)stream); }
+                if(a.states <= 64) { return launchToken<T, 16>(a, (hipStream_t)stream); }
+                return launchToken<T, 32>(a, (hipStream_t)stream);
+            }
+            return withStates(p, [&](auto np, auto slabs) { return launchScan<T, decltype(np)::value, decltype(slabs)::value>(a, p, (hipStream_t)stream); });
+        });
+        if(rc) { return rc; }
+        noteRows(scan->out, scan->sequences, scan->channels, sizeOf(scan->type));
+        if(scan->finalState) { gennmi_detail::noteDeviceWrite(scan->finalState, statesOf(scan->sequences) * scan->channels * scan->states * sizeof(float)); }
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_selective_scan_backward_workspace(const gennmi_scan_t *scan, size_t *bytes)
+{
+    return gennmi_detail::guarded("selective_scan_backward_workspace", [&] {
+        if(const int rc = checkScan("selective_scan_backward_workspace", scan, true)) { return rc; }
+        if(!bytes) { return fail(GENNMI_EINVAL, "selective_scan_backward_workspace: null result pointer"); }
+        *bytes = scanSpace(*scan, scanPlan(*scan, true), true).bytes;
+        return (int)GENNMI_OK;
+    });
+}
+
+int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_gradient_t *gradient, void *workspace, size_t workspaceBytes, void *stream)
+{
+    const char *what = "selective_scan_backward";
+    return gennmi_detail::guarded(what, [&] {
+        if(const int rc = checkScan(what, scan, true)) { return rc; }
+        if(!gradient) { return fail(GENNMI_EINVAL, "selective_scan_backward: null gradient"); }
+        const gennmi_scan_gradient_t &in = *gradient;
+        const uint32_t size = sizeOf(scan->type), width = scan->groups * scan->states;
+        if(const int rc = checkRows(what, "the gradient of out", in.out, scan->sequences, scan->channels, size)) { return rc; }
+        const struct { const char *which; const gennmi_rows_t *rows; uint32_t width; } written[] = {
+            {"the gradient of u", &in.u, scan->channels}, {"the gradient of delta", &in.delta, scan->channels}, {"the gradient of z", &in.z, scan->channels},
+            {"the gradient of B", &in.B, width}, {"the gradient of C", &in.C, width}};
+        for(const auto &w : written) {
+            if(!w.rows->data) { continue; }
+            if(const int rc = checkWrittenRows(what, w.which, *w.rows, scan->sequences, w.width, size)) { return rc; }
+            for(const void *p : {scan->u.data, scan->delta.data, scan->z.data, scan->B.data, scan->C.data, in.out.data}) {
+                if(p == w.rows->data) { return fail(GENNMI_EINVAL, std::string(what) + ": " + w.which + " is an array of its own"); }
+            }
+        }
+        if(in.z.data && !scan->z.data) { return fail(GENNMI_EINVAL, "selective_scan_backward: a gradient of z without z"); }
+        for(const void *p : {(const void*)in.finalState, (const void*)in.initialState, (const void*)in.A, (const void*)in.D, (const void*)in.deltaBias}) {
+            if((uintptr_t)p % 4) { return fail(GENNMI_EINVAL, "selective_scan_backward: an array of fp32 is not aligned"); }
+        }
+        const ScanPlan p = scanPlan(*scan, true);
+        const ScanSpace space = scanSpace(*scan, p, true);
+        if(const int rc = checkWorkspace(what, workspace, workspaceBytes, space.bytes)) { return rc; }
+        ScanArgs a;
+        if(const int rc = scanArgs(what, *scan, p, a)) { return rc; }
+        const uint64_t rows = totalRows(scan->sequences);
+        if((rows * 2 * width + 255) / 256 > MOST_BLOCKS) { return fail(GENNMI_EINVAL, "selective_scan_backward: more rows than one launch covers"); }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        auto at = [&](size_t offset) { return (float*)((char*)workspace + offset); };
+        a.finalState = nullptr;
+        ScanGradientArgs g{};
+        g.out = in.out; g.u = in.u; g.delta = in.delta; g.z = in.z; g.B = in.B; g.C = in.C;
+        g.finalState = in.finalState; g.initialState = in.initialState;
+        if(p.split) {
+            a.chunkState = at(space.state);
+            a.chunkTime = at(space.time);
+            g.chunkGradient = at(space.gradient);
+        }
+        g.sumA = in.A ? at(space.sumA) : nullptr;
+        g.sumD = in.D ? at(space.sumD) : nullptr;
+        g.sumBias = in.deltaBias ? at(space.sumBias) : nullptr;
+        g.sumBC = in.B.data || in.C.data ? at(space.sumBC) : nullptr;
+        g.rows = rows;
+        const hipStream_t s = (hipStream_t)stream;
+        if(a.numbers) {
+            const int rc = withType(scan->type, [&](auto t) {
+                typedef decltype(t) T;
+                const int rcScan = withStates(p, [&](auto np, auto slabs) { return launchScanBackward<T, decltype(np)::value, decltype(slabs)::value>(a, g, p, s); });
+                if(rcScan || !g.sumBC || !rows) { return rcScan; }
+                scanRowSumKernel<T><<<dim3((uint32_t)((rows * 2 * width + 255) / 256)), dim3(256), 0, s>>>(a, g);
+                return gennmi_detail::afterLaunch(what);
+            });
+            if(rc) { return rc; }
+        }
+        const struct { float *out, *sums; uint32_t each, width; } channelSums[] = {
+            {in.A, g.sumA, 1, scan->states}, {in.D, g.sumD, p.slabs, 1}, {in.deltaBias, g.sumBias, p.slabs, 1}};
+        for(const auto &c : channelSums) {
+            if(!c.out) { continue; }
+            const uint64_t items = (uint64_t)scan->channels * c.width;
+            scanChannelSumKernel<<<dim3((uint32_t)((items + 255) / 256)), dim3(256), 0, s>>>(c.sums, a.numbers, c.each, scan->channels, c.width, c.out);
+            if(const int rc = gennmi_detail::afterLaunch(what)) { return rc; }
+            gennmi_detail::noteDeviceWrite(c.out, items * sizeof(float));
+        }
+        for(const auto &w : written) { noteRows(*w.rows, scan->sequences, w.width, size); }
+        if(in.initialState) { gennmi_detail::noteDeviceWrite(in.initialState, (uint64_t)scan->sequences.count * scan->channels * scan->states * sizeof(float)); }
+        return (int)GENNMI_OK;
+    });
+}
+
+}

@@ -352,7 +352,9 @@ int gennmi_build_remap(uint32_t numSrcNeurons, uint32_t numTrgNeurons, uint32_t 
  * Binomial :254-262 {n, p} */
 enum { GENNMI_INIT_CONSTANT = 0, GENNMI_INIT_UNIFORM = 1, GENNMI_INIT_NORMAL = 2, GENNMI_INIT_NORMAL_CLIPPED = 3,
        GENNMI_INIT_NORMAL_CLIPPED_DELAY = 4, GENNMI_INIT_EXPONENTIAL = 5, GENNMI_INIT_GAMMA = 6, GENNMI_INIT_BINOMIAL = 7 };
-enum { GENNMI_TYPE_F32 = 0, GENNMI_TYPE_U32 = 1, GENNMI_TYPE_I32 = 2, GENNMI_TYPE_U16 = 3, GENNMI_TYPE_U8 = 4 };
+enum { GENNMI_TYPE_F32 = 0, GENNMI_TYPE_U32 = 1, GENNMI_TYPE_I32 = 2, GENNMI_TYPE_U16 = 3, GENNMI_TYPE_U8 = 4,
+       /* the 16-bit floating types: of the operators below only, gennmi_init_var does not take them */
+       GENNMI_TYPE_F16 = 5, GENNMI_TYPE_BF16 = 6 };
 /* genVariableInit / genSparseSynapseVariableRowInit (backendBase.h:246-251): fills `count` elements of a 16-byte aligned
  * device array; values are computed in fp32 and converted to the element type.  Per-synapse variables of a SPARSE
  * matrix are filled over the whole numPre*rowStride range, padding included (padding is never read). */
@@ -568,6 +570,132 @@ int gennmi_program_set_timing(gennmi_program *program, int enabled);
 int gennmi_program_get_time(gennmi_program *program, int timer, double *seconds);
 /* info = {calls of gennmi_program_update executed so far, of which replayed from a captured graph, launches made, graphs captured} */
 int gennmi_program_get_info(gennmi_program *program, unsigned long long info[4]);
+
+/* ---------------------------------------------------------------------------------------------
+ * Operators on sequences, and the step that trains their weights.  No counterparts in the reference, whose models step in
+ * time only and are trained by custom updates, a generated kernel per group of variables.
+ *
+ * Like every call that writes device memory they run the steps queued in runners first (gennmi_flush), and they tell
+ * the runners what they wrote (gennmi_note_device_write); they launch on `stream` (a hipStream_t; NULL: the null stream, with which the
+ * runners' streams are ordered) of the current device, and return without waiting.  All arrays are memory of that device.
+ * A call can be captured into a graph: nothing is allocated, copied or waited for.  While a stream is captured, steps queued in a
+ * runner make the call fail with GENNMI_ESTATE (run gennmi_flush before); the runners do not hear of what a replay wrote
+ * (call gennmi_note_device_write).  A workspace belongs to the call until the call has finished on its stream: calls that may
+ * run at the same time, and captured graphs that may, need a workspace each.  No result is a sum of atomics: the same call gives the same bits.
+ * ------------------------------------------------------------------------------------------- */
+/* Whether work on the stream is being captured into a graph (never the null stream's): for callers that keep a workspace between calls. */
+int gennmi_stream_is_capturing(void *stream, int *capturing);
+/* Rows of adjacent elements; strides count elements.  Row t of sequence s lies at data + s * sequenceStride + t * rowStride, or,
+ * where the sequences are packed (gennmi_sequences_t::offsets), at data + (offsets[s] + t) * rowStride. */
+typedef struct gennmi_rows_t {
+    void *data;
+    uint64_t rowStride, sequenceStride;
+} gennmi_rows_t;
+typedef struct gennmi_sequences_t {
+    uint32_t count;                       /* sequences */
+    uint32_t length;                      /* rows of each, 0 included; of packed ones the most: what a longer one has behind that is left alone */
+    const uint32_t *offsets;              /* NULL, or device [count + 1], ascending: sequences packed one behind another, of offsets[s + 1] - offsets[s] rows */
+    uint64_t rows;                        /* with offsets: rows that the arrays hold (offsets beyond that are cut to it) */
+    const int32_t *slots;                 /* NULL: sequence s has state s; or device [count]: the place of its state among numSlots.  A sequence whose slot is
+                                           * outside 0 .. numSlots - 1 is padding: nothing of it is read or written.  Two sequences must not share a state that
+                                           * is written.  Not for gradients. */
+    uint32_t numSlots, pad_;
+} gennmi_sequences_t;
+
+/* Short causal convolution, every channel by itself (depthwise):
+ *   s[t][c] = bias[c] + sum_k weight[c][k] * x[t - (taps - 1) + k][c],   out = s, or s * sigmoid(s) with `silu`.
+ * Rows before a sequence's first are those of its initial state, or zero.  Sums in fp32, one rounding at the end. */
+#define GENNMI_MAX_TAPS 8
+typedef struct gennmi_causal_conv_t {
+    gennmi_sequences_t sequences;
+    uint32_t type;                        /* of x, out and the states: GENNMI_TYPE_F32, _F16 or _BF16 */
+    uint32_t channels, taps, silu;        /* 1 <= taps <= GENNMI_MAX_TAPS */
+    gennmi_rows_t x, out;                 /* two arrays */
+    const float *weight, *bias;           /* [channels][taps]; [channels] or NULL */
+    const void *initialState;             /* [states][taps - 1][channels]: the inputs before the first row, oldest first; or NULL: zero */
+    void *finalState;                     /* the last taps - 1 inputs, or NULL; may be initialState itself */
+} gennmi_causal_conv_t;
+typedef struct gennmi_causal_conv_gradient_t {      /* `out` and `finalState` come in, the others go out (any may be NULL) and are overwritten */
+    gennmi_rows_t out, x;
+    const void *finalState;               /* gradient of the final state, or NULL: zero */
+    void *initialState;
+    float *weight, *bias;
+} gennmi_causal_conv_gradient_t;
+int gennmi_causal_conv(const gennmi_causal_conv_t *conv, void *stream);
+int gennmi_causal_conv_backward_workspace(const gennmi_causal_conv_t *conv, size_t *bytes);
+int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_causal_conv_gradient_t *gradient, void *workspace, size_t workspaceBytes,
+                                void *stream);
+
+/* Selective state space scan: every channel d drives `states` leaky units whose step in time, inputs and outputs depend on the row.
+ *   dt = delta[t][d] + deltaBias[d], then log(1 + exp(dt)) with `softplus`
+ *   h[t][d][n] = exp(dt * A[d][n]) * h[t - 1][d][n] + dt * u[t][d] * B[t][g][n]
+ *   out[t][d] = (sum_n C[t][g][n] * h[t][d][n] + D[d] * u[t][d]) * z[t][d] * sigmoid(z[t][d])
+ * where channels / groups neighbouring channels share the B and C of group g.  States and sums in fp32.  One row per sequence (a token of every
+ * running sequence) takes a kernel of its own, without a workspace. */
+#define GENNMI_MAX_SCAN_STATES 128
+typedef struct gennmi_scan_t {
+    gennmi_sequences_t sequences;
+    uint32_t type;                        /* of u, delta, B, C, z and out: GENNMI_TYPE_F32, _F16 or _BF16 */
+    uint32_t channels, states, groups;    /* groups divides channels; 1 <= states <= GENNMI_MAX_SCAN_STATES */
+    uint32_t softplus, pad_;
+    gennmi_rows_t u, delta, z, out;       /* [channels] a row; z.data NULL: no gate.  `out` is an array of its own */
+    gennmi_rows_t B, C;                   /* [groups][states] a row */
+    const float *A, *D, *deltaBias;       /* [channels][states]; [channels], D and deltaBias or NULL */
+    const float *initialState;            /* [states' places][channels][states], or NULL: zero */
+    float *finalState;                    /* after the last row, or NULL; may be initialState itself */
+} gennmi_scan_t;
+typedef struct gennmi_scan_gradient_t {             /* `out` and `finalState` come in, the others go out (any may be NULL) and are overwritten */
+    gennmi_rows_t out, u, delta, z, B, C;
+    const float *finalState;              /* gradient of the final state, or NULL: zero */
+    float *initialState, *A, *D, *deltaBias;
+} gennmi_scan_gradient_t;
+int gennmi_selective_scan_workspace(const gennmi_scan_t *scan, size_t *bytes);
+int gennmi_selective_scan(const gennmi_scan_t *scan, void *workspace, size_t workspaceBytes, void *stream);
+int gennmi_selective_scan_backward_workspace(const gennmi_scan_t *scan, size_t *bytes);
+int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_gradient_t *gradient, void *workspace, size_t workspaceBytes, void *stream);
+
+/* AdamW (Loshchilov & Hutter 2019) over many tensors in one launch:
+ *   g = gradientScale * gradient,  m = beta1 * m + (1 - beta1) * g,  v = beta2 * v + (1 - beta2) * g^2
+ *   weight = weight * (1 - rate * weightDecay) - rate * (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + epsilon)
+ * with t the number of the step, which the device counts.  States in 32 bits, or in 8 for blocks of GENNMI_ADAMW_BLOCK weights:
+ *   m = mScale * c / 448,  v = vScale * (c / 448)^2,   c in e4m3 (OCP), mScale = max |m| and vScale = max v of the block
+ * (the nearest code, ties to even; a positive v never gets the code 0, which would make the next step a division by epsilon).  The weights are updated from
+ * the states before they are coded. */
+#define GENNMI_ADAMW_BLOCK 256
+typedef struct gennmi_optimiser gennmi_optimiser;
+typedef struct gennmi_adamw_t {
+    double beta1, beta2, epsilon;
+    uint32_t stateBits, pad_;             /* 8 or 32 */
+} gennmi_adamw_t;
+typedef struct gennmi_parameter_t {       /* one tensor; tensors of an optimiser do not overlap */
+    void *weight;                         /* [count] GENNMI_TYPE_F32, _F16 or _BF16 (computed in fp32, rounded once) */
+    const void *gradient;                 /* [count] any of these */
+    void *copy;                           /* [count] F16 or BF16: the new weights rounded, or NULL */
+    void *m, *v;                          /* [count] fp32, or e4m3 codes */
+    float *mScale, *vScale;               /* 8 bits: [ceil(count / GENNMI_ADAMW_BLOCK)] */
+    uint64_t count;
+    uint32_t weightType, gradientType, copyType, pad_;
+    double weightDecay;
+} gennmi_parameter_t;
+typedef struct gennmi_adamw_step_t {
+    double rate;                          /* learning rate */
+    const float *rateDevice;              /* device: taken instead of `rate` when the step runs (a captured step), or NULL */
+    const float *gradientScale;           /* device: what gradients are multiplied with (clipping, loss scaling), or NULL: 1 */
+    const uint32_t *skip;                 /* device: not 0: the step leaves everything as it is and is not counted; or NULL */
+} gennmi_adamw_step_t;
+int gennmi_optimiser_create(gennmi_optimiser **optimiser, const gennmi_adamw_t *settings);
+int gennmi_optimiser_destroy(gennmi_optimiser *optimiser);
+/* As for a runner: tensors are pushed, finalise uploads their table, then steps.  Arrays stay the caller's. */
+int gennmi_optimiser_push(gennmi_optimiser *optimiser, const gennmi_parameter_t *parameter, uint32_t *idx);
+int gennmi_optimiser_finalise(gennmi_optimiser *optimiser);
+/* One launch.  Steps of one optimiser run one behind another: the caller orders them where it uses several streams. */
+int gennmi_optimiser_step(gennmi_optimiser *optimiser, const gennmi_adamw_step_t *step, void *stream);
+/* Steps counted so far, for a checkpoint beside the states; both wait for the device. */
+int gennmi_optimiser_get_step(gennmi_optimiser *optimiser, uint64_t *step);
+int gennmi_optimiser_set_step(gennmi_optimiser *optimiser, uint64_t step);
+/* sizeof() of gennmi_rows_t, gennmi_sequences_t, gennmi_causal_conv_t, gennmi_causal_conv_gradient_t, gennmi_scan_t, gennmi_scan_gradient_t,
+ * gennmi_adamw_t, gennmi_parameter_t, gennmi_adamw_step_t: what gennmi_abi_struct_sizes is for the descriptors of groups. */
+int gennmi_abi_operator_sizes(size_t sizes[9]);
 
 #ifdef __cplusplus
 }

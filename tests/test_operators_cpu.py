@@ -1,0 +1,216 @@
+"""Operators on sequences and the optimiser, as far as they go without a GPU: layouts of the descriptors, sizes of workspaces, and what the
+entry points refuse before they touch the device.  Also the 64-bit restatements that the GPU tests compare with, against differences."""
+import ctypes as C
+
+import pytest
+import torch
+
+import sequence_ref as ref
+from genn_amd import _abi
+
+F32, F16, BF16 = (_abi.FLOAT_TYPES[t] for t in ("float32", "float16", "bfloat16"))
+AT = 1 << 20            # an address that nothing may follow
+
+
+def conv(**changes):
+    c = _abi.CausalConv(type=BF16, channels=24, taps=4, silu=1, weight=AT, bias=AT, initialState=None, finalState=None)
+    c.sequences = _abi.Sequences(count=2, length=5)
+    c.x, c.out = _abi.Rows(AT, 24, 120), _abi.Rows(AT + 4096, 24, 120)
+    return changed(c, changes)
+
+
+def scan(**changes):
+    c = _abi.Scan(type=BF16, channels=24, states=16, groups=2, softplus=1, A=AT, D=AT, deltaBias=AT)
+    c.sequences = _abi.Sequences(count=2, length=5)
+    for k, name in enumerate(("u", "delta", "z", "out")):
+        setattr(c, name, _abi.Rows(AT + 4096 * k, 24, 120))
+    c.B, c.C = _abi.Rows(AT + 4096 * 5, 32, 160), _abi.Rows(AT + 4096 * 6, 32, 160)
+    return changed(c, changes)
+
+
+def changed(c, changes):
+    for name, value in changes.items():
+        at = c
+        *path, last = name.split("__")
+        for p in path:
+            at = getattr(at, p)
+        setattr(at, last, value)
+    return c
+
+
+def refused(rc, code, text):
+    said = _abi.load().gennmi_last_error().decode()
+    assert rc == code and text in said, (rc, said)
+
+
+def test_descriptors_have_the_librarys_layout():
+    sizes = (C.c_size_t * 9)()
+    assert _abi.load().gennmi_abi_operator_sizes(C.byref(sizes)) == 0
+    assert list(sizes) == [C.sizeof(s) for s in _abi.OPERATOR_STRUCTS]
+
+
+@pytest.mark.parametrize("change, code, text", [
+    (dict(type=1), -3, "element type"), (dict(type=7), -3, "element type"), (dict(taps=0), -3, "taps"), (dict(taps=9), -3, "taps"),
+    (dict(channels=0), -2, "channels"), (dict(weight=None), -2, "weight"), (dict(weight=AT + 2), -2, "aligned"), (dict(bias=AT + 1), -2, "aligned"),
+    (dict(x__data=None), -2, "x is missing"), (dict(x__data=AT + 1), -2, "aligned"), (dict(out__data=AT), -2, "same array"), (dict(out__data=None), -2, "out is missing"),
+    (dict(x__rowStride=23), -2, "rows overlap"), (dict(out__sequenceStride=0), -2, "sequences overlap"), (dict(out__rowStride=1 << 41), -2, "stride"),
+    (dict(initialState=AT + 1), -2, "state"), (dict(finalState=AT + 1), -2, "state"),
+    (dict(sequences__count=(1 << 24) + 1), -2, "more sequences"), (dict(sequences__length=1 << 31), -2, "more sequences"),
+    (dict(sequences__offsets=AT + 2, sequences__rows=10), -2, "offsets"), (dict(sequences__slots=AT, sequences__numSlots=0), -2, "numSlots"),
+    (dict(sequences__offsets=AT, sequences__rows=1 << 31), -2, "more sequences or rows"),
+    (dict(sequences__count=1 << 12, sequences__length=1 << 19), -2, "more sequences or rows"),
+    (dict(sequences__count=1, sequences__length=(1 << 31) - 1, channels=1 << 24, x__rowStride=1 << 24, out__rowStride=1 << 24), -2, "one launch"),
+])
+def test_causal_conv_refuses(change, code, text):
+    refused(_abi.load().gennmi_causal_conv(C.byref(conv(**change)), None), code, text)
+
+
+@pytest.mark.parametrize("change, code, text", [
+    (dict(type=2), -3, "element type"), (dict(states=0), -3, "states"), (dict(states=129), -3, "states"), (dict(channels=0), -2, "channels"),
+    (dict(groups=0), -2, "groups"), (dict(groups=5), -2, "groups"), (dict(A=None), -2, "A is missing"), (dict(A=AT + 1), -2, "aligned"),
+    (dict(D=AT + 2), -2, "aligned"), (dict(initialState=AT + 2), -2, "aligned"), (dict(out__data=AT), -2, "array of its own"),
+    (dict(out__data=None), -2, "out is missing"), (dict(delta__data=None), -2, "delta is missing"), (dict(z__rowStride=1), -2, "rows overlap"),
+    (dict(B__rowStride=31), -2, "rows overlap"), (dict(C__data=None), -2, "C is missing"), (dict(out__sequenceStride=23), -2, "sequences overlap"),
+    (dict(sequences__slots=AT + 2, sequences__numSlots=3), -2, "slots"), (dict(sequences__count=1 << 12, sequences__length=1 << 19), -2, "more sequences or rows"),
+])
+def test_selective_scan_refuses(change, code, text):
+    c = scan(**change)
+    refused(_abi.load().gennmi_selective_scan(C.byref(c), C.c_void_p(AT), 1 << 60, None), code, text)
+
+
+def test_calls_without_arguments_and_workspaces_are_refused():
+    lib = _abi.load()
+    size = C.c_size_t()
+    refused(lib.gennmi_causal_conv(None, None), -2, "null descriptor")
+    refused(lib.gennmi_selective_scan(None, None, 0, None), -2, "null descriptor")
+    refused(lib.gennmi_causal_conv_backward(C.byref(conv()), None, None, 0, None), -2, "null gradient")
+    refused(lib.gennmi_selective_scan_backward(C.byref(scan()), None, None, 0, None), -2, "null gradient")
+    refused(lib.gennmi_selective_scan_workspace(C.byref(scan()), None), -2, "null result")
+    refused(lib.gennmi_stream_is_capturing(None, None), -2, "null result")
+    # the gradients' checks
+    g = _abi.CausalConvGradient(out=_abi.Rows(AT + 8192, 24, 120), x=_abi.Rows(AT + 16384, 24, 120), weight=AT)
+    need = lib.gennmi_causal_conv_backward_workspace
+    assert need(C.byref(conv()), C.byref(size)) == 0 and size.value > 0
+    refused(lib.gennmi_causal_conv_backward(C.byref(conv()), C.byref(g), None, 0, None), -2, "workspace")
+    refused(lib.gennmi_causal_conv_backward(C.byref(conv()), C.byref(g), AT, size.value - 1, None), -2, "workspace")
+    refused(lib.gennmi_causal_conv_backward(C.byref(conv()), C.byref(g), AT + 4, size.value, None), -2, "16-byte")
+    refused(lib.gennmi_causal_conv_backward(C.byref(conv(sequences__slots=AT, sequences__numSlots=4)), C.byref(g), AT, size.value, None), -2, "slots")
+    g.x = _abi.Rows(AT, 24, 120)
+    refused(lib.gennmi_causal_conv_backward(C.byref(conv()), C.byref(g), AT, size.value, None), -2, "array of its own")
+    g = _abi.ScanGradient(out=_abi.Rows(AT + 4096 * 7, 24, 120), u=_abi.Rows(AT + 4096 * 8, 24, 120))
+    assert lib.gennmi_selective_scan_backward_workspace(C.byref(scan()), C.byref(size)) == 0 and size.value > 0
+    refused(lib.gennmi_selective_scan_backward(C.byref(scan()), C.byref(g), AT, size.value - 1, None), -2, "workspace")
+    refused(lib.gennmi_selective_scan_backward(C.byref(scan(z__data=None)), C.byref(changed(g, dict(z=_abi.Rows(AT + 4096 * 9, 24, 120)))), AT, size.value, None), -2, "without z")
+    g.z = _abi.Rows()
+    g.B = _abi.Rows(AT + 4096 * 5, 32, 160)
+    refused(lib.gennmi_selective_scan_backward(C.byref(scan()), C.byref(g), AT, size.value, None), -2, "array of its own")
+    g.B = _abi.Rows()
+    wide = scan(sequences__count=1, sequences__length=(1 << 31) - 1, channels=1 << 24, groups=1, z__data=None)
+    for name in ("u", "delta", "out"):
+        getattr(wide, name).rowStride = 1 << 24
+    large = changed(_abi.ScanGradient(out=_abi.Rows(AT + 4096 * 7, 1 << 24, 0)), {})
+    refused(lib.gennmi_selective_scan_backward(C.byref(wide), C.byref(large), AT, 1 << 62, None), -2, "one launch")
+    g.out = _abi.Rows()
+    refused(lib.gennmi_selective_scan_backward(C.byref(scan()), C.byref(g), AT, size.value, None), -2, "gradient of out is missing")
+
+
+def test_workspaces_of_packed_sequences_go_by_their_rows():
+    """Not by the number of sequences times the longest one, which may be far more than there are rows."""
+    lib, size = _abi.load(), C.c_size_t()
+    for entry in (lib.gennmi_selective_scan_workspace, lib.gennmi_selective_scan_backward_workspace):
+        c = scan(sequences__count=1000, sequences__length=8000, sequences__offsets=AT, sequences__rows=10000)
+        assert entry(C.byref(c), C.byref(size)) == 0
+        assert size.value < (10000 // 32 + 1000) * 24 * (16 * 3 + 4) * 4 + 10000 * 2 * 16 * 2 * 4 + 4096
+    c = scan(sequences__length=1)
+    assert lib.gennmi_selective_scan_workspace(C.byref(c), C.byref(size)) == 0 and size.value == 0     # (a token needs none)
+
+
+def parameter(**changes):
+    p = _abi.Parameter(weight=AT, gradient=AT + 8192, m=AT + 16384, v=AT + 32768, count=100, weightType=F32, gradientType=BF16)
+    return changed(p, changes)
+
+
+@pytest.mark.parametrize("change, code, text", [
+    (dict(weightType=1), -3, "element type"), (dict(gradientType=4), -3, "element type"), (dict(copy=AT + 65536, copyType=F32), -3, "element type"),
+    (dict(weight=None), -2, "missing"), (dict(gradient=None), -2, "missing"), (dict(v=None), -2, "missing"), (dict(weight=AT + 2), -2, "aligned"),
+    (dict(m=AT + 16385), -2, "aligned"), (dict(weightDecay=float("nan")), -2, "decay"), (dict(count=1 << 41), -2, "number of weights"),
+    (dict(m=AT + 4), -2, "arrays of their own"), (dict(v=AT + 16384), -2, "arrays of their own"), (dict(copy=AT + 100, copyType=BF16), -2, "arrays of their own"),
+])
+def test_optimiser_refuses_tensors(change, code, text):
+    lib, o = _abi.load(), C.c_void_p()
+    assert lib.gennmi_optimiser_create(C.byref(o), C.byref(_abi.AdamWSettings(beta1=0.9, beta2=0.99, epsilon=1e-8, stateBits=32))) == 0
+    refused(lib.gennmi_optimiser_push(o, C.byref(parameter(**change)), None), code, text)
+    lib.gennmi_optimiser_destroy(o)
+
+
+def test_optimiser_refuses_settings_order_and_overlaps():
+    lib, o = _abi.load(), C.c_void_p()
+    for wrong in (dict(stateBits=16), dict(beta1=1.0), dict(beta2=-0.1), dict(epsilon=float("nan")), dict(epsilon=-1.0), dict(beta1=float("nan"))):
+        s = changed(_abi.AdamWSettings(beta1=0.9, beta2=0.99, epsilon=1e-8, stateBits=8), wrong)
+        assert lib.gennmi_optimiser_create(C.byref(o), C.byref(s)) < 0 and not o
+    assert lib.gennmi_optimiser_create(C.byref(o), C.byref(_abi.AdamWSettings(beta1=0.9, beta2=0.99, epsilon=0.0, stateBits=8))) == 0
+    refused(lib.gennmi_optimiser_push(o, C.byref(parameter()), None), -2, "missing")          # (no scales)
+    eight = dict(mScale=AT + (1 << 17), vScale=AT + (1 << 18))
+    idx = C.c_uint32(7)
+    assert lib.gennmi_optimiser_push(o, C.byref(parameter(**eight)), C.byref(idx)) == 0 and idx.value == 0
+    refused(lib.gennmi_optimiser_push(o, C.byref(parameter(**eight)), None), -2, "pushed before")
+    refused(lib.gennmi_optimiser_push(o, C.byref(parameter(weight=AT + 396, m=AT + (1 << 21), v=AT + (1 << 22), **eight)), None), -2, "pushed before")
+    assert lib.gennmi_optimiser_push(o, C.byref(parameter(weight=AT + 400, m=AT + (1 << 21), v=AT + (1 << 22), **eight)), C.byref(idx)) == 0 and idx.value == 1
+    refused(lib.gennmi_optimiser_step(o, C.byref(_abi.AdamWStep(rate=1e-3)), None), -4, "not finalised")
+    refused(lib.gennmi_optimiser_step(None, None, None), -2, "null")
+    n = C.c_uint64()
+    refused(lib.gennmi_optimiser_get_step(o, C.byref(n)), -4, "not finalised")
+    refused(lib.gennmi_optimiser_set_step(o, 3), -4, "not finalised")
+    assert lib.gennmi_optimiser_destroy(o) == 0 and lib.gennmi_optimiser_destroy(None) == 0
+
+
+def test_python_layer_refuses_before_it_touches_the_device():
+    from genn_amd.operands import Operand
+    from genn_amd.sequence import CausalConvolution, SelectiveScan
+    for make in (lambda t: CausalConvolution(1, 1, 4, 4, dtype=t), lambda t: SelectiveScan(1, 1, 4, 4, dtype=t)):
+        with pytest.raises(NotImplementedError):
+            make("float64")
+    with pytest.raises(ValueError, match="not on the device"):
+        Operand(torch.zeros(3), "x")
+    with pytest.raises(TypeError, match="neither"):
+        Operand([1.0], "x")
+
+
+def test_gradients_of_the_restatements_are_those_of_differences():
+    """Along random directions, by central differences: off by a third derivative times step^2 (1e-10 here) and rounding over step (1e-16 / 1e-5)."""
+    gen = torch.Generator().manual_seed(3)
+    r = lambda *shape: torch.randn(*shape, generator=gen, dtype=torch.float64)
+    n, D, N, G, K = 9, 6, 3, 2, 4
+    arrays = dict(u=r(n, D), delta=r(n, D) * 0.5, A=-torch.rand(D, N, generator=gen, dtype=torch.float64), B=r(n, G, N), C=r(n, G, N), D=r(D),
+                  delta_bias=r(D), z=r(n, D), initial=r(D, N))
+    dout, dfinal = r(n, D), r(D, N)
+
+    def value(**a):
+        out, final = ref.scan(softplus=True, **a)
+        return float((out * dout).sum() + (final * dfinal).sum())
+
+    g = ref.scan(softplus=True, dout=dout, dfinal=dfinal, **arrays)
+    for name, x in arrays.items():
+        d = torch.randn(x.shape, generator=gen, dtype=torch.float64)
+        got = (value(**{**arrays, name: x + 1e-5 * d}) - value(**{**arrays, name: x - 1e-5 * d})) / 2e-5
+        assert abs(got - float((g[{"initial": "initial_state"}.get(name, name)] * d).sum())) < 1e-7, name
+    arrays = dict(x=r(n, D), weight=r(D, K), bias=r(D), initial=r(K - 1, D))
+    dfinal = r(K - 1, D)
+
+    def value(**a):
+        out, final = ref.causal_conv(silu=True, **a)
+        return float((out * dout).sum() + (final * dfinal).sum())
+
+    g = dict(zip(("x", "weight", "bias", "initial"), ref.causal_conv(silu=True, dout=dout, dfinal=dfinal, **arrays)))
+    for name, x in arrays.items():
+        d = torch.randn(x.shape, generator=gen, dtype=torch.float64)
+        got = (value(**{**arrays, name: x + 1e-5 * d}) - value(**{**arrays, name: x - 1e-5 * d})) / 2e-5
+        assert abs(got - float((g[name] * d).sum())) < 1e-7, name
+
+
+def test_codes_of_the_restatement_are_the_formats():
+    values = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    assert torch.equal(ref.E4M3, values)
+    assert torch.equal(ref.e4m3_codes(values), torch.arange(127))
+    between = (values[1:] + values[:-1]) / 2                # ties go to the even code
+    assert torch.equal(ref.e4m3_codes(between) % 2, torch.zeros(126, dtype=torch.int64))
