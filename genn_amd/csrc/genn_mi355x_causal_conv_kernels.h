@@ -243,18 +243,5 @@ void causalConvBackwardKernel(ConvArgs a, ConvGradientArgs g)
         }
     }
 }
-
-// Sums of the chunks, in 64 bits: there may be thousands, of either sign.
-__global__ __launch_bounds__(256)
-void causalConvReduceKernel(const float *partial, uint32_t numbers, uint32_t channels, uint32_t taps, float *weight, float *bias)
-{
-    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if(item >= (uint64_t)channels * (taps + 1)) { return; }
-    const uint32_t k = (uint32_t)(item / channels), c = (uint32_t)(item - (uint64_t)k * channels);
-    if(!(k < taps ? weight : bias)) { return; }
-    double sum = 0.0;
-    for(uint32_t n = 0; n < numbers; n++) { sum += partial[((uint64_t)n * (taps + 1) + k) * channels + c]; }
-    if(k < taps) { weight[(uint64_t)c * taps + k] = (float)sum; } else { bias[c] = (float)sum; }
-}
 }
 #endif

@@ -24,6 +24,36 @@ template<int WIDTH> __device__ inline float partner(float x)
         return __int_as_float((int)((threadIdx.x & WIDTH) ? s[0] : s[1]));
     }
 }
+// Two values become one register: lanes of the lower halves have a's sum with its partner, those of the upper halves b's.
+template<int WIDTH> __device__ inline float fold(float a, float b)
+{
+    if constexpr(WIDTH >= 16) {
+        const auto s = [&] {
+            if constexpr(WIDTH == 16) { return __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false); }
+            else { return __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false); }
+        }();
+        return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    else {
+        const bool upper = threadIdx.x & WIDTH;
+        return (upper ? b : a) + partner<WIDTH>(upper ? a : b);
+    }
+}
+// Sums over the 64 lanes of M values a lane, M a power of two: folded until one register is left, then added up.  Lane l has the sum of value l / (64 / M).
+template<int M, int WIDTH = 32> __device__ inline float sumOfLanes(const float (&v)[M])
+{
+    if constexpr(M > 1) {
+        float half[M / 2];
+        #pragma unroll
+        for(int i = 0; i < M / 2; i++) { half[i] = fold<WIDTH>(v[i], v[i + M / 2]); }
+        return sumOfLanes<M / 2, WIDTH / 2>(half);
+    }
+    else if constexpr(WIDTH >= 1) {
+        const float one[1] = {v[0] + partner<WIDTH>(v[0])};
+        return sumOfLanes<1, WIDTH / 2>(one);
+    }
+    else { return v[0]; }
+}
 template<int WIDTH = 32> __device__ inline float maxOfLanes(float x)
 {
     x = fmaxf(x, partner<WIDTH>(x));

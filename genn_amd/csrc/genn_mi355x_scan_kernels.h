@@ -34,7 +34,7 @@ struct ScanGradientArgs
     gennmi_rows_t out, u, delta, z, B, C;
     const float *finalState; float *initialState;
     float *chunkGradient;           // [numbers][states][channels]: what a chunk's rows give the state before it, then the gradient of the state behind it
-    float *sumA, *sumD, *sumBias;   // [numbers][states][channels], [numbers][slabs][channels] twice: sums over a chunk
+    float *sums;                    // [numbers][states + 2][channels]: sums over a chunk, for A, D and the bias
     float *sumBC;                   // [tiles][rows][2][states]: sums over a tile's channels, of B's gradient and of C's
     uint64_t rows;                  // rows of sumBC
 };
@@ -103,17 +103,30 @@ template<typename T, int NP, int R> struct StagedBC
 // What one wavefront wrote to LDS is read by its other lanes: LDS accesses of a wavefront are done in order, only the compiler has to keep it
 __device__ inline void waveFence() { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
+template<typename T> __device__ inline T *rowAt(T *rows, uint32_t t, uint64_t stride) { return rows + (uint64_t)t * stride; }
+// A value the compiler knows nothing of: what is computed from it is computed again, not kept in registers from where it was computed before
+__device__ inline float again(float x) { asm volatile("" : "+v"(x)); return x; }
+// Reads of LDS behind this point wait for the four values.  (Left alone, the compiler gathers the reads of many rows in front of all arithmetic, puts off
+// sums that nothing waits for until behind it, and spills hundreds of registers.)
+__device__ inline void readAfter(float &a, float &b, float &c, float &d) { asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : : "memory"); }
+
+// (a wavefront with fewer than NP states reads its last one again instead: a select costs less than a branch a state)
 template<int NP> __device__ inline void loadA(const ScanArgs &a, const ScanPlace &s, float (&A)[NP])
 {
+    const float *from = a.A + (uint64_t)s.channel * a.states + s.firstState;
     #pragma unroll
-    for(int n = 0; n < NP; n++) { A[n] = n < (int)s.numStates ? a.A[(uint64_t)s.channel * a.states + s.firstState + n] * LOG2E : 0.0f; }
+    for(int n = 0; n < NP; n++) { A[n] = from[min((uint32_t)n, s.numStates - 1)] * LOG2E; }
+    #pragma unroll
+    for(int n = 0; n < NP; n++) { A[n] = n < (int)s.numStates ? A[n] : 0.0f; }
 }
 template<int NP> __device__ inline void loadState(const ScanArgs &a, const ScanPlace &s, const float *state, uint64_t which, float (&h)[NP])
 {
     #pragma unroll
-    for(int n = 0; n < NP; n++) {
-        h[n] = state && n < (int)s.numStates ? state[(which * a.channels + s.channel) * a.states + s.firstState + n] : 0.0f;
-    }
+    for(int n = 0; n < NP; n++) { h[n] = 0.0f; }
+    if(!state) { return; }
+    const float *from = state + (which * a.channels + s.channel) * a.states + s.firstState;
+    #pragma unroll
+    for(int n = 0; n < NP; n++) { h[n] = from[min((uint32_t)n, s.numStates - 1)]; }
 }
 template<int NP> __device__ inline void storeState(const ScanArgs &a, const ScanPlace &s, float *state, uint64_t which, const float (&h)[NP])
 {
@@ -125,15 +138,17 @@ template<int NP> __device__ inline void storeState(const ScanArgs &a, const Scan
 }
 template<int NP> __device__ inline void loadChunk(const ScanArgs &a, const ScanPlace &s, const float *chunks, uint32_t number, float (&h)[NP])
 {
+    const float *from = chunks + ((uint64_t)number * a.states + s.firstState) * a.channels;
     #pragma unroll
-    for(int n = 0; n < NP; n++) { h[n] = n < (int)s.numStates ? chunks[((uint64_t)number * a.states + s.firstState + n) * a.channels + s.channel] : 0.0f; }
+    for(int n = 0; n < NP; n++) { h[n] = (from + (uint64_t)min((uint32_t)n, s.numStates - 1) * a.channels)[s.channel]; }
 }
 template<int NP> __device__ inline void storeChunk(const ScanArgs &a, const ScanPlace &s, float *chunks, uint32_t number, const float (&h)[NP])
 {
     if(!s.active) { return; }
+    float *to = chunks + ((uint64_t)number * a.states + s.firstState) * a.channels;
     #pragma unroll
     for(int n = 0; n < NP; n++) {
-        if(n < (int)s.numStates) { chunks[((uint64_t)number * a.states + s.firstState + n) * a.channels + s.channel] = h[n]; }
+        if(n < (int)s.numStates) { (to + (uint64_t)n * a.channels)[s.channel] = h[n]; }
     }
 }
 
@@ -375,59 +390,40 @@ void scanTokenKernel(ScanArgs a)
     }
 }
 
-// Sums over the 64 lanes of M values a lane, M = 64 / 2^k: in every step two values become one register, whose halves hold the two sums so far.
-// Afterwards lane l has the sum of value laneValue<M>(l) in v[0].
-template<int M> __device__ inline void sumLanes(float (&v)[M])
-{
-    const uint32_t lane = threadIdx.x & 63;
-    int width = 32;
-    #pragma unroll
-    for(int m = M; m > 1; m /= 2) {
-        const bool upper = lane & width;
-        #pragma unroll
-        for(int i = 0; i < m / 2; i++) {
-            const float keep = upper ? v[i + m / 2] : v[i], send = upper ? v[i] : v[i + m / 2];
-            v[i] = keep + __shfl_xor(send, width);
-        }
-        width /= 2;
-    }
-    for(; width >= 1; width /= 2) { v[0] += __shfl_xor(v[0], width); }
-}
-// which value that is: bit by bit, the highest lane bit chose between the two halves of the values
-template<int M> __device__ inline uint32_t laneValue()
-{
-    const uint32_t lane = threadIdx.x & 63;
-    return lane / (64 / M);
-}
-
 // Gradients of a chunk, from the state before it and the gradient of the state behind it.  The states in between are made again, a block of
 // R rows at a time: first one walk forward that keeps the state before every block (LDS), then from the last block to the first one walk
 // forward through a block that keeps its states in registers, and one back:
 //   dh = C gy + (what comes from the row behind);  dC = gy h, dB = dh dt u (summed over channels);  q = sum dh B, x = dh exp(dt A) h', r = sum x A
 //   du = dt q + D gy;  d(dt) = u q + r;  dA += x dt;  and exp(dt A) dh for the row before
+// A block's walks take PART of the states at a time, so that R * PART of them fit the registers of two wavefronts a SIMD.
 template<typename T, int NP, int R, int BLOCKS, bool SLABS>
-__global__ __launch_bounds__(SLABS ? 512 : 64)
+__global__ __launch_bounds__(SLABS ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
 {
-    constexpr int WAVES = SLABS ? 8 : 1;
+    constexpr int PART = 4, PARTS = NP / PART, SPREAD = 64 / (2 * PART);     // SPREAD: lanes that have the same sum over the lanes
     extern __shared__ float lds[];
     uint32_t number;
     const ScanPlace s = scanPlace<NP>(a, number);
-    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, channel = s.channel;
     float *const kept = lds + (size_t)slab * ((BLOCKS - 1) * NP * 64 + R * 2 * NP);     // [block][state][lane]
     float *const bc = kept + (BLOCKS - 1) * NP * 64;
     float *const sums = lds + (size_t)a.slabs * ((BLOCKS - 1) * NP * 64 + R * 2 * NP);  // SLABS: [slab][row][q, r, y][lane]
-    float A[NP], h[NP], carry[NP], dA[NP], dD = 0.0f, dBias = 0.0f;
+    float dA[NP], dD = 0.0f, dBias = 0.0f;
     #pragma unroll
     for(int n = 0; n < NP; n++) { dA[n] = 0.0f; }
     if(s.valid) {
-        const T *u = rowsOf<const T>(a.u, a.sequences, s.place) + s.channel, *delta = rowsOf<const T>(a.delta, a.sequences, s.place) + s.channel;
-        const T *z = a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) + s.channel : nullptr;
-        const T *dout = rowsOf<const T>(g.out, a.sequences, s.place) + s.channel;
+        const T *u = rowsOf<const T>(a.u, a.sequences, s.place), *delta = rowsOf<const T>(a.delta, a.sequences, s.place);
+        const T *z = a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) : nullptr, *dout = rowsOf<const T>(g.out, a.sequences, s.place);
+        T *du = g.u.data ? rowsOf<T>(g.u, a.sequences, s.place) : nullptr, *ddelta = g.delta.data ? rowsOf<T>(g.delta, a.sequences, s.place) : nullptr;
+        T *dz = z && g.z.data ? rowsOf<T>(g.z, a.sequences, s.place) : nullptr;
         const uint32_t bcAt = s.group * a.states + s.firstState;
         const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
-        const float bias = a.deltaBias ? a.deltaBias[s.channel] : 0.0f, skip = a.D ? a.D[s.channel] : 0.0f;
-        const uint64_t sumRow = a.sequences.offsets ? s.place.first : (uint64_t)s.place.sequence * a.sequences.length;
+        const float bias = a.deltaBias ? a.deltaBias[channel] : 0.0f, skip = a.D ? a.D[channel] : 0.0f;
+        // Sums over the channels of a row: part p's are with the lanes that are p modulo SPREAD, so a row's are written by one store
+        const uint64_t sumRow = (uint64_t)s.tile * g.rows + (a.sequences.offsets ? s.place.first : (uint64_t)s.place.sequence * a.sequences.length);
+        const uint32_t sumState = (lane % SPREAD) * PART + (lane / SPREAD) % PART, sumAt = (lane / (32)) * a.states + s.firstState + sumState;
+        const bool sumHere = lane % SPREAD < PARTS && sumState < s.numStates;
+        float A[NP], h[NP], carry[NP];
         loadA<NP>(a, s, A);
         if(a.chunkState) { loadChunk<NP>(a, s, a.chunkState, number, h); loadChunk<NP>(a, s, g.chunkGradient, number, carry); }
         else { loadState<NP>(a, s, a.initialState, s.place.state, h); loadState<NP>(a, s, g.finalState, s.place.state, carry); }
@@ -435,17 +431,24 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
         StagedBC<T, NP, R> stage;
         for(uint32_t b = 0; b + 1 < blocks; b++) {
             const uint32_t row = s.first + b * R;
+            T rawU[R], rawDelta[R];
+            #pragma unroll
+            for(int r = 0; r < R; r++) {
+                rawU[r] = rowAt(u, row + r, a.u.rowStride)[channel];
+                rawDelta[r] = rowAt(delta, row + r, a.delta.rowStride)[channel];
+            }
+            stage.fetch(B, C, a, row, end, s.numStates);
             #pragma unroll
             for(int n = 0; n < NP; n++) { kept[(b * NP + n) * 64 + lane] = h[n]; }
-            stage.fetch(B, C, a, row, end, s.numStates);
             waveFence();
             stage.store(bc);
             waveFence();
             #pragma unroll
             for(int r = 0; r < R; r++) {
-                float dt = widen(delta[(uint64_t)(row + r) * a.delta.rowStride]) + bias;
-                if(a.softplus) { dt = softplusOf(dt); }
-                const float w = dt * widen(u[(uint64_t)(row + r) * a.u.rowStride]);
+                float dt = widen(rawDelta[r]) + bias;
+                dt = a.softplus ? softplusOf(dt) : dt;
+                const float w = dt * widen(rawU[r]);
+                readAfter(h[0], h[1], h[2], h[3]);
                 #pragma unroll
                 for(int n = 0; n < NP; n++) { h[n] = __builtin_fmaf(exp2Of(dt * A[n]), h[n], w * bc[r * 2 * NP + n]); }
             }
@@ -457,93 +460,119 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
                 for(int n = 0; n < NP; n++) { h[n] = kept[(b * NP + n) * 64 + lane]; }
             }
             stage.fetch(B, C, a, row, end, s.numStates);
+            float dt[R], uu[R], gy[R], slope[R], q[R], rr[R], y[R], both[R];
+            {
+                T rawDelta[R], rawU[R], rawOut[R], rawZ[R];
+                #pragma unroll
+                for(int r = 0; r < R; r++) {
+                    const uint32_t t = min(row + r, end - 1);
+                    rawDelta[r] = rowAt(delta, t, a.delta.rowStride)[channel];
+                    rawU[r] = rowAt(u, t, a.u.rowStride)[channel];
+                    rawOut[r] = rowAt(dout, t, g.out.rowStride)[channel];
+                }
+                if(z) {
+                    #pragma unroll
+                    for(int r = 0; r < R; r++) { rawZ[r] = rowAt(z, min(row + r, end - 1), a.z.rowStride)[channel]; }
+                    #pragma unroll
+                    for(int r = 0; r < R; r++) { const float zr = widen(rawZ[r]); gy[r] = widen(rawOut[r]) * (zr * logistic(zr)); }
+                }
+                else {
+                    #pragma unroll
+                    for(int r = 0; r < R; r++) { gy[r] = widen(rawOut[r]); }
+                }
+                #pragma unroll
+                for(int r = 0; r < R; r++) {
+                    // (rows behind the end, and lanes without a channel: dt, u and gradient 0 leave everything as it is)
+                    const bool there = row + r < end && s.active;
+                    const float raw = widen(rawDelta[r]) + bias;
+                    const float time = a.softplus ? softplusOf(raw) : raw;
+                    slope[r] = a.softplus ? logistic(raw) : 1.0f;
+                    dt[r] = there ? time : 0.0f;
+                    uu[r] = there ? widen(rawU[r]) : 0.0f;
+                    gy[r] = there ? gy[r] : 0.0f;
+                    q[r] = rr[r] = y[r] = both[r] = 0.0f;
+                }
+            }
             waveFence();
             stage.store(bc);
             waveFence();
-            float hs[R][NP], dt[R], raw[R], uu[R], gy[R], zz[R], dd[R];
-            #pragma unroll
-            for(int r = 0; r < R; r++) {
-                // (rows behind the end, and lanes without a channel: dt, u and gradient 0 leave everything as it is)
-                const bool there = row + r < end && s.active;
-                const uint64_t t = min(row + r, end - 1);
-                raw[r] = widen(delta[t * a.delta.rowStride]) + bias;
-                dt[r] = there ? (a.softplus ? softplusOf(raw[r]) : raw[r]) : 0.0f;
-                uu[r] = there ? widen(u[t * a.u.rowStride]) : 0.0f;
-                dd[r] = there ? widen(dout[t * g.out.rowStride]) : 0.0f;
-                zz[r] = z && there ? widen(z[t * a.z.rowStride]) : 0.0f;
-                gy[r] = z ? dd[r] * zz[r] * logistic(zz[r]) : dd[r];
-                const float w = dt[r] * uu[r];
-                #pragma unroll
-                for(int n = 0; n < NP; n++) { hs[r][n] = __builtin_fmaf(exp2Of(dt[r] * A[n]), r ? hs[r - 1][n] : h[n], w * bc[r * 2 * NP + n]); }
-            }
-            #pragma unroll
-            for(int r = R - 1; r >= 0; r--) {
-                const float w = dt[r] * uu[r];
-                float q = 0.0f, rr = 0.0f, y = 0.0f, both[2 * NP];
-                #pragma unroll
-                for(int n = 0; n < NP; n++) {
-                    const float Bn = bc[r * 2 * NP + n], Cn = bc[(r * 2 + 1) * NP + n];
-                    const float decay = exp2Of(dt[r] * A[n]);
-                    const float dh = __builtin_fmaf(gy[r], Cn, carry[n]);
-                    y = __builtin_fmaf(Cn, hs[r][n], y);
-                    both[n] = dh * w;
-                    both[NP + n] = gy[r] * hs[r][n];
-                    q = __builtin_fmaf(dh, Bn, q);
-                    carry[n] = decay * dh;
-                    const float x = carry[n] * (r ? hs[r - 1][n] : h[n]);
-                    dA[n] = __builtin_fmaf(x, dt[r], dA[n]);
-                    rr = __builtin_fmaf(x, A[n], rr);
+            // what a row's channel gets, when its sums over the states are there
+            const auto finish = [&](int r) {
+                const uint32_t t = row + r;
+                if(!s.active) { return; }
+                if(du) { rowAt(du, t, g.u.rowStride)[channel] = narrow<T>(__builtin_fmaf(dt[r], q[r], skip * gy[r])); }
+                const float d = __builtin_fmaf(uu[r], q[r], rr[r] * LN2) * slope[r];
+                if(ddelta) { rowAt(ddelta, t, g.delta.rowStride)[channel] = narrow<T>(d); }
+                if(dz) {
+                    const float zr = widen(rowAt(z, t, a.z.rowStride)[channel]), sig = logistic(zr), dd = widen(rowAt(dout, t, g.out.rowStride)[channel]);
+                    rowAt(dz, t, g.z.rowStride)[channel] = narrow<T>(dd * __builtin_fmaf(skip, uu[r], y[r]) * (sig * (1.0f + zr * (1.0f - sig))));
                 }
-                if(g.sumBC) {
-                    sumLanes<2 * NP>(both);
-                    const uint32_t value = laneValue<2 * NP>(), n = value % NP, which = value / NP;
-                    if(row + r < end && lane % (32 / NP) == 0 && n < s.numStates) {
-                        g.sumBC[(((uint64_t)s.tile * g.rows + sumRow + row + r) * 2 + which) * a.states + s.firstState + n] = both[0];
+                dBias += d;
+                dD = __builtin_fmaf(gy[r], uu[r], dD);
+            };
+            #pragma unroll
+            for(int part = 0; part < PARTS; part++) {
+                float hs[R][PART], start[PART];
+                #pragma unroll
+                for(int k = 0; k < PART; k++) { start[k] = h[part * PART + k]; }
+                #pragma unroll
+                for(int r = 0; r < R; r++) {
+                    const float w = dt[r] * uu[r];
+                    float (&before)[PART] = r ? hs[r - 1] : start;
+                    readAfter(before[0], before[1], before[2], before[3]);
+                    #pragma unroll
+                    for(int k = 0; k < PART; k++) {
+                        const int n = part * PART + k;
+                        hs[r][k] = __builtin_fmaf(exp2Of(dt[r] * A[n]), before[k], w * bc[r * 2 * NP + n]);
                     }
                 }
-                if(SLABS) {
-                    sums[((slab * R + r) * 3) * 64 + lane] = q;
-                    sums[((slab * R + r) * 3 + 1) * 64 + lane] = rr;
-                    sums[((slab * R + r) * 3 + 2) * 64 + lane] = y;
-                }
-                else if(row + r < end && s.active) {
-                    const uint64_t t = row + r;
-                    if(g.u.data) { rowsOf<T>(g.u, a.sequences, s.place)[t * g.u.rowStride + s.channel] = narrow<T>(__builtin_fmaf(dt[r], q, skip * gy[r])); }
-                    float d = __builtin_fmaf(uu[r], q, rr * LN2);
-                    if(a.softplus) { d *= logistic(raw[r]); }
-                    if(g.delta.data) { rowsOf<T>(g.delta, a.sequences, s.place)[t * g.delta.rowStride + s.channel] = narrow<T>(d); }
-                    if(z && g.z.data) {
-                        const float sig = logistic(zz[r]);
-                        rowsOf<T>(g.z, a.sequences, s.place)[t * g.z.rowStride + s.channel] =
-                            narrow<T>(dd[r] * __builtin_fmaf(skip, uu[r], y) * (sig * (1.0f + zz[r] * (1.0f - sig))));
+                #pragma unroll
+                for(int r = R - 1; r >= 0; r--) {
+                    const float time = again(dt[r]), w = time * uu[r];
+                    const float (&before)[PART] = r ? hs[r - 1] : start;
+                    if(r < R - 1) { readAfter(q[r + 1], rr[r + 1], y[r + 1], both[r + 1]); }
+                    readAfter(carry[part * PART], carry[part * PART + 1], carry[part * PART + 2], carry[part * PART + 3]);
+                    readAfter(dA[part * PART], dA[part * PART + 1], dA[part * PART + 2], dA[part * PART + 3]);
+                    float terms[2 * PART];
+                    #pragma unroll
+                    for(int k = 0; k < PART; k++) {
+                        const int n = part * PART + k;
+                        const float Bn = bc[r * 2 * NP + n], Cn = bc[(r * 2 + 1) * NP + n];
+                        const float dh = __builtin_fmaf(gy[r], Cn, carry[n]);
+                        y[r] = __builtin_fmaf(Cn, hs[r][k], y[r]);
+                        terms[k] = dh * w;
+                        terms[PART + k] = gy[r] * hs[r][k];
+                        q[r] = __builtin_fmaf(dh, Bn, q[r]);
+                        carry[n] = exp2Of(time * A[n]) * dh;
+                        const float x = carry[n] * before[k];
+                        dA[n] = __builtin_fmaf(x, time, dA[n]);
+                        rr[r] = __builtin_fmaf(x, A[n], rr[r]);
                     }
-                    dBias += d;
-                    dD = __builtin_fmaf(gy[r], uu[r], dD);
+                    const float sum = gennmi_lanes::sumOfLanes<2 * PART>(terms);
+                    both[r] = lane % SPREAD == part ? sum : both[r];
+                    if(part == PARTS - 1 && row + r < end) {
+                        if(sumHere) { (g.sumBC + (sumRow + row + r) * 2 * a.states)[sumAt] = both[r]; }
+                        if(SLABS) {
+                            sums[((slab * R + r) * 3) * 64 + lane] = q[r];
+                            sums[((slab * R + r) * 3 + 1) * 64 + lane] = rr[r];
+                            sums[((slab * R + r) * 3 + 2) * 64 + lane] = y[r];
+                        }
+                        else { finish(r); }
+                    }
                 }
             }
             if(SLABS) {
                 __syncthreads();
                 #pragma unroll
                 for(int r = 0; r < R; r++) {
-                    if(row + r < end && r % a.slabs == slab && s.active) {
-                        const uint64_t t = row + r;
-                        float q = 0.0f, rr = 0.0f, y = 0.0f;
+                    if(r % a.slabs == slab && row + r < end) {
+                        q[r] = rr[r] = y[r] = 0.0f;
                         for(uint32_t k = 0; k < a.slabs; k++) {
-                            q += sums[((k * R + r) * 3) * 64 + lane];
-                            rr += sums[((k * R + r) * 3 + 1) * 64 + lane];
-                            y += sums[((k * R + r) * 3 + 2) * 64 + lane];
+                            q[r] += sums[((k * R + r) * 3) * 64 + lane];
+                            rr[r] += sums[((k * R + r) * 3 + 1) * 64 + lane];
+                            y[r] += sums[((k * R + r) * 3 + 2) * 64 + lane];
                         }
-                        if(g.u.data) { rowsOf<T>(g.u, a.sequences, s.place)[t * g.u.rowStride + s.channel] = narrow<T>(__builtin_fmaf(dt[r], q, skip * gy[r])); }
-                        float d = __builtin_fmaf(uu[r], q, rr * LN2);
-                        if(a.softplus) { d *= logistic(raw[r]); }
-                        if(g.delta.data) { rowsOf<T>(g.delta, a.sequences, s.place)[t * g.delta.rowStride + s.channel] = narrow<T>(d); }
-                        if(z && g.z.data) {
-                            const float sig = logistic(zz[r]);
-                            rowsOf<T>(g.z, a.sequences, s.place)[t * g.z.rowStride + s.channel] =
-                                narrow<T>(dd[r] * __builtin_fmaf(skip, uu[r], y) * (sig * (1.0f + zz[r] * (1.0f - sig))));
-                        }
-                        dBias += d;
-                        dD = __builtin_fmaf(gy[r], uu[r], dD);
+                        finish(r);
                     }
                 }
                 __syncthreads();
@@ -551,26 +580,27 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
         }
         if(!a.chunkState) { storeState<NP>(a, s, g.initialState, s.place.state, carry); }
     }
-    // (numbers without a chunk leave zeros)
-    if(g.sumA) { storeChunk<NP>(a, s, g.sumA, number, dA); }
+    // Sums over the chunk (numbers without a chunk leave zeros)
+    float *const to = g.sums + (uint64_t)number * (a.states + 2) * a.channels;
     if(s.active) {
-        const uint64_t at = ((uint64_t)number * a.slabs + slab) * a.channels + s.channel;
-        if(g.sumD) { g.sumD[at] = dD; }
-        if(g.sumBias) { g.sumBias[at] = dBias; }
+        #pragma unroll
+        for(int n = 0; n < NP; n++) { if(n < (int)s.numStates) { (to + (uint64_t)(s.firstState + n) * a.channels)[channel] = dA[n]; } }
+    }
+    if(SLABS) {
+        sums[(slab * 2) * 64 + lane] = dD;
+        sums[(slab * 2 + 1) * 64 + lane] = dBias;
+        __syncthreads();
+        if(slab == 0) {
+            dD = dBias = 0.0f;
+            for(uint32_t k = 0; k < a.slabs; k++) { dD += sums[(k * 2) * 64 + lane]; dBias += sums[(k * 2 + 1) * 64 + lane]; }
+        }
+    }
+    if(slab == 0 && s.active) {
+        (to + (uint64_t)a.states * a.channels)[channel] = dD;
+        (to + (uint64_t)(a.states + 1) * a.channels)[channel] = dBias;
     }
 }
 
-// Sums over the chunks of what belongs to a channel, in 64 bits: out[channel][n] of sums[number][n][channel]
-__global__ __launch_bounds__(256)
-void scanChannelSumKernel(const float *sums, uint32_t numbers, uint32_t each, uint32_t channels, uint32_t width, float *out)
-{
-    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if(item >= (uint64_t)channels * width) { return; }
-    const uint32_t n = (uint32_t)(item / channels), c = (uint32_t)(item - (uint64_t)n * channels);
-    double sum = 0.0;
-    for(uint64_t k = 0; k < (uint64_t)numbers * each; k++) { sum += sums[(k * width + n) * channels + c]; }
-    out[(uint64_t)c * width + n] = (float)sum;
-}
 // Sums over a group's tiles of what belongs to a row
 template<typename T>
 __global__ __launch_bounds__(256)

@@ -5,6 +5,41 @@
 using namespace gennmi_elements;
 using gennmi_detail::fail;
 
+namespace
+{
+// Sums over chunks, sums[number][n][channel], in 64 bits: there may be thousands, of either sign.  Row n of the sums goes to out[channel][n] for n < width,
+// behind those to more[0][channel] and more[1][channel].  The 16 wavefronts of a work-group have 64 channels and a sixteenth of the numbers each;
+// what they found is added up in the order of the numbers.
+struct ChunkSums { const float *sums; float *out, *more[2]; uint32_t numbers, channels, width, rows; };
+__global__ __launch_bounds__(1024)
+void chunkSumKernel(ChunkSums a)
+{
+    __shared__ double found[16][64];
+    const uint32_t parts = (a.channels + 63) / 64, n = blockIdx.x / parts, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t channel = (blockIdx.x - n * parts) * 64 + lane;
+    const uint32_t each = (a.numbers + 15) / 16, first = min(wave * each, a.numbers), last = min(first + each, a.numbers);
+    double sum = 0.0;
+    if(channel < a.channels) {
+        const float *at = a.sums + (uint64_t)n * a.channels + channel;
+        #pragma unroll 8
+        for(uint32_t k = first; k < last; k++) { sum += at[(uint64_t)k * a.rows * a.channels]; }
+    }
+    found[wave][lane] = sum;
+    __syncthreads();
+    if(wave || channel >= a.channels) { return; }
+    #pragma unroll
+    for(int k = 1; k < 16; k++) { sum += found[k][lane]; }
+    if(n < a.width) { if(a.out) { a.out[(uint64_t)channel * a.width + n] = (float)sum; } }
+    else if(a.more[n - a.width]) { a.more[n - a.width][channel] = (float)sum; }
+}
+int launchChunkSum(const char *what, const ChunkSums &a, hipStream_t stream)
+{
+    chunkSumKernel<<<dim3(a.rows * ((a.channels + 63) / 64)), dim3(1024), 0, stream>>>(a);
+    return gennmi_detail::afterLaunch(what);
+}
+}
+
+#include "genn_mi355x_lanes.h"
 #include "genn_mi355x_causal_conv_kernels.h"
 #include "genn_mi355x_scan_kernels.h"
 
@@ -157,7 +192,7 @@ ScanPlan scanPlan(const gennmi_scan_t &c, bool gradients)
     p.split = c.sequences.length > p.chunk;
     return p;
 }
-struct ScanSpace { size_t state, time, gradient, sumA, sumD, sumBias, sumBC, bytes; };
+struct ScanSpace { size_t state, time, gradient, sums, sumBC, bytes; };
 ScanSpace scanSpace(const gennmi_scan_t &c, const ScanPlan &p, bool gradients)
 {
     ScanSpace s{};
@@ -169,9 +204,7 @@ ScanSpace scanSpace(const gennmi_scan_t &c, const ScanPlan &p, bool gradients)
     }
     if(gradients) {
         if(p.split) { s.gradient = take(numbers * c.states * c.channels); }
-        s.sumA = take(numbers * c.states * c.channels);
-        s.sumD = take(numbers * p.slabs * c.channels);
-        s.sumBias = take(numbers * p.slabs * c.channels);
+        s.sums = take(numbers * (c.states + 2) * c.channels);
         s.sumBC = take((uint64_t)scanTiles(c) * totalRows(c.sequences) * 2 * c.states);
     }
     return s;
@@ -312,10 +345,8 @@ int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_c
         a.partial = sums ? (float*)workspace : nullptr;
         if(const int rc = runConv(what, *conv, convVector(*conv, gradient), &a, (hipStream_t)stream)) { return rc; }
         if(sums) {
-            const uint64_t items = (uint64_t)conv->channels * (conv->taps + 1);
-            causalConvReduceKernel<<<dim3((uint32_t)((items + 255) / 256)), dim3(256), 0, (hipStream_t)stream>>>(a.partial, (uint32_t)chunkNumbers(conv->sequences, convChunk(*conv)),
-                                                                                                                conv->channels, conv->taps, g.weight, g.bias);
-            if(const int rc = gennmi_detail::afterLaunch(what)) { return rc; }
+            const ChunkSums c{a.partial, g.weight, {g.bias, nullptr}, (uint32_t)chunkNumbers(conv->sequences, convChunk(*conv)), conv->channels, conv->taps, conv->taps + 1};
+            if(const int rc = launchChunkSum(what, c, (hipStream_t)stream)) { return rc; }
         }
         noteRows(g.x, conv->sequences, conv->channels, size);
         if(g.initialState) { gennmi_detail::noteDeviceWrite(g.initialState, (uint64_t)conv->sequences.count * (conv->taps - 1) * conv->channels * size); }
@@ -421,30 +452,24 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
             a.chunkTime = at(space.time);
             g.chunkGradient = at(space.gradient);
         }
-        g.sumA = in.A ? at(space.sumA) : nullptr;
-        g.sumD = in.D ? at(space.sumD) : nullptr;
-        g.sumBias = in.deltaBias ? at(space.sumBias) : nullptr;
-        g.sumBC = in.B.data || in.C.data ? at(space.sumBC) : nullptr;
+        g.sums = at(space.sums);
+        g.sumBC = at(space.sumBC);      // (written whatever gradients are asked for)
         g.rows = rows;
         const hipStream_t s = (hipStream_t)stream;
         if(a.numbers) {
             const int rc = withType(scan->type, [&](auto t) {
                 typedef decltype(t) T;
                 const int rcScan = withStates(p, [&](auto np, auto slabs) { return launchScanBackward<T, decltype(np)::value, decltype(slabs)::value>(a, g, p, s); });
-                if(rcScan || !g.sumBC || !rows) { return rcScan; }
+                if(rcScan || !(in.B.data || in.C.data) || !rows) { return rcScan; }
                 scanRowSumKernel<T><<<dim3((uint32_t)((rows * 2 * width + 255) / 256)), dim3(256), 0, s>>>(a, g);
                 return gennmi_detail::afterLaunch(what);
             });
             if(rc) { return rc; }
         }
-        const struct { float *out, *sums; uint32_t each, width; } channelSums[] = {
-            {in.A, g.sumA, 1, scan->states}, {in.D, g.sumD, p.slabs, 1}, {in.deltaBias, g.sumBias, p.slabs, 1}};
-        for(const auto &c : channelSums) {
-            if(!c.out) { continue; }
-            const uint64_t items = (uint64_t)scan->channels * c.width;
-            scanChannelSumKernel<<<dim3((uint32_t)((items + 255) / 256)), dim3(256), 0, s>>>(c.sums, a.numbers, c.each, scan->channels, c.width, c.out);
-            if(const int rc = gennmi_detail::afterLaunch(what)) { return rc; }
-            gennmi_detail::noteDeviceWrite(c.out, items * sizeof(float));
+        if(in.A || in.D || in.deltaBias) {
+            if(const int rc = launchChunkSum(what, {g.sums, in.A, {in.D, in.deltaBias}, a.numbers, a.channels, a.states, a.states + 2}, s)) { return rc; }
+            const struct { float *out; uint64_t count; } sums[] = {{in.A, (uint64_t)a.channels * a.states}, {in.D, a.channels}, {in.deltaBias, a.channels}};
+            for(const auto &c : sums) { if(c.out) { gennmi_detail::noteDeviceWrite(c.out, c.count * sizeof(float)); } }
         }
         for(const auto &w : written) { noteRows(*w.rows, scan->sequences, w.width, size); }
         if(in.initialState) { gennmi_detail::noteDeviceWrite(in.initialState, (uint64_t)scan->sequences.count * scan->channels * scan->states * sizeof(float)); }

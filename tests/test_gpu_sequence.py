@@ -205,6 +205,35 @@ def test_selective_scan(lengths, channels, states, groups, dtype, softplus, gate
     assert all(torch.equal(first[n], g) for n, g in grads.items())
 
 
+@pytest.mark.parametrize("states", [7, 16, 40])
+def test_gradients_asked_for_one_by_one(states):
+    """Whichever are asked for, they are the same, and nothing else is written."""
+    from genn_amd.sequence import CausalConvolution, SelectiveScan
+    r, S, n, D, N, K = generator(states), 2, 75, 66, states, 4
+    on = lambda *shape: r(*shape).cuda()
+    s = SelectiveScan(S, n, D, N, softplus=True)
+    s.bind(u=on(S, n, D), delta=on(S, n, D), A=-torch.rand(D, N).cuda(), B=on(S, n, N), C=on(S, n, N), D=on(D), delta_bias=on(D), z=on(S, n, D), initial_state=on(S, D, N))
+    c = CausalConvolution(S, n, D, K, silu=True)
+    c.bind(x=on(S, n, D), weight=on(D, K), bias=on(D), initial_state=on(S, K - 1, D))
+    row = (S, n, D)
+    for op, shapes in ((s, dict(u=row, delta=row, z=row, A=(D, N), B=(S, n, N), C=(S, n, N), D=(D,), delta_bias=(D,), initial_state=(S, D, N))),
+                       (c, dict(x=row, weight=(D, K), bias=(D,), initial_state=(S, K - 1, D)))):
+        dout = on(S, n, D)
+        every = {k: torch.zeros(shape).cuda() for k, shape in shapes.items()}
+        op.bind_gradients(out=dout, **every)
+        op.backward()
+        torch.cuda.synchronize()
+        for name, shape in shapes.items():
+            one = torch.zeros(shape).cuda()
+            op.bind_gradients(out=dout, **{name: one})
+            op.backward()
+            torch.cuda.synchronize()
+            assert torch.equal(one, every[name]) and one.abs().sum() > 0, name
+        op.bind_gradients(out=dout)
+        op.backward()
+        torch.cuda.synchronize()
+
+
 def test_tokens_continue_a_prompt_and_padding_is_left_alone():
     """A prompt's state, then one row at a time, gives what the whole sequence gives; sequences whose slot is none are neither read nor written."""
     from genn_amd.sequence import CausalConvolution, SelectiveScan
