@@ -27,12 +27,23 @@ struct ConvGradientArgs
 
 __device__ inline float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f)); }
 
-template<typename T, int VEC> __device__ inline void loadRow(const T *from, float (&to)[VEC])
+template<typename T, int VEC> __device__ inline void widenRow(const Pack<T, VEC> &p, float (&to)[VEC])
 {
-    const Pack<T, VEC> p = *(const Pack<T, VEC>*)from;
     #pragma unroll
     for(int v = 0; v < VEC; v++) { to[v] = widen(p.v[v]); }
 }
+template<typename T, int VEC> __device__ inline void loadRow(const T *from, float (&to)[VEC]) { widenRow<T, VEC>(*(const Pack<T, VEC>*)from, to); }
+// AHEAD rows on their way while as many before them are worked on; behind row `last` that one again
+constexpr int AHEAD = 4;
+template<typename T, int VEC> struct RowsAhead
+{
+    Pack<T, VEC> raw[AHEAD];
+    __device__ inline void fetch(const T *rows, uint64_t stride, uint32_t row, uint32_t last)
+    {
+        #pragma unroll
+        for(int r = 0; r < AHEAD; r++) { raw[r] = *(const Pack<T, VEC>*)(rows + (uint64_t)min(row + r, last) * stride); }
+    }
+};
 template<typename T, int VEC> __device__ inline void storeRow(T *to, const float (&from)[VEC])
 {
     Pack<T, VEC> p;
@@ -131,29 +142,35 @@ template<typename T, int K, int VEC>
 __global__ __launch_bounds__(256)
 void causalConvKernel(ConvArgs a)
 {
-    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint32_t number = (uint32_t)(item / a.vectors);
-    if(number >= a.numbers) { return; }
-    const uint32_t channel = (uint32_t)(item - (uint64_t)number * a.vectors) * VEC;
+    uint32_t number, channel;
+    divideItem(a.vectors, number, channel);
+    channel *= VEC;
     Place p;
-    if(!convPlace(a, number, p)) { return; }
+    if(number >= a.numbers || !convPlace(a, number, p)) { return; }
     const T *x = rowsOf<const T>(a.x, a.sequences, p);
-    T *out = rowsOf<T>(a.out, a.sequences, p);
+    T *out = rowsOf<T>(a.out, a.sequences, p) + channel;
     const uint32_t first = p.index * a.sequences.chunk, last = (uint32_t)min((uint64_t)first + a.sequences.chunk, (uint64_t)p.length);
     float w[K][VEC], window[K][VEC], bias[VEC];
+    RowsAhead<T, VEC> next;
+    if(first < last) { next.fetch(x + channel, a.x.rowStride, first, last - 1); }
     loadWindow<T, K, VEC>(a, x, p, first, channel, window);
     if(K > 1 && p.index == 0 && a.finalState) { storeState<T, K, VEC>(a, x, p, channel, window); }
     loadWeights<K, VEC>(a, channel, w, bias);
-    for(uint32_t t = first; t < last; t++) {
-        shift<K, VEC>(window);
-        loadRow<T, VEC>(x + (uint64_t)t * a.x.rowStride + channel, window[K - 1]);
-        float s[VEC];
-        product<K, VEC>(w, window, bias, s);
-        if(a.silu) {
-            #pragma unroll
-            for(int v = 0; v < VEC; v++) { s[v] *= sigmoid(s[v]); }
+    for(uint32_t t = first; t < last; t += AHEAD) {
+        const RowsAhead<T, VEC> rows = next;
+        if(t + AHEAD < last) { next.fetch(x + channel, a.x.rowStride, t + AHEAD, last - 1); }
+        #pragma unroll
+        for(int r = 0; r < AHEAD; r++) {
+            shift<K, VEC>(window);
+            widenRow<T, VEC>(rows.raw[r], window[K - 1]);
+            float s[VEC];
+            product<K, VEC>(w, window, bias, s);
+            if(a.silu) {
+                #pragma unroll
+                for(int v = 0; v < VEC; v++) { s[v] *= sigmoid(s[v]); }
+            }
+            if(t + r < last) { storeRow<T, VEC>(out + (uint64_t)(t + r) * a.out.rowStride, s); }
         }
-        storeRow<T, VEC>(out + (uint64_t)t * a.out.rowStride + channel, s);
     }
 }
 
@@ -165,10 +182,10 @@ template<typename T, int K, int VEC>
 __global__ __launch_bounds__(256)
 void causalConvBackwardKernel(ConvArgs a, ConvGradientArgs g)
 {
-    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint32_t number = (uint32_t)(item / a.vectors);
+    uint32_t number, channel;
+    divideItem(a.vectors, number, channel);
+    channel *= VEC;
     if(number >= a.numbers) { return; }
-    const uint32_t channel = (uint32_t)(item - (uint64_t)number * a.vectors) * VEC;
     float w[K][VEC], window[K][VEC], bias[VEC], ds[K][VEC], dw[K][VEC], db[VEC];
     #pragma unroll
     for(int v = 0; v < VEC; v++) {
@@ -183,54 +200,73 @@ void causalConvBackwardKernel(ConvArgs a, ConvGradientArgs g)
         T *dstate = (T*)g.initialState;
         const T *dfinal = (const T*)g.finalState;
         const uint32_t first = p.index * a.sequences.chunk, last = (uint32_t)min((uint64_t)first + a.sequences.chunk, (uint64_t)p.length);
+        RowsAhead<T, VEC> nextX, nextOut;
+        if(p.length) {
+            nextX.fetch(x + channel, a.x.rowStride, first, p.length - 1);
+            nextOut.fetch(dout + channel, g.out.rowStride, first, p.length - 1);
+        }
         loadWindow<T, K, VEC>(a, x, p, first, channel, window);
         loadWeights<K, VEC>(a, channel, w, bias);
         // (dx of rows before `last`; in the first chunk of rows -(K - 1) on)
         const long long from = p.index == 0 ? -(long long)(K - 1) : (long long)first;
-        for(uint64_t t = first; t < (uint64_t)last + (K - 1); t++) {
-            shift<K, VEC>(window);
-            shift<K, VEC>(ds);
-            if(t < p.length) {
-                loadRow<T, VEC>(x + t * a.x.rowStride + channel, window[K - 1]);
-                loadRow<T, VEC>(dout + t * g.out.rowStride + channel, ds[K - 1]);
-                if(a.silu) {
-                    float s[VEC];
-                    product<K, VEC>(w, window, bias, s);
-                    #pragma unroll
-                    for(int v = 0; v < VEC; v++) { const float q = sigmoid(s[v]); ds[K - 1][v] *= q * (1.0f + s[v] * (1.0f - q)); }
-                }
-                if(t < last) {
+        const uint32_t walk = last + (K - 1);
+        for(uint32_t group = first; group < walk; group += AHEAD) {
+            const RowsAhead<T, VEC> rowsX = nextX, rowsOut = nextOut;
+            if(group + AHEAD < walk && p.length) {
+                nextX.fetch(x + channel, a.x.rowStride, group + AHEAD, p.length - 1);
+                nextOut.fetch(dout + channel, g.out.rowStride, group + AHEAD, p.length - 1);
+            }
+            // Rows that need no looking after: all of the chunk's own, and so are those whose dx is complete with them
+            const bool plain = (long long)group - (K - 1) >= (long long)first && group + AHEAD <= last;
+            const auto walkRows = [&](auto known) {
+                constexpr bool PLAIN = decltype(known)::value;
+                #pragma unroll
+                for(int r = 0; r < AHEAD; r++) {
+                    const uint32_t t = group + r;
+                    shift<K, VEC>(window);
+                    shift<K, VEC>(ds);
+                    // (ds of rows that are not there is zero, and their inputs, which may be anything, count for nothing)
+                    widenRow<T, VEC>(rowsX.raw[r], window[K - 1]);
+                    widenRow<T, VEC>(rowsOut.raw[r], ds[K - 1]);
+                    if(a.silu) {
+                        float s[VEC];
+                        product<K, VEC>(w, window, bias, s);
+                        #pragma unroll
+                        for(int v = 0; v < VEC; v++) { const float q = sigmoid(s[v]); ds[K - 1][v] *= q * (1.0f + s[v] * (1.0f - q)); }
+                    }
+                    if(!PLAIN && t >= p.length) {
+                        #pragma unroll
+                        for(int v = 0; v < VEC; v++) { ds[K - 1][v] = 0.0f; }
+                    }
+                    if(PLAIN || t < last) {
+                        #pragma unroll
+                        for(int v = 0; v < VEC; v++) {
+                            db[v] += ds[K - 1][v];
+                            #pragma unroll
+                            for(int k = 0; k < K; k++) { dw[k][v] = __builtin_fmaf(ds[K - 1][v], window[k][v], dw[k][v]); }
+                        }
+                    }
+                    const long long row = (long long)t - (K - 1);
+                    if(!PLAIN && !(row >= from && t < walk)) { continue; }
+                    float d[VEC];
                     #pragma unroll
                     for(int v = 0; v < VEC; v++) {
-                        db[v] += ds[K - 1][v];
+                        d[v] = 0.0f;
                         #pragma unroll
-                        for(int k = 0; k < K; k++) { dw[k][v] = __builtin_fmaf(ds[K - 1][v], window[k][v], dw[k][v]); }
+                        for(int k = 0; k < K; k++) { d[v] = __builtin_fmaf(w[k][v], ds[K - 1 - k][v], d[v]); }
                     }
+                    const long long behind = row - ((long long)p.length - (K - 1));         // its place in the final state
+                    if(!PLAIN && dfinal && behind >= 0) {
+                        float f[VEC];
+                        loadRow<T, VEC>(dfinal + ((uint64_t)p.state * (K - 1) + (uint64_t)behind) * a.channels + channel, f);
+                        #pragma unroll
+                        for(int v = 0; v < VEC; v++) { d[v] += f[v]; }
+                    }
+                    if(PLAIN || row >= 0) { if(dx) { storeRow<T, VEC>(dx + (uint64_t)row * g.x.rowStride + channel, d); } }
+                    else if(dstate) { storeRow<T, VEC>(dstate + ((uint64_t)p.state * (K - 1) + (uint64_t)(row + K - 1)) * a.channels + channel, d); }
                 }
-            }
-            else {
-                #pragma unroll
-                for(int v = 0; v < VEC; v++) { ds[K - 1][v] = 0.0f; }
-            }
-            const long long row = (long long)t - (K - 1);
-            if(row >= from) {
-                float d[VEC];
-                #pragma unroll
-                for(int v = 0; v < VEC; v++) {
-                    d[v] = 0.0f;
-                    #pragma unroll
-                    for(int k = 0; k < K; k++) { d[v] = __builtin_fmaf(w[k][v], ds[K - 1 - k][v], d[v]); }
-                }
-                const long long behind = row - ((long long)p.length - (K - 1));         // its place in the final state
-                if(dfinal && behind >= 0) {
-                    float f[VEC];
-                    loadRow<T, VEC>(dfinal + ((uint64_t)p.state * (K - 1) + (uint64_t)behind) * a.channels + channel, f);
-                    #pragma unroll
-                    for(int v = 0; v < VEC; v++) { d[v] += f[v]; }
-                }
-                if(row >= 0) { if(dx) { storeRow<T, VEC>(dx + (uint64_t)row * g.x.rowStride + channel, d); } }
-                else if(dstate) { storeRow<T, VEC>(dstate + ((uint64_t)p.state * (K - 1) + (uint64_t)(row + K - 1)) * a.channels + channel, d); }
-            }
+            };
+            if(__all(plain)) { walkRows(std::true_type{}); } else { walkRows(std::false_type{}); }
         }
     }
     if(g.partial) {

@@ -152,6 +152,39 @@ template<int NP> __device__ inline void storeChunk(const ScanArgs &a, const Scan
     }
 }
 
+// One row of a channel's array, R of them, fetched a block of rows before they are needed (rows behind the last one are that one again)
+template<typename T, int R> struct StagedRows
+{
+    T raw[R];
+    __device__ inline void fetch(const T *rows, uint64_t stride, uint32_t channel, uint32_t row, uint32_t end)
+    {
+        #pragma unroll
+        for(int r = 0; r < R; r++) { raw[r] = rowAt(rows, min(row + r, end - 1), stride)[channel]; }
+    }
+};
+// dt and dt u of a block of rows; zero behind the end, which leaves every state as it is
+template<typename T, int R>
+__device__ inline void times(const ScanArgs &a, const StagedRows<T, R> &delta, const StagedRows<T, R> &u, float bias, uint32_t there, float (&dt)[R], float (&w)[R])
+{
+    #pragma unroll
+    for(int r = 0; r < R; r++) { dt[r] = widen(delta.raw[r]) + bias; }
+    if(a.softplus) {
+        #pragma unroll
+        for(int r = 0; r < R; r++) { dt[r] = softplusOf(dt[r]); }
+    }
+    #pragma unroll
+    for(int r = 0; r < R; r++) {
+        dt[r] = r < (int)there ? dt[r] : 0.0f;
+        w[r] = r < (int)there ? dt[r] * widen(u.raw[r]) : 0.0f;
+    }
+}
+// The gate, z sigmoid(z)
+template<typename T, int R> __device__ inline void gates(const StagedRows<T, R> &z, float (&gate)[R])
+{
+    #pragma unroll
+    for(int r = 0; r < R; r++) { const float x = widen(z.raw[r]); gate[r] = x * logistic(x); }
+}
+
 // First kernel of a split scan: every chunk from a state of zero.  With GRADIENT also sum_t (prod_{s <= t} exp(dt_s A)) C_t g_t, what the chunk's rows
 // give the gradient of the state before it.
 template<typename T, int NP, bool GRADIENT, bool SLABS>
@@ -163,64 +196,103 @@ void scanChunkKernel(ScanArgs a, ScanGradientArgs g)
     uint32_t number;
     const ScanPlace s = scanPlace<NP>(a, number);
     if(!s.valid) { return; }
-    float *const bc = staged[threadIdx.x >> 6];
-    const T *u = rowsOf<const T>(a.u, a.sequences, s.place) + s.channel, *delta = rowsOf<const T>(a.delta, a.sequences, s.place) + s.channel;
+    float *const bc = staged[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
+    const uint32_t channel = s.channel;
+    const T *u = rowsOf<const T>(a.u, a.sequences, s.place), *delta = rowsOf<const T>(a.delta, a.sequences, s.place);
     const uint32_t bcAt = s.group * a.states + s.firstState;
     const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
-    const T *dout = GRADIENT ? rowsOf<const T>(g.out, a.sequences, s.place) + s.channel : nullptr;
-    const T *z = GRADIENT && a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) + s.channel : nullptr;
-    const float bias = a.deltaBias ? a.deltaBias[s.channel] : 0.0f;
+    const T *dout = GRADIENT ? rowsOf<const T>(g.out, a.sequences, s.place) : nullptr;
+    const T *z = GRADIENT && a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) : nullptr;
+    const float bias = a.deltaBias ? a.deltaBias[channel] : 0.0f;
     float A[NP], h[NP], G[NP], P[NP], time = 0.0f;
     loadA<NP>(a, s, A);
     #pragma unroll
     for(int n = 0; n < NP; n++) { h[n] = G[n] = 0.0f; P[n] = 1.0f; }
     const uint32_t end = s.first + s.rows;
-    StagedBC<T, NP, R> next;
-    next.fetch(B, C, a, s.first, end, s.numStates);
+    StagedBC<T, NP, R> stage;
+    StagedRows<T, R> rawU, rawDelta, rawOut, rawZ;
+    const auto fetch = [&](uint32_t row) {
+        stage.fetch(B, C, a, row, end, s.numStates);
+        rawU.fetch(u, a.u.rowStride, channel, row, end);
+        rawDelta.fetch(delta, a.delta.rowStride, channel, row, end);
+        if(GRADIENT) { rawOut.fetch(dout, g.out.rowStride, channel, row, end); }
+        if(GRADIENT && z) { rawZ.fetch(z, a.z.rowStride, channel, row, end); }
+    };
+    if(s.rows) { fetch(s.first); }
     for(uint32_t row = s.first; row < end; row += R) {
-        waveFence();
-        next.store(bc);
-        waveFence();
-        if(row + R < end) { next.fetch(B, C, a, row + R, end, s.numStates); }
-        T rawU[R], rawDelta[R], rawOut[R], rawZ[R];
-        #pragma unroll
-        for(int r = 0; r < R; r++) {
-            const uint64_t t = min(row + r, end - 1);
-            rawU[r] = u[t * a.u.rowStride];
-            rawDelta[r] = delta[t * a.delta.rowStride];
-            if(GRADIENT) {
-                rawOut[r] = dout[t * g.out.rowStride];
-                if(z) { rawZ[r] = z[t * a.z.rowStride]; }
+        float dt[R], w[R], gy[R];
+        times<T, R>(a, rawDelta, rawU, bias, end - row, dt, w);
+        if(GRADIENT) {
+            #pragma unroll
+            for(int r = 0; r < R; r++) { gy[r] = r < (int)(end - row) ? widen(rawOut.raw[r]) : 0.0f; }
+            if(z) {
+                float gate[R];
+                gates<T, R>(rawZ, gate);
+                #pragma unroll
+                for(int r = 0; r < R; r++) { gy[r] *= gate[r]; }
             }
         }
+        waveFence();
+        stage.store(bc);
+        waveFence();
+        if(row + R < end) { fetch(row + R); }
+        float nextB[NP], nextC[NP];
+        #pragma unroll
+        for(int n = 0; n < NP; n++) { nextB[n] = bc[n]; if(GRADIENT) { nextC[n] = bc[NP + n]; } }
         #pragma unroll
         for(int r = 0; r < R; r++) {
-            if(row + r >= end) { break; }
-            float dt = widen(rawDelta[r]) + bias;
-            if(a.softplus) { dt = softplusOf(dt); }
-            const float w = dt * widen(rawU[r]);
-            float gy = 0.0f;
-            if(GRADIENT) {
-                gy = widen(rawOut[r]);
-                if(z) { const float zr = widen(rawZ[r]); gy *= zr * logistic(zr); }
+            float Bn[NP], Cn[NP];
+            #pragma unroll
+            for(int n = 0; n < NP; n++) { Bn[n] = nextB[n]; Cn[n] = nextC[n]; }
+            if(r + 1 < R) {
+                // (a row's inputs are read while the row before is worked on, and no sooner)
+                readAfter(h[NP - 4], h[NP - 3], h[NP - 2], h[NP - 1]);
+                if(GRADIENT) { readAfter(G[NP - 4], G[NP - 3], G[NP - 2], G[NP - 1]); }
+                #pragma unroll
+                for(int n = 0; n < NP; n++) { nextB[n] = bc[(r + 1) * 2 * NP + n]; if(GRADIENT) { nextC[n] = bc[((r + 1) * 2 + 1) * NP + n]; } }
             }
-            time += dt;
+            time += dt[r];
             #pragma unroll
             for(int n = 0; n < NP; n++) {
-                const float decay = exp2Of(dt * A[n]);
-                h[n] = __builtin_fmaf(decay, h[n], w * bc[r * 2 * NP + n]);
+                const float decay = exp2Of(dt[r] * A[n]);
+                h[n] = __builtin_fmaf(decay, h[n], w[r] * Bn[n]);
                 if(GRADIENT) {
                     P[n] *= decay;
-                    G[n] = __builtin_fmaf(P[n], gy * bc[(r * 2 + 1) * NP + n], G[n]);
+                    G[n] = __builtin_fmaf(P[n], gy[r] * Cn[n], G[n]);
                 }
             }
         }
     }
     storeChunk<NP>(a, s, a.chunkState, number, h);
-    if(s.firstState == 0 && s.active) { a.chunkTime[(uint64_t)number * a.channels + s.channel] = time; }
+    if(s.firstState == 0 && s.active) { a.chunkTime[(uint64_t)number * a.channels + channel] = time; }
     if(GRADIENT) { storeChunk<NP>(a, s, g.chunkGradient, number, G); }
 }
 
+// One walk over the chunks of a state, forwards or backwards: what a chunk adds is replaced by what there was before it.  A trip to memory is as long as
+// dozens of chunks' arithmetic, so what AHEAD chunks add is fetched before the AHEAD before those are worked on.
+template<bool BACKWARDS> __device__ inline float walkChunks(float *state, uint64_t stride, const float *time, uint32_t channels, uint32_t chunks, float A, float h)
+{
+    constexpr uint32_t AHEAD = 8;
+    const auto chunk = [&](uint32_t k) { return BACKWARDS ? chunks - 1 - min(k, chunks - 1) : min(k, chunks - 1); };
+    float adds[AHEAD], times[AHEAD];
+    #pragma unroll
+    for(uint32_t k = 0; k < AHEAD; k++) { adds[k] = state[chunk(k) * stride]; times[k] = time[(uint64_t)chunk(k) * channels]; }
+    for(uint32_t first = 0; first < chunks; first += AHEAD) {
+        float nextAdds[AHEAD], nextTimes[AHEAD];
+        #pragma unroll
+        for(uint32_t k = 0; k < AHEAD; k++) { nextAdds[k] = state[chunk(first + AHEAD + k) * stride]; nextTimes[k] = time[(uint64_t)chunk(first + AHEAD + k) * channels]; }
+        #pragma unroll
+        for(uint32_t k = 0; k < AHEAD; k++) {
+            if(first + k < chunks) {
+                state[chunk(first + k) * stride] = h;
+                h = __builtin_fmaf(exp2Of(times[k] * A), h, adds[k]);
+            }
+            adds[k] = nextAdds[k];
+            times[k] = nextTimes[k];
+        }
+    }
+    return h;
+}
 // Second kernel: a lane has one state of one channel of one sequence and walks over the chunks, leaving in each one's place the state it starts from,
 // and (GRADIENT) back again, leaving the gradient of the state behind each.
 template<bool GRADIENT>
@@ -233,28 +305,15 @@ void scanJoinKernel(ScanArgs a, ScanGradientArgs g)
     const uint32_t channel = part * 64 + threadIdx.x;
     Place p;
     if(!describe(a.sequences, sequence, p) || channel >= a.channels) { return; }
-    const uint64_t chunk0 = firstChunk(a.sequences, sequence);
+    const uint64_t chunk0 = firstChunk(a.sequences, sequence), stride = (uint64_t)a.states * a.channels;
     const uint32_t chunks = max(1u, (uint32_t)(((uint64_t)p.length + a.sequences.chunk - 1) / a.sequences.chunk));
     const float A = a.A[(uint64_t)channel * a.states + n] * LOG2E;
-    const uint64_t at = ((uint64_t)p.state * a.channels + channel) * a.states + n;
-    float *state = a.chunkState + (chunk0 * a.states + n) * a.channels + channel;
+    const uint64_t at = ((uint64_t)p.state * a.channels + channel) * a.states + n, first = (chunk0 * a.states + n) * a.channels + channel;
     const float *time = a.chunkTime + chunk0 * a.channels + channel;
-    const uint64_t stride = (uint64_t)a.states * a.channels;
-    float h = a.initialState ? a.initialState[at] : 0.0f;
-    for(uint32_t c = 0; c < chunks; c++) {
-        const float adds = state[c * stride];
-        state[c * stride] = h;
-        h = __builtin_fmaf(exp2Of(time[(uint64_t)c * a.channels] * A), h, adds);
-    }
+    const float h = walkChunks<false>(a.chunkState + first, stride, time, a.channels, chunks, A, a.initialState ? a.initialState[at] : 0.0f);
     if(!GRADIENT) { if(a.finalState) { a.finalState[at] = h; } }
     else {
-        float *gradient = g.chunkGradient + (chunk0 * a.states + n) * a.channels + channel;
-        float r = g.finalState ? g.finalState[at] : 0.0f;
-        for(uint32_t c = chunks; c-- > 0; ) {
-            const float adds = gradient[c * stride];
-            gradient[c * stride] = r;
-            r = __builtin_fmaf(exp2Of(time[(uint64_t)c * a.channels] * A), r, adds);
-        }
+        const float r = walkChunks<true>(g.chunkGradient + first, stride, time, a.channels, chunks, A, g.finalState ? g.finalState[at] : 0.0f);
         if(g.initialState) { g.initialState[at] = r; }
     }
 }
@@ -270,65 +329,76 @@ void scanKernel(ScanArgs a)
     uint32_t number;
     const ScanPlace s = scanPlace<NP>(a, number);
     if(!s.valid) { return; }
-    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, channel = s.channel;
     float *const bc = staged[slab];
-    const T *u = rowsOf<const T>(a.u, a.sequences, s.place) + s.channel, *delta = rowsOf<const T>(a.delta, a.sequences, s.place) + s.channel;
-    const T *z = a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) + s.channel : nullptr;
-    T *out = rowsOf<T>(a.out, a.sequences, s.place) + s.channel;
+    const T *u = rowsOf<const T>(a.u, a.sequences, s.place), *delta = rowsOf<const T>(a.delta, a.sequences, s.place);
+    const T *z = a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) : nullptr;
+    T *out = rowsOf<T>(a.out, a.sequences, s.place);
     const uint32_t bcAt = s.group * a.states + s.firstState;
     const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
-    const float bias = a.deltaBias ? a.deltaBias[s.channel] : 0.0f, skip = a.D ? a.D[s.channel] : 0.0f;
+    const float bias = a.deltaBias ? a.deltaBias[channel] : 0.0f, skip = a.D ? a.D[channel] : 0.0f;
     float A[NP], h[NP];
     loadA<NP>(a, s, A);
     if(a.chunkState) { loadChunk<NP>(a, s, a.chunkState, number, h); } else { loadState<NP>(a, s, a.initialState, s.place.state, h); }
     const uint32_t end = s.first + s.rows;
-    StagedBC<T, NP, R> next;
-    next.fetch(B, C, a, s.first, end, s.numStates);
+    StagedBC<T, NP, R> stage;
+    StagedRows<T, R> rawU, rawDelta, rawZ;
+    const auto fetch = [&](uint32_t row) {
+        stage.fetch(B, C, a, row, end, s.numStates);
+        rawU.fetch(u, a.u.rowStride, channel, row, end);
+        rawDelta.fetch(delta, a.delta.rowStride, channel, row, end);
+        if(z) { rawZ.fetch(z, a.z.rowStride, channel, row, end); }
+    };
+    if(s.rows) { fetch(s.first); }
     uint32_t turn = 0;
     for(uint32_t row = s.first; row < end; row += R, turn ^= 1) {
+        float dt[R], w[R], y[R], gate[R], direct[R];
+        times<T, R>(a, rawDelta, rawU, bias, end - row, dt, w);
+        #pragma unroll
+        for(int r = 0; r < R; r++) { direct[r] = skip * widen(rawU.raw[r]); gate[r] = 1.0f; }
+        if(z) { gates<T, R>(rawZ, gate); }
         waveFence();
-        next.store(bc);
+        stage.store(bc);
         waveFence();
-        if(row + R < end) { next.fetch(B, C, a, row + R, end, s.numStates); }
-        T rawU[R], rawDelta[R], rawZ[R];
+        if(row + R < end) { fetch(row + R); }
+        float nextB[NP], nextC[NP];
+        #pragma unroll
+        for(int n = 0; n < NP; n++) { nextB[n] = bc[n]; nextC[n] = bc[NP + n]; }
         #pragma unroll
         for(int r = 0; r < R; r++) {
-            const uint64_t t = min(row + r, end - 1);
-            rawU[r] = u[t * a.u.rowStride];
-            rawDelta[r] = delta[t * a.delta.rowStride];
-            if(z) { rawZ[r] = z[t * a.z.rowStride]; }
-        }
-        #pragma unroll
-        for(int r = 0; r < R; r++) {
-            if(row + r >= end) { break; }
-            float dt = widen(rawDelta[r]) + bias;
-            if(a.softplus) { dt = softplusOf(dt); }
-            const float w = dt * widen(rawU[r]);
-            float y = 0.0f, y1 = 0.0f;
+            float Bn[NP], Cn[NP];
+            #pragma unroll
+            for(int n = 0; n < NP; n++) { Bn[n] = nextB[n]; Cn[n] = nextC[n]; }
+            if(r + 1 < R) {
+                // (a row's inputs are read while the row before is worked on, and no sooner)
+                if(r) { readAfter(h[NP - 3], h[NP - 2], h[NP - 1], y[r - 1]); }
+                #pragma unroll
+                for(int n = 0; n < NP; n++) { nextB[n] = bc[(r + 1) * 2 * NP + n]; nextC[n] = bc[((r + 1) * 2 + 1) * NP + n]; }
+            }
+            float y0 = SLABS ? 0.0f : direct[r], y1 = 0.0f;
             #pragma unroll
             for(int n = 0; n < NP; n++) {
-                const float decay = exp2Of(dt * A[n]);
-                h[n] = __builtin_fmaf(decay, h[n], w * bc[r * 2 * NP + n]);
-                if(n & 1) { y1 = __builtin_fmaf(h[n], bc[(r * 2 + 1) * NP + n], y1); } else { y = __builtin_fmaf(h[n], bc[(r * 2 + 1) * NP + n], y); }
+                h[n] = __builtin_fmaf(exp2Of(dt[r] * A[n]), h[n], w[r] * Bn[n]);
+                if(n & 1) { y1 = __builtin_fmaf(h[n], Cn[n], y1); } else { y0 = __builtin_fmaf(h[n], Cn[n], y0); }
             }
-            y += y1;
-            if(SLABS) { sums[turn][slab][r][lane] = y; }
-            else if(s.active) {
-                y = __builtin_fmaf(skip, widen(rawU[r]), y);
-                if(z) { const float zr = widen(rawZ[r]); y *= zr * logistic(zr); }
-                out[(uint64_t)(row + r) * a.out.rowStride] = narrow<T>(y);
-            }
+            y[r] = y0 + y1;
         }
         if(SLABS) {
+            #pragma unroll
+            for(int r = 0; r < R; r++) { sums[turn][slab][r][lane] = y[r]; }
             __syncthreads();        // (the other half of `sums` is written next, so one barrier a block of rows does)
             #pragma unroll
             for(int r = 0; r < R; r++) {
-                if(row + r < end && r % a.slabs == slab && s.active) {
-                    float y = skip * widen(rawU[r]);
-                    for(uint32_t k = 0; k < a.slabs; k++) { y += sums[turn][k][r][lane]; }
-                    if(z) { const float zr = widen(rawZ[r]); y *= zr * logistic(zr); }
-                    out[(uint64_t)(row + r) * a.out.rowStride] = narrow<T>(y);
+                if(r % a.slabs == slab) {
+                    y[r] = direct[r];
+                    for(uint32_t k = 0; k < a.slabs; k++) { y[r] += sums[turn][k][r][lane]; }
                 }
+            }
+        }
+        if(s.active) {
+            #pragma unroll
+            for(int r = 0; r < R; r++) {
+                if(row + r < end && (!SLABS || r % a.slabs == slab)) { rowAt(out, row + r, a.out.rowStride)[channel] = narrow<T>(y[r] * gate[r]); }
             }
         }
     }
@@ -336,56 +406,111 @@ void scanKernel(ScanArgs a)
 }
 
 // One row a sequence (a token): the states of a sequence's channel are neighbours in memory, and reading and writing them is all there is to it.
-// LANES lanes have four each; what they give the output is added up between them.
-template<typename T, int LANES, bool QUADS>
+// LANES lanes have four each; what they give the output is added up between them.  A lane does the same states of EACH sequences, whose A it then
+// reads once, and whose loads are all on their way before the first is needed.
+template<typename T, int LANES, bool QUADS, int EACH>
 __global__ __launch_bounds__(256)
 void scanTokenKernel(ScanArgs a)
 {
-    const uint64_t item = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const uint32_t part = threadIdx.x % LANES;
-    const uint32_t sequence = (uint32_t)(item / a.channels), channel = (uint32_t)(item - (uint64_t)sequence * a.channels);
-    Place p;
-    if(sequence >= a.sequences.count || !describe(a.sequences, sequence, p)) { return; }
-    const uint64_t at = ((uint64_t)p.state * a.channels + channel) * a.states;
-    const uint32_t n0 = part * 4;
-    float h[4];
-    #pragma unroll
-    for(int k = 0; k < 4; k++) { h[k] = 0.0f; }
-    if(a.initialState && n0 < a.states) {
-        if(QUADS) { *(float4*)h = *(const float4*)(a.initialState + at + n0); }
-        else {
-            #pragma unroll
-            for(int k = 0; k < 4; k++) { if(n0 + k < a.states) { h[k] = a.initialState[at + n0 + k]; } }
-        }
-    }
-    if(p.length) {          // (a packed sequence may have none)
-        const uint32_t group = channel / a.groupChannels;
-        const float u = widen(rowsOf<const T>(a.u, a.sequences, p)[channel]);
-        float dt = widen(rowsOf<const T>(a.delta, a.sequences, p)[channel]) + (a.deltaBias ? a.deltaBias[channel] : 0.0f);
-        if(a.softplus) { dt = softplusOf(dt); }
-        const T *B = rowsOf<const T>(a.B, a.sequences, p) + group * a.states, *C = rowsOf<const T>(a.C, a.sequences, p) + group * a.states;
-        const float *A = a.A + (uint64_t)channel * a.states;
-        float y = 0.0f;
+    uint32_t first, channel;
+    divideItem(a.channels * LANES, first, channel);
+    const uint32_t part = threadIdx.x % LANES, n0 = part * 4;
+    channel /= LANES;
+    first *= EACH;
+    if(first >= a.sequences.count) { return; }
+    const uint32_t bcAt = (channel / a.groupChannels) * a.states + n0;
+    const bool here = n0 < a.states;
+    const auto load4 = [&](const auto *from, float (&to)[4], uint32_t k0) {
+        typedef std::remove_cv_t<std::remove_reference_t<decltype(*from)>> E;
         #pragma unroll
-        for(int k = 0; k < 4; k++) {
-            if(n0 + k < a.states) {
-                h[k] = __builtin_fmaf(exp2Of(dt * (A[n0 + k] * LOG2E)), h[k], dt * u * widen(B[n0 + k]));
-                y = __builtin_fmaf(h[k], widen(C[n0 + k]), y);
+        for(int k = 0; k < 4; k++) { to[k] = 0.0f; }
+        if(QUADS) {
+            if(here) {
+                const Pack<E, 4> q = *(const Pack<E, 4>*)from;
+                #pragma unroll
+                for(int k = 0; k < 4; k++) { to[k] = widen(q.v[k]); }
             }
         }
-        #pragma unroll
-        for(int mask = 1; mask < LANES; mask *= 2) { y += __shfl_xor(y, mask); }
-        if(part == 0) {
-            if(a.D) { y = __builtin_fmaf(a.D[channel], u, y); }
-            if(a.z.data) { const float z = widen(rowsOf<const T>(a.z, a.sequences, p)[channel]); y *= z * logistic(z); }
-            rowsOf<T>(a.out, a.sequences, p)[channel] = narrow<T>(y);
-        }
-    }
-    if(a.finalState && n0 < a.states) {
-        if(QUADS) { *(float4*)(a.finalState + at + n0) = *(const float4*)h; }
         else {
             #pragma unroll
-            for(int k = 0; k < 4; k++) { if(n0 + k < a.states) { a.finalState[at + n0 + k] = h[k]; } }
+            for(int k = 0; k < 4; k++) { if(k0 + k < a.states) { to[k] = widen(from[k]); } }
+        }
+    };
+    float A[4], h[EACH][4], B[EACH][4], C[EACH][4], u[EACH], dt[EACH], z[EACH];
+    Place p[EACH];
+    bool valid[EACH];
+    // (all slots, then all states and rows: a load that waits for one in between would wait for everything asked for before.  What is padding reads the
+    // first state and its own rows, and writes nothing.)
+    #pragma unroll
+    for(int i = 0; i < EACH; i++) {
+        p[i].sequence = min(first + i, a.sequences.count - 1);
+        p[i].first = 0;
+        p[i].length = a.sequences.length;
+        p[i].state = a.sequences.slots ? a.sequences.slots[p[i].sequence] : (int32_t)p[i].sequence;
+    }
+    #pragma unroll
+    for(int i = 0; i < EACH; i++) {
+        valid[i] = first + i < a.sequences.count && (!a.sequences.slots || (p[i].state >= 0 && (uint32_t)p[i].state < a.sequences.numSlots));
+        p[i].state = valid[i] ? p[i].state : 0;
+        #pragma unroll
+        for(int k = 0; k < 4; k++) { h[i][k] = 0.0f; }
+        if(a.initialState) { load4(a.initialState + ((uint64_t)p[i].state * a.channels + channel) * a.states + n0, h[i], n0); }
+    }
+    const auto rows = [&](int i) {
+        load4(rowsOf<const T>(a.B, a.sequences, p[i]) + bcAt, B[i], n0);
+        load4(rowsOf<const T>(a.C, a.sequences, p[i]) + bcAt, C[i], n0);
+        u[i] = widen(rowsOf<const T>(a.u, a.sequences, p[i])[channel]);
+        dt[i] = widen(rowsOf<const T>(a.delta, a.sequences, p[i])[channel]);
+        z[i] = a.z.data ? widen(rowsOf<const T>(a.z, a.sequences, p[i])[channel]) : 0.0f;
+    };
+    if(a.sequences.offsets) {
+        #pragma unroll
+        for(int i = 0; i < EACH; i++) {
+            u[i] = dt[i] = z[i] = 0.0f;
+            describe(a.sequences, p[i].sequence, p[i]);
+            if(!valid[i]) { p[i].length = 0; p[i].state = 0; }
+            if(p[i].length) { rows(i); }        // (a packed sequence may have none)
+        }
+    }
+    else if(a.sequences.length) {
+        #pragma unroll
+        for(int i = 0; i < EACH; i++) { rows(i); }
+    }
+    load4(a.A + (uint64_t)channel * a.states + n0, A, n0);
+    const float bias = a.deltaBias ? a.deltaBias[channel] : 0.0f, skip = a.D ? a.D[channel] : 0.0f;
+    #pragma unroll
+    for(int i = 0; i < EACH; i++) {
+        if(!valid[i]) { continue; }
+        if(p[i].length) {
+            float time = dt[i] + bias, y = 0.0f;
+            if(a.softplus) { time = softplusOf(time); }
+            const float w = time * u[i];
+            #pragma unroll
+            for(int k = 0; k < 4; k++) {
+                if(QUADS || n0 + k < a.states) {
+                    h[i][k] = __builtin_fmaf(exp2Of(time * (A[k] * LOG2E)), h[i][k], w * B[i][k]);
+                    y = __builtin_fmaf(h[i][k], C[i][k], y);
+                }
+            }
+            // (lanes behind the last state have zeros)
+            if constexpr(LANES > 1) { y += gennmi_lanes::partner<1>(y); }
+            if constexpr(LANES > 2) { y += gennmi_lanes::partner<2>(y); }
+            if constexpr(LANES > 4) { y += gennmi_lanes::partner<4>(y); }
+            if constexpr(LANES > 8) { y += gennmi_lanes::partner<8>(y); }
+            if constexpr(LANES > 16) { y += gennmi_lanes::partner<16>(y); }
+            if(part == 0) {
+                y = __builtin_fmaf(skip, u[i], y);
+                if(a.z.data) { y *= z[i] * logistic(z[i]); }
+                rowsOf<T>(a.out, a.sequences, p[i])[channel] = narrow<T>(y);
+            }
+        }
+        if(a.finalState && here) {
+            float *state = a.finalState + ((uint64_t)p[i].state * a.channels + channel) * a.states + n0;
+            if(QUADS) { *(Pack<float, 4>*)state = Pack<float, 4>{{h[i][0], h[i][1], h[i][2], h[i][3]}}; }
+            else {
+                #pragma unroll
+                for(int k = 0; k < 4; k++) { if(n0 + k < a.states) { state[k] = h[i][k]; } }
+            }
         }
     }
 }

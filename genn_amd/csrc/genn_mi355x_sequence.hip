@@ -1,5 +1,7 @@
 // Operators on sequences: a short causal convolution and a selective state space scan, with their gradients, for whole sequences and for
 // single tokens.  Entry points and their checks; the kernels are in the headers included below.
+#include <type_traits>
+
 #include "genn_mi355x_elements.h"
 
 using namespace gennmi_elements;
@@ -67,7 +69,8 @@ uint64_t totalRows(const gennmi_sequences_t &s) { return s.offsets ? s.rows : (u
 constexpr uint64_t MOST_BLOCKS = 0x7fffffffull;
 
 // ---- causal convolution
-constexpr uint32_t CONV_ROWS = 16;          // rows of a chunk; at least taps - 1, which only the first chunk then reads of the initial state
+// Rows of a chunk: at least taps - 1, so that only the first chunk reads the initial state
+constexpr uint32_t CONV_ROWS = 16, CONV_GRADIENT_ROWS = 64, CONV_GRADIENT_THREADS = 1u << 17;
 
 int checkConv(const char *what, const gennmi_causal_conv_t *c, bool gradients)
 {
@@ -87,25 +90,32 @@ int checkConv(const char *what, const gennmi_causal_conv_t *c, bool gradients)
     if((uintptr_t)c->initialState % size || (uintptr_t)c->finalState % size) { return fail(GENNMI_EINVAL, name + ": a state is not aligned to its elements"); }
     return GENNMI_OK;
 }
-// Channels of a thread: four where every row and state of them is one aligned access, else one
+// Channels of a thread: four, for gradients two, where every row and state of them is one aligned access, else one.  (Gradients keep four rows of
+// taps a channel in registers: with four channels a thread two wavefronts fit a SIMD, and 8 x 2048 rows of 2048 channels take 67 us instead of 60.)
 uint32_t convVector(const gennmi_causal_conv_t &c, const gennmi_causal_conv_gradient_t *g)
 {
-    const uint32_t bytes = 4 * sizeOf(c.type);
-    bool whole = c.channels % 4 == 0;
-    auto rows = [&](const gennmi_rows_t &r) { whole = whole && (uintptr_t)r.data % bytes == 0 && r.rowStride % 4 == 0 && r.sequenceStride % 4 == 0; };
+    const uint32_t vector = g ? 2 : 4, bytes = vector * sizeOf(c.type);
+    bool whole = c.channels % vector == 0;
+    auto rows = [&](const gennmi_rows_t &r) { whole = whole && (uintptr_t)r.data % bytes == 0 && r.rowStride % vector == 0 && r.sequenceStride % vector == 0; };
     auto array = [&](const void *p) { whole = whole && (uintptr_t)p % bytes == 0; };
     rows(c.x);
     array(c.initialState);
     if(g) { rows(g->out); rows(g->x); array(g->initialState); array(g->finalState); }
     else { rows(c.out); array(c.finalState); }
-    return whole ? 4 : 1;
+    return whole ? vector : 1;
 }
-// (a single row needs no chunks, and the whole of a shorter sequence is one)
-uint32_t convChunk(const gennmi_causal_conv_t &) { return CONV_ROWS; }
-ConvArgs convArgs(const gennmi_causal_conv_t &c, uint32_t vector)
+// Gradients walk taps - 1 rows beyond a chunk and write a sum for every tap behind it: the longer the chunks the better, as long as there are threads
+// for the whole chip (the case above with 16, 32 and 64 rows: 73, 60 and 53 us).  The forward pass has neither (15, 16 and 22 us for 4096 x 4096).
+uint32_t convChunk(const gennmi_causal_conv_t &c, bool gradients)
+{
+    if(!gradients) { return CONV_ROWS; }
+    uint32_t chunk = CONV_GRADIENT_ROWS;
+    while(chunk > CONV_ROWS && totalRows(c.sequences) / chunk * (c.channels / 2) < CONV_GRADIENT_THREADS) { chunk /= 2; }
+    return chunk;
+}
+ConvArgs convArgs(const gennmi_causal_conv_t &c, uint32_t vector, uint32_t chunk)
 {
     ConvArgs a{};
-    const uint32_t chunk = convChunk(c);
     a.sequences = sequencesOf(c.sequences, chunk);
     a.x = c.x;
     a.out = c.out;
@@ -120,27 +130,36 @@ ConvArgs convArgs(const gennmi_causal_conv_t &c, uint32_t vector)
     a.numbers = (uint32_t)chunkNumbers(c.sequences, chunk);
     return a;
 }
-template<typename T, int VEC> void launchConv(const ConvArgs &a, const ConvGradientArgs *g, dim3 grid, hipStream_t stream)
+#define EACH_TAPS TAPS(1) TAPS(2) TAPS(3) TAPS(4) TAPS(5) TAPS(6) TAPS(7) TAPS(8)
+template<typename T, int VEC> void launchConv(const ConvArgs &a, dim3 grid, hipStream_t stream)
 {
-    switch(a.taps) {
-#define TAPS(K) case K: if(g) { causalConvBackwardKernel<T, K, VEC><<<grid, dim3(256), 0, stream>>>(a, *g); } \
-                        else { causalConvKernel<T, K, VEC><<<grid, dim3(256), 0, stream>>>(a); } break;
-    TAPS(1) TAPS(2) TAPS(3) TAPS(4) TAPS(5) TAPS(6) TAPS(7) TAPS(8)
+#define TAPS(K) case K: causalConvKernel<T, K, VEC><<<grid, dim3(256), 0, stream>>>(a); break;
+    switch(a.taps) { EACH_TAPS }
 #undef TAPS
-    }
 }
+template<typename T, int VEC> void launchConvBackward(const ConvArgs &a, const ConvGradientArgs &g, dim3 grid, hipStream_t stream)
+{
+#define TAPS(K) case K: causalConvBackwardKernel<T, K, VEC><<<grid, dim3(256), 0, stream>>>(a, g); break;
+    switch(a.taps) { EACH_TAPS }
+#undef TAPS
+}
+#undef EACH_TAPS
 int runConv(const char *what, const gennmi_causal_conv_t &c, uint32_t vector, const ConvGradientArgs *g, hipStream_t stream)
 {
-    const ConvArgs a = convArgs(c, vector);
+    const uint32_t chunk = convChunk(c, g != nullptr);
+    const ConvArgs a = convArgs(c, vector, chunk);
     const uint64_t blocks = ((uint64_t)a.numbers * a.vectors + 255) / 256;
-    if(chunkNumbers(c.sequences, convChunk(c)) > MOST_BLOCKS || blocks > MOST_BLOCKS) { return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers"); }
+    if(chunkNumbers(c.sequences, chunk) > MOST_BLOCKS || blocks > MOST_BLOCKS) { return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers"); }
     if(!blocks) { return GENNMI_OK; }
     return withType(c.type, [&](auto t) {
-        if(vector == 4) { launchConv<decltype(t), 4>(a, g, dim3((uint32_t)blocks), stream); } else { launchConv<decltype(t), 1>(a, g, dim3((uint32_t)blocks), stream); }
+        const dim3 grid((uint32_t)blocks);
+        if(g) { if(vector == 2) { launchConvBackward<decltype(t), 2>(a, *g, grid, stream); } else { launchConvBackward<decltype(t), 1>(a, *g, grid, stream); } }
+        else if(vector == 4) { launchConv<decltype(t), 4>(a, grid, stream); }
+        else { launchConv<decltype(t), 1>(a, grid, stream); }
         return gennmi_detail::afterLaunch(what);
     });
 }
-size_t convWorkspace(const gennmi_causal_conv_t &c) { return (size_t)chunkNumbers(c.sequences, convChunk(c)) * (c.taps + 1) * c.channels * sizeof(float); }
+size_t convWorkspace(const gennmi_causal_conv_t &c) { return (size_t)chunkNumbers(c.sequences, convChunk(c, true)) * (c.taps + 1) * c.channels * sizeof(float); }
 
 // ---- selective scan
 int checkScan(const char *what, const gennmi_scan_t *c, bool gradients)
@@ -170,6 +189,7 @@ int checkScan(const char *what, const gennmi_scan_t *c, bool gradients)
     return GENNMI_OK;
 }
 
+constexpr uint64_t TOKEN_THREADS = 256 * 2048;      // of one launch, from which a lane takes several sequences' tokens
 struct ScanPlan { uint32_t slab, slabs, chunk; bool split; };
 constexpr uint32_t SCAN_BLOCK_ROWS = 8, SCAN_BACKWARD_BLOCKS = 4;
 uint32_t scanTiles(const gennmi_scan_t &c) { return c.groups * ((c.channels / c.groups + 63) / 64); }
@@ -213,7 +233,8 @@ int scanArgs(const char *what, const gennmi_scan_t &c, const ScanPlan &p, ScanAr
 {
     a = ScanArgs{};
     const uint64_t numbers = chunkNumbers(c.sequences, p.chunk), tiles = scanTiles(c);
-    if(numbers * tiles > MOST_BLOCKS || (uint64_t)c.sequences.count * c.states * ((c.channels + 63) / 64) > MOST_BLOCKS) {
+    if(numbers * tiles > MOST_BLOCKS || (uint64_t)c.sequences.count * c.states * ((c.channels + 63) / 64) > MOST_BLOCKS ||
+       (uint64_t)c.sequences.count * c.channels / 8 > MOST_BLOCKS) {
         return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers");
     }
     a.sequences = sequencesOf(c.sequences, p.chunk);
@@ -248,9 +269,20 @@ template<typename T, int NP, bool SLABS> int launchScan(const ScanArgs &a, const
 }
 template<typename T, int LANES> int launchToken(const ScanArgs &a, hipStream_t stream)
 {
-    const bool quads = a.states % 4 == 0 && (uintptr_t)a.initialState % 16 == 0 && (uintptr_t)a.finalState % 16 == 0;
-    const dim3 grid((uint32_t)(((uint64_t)a.sequences.count * a.channels * LANES + 255) / 256));
-    if(quads) { scanTokenKernel<T, LANES, true><<<grid, dim3(256), 0, stream>>>(a); } else { scanTokenKernel<T, LANES, false><<<grid, dim3(256), 0, stream>>>(a); }
+    // four states a lane in one access, where every array lies so
+    const auto fours = [](const void *p, uint32_t size) { return (uintptr_t)p % (4 * size) == 0; };
+    const auto rows = [&](const gennmi_rows_t &r) { return fours(r.data, sizeof(T)) && r.rowStride % 4 == 0 && r.sequenceStride % 4 == 0; };
+    const bool quads = a.states % 4 == 0 && fours(a.A, 4) && fours(a.initialState, 4) && fours(a.finalState, 4) && rows(a.B) && rows(a.C);
+    // several sequences a lane, where that leaves work-groups enough for the chip
+    constexpr uint32_t MANY = 4;
+    const uint64_t threads = (uint64_t)a.sequences.count * a.channels * LANES;
+    const bool many = threads / MANY >= TOKEN_THREADS;
+    const uint64_t groups = many ? (a.sequences.count + MANY - 1) / MANY : a.sequences.count;
+    const dim3 grid((uint32_t)((groups * a.channels * LANES + 255) / 256));
+    if(quads && many) { scanTokenKernel<T, LANES, true, MANY><<<grid, dim3(256), 0, stream>>>(a); }
+    else if(quads) { scanTokenKernel<T, LANES, true, 1><<<grid, dim3(256), 0, stream>>>(a); }
+    else if(many) { scanTokenKernel<T, LANES, false, MANY><<<grid, dim3(256), 0, stream>>>(a); }
+    else { scanTokenKernel<T, LANES, false, 1><<<grid, dim3(256), 0, stream>>>(a); }
     return gennmi_detail::afterLaunch("selective_scan");
 }
 template<typename T, int NP, bool SLABS> int launchScanBackward(const ScanArgs &a, const ScanGradientArgs &g, const ScanPlan &p, hipStream_t stream)
@@ -345,7 +377,7 @@ int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_c
         a.partial = sums ? (float*)workspace : nullptr;
         if(const int rc = runConv(what, *conv, convVector(*conv, gradient), &a, (hipStream_t)stream)) { return rc; }
         if(sums) {
-            const ChunkSums c{a.partial, g.weight, {g.bias, nullptr}, (uint32_t)chunkNumbers(conv->sequences, convChunk(*conv)), conv->channels, conv->taps, conv->taps + 1};
+            const ChunkSums c{a.partial, g.weight, {g.bias, nullptr}, (uint32_t)chunkNumbers(conv->sequences, convChunk(*conv, true)), conv->channels, conv->taps, conv->taps + 1};
             if(const int rc = launchChunkSum(what, c, (hipStream_t)stream)) { return rc; }
         }
         noteRows(g.x, conv->sequences, conv->channels, size);
