@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
+
 namespace gennmi_lanes
 {
 // The value of the lane's partner in the other half of its group of 2 WIDTH lanes.  Lane l's partner is l ^ WIDTH for WIDTH 1, 2, 16 and 32; for 4 and 8
@@ -54,11 +56,20 @@ template<int M, int WIDTH = 32> __device__ inline float sumOfLanes(const float (
     }
     else { return v[0]; }
 }
-template<int WIDTH = 32> __device__ inline float maxOfLanes(float x)
+// Of two values' bits, over all lanes: of floats that are not negative the maximum, and not a number where one of them is not.  The halves of the wavefront
+// have one value each after the first step.
+__device__ inline void maxOfLanes(uint32_t &a, uint32_t &b)
 {
-    x = fmaxf(x, partner<WIDTH>(x));
-    if constexpr(WIDTH > 1) { return maxOfLanes<WIDTH / 2>(x); }
-    return x;
+    const auto halves = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    uint32_t x = max(halves[0], halves[1]);
+    const auto rows = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(rows[0], rows[1]);
+    x = max(x, __float_as_uint(partner<8>(__uint_as_float(x))));
+    x = max(x, __float_as_uint(partner<4>(__uint_as_float(x))));
+    x = max(x, __float_as_uint(partner<2>(__uint_as_float(x))));
+    x = max(x, __float_as_uint(partner<1>(__uint_as_float(x))));
+    a = __builtin_amdgcn_readlane(x, 0);
+    b = __builtin_amdgcn_readlane(x, 32);
 }
 }
 #endif

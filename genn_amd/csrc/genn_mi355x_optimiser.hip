@@ -1,9 +1,13 @@
 // AdamW over many tensors in one launch, with states in 32 bits or in 8.
 //
 // Bound by memory: a weight is read and written with its gradient and states, 28 bytes in 32 bits with fp32 gradients, 16 in 8 bits, for some
-// 30 to 80 operations.  A work-group takes CHUNK neighbouring weights of one tensor (a table says which), four a lane in one access each.  In
+// 25 to 60 operations.  A work-group takes CHUNK neighbouring weights of one tensor (a table says which), four a lane in one access each.  In
 // 8 bits the 256 weights that share a scale are one wavefront's four a lane, so their maxima are found in registers and codes are written by the
 // pass that made the states.  The number of the step is the device's: the work-group that ends last counts it, so a captured step counts as well.
+//
+// One access an array and lane, and many short work-groups: 80 M weights in 32 bits (fp32 weights, bf16 gradients and copy) with CHUNK 1024, 2048, 4096, 8192
+// take 411, 428, 441, 449 us, 130 M in 8 bits 369, 373, 410, 409; work-groups that stay and go through the table 466 and more; the next
+// block's loads ahead of the arithmetic 436 and 457 (registers).
 #include <cmath>
 #include <new>
 #include <type_traits>
@@ -17,7 +21,7 @@ using gennmi_detail::fail;
 
 namespace
 {
-constexpr uint32_t CHUNK = 4096;        // weights of a work-group: a multiple of GENNMI_ADAMW_BLOCK * 4
+constexpr uint32_t CHUNK = 1024;        // weights of a work-group: a block each for its four wavefronts
 static_assert(GENNMI_ADAMW_BLOCK == 256, "a block is the four weights a lane of one wavefront");
 
 struct ParameterDev
@@ -28,8 +32,20 @@ struct ParameterDev
     double weightDecay;
 };
 struct ChunkDev { uint32_t parameter, index; };
-// What the device knows of time: beta^t of the steps so far
-struct CounterDev { double power1, power2; unsigned long long step; uint32_t ended, pad; };
+constexpr uint64_t STREAM_BYTES = 64ull << 20;      // of a step, from which nothing of it stays in the L2 caches (32 MiB) for whoever comes next
+// What the device knows of time: for the step to come, beta^t and 1 / (1 - beta^t); and work-groups that have ended, counted in GROUPS places (cache
+// lines of their own) and the places that are full in another: one place takes 86 million counts a second, fewer than work-groups can end
+constexpr uint32_t GROUPS = 32, LINE = 32;
+struct CounterDev { double power1, power2; unsigned long long step; float correct1, correct2; uint32_t pad[LINE - 8]; uint32_t ended[(GROUPS + 1) * LINE]; };
+// ... from beta^(t - 1)
+__host__ __device__ inline void setCounter(CounterDev &c, double beta1, double beta2, double before1, double before2, unsigned long long step)
+{
+    c.power1 = before1 * beta1;
+    c.power2 = before2 * beta2;
+    c.correct1 = (float)(1.0 / (1.0 - c.power1));
+    c.correct2 = (float)(1.0 / (1.0 - c.power2));
+    c.step = step;
+}
 
 struct StepArgs
 {
@@ -40,11 +56,29 @@ struct StepArgs
     const float *rateDevice, *gradientScale; const uint32_t *skip;
 };
 
-template<typename T> __device__ inline void load4(const void *array, uint64_t at, uint32_t there, bool whole, float (&x)[4])
+// Four neighbouring elements; STREAM: which nobody reads again soon
+template<bool STREAM, typename P> __device__ inline P loadPack(const P *from)
+{
+    if constexpr(!STREAM) { return *from; }
+    else {
+        typedef uint32_t Words __attribute__((ext_vector_type(sizeof(P) / 4)));
+        const Words w = __builtin_nontemporal_load((const Words*)from);
+        return __builtin_bit_cast(P, w);
+    }
+}
+template<bool STREAM, typename P> __device__ inline void storePack(P *to, const P &p)
+{
+    if constexpr(!STREAM) { *to = p; }
+    else {
+        typedef uint32_t Words __attribute__((ext_vector_type(sizeof(P) / 4)));
+        __builtin_nontemporal_store(__builtin_bit_cast(Words, p), (Words*)to);
+    }
+}
+template<bool STREAM, typename T> __device__ inline void load4(const void *array, uint64_t at, uint32_t there, bool whole, float (&x)[4])
 {
     const T *from = (const T*)array + at;
     if(whole && there == 4) {
-        const Pack<T, 4> p = *(const Pack<T, 4>*)from;
+        const Pack<T, 4> p = loadPack<STREAM>((const Pack<T, 4>*)from);
         #pragma unroll
         for(int k = 0; k < 4; k++) { x[k] = widen(p.v[k]); }
     }
@@ -53,45 +87,45 @@ template<typename T> __device__ inline void load4(const void *array, uint64_t at
         for(int k = 0; k < 4; k++) { x[k] = k < (int)there ? widen(from[k]) : 0.0f; }
     }
 }
-__device__ inline void load4(const void *array, uint32_t type, uint64_t at, uint32_t there, bool whole, float (&x)[4])
+template<bool STREAM> __device__ inline void load4(const void *array, uint32_t type, uint64_t at, uint32_t there, bool whole, float (&x)[4])
 {
-    if(type == GENNMI_TYPE_F32) { load4<float>(array, at, there, whole, x); }
-    else if(type == GENNMI_TYPE_F16) { load4<f16>(array, at, there, whole, x); }
-    else { load4<bf16>(array, at, there, whole, x); }
+    if(type == GENNMI_TYPE_F32) { load4<STREAM, float>(array, at, there, whole, x); }
+    else if(type == GENNMI_TYPE_F16) { load4<STREAM, f16>(array, at, there, whole, x); }
+    else { load4<STREAM, bf16>(array, at, there, whole, x); }
 }
-template<typename T> __device__ inline void store4(void *array, uint64_t at, uint32_t there, bool whole, const float (&x)[4])
+template<bool STREAM, typename T> __device__ inline void store4(void *array, uint64_t at, uint32_t there, bool whole, const float (&x)[4])
 {
     T *to = (T*)array + at;
     if(whole && there == 4) {
         Pack<T, 4> p;
         #pragma unroll
         for(int k = 0; k < 4; k++) { p.v[k] = narrow<T>(x[k]); }
-        *(Pack<T, 4>*)to = p;
+        storePack<STREAM>((Pack<T, 4>*)to, p);
     }
     else {
         #pragma unroll
         for(int k = 0; k < 4; k++) { if(k < (int)there) { to[k] = narrow<T>(x[k]); } }
     }
 }
-__device__ inline void store4(void *array, uint32_t type, uint64_t at, uint32_t there, bool whole, const float (&x)[4])
+template<bool STREAM> __device__ inline void store4(void *array, uint32_t type, uint64_t at, uint32_t there, bool whole, const float (&x)[4])
 {
-    if(type == GENNMI_TYPE_F32) { store4<float>(array, at, there, whole, x); }
-    else if(type == GENNMI_TYPE_F16) { store4<f16>(array, at, there, whole, x); }
-    else { store4<bf16>(array, at, there, whole, x); }
+    if(type == GENNMI_TYPE_F32) { store4<STREAM, float>(array, at, there, whole, x); }
+    else if(type == GENNMI_TYPE_F16) { store4<STREAM, f16>(array, at, there, whole, x); }
+    else { store4<STREAM, bf16>(array, at, there, whole, x); }
 }
-__device__ inline uint32_t loadCodes(const void *array, uint64_t at, uint32_t there, bool whole)
+template<bool STREAM> __device__ inline uint32_t loadCodes(const void *array, uint64_t at, uint32_t there, bool whole)
 {
     const uint8_t *from = (const uint8_t*)array + at;
-    if(whole && there == 4) { return *(const uint32_t*)from; }
+    if(whole && there == 4) { return loadPack<STREAM>((const uint32_t*)from); }
     uint32_t codes = 0;
     #pragma unroll
     for(int k = 0; k < 4; k++) { if(k < (int)there) { codes |= (uint32_t)from[k] << (8 * k); } }
     return codes;
 }
-__device__ inline void storeCodes(void *array, uint64_t at, uint32_t there, bool whole, uint32_t codes)
+template<bool STREAM> __device__ inline void storeCodes(void *array, uint64_t at, uint32_t there, bool whole, uint32_t codes)
 {
     uint8_t *to = (uint8_t*)array + at;
-    if(whole && there == 4) { *(uint32_t*)to = codes; }
+    if(whole && there == 4) { storePack<STREAM>((uint32_t*)to, codes); }
     else {
         #pragma unroll
         for(int k = 0; k < 4; k++) { if(k < (int)there) { to[k] = (uint8_t)(codes >> (8 * k)); } }
@@ -116,105 +150,116 @@ __device__ inline float roundToOdd(double r)
     if(off == 0.0 || off != off || (bits & 1)) { return f; }
     return __uint_as_float((off > 0.0) == (r > 0.0) ? bits + 1 : bits - 1);
 }
-// 448 sqrt(v / V), ready to be rounded to e4m3: in 32 bits, and in 64 where that lies as near to the border between two codes as its error
-__device__ inline float scaledRoot(double v, float inverse, double V)
-{
-    const float r = 448.0f * __builtin_amdgcn_sqrtf((float)v * inverse);
-    // borders: halfway between neighbours of 4 bits' mantissa, or of multiples of 2^-9 below 2^-6
-    const uint32_t low = (__float_as_uint(r) & 0xfffffu) - 0x80000u + 16u;
-    const float t = r * 512.0f;
-    const bool near = r >= 0.015625f ? low < 32u : fabsf(t - floorf(t) - 0.5f) < 1e-4f;
-    return near && V > 0.0 ? roundToOdd(448.0 * sqrt(v / V)) : r;
-}
-
-template<bool EIGHT>
+template<bool EIGHT, bool STREAM>
 __global__ __launch_bounds__(256)
 void adamwKernel(StepArgs a)
 {
     if(a.skip && *a.skip) { return; }
-    const double power1 = a.counter->power1 * a.beta1, power2 = a.counter->power2 * a.beta2;
-    if(blockIdx.x < a.numChunks) {
-        const ChunkDev chunk = a.chunks[blockIdx.x];
-        const ParameterDev p = a.parameters[chunk.parameter];
+    const ChunkDev chunk = a.chunks[blockIdx.x];
+    const ParameterDev p = a.parameters[chunk.parameter];
+    const uint64_t block = (uint64_t)chunk.index * (CHUNK / 256) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = block * 256 + (threadIdx.x & 63) * 4;
+    if(block * 256 < p.count) {
         const double rate = a.rateDevice ? (double)*a.rateDevice : a.rate;
-        const float scale = a.gradientScale ? *a.gradientScale : 1.0f;
-        const float keep = (float)(1.0 - rate * p.weightDecay), step = (float)rate;
-        const float correct1 = (float)(1.0 / (1.0 - power1)), correct2 = (float)(1.0 / (1.0 - power2));
+        const float scale = a.gradientScale ? *a.gradientScale : 1.0f, step = (float)rate, keep = (float)(1.0 - rate * p.weightDecay);
+        const float correct1 = a.counter->correct1, correct2 = a.counter->correct2;
+        const uint32_t there = at < p.count ? (uint32_t)(p.count - at < 4 ? p.count - at : 4) : 0;
         const bool whole = p.whole;
-        for(uint32_t k = 0; k < CHUNK / 1024; k++) {
-            const uint64_t block = (uint64_t)chunk.index * (CHUNK / 256) + k * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-            const uint64_t at = block * 256 + (threadIdx.x & 63) * 4;
-            if(block * 256 >= p.count) { break; }
-            const uint32_t there = at < p.count ? (uint32_t)(p.count - at < 4 ? p.count - at : 4) : 0;
-            float w[4], g[4], m[4], v[4];
-            load4(p.weight, p.weightType, at, there, whole, w);
-            load4(p.gradient, p.gradientType, at, there, whole, g);
-            #pragma unroll
-            for(int i = 0; i < 4; i++) { g[i] *= scale; }
-            if(!EIGHT) {
-                load4<float>(p.m, at, there, whole, m);
-                load4<float>(p.v, at, there, whole, v);
-                #pragma unroll
-                for(int i = 0; i < 4; i++) {
-                    m[i] = __builtin_fmaf((float)a.beta1, m[i], (float)(1.0 - a.beta1) * g[i]);
-                    v[i] = __builtin_fmaf((float)a.beta2, v[i], (float)(1.0 - a.beta2) * g[i] * g[i]);
+        float w[4], g[4], m[4], v[4];
+        load4<STREAM>(p.weight, p.weightType, at, there, whole, w);
+        load4<STREAM>(p.gradient, p.gradientType, at, there, whole, g);
+        #pragma unroll
+        for(int i = 0; i < 4; i++) { g[i] *= scale; }
+                if(!EIGHT) {
+            load4<STREAM, float>(p.m, at, there, whole, m);
+            load4<STREAM, float>(p.v, at, there, whole, v);
+                    #pragma unroll
+                    for(int i = 0; i < 4; i++) {
+                        m[i] = __builtin_fmaf((float)a.beta1, m[i], (float)(1.0 - a.beta1) * g[i]);
+                        v[i] = __builtin_fmaf((float)a.beta2, v[i], (float)(1.0 - a.beta2) * g[i] * g[i]);
+                    }
+                    store4<STREAM, float>(p.m, at, there, whole, m);
+                    store4<STREAM, float>(p.v, at, there, whole, v);
                 }
-                store4<float>(p.m, at, there, whole, m);
-                store4<float>(p.v, at, there, whole, v);
-            }
-            else {
-                // In 64 bits (as fast here as 32): the codes are those of the formula, not of its rounding errors next to a border
-                decode(loadCodes(p.m, at, there, whole), m);
-                decode(loadCodes(p.v, at, there, whole), v);
-                const double unitM = (double)p.mScale[block] * (1.0 / 448.0), unitV = (double)p.vScale[block] * (1.0 / (448.0 * 448.0));
-                double m64[4], v64[4];
-                float mostM = 0.0f, mostV = 0.0f;
-                bool oddM = false, oddV = false;        // not a number somewhere: maxima pass those over
-                #pragma unroll
-                for(int i = 0; i < 4; i++) {
-                    const double gradient = g[i], c = v[i];
-                    m64[i] = __builtin_fma(a.beta1, (double)m[i] * unitM, (1.0 - a.beta1) * gradient);
-                    v64[i] = __builtin_fma(a.beta2, c * c * unitV, (1.0 - a.beta2) * gradient * gradient);
-                    m[i] = (float)m64[i];
-                    v[i] = (float)v64[i];
-                    mostM = fmaxf(mostM, fabsf(m[i]));
-                    mostV = fmaxf(mostV, v[i]);
-                    oddM = oddM || m[i] != m[i];
-                    oddV = oddV || v[i] != v[i];
+                else {
+                    // States in 64 bits (as fast here as 32), so that the scales are those of the formula and not of its rounding errors.  The codes are found in
+                    // 32 bits, from values 2^-20 of themselves below and above: where the two differ, a border between codes lies so near that 64 bits have to
+                    // say on which side (one wavefront in 60).
+                    decode(loadCodes<STREAM>(p.m, at, there, whole), m);
+                    decode(loadCodes<STREAM>(p.v, at, there, whole), v);
+                    const double unitM = a.beta1 * ((double)p.mScale[block] * (1.0 / 448.0)), unitV = a.beta2 * ((double)p.vScale[block] * (1.0 / (448.0 * 448.0)));
+                    double m64[4], v64[4];
+                    uint32_t bitsM = 0, bitsV = 0;
+                    #pragma unroll
+                    for(int i = 0; i < 4; i++) {
+                        const double gradient = g[i];
+                        m64[i] = __builtin_fma((double)m[i], unitM, (1.0 - a.beta1) * gradient);
+                        v64[i] = __builtin_fma((1.0 - a.beta2) * gradient, gradient, (double)(v[i] * v[i]) * unitV);
+                        m[i] = (float)m64[i];
+                        v[i] = (float)v64[i];
+                        bitsM = max(bitsM, __float_as_uint(fabsf(m[i])));
+                        bitsV = max(bitsV, __float_as_uint(v[i]));
+                    }
+                    gennmi_lanes::maxOfLanes(bitsM, bitsV);
+                    const float M = __uint_as_float(bitsM), V = __uint_as_float(bitsV);
+                    constexpr float BELOW = 448.0f * (1.0f - 0x1p-20f), ABOVE = 448.0f * (1.0f + 0x1p-20f), LEAST = 0x1p-18f / (448.0f * 448.0f);
+                    const float inverseM = M > 0.0f ? __builtin_amdgcn_rcpf(M) : M, inverseV = V > 0.0f ? __builtin_amdgcn_rcpf(V) : V;
+                    const float belowM = BELOW * inverseM, aboveM = ABOVE * inverseM;
+                    float lowM[4], highM[4], lowV[4], highV[4];
+                    #pragma unroll
+                    for(int i = 0; i < 4; i++) {
+                        lowM[i] = m[i] * belowM;
+                        highM[i] = m[i] * aboveM;
+                        // (a positive v has a code of its own: at least the root of LEAST)
+                        const float share = v[i] * inverseV, root = __builtin_amdgcn_sqrtf(v[i] > 0.0f && share < LEAST ? LEAST : share);
+                        lowV[i] = root * BELOW;
+                        highV[i] = root * ABOVE;
+                    }
+                    uint32_t codesM = encode(lowM), codesV = encode(lowV);
+                    // (nor do quotients of 32 bits do where the largest of a block are so small that inverses or others' are subnormal)
+                    const bool near = codesM != encode(highM) || codesV != encode(highV) || M < 1e-25f || V < 1e-25f;
+                    if(__ballot(near)) {
+                        #pragma unroll
+                        for(int i = 0; i < 4; i++) {
+                            if(M > 0.0f) { lowM[i] = roundToOdd(m64[i] * (448.0 / (double)M)); }
+                            if(V > 0.0f) { lowV[i] = roundToOdd(448.0 * sqrt(v64[i] / (double)V)); }
+                            lowV[i] = v[i] > 0.0f && lowV[i] < 0x1p-9f ? 0x1p-9f : lowV[i];
+                        }
+                        codesM = encode(lowM);
+                        codesV = encode(lowV);
+                    }
+                    storeCodes<STREAM>(p.m, at, there, whole, codesM);
+                    storeCodes<STREAM>(p.v, at, there, whole, codesV);
+                    if((threadIdx.x & 63) == 0) { p.mScale[block] = M; p.vScale[block] = V; }
                 }
-                mostM = gennmi_lanes::maxOfLanes(mostM);
-                mostV = gennmi_lanes::maxOfLanes(mostV);
-                if(__ballot(oddM)) { mostM = __builtin_nanf(""); }
-                if(__ballot(oddV)) { mostV = __builtin_nanf(""); }
-                const double inverseM = mostM > 0.0f ? 448.0 / (double)mostM : (double)mostM;
-                const float inverseV = mostV > 0.0f ? 1.0f / mostV : mostV;
-                float codesM[4], codesV[4];
-                #pragma unroll
-                for(int i = 0; i < 4; i++) {
-                    codesM[i] = roundToOdd(m64[i] * inverseM);
-                    codesV[i] = scaledRoot(v64[i], inverseV, (double)mostV);
-                    if(v64[i] > 0.0 && codesV[i] < 0.001953125f) { codesV[i] = 0.001953125f; }
+                if(a.epsilon >= 1e-12f) {
+                    // (one instruction each for root and inverse: their last bit, and subnormal second moments, do not matter beside epsilon)
+                    #pragma unroll
+                    for(int i = 0; i < 4; i++) {
+                        const float change = m[i] * correct1 * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[i] * correct2) + a.epsilon);
+                        w[i] = __builtin_fmaf(-step, change, w[i] * keep);
+                    }
                 }
-                storeCodes(p.m, at, there, whole, encode(codesM));
-                storeCodes(p.v, at, there, whole, encode(codesV));
-                if((threadIdx.x & 63) == 0) { p.mScale[block] = mostM; p.vScale[block] = mostV; }
-            }
-            #pragma unroll
-            for(int i = 0; i < 4; i++) {
-                const float change = m[i] * correct1 / (sqrtf(v[i] * correct2) + a.epsilon);
-                w[i] = __builtin_fmaf(-step, change, w[i] * keep);
-            }
-            store4(p.weight, p.weightType, at, there, whole, w);
-            if(p.copy) { store4(p.copy, p.copyType, at, there, whole, w); }
-        }
+                else {
+                    #pragma unroll
+                    for(int i = 0; i < 4; i++) {
+                        const float change = m[i] * correct1 / (sqrtf(v[i] * correct2) + a.epsilon);
+                        w[i] = __builtin_fmaf(-step, change, w[i] * keep);
+                    }
+                }
+                store4<STREAM>(p.weight, p.weightType, at, there, whole, w);
+                if(p.copy) { store4<STREAM>(p.copy, p.copyType, at, there, whole, w); }
     }
-    // (every work-group has read the powers before it is counted here)
+    // (every work-group has read what it needs of the counter before it is counted here)
     __syncthreads();
-    if(threadIdx.x == 0 && atomicAdd(&a.counter->ended, 1u) == gridDim.x - 1) {
-        a.counter->ended = 0;
-        a.counter->power1 = power1;
-        a.counter->power2 = power2;
-        a.counter->step++;
+    if(threadIdx.x) { return; }
+    if(gridDim.x > GROUPS) {
+        uint32_t *const place = a.counter->ended + (1 + blockIdx.x % GROUPS) * LINE;
+        if(atomicAdd(place, 1u) != (gridDim.x - 1 - blockIdx.x % GROUPS) / GROUPS) { return; }
+        *place = 0;
+    }
+    if(atomicAdd(a.counter->ended, 1u) == min(gridDim.x, GROUPS) - 1) {
+        a.counter->ended[0] = 0;
+        setCounter(*a.counter, a.beta1, a.beta2, a.counter->power1, a.counter->power2, a.counter->step + 1);
     }
 }
 
@@ -225,6 +270,7 @@ struct gennmi_optimiser
     gennmi_adamw_t settings{};
     std::vector<gennmi_parameter_t> parameters;
     std::vector<ParameterDev> table;
+    uint64_t bytes = 0;             // that a step reads and writes
     ParameterDev *dParameters = nullptr; ChunkDev *dChunks = nullptr; CounterDev *dCounter = nullptr;
     uint32_t numChunks = 0;
     bool finalised = false;
@@ -291,6 +337,7 @@ int gennmi_optimiser_push(gennmi_optimiser *optimiser, const gennmi_parameter_t 
         ParameterDev d{p.weight, p.gradient, p.copy, p.m, p.v, p.mScale, p.vScale, p.count, p.weightType, p.gradientType, p.copyType, 0, p.weightDecay};
         d.whole = (uintptr_t)p.weight % (4 * weightSize) == 0 && (uintptr_t)p.gradient % (4 * gradientSize) == 0 && (uintptr_t)p.copy % 8 == 0 &&
                   (uintptr_t)p.m % (4 * stateSize) == 0 && (uintptr_t)p.v % (4 * stateSize) == 0;
+        optimiser->bytes += p.count * (2 * weightSize + gradientSize + 4 * stateSize + (p.copy ? 2 : 0));
         optimiser->parameters.push_back(p);
         optimiser->table.push_back(d);
         if(idx) { *idx = (uint32_t)optimiser->parameters.size() - 1; }
@@ -309,6 +356,8 @@ int gennmi_optimiser_finalise(gennmi_optimiser *optimiser)
             if(chunks.size() + of > 0x7fffffffull) { return fail(GENNMI_EINVAL, "optimiser_finalise: more weights than one launch covers"); }
             for(uint64_t c = 0; c < of; c++) { chunks.push_back({(uint32_t)k, (uint32_t)c}); }
         }
+        if(chunks.empty()) { chunks.push_back({(uint32_t)optimiser->table.size(), 0}); }        // (a step of nothing counts: a tensor without weights)
+        optimiser->table.push_back(ParameterDev{});
         // (arrays of an earlier attempt that failed half-way are freed with the optimiser)
         auto upload = [&](auto **to, const auto &from) {
             if(const int rc = gennmi_malloc((void**)to, from.size() * sizeof(from[0]))) { return rc; }
@@ -316,7 +365,9 @@ int gennmi_optimiser_finalise(gennmi_optimiser *optimiser)
         };
         if(!optimiser->dParameters) { if(const int rc = upload(&optimiser->dParameters, optimiser->table)) { return rc; } }
         if(!optimiser->dChunks) { if(const int rc = upload(&optimiser->dChunks, chunks)) { return rc; } }
-        if(!optimiser->dCounter) { if(const int rc = upload(&optimiser->dCounter, std::vector<CounterDev>(1, CounterDev{1.0, 1.0, 0, 0, 0}))) { return rc; } }
+        std::vector<CounterDev> counter(1, CounterDev{});
+        setCounter(counter[0], optimiser->settings.beta1, optimiser->settings.beta2, 1.0, 1.0, 0);
+        if(!optimiser->dCounter) { if(const int rc = upload(&optimiser->dCounter, counter)) { return rc; } }
         optimiser->numChunks = (uint32_t)chunks.size();
         optimiser->finalised = true;
         return (int)GENNMI_OK;
@@ -336,9 +387,12 @@ int gennmi_optimiser_step(gennmi_optimiser *optimiser, const gennmi_adamw_step_t
         const gennmi_optimiser &o = *optimiser;
         const StepArgs a{o.dParameters, o.dChunks, o.dCounter, o.numChunks, 0, o.settings.beta1, o.settings.beta2, step->rate, (float)o.settings.epsilon,
                          step->rateDevice, step->gradientScale, step->skip};
-        const dim3 grid(o.numChunks ? o.numChunks : 1);
-        if(o.settings.stateBits == 8) { adamwKernel<true><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
-        else { adamwKernel<false><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
+        const dim3 grid(o.numChunks);
+        const bool eight = o.settings.stateBits == 8, streaming = o.bytes > STREAM_BYTES;
+        if(eight && streaming) { adamwKernel<true, true><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
+        else if(eight) { adamwKernel<true, false><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
+        else if(streaming) { adamwKernel<false, true><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
+        else { adamwKernel<false, false><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
         if(const int rc = gennmi_detail::afterLaunch("optimiser_step")) { return rc; }
         for(const gennmi_parameter_t &p : o.parameters) {
             if(p.count) { gennmi_detail::noteDeviceWrite(p.weight, p.count * sizeOf(p.weightType)); }
@@ -366,7 +420,9 @@ int gennmi_optimiser_set_step(gennmi_optimiser *optimiser, uint64_t step)
         if(!optimiser) { return fail(GENNMI_EINVAL, "optimiser_set_step: null argument"); }
         if(!optimiser->finalised) { return fail(GENNMI_ESTATE, "optimiser_set_step: the optimiser is not finalised"); }
         if(const int rc = gennmi_synchronize()) { return rc; }
-        const CounterDev counter{std::pow(optimiser->settings.beta1, (double)step), std::pow(optimiser->settings.beta2, (double)step), step, 0, 0};
+        CounterDev counter{};
+        const double beta1 = optimiser->settings.beta1, beta2 = optimiser->settings.beta2;
+        setCounter(counter, beta1, beta2, std::pow(beta1, (double)step), std::pow(beta2, (double)step), step);
         return gennmi_memcpy_to_device(optimiser->dCounter, &counter, sizeof(counter));
     });
 }
