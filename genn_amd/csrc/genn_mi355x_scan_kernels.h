@@ -41,13 +41,12 @@ struct ScanGradientArgs
 
 __device__ inline float exp2Of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float logistic(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2Of(x * -LOG2E)); }
-// log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|).  With f the rounded 1 + e, log(1 + e) = log(f) e / (f - 1) to the last bits,
-// also where e is small and f has lost most of it.
+// log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|).  Where e is small, f = 1 + e as rounded has lost most of it: log(1 + e) = log(f) + log((1 + e) / f),
+// and the second is e - (f - 1) to the last bits (that difference is exact, below 2^-24, and f is at most 2).
 __device__ inline float softplusOf(float x)
 {
-    const float e = exp2Of(fabsf(x) * -LOG2E), f = 1.0f + e, d = f - 1.0f;
-    const float tail = d == 0.0f ? e : __builtin_amdgcn_logf(f) * LN2 * (e * __builtin_amdgcn_rcpf(d));
-    return x != x ? x : fmaxf(x, 0.0f) + tail;
+    const float e = exp2Of(fabsf(x) * -LOG2E), f = 1.0f + e;
+    return fmaxf(x, 0.0f) + __builtin_fmaf(__builtin_amdgcn_logf(f), LN2, e - (f - 1.0f));
 }
 
 // Where a work-group is: a chunk and a tile of channels
@@ -77,40 +76,66 @@ template<int NP> __device__ inline ScanPlace scanPlace(const ScanArgs &a, uint32
 }
 
 // B and C of R rows, of a wavefront's states, in LDS as [row][B, C][NP], zero where there is no row or state.  A lane fetches
-// R * 2 * NP / 64 of the values, a block of rows before they are needed.
+// R * 2 * NP / 64 of the values, of B or of C and of one state all of them, a block of rows before they are needed.
 template<typename T, int NP, int R> struct StagedBC
 {
-    static constexpr int EACH = R * 2 * NP / 64;
+    static constexpr int EACH = R * 2 * NP / 64, LANES = 2 * NP;        // LANES: that a row takes
+    const T *at;
+    uint64_t stride;
+    bool here;
     T raw[EACH];
-    __device__ inline void fetch(const T *B, const T *C, const ScanArgs &a, uint32_t row, uint32_t rows, uint32_t numStates)
+    __device__ inline StagedBC(const T *B, const T *C, const ScanArgs &a, uint32_t numStates)
     {
-        const uint32_t lane = threadIdx.x & 63;
-        #pragma unroll
-        for(int q = 0; q < EACH; q++) {
-            const uint32_t e = q * 64 + lane, r = e / (2 * NP), n = e % NP;
-            const bool isC = (e / NP) & 1;
-            raw[q] = T(0.0f);
-            if(row + r < rows && n < numStates) { raw[q] = isC ? C[(uint64_t)(row + r) * a.C.rowStride + n] : B[(uint64_t)(row + r) * a.B.rowStride + n]; }
-        }
+        const uint32_t lane = threadIdx.x & 63, n = lane % NP;
+        const bool isC = (lane / NP) & 1;
+        at = (isC ? C : B) + min(n, numStates - 1);
+        stride = isC ? a.C.rowStride : a.B.rowStride;
+        here = n < numStates;
     }
-    __device__ inline void store(float *lds) const
+    __device__ static inline uint32_t rowOf(int q) { return q * (64 / LANES) + (threadIdx.x & 63) / LANES; }
+    __device__ inline void fetch(uint32_t row, uint32_t end)
     {
-        const uint32_t lane = threadIdx.x & 63;
         #pragma unroll
-        for(int q = 0; q < EACH; q++) { lds[q * 64 + lane] = widen(raw[q]); }
+        for(int q = 0; q < EACH; q++) { raw[q] = at[min(row + rowOf(q), end - 1) * stride]; }
+    }
+    __device__ inline void store(float *lds, uint32_t row, uint32_t end) const
+    {
+        #pragma unroll
+        for(int q = 0; q < EACH; q++) { lds[q * 64 + (threadIdx.x & 63)] = here && row + rowOf(q) < end ? widen(raw[q]) : 0.0f; }
     }
 };
 // What one wavefront wrote to LDS is read by its other lanes: LDS accesses of a wavefront are done in order, only the compiler has to keep it
 __device__ inline void waveFence() { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
-template<typename T> __device__ inline T *rowAt(T *rows, uint32_t t, uint64_t stride) { return rows + (uint64_t)t * stride; }
-// A value the compiler knows nothing of: what is computed from it is computed again, not kept in registers from where it was computed before
-__device__ inline float again(float x) { asm volatile("" : "+v"(x)); return x; }
+// An element of a row.  The row's address is the same for all lanes, the element's place in it (in bytes) fits 32 bits: loads and stores take the two so,
+// without 64-bit arithmetic in every lane, if the compiler does not get to see how the row's address is made.
+template<typename T> __device__ inline uint64_t rowAddress(T *rows, uint32_t t, uint64_t stride)
+{
+    uint64_t address = (uint64_t)(rows + (uint64_t)t * stride);
+    asm("" : "+s"(address));
+    return address;
+}
+template<typename T> __device__ inline T loadAt(const T *rows, uint32_t t, uint64_t stride, uint32_t place)
+{
+    return *(const __attribute__((address_space(1))) T*)((const __attribute__((address_space(1))) char*)rowAddress(rows, t, stride) + place);
+}
+template<typename T> __device__ inline void storeAt(T *rows, uint32_t t, uint64_t stride, uint32_t place, T value)
+{
+    *(__attribute__((address_space(1))) T*)((__attribute__((address_space(1))) char*)rowAddress(rows, t, stride) + place) = value;
+}
 // Reads of LDS behind this point wait for the four values.  (Left alone, the compiler gathers the reads of many rows in front of all arithmetic, puts off
 // sums that nothing waits for until behind it, and spills hundreds of registers.)
 __device__ inline void readAfter(float &a, float &b, float &c, float &d) { asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : : "memory"); }
 
 // (a wavefront with fewer than NP states reads its last one again instead: a select costs less than a branch a state)
+__device__ inline void readAfter(float &a, float &b) { asm volatile("" : "+v"(a), "+v"(b) : : "memory"); }
+// ... COUNT values from the one at `first` on
+template<int COUNT, int N> __device__ inline void readAfter(float (&x)[N], int first = 0)
+{
+    #pragma unroll
+    for(int n = 0; n < COUNT; n += 2) { readAfter(x[first + n], x[first + n + 1]); }
+}
+
 template<int NP> __device__ inline void loadA(const ScanArgs &a, const ScanPlace &s, float (&A)[NP])
 {
     const float *from = a.A + (uint64_t)s.channel * a.states + s.firstState;
@@ -156,10 +181,10 @@ template<int NP> __device__ inline void storeChunk(const ScanArgs &a, const Scan
 template<typename T, int R> struct StagedRows
 {
     T raw[R];
-    __device__ inline void fetch(const T *rows, uint64_t stride, uint32_t channel, uint32_t row, uint32_t end)
+    __device__ inline void fetch(const T *rows, uint64_t stride, uint32_t place, uint32_t row, uint32_t end)
     {
         #pragma unroll
-        for(int r = 0; r < R; r++) { raw[r] = rowAt(rows, min(row + r, end - 1), stride)[channel]; }
+        for(int r = 0; r < R; r++) { raw[r] = loadAt(rows, min(row + r, end - 1), stride, place); }
     }
 };
 // dt and dt u of a block of rows; zero behind the end, which leaves every state as it is
@@ -173,9 +198,10 @@ __device__ inline void times(const ScanArgs &a, const StagedRows<T, R> &delta, c
         for(int r = 0; r < R; r++) { dt[r] = softplusOf(dt[r]); }
     }
     #pragma unroll
-    for(int r = 0; r < R; r++) {
-        dt[r] = r < (int)there ? dt[r] : 0.0f;
-        w[r] = r < (int)there ? dt[r] * widen(u.raw[r]) : 0.0f;
+    for(int r = 0; r < R; r++) { w[r] = dt[r] * widen(u.raw[r]); }
+    if(there < R) {
+        #pragma unroll
+        for(int r = 0; r < R; r++) { if(r >= (int)there) { dt[r] = w[r] = 0.0f; } }
     }
 }
 // The gate, z sigmoid(z)
@@ -197,7 +223,7 @@ void scanChunkKernel(ScanArgs a, ScanGradientArgs g)
     const ScanPlace s = scanPlace<NP>(a, number);
     if(!s.valid) { return; }
     float *const bc = staged[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
-    const uint32_t channel = s.channel;
+    const uint32_t channel = s.channel, place = channel * (uint32_t)sizeof(T);
     const T *u = rowsOf<const T>(a.u, a.sequences, s.place), *delta = rowsOf<const T>(a.delta, a.sequences, s.place);
     const uint32_t bcAt = s.group * a.states + s.firstState;
     const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
@@ -209,14 +235,14 @@ void scanChunkKernel(ScanArgs a, ScanGradientArgs g)
     #pragma unroll
     for(int n = 0; n < NP; n++) { h[n] = G[n] = 0.0f; P[n] = 1.0f; }
     const uint32_t end = s.first + s.rows;
-    StagedBC<T, NP, R> stage;
+    StagedBC<T, NP, R> stage(B, C, a, s.numStates);
     StagedRows<T, R> rawU, rawDelta, rawOut, rawZ;
     const auto fetch = [&](uint32_t row) {
-        stage.fetch(B, C, a, row, end, s.numStates);
-        rawU.fetch(u, a.u.rowStride, channel, row, end);
-        rawDelta.fetch(delta, a.delta.rowStride, channel, row, end);
-        if(GRADIENT) { rawOut.fetch(dout, g.out.rowStride, channel, row, end); }
-        if(GRADIENT && z) { rawZ.fetch(z, a.z.rowStride, channel, row, end); }
+        stage.fetch(row, end);
+        rawU.fetch(u, a.u.rowStride, place, row, end);
+        rawDelta.fetch(delta, a.delta.rowStride, place, row, end);
+        if(GRADIENT) { rawOut.fetch(dout, g.out.rowStride, place, row, end); }
+        if(GRADIENT && z) { rawZ.fetch(z, a.z.rowStride, place, row, end); }
     };
     if(s.rows) { fetch(s.first); }
     for(uint32_t row = s.first; row < end; row += R) {
@@ -233,9 +259,9 @@ void scanChunkKernel(ScanArgs a, ScanGradientArgs g)
             }
         }
         waveFence();
-        stage.store(bc);
+        stage.store(bc, row, end);
         waveFence();
-        if(row + R < end) { fetch(row + R); }
+        fetch(row + R);         // (behind the last block: its last row, for nothing)
         float nextB[NP], nextC[NP];
         #pragma unroll
         for(int n = 0; n < NP; n++) { nextB[n] = bc[n]; if(GRADIENT) { nextC[n] = bc[NP + n]; } }
@@ -246,8 +272,8 @@ void scanChunkKernel(ScanArgs a, ScanGradientArgs g)
             for(int n = 0; n < NP; n++) { Bn[n] = nextB[n]; Cn[n] = nextC[n]; }
             if(r + 1 < R) {
                 // (a row's inputs are read while the row before is worked on, and no sooner)
-                readAfter(h[NP - 4], h[NP - 3], h[NP - 2], h[NP - 1]);
-                if(GRADIENT) { readAfter(G[NP - 4], G[NP - 3], G[NP - 2], G[NP - 1]); }
+                readAfter<NP>(h);
+                if(GRADIENT) { readAfter<NP>(G); readAfter<NP>(P); }
                 #pragma unroll
                 for(int n = 0; n < NP; n++) { nextB[n] = bc[(r + 1) * 2 * NP + n]; if(GRADIENT) { nextC[n] = bc[((r + 1) * 2 + 1) * NP + n]; } }
             }
@@ -329,7 +355,7 @@ void scanKernel(ScanArgs a)
     uint32_t number;
     const ScanPlace s = scanPlace<NP>(a, number);
     if(!s.valid) { return; }
-    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, channel = s.channel;
+    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, channel = s.channel, place = channel * (uint32_t)sizeof(T);
     float *const bc = staged[slab];
     const T *u = rowsOf<const T>(a.u, a.sequences, s.place), *delta = rowsOf<const T>(a.delta, a.sequences, s.place);
     const T *z = a.z.data ? rowsOf<const T>(a.z, a.sequences, s.place) : nullptr;
@@ -341,13 +367,13 @@ void scanKernel(ScanArgs a)
     loadA<NP>(a, s, A);
     if(a.chunkState) { loadChunk<NP>(a, s, a.chunkState, number, h); } else { loadState<NP>(a, s, a.initialState, s.place.state, h); }
     const uint32_t end = s.first + s.rows;
-    StagedBC<T, NP, R> stage;
+    StagedBC<T, NP, R> stage(B, C, a, s.numStates);
     StagedRows<T, R> rawU, rawDelta, rawZ;
     const auto fetch = [&](uint32_t row) {
-        stage.fetch(B, C, a, row, end, s.numStates);
-        rawU.fetch(u, a.u.rowStride, channel, row, end);
-        rawDelta.fetch(delta, a.delta.rowStride, channel, row, end);
-        if(z) { rawZ.fetch(z, a.z.rowStride, channel, row, end); }
+        stage.fetch(row, end);
+        rawU.fetch(u, a.u.rowStride, place, row, end);
+        rawDelta.fetch(delta, a.delta.rowStride, place, row, end);
+        if(z) { rawZ.fetch(z, a.z.rowStride, place, row, end); }
     };
     if(s.rows) { fetch(s.first); }
     uint32_t turn = 0;
@@ -358,9 +384,9 @@ void scanKernel(ScanArgs a)
         for(int r = 0; r < R; r++) { direct[r] = skip * widen(rawU.raw[r]); gate[r] = 1.0f; }
         if(z) { gates<T, R>(rawZ, gate); }
         waveFence();
-        stage.store(bc);
+        stage.store(bc, row, end);
         waveFence();
-        if(row + R < end) { fetch(row + R); }
+        fetch(row + R);         // (behind the last block: its last row, for nothing)
         float nextB[NP], nextC[NP];
         #pragma unroll
         for(int n = 0; n < NP; n++) { nextB[n] = bc[n]; nextC[n] = bc[NP + n]; }
@@ -371,7 +397,8 @@ void scanKernel(ScanArgs a)
             for(int n = 0; n < NP; n++) { Bn[n] = nextB[n]; Cn[n] = nextC[n]; }
             if(r + 1 < R) {
                 // (a row's inputs are read while the row before is worked on, and no sooner)
-                if(r) { readAfter(h[NP - 3], h[NP - 2], h[NP - 1], y[r - 1]); }
+                readAfter<NP>(h);
+                if(r) { readAfter(y[r - 1], h[0], h[1], h[2]); }
                 #pragma unroll
                 for(int n = 0; n < NP; n++) { nextB[n] = bc[(r + 1) * 2 * NP + n]; nextC[n] = bc[((r + 1) * 2 + 1) * NP + n]; }
             }
@@ -398,7 +425,7 @@ void scanKernel(ScanArgs a)
         if(s.active) {
             #pragma unroll
             for(int r = 0; r < R; r++) {
-                if(row + r < end && (!SLABS || r % a.slabs == slab)) { rowAt(out, row + r, a.out.rowStride)[channel] = narrow<T>(y[r] * gate[r]); }
+                if(row + r < end && (!SLABS || r % a.slabs == slab)) { storeAt(out, row + r, a.out.rowStride, place, narrow<T>(y[r] * gate[r])); }
             }
         }
     }
@@ -520,19 +547,24 @@ void scanTokenKernel(ScanArgs a)
 // forward through a block that keeps its states in registers, and one back:
 //   dh = C gy + (what comes from the row behind);  dC = gy h, dB = dh dt u (summed over channels);  q = sum dh B, x = dh exp(dt A) h', r = sum x A
 //   du = dt q + D gy;  d(dt) = u q + r;  dA += x dt;  and exp(dt A) dh for the row before
-// A block's walks take PART of the states at a time, so that R * PART of them fit the registers of two wavefronts a SIMD.
+// A block's walks take PART of the states at a time, so that R * PART of them, and as many decays, fit the registers of two wavefronts a SIMD.
 template<typename T, int NP, int R, int BLOCKS, bool SLABS>
 __global__ __launch_bounds__(SLABS ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
 {
-    constexpr int PART = 4, PARTS = NP / PART, SPREAD = 64 / (2 * PART);     // SPREAD: lanes that have the same sum over the lanes
-    extern __shared__ float lds[];
+    constexpr int PART = 2, PARTS = NP / PART, SPREAD = 64 / (2 * PART);     // SPREAD: lanes that have the same sum over the lanes
+    constexpr int SPACE = BLOCKS * NP * 64 + R * 2 * NP * 2;                 // floats of LDS a wavefront
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     uint32_t number;
     const ScanPlace s = scanPlace<NP>(a, number);
-    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, channel = s.channel;
-    float *const kept = lds + (size_t)slab * ((BLOCKS - 1) * NP * 64 + R * 2 * NP);     // [block][state][lane]
-    float *const bc = kept + (BLOCKS - 1) * NP * 64;
-    float *const sums = lds + (size_t)a.slabs * ((BLOCKS - 1) * NP * 64 + R * 2 * NP);  // SLABS: [slab][row][q, r, y][lane]
+    const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, channel = s.channel, place = channel * (uint32_t)sizeof(T);
+    float *const kept = lds + (size_t)slab * SPACE;       // [block][part][lane][PART]: the states before a block
+    float *const bc = kept + BLOCKS * NP * 64, *const rowSums = bc + R * 2 * NP;     // both [row][B, C][NP]
+    float *const sums = lds + (size_t)a.slabs * SPACE;      // SLABS: [slab][row][q, r, y][lane]
+    const auto keep = [&](uint32_t b, const float (&h)[NP]) {
+        #pragma unroll
+        for(int n = 0; n < NP; n++) { kept[((b * PARTS + n / PART) * 64 + lane) * PART + n % PART] = h[n]; }
+    };
     float dA[NP], dD = 0.0f, dBias = 0.0f;
     #pragma unroll
     for(int n = 0; n < NP; n++) { dA[n] = 0.0f; }
@@ -544,60 +576,63 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
         const uint32_t bcAt = s.group * a.states + s.firstState;
         const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
         const float bias = a.deltaBias ? a.deltaBias[channel] : 0.0f, skip = a.D ? a.D[channel] : 0.0f;
-        // Sums over the channels of a row: part p's are with the lanes that are p modulo SPREAD, so a row's are written by one store
         const uint64_t sumRow = (uint64_t)s.tile * g.rows + (a.sequences.offsets ? s.place.first : (uint64_t)s.place.sequence * a.sequences.length);
-        const uint32_t sumState = (lane % SPREAD) * PART + (lane / SPREAD) % PART, sumAt = (lane / (32)) * a.states + s.firstState + sumState;
-        const bool sumHere = lane % SPREAD < PARTS && sumState < s.numStates;
+        // (where this lane's sum over the lanes goes, SPREAD of them to the same place)
+        float *const rowSum = rowSums + (lane / 32) * NP + (lane / SPREAD) % PART;
         float A[NP], h[NP], carry[NP];
         loadA<NP>(a, s, A);
         if(a.chunkState) { loadChunk<NP>(a, s, a.chunkState, number, h); loadChunk<NP>(a, s, g.chunkGradient, number, carry); }
         else { loadState<NP>(a, s, a.initialState, s.place.state, h); loadState<NP>(a, s, g.finalState, s.place.state, carry); }
         const uint32_t end = s.first + s.rows, blocks = (s.rows + R - 1) / R;
-        StagedBC<T, NP, R> stage;
+        StagedBC<T, NP, R> stage(B, C, a, s.numStates);
         for(uint32_t b = 0; b + 1 < blocks; b++) {
             const uint32_t row = s.first + b * R;
             T rawU[R], rawDelta[R];
             #pragma unroll
             for(int r = 0; r < R; r++) {
-                rawU[r] = rowAt(u, row + r, a.u.rowStride)[channel];
-                rawDelta[r] = rowAt(delta, row + r, a.delta.rowStride)[channel];
+                rawU[r] = loadAt(u, row + r, a.u.rowStride, place);
+                rawDelta[r] = loadAt(delta, row + r, a.delta.rowStride, place);
             }
-            stage.fetch(B, C, a, row, end, s.numStates);
+            stage.fetch(row, end);
+            keep(b, h);
+            waveFence();
+            stage.store(bc, row, end);
+            waveFence();
+            float nextB[NP];
             #pragma unroll
-            for(int n = 0; n < NP; n++) { kept[(b * NP + n) * 64 + lane] = h[n]; }
-            waveFence();
-            stage.store(bc);
-            waveFence();
+            for(int n = 0; n < NP; n++) { nextB[n] = bc[n]; }
             #pragma unroll
             for(int r = 0; r < R; r++) {
-                float dt = widen(rawDelta[r]) + bias;
+                float dt = widen(rawDelta[r]) + bias, Bn[NP];
                 dt = a.softplus ? softplusOf(dt) : dt;
                 const float w = dt * widen(rawU[r]);
-                readAfter(h[0], h[1], h[2], h[3]);
+                readAfter<NP>(h);
                 #pragma unroll
-                for(int n = 0; n < NP; n++) { h[n] = __builtin_fmaf(exp2Of(dt * A[n]), h[n], w * bc[r * 2 * NP + n]); }
+                for(int n = 0; n < NP; n++) {
+                    Bn[n] = nextB[n];
+                    if(r + 1 < R) { nextB[n] = bc[(r + 1) * 2 * NP + n]; }
+                }
+                #pragma unroll
+                for(int n = 0; n < NP; n++) { h[n] = __builtin_fmaf(exp2Of(dt * A[n]), h[n], w * Bn[n]); }
             }
         }
+        if(blocks) { keep(blocks - 1, h); }
         for(uint32_t b = blocks; b-- > 0; ) {
             const uint32_t row = s.first + b * R;
-            if(b + 1 < blocks) {
-                #pragma unroll
-                for(int n = 0; n < NP; n++) { h[n] = kept[(b * NP + n) * 64 + lane]; }
-            }
-            stage.fetch(B, C, a, row, end, s.numStates);
-            float dt[R], uu[R], gy[R], slope[R], q[R], rr[R], y[R], both[R];
+            stage.fetch(row, end);
+            float dt[R], uu[R], gy[R], q[R], rr[R], y[R];
             {
                 T rawDelta[R], rawU[R], rawOut[R], rawZ[R];
                 #pragma unroll
                 for(int r = 0; r < R; r++) {
                     const uint32_t t = min(row + r, end - 1);
-                    rawDelta[r] = rowAt(delta, t, a.delta.rowStride)[channel];
-                    rawU[r] = rowAt(u, t, a.u.rowStride)[channel];
-                    rawOut[r] = rowAt(dout, t, g.out.rowStride)[channel];
+                    rawDelta[r] = loadAt(delta, t, a.delta.rowStride, place);
+                    rawU[r] = loadAt(u, t, a.u.rowStride, place);
+                    rawOut[r] = loadAt(dout, t, g.out.rowStride, place);
                 }
                 if(z) {
                     #pragma unroll
-                    for(int r = 0; r < R; r++) { rawZ[r] = rowAt(z, min(row + r, end - 1), a.z.rowStride)[channel]; }
+                    for(int r = 0; r < R; r++) { rawZ[r] = loadAt(z, min(row + r, end - 1), a.z.rowStride, place); }
                     #pragma unroll
                     for(int r = 0; r < R; r++) { const float zr = widen(rawZ[r]); gy[r] = widen(rawOut[r]) * (zr * logistic(zr)); }
                 }
@@ -611,72 +646,90 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
                     const bool there = row + r < end && s.active;
                     const float raw = widen(rawDelta[r]) + bias;
                     const float time = a.softplus ? softplusOf(raw) : raw;
-                    slope[r] = a.softplus ? logistic(raw) : 1.0f;
                     dt[r] = there ? time : 0.0f;
                     uu[r] = there ? widen(rawU[r]) : 0.0f;
                     gy[r] = there ? gy[r] : 0.0f;
-                    q[r] = rr[r] = y[r] = both[r] = 0.0f;
+                    q[r] = rr[r] = y[r] = 0.0f;
                 }
             }
             waveFence();
-            stage.store(bc);
+            stage.store(bc, row, end);
             waveFence();
             // what a row's channel gets, when its sums over the states are there
             const auto finish = [&](int r) {
                 const uint32_t t = row + r;
                 if(!s.active) { return; }
-                if(du) { rowAt(du, t, g.u.rowStride)[channel] = narrow<T>(__builtin_fmaf(dt[r], q[r], skip * gy[r])); }
-                const float d = __builtin_fmaf(uu[r], q[r], rr[r] * LN2) * slope[r];
-                if(ddelta) { rowAt(ddelta, t, g.delta.rowStride)[channel] = narrow<T>(d); }
+                if(du) { storeAt(du, t, g.u.rowStride, place, narrow<T>(__builtin_fmaf(dt[r], q[r], skip * gy[r]))); }
+                float d = __builtin_fmaf(uu[r], q[r], rr[r] * LN2);
+                if(a.softplus) { d *= logistic(widen(loadAt(delta, t, a.delta.rowStride, place)) + bias); }
+                if(ddelta) { storeAt(ddelta, t, g.delta.rowStride, place, narrow<T>(d)); }
                 if(dz) {
-                    const float zr = widen(rowAt(z, t, a.z.rowStride)[channel]), sig = logistic(zr), dd = widen(rowAt(dout, t, g.out.rowStride)[channel]);
-                    rowAt(dz, t, g.z.rowStride)[channel] = narrow<T>(dd * __builtin_fmaf(skip, uu[r], y[r]) * (sig * (1.0f + zr * (1.0f - sig))));
+                    const float zr = widen(loadAt(z, t, a.z.rowStride, place)), sig = logistic(zr), dd = widen(loadAt(dout, t, g.out.rowStride, place));
+                    storeAt(dz, t, g.z.rowStride, place, narrow<T>(dd * __builtin_fmaf(skip, uu[r], y[r]) * (sig * (1.0f + zr * (1.0f - sig)))));
                 }
                 dBias += d;
                 dD = __builtin_fmaf(gy[r], uu[r], dD);
             };
             #pragma unroll
             for(int part = 0; part < PARTS; part++) {
-                float hs[R][PART], start[PART];
+                float hs[R][PART], decay[R][PART], start[PART];
                 #pragma unroll
-                for(int k = 0; k < PART; k++) { start[k] = h[part * PART + k]; }
+                for(int k = 0; k < PART; k++) { start[k] = kept[((b * PARTS + part) * 64 + lane) * PART + k]; }
+                float nextB[PART], nextC[PART], terms[2 * PART];
+                #pragma unroll
+                for(int k = 0; k < PART; k++) { nextB[k] = bc[part * PART + k]; }
                 #pragma unroll
                 for(int r = 0; r < R; r++) {
                     const float w = dt[r] * uu[r];
-                    float (&before)[PART] = r ? hs[r - 1] : start;
-                    readAfter(before[0], before[1], before[2], before[3]);
+                    float (&before)[PART] = r ? hs[r - 1] : start, Bn[PART];
+                    readAfter<PART>(before);
+                    #pragma unroll
+                    for(int k = 0; k < PART; k++) {
+                        Bn[k] = nextB[k];
+                        if(r + 1 < R) { nextB[k] = bc[(r + 1) * 2 * NP + part * PART + k]; }
+                    }
                     #pragma unroll
                     for(int k = 0; k < PART; k++) {
                         const int n = part * PART + k;
-                        hs[r][k] = __builtin_fmaf(exp2Of(dt[r] * A[n]), before[k], w * bc[r * 2 * NP + n]);
+                        decay[r][k] = exp2Of(dt[r] * A[n]);
+                        hs[r][k] = __builtin_fmaf(decay[r][k], before[k], w * Bn[k]);
                     }
                 }
                 #pragma unroll
+                for(int k = 0; k < PART; k++) { terms[k] = terms[PART + k] = 0.0f; nextB[k] = bc[(R - 1) * 2 * NP + part * PART + k]; nextC[k] = bc[((R - 1) * 2 + 1) * NP + part * PART + k]; }
+                #pragma unroll
                 for(int r = R - 1; r >= 0; r--) {
-                    const float time = again(dt[r]), w = time * uu[r];
+                    const float w = dt[r] * uu[r];
                     const float (&before)[PART] = r ? hs[r - 1] : start;
-                    if(r < R - 1) { readAfter(q[r + 1], rr[r + 1], y[r + 1], both[r + 1]); }
-                    readAfter(carry[part * PART], carry[part * PART + 1], carry[part * PART + 2], carry[part * PART + 3]);
-                    readAfter(dA[part * PART], dA[part * PART + 1], dA[part * PART + 2], dA[part * PART + 3]);
-                    float terms[2 * PART];
+                    float Bn[PART], Cn[PART];
+                    if(r < R - 1) {
+                        readAfter(q[r + 1], rr[r + 1], y[r + 1], carry[part * PART]);
+                        readAfter<2 * PART>(terms);
+                    }
+                    readAfter<PART>(dA, part * PART);
+                    // (the sums of the row behind: a chain of dependent steps, which this row's arithmetic fills)
+                    if(r < R - 1) { rowSum[(r + 1) * 2 * NP + part * PART] = gennmi_lanes::sumOfLanes<2 * PART>(terms); }
+                    #pragma unroll
+                    for(int k = 0; k < PART; k++) {
+                        Bn[k] = nextB[k];
+                        Cn[k] = nextC[k];
+                        if(r) { nextB[k] = bc[(r - 1) * 2 * NP + part * PART + k]; nextC[k] = bc[((r - 1) * 2 + 1) * NP + part * PART + k]; }
+                    }
                     #pragma unroll
                     for(int k = 0; k < PART; k++) {
                         const int n = part * PART + k;
-                        const float Bn = bc[r * 2 * NP + n], Cn = bc[(r * 2 + 1) * NP + n];
-                        const float dh = __builtin_fmaf(gy[r], Cn, carry[n]);
-                        y[r] = __builtin_fmaf(Cn, hs[r][k], y[r]);
+                        const float dh = __builtin_fmaf(gy[r], Cn[k], carry[n]);
+                        y[r] = __builtin_fmaf(Cn[k], hs[r][k], y[r]);
                         terms[k] = dh * w;
                         terms[PART + k] = gy[r] * hs[r][k];
-                        q[r] = __builtin_fmaf(dh, Bn, q[r]);
-                        carry[n] = exp2Of(time * A[n]) * dh;
+                        q[r] = __builtin_fmaf(dh, Bn[k], q[r]);
+                        carry[n] = decay[r][k] * dh;
                         const float x = carry[n] * before[k];
-                        dA[n] = __builtin_fmaf(x, time, dA[n]);
+                        dA[n] = __builtin_fmaf(x, dt[r], dA[n]);
                         rr[r] = __builtin_fmaf(x, A[n], rr[r]);
                     }
-                    const float sum = gennmi_lanes::sumOfLanes<2 * PART>(terms);
-                    both[r] = lane % SPREAD == part ? sum : both[r];
+                    if(r == 0) { rowSum[part * PART] = gennmi_lanes::sumOfLanes<2 * PART>(terms); }
                     if(part == PARTS - 1 && row + r < end) {
-                        if(sumHere) { (g.sumBC + (sumRow + row + r) * 2 * a.states)[sumAt] = both[r]; }
                         if(SLABS) {
                             sums[((slab * R + r) * 3) * 64 + lane] = q[r];
                             sums[((slab * R + r) * 3 + 1) * 64 + lane] = rr[r];
@@ -685,6 +738,12 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
                         else { finish(r); }
                     }
                 }
+            }
+            waveFence();
+            #pragma unroll
+            for(int e = 0; e < R * 2 * NP / 64; e++) {
+                const uint32_t at = e * 64 + lane, r = at / (2 * NP), which = (at / NP) % 2, n = at % NP;
+                if(row + r < end && n < s.numStates) { (g.sumBC + (sumRow + row + r) * 2 * a.states)[which * a.states + s.firstState + n] = rowSums[at]; }
             }
             if(SLABS) {
                 __syncthreads();

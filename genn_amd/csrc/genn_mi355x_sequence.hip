@@ -191,7 +191,11 @@ int checkScan(const char *what, const gennmi_scan_t *c, bool gradients)
 
 constexpr uint64_t TOKEN_THREADS = 256 * 2048;      // of one launch, from which a lane takes several sequences' tokens
 struct ScanPlan { uint32_t slab, slabs, chunk; bool split; };
-constexpr uint32_t SCAN_BLOCK_ROWS = 8, SCAN_BACKWARD_BLOCKS = 4;
+constexpr uint32_t SCAN_BLOCK_ROWS = 8;
+// Blocks of rows of a chunk of gradients: what is kept of each takes 4 KiB of LDS a wavefront, and eight wavefronts of one, or of a work-group of
+// several, should fit a compute unit's 160
+constexpr uint32_t gradientBlocks(uint32_t slabs) { return slabs > 1 ? 2 : 4; }
+
 uint32_t scanTiles(const gennmi_scan_t &c) { return c.groups * ((c.channels / c.groups + 63) / 64); }
 // States of a wavefront, wavefronts of a work-group, rows of a chunk
 ScanPlan scanPlan(const gennmi_scan_t &c, bool gradients)
@@ -199,7 +203,7 @@ ScanPlan scanPlan(const gennmi_scan_t &c, bool gradients)
     ScanPlan p;
     p.slab = c.states <= 8 ? 8 : 16;
     p.slabs = (c.states + p.slab - 1) / p.slab;
-    if(gradients) { p.chunk = SCAN_BLOCK_ROWS * SCAN_BACKWARD_BLOCKS; }
+    if(gradients) { p.chunk = SCAN_BLOCK_ROWS * gradientBlocks(p.slabs); }
     else {
         // enough chunks for a few wavefronts on each of the chip's 1024 SIMDs, of 64 rows at least
         const uint64_t waves = (uint64_t)scanTiles(c) * p.slabs;
@@ -294,8 +298,9 @@ template<typename T, int NP, bool SLABS> int launchScanBackward(const ScanArgs &
         scanJoinKernel<true><<<dim3(a.sequences.count * a.states * ((a.channels + 63) / 64)), dim3(64), 0, stream>>>(a, g);
         if(const int rc = gennmi_detail::afterLaunch("selective_scan_backward")) { return rc; }
     }
-    const size_t lds = sizeof(float) * (p.slabs * ((SCAN_BACKWARD_BLOCKS - 1) * NP * 64 + SCAN_BLOCK_ROWS * 2 * NP) + (SLABS ? p.slabs * SCAN_BLOCK_ROWS * 3 * 64 : 0));
-    auto kernel = scanBackwardKernel<T, NP, (int)SCAN_BLOCK_ROWS, (int)SCAN_BACKWARD_BLOCKS, SLABS>;
+    constexpr uint32_t BLOCKS = gradientBlocks(SLABS ? 2 : 1);
+    const size_t lds = sizeof(float) * (p.slabs * (BLOCKS * NP * 64 + SCAN_BLOCK_ROWS * 2 * NP * 2) + (SLABS ? p.slabs * SCAN_BLOCK_ROWS * 3 * 64 : 0));
+    auto kernel = scanBackwardKernel<T, NP, (int)SCAN_BLOCK_ROWS, (int)BLOCKS, SLABS>;
     if(lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if(e != hipSuccess) { return fail(GENNMI_EHIP, std::string("selective_scan_backward: ") + hipGetErrorString(e)); }
