@@ -127,7 +127,6 @@ template<typename T> __device__ inline void storeAt(T *rows, uint32_t t, uint64_
 // sums that nothing waits for until behind it, and spills hundreds of registers.)
 __device__ inline void readAfter(float &a, float &b, float &c, float &d) { asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : : "memory"); }
 
-// (a wavefront with fewer than NP states reads its last one again instead: a select costs less than a branch a state)
 __device__ inline void readAfter(float &a, float &b) { asm volatile("" : "+v"(a), "+v"(b) : : "memory"); }
 // ... COUNT values from the one at `first` on
 template<int COUNT, int N> __device__ inline void readAfter(float (&x)[N], int first = 0)
@@ -136,29 +135,50 @@ template<int COUNT, int N> __device__ inline void readAfter(float (&x)[N], int f
     for(int n = 0; n < COUNT; n += 2) { readAfter(x[first + n], x[first + n + 1]); }
 }
 
+// A lane's states of its channel, which are neighbours in memory: four an access where they lie so (a quarter of the trips through the cache, whose
+// lines hold the states of two lanes or so), else one; a wavefront with fewer than NP reads its last one again instead
+template<int NP> __device__ inline void loadNeighbours(const float *from, uint32_t count, bool fours, float (&x)[NP])
+{
+    if(fours) {
+        #pragma unroll
+        for(int n = 0; n < NP; n += 4) {
+            const Pack<float, 4> p = *(const Pack<float, 4>*)(from + n);
+            #pragma unroll
+            for(int k = 0; k < 4; k++) { x[n + k] = p.v[k]; }
+        }
+    }
+    else {
+        #pragma unroll
+        for(int n = 0; n < NP; n++) { x[n] = from[min((uint32_t)n, count - 1)]; }
+    }
+}
+template<int NP> __device__ inline bool inFours(const ScanArgs &a, const ScanPlace &s, const float *states)
+{
+    return s.numStates == NP && a.states % 4 == 0 && (uint64_t)states % 16 == 0;
+}
 template<int NP> __device__ inline void loadA(const ScanArgs &a, const ScanPlace &s, float (&A)[NP])
 {
-    const float *from = a.A + (uint64_t)s.channel * a.states + s.firstState;
+    loadNeighbours<NP>(a.A + (uint64_t)s.channel * a.states + s.firstState, s.numStates, inFours<NP>(a, s, a.A), A);
     #pragma unroll
-    for(int n = 0; n < NP; n++) { A[n] = from[min((uint32_t)n, s.numStates - 1)] * LOG2E; }
-    #pragma unroll
-    for(int n = 0; n < NP; n++) { A[n] = n < (int)s.numStates ? A[n] : 0.0f; }
+    for(int n = 0; n < NP; n++) { A[n] = n < (int)s.numStates ? A[n] * LOG2E : 0.0f; }
 }
 template<int NP> __device__ inline void loadState(const ScanArgs &a, const ScanPlace &s, const float *state, uint64_t which, float (&h)[NP])
 {
     #pragma unroll
     for(int n = 0; n < NP; n++) { h[n] = 0.0f; }
-    if(!state) { return; }
-    const float *from = state + (which * a.channels + s.channel) * a.states + s.firstState;
-    #pragma unroll
-    for(int n = 0; n < NP; n++) { h[n] = from[min((uint32_t)n, s.numStates - 1)]; }
+    if(state) { loadNeighbours<NP>(state + (which * a.channels + s.channel) * a.states + s.firstState, s.numStates, inFours<NP>(a, s, state), h); }
 }
 template<int NP> __device__ inline void storeState(const ScanArgs &a, const ScanPlace &s, float *state, uint64_t which, const float (&h)[NP])
 {
     if(!state || !s.active) { return; }
-    #pragma unroll
-    for(int n = 0; n < NP; n++) {
-        if(n < (int)s.numStates) { state[(which * a.channels + s.channel) * a.states + s.firstState + n] = h[n]; }
+    float *const to = state + (which * a.channels + s.channel) * a.states + s.firstState;
+    if(inFours<NP>(a, s, state)) {
+        #pragma unroll
+        for(int n = 0; n < NP; n += 4) { *(Pack<float, 4>*)(to + n) = Pack<float, 4>{{h[n], h[n + 1], h[n + 2], h[n + 3]}}; }
+    }
+    else {
+        #pragma unroll
+        for(int n = 0; n < NP; n++) { if(n < (int)s.numStates) { to[n] = h[n]; } }
     }
 }
 template<int NP> __device__ inline void loadChunk(const ScanArgs &a, const ScanPlace &s, const float *chunks, uint32_t number, float (&h)[NP])

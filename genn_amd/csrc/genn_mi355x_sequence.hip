@@ -1,5 +1,6 @@
 // Operators on sequences: a short causal convolution and a selective state space scan, with their gradients, for whole sequences and for
 // single tokens.  Entry points and their checks; the kernels are in the headers included below.
+#include <cmath>
 #include <type_traits>
 
 #include "genn_mi355x_elements.h"
@@ -204,14 +205,26 @@ ScanPlan scanPlan(const gennmi_scan_t &c, bool gradients)
     p.slab = c.states <= 8 ? 8 : 16;
     p.slabs = (c.states + p.slab - 1) / p.slab;
     if(gradients) { p.chunk = SCAN_BLOCK_ROWS * gradientBlocks(p.slabs); }
+    else if(c.sequences.length <= 1) { p.chunk = 1; }
     else {
-        // enough chunks for a few wavefronts on each of the chip's 1024 SIMDs, of 64 rows at least
-        const uint64_t waves = (uint64_t)scanTiles(c) * p.slabs;
-        const uint64_t rows = std::max<uint64_t>(1, totalRows(c.sequences));
-        const uint64_t chunks = std::max<uint64_t>(1, 2048 / waves);
-        p.chunk = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(64, (rows + chunks - 1) / chunks + 7) / 8 * 8, 0x7ffffff8u);
-        // (a split costs every state twice: not worth it for less than twice the wavefronts)
-        if((uint64_t)p.chunk * 2 > c.sequences.length) { p.chunk = std::max(1u, c.sequences.length); }
+        // The chunk (or the whole sequence, which is walked once instead of twice) that the busiest SIMD is through with first.  A row takes a wavefront's SIMD a
+        // certain time however many share it, but a quarter more where one is alone; a chunk takes as long as 4 rows more, and in the walk over the chunks as
+        // long as an eighth of a row.  4096 rows x 2048 channels in chunks of 32, 64, 128: 93, 90, 106 us; 33 sequences of 8011 rows in all x 1002 channels
+        // in chunks of 32, 48, 64, 96: 108, 108, 118, 134 us.
+        constexpr uint64_t SIMDS = 1024;
+        const uint64_t rows = totalRows(c.sequences), wavesEach = (uint64_t)scanTiles(c) * p.slabs, length = std::max(1u, c.sequences.length);
+        const auto shares = [&](double chunks) {
+            // (how packed sequences fall into chunks is the device's to know: half a share for what does not come out even)
+            const double even = chunks * wavesEach / SIMDS, share = c.sequences.offsets ? even + 0.5 : std::ceil(even);
+            return share <= 1.0 ? 1.25 : share;
+        };
+        double best = shares(c.sequences.count) * length * 0.55;
+        p.chunk = (uint32_t)length;
+        for(uint32_t chunk = 32; chunk <= 256 && chunk < length; chunk += 8) {
+            const double chunks = c.sequences.offsets ? (double)rows / chunk + 0.5 * c.sequences.count : (double)c.sequences.count * ((length + chunk - 1) / chunk);
+            const double cost = shares(chunks) * (chunk + 4) + 0.13 * (length / chunk);
+            if(cost < best) { best = cost; p.chunk = chunk; }
+        }
     }
     p.split = c.sequences.length > p.chunk;
     return p;
