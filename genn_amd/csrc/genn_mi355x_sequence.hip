@@ -204,7 +204,11 @@ ScanPlan scanPlan(const gennmi_scan_t &c, bool gradients)
     ScanPlan p;
     p.slab = c.states <= 8 ? 8 : 16;
     p.slabs = (c.states + p.slab - 1) / p.slab;
-    if(gradients) { p.chunk = SCAN_BLOCK_ROWS * gradientBlocks(p.slabs); }
+    if(gradients) {
+        // shorter chunks where the longest would leave SIMDs without a wavefront (3 x 301 rows of 511 channels: 64 us in chunks of 32 rows, of 8 39)
+        p.chunk = SCAN_BLOCK_ROWS * gradientBlocks(p.slabs);
+        while(p.chunk > SCAN_BLOCK_ROWS && totalRows(c.sequences) / p.chunk * scanTiles(c) * p.slabs < 1024) { p.chunk /= 2; }
+    }
     else if(c.sequences.length <= 1) { p.chunk = 1; }
     else {
         // The chunk (or the whole sequence, which is walked once instead of twice) that the busiest SIMD is through with first.  A row takes a wavefront's SIMD a

@@ -120,7 +120,7 @@ def test_workspaces_of_packed_sequences_go_by_their_rows():
     for entry in (lib.gennmi_selective_scan_workspace, lib.gennmi_selective_scan_backward_workspace):
         c = scan(sequences__count=1000, sequences__length=8000, sequences__offsets=AT, sequences__rows=10000)
         assert entry(C.byref(c), C.byref(size)) == 0
-        assert size.value < (10000 // 32 + 1000) * 24 * (16 * 3 + 4) * 4 + 10000 * 2 * 16 * 2 * 4 + 4096
+        assert size.value < (10000 // 8 + 1000) * 24 * (16 * 3 + 4) * 4 + 10000 * 2 * 16 * 2 * 4 + 4096
     c = scan(sequences__length=1)
     assert lib.gennmi_selective_scan_workspace(C.byref(c), C.byref(size)) == 0 and size.value == 0     # (a token needs none)
 
