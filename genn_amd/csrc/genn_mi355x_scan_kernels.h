@@ -453,21 +453,22 @@ void scanKernel(ScanArgs a)
 }
 
 // One row a sequence (a token): the states of a sequence's channel are neighbours in memory, and reading and writing them is all there is to it.
-// LANES lanes have four each; what they give the output is added up between them.  A lane does the same states of EACH sequences, whose A it then
-// reads once, and whose loads are all on their way before the first is needed.
-template<typename T, int LANES, bool QUADS, int EACH>
+// LANES lanes have four each; what they give the output is added up between them.  256 sequences of 4096 channels of 16 states take 31 us (4.6 TB/s), with
+// two or four sequences a lane (which share A) 32 and 38.
+template<typename T, int LANES, bool QUADS>
 __global__ __launch_bounds__(256)
 void scanTokenKernel(ScanArgs a)
 {
-    uint32_t first, channel;
-    divideItem(a.channels * LANES, first, channel);
+    uint32_t sequence, channel;
+    divideItem(a.channels * LANES, sequence, channel);
     const uint32_t part = threadIdx.x % LANES, n0 = part * 4;
     channel /= LANES;
-    first *= EACH;
-    if(first >= a.sequences.count) { return; }
+    if(sequence >= a.sequences.count) { return; }
+    Place p;
+    if(!describe(a.sequences, sequence, p)) { return; }
     const uint32_t bcAt = (channel / a.groupChannels) * a.states + n0;
     const bool here = n0 < a.states;
-    const auto load4 = [&](const auto *from, float (&to)[4], uint32_t k0) {
+    const auto load4 = [&](const auto *from, float (&to)[4]) {
         typedef std::remove_cv_t<std::remove_reference_t<decltype(*from)>> E;
         #pragma unroll
         for(int k = 0; k < 4; k++) { to[k] = 0.0f; }
@@ -480,84 +481,46 @@ void scanTokenKernel(ScanArgs a)
         }
         else {
             #pragma unroll
-            for(int k = 0; k < 4; k++) { if(k0 + k < a.states) { to[k] = widen(from[k]); } }
+            for(int k = 0; k < 4; k++) { if(n0 + k < a.states) { to[k] = widen(from[k]); } }
         }
     };
-    float A[4], h[EACH][4], B[EACH][4], C[EACH][4], u[EACH], dt[EACH], z[EACH];
-    Place p[EACH];
-    bool valid[EACH];
-    // (all slots, then all states and rows: a load that waits for one in between would wait for everything asked for before.  What is padding reads the
-    // first state and its own rows, and writes nothing.)
-    #pragma unroll
-    for(int i = 0; i < EACH; i++) {
-        p[i].sequence = min(first + i, a.sequences.count - 1);
-        p[i].first = 0;
-        p[i].length = a.sequences.length;
-        p[i].state = a.sequences.slots ? a.sequences.slots[p[i].sequence] : (int32_t)p[i].sequence;
-    }
-    #pragma unroll
-    for(int i = 0; i < EACH; i++) {
-        valid[i] = first + i < a.sequences.count && (!a.sequences.slots || (p[i].state >= 0 && (uint32_t)p[i].state < a.sequences.numSlots));
-        p[i].state = valid[i] ? p[i].state : 0;
+    const uint64_t at = ((uint64_t)p.state * a.channels + channel) * a.states + n0;
+    float h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if(a.initialState) { load4(a.initialState + at, h); }
+    if(p.length) {          // (a packed sequence may have none)
+        float A[4], B[4], C[4], y = 0.0f;
+        load4(rowsOf<const T>(a.B, a.sequences, p) + bcAt, B);
+        load4(rowsOf<const T>(a.C, a.sequences, p) + bcAt, C);
+        load4(a.A + (uint64_t)channel * a.states + n0, A);
+        const float u = widen(rowsOf<const T>(a.u, a.sequences, p)[channel]), z = a.z.data ? widen(rowsOf<const T>(a.z, a.sequences, p)[channel]) : 0.0f;
+        float time = widen(rowsOf<const T>(a.delta, a.sequences, p)[channel]) + (a.deltaBias ? a.deltaBias[channel] : 0.0f);
+        if(a.softplus) { time = softplusOf(time); }
+        const float w = time * u;
         #pragma unroll
-        for(int k = 0; k < 4; k++) { h[i][k] = 0.0f; }
-        if(a.initialState) { load4(a.initialState + ((uint64_t)p[i].state * a.channels + channel) * a.states + n0, h[i], n0); }
-    }
-    const auto rows = [&](int i) {
-        load4(rowsOf<const T>(a.B, a.sequences, p[i]) + bcAt, B[i], n0);
-        load4(rowsOf<const T>(a.C, a.sequences, p[i]) + bcAt, C[i], n0);
-        u[i] = widen(rowsOf<const T>(a.u, a.sequences, p[i])[channel]);
-        dt[i] = widen(rowsOf<const T>(a.delta, a.sequences, p[i])[channel]);
-        z[i] = a.z.data ? widen(rowsOf<const T>(a.z, a.sequences, p[i])[channel]) : 0.0f;
-    };
-    if(a.sequences.offsets) {
-        #pragma unroll
-        for(int i = 0; i < EACH; i++) {
-            u[i] = dt[i] = z[i] = 0.0f;
-            describe(a.sequences, p[i].sequence, p[i]);
-            if(!valid[i]) { p[i].length = 0; p[i].state = 0; }
-            if(p[i].length) { rows(i); }        // (a packed sequence may have none)
+        for(int k = 0; k < 4; k++) {
+            if(QUADS || n0 + k < a.states) {
+                h[k] = __builtin_fmaf(exp2Of(time * (A[k] * LOG2E)), h[k], w * B[k]);
+                y = __builtin_fmaf(h[k], C[k], y);
+            }
+        }
+        // (lanes behind the last state have zeros)
+        if constexpr(LANES > 1) { y += gennmi_lanes::partner<1>(y); }
+        if constexpr(LANES > 2) { y += gennmi_lanes::partner<2>(y); }
+        if constexpr(LANES > 4) { y += gennmi_lanes::partner<4>(y); }
+        if constexpr(LANES > 8) { y += gennmi_lanes::partner<8>(y); }
+        if constexpr(LANES > 16) { y += gennmi_lanes::partner<16>(y); }
+        if(part == 0) {
+            if(a.D) { y = __builtin_fmaf(a.D[channel], u, y); }
+            if(a.z.data) { y *= z * logistic(z); }
+            rowsOf<T>(a.out, a.sequences, p)[channel] = narrow<T>(y);
         }
     }
-    else if(a.sequences.length) {
-        #pragma unroll
-        for(int i = 0; i < EACH; i++) { rows(i); }
-    }
-    load4(a.A + (uint64_t)channel * a.states + n0, A, n0);
-    const float bias = a.deltaBias ? a.deltaBias[channel] : 0.0f, skip = a.D ? a.D[channel] : 0.0f;
-    #pragma unroll
-    for(int i = 0; i < EACH; i++) {
-        if(!valid[i]) { continue; }
-        if(p[i].length) {
-            float time = dt[i] + bias, y = 0.0f;
-            if(a.softplus) { time = softplusOf(time); }
-            const float w = time * u[i];
+    if(a.finalState && here) {
+        float *state = a.finalState + at;
+        if(QUADS) { *(Pack<float, 4>*)state = Pack<float, 4>{{h[0], h[1], h[2], h[3]}}; }
+        else {
             #pragma unroll
-            for(int k = 0; k < 4; k++) {
-                if(QUADS || n0 + k < a.states) {
-                    h[i][k] = __builtin_fmaf(exp2Of(time * (A[k] * LOG2E)), h[i][k], w * B[i][k]);
-                    y = __builtin_fmaf(h[i][k], C[i][k], y);
-                }
-            }
-            // (lanes behind the last state have zeros)
-            if constexpr(LANES > 1) { y += gennmi_lanes::partner<1>(y); }
-            if constexpr(LANES > 2) { y += gennmi_lanes::partner<2>(y); }
-            if constexpr(LANES > 4) { y += gennmi_lanes::partner<4>(y); }
-            if constexpr(LANES > 8) { y += gennmi_lanes::partner<8>(y); }
-            if constexpr(LANES > 16) { y += gennmi_lanes::partner<16>(y); }
-            if(part == 0) {
-                y = __builtin_fmaf(skip, u[i], y);
-                if(a.z.data) { y *= z[i] * logistic(z[i]); }
-                rowsOf<T>(a.out, a.sequences, p[i])[channel] = narrow<T>(y);
-            }
-        }
-        if(a.finalState && here) {
-            float *state = a.finalState + ((uint64_t)p[i].state * a.channels + channel) * a.states + n0;
-            if(QUADS) { *(Pack<float, 4>*)state = Pack<float, 4>{{h[i][0], h[i][1], h[i][2], h[i][3]}}; }
-            else {
-                #pragma unroll
-                for(int k = 0; k < 4; k++) { if(n0 + k < a.states) { state[k] = h[i][k]; } }
-            }
+            for(int k = 0; k < 4; k++) { if(n0 + k < a.states) { state[k] = h[k]; } }
         }
     }
 }

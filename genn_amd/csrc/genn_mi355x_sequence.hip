@@ -190,7 +190,6 @@ int checkScan(const char *what, const gennmi_scan_t *c, bool gradients)
     return GENNMI_OK;
 }
 
-constexpr uint64_t TOKEN_THREADS = 256 * 2048;      // of one launch, from which a lane takes several sequences' tokens
 struct ScanPlan { uint32_t slab, slabs, chunk; bool split; };
 constexpr uint32_t SCAN_BLOCK_ROWS = 8;
 // Blocks of rows of a chunk of gradients: what is kept of each takes 4 KiB of LDS a wavefront, and eight wavefronts of one, or of a work-group of
@@ -294,16 +293,8 @@ template<typename T, int LANES> int launchToken(const ScanArgs &a, hipStream_t s
     const auto fours = [](const void *p, uint32_t size) { return (uintptr_t)p % (4 * size) == 0; };
     const auto rows = [&](const gennmi_rows_t &r) { return fours(r.data, sizeof(T)) && r.rowStride % 4 == 0 && r.sequenceStride % 4 == 0; };
     const bool quads = a.states % 4 == 0 && fours(a.A, 4) && fours(a.initialState, 4) && fours(a.finalState, 4) && rows(a.B) && rows(a.C);
-    // several sequences a lane, where that leaves work-groups enough for the chip
-    constexpr uint32_t MANY = 4;
-    const uint64_t threads = (uint64_t)a.sequences.count * a.channels * LANES;
-    const bool many = threads / MANY >= TOKEN_THREADS;
-    const uint64_t groups = many ? (a.sequences.count + MANY - 1) / MANY : a.sequences.count;
-    const dim3 grid((uint32_t)((groups * a.channels * LANES + 255) / 256));
-    if(quads && many) { scanTokenKernel<T, LANES, true, MANY><<<grid, dim3(256), 0, stream>>>(a); }
-    else if(quads) { scanTokenKernel<T, LANES, true, 1><<<grid, dim3(256), 0, stream>>>(a); }
-    else if(many) { scanTokenKernel<T, LANES, false, MANY><<<grid, dim3(256), 0, stream>>>(a); }
-    else { scanTokenKernel<T, LANES, false, 1><<<grid, dim3(256), 0, stream>>>(a); }
+    const dim3 grid((uint32_t)(((uint64_t)a.sequences.count * a.channels * LANES + 255) / 256));
+    if(quads) { scanTokenKernel<T, LANES, true><<<grid, dim3(256), 0, stream>>>(a); } else { scanTokenKernel<T, LANES, false><<<grid, dim3(256), 0, stream>>>(a); }
     return gennmi_detail::afterLaunch("selective_scan");
 }
 template<typename T, int NP, bool SLABS> int launchScanBackward(const ScanArgs &a, const ScanGradientArgs &g, const ScanPlan &p, hipStream_t stream)
