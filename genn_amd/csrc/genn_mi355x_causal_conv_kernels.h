@@ -51,14 +51,24 @@ template<typename T, int VEC> __device__ inline void storeRow(T *to, const float
     for(int v = 0; v < VEC; v++) { p.v[v] = narrow<T>(from[v]); }
     *(Pack<T, VEC>*)to = p;
 }
+// (a thread's weights are neighbours in memory: taken four at a time where they lie so)
 template<int K, int VEC> __device__ inline void loadWeights(const ConvArgs &a, uint32_t channel, float (&w)[K][VEC], float (&bias)[VEC])
 {
-    #pragma unroll
-    for(int v = 0; v < VEC; v++) {
-        bias[v] = a.bias ? a.bias[channel + v] : 0.0f;
+    const float *from = a.weight + (uint64_t)channel * K;
+    if(K * VEC % 4 == 0 && (uintptr_t)a.weight % 16 == 0) {
         #pragma unroll
-        for(int k = 0; k < K; k++) { w[k][v] = a.weight[(uint64_t)(channel + v) * K + k]; }
+        for(int i = 0; i < K * VEC / 4; i++) {
+            const Pack<float, 4> p = *(const Pack<float, 4>*)(from + 4 * i);
+            #pragma unroll
+            for(int j = 0; j < 4; j++) { w[(4 * i + j) % K][(4 * i + j) / K] = p.v[j]; }
+        }
     }
+    else {
+        #pragma unroll
+        for(int i = 0; i < K * VEC; i++) { w[i % K][i / K] = from[i]; }
+    }
+    #pragma unroll
+    for(int v = 0; v < VEC; v++) { bias[v] = a.bias ? a.bias[channel + v] : 0.0f; }
 }
 // The K - 1 rows before row `first` of the sequence, as window[1 ..]
 template<typename T, int K, int VEC>
