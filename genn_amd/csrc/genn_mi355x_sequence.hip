@@ -203,30 +203,30 @@ ScanPlan scanPlan(const gennmi_scan_t &c, bool gradients)
     ScanPlan p;
     p.slab = c.states <= 8 ? 8 : 16;
     p.slabs = (c.states + p.slab - 1) / p.slab;
+    // The chunk (or, of a forward scan, the whole sequence, which is walked once instead of twice) that the busiest SIMD is through with first.  A row takes a
+    // wavefront's SIMD a certain time however many share it, but a quarter more where one is alone; a chunk takes as long as 4 rows more, and in the walk
+    // over the chunks as long as an eighth of a row.  4096 rows x 2048 channels in chunks of 32, 64, 128: 93, 90, 106 us; 33 sequences of 8011 rows in all x
+    // 1002 channels in chunks of 32, 48, 64, 96: 108, 108, 118, 134 us.  Gradients of 3 sequences of 301 rows x 511 channels in chunks of 32 and 8: 64, 39 us,
+    // of one of 7900 rows x 65 channels in chunks of 8 and 32: 213, 125 us.
+    constexpr uint64_t SIMDS = 1024;
+    const uint64_t rows = totalRows(c.sequences), wavesEach = (uint64_t)scanTiles(c) * p.slabs, length = std::max(1u, c.sequences.length);
+    const auto cost = [&](uint32_t chunk) {
+        // (how packed sequences fall into chunks is the device's to know: half a share for what does not come out even)
+        const double chunks = c.sequences.offsets ? (double)rows / chunk + 0.5 * c.sequences.count : (double)c.sequences.count * ((length + chunk - 1) / chunk);
+        const double even = chunks * wavesEach / SIMDS, share = c.sequences.offsets ? even + 0.5 : std::ceil(even);
+        return std::max(1.25, share) * (chunk + 4) + 0.13 * (length / chunk);
+    };
     if(gradients) {
-        // shorter chunks where the longest would leave SIMDs without a wavefront (3 x 301 rows of 511 channels: 64 us in chunks of 32 rows, of 8 39)
-        p.chunk = SCAN_BLOCK_ROWS * gradientBlocks(p.slabs);
-        while(p.chunk > SCAN_BLOCK_ROWS && totalRows(c.sequences) / p.chunk * scanTiles(c) * p.slabs < 1024) { p.chunk /= 2; }
+        p.chunk = SCAN_BLOCK_ROWS;
+        for(uint32_t blocks = 2; blocks <= gradientBlocks(p.slabs); blocks *= 2) {
+            if(cost(SCAN_BLOCK_ROWS * blocks) < cost(p.chunk)) { p.chunk = SCAN_BLOCK_ROWS * blocks; }
+        }
     }
-    else if(c.sequences.length <= 1) { p.chunk = 1; }
     else {
-        // The chunk (or the whole sequence, which is walked once instead of twice) that the busiest SIMD is through with first.  A row takes a wavefront's SIMD a
-        // certain time however many share it, but a quarter more where one is alone; a chunk takes as long as 4 rows more, and in the walk over the chunks as
-        // long as an eighth of a row.  4096 rows x 2048 channels in chunks of 32, 64, 128: 93, 90, 106 us; 33 sequences of 8011 rows in all x 1002 channels
-        // in chunks of 32, 48, 64, 96: 108, 108, 118, 134 us.
-        constexpr uint64_t SIMDS = 1024;
-        const uint64_t rows = totalRows(c.sequences), wavesEach = (uint64_t)scanTiles(c) * p.slabs, length = std::max(1u, c.sequences.length);
-        const auto shares = [&](double chunks) {
-            // (how packed sequences fall into chunks is the device's to know: half a share for what does not come out even)
-            const double even = chunks * wavesEach / SIMDS, share = c.sequences.offsets ? even + 0.5 : std::ceil(even);
-            return share <= 1.0 ? 1.25 : share;
-        };
-        double best = shares(c.sequences.count) * length * 0.55;
         p.chunk = (uint32_t)length;
-        for(uint32_t chunk = 32; chunk <= 256 && chunk < length; chunk += 8) {
-            const double chunks = c.sequences.offsets ? (double)rows / chunk + 0.5 * c.sequences.count : (double)c.sequences.count * ((length + chunk - 1) / chunk);
-            const double cost = shares(chunks) * (chunk + 4) + 0.13 * (length / chunk);
-            if(cost < best) { best = cost; p.chunk = chunk; }
+        double best = std::max(1.25, std::ceil((double)c.sequences.count * wavesEach / SIMDS)) * length * 0.55;
+        for(uint32_t chunk = 32; chunk <= 1024 && chunk < length; chunk += chunk < 256 ? 8 : 64) {
+            if(cost(chunk) < best) { best = cost(chunk); p.chunk = chunk; }
         }
     }
     p.split = c.sequences.length > p.chunk;
