@@ -316,24 +316,31 @@ int gennmi_optimiser_push(gennmi_optimiser *optimiser, const gennmi_parameter_t 
             return fail(GENNMI_EINVAL, "optimiser_push: an array is not aligned to its elements");
         }
         if(!std::isfinite(p.weightDecay)) { return fail(GENNMI_EINVAL, "optimiser_push: weight decay"); }
-        // (two tensors that share weights or states would be updated twice, by work-groups that do not wait for one another)
-        const size_t stateSize = eight ? 1 : 4;
-        auto overlap = [](const void *a, size_t aBytes, const void *b, size_t bBytes) {
-            return (uintptr_t)a < (uintptr_t)b + bBytes && (uintptr_t)b < (uintptr_t)a + aBytes;
+        // (work-groups do not wait for one another: nothing that a step writes may be anything else that it reads or writes)
+        const auto shared = [&](const gennmi_parameter_t &x, const gennmi_parameter_t &y) {
+            struct Range { const void *ptr; size_t bytes; };
+            const auto ranges = [&](const gennmi_parameter_t &q, Range (&r)[7]) {
+                const size_t stateSize = eight ? 1 : 4, scales = eight ? (q.count + GENNMI_ADAMW_BLOCK - 1) / GENNMI_ADAMW_BLOCK * sizeof(float) : 0;
+                const Range all[7] = {{q.weight, q.count * sizeOf(q.weightType)}, {q.m, q.count * stateSize}, {q.v, q.count * stateSize}, {q.copy, q.copy ? q.count * 2 : 0},
+                                      {q.mScale, scales}, {q.vScale, scales}, {q.gradient, q.count * sizeOf(q.gradientType)}};
+                for(int k = 0; k < 7; k++) { r[k] = all[k]; }
+            };
+            Range a[7], b[7];
+            ranges(x, a);
+            ranges(y, b);
+            for(int i = 0; i < 7; i++) {
+                for(int j = 0; j < 7; j++) {
+                    if((i == 6 && j == 6) || (&x == &y && i == j)) { continue; }        // (gradients are only read)
+                    if((uintptr_t)a[i].ptr < (uintptr_t)b[j].ptr + b[j].bytes && (uintptr_t)b[j].ptr < (uintptr_t)a[i].ptr + a[i].bytes) { return true; }
+                }
+            }
+            return false;
         };
-        const struct { const void *ptr; size_t bytes; } mine[] = {{p.weight, p.count * weightSize}, {p.m, p.count * stateSize}, {p.v, p.count * stateSize},
-                                                                  {p.copy, p.copy ? p.count * 2 : 0}};
-        for(size_t i = 0; i < 4; i++) {
-            for(size_t j = 0; j < i; j++) {
-                if(overlap(mine[i].ptr, mine[i].bytes, mine[j].ptr, mine[j].bytes)) { return fail(GENNMI_EINVAL, "optimiser_push: weight, states and copy are arrays of their own"); }
-            }
-        }
+        if(shared(p, p)) { return fail(GENNMI_EINVAL, "optimiser_push: weight, gradient, states, scales and copy are arrays of their own"); }
         for(const gennmi_parameter_t &q : optimiser->parameters) {
-            if(overlap(p.weight, p.count * weightSize, q.weight, q.count * sizeOf(q.weightType)) || overlap(p.m, p.count * stateSize, q.m, q.count * stateSize) ||
-               overlap(p.v, p.count * stateSize, q.v, q.count * stateSize)) {
-                return fail(GENNMI_EINVAL, "optimiser_push: overlaps a tensor that was pushed before");
-            }
+            if(shared(p, q)) { return fail(GENNMI_EINVAL, "optimiser_push: overlaps a tensor that was pushed before"); }
         }
+        const size_t stateSize = eight ? 1 : 4;
         ParameterDev d{p.weight, p.gradient, p.copy, p.m, p.v, p.mScale, p.vScale, p.count, p.weightType, p.gradientType, p.copyType, 0, p.weightDecay};
         d.whole = (uintptr_t)p.weight % (4 * weightSize) == 0 && (uintptr_t)p.gradient % (4 * gradientSize) == 0 && (uintptr_t)p.copy % 8 == 0 &&
                   (uintptr_t)p.m % (4 * stateSize) == 0 && (uintptr_t)p.v % (4 * stateSize) == 0;

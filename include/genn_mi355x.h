@@ -667,7 +667,7 @@ typedef struct gennmi_adamw_t {
     double beta1, beta2, epsilon;
     uint32_t stateBits, pad_;             /* 8 or 32 */
 } gennmi_adamw_t;
-typedef struct gennmi_parameter_t {       /* one tensor; tensors of an optimiser do not overlap */
+typedef struct gennmi_parameter_t {       /* one tensor; its arrays overlap neither each other nor those of another (two may have one gradient) */
     void *weight;                         /* [count] GENNMI_TYPE_F32, _F16 or _BF16 (computed in fp32, rounded once) */
     const void *gradient;                 /* [count] any of these */
     void *copy;                           /* [count] F16 or BF16: the new weights rounded, or NULL */

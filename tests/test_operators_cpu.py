@@ -135,6 +135,7 @@ def parameter(**changes):
     (dict(weight=None), -2, "missing"), (dict(gradient=None), -2, "missing"), (dict(v=None), -2, "missing"), (dict(weight=AT + 2), -2, "aligned"),
     (dict(m=AT + 16385), -2, "aligned"), (dict(weightDecay=float("nan")), -2, "decay"), (dict(count=1 << 41), -2, "number of weights"),
     (dict(m=AT + 4), -2, "arrays of their own"), (dict(v=AT + 16384), -2, "arrays of their own"), (dict(copy=AT + 100, copyType=BF16), -2, "arrays of their own"),
+    (dict(gradient=AT + 200), -2, "arrays of their own"), (dict(gradient=AT + 16384 + 396), -2, "arrays of their own"),
 ])
 def test_optimiser_refuses_tensors(change, code, text):
     lib, o = _abi.load(), C.c_void_p()
@@ -155,7 +156,13 @@ def test_optimiser_refuses_settings_order_and_overlaps():
     assert lib.gennmi_optimiser_push(o, C.byref(parameter(**eight)), C.byref(idx)) == 0 and idx.value == 0
     refused(lib.gennmi_optimiser_push(o, C.byref(parameter(**eight)), None), -2, "pushed before")
     refused(lib.gennmi_optimiser_push(o, C.byref(parameter(weight=AT + 396, m=AT + (1 << 21), v=AT + (1 << 22), **eight)), None), -2, "pushed before")
-    assert lib.gennmi_optimiser_push(o, C.byref(parameter(weight=AT + 400, m=AT + (1 << 21), v=AT + (1 << 22), **eight)), C.byref(idx)) == 0 and idx.value == 1
+    scales = dict(mScale=AT + (1 << 19), vScale=AT + (1 << 20))
+    assert lib.gennmi_optimiser_push(o, C.byref(parameter(weight=AT + 400, m=AT + (1 << 21), v=AT + (1 << 22), **scales)), C.byref(idx)) == 0 and idx.value == 1
+    third = dict(weight=AT + (1 << 23), m=AT + (1 << 24), v=AT + (1 << 25))
+    refused(lib.gennmi_optimiser_push(o, C.byref(parameter(**{**eight, **third})), None), -2, "pushed before")              # (the scales of the first)
+    own = dict(mScale=AT + (1 << 26), vScale=AT + (1 << 27))
+    refused(lib.gennmi_optimiser_push(o, C.byref(parameter(**{**own, **third, "gradient": AT + 4})), None), -2, "pushed before")     # (weights of the first)
+    assert lib.gennmi_optimiser_push(o, C.byref(parameter(**{**own, **third})), C.byref(idx)) == 0 and idx.value == 2       # (the gradient of the first)
     refused(lib.gennmi_optimiser_step(o, C.byref(_abi.AdamWStep(rate=1e-3)), None), -4, "not finalised")
     refused(lib.gennmi_optimiser_step(None, None, None), -2, "null")
     n = C.c_uint64()
