@@ -304,6 +304,54 @@ def test_what_is_not_finite_stays_where_it_belongs():
     assert torch.all(final[0, 0::2] == 1.0) and torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("sequences, length", [(0, 5), (3, 0)])
+def test_nothing_to_do_leaves_states_and_gives_zero_gradients(sequences, length):
+    from genn_amd.sequence import CausalConvolution, SelectiveScan
+    D, N, K = 6, 4, 3
+    rows = lambda w: torch.zeros(sequences, length, w).cuda()
+    first, last, window, moved = torch.rand(sequences, D, N).cuda(), torch.zeros(sequences, D, N).cuda(), torch.rand(sequences, K - 1, D).cuda(), torch.zeros(sequences, K - 1, D).cuda()
+    weight, A, grads = torch.rand(D, K).cuda(), -torch.rand(D, N).cuda(), {}
+    c, s = CausalConvolution(sequences, length, D, K), SelectiveScan(sequences, length, D, N)
+    c.bind(x=rows(D), weight=weight, out=rows(D), initial_state=window, final_state=moved)
+    s.bind(u=rows(D), delta=rows(D), A=A, B=rows(N), C=rows(N), out=rows(D), initial_state=first, final_state=last)
+    c.run()
+    s.run()
+    dlast, dmoved, dfirst, dwindow = torch.rand(sequences, D, N).cuda(), torch.rand(sequences, K - 1, D).cuda(), torch.zeros(sequences, D, N).cuda(), torch.zeros(sequences, K - 1, D).cuda()
+    dA, dw = torch.ones(D, N).cuda(), torch.ones(D, K).cuda()
+    c.bind_gradients(out=rows(D), x=rows(D), weight=dw, final_state=dmoved, initial_state=dwindow)
+    s.bind_gradients(out=rows(D), u=rows(D), A=dA, B=rows(N), final_state=dlast, initial_state=dfirst)
+    c.backward()
+    s.backward()
+    torch.cuda.synchronize()
+    for got, want in ((last, first), (moved, window), (dfirst, dlast), (dwindow, dmoved)):
+        assert torch.equal(got, want)
+    assert torch.all(dA == 0) and torch.all(dw == 0)
+
+
+def test_gradients_of_a_long_convolution():
+    """Enough rows for the longest chunks; a few channels of it against the restatement."""
+    from genn_amd.sequence import CausalConvolution
+    S, n, D, K = 4, 2100, 2048, 4
+    x, dout, dx = (torch.randn(S, n, D, device="cuda").to(torch.bfloat16) for _ in range(3))
+    weight, bias, dw, db = torch.randn(D, K, device="cuda"), torch.randn(D, device="cuda"), torch.empty(D, K, device="cuda"), torch.empty(D, device="cuda")
+    c = CausalConvolution(S, n, D, K, dtype="bfloat16", silu=True)
+    c.bind(x=x, weight=weight, bias=bias)
+    c.bind_gradients(out=dout, x=dx, weight=dw, bias=db)
+    c.backward()
+    torch.cuda.synchronize()
+    some = torch.tensor([0, 1, 777, 2047])
+    take = lambda t: t[..., some.cuda()].cpu()
+    w, b, sums, sizes = weight[some.cuda()].cpu(), bias[some.cuda()].cpu(), [0, 0], [0, 0]
+    for k in range(S):
+        args = (take(x[k]), w, b, True, None, take(dout[k]))
+        want, size = ref.causal_conv(*args), ref.causal_conv(*args, magnitudes=True)
+        close(f"dx of {k}", take(dx[k]), want[0], size[0], 2 * K + 16, torch.bfloat16)
+        for i in (0, 1):
+            sums[i], sizes[i] = sums[i] + want[i + 1], sizes[i] + size[i + 1]
+    close("dweight", dw[some.cuda()], sums[0], sizes[0], K + 64 + 20)        # (sums of 64 rows, then in 64 bits)
+    close("dbias", db[some.cuda()], sums[1], sizes[1], K + 64 + 20)
+
+
 @pytest.mark.parametrize("shift", [0, 1, 3])
 def test_any_alignment_gives_the_same(shift):
     """Rows that begin anywhere take the element-wise accesses: same sums."""
