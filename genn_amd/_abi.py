@@ -96,7 +96,7 @@ class Rows(C.Structure):
 
 class Sequences(C.Structure):
     _fields_ = [("count", C.c_uint32), ("length", C.c_uint32), ("offsets", p_u32), ("rows", C.c_uint64), ("slots", C.c_void_p),
-                ("numSlots", C.c_uint32), ("pad_", C.c_uint32)]
+                ("numSlots", C.c_uint32), ("device", C.c_uint32)]
 
 
 class CausalConv(C.Structure):

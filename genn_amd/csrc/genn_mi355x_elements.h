@@ -18,10 +18,16 @@ void noteDeviceWrite(const void *dev, size_t bytes);
 int flushQueuedSteps();
 bool stepsQueued();
 
-// What every operator does before it launches: steps queued in runners run first.  Under capture they cannot: their launches would
-// join the null stream's order, which a capture forbids.
-inline int beforeLaunch(hipStream_t stream)
+// What every operator does before it launches: it makes sure of the device (0, or 1 + the arrays'), and steps queued in runners run first.
+// Under capture they cannot: their launches would join the null stream's order, which a capture forbids.
+inline int beforeLaunch(hipStream_t stream, uint32_t device)
 {
+    if(device) {
+        int current = -1;
+        const hipError_t e = hipGetDevice(&current);
+        if(e != hipSuccess) { return fail(GENNMI_EHIP, std::string("current device: ") + hipGetErrorString(e)); }
+        if((uint32_t)current != device - 1) { return fail(GENNMI_ESTATE, "the current device is " + std::to_string(current) + ", the arrays are on device " + std::to_string(device - 1)); }
+    }
     if(!stepsQueued()) { return GENNMI_OK; }
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if(stream && hipStreamIsCapturing(stream, &status) == hipSuccess && status != hipStreamCaptureStatusNone) {

@@ -169,85 +169,85 @@ void adamwKernel(StepArgs a)
         load4<STREAM>(p.gradient, p.gradientType, at, there, whole, g);
         #pragma unroll
         for(int i = 0; i < 4; i++) { g[i] *= scale; }
-                if(!EIGHT) {
+        if(!EIGHT) {
             load4<STREAM, float>(p.m, at, there, whole, m);
             load4<STREAM, float>(p.v, at, there, whole, v);
-                    #pragma unroll
-                    for(int i = 0; i < 4; i++) {
-                        m[i] = __builtin_fmaf((float)a.beta1, m[i], (float)(1.0 - a.beta1) * g[i]);
-                        v[i] = __builtin_fmaf((float)a.beta2, v[i], (float)(1.0 - a.beta2) * g[i] * g[i]);
-                    }
-                    store4<STREAM, float>(p.m, at, there, whole, m);
-                    store4<STREAM, float>(p.v, at, there, whole, v);
+            #pragma unroll
+            for(int i = 0; i < 4; i++) {
+                m[i] = __builtin_fmaf((float)a.beta1, m[i], (float)(1.0 - a.beta1) * g[i]);
+                v[i] = __builtin_fmaf((float)a.beta2, v[i], (float)(1.0 - a.beta2) * g[i] * g[i]);
+            }
+            store4<STREAM, float>(p.m, at, there, whole, m);
+            store4<STREAM, float>(p.v, at, there, whole, v);
+        }
+        else {
+            // States in 64 bits (as fast here as 32), so that the scales are those of the formula and not of its rounding errors.  The codes are found in
+            // 32 bits, from values 2^-20 of themselves below and above: where the two differ, a border between codes lies so near that 64 bits have to
+            // say on which side (one wavefront in 60).
+            decode(loadCodes<STREAM>(p.m, at, there, whole), m);
+            decode(loadCodes<STREAM>(p.v, at, there, whole), v);
+            const double unitM = a.beta1 * ((double)p.mScale[block] * (1.0 / 448.0)), unitV = a.beta2 * ((double)p.vScale[block] * (1.0 / (448.0 * 448.0)));
+            double m64[4], v64[4];
+            uint32_t bitsM = 0, bitsV = 0;
+            #pragma unroll
+            for(int i = 0; i < 4; i++) {
+                const double gradient = g[i];
+                m64[i] = __builtin_fma((double)m[i], unitM, (1.0 - a.beta1) * gradient);
+                v64[i] = __builtin_fma((1.0 - a.beta2) * gradient, gradient, (double)(v[i] * v[i]) * unitV);
+                m[i] = (float)m64[i];
+                v[i] = (float)v64[i];
+                bitsM = max(bitsM, __float_as_uint(fabsf(m[i])));
+                bitsV = max(bitsV, __float_as_uint(v[i]));
+            }
+            gennmi_lanes::maxOfLanes(bitsM, bitsV);
+            const float M = __uint_as_float(bitsM), V = __uint_as_float(bitsV);
+            constexpr float BELOW = 448.0f * (1.0f - 0x1p-20f), ABOVE = 448.0f * (1.0f + 0x1p-20f), LEAST = 0x1p-18f / (448.0f * 448.0f);
+            const float inverseM = M > 0.0f ? __builtin_amdgcn_rcpf(M) : M, inverseV = V > 0.0f ? __builtin_amdgcn_rcpf(V) : V;
+            const float belowM = BELOW * inverseM, aboveM = ABOVE * inverseM;
+            float lowM[4], highM[4], lowV[4], highV[4];
+            #pragma unroll
+            for(int i = 0; i < 4; i++) {
+                lowM[i] = m[i] * belowM;
+                highM[i] = m[i] * aboveM;
+                // (a positive v has a code of its own: at least the root of LEAST)
+                const float share = v[i] * inverseV, root = __builtin_amdgcn_sqrtf(v[i] > 0.0f && share < LEAST ? LEAST : share);
+                lowV[i] = root * BELOW;
+                highV[i] = root * ABOVE;
+            }
+            uint32_t codesM = encode(lowM), codesV = encode(lowV);
+            // (nor do quotients of 32 bits do where the largest of a block are so small that inverses or others' are subnormal)
+            const bool near = codesM != encode(highM) || codesV != encode(highV) || (M > 0.0f && M < 1e-25f) || (V > 0.0f && V < 1e-25f);
+            if(__ballot(near)) {
+                #pragma unroll
+                for(int i = 0; i < 4; i++) {
+                    if(M > 0.0f) { lowM[i] = roundToOdd(m64[i] * (448.0 / (double)M)); }
+                    if(V > 0.0f) { lowV[i] = roundToOdd(448.0 * sqrt(v64[i] / (double)V)); }
+                    lowV[i] = v[i] > 0.0f && lowV[i] < 0x1p-9f ? 0x1p-9f : lowV[i];
                 }
-                else {
-                    // States in 64 bits (as fast here as 32), so that the scales are those of the formula and not of its rounding errors.  The codes are found in
-                    // 32 bits, from values 2^-20 of themselves below and above: where the two differ, a border between codes lies so near that 64 bits have to
-                    // say on which side (one wavefront in 60).
-                    decode(loadCodes<STREAM>(p.m, at, there, whole), m);
-                    decode(loadCodes<STREAM>(p.v, at, there, whole), v);
-                    const double unitM = a.beta1 * ((double)p.mScale[block] * (1.0 / 448.0)), unitV = a.beta2 * ((double)p.vScale[block] * (1.0 / (448.0 * 448.0)));
-                    double m64[4], v64[4];
-                    uint32_t bitsM = 0, bitsV = 0;
-                    #pragma unroll
-                    for(int i = 0; i < 4; i++) {
-                        const double gradient = g[i];
-                        m64[i] = __builtin_fma((double)m[i], unitM, (1.0 - a.beta1) * gradient);
-                        v64[i] = __builtin_fma((1.0 - a.beta2) * gradient, gradient, (double)(v[i] * v[i]) * unitV);
-                        m[i] = (float)m64[i];
-                        v[i] = (float)v64[i];
-                        bitsM = max(bitsM, __float_as_uint(fabsf(m[i])));
-                        bitsV = max(bitsV, __float_as_uint(v[i]));
-                    }
-                    gennmi_lanes::maxOfLanes(bitsM, bitsV);
-                    const float M = __uint_as_float(bitsM), V = __uint_as_float(bitsV);
-                    constexpr float BELOW = 448.0f * (1.0f - 0x1p-20f), ABOVE = 448.0f * (1.0f + 0x1p-20f), LEAST = 0x1p-18f / (448.0f * 448.0f);
-                    const float inverseM = M > 0.0f ? __builtin_amdgcn_rcpf(M) : M, inverseV = V > 0.0f ? __builtin_amdgcn_rcpf(V) : V;
-                    const float belowM = BELOW * inverseM, aboveM = ABOVE * inverseM;
-                    float lowM[4], highM[4], lowV[4], highV[4];
-                    #pragma unroll
-                    for(int i = 0; i < 4; i++) {
-                        lowM[i] = m[i] * belowM;
-                        highM[i] = m[i] * aboveM;
-                        // (a positive v has a code of its own: at least the root of LEAST)
-                        const float share = v[i] * inverseV, root = __builtin_amdgcn_sqrtf(v[i] > 0.0f && share < LEAST ? LEAST : share);
-                        lowV[i] = root * BELOW;
-                        highV[i] = root * ABOVE;
-                    }
-                    uint32_t codesM = encode(lowM), codesV = encode(lowV);
-                    // (nor do quotients of 32 bits do where the largest of a block are so small that inverses or others' are subnormal)
-                    const bool near = codesM != encode(highM) || codesV != encode(highV) || M < 1e-25f || V < 1e-25f;
-                    if(__ballot(near)) {
-                        #pragma unroll
-                        for(int i = 0; i < 4; i++) {
-                            if(M > 0.0f) { lowM[i] = roundToOdd(m64[i] * (448.0 / (double)M)); }
-                            if(V > 0.0f) { lowV[i] = roundToOdd(448.0 * sqrt(v64[i] / (double)V)); }
-                            lowV[i] = v[i] > 0.0f && lowV[i] < 0x1p-9f ? 0x1p-9f : lowV[i];
-                        }
-                        codesM = encode(lowM);
-                        codesV = encode(lowV);
-                    }
-                    storeCodes<STREAM>(p.m, at, there, whole, codesM);
-                    storeCodes<STREAM>(p.v, at, there, whole, codesV);
-                    if((threadIdx.x & 63) == 0) { p.mScale[block] = M; p.vScale[block] = V; }
-                }
-                if(a.epsilon >= 1e-12f) {
-                    // (one instruction each for root and inverse: their last bit, and subnormal second moments, do not matter beside epsilon)
-                    #pragma unroll
-                    for(int i = 0; i < 4; i++) {
-                        const float change = m[i] * correct1 * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[i] * correct2) + a.epsilon);
-                        w[i] = __builtin_fmaf(-step, change, w[i] * keep);
-                    }
-                }
-                else {
-                    #pragma unroll
-                    for(int i = 0; i < 4; i++) {
-                        const float change = m[i] * correct1 / (sqrtf(v[i] * correct2) + a.epsilon);
-                        w[i] = __builtin_fmaf(-step, change, w[i] * keep);
-                    }
-                }
-                store4<STREAM>(p.weight, p.weightType, at, there, whole, w);
-                if(p.copy) { store4<STREAM>(p.copy, p.copyType, at, there, whole, w); }
+                codesM = encode(lowM);
+                codesV = encode(lowV);
+            }
+            storeCodes<STREAM>(p.m, at, there, whole, codesM);
+            storeCodes<STREAM>(p.v, at, there, whole, codesV);
+            if((threadIdx.x & 63) == 0) { p.mScale[block] = M; p.vScale[block] = V; }
+        }
+        if(a.epsilon >= 1e-12f) {
+            // (one instruction each for root and inverse: their last bit, and subnormal second moments, do not matter beside epsilon)
+            #pragma unroll
+            for(int i = 0; i < 4; i++) {
+                const float change = m[i] * correct1 * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[i] * correct2) + a.epsilon);
+                w[i] = __builtin_fmaf(-step, change, w[i] * keep);
+            }
+        }
+        else {
+            #pragma unroll
+            for(int i = 0; i < 4; i++) {
+                const float change = m[i] * correct1 / (sqrtf(v[i] * correct2) + a.epsilon);
+                w[i] = __builtin_fmaf(-step, change, w[i] * keep);
+            }
+        }
+        store4<STREAM>(p.weight, p.weightType, at, there, whole, w);
+        if(p.copy) { store4<STREAM>(p.copy, p.copyType, at, there, whole, w); }
     }
     // (every work-group has read what it needs of the counter before it is counted here)
     __syncthreads();
@@ -272,7 +272,7 @@ struct gennmi_optimiser
     std::vector<ParameterDev> table;
     uint64_t bytes = 0;             // that a step reads and writes
     ParameterDev *dParameters = nullptr; ChunkDev *dChunks = nullptr; CounterDev *dCounter = nullptr;
-    uint32_t numChunks = 0;
+    uint32_t numChunks = 0, device = 0;         // device: 1 + the one that was current when the table was uploaded
     bool finalised = false;
     ~gennmi_optimiser() { (void)gennmi_free(dParameters); (void)gennmi_free(dChunks); (void)gennmi_free(dCounter); }
 };
@@ -375,6 +375,9 @@ int gennmi_optimiser_finalise(gennmi_optimiser *optimiser)
         std::vector<CounterDev> counter(1, CounterDev{});
         setCounter(counter[0], optimiser->settings.beta1, optimiser->settings.beta2, 1.0, 1.0, 0);
         if(!optimiser->dCounter) { if(const int rc = upload(&optimiser->dCounter, counter)) { return rc; } }
+        int device = 0;
+        if(const hipError_t e = hipGetDevice(&device)) { return fail(GENNMI_EHIP, std::string("optimiser_finalise: ") + hipGetErrorString(e)); }
+        optimiser->device = 1 + (uint32_t)device;
         optimiser->numChunks = (uint32_t)chunks.size();
         optimiser->finalised = true;
         return (int)GENNMI_OK;
@@ -390,8 +393,8 @@ int gennmi_optimiser_step(gennmi_optimiser *optimiser, const gennmi_adamw_step_t
         for(const void *p : {(const void*)step->rateDevice, (const void*)step->gradientScale, (const void*)step->skip}) {
             if((uintptr_t)p % 4) { return fail(GENNMI_EINVAL, "optimiser_step: a device value is not aligned"); }
         }
-        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
         const gennmi_optimiser &o = *optimiser;
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, o.device)) { return rc; }
         const StepArgs a{o.dParameters, o.dChunks, o.dCounter, o.numChunks, 0, o.settings.beta1, o.settings.beta2, step->rate, (float)o.settings.epsilon,
                          step->rateDevice, step->gradientScale, step->skip};
         const dim3 grid(o.numChunks);

@@ -331,7 +331,8 @@ template<bool BACKWARDS> __device__ inline float walkChunks(float *state, uint64
         for(uint32_t k = 0; k < AHEAD; k++) {
             if(first + k < chunks) {
                 state[chunk(first + k) * stride] = h;
-                h = __builtin_fmaf(exp2Of(times[k] * A), h, adds[k]);
+                // (where A is positive a chunk's decay may be infinite: of nothing, nothing is left all the same)
+                h = h == 0.0f ? adds[k] : __builtin_fmaf(exp2Of(times[k] * A), h, adds[k]);
             }
             adds[k] = nextAdds[k];
             times[k] = nextTimes[k];

@@ -343,7 +343,7 @@ int gennmi_causal_conv(const gennmi_causal_conv_t *conv, void *stream)
 {
     return gennmi_detail::guarded("causal_conv", [&] {
         if(const int rc = checkConv("causal_conv", conv, false)) { return rc; }
-        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, conv->sequences.device)) { return rc; }
         if(const int rc = runConv("causal_conv", *conv, convVector(*conv, nullptr), nullptr, (hipStream_t)stream)) { return rc; }
         const uint32_t size = sizeOf(conv->type);
         noteRows(conv->out, conv->sequences, conv->channels, size);
@@ -379,9 +379,10 @@ int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_c
         if((uintptr_t)g.finalState % size || (uintptr_t)g.initialState % size || (uintptr_t)g.weight % 4 || (uintptr_t)g.bias % 4) {
             return fail(GENNMI_EINVAL, "causal_conv_backward: an array is not aligned to its elements");
         }
+        if(g.initialState && g.initialState == g.finalState) { return fail(GENNMI_EINVAL, "causal_conv_backward: the gradient of initialState is an array of its own"); }
         const bool sums = g.weight || g.bias;
         if(const int rc = checkWorkspace(what, workspace, workspaceBytes, sums ? convWorkspace(*conv) : 0)) { return rc; }
-        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, conv->sequences.device)) { return rc; }
         ConvGradientArgs a{};
         a.out = g.out;
         a.x = g.x;
@@ -421,7 +422,7 @@ int gennmi_selective_scan(const gennmi_scan_t *scan, void *workspace, size_t wor
         if(const int rc = checkWorkspace(what, workspace, workspaceBytes, space.bytes)) { return rc; }
         ScanArgs a;
         if(const int rc = scanArgs(what, *scan, p, a)) { return rc; }
-        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, scan->sequences.device)) { return rc; }
         if(!scan->sequences.count) { return (int)GENNMI_OK; }
         if(p.split) {
             a.chunkState = (float*)((char*)workspace + space.state);
@@ -471,7 +472,9 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
         for(const auto &w : written) {
             if(!w.rows->data) { continue; }
             if(const int rc = checkWrittenRows(what, w.which, *w.rows, scan->sequences, w.width, size)) { return rc; }
-            for(const void *p : {scan->u.data, scan->delta.data, scan->z.data, scan->B.data, scan->C.data, in.out.data}) {
+            const void *others[] = {scan->u.data, scan->delta.data, scan->z.data, scan->B.data, scan->C.data, in.out.data,
+                                    w.rows == &in.u ? nullptr : in.u.data, w.rows == &in.delta ? nullptr : in.delta.data, w.rows == &in.z ? nullptr : in.z.data, w.rows == &in.B ? nullptr : in.B.data};
+            for(const void *p : others) {
                 if(p == w.rows->data) { return fail(GENNMI_EINVAL, std::string(what) + ": " + w.which + " is an array of its own"); }
             }
         }
@@ -486,7 +489,7 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
         if(const int rc = scanArgs(what, *scan, p, a)) { return rc; }
         const uint64_t rows = totalRows(scan->sequences);
         if((rows * 2 * width + 255) / 256 > MOST_BLOCKS) { return fail(GENNMI_EINVAL, "selective_scan_backward: more rows than one launch covers"); }
-        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream)) { return rc; }
+        if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, scan->sequences.device)) { return rc; }
         auto at = [&](size_t offset) { return (float*)((char*)workspace + offset); };
         a.finalState = nullptr;
         ScanGradientArgs g{};

@@ -17,7 +17,7 @@ class AdamW:
         optimiser.step()                                    # one launch for all of them
 
     States are float32, or with ``state_bits=8`` codes in e4m3 with a float32 scale for each block of 256 weights.  The optimiser makes them
-    (zero) unless they are given.  Weights that a model's runner holds copies of reach it before its next step."""
+    (zero) unless they are given.  A step while another device than the optimiser's is current is refused.  Weights that a model's runner holds copies of reach it before its next step."""
 
     def __init__(self, learning_rate=1e-3, beta1=0.9, beta2=0.999, epsilon=1e-8, state_bits=32, device=0):
         self._lib = _abi.load()
@@ -81,11 +81,12 @@ class AdamW:
 
     def step(self, learning_rate=None, gradient_scale=None, skip=None, stream=0):
         """``learning_rate``: a number, or a float32 array of one element on the device that the step reads when it runs.  ``gradient_scale`` (float32) and
-        ``skip`` (int32 or uint32: not 0 leaves everything as it is): such arrays, or None."""
+        ``skip`` (int32 or uint32: not 0 leaves everything as it is): such arrays, or None.  A captured step goes on reading the arrays that it was given."""
         s = self._step
         rate = self.learning_rate if learning_rate is None else learning_rate
         on_device = not isinstance(rate, (int, float))
         s.rate, s.rateDevice = (0.0, self._scalar(rate, "learning_rate", "float32")) if on_device else (rate, None)
+        self._values = (rate, gradient_scale, skip)         # (kept alive until the next step)
         s.gradientScale = None if gradient_scale is None else self._scalar(gradient_scale, "gradient_scale", "float32")
         s.skip = None if skip is None else self._scalar(skip, "skip", ("int32", "uint32"))
         rc = self._lib.gennmi_optimiser_step(self._optimiser, self._reference, stream)

@@ -3,7 +3,7 @@ scan, for whole sequences (with gradients) and for one token of every running se
 
 As a model's arrays are handed to its runner once and stepped many times, an operator's arrays are bound once (checked then) and
 ``run()`` / ``backward()`` are single calls of the library.  Arrays are ``Array`` objects of this package or tensors on the device.
-``stream`` is the address of a HIP stream; 0, the default, is the null stream.
+``stream`` is the address of a HIP stream; 0, the default, is the null stream.  A call while another device than the operator's is current is refused.
 """
 import ctypes as C
 
@@ -51,7 +51,7 @@ class _SequenceOperator:
 
     def _sequences(self, offsets, slots, first, given):
         """The descriptor of the sequences; ``first``: the array whose rows a packed operator counts."""
-        s = _abi.Sequences(count=self.sequences, length=self.length)
+        s = _abi.Sequences(count=self.sequences, length=self.length, device=self.device + 1)
         self._packed = None
         if offsets is not None:
             s.offsets = self._flat(offsets, "offsets", (self.sequences + 1,), ("int32", "uint32"), given)

@@ -599,7 +599,8 @@ typedef struct gennmi_sequences_t {
     const int32_t *slots;                 /* NULL: sequence s has state s; or device [count]: the place of its state among numSlots.  A sequence whose slot is
                                            * outside 0 .. numSlots - 1 is padding: nothing of it is read or written.  Two sequences must not share a state that
                                            * is written.  Not for gradients. */
-    uint32_t numSlots, pad_;
+    uint32_t numSlots;
+    uint32_t device;                      /* 0, or 1 + the device whose memory the arrays are: the call fails with GENNMI_ESTATE while another one is current */
 } gennmi_sequences_t;
 
 /* Short causal convolution, every channel by itself (depthwise):
@@ -618,7 +619,7 @@ typedef struct gennmi_causal_conv_t {
 typedef struct gennmi_causal_conv_gradient_t {      /* `out` and `finalState` come in, the others go out (any may be NULL) and are overwritten */
     gennmi_rows_t out, x;
     const void *finalState;               /* gradient of the final state, or NULL: zero */
-    void *initialState;
+    void *initialState;                   /* (not the array of finalState) */
     float *weight, *bias;
 } gennmi_causal_conv_gradient_t;
 int gennmi_causal_conv(const gennmi_causal_conv_t *conv, void *stream);
@@ -630,7 +631,9 @@ int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_c
  *   dt = delta[t][d] + deltaBias[d], then log(1 + exp(dt)) with `softplus`
  *   h[t][d][n] = exp(dt * A[d][n]) * h[t - 1][d][n] + dt * u[t][d] * B[t][g][n]
  *   out[t][d] = (sum_n C[t][g][n] * h[t][d][n] + D[d] * u[t][d]) * z[t][d] * sigmoid(z[t][d])
- * where channels / groups neighbouring channels share the B and C of group g.  States and sums in fp32.  One row per sequence (a token of every
+ * where channels / groups neighbouring channels share the B and C of group g.  States and sums in fp32.  Long sequences
+ * are cut into chunks of up to 1024 rows (gradients: 32) whose decay is one factor: where dt A > 0 for long, the growth over a chunk has to stay
+ * below 2^128, unless a forward scan's state is zero.  One row per sequence (a token of every
  * running sequence) takes a kernel of its own, without a workspace. */
 #define GENNMI_MAX_SCAN_STATES 128
 typedef struct gennmi_scan_t {
@@ -688,7 +691,8 @@ int gennmi_optimiser_destroy(gennmi_optimiser *optimiser);
 /* As for a runner: tensors are pushed, finalise uploads their table, then steps.  Arrays stay the caller's. */
 int gennmi_optimiser_push(gennmi_optimiser *optimiser, const gennmi_parameter_t *parameter, uint32_t *idx);
 int gennmi_optimiser_finalise(gennmi_optimiser *optimiser);
-/* One launch.  Steps of one optimiser run one behind another: the caller orders them where it uses several streams. */
+/* One launch, on the device that was current in finalise (GENNMI_ESTATE while another one is).  Steps of one optimiser run one behind another: the
+ * caller orders them where it uses several streams. */
 int gennmi_optimiser_step(gennmi_optimiser *optimiser, const gennmi_adamw_step_t *step, void *stream);
 /* Steps counted so far, for a checkpoint beside the states; both wait for the device. */
 int gennmi_optimiser_get_step(gennmi_optimiser *optimiser, uint64_t *step);

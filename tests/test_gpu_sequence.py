@@ -328,6 +328,87 @@ def test_nothing_to_do_leaves_states_and_gives_zero_gradients(sequences, length)
     assert torch.all(dA == 0) and torch.all(dw == 0)
 
 
+def test_another_current_device_is_refused():
+    """(the descriptors say that their arrays are the second device's, while the first is current)"""
+    from genn_amd.sequence import CausalConvolution, SelectiveScan
+    t, A = torch.ones(1, 3, 4).cuda(), -torch.ones(4, 4).cuda()
+    out = torch.zeros(1, 3, 4).cuda()
+    c, s = CausalConvolution(1, 3, 4, 4), SelectiveScan(1, 3, 4, 4)
+    c.bind(x=t, weight=A, out=out)
+    s.bind(u=t, delta=t, A=A, B=t, C=t, out=out)
+    for op in (c, s):
+        op.bind_gradients(out=t)
+        assert op._descriptor.sequences.device == 1
+        op._descriptor.sequences.device = 2
+        for call in (op.run, op.backward):
+            with pytest.raises(_abi.GennmiError, match="on device 1"):
+                call()
+    torch.cuda.synchronize()
+    assert torch.all(out == 0)
+
+
+def test_a_state_of_nothing_stays_nothing_however_fast_units_grow():
+    """Units with A > 0, no input for 500 rows and then some: a chunk's growth is infinite in fp32, a state of zero stays zero."""
+    from genn_amd.sequence import SelectiveScan
+    n, D, N = 520, 64, 16
+    u = torch.zeros(1, n, D)
+    u[:, 500:] = 1.0
+    B, A, delta, out, final = torch.ones(1, n, N).cuda(), torch.ones(D, N).cuda(), torch.full((1, n, D), 3.0).cuda(), torch.empty(1, n, D).cuda(), torch.empty(1, D, N).cuda()
+    delta[:, 500:] = 0.5
+    s = SelectiveScan(1, n, D, N)
+    s.bind(u=u.cuda(), delta=delta, A=A, B=B, C=B, out=out, final_state=final)
+    assert s.workspace_bytes > 0
+    s.run()
+    torch.cuda.synchronize()
+    args = dict(u=u[0], delta=delta[0].cpu(), A=A.cpu(), B=B[0].cpu().view(n, 1, N), C=B[0].cpu().view(n, 1, N))
+    want, last = ref.scan(**args)
+    close("out", out[0], want, want, 2 * 20 + N + 12 + 4 * 10)             # (growth e^0.5 a row, 20 rows: what exponents of up to 10 are off by as well)
+    close("final state", final[0], last, last, 2 * 20 + N + 12 + 4 * 10)
+
+
+def test_rows_behind_the_longest_that_is_allowed_are_left_alone():
+    """Packed sequences of 70 and 3 rows where `length` is 40: the first is cut."""
+    from genn_amd.sequence import CausalConvolution, SelectiveScan
+    r, rows, D, N, K, most = generator(12), 73, 20, 16, 4, 40
+    x, delta, B, C, dout = r(rows, D), r(rows, D).abs(), r(rows, N), r(rows, N), r(rows, D)
+    A, weight = -torch.rand(D, N), r(D, K)
+    offsets = torch.tensor([0, 70, 73], dtype=torch.int32).cuda()
+    mine, left = [slice(0, 40), slice(70, 73)], slice(40, 70)
+    full = lambda w: torch.full((rows, w), 7.0).cuda()
+    out, dx, dB, dC, dw, dA = full(D), full(D), full(N), full(N), torch.empty(D, K).cuda(), torch.empty(D, N).cuda()
+    c, s = CausalConvolution(2, most, D, K), SelectiveScan(2, most, D, N)
+    c.bind(x=x.cuda(), weight=weight.cuda(), out=out, offsets=offsets)
+    c.bind_gradients(out=dout.cuda(), x=dx, weight=dw)
+    c.run()
+    c.backward()
+    torch.cuda.synchronize()
+    want = [ref.causal_conv(x[p], weight, None, False)[0] for p in mine]
+    size = [ref.causal_conv(x[p], weight, None, False, magnitudes=True)[0] for p in mine]
+    grads, sizes = ([ref.causal_conv(x[p], weight, None, False, dout=dout[p], magnitudes=m) for p in mine] for m in (False, True))
+    for k, p in enumerate(mine):
+        close("conv", out[p], want[k], size[k], K + 8)
+        close("dx", dx[p], grads[k][0], sizes[k][0], K + 8)
+    close("dweight", dw, grads[0][1] + grads[1][1], sizes[0][1] + sizes[1][1], K + 64 + 20)
+    assert torch.all(out[left] == 7.0) and torch.all(dx[left] == 7.0)
+    out.fill_(7.0)
+    dx.fill_(7.0)
+    s.bind(u=x.cuda(), delta=delta.cuda(), A=A.cuda(), B=B.cuda(), C=C.cuda(), out=out, offsets=offsets)
+    s.bind_gradients(out=dout.cuda(), u=dx, A=dA, B=dB, C=dC)
+    s.run()
+    s.backward()
+    torch.cuda.synchronize()
+    of = lambda p: dict(u=x[p], delta=delta[p], A=A, B=B[p].view(-1, 1, N), C=C[p].view(-1, 1, N))
+    grads, sizes = ([ref.scan(**of(p), dout=dout[p], magnitudes=m) for p in mine] for m in (False, True))
+    for k, p in enumerate(mine):
+        close("scan", out[p], ref.scan(**of(p))[0], ref.scan(**of(p), magnitudes=True)[0], 2 * most + N + 12)
+        close("du", dx[p], grads[k]["u"], sizes[k]["u"], 4 * most + N + 40)
+        for name, got in (("B", dB), ("C", dC)):
+            close(f"d{name}", got[p], grads[k][name].view(-1, N), sizes[k][name].view(-1, N), 4 * most + N + 47)
+    close("dA", dA, grads[0]["A"] + grads[1]["A"], sizes[0]["A"] + sizes[1]["A"], 4 * most + N + 80)
+    for t in (out, dx, dB, dC):
+        assert torch.all(t[left] == 7.0)
+
+
 def test_gradients_of_a_long_convolution():
     """Enough rows for the longest chunks; a few channels of it against the restatement."""
     from genn_amd.sequence import CausalConvolution

@@ -97,6 +97,12 @@ def test_calls_without_arguments_and_workspaces_are_refused():
     refused(lib.gennmi_causal_conv_backward(C.byref(conv(sequences__slots=AT, sequences__numSlots=4)), C.byref(g), AT, size.value, None), -2, "slots")
     g.x = _abi.Rows(AT, 24, 120)
     refused(lib.gennmi_causal_conv_backward(C.byref(conv()), C.byref(g), AT, size.value, None), -2, "array of its own")
+    g = _abi.CausalConvGradient(out=_abi.Rows(AT + 8192, 24, 120), initialState=AT, finalState=AT)
+    refused(lib.gennmi_causal_conv_backward(C.byref(conv()), C.byref(g), AT, size.value, None), -2, "array of its own")
+    g = _abi.ScanGradient(out=_abi.Rows(AT + 4096 * 7, 24, 120), u=_abi.Rows(AT + 4096 * 8, 24, 120), delta=_abi.Rows(AT + 4096 * 8, 24, 120))
+    refused(lib.gennmi_selective_scan_backward(C.byref(scan()), C.byref(g), AT, 1 << 60, None), -2, "array of its own")
+    g = _abi.ScanGradient(out=_abi.Rows(AT + 4096 * 7, 24, 120), B=_abi.Rows(AT + 4096 * 8, 32, 160), C=_abi.Rows(AT + 4096 * 8, 32, 160))
+    refused(lib.gennmi_selective_scan_backward(C.byref(scan()), C.byref(g), AT, 1 << 60, None), -2, "array of its own")
     g = _abi.ScanGradient(out=_abi.Rows(AT + 4096 * 7, 24, 120), u=_abi.Rows(AT + 4096 * 8, 24, 120))
     assert lib.gennmi_selective_scan_backward_workspace(C.byref(scan()), C.byref(size)) == 0 and size.value > 0
     refused(lib.gennmi_selective_scan_backward(C.byref(scan()), C.byref(g), AT, size.value - 1, None), -2, "workspace")
