@@ -10,6 +10,12 @@
 // over the states meet in LDS.  Where channels and sequences are too few to fill the chip, sequences are cut into chunks: one kernel
 // finds what each chunk adds to a state that comes in as zero (and the sum of dt, which says what becomes of one that does not), a second
 // walks over the chunks, and the third does the work from the right state.
+//
+// Bound by vector instructions, not by memory: a state takes a row a product and an exponential (two slots of a SIMD's issue) for its decay, a product and a sum
+// for what comes in, a sum for y, 6 slots, of which the first kernel of a split scan needs 5 as well.  At 39.3 T lane-slots a second 4096 rows x 2048 channels x 16
+// states are 38 us of these alone, their 68 MB 14 us.  They take 81 us in bf16: 37 the first kernel, 8 the second, 46 the third, with the vector
+// units busy for three quarters of the time (softplus, gate and conversions are a fifth of their instructions).  What there is to gain by matrix instructions is
+// nothing: every state of every channel has decays of its own.
 #ifndef GENN_MI355X_SCAN_KERNELS_H
 #define GENN_MI355X_SCAN_KERNELS_H
 
@@ -532,6 +538,10 @@ void scanTokenKernel(ScanArgs a)
 //   dh = C gy + (what comes from the row behind);  dC = gy h, dB = dh dt u (summed over channels);  q = sum dh B, x = dh exp(dt A) h', r = sum x A
 //   du = dt q + D gy;  d(dt) = u q + r;  dA += x dt;  and exp(dt A) dh for the row before
 // A block's walks take PART of the states at a time, so that R * PART of them, and as many decays, fit the registers of two wavefronts a SIMD.
+//
+// Bound by vector instructions: 444 a row and wavefront of 16 states, a fifth of them the sums over channels, and units busy for 74 % of the time (251 registers, so two
+// wavefronts a SIMD; 18 KiB of LDS each).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 690 us, the first 209, the second 56 (memory, 4.8 TB/s), sums
+// over tiles 23 and over chunks 17.  PART 4 spills (813 us), so do three wavefronts a SIMD (1240), without the ties of readAfter it was 9.4 ms.
 template<typename T, int NP, int R, int BLOCKS, bool SLABS>
 __global__ __launch_bounds__(SLABS ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
