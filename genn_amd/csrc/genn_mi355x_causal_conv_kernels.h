@@ -90,21 +90,22 @@ template<typename T, int K, int VEC>
 __device__ inline void storeState(const ConvArgs &a, const T *x, const Place &p, uint32_t channel, const float (&window)[K][VEC])
 {
     T *to = (T*)a.finalState + (uint64_t)p.state * (K - 1) * a.channels + channel;
+    float rows[K][VEC];         // (all read before the first is written: one trip to memory)
     #pragma unroll
     for(int j = 1; j < K; j++) {
         const long long t = (long long)p.length - (K - j);
-        float row[VEC];
-        if(t >= 0) { loadRow<T, VEC>(x + (uint64_t)t * a.x.rowStride + channel, row); }
+        if(t >= 0) { loadRow<T, VEC>(x + (uint64_t)t * a.x.rowStride + channel, rows[j]); }
         else {
             // row t lies -t rows before the first: window[K + t]
             #pragma unroll
             for(int i = 1; i < K; i++) {
                 #pragma unroll
-                for(int v = 0; v < VEC; v++) { row[v] = i == 1 || i == K + t ? window[i][v] : row[v]; }
+                for(int v = 0; v < VEC; v++) { rows[j][v] = i == 1 || i == K + t ? window[i][v] : rows[j][v]; }
             }
         }
-        storeRow<T, VEC>(to + (uint64_t)(j - 1) * a.channels, row);
     }
+    #pragma unroll
+    for(int j = 1; j < K; j++) { storeRow<T, VEC>(to + (uint64_t)(j - 1) * a.channels, rows[j]); }
 }
 
 template<int K, int VEC>
@@ -164,8 +165,8 @@ void causalConvKernel(ConvArgs a)
     RowsAhead<T, VEC> next;
     if(first < last) { next.fetch(x + channel, a.x.rowStride, first, last - 1); }
     loadWindow<T, K, VEC>(a, x, p, first, channel, window);
-    if(K > 1 && p.index == 0 && a.finalState) { storeState<T, K, VEC>(a, x, p, channel, window); }
     loadWeights<K, VEC>(a, channel, w, bias);
+    if(K > 1 && p.index == 0 && a.finalState) { storeState<T, K, VEC>(a, x, p, channel, window); }
     for(uint32_t t = first; t < last; t += AHEAD) {
         const RowsAhead<T, VEC> rows = next;
         if(t + AHEAD < last) { next.fetch(x + channel, a.x.rowStride, t + AHEAD, last - 1); }
