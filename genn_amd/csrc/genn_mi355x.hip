@@ -232,6 +232,7 @@ namespace gennmi_detail
 // error reporting and write tracking for the library's other translation units
 int fail(int code, const std::string &msg) { return ::fail(code, msg); }
 void noteDeviceWrite(const void *dev, size_t bytes) { ::noteDeviceWrite(dev, bytes); }
+bool anyRunners() { std::lock_guard<std::mutex> lock(g_runnersMutex); return !g_runners.empty(); }
 int flushQueuedSteps() { return ::flushQueuedSteps(); }
 bool stepsQueued();                     // whether that would have anything to do (defined behind the programs)
 int prepareStaticScratch();             // looks up the current device's copy of the static counter array (defined with it)

@@ -15,6 +15,7 @@ namespace gennmi_detail
 // (defined beside the runner)
 int fail(int code, const std::string &msg);
 void noteDeviceWrite(const void *dev, size_t bytes);
+bool anyRunners();          // that would have to be told
 int flushQueuedSteps();
 bool stepsQueued();
 
@@ -156,26 +157,24 @@ __device__ inline void divideItem(uint32_t by, uint32_t &quotient, uint32_t &res
     }
 }
 
-// host side
+// host side (a call of a few microseconds: texts are put together for a refusal only)
 inline int checkSequences(const char *what, const gennmi_sequences_t &s, bool gradients)
 {
-    using gennmi_detail::fail;
-    const std::string name(what);
-    if(s.slots && gradients) { return fail(GENNMI_EINVAL, name + ": slots are not for gradients"); }
-    if(s.count > (1u << 24) || s.length > 0x7fffffffu || (s.offsets ? s.rows : (uint64_t)s.count * s.length) > 0x7fffffffull) { return fail(GENNMI_EINVAL, name + ": more sequences or rows than the kernels number"); }
-    if(s.slots && s.numSlots == 0) { return fail(GENNMI_EINVAL, name + ": slots, but no states (numSlots is 0)"); }
-    if((uintptr_t)s.offsets % 4 || (uintptr_t)s.slots % 4) { return fail(GENNMI_EINVAL, name + ": offsets or slots not aligned"); }
+    const auto refuse = [&](const char *why) { return gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + why); };
+    if(s.slots && gradients) { return refuse(": slots are not for gradients"); }
+    if(s.count > (1u << 24) || s.length > 0x7fffffffu || (s.offsets ? s.rows : (uint64_t)s.count * s.length) > 0x7fffffffull) { return refuse(": more sequences or rows than the kernels number"); }
+    if(s.slots && s.numSlots == 0) { return refuse(": slots, but no states (numSlots is 0)"); }
+    if((uintptr_t)s.offsets % 4 || (uintptr_t)s.slots % 4) { return refuse(": offsets or slots not aligned"); }
     return GENNMI_OK;
 }
 inline int checkRows(const char *what, const char *which, const gennmi_rows_t &r, const gennmi_sequences_t &s, uint32_t width, uint32_t size)
 {
-    using gennmi_detail::fail;
-    const std::string name = std::string(what) + ": " + which;
+    const auto refuse = [&](const char *why) { return gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": " + which + why); };
     if(!(s.offsets ? s.rows : (uint64_t)s.count * s.length)) { return GENNMI_OK; }       // (nothing of it is touched)
-    if(!r.data) { return fail(GENNMI_EINVAL, name + " is missing"); }
-    if((uintptr_t)r.data % size) { return fail(GENNMI_EINVAL, name + " is not aligned to its elements"); }
-    if(s.length > 1 && r.rowStride < width) { return fail(GENNMI_EINVAL, name + ": rows overlap (rowStride)"); }
-    if(r.rowStride > (1ull << 40) || r.sequenceStride > (1ull << 50)) { return fail(GENNMI_EINVAL, name + ": stride out of range"); }
+    if(!r.data) { return refuse(" is missing"); }
+    if((uintptr_t)r.data % size) { return refuse(" is not aligned to its elements"); }
+    if(s.length > 1 && r.rowStride < width) { return refuse(": rows overlap (rowStride)"); }
+    if(r.rowStride > (1ull << 40) || r.sequenceStride > (1ull << 50)) { return refuse(": stride out of range"); }
     return GENNMI_OK;
 }
 // What is written: one row of a sequence and another must not share elements either

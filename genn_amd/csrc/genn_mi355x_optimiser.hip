@@ -158,6 +158,8 @@ void adamwKernel(StepArgs a)
     if(a.skip && *a.skip) { return; }
     const ChunkDev chunk = a.chunks[blockIdx.x];
     const ParameterDev p = a.parameters[chunk.parameter];
+    const double before1 = a.counter->power1, before2 = a.counter->power2;
+    const unsigned long long stepsBefore = a.counter->step;
     const uint64_t block = (uint64_t)chunk.index * (CHUNK / 256) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = block * 256 + (threadIdx.x & 63) * 4;
     if(block * 256 < p.count) {
         const double rate = a.rateDevice ? (double)*a.rateDevice : a.rate;
@@ -250,8 +252,8 @@ void adamwKernel(StepArgs a)
         store4<STREAM>(p.weight, p.weightType, at, there, whole, w);
         if(p.copy) { store4<STREAM>(p.copy, p.copyType, at, there, whole, w); }
     }
-    // (every work-group has read what it needs of the counter before it is counted here)
-    __syncthreads();
+    // (every wavefront has read what it needs of the counter before its work-group is counted; what it wrote need not have arrived)
+    __builtin_amdgcn_s_barrier();
     if(threadIdx.x) { return; }
     if(gridDim.x > GROUPS) {
         uint32_t *const place = a.counter->ended + (1 + blockIdx.x % GROUPS) * LINE;
@@ -260,7 +262,7 @@ void adamwKernel(StepArgs a)
     }
     if(atomicAdd(a.counter->ended, 1u) == min(gridDim.x, GROUPS) - 1) {
         a.counter->ended[0] = 0;
-        setCounter(*a.counter, a.beta1, a.beta2, a.counter->power1, a.counter->power2, a.counter->step + 1);
+        setCounter(*a.counter, a.beta1, a.beta2, before1, before2, stepsBefore + 1);
     }
 }
 
@@ -405,6 +407,7 @@ int gennmi_optimiser_step(gennmi_optimiser *optimiser, const gennmi_adamw_step_t
         else if(streaming) { adamwKernel<false, true><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
         else { adamwKernel<false, false><<<grid, dim3(256), 0, (hipStream_t)stream>>>(a); }
         if(const int rc = gennmi_detail::afterLaunch("optimiser_step")) { return rc; }
+        if(!gennmi_detail::anyRunners()) { return (int)GENNMI_OK; }         // (dozens of tensors: asked once)
         for(const gennmi_parameter_t &p : o.parameters) {
             if(p.count) { gennmi_detail::noteDeviceWrite(p.weight, p.count * sizeOf(p.weightType)); }
         }

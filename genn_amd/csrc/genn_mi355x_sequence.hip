@@ -76,19 +76,19 @@ constexpr uint32_t CONV_ROWS = 16, CONV_GRADIENT_ROWS = 64, CONV_GRADIENT_THREAD
 int checkConv(const char *what, const gennmi_causal_conv_t *c, bool gradients)
 {
     if(!c) { return fail(GENNMI_EINVAL, std::string(what) + ": null descriptor"); }
-    const std::string name(what);
+    const auto refuse = [&](int code, const char *why) { return fail(code, std::string(what) + why); };
     const uint32_t size = sizeOf(c->type);
-    if(!size) { return fail(GENNMI_EUNSUPPORTED, name + ": unknown element type"); }
-    if(c->taps < 1 || c->taps > GENNMI_MAX_TAPS) { return fail(GENNMI_EUNSUPPORTED, name + ": number of taps"); }
-    if(c->channels < 1 || c->channels > (1u << 24)) { return fail(GENNMI_EINVAL, name + ": number of channels"); }
+    if(!size) { return refuse(GENNMI_EUNSUPPORTED, ": unknown element type"); }
+    if(c->taps < 1 || c->taps > GENNMI_MAX_TAPS) { return refuse(GENNMI_EUNSUPPORTED, ": number of taps"); }
+    if(c->channels < 1 || c->channels > (1u << 24)) { return refuse(GENNMI_EINVAL, ": number of channels"); }
     if(const int rc = checkSequences(what, c->sequences, gradients)) { return rc; }
     if(const int rc = checkRows(what, "x", c->x, c->sequences, c->channels, size)) { return rc; }
     if(!gradients) {
         if(const int rc = checkWrittenRows(what, "out", c->out, c->sequences, c->channels, size)) { return rc; }
-        if(c->out.data && c->out.data == c->x.data) { return fail(GENNMI_EINVAL, name + ": out and x are the same array"); }
+        if(c->out.data && c->out.data == c->x.data) { return refuse(GENNMI_EINVAL, ": out and x are the same array"); }
     }
-    if(!c->weight || (uintptr_t)c->weight % 4 || (uintptr_t)c->bias % 4) { return fail(GENNMI_EINVAL, name + ": weight is missing, or weight or bias not aligned"); }
-    if((uintptr_t)c->initialState % size || (uintptr_t)c->finalState % size) { return fail(GENNMI_EINVAL, name + ": a state is not aligned to its elements"); }
+    if(!c->weight || (uintptr_t)c->weight % 4 || (uintptr_t)c->bias % 4) { return refuse(GENNMI_EINVAL, ": weight is missing, or weight or bias not aligned"); }
+    if((uintptr_t)c->initialState % size || (uintptr_t)c->finalState % size) { return refuse(GENNMI_EINVAL, ": a state is not aligned to its elements"); }
     return GENNMI_OK;
 }
 // Channels of a thread: four, for gradients two, where every row and state of them is one aligned access, else one.  (Gradients keep four rows of
@@ -166,11 +166,11 @@ size_t convWorkspace(const gennmi_causal_conv_t &c) { return (size_t)chunkNumber
 int checkScan(const char *what, const gennmi_scan_t *c, bool gradients)
 {
     if(!c) { return fail(GENNMI_EINVAL, std::string(what) + ": null descriptor"); }
-    const std::string name(what);
+    const auto refuse = [&](int code, const char *why) { return fail(code, std::string(what) + why); };
     const uint32_t size = sizeOf(c->type);
-    if(!size) { return fail(GENNMI_EUNSUPPORTED, name + ": unknown element type"); }
-    if(c->states < 1 || c->states > GENNMI_MAX_SCAN_STATES) { return fail(GENNMI_EUNSUPPORTED, name + ": number of states"); }
-    if(c->channels < 1 || c->channels > (1u << 24) || c->groups < 1 || c->channels % c->groups) { return fail(GENNMI_EINVAL, name + ": number of channels or groups"); }
+    if(!size) { return refuse(GENNMI_EUNSUPPORTED, ": unknown element type"); }
+    if(c->states < 1 || c->states > GENNMI_MAX_SCAN_STATES) { return refuse(GENNMI_EUNSUPPORTED, ": number of states"); }
+    if(c->channels < 1 || c->channels > (1u << 24) || c->groups < 1 || c->channels % c->groups) { return refuse(GENNMI_EINVAL, ": number of channels or groups"); }
     if(const int rc = checkSequences(what, c->sequences, gradients)) { return rc; }
     if(const int rc = checkRows(what, "u", c->u, c->sequences, c->channels, size)) { return rc; }
     if(const int rc = checkRows(what, "delta", c->delta, c->sequences, c->channels, size)) { return rc; }
@@ -180,12 +180,12 @@ int checkScan(const char *what, const gennmi_scan_t *c, bool gradients)
     if(!gradients) {
         if(const int rc = checkWrittenRows(what, "out", c->out, c->sequences, c->channels, size)) { return rc; }
         for(const void *p : {c->u.data, c->delta.data, c->z.data, c->B.data, c->C.data}) {
-            if(p && p == c->out.data) { return fail(GENNMI_EINVAL, name + ": out is an array of its own"); }
+            if(p && p == c->out.data) { return refuse(GENNMI_EINVAL, ": out is an array of its own"); }
         }
     }
-    if(!c->A) { return fail(GENNMI_EINVAL, name + ": A is missing"); }
+    if(!c->A) { return refuse(GENNMI_EINVAL, ": A is missing"); }
     for(const void *p : {(const void*)c->A, (const void*)c->D, (const void*)c->deltaBias, (const void*)c->initialState, (const void*)c->finalState}) {
-        if((uintptr_t)p % 4) { return fail(GENNMI_EINVAL, name + ": an array of fp32 is not aligned"); }
+        if((uintptr_t)p % 4) { return refuse(GENNMI_EINVAL, ": an array of fp32 is not aligned"); }
     }
     return GENNMI_OK;
 }

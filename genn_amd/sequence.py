@@ -142,7 +142,8 @@ class CausalConvolution(_SequenceOperator):
         self._bound, self._descriptor, self._reference, self._gradients = given, c, C.byref(c), None
 
     def run(self, stream=0):
-        self._need(self._bound, "bind()")
+        if self._bound is None:
+            raise RuntimeError("bind() must be called first")
         rc = self._lib.gennmi_causal_conv(self._reference, stream)
         if rc:
             _abi.check(rc)
@@ -212,7 +213,8 @@ class SelectiveScan(_SequenceOperator):
 
     def run(self, stream=0, workspace=None):
         """``workspace``: ``workspace_bytes`` on the device, for a call that is captured into a graph (which keeps using it)."""
-        self._need(self._bound, "bind()")
+        if self._bound is None:
+            raise RuntimeError("bind() must be called first")
         address, size = self._workspace("forward", workspace, self.workspace_bytes, stream) if self.workspace_bytes else (None, 0)
         rc = self._lib.gennmi_selective_scan(self._reference, address, size, stream)
         if rc:
