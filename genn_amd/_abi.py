@@ -232,6 +232,7 @@ SYMBOLS = {
     "gennmi_runner_get_info": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32 * 4)]),
     "gennmi_runner_event_count": (C.c_int, [C.c_void_p, C.POINTER(_ULL)]),
     "gennmi_stream_is_capturing": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
+    "gennmi_current_device": (C.c_int, [C.POINTER(C.c_int)]),
     "gennmi_causal_conv": (C.c_int, [C.POINTER(CausalConv), C.c_void_p]),
     "gennmi_causal_conv_backward_workspace": (C.c_int, [C.POINTER(CausalConv), C.POINTER(C.c_size_t)]),
     "gennmi_causal_conv_backward": (C.c_int, [C.POINTER(CausalConv), C.POINTER(CausalConvGradient), C.c_void_p, C.c_size_t, C.c_void_p]),

@@ -339,6 +339,13 @@ int gennmi_stream_is_capturing(void *stream, int *capturing)
     return GENNMI_OK;
 }
 
+int gennmi_current_device(int *device)
+{
+    if(!device) { return fail(GENNMI_EINVAL, "current_device: null result pointer"); }
+    const hipError_t e = hipGetDevice(device);
+    return e == hipSuccess ? (int)GENNMI_OK : fail(GENNMI_EHIP, std::string("current_device: ") + hipGetErrorString(e));
+}
+
 int gennmi_causal_conv(const gennmi_causal_conv_t *conv, void *stream)
 {
     return gennmi_detail::guarded("causal_conv", [&] {

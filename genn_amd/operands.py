@@ -1,9 +1,9 @@
 """Device arrays as the operators take them: an ``Array`` of this package, or a tensor that says where it lies, what it holds and how
 (``data_ptr()``, ``dtype``, ``shape``, ``stride()``: torch's do).  Nothing is copied or cast."""
+import ctypes as C
+
 from . import _abi
 from .genn_model import Array
-
-ITEM_SIZES = {"float32": 4, "float16": 2, "bfloat16": 2, "float8_e4m3fn": 1, "uint8": 1, "int32": 4, "uint32": 4}
 
 
 class Operand:
@@ -71,6 +71,14 @@ class Operand:
         if min(strides) < 0:
             raise ValueError(f"{self.name}: negative stride")
         return _abi.Rows(self.address, row, sequence)
+
+
+def current_device(lib, device):
+    """What is allocated lies on the device that is current: it has to be the operator's."""
+    now = C.c_int()
+    _abi.check(lib.gennmi_current_device(C.byref(now)))
+    if now.value != device:
+        raise ValueError(f"the current device is {now.value}, the operator's is {device}")
 
 
 def same_device(operands, device):

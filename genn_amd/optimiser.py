@@ -1,9 +1,10 @@
 """AdamW over many tensors in one launch, over the C ABI in include/genn_mi355x.h."""
 import ctypes as C
+from numbers import Real
 
 from . import _abi
 from .genn_model import Array
-from .operands import Operand, same_device
+from .operands import Operand, current_device, same_device
 
 BLOCK = 256         # weights that share a scale of the states in 8 bits
 
@@ -51,6 +52,7 @@ class AdamW:
         """One tensor.  ``copy``: float16 or bfloat16, receives the new weights rounded (the ones a forward pass reads)."""
         if not self._optimiser:
             raise RuntimeError("the optimiser has been freed")
+        current_device(self._lib, self.device)
         count = 1
         for n in Operand(weights, "weights").shape:
             count *= n
@@ -76,6 +78,7 @@ class AdamW:
         return index.value
 
     def build(self):
+        current_device(self._lib, self.device)
         _abi.check(self._lib.gennmi_optimiser_finalise(self._optimiser))
         self._built = True
 
@@ -84,7 +87,7 @@ class AdamW:
         ``skip`` (int32 or uint32: not 0 leaves everything as it is): such arrays, or None.  A captured step goes on reading the arrays that it was given."""
         s = self._step
         rate = self.learning_rate if learning_rate is None else learning_rate
-        on_device = not isinstance(rate, (int, float))
+        on_device = not isinstance(rate, (int, float)) and not isinstance(rate, Real)       # (numpy's numbers are the second)
         s.rate, s.rateDevice = (0.0, self._scalar(rate, "learning_rate", "float32")) if on_device else (rate, None)
         self._values = (rate, gradient_scale, skip)         # (kept alive until the next step)
         s.gradientScale = None if gradient_scale is None else self._scalar(gradient_scale, "gradient_scale", "float32")

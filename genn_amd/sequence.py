@@ -9,20 +9,23 @@ import ctypes as C
 
 from . import _abi
 from .genn_model import Array
-from .operands import Operand, same_device
+from .operands import Operand, current_device, same_device
+
+
+def _count(n, name):
+    """As the descriptors' 32 bits take it."""
+    if not 0 <= n < 1 << 31:
+        raise ValueError(f"{name} is a count below 2^31, not {n}")
+    return int(n)
 
 
 class _SequenceOperator:
-    _names = ()
-
-    def __init__(self, sequences, length, dtype, rows, device):
+    def __init__(self, sequences, length, dtype, device):
         if dtype not in _abi.FLOAT_TYPES:
             raise NotImplementedError(f"element type {dtype}")
-        if sequences < 0 or length < 0:
-            raise ValueError("sequences and length are counts")
+        self.sequences, self.length, self.dtype, self.device = _count(sequences, "sequences"), _count(length, "length"), dtype, device
         self._lib = _abi.load()
         _abi.check(self._lib.gennmi_init(device))
-        self.sequences, self.length, self.dtype, self.device = int(sequences), int(length), dtype, device
         self._bound = self._gradients = None        # operands (kept alive) of the descriptors
         self._packed = None
         self._workspaces = {}           # (stream, which pass): one each, as calls on different streams may overlap
@@ -89,6 +92,7 @@ class _SequenceOperator:
                 raise ValueError("the stream is being captured: give the call a workspace of its own, which the graph then keeps using")
         own = self._workspaces.get((key, stream))
         if own is None or own.count < needed:
+            current_device(self._lib, self.device)
             if own is not None:
                 own.free()
             own = self._workspaces[key, stream] = Array(needed, "uint8", device_only=True)
@@ -120,8 +124,8 @@ class CausalConvolution(_SequenceOperator):
     with the same array as initial and final state is a token of every running sequence."""
 
     def __init__(self, sequences, length, channels, taps, dtype="float32", silu=False, device=0):
-        super().__init__(sequences, length, dtype, None, device)
-        self.channels, self.taps, self.silu = int(channels), int(taps), bool(silu)
+        super().__init__(sequences, length, dtype, device)
+        self.channels, self.taps, self.silu = _count(channels, "channels"), _count(taps, "taps"), bool(silu)
         self._width = self.channels
 
     def bind(self, x, weight, bias=None, out=None, initial_state=None, final_state=None, offsets=None, slots=None):
@@ -182,8 +186,8 @@ class SelectiveScan(_SequenceOperator):
     every running sequence."""
 
     def __init__(self, sequences, length, channels, states, groups=1, dtype="float32", softplus=False, device=0):
-        super().__init__(sequences, length, dtype, None, device)
-        self.channels, self.states, self.groups, self.softplus = int(channels), int(states), int(groups), bool(softplus)
+        super().__init__(sequences, length, dtype, device)
+        self.channels, self.states, self.groups, self.softplus = _count(channels, "channels"), _count(states, "states"), _count(groups, "groups"), bool(softplus)
         self._width = self.channels
 
     def bind(self, u, delta, A, B, C, out=None, D=None, delta_bias=None, z=None, initial_state=None, final_state=None, offsets=None, slots=None):

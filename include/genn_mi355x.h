@@ -585,6 +585,8 @@ int gennmi_program_get_info(gennmi_program *program, unsigned long long info[4])
  * ------------------------------------------------------------------------------------------- */
 /* Whether work on the stream is being captured into a graph (never the null stream's): for callers that keep a workspace between calls. */
 int gennmi_stream_is_capturing(void *stream, int *capturing);
+/* The device that calls of this thread launch and allocate on: for callers that keep arrays of one device. */
+int gennmi_current_device(int *device);
 /* Rows of adjacent elements; strides count elements.  Row t of sequence s lies at data + s * sequenceStride + t * rowStride, or,
  * where the sequences are packed (gennmi_sequences_t::offsets), at data + (offsets[s] + t) * rowStride. */
 typedef struct gennmi_rows_t {

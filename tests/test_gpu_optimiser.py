@@ -207,6 +207,32 @@ def test_a_checkpoint_continues_where_it_was_taken():
     assert other.steps == 4 and all(torch.equal(a, b) for a, b in zip(again, w))
 
 
+def test_rates_of_any_kind_of_number():
+    import numpy as np
+    results = []
+    for rate in (0.5, np.float32(0.5), np.float64(0.5), torch.tensor(0.5).cuda()):
+        w, g = torch.ones(10).cuda(), torch.ones(10).cuda()
+        opt = AdamW()
+        opt.add(w, g)
+        opt.build()
+        opt.step(rate)
+        torch.cuda.synchronize()
+        results.append(w.clone())
+    assert all(torch.equal(results[0], r) for r in results) and float(results[0][0]) < 0.6
+
+
+def test_another_current_device_is_refused():
+    """(an optimiser that says it belongs to the second device, while the first is current)"""
+    w = torch.ones(10).cuda()
+    opt = AdamW()
+    opt.add(w, w.clone())
+    opt.device = 1
+    with pytest.raises(ValueError, match="current device is 0"):
+        opt.add(w.clone(), w.clone())
+    with pytest.raises(ValueError, match="current device is 0"):
+        opt.build()
+
+
 def test_what_the_layer_refuses():
     opt = AdamW()
     w = torch.zeros(10).cuda()

@@ -577,6 +577,9 @@ def test_arrays_of_the_package_and_what_the_layer_refuses():
     with pytest.raises(_abi.GennmiError, match="same array"):
         c.bind(x=t, weight=w, out=t)
         c.run()
+    for wrong in (dict(length=1 << 31), dict(sequences=-1), dict(channels=1 << 40), dict(taps=-2)):
+        with pytest.raises(ValueError, match="below 2"):
+            CausalConvolution(**{**dict(sequences=2, length=n, channels=D, taps=K), **wrong})
     s = SelectiveScan(2, n, D, N)
     with pytest.raises(RuntimeError, match="bind"):
         s.run()

@@ -87,6 +87,7 @@ def test_calls_without_arguments_and_workspaces_are_refused():
     refused(lib.gennmi_selective_scan_backward(C.byref(scan()), None, None, 0, None), -2, "null gradient")
     refused(lib.gennmi_selective_scan_workspace(C.byref(scan()), None), -2, "null result")
     refused(lib.gennmi_stream_is_capturing(None, None), -2, "null result")
+    refused(lib.gennmi_current_device(None), -2, "null result")
     # the gradients' checks
     g = _abi.CausalConvGradient(out=_abi.Rows(AT + 8192, 24, 120), x=_abi.Rows(AT + 16384, 24, 120), weight=AT)
     need = lib.gennmi_causal_conv_backward_workspace
