@@ -41,18 +41,15 @@ template<int WIDTH> __device__ inline float fold(float a, float b)
         return (upper ? b : a) + partner<WIDTH>(upper ? a : b);
     }
 }
-// Sums over the 64 lanes of M values a lane, M a power of two: folded until one register is left, then added up.  Lane l has the sum of value l / (64 / M).
-template<int M, int WIDTH = 32> __device__ inline float sumOfLanes(const float (&v)[M])
+// Of M values a lane, M a power of two, one register is left: lane l has its share of the sum over the lanes of value l / (64 / M), as the 64 / M lanes of that
+// value together have all of it.
+template<int M, int WIDTH = 32> __device__ inline float shareOfLanes(const float (&v)[M])
 {
     if constexpr(M > 1) {
         float half[M / 2];
         #pragma unroll
         for(int i = 0; i < M / 2; i++) { half[i] = fold<WIDTH>(v[i], v[i + M / 2]); }
-        return sumOfLanes<M / 2, WIDTH / 2>(half);
-    }
-    else if constexpr(WIDTH >= 1) {
-        const float one[1] = {v[0] + partner<WIDTH>(v[0])};
-        return sumOfLanes<1, WIDTH / 2>(one);
+        return shareOfLanes<M / 2, WIDTH / 2>(half);
     }
     else { return v[0]; }
 }

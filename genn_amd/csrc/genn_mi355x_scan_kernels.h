@@ -539,21 +539,23 @@ void scanTokenKernel(ScanArgs a)
 //   du = dt q + D gy;  d(dt) = u q + r;  dA += x dt;  and exp(dt A) dh for the row before
 // A block's walks take PART of the states at a time, so that R * PART of them, and as many decays, fit the registers of two wavefronts a SIMD.
 //
-// Bound by vector instructions: 444 a row and wavefront of 16 states, a fifth of them the sums over channels, and units busy for 74 % of the time (251 registers, so two
-// wavefronts a SIMD; 18 KiB of LDS each).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 690 us, the first 209, the second 56 (memory, 4.8 TB/s), sums
+// Bound by vector instructions: 420 a row and wavefront of 16 states, an eighth of them the sums over channels (all of them in registers: 444 and 690 us), and units
+// busy for three quarters of the time (252 registers, so two wavefronts a SIMD; 20 KiB of LDS each, all that there is for eight).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 667 us, the first 209, the second 56 (memory, 4.8 TB/s), sums
 // over tiles 23 and over chunks 17.  PART 4 spills (813 us), so do three wavefronts a SIMD (1240), without the ties of readAfter it was 9.4 ms.
 template<typename T, int NP, int R, int BLOCKS, bool SLABS>
 __global__ __launch_bounds__(SLABS ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
 {
-    constexpr int PART = 2, PARTS = NP / PART, SPREAD = 64 / (2 * PART);     // SPREAD: lanes that have the same sum over the lanes
-    constexpr int SPACE = BLOCKS * NP * 64 + R * 2 * NP * 2;                 // floats of LDS a wavefront
+    constexpr int PART = 2, PARTS = NP / PART;
+    constexpr int SPACE = BLOCKS * NP * 64 + R * 2 * NP * 2 + R * 64;        // floats of LDS a wavefront
+    static_assert(PART == 2 && R == 8, "the lanes' shares of a part's sums are eight values a lane");
     extern __shared__ __attribute__((aligned(16))) float lds[];
     uint32_t number;
     const ScanPlace s = scanPlace<NP>(a, number);
     const uint32_t slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, channel = s.channel, place = channel * (uint32_t)sizeof(T);
     float *const kept = lds + (size_t)slab * SPACE;       // [block][part][lane][PART]: the states before a block
     float *const bc = kept + BLOCKS * NP * 64, *const rowSums = bc + R * 2 * NP;     // both [row][B, C][NP]
+    float *const shares = rowSums + R * 2 * NP;             // [row][lane]: of a part's sums over the lanes, 16 lanes for each of B's two and C's two
     float *const sums = lds + (size_t)a.slabs * SPACE;      // SLABS: [slab][row][q, r, y][lane]
     const auto keep = [&](uint32_t b, const float (&h)[NP]) {
         #pragma unroll
@@ -571,8 +573,18 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
         const T *B = rowsOf<const T>(a.B, a.sequences, s.place) + bcAt, *C = rowsOf<const T>(a.C, a.sequences, s.place) + bcAt;
         const float bias = a.deltaBias ? a.deltaBias[channel] : 0.0f, skip = a.D ? a.D[channel] : 0.0f;
         const uint64_t sumRow = (uint64_t)s.tile * g.rows + (a.sequences.offsets ? s.place.first : (uint64_t)s.place.sequence * a.sequences.length);
-        // (where this lane's sum over the lanes goes, SPREAD of them to the same place)
-        float *const rowSum = rowSums + (lane / 32) * NP + (lane / SPREAD) % PART;
+        // Sums over the lanes of what a part gives B and C: folded in registers as far as two exchanges go, the rest through LDS for all rows of the block at once, where
+        // a lane adds up half of the 16 shares of one value of one row
+        float *const rowSum = rowSums + lane / 8 * 2 * NP + lane % 8 / 4 * NP + lane % 4 / 2;
+        const auto addShares = [&](int part) {
+            float x[8];
+            const Pack<float, 4> *const from = (const Pack<float, 4>*)(shares + lane * 8);
+            const Pack<float, 4> low = from[0], high = from[1];
+            #pragma unroll
+            for(int k = 0; k < 4; k++) { x[k] = low.v[k] + high.v[k]; }
+            const float sum = (x[0] + x[2]) + (x[1] + x[3]);
+            rowSum[part * PART] = sum + gennmi_lanes::partner<1>(sum);
+        };
         float A[NP], h[NP], carry[NP];
         loadA<NP>(a, s, A);
         if(a.chunkState) { loadChunk<NP>(a, s, a.chunkState, number, h); loadChunk<NP>(a, s, g.chunkGradient, number, carry); }
@@ -667,11 +679,13 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
             #pragma unroll
             for(int part = 0; part < PARTS; part++) {
                 float hs[R][PART], decay[R][PART], start[PART];
+                waveFence();
                 #pragma unroll
                 for(int k = 0; k < PART; k++) { start[k] = kept[((b * PARTS + part) * 64 + lane) * PART + k]; }
                 float nextB[PART], nextC[PART], terms[2 * PART];
                 #pragma unroll
                 for(int k = 0; k < PART; k++) { nextB[k] = bc[part * PART + k]; }
+                if(part) { addShares(part - 1); }           // (of the part before: its trip through LDS is one with that of this part's states)
                 #pragma unroll
                 for(int r = 0; r < R; r++) {
                     const float w = dt[r] * uu[r];
@@ -702,7 +716,7 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
                     }
                     readAfter<PART>(dA, part * PART);
                     // (the sums of the row behind: a chain of dependent steps, which this row's arithmetic fills)
-                    if(r < R - 1) { rowSum[(r + 1) * 2 * NP + part * PART] = gennmi_lanes::sumOfLanes<2 * PART>(terms); }
+                    if(r < R - 1) { shares[(r + 1) * 64 + lane] = gennmi_lanes::shareOfLanes<2 * PART>(terms); }
                     #pragma unroll
                     for(int k = 0; k < PART; k++) {
                         Bn[k] = nextB[k];
@@ -722,7 +736,7 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
                         dA[n] = __builtin_fmaf(x, dt[r], dA[n]);
                         rr[r] = __builtin_fmaf(x, A[n], rr[r]);
                     }
-                    if(r == 0) { rowSum[part * PART] = gennmi_lanes::sumOfLanes<2 * PART>(terms); }
+                    if(r == 0) { shares[lane] = gennmi_lanes::shareOfLanes<2 * PART>(terms); }
                     if(part == PARTS - 1 && row + r < end) {
                         if(SLABS) {
                             sums[((slab * R + r) * 3) * 64 + lane] = q[r];
@@ -733,6 +747,8 @@ void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)
                     }
                 }
             }
+            waveFence();
+            addShares(PARTS - 1);
             waveFence();
             #pragma unroll
             for(int e = 0; e < R * 2 * NP / 64; e++) {

@@ -307,7 +307,7 @@ template<typename T, int NP, bool SLABS> int launchScanBackward(const ScanArgs &
         if(const int rc = gennmi_detail::afterLaunch("selective_scan_backward")) { return rc; }
     }
     constexpr uint32_t BLOCKS = gradientBlocks(SLABS ? 2 : 1);
-    const size_t lds = sizeof(float) * (p.slabs * (BLOCKS * NP * 64 + SCAN_BLOCK_ROWS * 2 * NP * 2) + (SLABS ? p.slabs * SCAN_BLOCK_ROWS * 3 * 64 : 0));
+    const size_t lds = sizeof(float) * (p.slabs * (BLOCKS * NP * 64 + SCAN_BLOCK_ROWS * (2 * NP * 2 + 64)) + (SLABS ? p.slabs * SCAN_BLOCK_ROWS * 3 * 64 : 0));
     auto kernel = scanBackwardKernel<T, NP, (int)SCAN_BLOCK_ROWS, (int)BLOCKS, SLABS>;
     if(lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
