@@ -174,7 +174,7 @@ inline int checkRows(const char *what, const char *which, const gennmi_rows_t &r
     if(!r.data) { return refuse(" is missing"); }
     if((uintptr_t)r.data % size) { return refuse(" is not aligned to its elements"); }
     if(s.length > 1 && r.rowStride < width) { return refuse(": rows overlap (rowStride)"); }
-    if(r.rowStride > (1ull << 40) || r.sequenceStride > (1ull << 50)) { return refuse(": stride out of range"); }
+    if((r.rowStride > 0xffffffffull && (s.length > 1 || s.offsets)) || r.sequenceStride > (1ull << 50)) { return refuse(": stride out of range"); }
     return GENNMI_OK;
 }
 // What is written: one row of a sequence and another must not share elements either

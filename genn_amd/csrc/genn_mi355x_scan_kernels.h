@@ -13,7 +13,7 @@
 //
 // Bound by vector instructions, not by memory: a state takes a row a product and an exponential (two slots of a SIMD's issue) for its decay, a product and a sum
 // for what comes in, a sum for y, 6 slots, of which the first kernel of a split scan needs 5 as well.  At 39.3 T lane-slots a second 4096 rows x 2048 channels x 16
-// states are 38 us of these alone, their 68 MB 14 us.  They take 81 us in bf16: 37 the first kernel, 8 the second, 46 the third, with the vector
+// states are 38 us of these alone, their 68 MB 14 us.  They take 79 us in bf16: 37 the first kernel, 8 the second, 45 the third, with the vector
 // units busy for three quarters of the time (softplus, gate and conversions are a fifth of their instructions).  What there is to gain by matrix instructions is
 // nothing: every state of every channel has decays of its own.
 #ifndef GENN_MI355X_SCAN_KERNELS_H
@@ -87,7 +87,7 @@ template<typename T, int NP, int R> struct StagedBC
 {
     static constexpr int EACH = R * 2 * NP / 64, LANES = 2 * NP;        // LANES: that a row takes
     const T *at;
-    uint64_t stride;
+    uint32_t stride;
     bool here;
     T raw[EACH];
     __device__ inline StagedBC(const T *B, const T *C, const ScanArgs &a, uint32_t numStates)
@@ -95,14 +95,14 @@ template<typename T, int NP, int R> struct StagedBC
         const uint32_t lane = threadIdx.x & 63, n = lane % NP;
         const bool isC = (lane / NP) & 1;
         at = (isC ? C : B) + min(n, numStates - 1);
-        stride = isC ? a.C.rowStride : a.B.rowStride;
+        stride = (uint32_t)(isC ? a.C.rowStride : a.B.rowStride);
         here = n < numStates;
     }
     __device__ static inline uint32_t rowOf(int q) { return q * (64 / LANES) + (threadIdx.x & 63) / LANES; }
     __device__ inline void fetch(uint32_t row, uint32_t end)
     {
         #pragma unroll
-        for(int q = 0; q < EACH; q++) { raw[q] = at[min(row + rowOf(q), end - 1) * stride]; }
+        for(int q = 0; q < EACH; q++) { raw[q] = at[(uint64_t)min(row + rowOf(q), end - 1) * stride]; }
     }
     __device__ inline void store(float *lds, uint32_t row, uint32_t end) const
     {
@@ -203,11 +203,12 @@ template<int NP> __device__ inline void storeChunk(const ScanArgs &a, const Scan
     }
 }
 
-// One row of a channel's array, R of them, fetched a block of rows before they are needed (rows behind the last one are that one again)
+// One row of a channel's array, R of them, fetched a block of rows before they are needed (rows behind the last one are that one again).  Strides of rows fit 32 bits: two
+// scalar products for an address instead of four (a scan of 4096 rows x 2048 channels 81.5 -> 79.3 us; the same in the walk back of the gradients: 870 -> 907, other registers)
 template<typename T, int R> struct StagedRows
 {
     T raw[R];
-    __device__ inline void fetch(const T *rows, uint64_t stride, uint32_t place, uint32_t row, uint32_t end)
+    __device__ inline void fetch(const T *rows, uint32_t stride, uint32_t place, uint32_t row, uint32_t end)
     {
         #pragma unroll
         for(int r = 0; r < R; r++) { raw[r] = loadAt(rows, min(row + r, end - 1), stride, place); }
@@ -452,7 +453,7 @@ void scanKernel(ScanArgs a)
         if(s.active) {
             #pragma unroll
             for(int r = 0; r < R; r++) {
-                if(row + r < end && (!SLABS || r % a.slabs == slab)) { storeAt(out, row + r, a.out.rowStride, place, narrow<T>(y[r] * gate[r])); }
+                if(row + r < end && (!SLABS || r % a.slabs == slab)) { storeAt(out, row + r, (uint32_t)a.out.rowStride, place, narrow<T>(y[r] * gate[r])); }
             }
         }
     }
@@ -540,7 +541,7 @@ void scanTokenKernel(ScanArgs a)
 // A block's walks take PART of the states at a time, so that R * PART of them, and as many decays, fit the registers of two wavefronts a SIMD.
 //
 // Bound by vector instructions: 420 a row and wavefront of 16 states, an eighth of them the sums over channels (all of them in registers: 444 and 690 us), and units
-// busy for three quarters of the time (252 registers, so two wavefronts a SIMD; 20 KiB of LDS each, all that there is for eight).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 667 us, the first 209, the second 56 (memory, 4.8 TB/s), sums
+// busy for three quarters of the time (252 registers, so two wavefronts a SIMD; 20 KiB of LDS each, all that there is for eight).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 670 us, the first 207, the second 57 (memory, 4.8 TB/s), sums
 // over tiles 23 and over chunks 17.  PART 4 spills (813 us), so do three wavefronts a SIMD (1240), without the ties of readAfter it was 9.4 ms.
 template<typename T, int NP, int R, int BLOCKS, bool SLABS>
 __global__ __launch_bounds__(SLABS ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2, 2)))

@@ -588,7 +588,8 @@ int gennmi_stream_is_capturing(void *stream, int *capturing);
 /* The device that calls of this thread launch and allocate on: for callers that keep arrays of one device. */
 int gennmi_current_device(int *device);
 /* Rows of adjacent elements; strides count elements.  Row t of sequence s lies at data + s * sequenceStride + t * rowStride, or,
- * where the sequences are packed (gennmi_sequences_t::offsets), at data + (offsets[s] + t) * rowStride. */
+ * where the sequences are packed (gennmi_sequences_t::offsets), at data + (offsets[s] + t) * rowStride.  rowStride (where there is a second row) is below 2^32,
+ * sequenceStride up to 2^50. */
 typedef struct gennmi_rows_t {
     void *data;
     uint64_t rowStride, sequenceStride;

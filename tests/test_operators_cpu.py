@@ -53,7 +53,7 @@ def test_descriptors_have_the_librarys_layout():
     (dict(type=1), -3, "element type"), (dict(type=7), -3, "element type"), (dict(taps=0), -3, "taps"), (dict(taps=9), -3, "taps"),
     (dict(channels=0), -2, "channels"), (dict(weight=None), -2, "weight"), (dict(weight=AT + 2), -2, "aligned"), (dict(bias=AT + 1), -2, "aligned"),
     (dict(x__data=None), -2, "x is missing"), (dict(x__data=AT + 1), -2, "aligned"), (dict(out__data=AT), -2, "same array"), (dict(out__data=None), -2, "out is missing"),
-    (dict(x__rowStride=23), -2, "rows overlap"), (dict(out__sequenceStride=0), -2, "sequences overlap"), (dict(out__rowStride=1 << 41), -2, "stride"),
+    (dict(x__rowStride=23), -2, "rows overlap"), (dict(out__sequenceStride=0), -2, "sequences overlap"), (dict(out__rowStride=1 << 41), -2, "stride"), (dict(x__rowStride=1 << 32), -2, "stride"),
     (dict(initialState=AT + 1), -2, "state"), (dict(finalState=AT + 1), -2, "state"),
     (dict(sequences__count=(1 << 24) + 1), -2, "more sequences"), (dict(sequences__length=1 << 31), -2, "more sequences"),
     (dict(sequences__offsets=AT + 2, sequences__rows=10), -2, "offsets"), (dict(sequences__slots=AT, sequences__numSlots=0), -2, "numSlots"),
@@ -128,7 +128,7 @@ def test_workspaces_of_packed_sequences_go_by_their_rows():
         c = scan(sequences__count=1000, sequences__length=8000, sequences__offsets=AT, sequences__rows=10000)
         assert entry(C.byref(c), C.byref(size)) == 0
         assert size.value < (10000 // 8 + 1000) * 24 * (16 * 3 + 4) * 4 + 10000 * 2 * 16 * 2 * 4 + 4096
-    c = scan(sequences__length=1)
+    c = scan(sequences__length=1, u__rowStride=1 << 33)         # (the stride of rows that are not there)
     assert lib.gennmi_selective_scan_workspace(C.byref(c), C.byref(size)) == 0 and size.value == 0     # (a token needs none)
 
 
