@@ -61,9 +61,10 @@ Sequences sequencesOf(const gennmi_sequences_t &s, uint32_t chunk)
     d.perSequence = std::max(1u, (s.length + chunk - 1) / chunk);
     return d;
 }
-// Chunk numbers: see Sequences
+// Chunk numbers: see Sequences.  Without sequences none, however many rows packed arrays hold: kernels look for the sequence of a number.
 uint64_t chunkNumbers(const gennmi_sequences_t &s, uint32_t chunk)
 {
+    if(!s.count) { return 0; }
     return s.offsets ? s.rows / chunk + s.count : (uint64_t)s.count * std::max(1u, (s.length + chunk - 1) / chunk);
 }
 uint64_t totalRows(const gennmi_sequences_t &s) { return s.offsets ? s.rows : (uint64_t)s.count * s.length; }

@@ -328,6 +328,29 @@ def test_nothing_to_do_leaves_states_and_gives_zero_gradients(sequences, length)
     assert torch.all(dA == 0) and torch.all(dw == 0)
 
 
+@pytest.mark.parametrize("length", [4, 500])
+def test_packed_arrays_without_sequences(length):
+    """Rows that belong to no sequence are left alone, and sums over sequences are zero."""
+    from genn_amd.sequence import CausalConvolution, SelectiveScan
+    rows, D, N, K = 300, 20, 6, 3
+    full = lambda *shape: torch.full(shape, 7.0).cuda()
+    offsets = torch.zeros(1, dtype=torch.int32).cuda()
+    c, s = CausalConvolution(0, length, D, K), SelectiveScan(0, length, D, N)
+    out = {k: full(rows, D) for k in ("c", "s", "x", "u", "delta", "z")}
+    sums = {k: full(*shape) for k, shape in (("weight", (D, K)), ("bias", (D,)), ("A", (D, N)), ("D", (D,)), ("delta_bias", (D,)))}
+    dB, dC = full(rows, N), full(rows, N)
+    c.bind(x=full(rows, D), weight=full(D, K), bias=full(D), out=out["c"], offsets=offsets)
+    s.bind(u=full(rows, D), delta=full(rows, D), A=full(D, N), B=full(rows, N), C=full(rows, N), D=full(D), delta_bias=full(D), z=full(rows, D), out=out["s"], offsets=offsets)
+    c.bind_gradients(out=full(rows, D), x=out["x"], weight=sums["weight"], bias=sums["bias"])
+    s.bind_gradients(out=full(rows, D), u=out["u"], delta=out["delta"], z=out["z"], B=dB, C=dC, A=sums["A"], D=sums["D"], delta_bias=sums["delta_bias"])
+    for op in (c, s):
+        op.run()
+        op.backward()
+    torch.cuda.synchronize()
+    assert all(torch.all(t == 7.0) for t in (*out.values(), dB, dC))
+    assert all(torch.all(t == 0.0) for t in sums.values())
+
+
 def test_another_current_device_is_refused():
     """(the descriptors say that their arrays are the second device's, while the first is current)"""
     from genn_amd.sequence import CausalConvolution, SelectiveScan

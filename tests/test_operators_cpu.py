@@ -132,6 +132,17 @@ def test_workspaces_of_packed_sequences_go_by_their_rows():
     assert lib.gennmi_selective_scan_workspace(C.byref(c), C.byref(size)) == 0 and size.value == 0     # (a token needs none)
 
 
+def test_packed_arrays_without_sequences_have_no_chunks():
+    """Rows that belong to no sequence: there is nothing to sum over, and nothing to keep for it (offsets has one element)."""
+    lib, size = _abi.load(), C.c_size_t()
+    none = dict(sequences__count=0, sequences__offsets=AT, sequences__rows=10000)
+    assert lib.gennmi_causal_conv_backward_workspace(C.byref(conv(sequences__length=100, **none)), C.byref(size)) == 0 and size.value == 0
+    for length in (4, 8000):
+        assert lib.gennmi_selective_scan_workspace(C.byref(scan(sequences__length=length, **none)), C.byref(size)) == 0 and size.value == 0
+        assert lib.gennmi_selective_scan_backward_workspace(C.byref(scan(sequences__length=length, **none)), C.byref(size)) == 0
+        assert size.value <= 2 * 10000 * 2 * 16 * 4 + 256           # (only what goes by rows)
+
+
 def parameter(**changes):
     p = _abi.Parameter(weight=AT, gradient=AT + 8192, m=AT + 16384, v=AT + 32768, count=100, weightType=F32, gradientType=BF16)
     return changed(p, changes)
