@@ -142,20 +142,16 @@ template<typename T> __device__ inline T *rowsOf(const gennmi_rows_t &r, const S
     return (T*)r.data + (s.offsets ? p.first * r.rowStride : (uint64_t)p.sequence * r.sequenceStride);
 }
 
-// A thread's number in its launch of 256 a work-group, divided by `by` (a division of 64 bits is some hundred instructions)
+// A thread's number in its launch of 256 a work-group, divided by `by` (32 bits do: see mostBlocks)
 __device__ inline void divideItem(uint32_t by, uint32_t &quotient, uint32_t &rest)
 {
-    if(gridDim.x <= (1u << 24)) {
-        const uint32_t item = blockIdx.x * 256 + threadIdx.x;
-        quotient = item / by;
-        rest = item - quotient * by;
-    }
-    else {
-        const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-        quotient = (uint32_t)(item / by);
-        rest = (uint32_t)(item - (uint64_t)quotient * by);
-    }
+    const uint32_t item = blockIdx.x * 256 + threadIdx.x;
+    quotient = item / by;
+    rest = item - quotient * by;
 }
+
+// Work-groups of that many threads that one launch takes: its threads are numbered in 32 bits
+constexpr uint64_t mostBlocks(uint32_t threads) { return 0xffffffffull / threads; }
 
 // host side (a call of a few microseconds: texts are put together for a refusal only)
 inline int checkSequences(const char *what, const gennmi_sequences_t &s, bool gradients)

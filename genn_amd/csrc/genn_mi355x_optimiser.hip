@@ -363,7 +363,7 @@ int gennmi_optimiser_finalise(gennmi_optimiser *optimiser)
         std::vector<ChunkDev> chunks;
         for(size_t k = 0; k < optimiser->table.size(); k++) {
             const uint64_t of = (optimiser->table[k].count + CHUNK - 1) / CHUNK;
-            if(chunks.size() + of > 0x7fffffffull) { return fail(GENNMI_EINVAL, "optimiser_finalise: more weights than one launch covers"); }
+            if(chunks.size() + of > mostBlocks(256)) { return fail(GENNMI_EINVAL, "optimiser_finalise: more weights than one launch covers"); }
             for(uint64_t c = 0; c < of; c++) { chunks.push_back({(uint32_t)k, (uint32_t)c}); }
         }
         if(chunks.empty()) { chunks.push_back({(uint32_t)optimiser->table.size(), 0}); }        // (a step of nothing counts: a tensor without weights)

@@ -35,11 +35,13 @@ void chunkSumKernel(ChunkSums a)
     if(n < a.width) { if(a.out) { a.out[(uint64_t)channel * a.width + n] = (float)sum; } }
     else if(a.more[n - a.width]) { a.more[n - a.width][channel] = (float)sum; }
 }
+uint64_t chunkSumBlocks(uint32_t rows, uint32_t channels) { return (uint64_t)rows * ((channels + 63) / 64); }
 int launchChunkSum(const char *what, const ChunkSums &a, hipStream_t stream)
 {
-    chunkSumKernel<<<dim3(a.rows * ((a.channels + 63) / 64)), dim3(1024), 0, stream>>>(a);
+    chunkSumKernel<<<dim3((uint32_t)chunkSumBlocks(a.rows, a.channels)), dim3(1024), 0, stream>>>(a);
     return gennmi_detail::afterLaunch(what);
 }
+int tooMany(const char *what) { return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers"); }
 }
 
 #include "genn_mi355x_lanes.h"
@@ -68,7 +70,6 @@ uint64_t chunkNumbers(const gennmi_sequences_t &s, uint32_t chunk)
     return s.offsets ? s.rows / chunk + s.count : (uint64_t)s.count * std::max(1u, (s.length + chunk - 1) / chunk);
 }
 uint64_t totalRows(const gennmi_sequences_t &s) { return s.offsets ? s.rows : (uint64_t)s.count * s.length; }
-constexpr uint64_t MOST_BLOCKS = 0x7fffffffull;
 
 // ---- causal convolution
 // Rows of a chunk: at least taps - 1, so that only the first chunk reads the initial state
@@ -146,12 +147,12 @@ template<typename T, int VEC> void launchConvBackward(const ConvArgs &a, const C
 #undef TAPS
 }
 #undef EACH_TAPS
+uint64_t convBlocks(const gennmi_causal_conv_t &c, uint32_t vector, uint32_t chunk) { return (chunkNumbers(c.sequences, chunk) * (c.channels / vector) + 255) / 256; }
 int runConv(const char *what, const gennmi_causal_conv_t &c, uint32_t vector, const ConvGradientArgs *g, hipStream_t stream)
 {
     const uint32_t chunk = convChunk(c, g != nullptr);
     const ConvArgs a = convArgs(c, vector, chunk);
-    const uint64_t blocks = ((uint64_t)a.numbers * a.vectors + 255) / 256;
-    if(chunkNumbers(c.sequences, chunk) > MOST_BLOCKS || blocks > MOST_BLOCKS) { return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers"); }
+    const uint64_t blocks = convBlocks(c, vector, chunk);
     if(!blocks) { return GENNMI_OK; }
     return withType(c.type, [&](auto t) {
         const dim3 grid((uint32_t)blocks);
@@ -250,14 +251,20 @@ ScanSpace scanSpace(const gennmi_scan_t &c, const ScanPlan &p, bool gradients)
     }
     return s;
 }
-int scanArgs(const char *what, const gennmi_scan_t &c, const ScanPlan &p, ScanArgs &a)
+// A token's states are shared by that many lanes, four each
+uint32_t tokenLanes(uint32_t states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : states <= 64 ? 16 : 32; }
+uint64_t tokenBlocks(const gennmi_scan_t &c) { return ((uint64_t)c.sequences.count * c.channels * tokenLanes(c.states) + 255) / 256; }
+// Whether the launches of a pass, but for the closing sums of gradients, cover it
+bool scanFits(const gennmi_scan_t &c, const ScanPlan &p, bool gradients)
 {
-    a = ScanArgs{};
+    if(!gradients && c.sequences.length <= 1) { return tokenBlocks(c) <= mostBlocks(256); }
+    const bool join = p.split && (uint64_t)c.sequences.count * c.states * ((c.channels + 63) / 64) > mostBlocks(64);
+    return chunkNumbers(c.sequences, p.chunk) * scanTiles(c) <= mostBlocks(64 * p.slabs) && !join;
+}
+ScanArgs scanArgs(const gennmi_scan_t &c, const ScanPlan &p)
+{
+    ScanArgs a{};
     const uint64_t numbers = chunkNumbers(c.sequences, p.chunk), tiles = scanTiles(c);
-    if(numbers * tiles > MOST_BLOCKS || (uint64_t)c.sequences.count * c.states * ((c.channels + 63) / 64) > MOST_BLOCKS ||
-       (uint64_t)c.sequences.count * c.channels / 8 > MOST_BLOCKS) {
-        return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers");
-    }
     a.sequences = sequencesOf(c.sequences, p.chunk);
     a.u = c.u; a.delta = c.delta; a.z = c.z; a.out = c.out; a.B = c.B; a.C = c.C;
     a.A = c.A; a.D = c.D; a.deltaBias = c.deltaBias;
@@ -268,7 +275,7 @@ int scanArgs(const char *what, const gennmi_scan_t &c, const ScanPlan &p, ScanAr
     a.tiles = (uint32_t)tiles;
     a.numbers = (uint32_t)numbers;
     a.slabs = p.slabs;
-    return GENNMI_OK;
+    return a;
 }
 int checkWorkspace(const char *what, const void *workspace, size_t have, size_t need)
 {
@@ -288,13 +295,13 @@ template<typename T, int NP, bool SLABS> int launchScan(const ScanArgs &a, const
     scanKernel<T, NP, SLABS><<<grid, threads, 0, stream>>>(a);
     return gennmi_detail::afterLaunch("selective_scan");
 }
-template<typename T, int LANES> int launchToken(const ScanArgs &a, hipStream_t stream)
+template<typename T, int LANES> int launchToken(const ScanArgs &a, uint32_t blocks, hipStream_t stream)
 {
     // four states a lane in one access, where every array lies so
     const auto fours = [](const void *p, uint32_t size) { return (uintptr_t)p % (4 * size) == 0; };
     const auto rows = [&](const gennmi_rows_t &r) { return fours(r.data, sizeof(T)) && r.rowStride % 4 == 0 && r.sequenceStride % 4 == 0; };
     const bool quads = a.states % 4 == 0 && fours(a.A, 4) && fours(a.initialState, 4) && fours(a.finalState, 4) && rows(a.B) && rows(a.C);
-    const dim3 grid((uint32_t)(((uint64_t)a.sequences.count * a.channels * LANES + 255) / 256));
+    const dim3 grid(blocks);
     if(quads) { scanTokenKernel<T, LANES, true><<<grid, dim3(256), 0, stream>>>(a); } else { scanTokenKernel<T, LANES, false><<<grid, dim3(256), 0, stream>>>(a); }
     return gennmi_detail::afterLaunch("selective_scan");
 }
@@ -351,8 +358,10 @@ int gennmi_causal_conv(const gennmi_causal_conv_t *conv, void *stream)
 {
     return gennmi_detail::guarded("causal_conv", [&] {
         if(const int rc = checkConv("causal_conv", conv, false)) { return rc; }
+        const uint32_t vector = convVector(*conv, nullptr);
+        if(convBlocks(*conv, vector, convChunk(*conv, false)) > mostBlocks(256)) { return tooMany("causal_conv"); }
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, conv->sequences.device)) { return rc; }
-        if(const int rc = runConv("causal_conv", *conv, convVector(*conv, nullptr), nullptr, (hipStream_t)stream)) { return rc; }
+        if(const int rc = runConv("causal_conv", *conv, vector, nullptr, (hipStream_t)stream)) { return rc; }
         const uint32_t size = sizeOf(conv->type);
         noteRows(conv->out, conv->sequences, conv->channels, size);
         if(conv->finalState) { gennmi_detail::noteDeviceWrite(conv->finalState, statesOf(conv->sequences) * (conv->taps - 1) * conv->channels * size); }
@@ -389,6 +398,8 @@ int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_c
         }
         if(g.initialState && g.initialState == g.finalState) { return fail(GENNMI_EINVAL, "causal_conv_backward: the gradient of initialState is an array of its own"); }
         const bool sums = g.weight || g.bias;
+        const uint32_t vector = convVector(*conv, gradient);
+        if(convBlocks(*conv, vector, convChunk(*conv, true)) > mostBlocks(256) || (sums && chunkSumBlocks(conv->taps + 1, conv->channels) > mostBlocks(1024))) { return tooMany(what); }
         if(const int rc = checkWorkspace(what, workspace, workspaceBytes, sums ? convWorkspace(*conv) : 0)) { return rc; }
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, conv->sequences.device)) { return rc; }
         ConvGradientArgs a{};
@@ -397,7 +408,7 @@ int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_c
         a.finalState = g.finalState;
         a.initialState = g.initialState;
         a.partial = sums ? (float*)workspace : nullptr;
-        if(const int rc = runConv(what, *conv, convVector(*conv, gradient), &a, (hipStream_t)stream)) { return rc; }
+        if(const int rc = runConv(what, *conv, vector, &a, (hipStream_t)stream)) { return rc; }
         if(sums) {
             const ChunkSums c{a.partial, g.weight, {g.bias, nullptr}, (uint32_t)chunkNumbers(conv->sequences, convChunk(*conv, true)), conv->channels, conv->taps, conv->taps + 1};
             if(const int rc = launchChunkSum(what, c, (hipStream_t)stream)) { return rc; }
@@ -415,7 +426,9 @@ int gennmi_selective_scan_workspace(const gennmi_scan_t *scan, size_t *bytes)
     return gennmi_detail::guarded("selective_scan_workspace", [&] {
         if(const int rc = checkScan("selective_scan_workspace", scan, false)) { return rc; }
         if(!bytes) { return fail(GENNMI_EINVAL, "selective_scan_workspace: null result pointer"); }
-        *bytes = scanSpace(*scan, scanPlan(*scan, false), false).bytes;
+        const ScanPlan p = scanPlan(*scan, false);
+        if(!scanFits(*scan, p, false)) { return tooMany("selective_scan_workspace"); }
+        *bytes = scanSpace(*scan, p, false).bytes;
         return (int)GENNMI_OK;
     });
 }
@@ -426,10 +439,10 @@ int gennmi_selective_scan(const gennmi_scan_t *scan, void *workspace, size_t wor
     return gennmi_detail::guarded(what, [&] {
         if(const int rc = checkScan(what, scan, false)) { return rc; }
         const ScanPlan p = scanPlan(*scan, false);
+        if(!scanFits(*scan, p, false)) { return tooMany(what); }
         const ScanSpace space = scanSpace(*scan, p, false);
         if(const int rc = checkWorkspace(what, workspace, workspaceBytes, space.bytes)) { return rc; }
-        ScanArgs a;
-        if(const int rc = scanArgs(what, *scan, p, a)) { return rc; }
+        ScanArgs a = scanArgs(*scan, p);
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, scan->sequences.device)) { return rc; }
         if(!scan->sequences.count) { return (int)GENNMI_OK; }
         if(p.split) {
@@ -439,12 +452,15 @@ int gennmi_selective_scan(const gennmi_scan_t *scan, void *workspace, size_t wor
         const int rc = withType(scan->type, [&](auto t) {
             typedef decltype(t) T;
             if(scan->sequences.length <= 1) {
-                if(a.states <= 4) { return launchToken<T, 1>(a, (hipStream_t)stream); }
-                if(a.states <= 8) { return launchToken<T, 2>(a, (hipStream_t)stream); }
-                if(a.states <= 16) { return launchToken<T, 4>(a, (hipStream_t)stream); }
-                if(a.states <= 32) { return launchToken<T, 8>(a, (hipStream_t)stream); }
-                if(a.states <= 64) { return launchToken<T, 16>(a, (hipStream_t)stream); }
-                return launchToken<T, 32>(a, (hipStream_t)stream);
+                const uint32_t blocks = (uint32_t)tokenBlocks(*scan);
+                switch(tokenLanes(a.states)) {
+                case 1: return launchToken<T, 1>(a, blocks, (hipStream_t)stream);
+                case 2: return launchToken<T, 2>(a, blocks, (hipStream_t)stream);
+                case 4: return launchToken<T, 4>(a, blocks, (hipStream_t)stream);
+                case 8: return launchToken<T, 8>(a, blocks, (hipStream_t)stream);
+                case 16: return launchToken<T, 16>(a, blocks, (hipStream_t)stream);
+                default: return launchToken<T, 32>(a, blocks, (hipStream_t)stream);
+                }
             }
             return withStates(p, [&](auto np, auto slabs) { return launchScan<T, decltype(np)::value, decltype(slabs)::value>(a, p, (hipStream_t)stream); });
         });
@@ -460,7 +476,9 @@ int gennmi_selective_scan_backward_workspace(const gennmi_scan_t *scan, size_t *
     return gennmi_detail::guarded("selective_scan_backward_workspace", [&] {
         if(const int rc = checkScan("selective_scan_backward_workspace", scan, true)) { return rc; }
         if(!bytes) { return fail(GENNMI_EINVAL, "selective_scan_backward_workspace: null result pointer"); }
-        *bytes = scanSpace(*scan, scanPlan(*scan, true), true).bytes;
+        const ScanPlan p = scanPlan(*scan, true);
+        if(!scanFits(*scan, p, true)) { return tooMany("selective_scan_backward_workspace"); }
+        *bytes = scanSpace(*scan, p, true).bytes;
         return (int)GENNMI_OK;
     });
 }
@@ -491,12 +509,12 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
             if((uintptr_t)p % 4) { return fail(GENNMI_EINVAL, "selective_scan_backward: an array of fp32 is not aligned"); }
         }
         const ScanPlan p = scanPlan(*scan, true);
+        const uint64_t rows = totalRows(scan->sequences), rowSumBlocks = in.B.data || in.C.data ? (rows * 2 * width + 255) / 256 : 0;
+        const uint64_t sumBlocks = in.A || in.D || in.deltaBias ? chunkSumBlocks(scan->states + 2, scan->channels) : 0;
+        if(!scanFits(*scan, p, true) || rowSumBlocks > mostBlocks(256) || sumBlocks > mostBlocks(1024)) { return tooMany(what); }
         const ScanSpace space = scanSpace(*scan, p, true);
         if(const int rc = checkWorkspace(what, workspace, workspaceBytes, space.bytes)) { return rc; }
-        ScanArgs a;
-        if(const int rc = scanArgs(what, *scan, p, a)) { return rc; }
-        const uint64_t rows = totalRows(scan->sequences);
-        if((rows * 2 * width + 255) / 256 > MOST_BLOCKS) { return fail(GENNMI_EINVAL, "selective_scan_backward: more rows than one launch covers"); }
+        ScanArgs a = scanArgs(*scan, p);
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, scan->sequences.device)) { return rc; }
         auto at = [&](size_t offset) { return (float*)((char*)workspace + offset); };
         a.finalState = nullptr;
@@ -516,8 +534,8 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
             const int rc = withType(scan->type, [&](auto t) {
                 typedef decltype(t) T;
                 const int rcScan = withStates(p, [&](auto np, auto slabs) { return launchScanBackward<T, decltype(np)::value, decltype(slabs)::value>(a, g, p, s); });
-                if(rcScan || !(in.B.data || in.C.data) || !rows) { return rcScan; }
-                scanRowSumKernel<T><<<dim3((uint32_t)((rows * 2 * width + 255) / 256)), dim3(256), 0, s>>>(a, g);
+                if(rcScan || !rowSumBlocks) { return rcScan; }
+                scanRowSumKernel<T><<<dim3((uint32_t)rowSumBlocks), dim3(256), 0, s>>>(a, g);
                 return gennmi_detail::afterLaunch(what);
             });
             if(rc) { return rc; }

@@ -582,6 +582,8 @@ int gennmi_program_get_info(gennmi_program *program, unsigned long long info[4])
  * runner make the call fail with GENNMI_ESTATE (run gennmi_flush before); the runners do not hear of what a replay wrote
  * (call gennmi_note_device_write).  A workspace belongs to the call until the call has finished on its stream: calls that may
  * run at the same time, and captured graphs that may, need a workspace each.  No result is a sum of atomics: the same call gives the same bits.
+ * A launch has fewer than 2^32 threads: what would take more (2^30 channels of tokens in all at 16 states, say) is refused with GENNMI_EINVAL before
+ * anything runs.
  * ------------------------------------------------------------------------------------------- */
 /* Whether work on the stream is being captured into a graph (never the null stream's): for callers that keep a workspace between calls. */
 int gennmi_stream_is_capturing(void *stream, int *capturing);
@@ -666,7 +668,7 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
  * with t the number of the step, which the device counts.  States in 32 bits, or in 8 for blocks of GENNMI_ADAMW_BLOCK weights:
  *   m = mScale * c / 448,  v = vScale * (c / 448)^2,   c in e4m3 (OCP), mScale = max |m| and vScale = max v of the block
  * (the nearest code, ties to even; a positive v never gets the code 0, which would make the next step a division by epsilon).  The weights are updated from
- * the states before they are coded. */
+ * the states before they are coded.  An optimiser has fewer than 2^34 weights. */
 #define GENNMI_ADAMW_BLOCK 256
 typedef struct gennmi_optimiser gennmi_optimiser;
 typedef struct gennmi_adamw_t {

@@ -143,6 +143,63 @@ def test_packed_arrays_without_sequences_have_no_chunks():
         assert size.value <= 2 * 10000 * 2 * 16 * 4 + 256           # (only what goes by rows)
 
 
+def reaches_the_device(rc):
+    """(the descriptors name a device that is not there, so nothing is launched)"""
+    said = _abi.load().gennmi_last_error().decode()
+    assert rc not in (0, -2) and "current device" in said, (rc, said)
+
+
+WIDE = 1 << 24          # channels
+
+
+def wide(make, count, length, channels=WIDE, states=None, **changes):
+    rows = {f"{r}__{k}": v for r in (("x", "out") if states is None else ("u", "delta", "z", "out")) for k, v in (("rowStride", channels), ("sequenceStride", channels * length))}
+    if states is not None:
+        rows.update({f"{r}__{k}": v for r in "BC" for k, v in (("rowStride", states), ("sequenceStride", states * length))}, states=states, groups=1)
+    return make(**rows, channels=channels, sequences__count=count, sequences__length=length, sequences__device=78, **changes)
+
+
+def test_launches_of_2_to_the_32_threads_are_refused_before_anything_runs():
+    """The last size that every launch of a call covers, and the first that one of them does not."""
+    lib, size, space = _abi.load(), C.c_size_t(), (C.c_void_p(AT), 1 << 62)
+    many = "more rows than one launch covers"
+    # convolution: four channels a thread, 16 rows; gradients: two, 64 rows
+    reaches_the_device(lib.gennmi_causal_conv(C.byref(wide(conv, 1, 1023 * 16)), None))
+    refused(lib.gennmi_causal_conv(C.byref(wide(conv, 1, 1023 * 16 + 1)), None), -2, many)
+    g = _abi.CausalConvGradient(out=_abi.Rows(AT + 8192, WIDE, 0))
+    reaches_the_device(lib.gennmi_causal_conv_backward(C.byref(wide(conv, 1, 511 * 64)), C.byref(g), None, 0, None))
+    refused(lib.gennmi_causal_conv_backward(C.byref(wide(conv, 1, 511 * 64 + 1)), C.byref(g), None, 0, None), -2, many)
+    # scan: a wavefront for 64 channels of a sequence and 16 states; a token: a lane for four states
+    for count, length, states in ((255, 2, 16), (31, 2, 128), (63, 1, 16), (7, 1, 128)):
+        for more in (0, 1):
+            c = wide(scan, count + more, length, states=states)
+            rc = lib.gennmi_selective_scan(C.byref(c), *space, None)
+            refused(rc, -2, many) if more else reaches_the_device(rc)
+            rc = lib.gennmi_selective_scan_workspace(C.byref(c), C.byref(size))
+            refused(rc, -2, many) if more else None
+            assert more or rc == 0
+    # gradients: the walk over chunks, a wavefront for a state of a sequence; then the sums of B and C, and those over chunks
+    for count, length, channels, states, gradients in (((1 << 22) - 1, 33, 1, 16, {}), (1, 134217720, 1, 16, dict(B=_abi.Rows(AT + (1 << 20), 16, 0))),
+                                                       (1, 2, 64 * 32767, 126, dict(A=AT + (1 << 20)))):
+        g = _abi.ScanGradient(out=_abi.Rows(AT + 4096 * 7, channels, channels * length), **gradients)
+        for more in (0, 1):
+            at = dict(count=count + (more if count > 1 else 0), length=length + (more if length > 100 else 0), channels=channels + (more if channels > 1 else 0), states=states)
+            g.out.rowStride, g.out.sequenceStride = at["channels"], at["channels"] * at["length"]
+            rc = lib.gennmi_selective_scan_backward(C.byref(wide(scan, **at)), C.byref(g), *space, None)
+            refused(rc, -2, many) if more else reaches_the_device(rc)
+    c = wide(scan, 1 << 22, 33, channels=1, states=16)
+    refused(lib.gennmi_selective_scan_backward_workspace(C.byref(c), C.byref(size)), -2, many)
+    # an optimiser: a work-group of 256 threads for 1024 weights
+    o, at = C.c_void_p(), 1 << 50
+    for count, more in ((((1 << 24) - 1) * 1024, False), (((1 << 24) - 1) * 1024 + 1, True)):
+        assert lib.gennmi_optimiser_create(C.byref(o), C.byref(_abi.AdamWSettings(beta1=0.9, beta2=0.99, epsilon=1e-8, stateBits=32))) == 0
+        assert lib.gennmi_optimiser_push(o, C.byref(parameter(weight=at, gradient=2 * at, m=3 * at, v=4 * at, count=count)), None) == 0
+        rc = lib.gennmi_optimiser_finalise(o)
+        refused(rc, -2, "one launch") if more else None
+        assert more or rc != -2
+        lib.gennmi_optimiser_destroy(o)
+
+
 def parameter(**changes):
     p = _abi.Parameter(weight=AT, gradient=AT + 8192, m=AT + 16384, v=AT + 32768, count=100, weightType=F32, gradientType=BF16)
     return changed(p, changes)
