@@ -277,7 +277,12 @@ struct gennmi_optimiser
     ParameterDev *dParameters = nullptr; ChunkDev *dChunks = nullptr; CounterDev *dCounter = nullptr;
     uint32_t numChunks = 0, device = 0;         // device: 1 + the one that was current when the table was uploaded
     bool finalised = false;
-    ~gennmi_optimiser() { (void)gennmi_free(dParameters); (void)gennmi_free(dChunks); (void)gennmi_free(dCounter); }
+    void freeTables()
+    {
+        (void)gennmi_free(dParameters); (void)gennmi_free(dChunks); (void)gennmi_free(dCounter);
+        dParameters = nullptr; dChunks = nullptr; dCounter = nullptr;
+    }
+    ~gennmi_optimiser() { freeTables(); }
 };
 
 extern "C" {
@@ -367,19 +372,19 @@ int gennmi_optimiser_finalise(gennmi_optimiser *optimiser)
             for(uint64_t c = 0; c < of; c++) { chunks.push_back({(uint32_t)k, (uint32_t)c}); }
         }
         if(chunks.empty()) { chunks.push_back({(uint32_t)optimiser->table.size(), 0}); }        // (a step of nothing counts: a tensor without weights)
-        optimiser->table.push_back(ParameterDev{});
-        // (arrays of an earlier attempt that failed half-way are freed with the optimiser)
-        auto upload = [&](auto **to, const auto &from) {
-            if(const int rc = gennmi_malloc((void**)to, from.size() * sizeof(from[0]))) { return rc; }
-            return from.empty() ? (int)GENNMI_OK : gennmi_memcpy_to_device(*to, from.data(), from.size() * sizeof(from[0]));
-        };
-        if(!optimiser->dParameters) { if(const int rc = upload(&optimiser->dParameters, optimiser->table)) { return rc; } }
-        if(!optimiser->dChunks) { if(const int rc = upload(&optimiser->dChunks, chunks)) { return rc; } }
+        std::vector<ParameterDev> table = optimiser->table;
+        table.push_back(ParameterDev{});
         std::vector<CounterDev> counter(1, CounterDev{});
         setCounter(counter[0], optimiser->settings.beta1, optimiser->settings.beta2, 1.0, 1.0, 0);
-        if(!optimiser->dCounter) { if(const int rc = upload(&optimiser->dCounter, counter)) { return rc; } }
-        int device = 0;
-        if(const hipError_t e = hipGetDevice(&device)) { return fail(GENNMI_EHIP, std::string("optimiser_finalise: ") + hipGetErrorString(e)); }
+        const auto upload = [&](auto **to, const auto &from) {
+            if(const int rc = gennmi_malloc((void**)to, from.size() * sizeof(from[0]))) { return rc; }
+            return gennmi_memcpy_to_device(*to, from.data(), from.size() * sizeof(from[0]));
+        };
+        int device = 0, rc = upload(&optimiser->dParameters, table);
+        if(!rc) { rc = upload(&optimiser->dChunks, chunks); }
+        if(!rc) { rc = upload(&optimiser->dCounter, counter); }
+        if(!rc) { if(const hipError_t e = hipGetDevice(&device)) { rc = fail(GENNMI_EHIP, std::string("optimiser_finalise: ") + hipGetErrorString(e)); } }
+        if(rc) { optimiser->freeTables(); return rc; }          // (another attempt begins anew)
         optimiser->device = 1 + (uint32_t)device;
         optimiser->numChunks = (uint32_t)chunks.size();
         optimiser->finalised = true;

@@ -1,6 +1,10 @@
 """Operators on sequences and the optimiser, as far as they go without a GPU: layouts of the descriptors, sizes of workspaces, and what the
 entry points refuse before they touch the device.  Also the 64-bit restatements that the GPU tests compare with, against differences."""
 import ctypes as C
+import json
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -244,6 +248,62 @@ def test_optimiser_refuses_settings_order_and_overlaps():
     refused(lib.gennmi_optimiser_get_step(o, C.byref(n)), -4, "not finalised")
     refused(lib.gennmi_optimiser_set_step(o, 3), -4, "not finalised")
     assert lib.gennmi_optimiser_destroy(o) == 0 and lib.gennmi_optimiser_destroy(None) == 0
+
+
+# The runtime's calls that an optimiser's table takes, on host memory: copy number `failing` (counted from 1) fails
+RUNTIME = r"""
+#include <stdlib.h>
+#include <string.h>
+int failing = 0, copies = 0, live = 0;
+struct { void *ptr; size_t bytes; } block[64];
+int hipMalloc(void **p, size_t n) { *p = calloc(1, n); block[live].ptr = *p; block[live++].bytes = n; return 0; }
+int hipFree(void *p)
+{
+    for(int k = 0; k < live; k++) { if(block[k].ptr == p) { for(live--; k < live; k++) { block[k] = block[k + 1]; } free(p); return 0; } }
+    return p ? 1 : 0;
+}
+int hipMemcpy(void *to, const void *from, size_t n, int kind) { (void)kind; if(++copies == failing) { return 2; } memcpy(to, from, n); return 0; }
+int hipGetDevice(int *device) { *device = 0; return 0; }
+"""
+FINALISE = """
+import ctypes as C, json, sys
+runtime = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+sys.path.insert(0, sys.argv[2])
+from genn_amd import _abi
+lib, said = _abi.load(), []
+for tensors in (2, 0):
+    for failing in range(4):
+        o = C.c_void_p()
+        C.c_int.in_dll(runtime, "copies").value, C.c_int.in_dll(runtime, "failing").value = 0, failing
+        assert lib.gennmi_optimiser_create(C.byref(o), C.byref(_abi.AdamWSettings(beta1=0.9, beta2=0.99, epsilon=1e-8, stateBits=32))) == 0
+        for k in range(tensors):
+            at = (k + 1) << 30
+            p = _abi.Parameter(weight=at, gradient=at + 65536, m=2 * at + (1 << 20), v=at + 262144, count=3000 + k, weightDecay=0.5)
+            assert lib.gennmi_optimiser_push(o, C.byref(p), None) == 0
+        first = lib.gennmi_optimiser_finalise(o)
+        live = C.c_int.in_dll(runtime, "live").value
+        assert (first != 0) == (failing > 0) and (first == 0 or live == 0), (first, live)
+        assert first == 0 or lib.gennmi_optimiser_finalise(o) == 0
+        blocks = (C.c_size_t * 128).in_dll(runtime, "block")
+        said.append([tensors] + [C.string_at(blocks[2 * k], blocks[2 * k + 1]).hex() for k in range(C.c_int.in_dll(runtime, "live").value)])
+        lib.gennmi_optimiser_destroy(o)
+        assert C.c_int.in_dll(runtime, "live").value == 0
+print(json.dumps(said))
+"""
+
+
+def test_a_table_whose_copy_failed_is_made_anew(tmp_path):
+    """Whichever copy of finalise fails, the next attempt uploads what a first one would have, and nothing else is kept."""
+    source, shared = tmp_path / "runtime.c", tmp_path / "runtime.so"
+    source.write_text(RUNTIME)
+    subprocess.check_call(["gcc", "-shared", "-fPIC", "-o", str(shared), str(source)])
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FINALISE, str(shared), root], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr
+    said = json.loads(done.stdout)
+    assert len(said) == 8 and all(len(s) == 4 for s in said)
+    for k in range(8):
+        assert said[k] == said[k // 4 * 4], k
 
 
 def test_python_layer_refuses_before_it_touches_the_device():
