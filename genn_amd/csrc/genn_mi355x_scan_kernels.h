@@ -238,6 +238,15 @@ template<typename T, int R> __device__ inline void gates(const StagedRows<T, R> 
     for(int r = 0; r < R; r++) { const float x = widen(z.raw[r]); gate[r] = x * logistic(x); }
 }
 
+// Whether a lane has an infinite value
+template<int R> __device__ inline bool anyInfinite(const float (&w)[R])
+{
+    float most = 0.0f;
+    #pragma unroll
+    for(int r = 0; r < R; r++) { most = fmaxf(most, fabsf(w[r])); }
+    return __any(most == __builtin_inff());
+}
+
 // First kernel of a split scan: every chunk from a state of zero.  With GRADIENT also sum_t (prod_{s <= t} exp(dt_s A)) C_t g_t, what the chunk's rows
 // give the gradient of the state before it.
 template<typename T, int NP, bool GRADIENT, bool SLABS>
@@ -394,6 +403,9 @@ void scanKernel(ScanArgs a)
     float A[NP], h[NP];
     loadA<NP>(a, s, A);
     if(a.chunkState) { loadChunk<NP>(a, s, a.chunkState, number, h); } else { loadState<NP>(a, s, a.initialState, s.place.state, h); }
+    // States that are not there have decay 1 and B = C = 0, and are 0 for as long as what they are multiplied with is finite
+    #pragma unroll
+    for(int n = 0; n < NP; n++) { h[n] = n < (int)s.numStates ? h[n] : 0.0f; }
     const uint32_t end = s.first + s.rows;
     StagedBC<T, NP, R> stage(B, C, a, s.numStates);
     StagedRows<T, R> rawU, rawDelta, rawZ;
@@ -415,28 +427,50 @@ void scanKernel(ScanArgs a)
         stage.store(bc, row, end);
         waveFence();
         fetch(row + R);         // (behind the last block: its last row, for nothing)
-        float nextB[NP], nextC[NP];
-        #pragma unroll
-        for(int n = 0; n < NP; n++) { nextB[n] = bc[n]; nextC[n] = bc[NP + n]; }
-        #pragma unroll
-        for(int r = 0; r < R; r++) {
-            float Bn[NP], Cn[NP];
+        if(s.numStates < NP && anyInfinite<R>(w)) {
+            // (rare: the states that are there, one row after another)
             #pragma unroll
-            for(int n = 0; n < NP; n++) { Bn[n] = nextB[n]; Cn[n] = nextC[n]; }
-            if(r + 1 < R) {
-                // (a row's inputs are read while the row before is worked on, and no sooner)
-                readAfter<NP>(h);
-                if(r) { readAfter(y[r - 1], h[0], h[1], h[2]); }
+            for(int r = 0; r < R; r++) { y[r] = 0.0f; }
+            #pragma nounroll
+            for(int r = 0; r < R; r++) {
+                float time = 0.0f, in = 0.0f, y0 = 0.0f, y1 = 0.0f;
                 #pragma unroll
-                for(int n = 0; n < NP; n++) { nextB[n] = bc[(r + 1) * 2 * NP + n]; nextC[n] = bc[((r + 1) * 2 + 1) * NP + n]; }
+                for(int k = 0; k < R; k++) { time = k == r ? dt[k] : time; in = k == r ? w[k] : in; y0 = k == r && !SLABS ? direct[k] : y0; }
+                #pragma unroll
+                for(int n = 0; n < NP; n++) {
+                    if(n >= (int)s.numStates) { break; }
+                    h[n] = __builtin_fmaf(exp2Of(time * A[n]), h[n], in * bc[r * 2 * NP + n]);
+                    const float c = bc[(r * 2 + 1) * NP + n];
+                    if(n & 1) { y1 = __builtin_fmaf(h[n], c, y1); } else { y0 = __builtin_fmaf(h[n], c, y0); }
+                }
+                #pragma unroll
+                for(int k = 0; k < R; k++) { y[k] = k == r ? y0 + y1 : y[k]; }
             }
-            float y0 = SLABS ? 0.0f : direct[r], y1 = 0.0f;
+        }
+        else {
+            float nextB[NP], nextC[NP];
             #pragma unroll
-            for(int n = 0; n < NP; n++) {
-                h[n] = __builtin_fmaf(exp2Of(dt[r] * A[n]), h[n], w[r] * Bn[n]);
-                if(n & 1) { y1 = __builtin_fmaf(h[n], Cn[n], y1); } else { y0 = __builtin_fmaf(h[n], Cn[n], y0); }
+            for(int n = 0; n < NP; n++) { nextB[n] = bc[n]; nextC[n] = bc[NP + n]; }
+            #pragma unroll
+            for(int r = 0; r < R; r++) {
+                float Bn[NP], Cn[NP];
+                #pragma unroll
+                for(int n = 0; n < NP; n++) { Bn[n] = nextB[n]; Cn[n] = nextC[n]; }
+                if(r + 1 < R) {
+                    // (a row's inputs are read while the row before is worked on, and no sooner)
+                    readAfter<NP>(h);
+                    if(r) { readAfter(y[r - 1], h[0], h[1], h[2]); }
+                    #pragma unroll
+                    for(int n = 0; n < NP; n++) { nextB[n] = bc[(r + 1) * 2 * NP + n]; nextC[n] = bc[((r + 1) * 2 + 1) * NP + n]; }
+                }
+                float y0 = SLABS ? 0.0f : direct[r], y1 = 0.0f;
+                #pragma unroll
+                for(int n = 0; n < NP; n++) {
+                    h[n] = __builtin_fmaf(exp2Of(dt[r] * A[n]), h[n], w[r] * Bn[n]);
+                    if(n & 1) { y1 = __builtin_fmaf(h[n], Cn[n], y1); } else { y0 = __builtin_fmaf(h[n], Cn[n], y0); }
+                }
+                y[r] = y0 + y1;
             }
-            y[r] = y0 + y1;
         }
         if(SLABS) {
             #pragma unroll
@@ -503,7 +537,8 @@ void scanTokenKernel(ScanArgs a)
         const float u = widen(rowsOf<const T>(a.u, a.sequences, p)[channel]), z = a.z.data ? widen(rowsOf<const T>(a.z, a.sequences, p)[channel]) : 0.0f;
         float time = widen(rowsOf<const T>(a.delta, a.sequences, p)[channel]) + (a.deltaBias ? a.deltaBias[channel] : 0.0f);
         if(a.softplus) { time = softplusOf(time); }
-        const float w = time * u;
+        float w = time * u;
+        if(!here) { time = w = 0.0f; }          // (what is infinite, times nothing)
         #pragma unroll
         for(int k = 0; k < 4; k++) {
             if(QUADS || n0 + k < a.states) {
@@ -511,7 +546,7 @@ void scanTokenKernel(ScanArgs a)
                 y = __builtin_fmaf(h[k], C[k], y);
             }
         }
-        // (lanes behind the last state have zeros)
+        // (lanes behind the last state have added zeros)
         if constexpr(LANES > 1) { y += gennmi_lanes::partner<1>(y); }
         if constexpr(LANES > 2) { y += gennmi_lanes::partner<2>(y); }
         if constexpr(LANES > 4) { y += gennmi_lanes::partner<4>(y); }

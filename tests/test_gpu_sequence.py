@@ -304,6 +304,32 @@ def test_what_is_not_finite_stays_where_it_belongs():
     assert torch.all(final[0, 0::2] == 1.0) and torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("length", [1, 30, 500])
+@pytest.mark.parametrize("states", [1, 5, 8, 11, 20, 40])
+def test_what_is_infinite_stays_infinite(states, length):
+    """An infinite input or state gives the infinities of the formula, whatever the number of states (a wavefront has registers for 8 or 16 of them)."""
+    from genn_amd.sequence import SelectiveScan
+    r, D, N = generator(states + length), 70, states
+    u, delta, B, C = r(length, D), torch.rand(length, D) * 0.02 + 0.01, torch.rand(length, N) + 0.1, torch.rand(length, N) + 0.1
+    A, initial = -torch.rand(D, N), r(D, N)
+    u[min(12, length - 1), 3], u[0, 65], delta[length // 2, 68], u[length // 2, 68] = float("inf"), float("-inf"), float("inf"), 1.0
+    initial[7, 0], initial[9, N - 1] = float("inf"), float("-inf")
+    out, final = torch.empty(length, D).cuda(), torch.empty(1, D, N).cuda()
+    s = SelectiveScan(1, length, D, N)
+    s.bind(u=u.cuda(), delta=delta.cuda(), A=A.cuda(), B=B.cuda(), C=C.cuda(), D=torch.ones(D).cuda(), out=out, initial_state=initial.cuda().view(1, D, N), final_state=final)
+    s.run()
+    torch.cuda.synchronize()
+    args = dict(u=u, delta=delta, A=A, B=B.view(length, 1, N), C=C.view(length, 1, N), D=torch.ones(D), initial=initial)
+    want = ref.scan(**args)
+    sizes = ref.scan(magnitudes=True, **args)
+    assert torch.isinf(want[0][-1, [3, 7, 9, 65, 68]]).all() and torch.isfinite(want[0][:, 10:60]).all()
+    for got, w, size in ((out, want[0], sizes[0]), (final[0], want[1], sizes[1])):
+        got, odd = got.cpu().double(), ~torch.isfinite(w)
+        assert torch.allclose(got[odd], w[odd], rtol=0, atol=0, equal_nan=True)
+        assert torch.isfinite(got[~odd]).all()
+        close("finite ones", got[~odd], w[~odd], size[~odd], 2 * length + N + 12)
+
+
 @pytest.mark.parametrize("sequences, length", [(0, 5), (3, 0)])
 def test_nothing_to_do_leaves_states_and_gives_zero_gradients(sequences, length):
     from genn_amd.sequence import CausalConvolution, SelectiveScan
