@@ -421,7 +421,7 @@ void scanKernel(ScanArgs a)
         float dt[R], w[R], y[R], gate[R], direct[R];
         times<T, R>(a, rawDelta, rawU, bias, end - row, dt, w);
         #pragma unroll
-        for(int r = 0; r < R; r++) { direct[r] = skip * widen(rawU.raw[r]); gate[r] = 1.0f; }
+        for(int r = 0; r < R; r++) { direct[r] = a.D ? skip * widen(rawU.raw[r]) : 0.0f; gate[r] = 1.0f; }
         if(z) { gates<T, R>(rawZ, gate); }
         waveFence();
         stage.store(bc, row, end);

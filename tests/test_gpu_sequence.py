@@ -330,6 +330,27 @@ def test_what_is_infinite_stays_infinite(states, length):
         close("finite ones", got[~odd], w[~odd], size[~odd], 2 * length + N + 12)
 
 
+@pytest.mark.parametrize("length", [1, 30, 500])
+@pytest.mark.parametrize("states", [8, 20])
+def test_an_infinite_input_without_a_direct_path(states, length):
+    """Without D the outputs have no share of u but by the states, which are infinite from there on."""
+    from genn_amd.sequence import SelectiveScan
+    r, D, N = generator(states + length), 70, states
+    u, delta, B, C = r(length, D), torch.rand(length, D) * 0.02 + 0.01, torch.rand(length, N) + 0.1, torch.rand(length, N) + 0.1
+    A = -torch.rand(D, N)
+    at = min(12, length - 1)
+    u[at, 3], u[at, 66] = float("inf"), float("-inf")
+    out = torch.empty(length, D).cuda()
+    s = SelectiveScan(1, length, D, N)
+    s.bind(u=u.cuda(), delta=delta.cuda(), A=A.cuda(), B=B.cuda(), C=C.cuda(), out=out)
+    s.run()
+    torch.cuda.synchronize()
+    got = out.cpu()
+    assert torch.all(got[at:, 3] == float("inf")) and torch.all(got[at:, 66] == float("-inf"))
+    got[at:, [3, 66]] = 0.0
+    assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("sequences, length", [(0, 5), (3, 0)])
 def test_nothing_to_do_leaves_states_and_gives_zero_gradients(sequences, length):
     from genn_amd.sequence import CausalConvolution, SelectiveScan
