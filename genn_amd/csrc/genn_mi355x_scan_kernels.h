@@ -347,8 +347,11 @@ template<bool BACKWARDS> __device__ inline float walkChunks(float *state, uint64
         for(uint32_t k = 0; k < AHEAD; k++) {
             if(first + k < chunks) {
                 state[chunk(first + k) * stride] = h;
-                // (where A is positive a chunk's decay may be infinite: of nothing, nothing is left all the same)
-                h = h == 0.0f ? adds[k] : __builtin_fmaf(exp2Of(times[k] * A), h, adds[k]);
+                // A chunk's decay may be infinite, where A is positive (of nothing, nothing is left all the same), or less than there is in 32 bits: it is
+                // the smallest positive value then, which no finite state can tell from nothing, and which leaves an infinite one as it is
+                // (nothing known of A or dt makes what the chunk adds unknown, if it has a row)
+                const float decay = fmaxf(exp2Of(times[k] * A), 0x1p-149f);
+                h = h == 0.0f ? adds[k] : __builtin_fmaf(decay, h, adds[k]);
             }
             adds[k] = nextAdds[k];
             times[k] = nextTimes[k];

@@ -351,6 +351,26 @@ def test_an_infinite_input_without_a_direct_path(states, length):
     assert torch.isfinite(got).all()
 
 
+def test_an_infinite_state_outlasts_decays_that_round_to_zero():
+    """A row's decay is e^-16, that of a chunk of rows is none in 32 bits: what is infinite stays so row by row, and over chunks."""
+    from genn_amd.sequence import SelectiveScan
+    n, D, N = 600, 64, 16
+    initial = torch.ones(1, D, N)
+    initial[0, 5, 3], initial[0, 6, 0] = float("inf"), float("-inf")
+    one = lambda *shape: torch.ones(*shape).cuda()
+    out, final = torch.empty(1, n, D).cuda(), torch.empty(1, D, N).cuda()
+    s = SelectiveScan(1, n, D, N)
+    s.bind(u=one(1, n, D), delta=one(1, n, D), A=-16 * one(D, N), B=one(1, n, N), C=one(1, n, N), out=out, initial_state=initial.cuda(), final_state=final)
+    assert s.workspace_bytes > 0            # (in chunks)
+    s.run()
+    torch.cuda.synchronize()
+    out, final = out[0].cpu(), final[0].cpu()
+    assert torch.all(out[:, 5] == float("inf")) and torch.all(out[:, 6] == float("-inf"))
+    assert final[5, 3] == float("inf") and final[6, 0] == float("-inf")
+    out[:, 5:7], final[5, 3], final[6, 0] = 0.0, 0.0, 0.0
+    assert torch.isfinite(out).all() and torch.isfinite(final).all()
+
+
 @pytest.mark.parametrize("sequences, length", [(0, 5), (3, 0)])
 def test_nothing_to_do_leaves_states_and_gives_zero_gradients(sequences, length):
     from genn_amd.sequence import CausalConvolution, SelectiveScan
