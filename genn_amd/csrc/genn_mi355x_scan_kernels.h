@@ -162,11 +162,18 @@ template<int NP> __device__ inline bool inFours(const ScanArgs &a, const ScanPla
 {
     return s.numStates == NP && a.states % 4 == 0 && (uint64_t)states % 16 == 0;
 }
+// What exp2 takes of A.  An infinite one (a unit that forgets everything) as the largest number: no time at all, which rows behind the end and sequences without
+// rows take, is not to change a state, and any other is the same.
+__device__ inline float exponentOf(float A)
+{
+    const float x = A * LOG2E;
+    return fabsf(x) == __builtin_inff() ? __builtin_copysignf(3.402823466e38f, x) : x;
+}
 template<int NP> __device__ inline void loadA(const ScanArgs &a, const ScanPlace &s, float (&A)[NP])
 {
     loadNeighbours<NP>(a.A + (uint64_t)s.channel * a.states + s.firstState, s.numStates, inFours<NP>(a, s, a.A), A);
     #pragma unroll
-    for(int n = 0; n < NP; n++) { A[n] = n < (int)s.numStates ? A[n] * LOG2E : 0.0f; }
+    for(int n = 0; n < NP; n++) { A[n] = n < (int)s.numStates ? exponentOf(A[n]) : 0.0f; }
 }
 template<int NP> __device__ inline void loadState(const ScanArgs &a, const ScanPlace &s, const float *state, uint64_t which, float (&h)[NP])
 {
@@ -373,7 +380,7 @@ void scanJoinKernel(ScanArgs a, ScanGradientArgs g)
     if(!describe(a.sequences, sequence, p) || channel >= a.channels) { return; }
     const uint64_t chunk0 = firstChunk(a.sequences, sequence), stride = (uint64_t)a.states * a.channels;
     const uint32_t chunks = max(1u, (uint32_t)(((uint64_t)p.length + a.sequences.chunk - 1) / a.sequences.chunk));
-    const float A = a.A[(uint64_t)channel * a.states + n] * LOG2E;
+    const float A = exponentOf(a.A[(uint64_t)channel * a.states + n]);
     const uint64_t at = ((uint64_t)p.state * a.channels + channel) * a.states + n, first = (chunk0 * a.states + n) * a.channels + channel;
     const float *time = a.chunkTime + chunk0 * a.channels + channel;
     const float h = walkChunks<false>(a.chunkState + first, stride, time, a.channels, chunks, A, a.initialState ? a.initialState[at] : 0.0f);

@@ -371,6 +371,39 @@ def test_an_infinite_state_outlasts_decays_that_round_to_zero():
     assert torch.isfinite(out).all() and torch.isfinite(final).all()
 
 
+@pytest.mark.parametrize("lengths", [[5], [0, 13, 0], [0, 500, 3, 0]])
+def test_units_that_forget_everything(lengths):
+    """A = -infinity: a row's state is what comes in with it; sequences without rows keep theirs.  Also one whose product with log2(e) is infinite."""
+    from genn_amd.sequence import SelectiveScan
+    S, D, N = len(lengths), 20, 5
+    parts, offsets = split(lengths)
+    rows, r = sum(lengths), generator(sum(lengths))
+    u, delta, B, C, dout = r(rows, D), torch.rand(rows, D) + 0.1, r(rows, N), r(rows, N), r(rows, D)
+    A, initial, dfinal = -torch.rand(D, N), r(S, D, N), r(S, D, N)
+    A[3], A[7, 2], A[11, 4] = float("-inf"), float("-inf"), -3e38
+    grads = {k: torch.empty(rows, w).cuda() for k, w in (("u", D), ("B", N), ("C", N))}
+    grads.update(A=torch.empty(D, N).cuda(), initial_state=torch.empty(S, D, N).cuda())
+    out, final = torch.empty(rows, D).cuda(), torch.empty(S, D, N).cuda()
+    s = SelectiveScan(S, max(lengths), D, N)
+    s.bind(u=u.cuda(), delta=delta.cuda(), A=A.cuda(), B=B.cuda(), C=C.cuda(), out=out, initial_state=initial.cuda(), final_state=final, offsets=offsets)
+    s.run()
+    s.bind_gradients(out=dout.cuda(), final_state=dfinal.cuda(), **grads)
+    s.backward()
+    torch.cuda.synchronize()
+    dA, sizeA = 0, 0
+    for k, p in enumerate(parts):
+        args = dict(u=u[p], delta=delta[p], A=A, B=B[p].view(-1, 1, N), C=C[p].view(-1, 1, N), initial=initial[k])
+        want, size = (ref.scan(magnitudes=m, **args) for m in (False, True))
+        close(f"out of {k}", out[p], want[0], size[0], 2 * lengths[k] + N + 12)
+        close(f"final state of {k}", final[k], want[1], size[1], 2 * lengths[k] + N + 12)
+        want, size = (ref.scan(magnitudes=m, dout=dout[p], dfinal=dfinal[k], **args) for m in (False, True))
+        for name in ("u", "B", "C"):
+            close(f"d{name} of {k}", grads[name][p], want[name].reshape(-1, grads[name].shape[1]), size[name].reshape(-1, grads[name].shape[1]), 4 * lengths[k] + N + 48)
+        close(f"dinitial of {k}", grads["initial_state"][k], want["initial_state"], size["initial_state"], 4 * lengths[k] + N + 40)
+        dA, sizeA = dA + want["A"], sizeA + size["A"]
+    close("dA", grads["A"], dA, sizeA, 4 * max(lengths) + N + 80)
+
+
 @pytest.mark.parametrize("sequences, length", [(0, 5), (3, 0)])
 def test_nothing_to_do_leaves_states_and_gives_zero_gradients(sequences, length):
     from genn_amd.sequence import CausalConvolution, SelectiveScan
