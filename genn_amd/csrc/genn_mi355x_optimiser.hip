@@ -218,8 +218,9 @@ void adamwKernel(StepArgs a)
                 highV[i] = root * ABOVE;
             }
             uint32_t codesM = encode(lowM), codesV = encode(lowV);
-            // (nor do quotients of 32 bits do where the largest of a block are so small that inverses or others' are subnormal)
-            const bool near = codesM != encode(highM) || codesV != encode(highV) || (M > 0.0f && M < 1e-25f) || (V > 0.0f && V < 1e-25f);
+            // (nor do quotients of 32 bits do where the largest of a block are so small that inverses or others' are subnormal, or so large that their inverses are)
+            const auto extreme = [](float most) { return (most > 0.0f && most < 1e-25f) || (most > 0x1p125f && most < __builtin_inff()); };
+            const bool near = codesM != encode(highM) || codesV != encode(highV) || extreme(M) || extreme(V);
             if(__ballot(near)) {
                 #pragma unroll
                 for(int i = 0; i < 4; i++) {

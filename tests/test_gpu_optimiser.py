@@ -134,6 +134,28 @@ def test_a_positive_second_moment_never_becomes_zero():
     assert float(w.abs().max()) < 0.02
 
 
+@pytest.mark.parametrize("largest", [1e-20, 1.0, 1e15, 3e19, 5e19, 8e19])
+def test_codes_of_any_size(largest):
+    """Codes do not depend on how large a block's gradients are, up to second moments (here 3.2e38) at the end of fp32's range."""
+    gen = torch.Generator().manual_seed(4)
+    g = torch.rand(512, generator=gen) * largest
+    g[100], g[300] = largest, largest
+    # (first moments of up to 3e38 as well, from a state that was that large)
+    codes, scale = torch.full((512,), 126, dtype=torch.uint8).cuda(), torch.tensor([1.0, 3e38]).cuda()
+    w, m, v, V = torch.zeros(512).cuda(), torch.zeros(512, dtype=torch.uint8).cuda(), torch.zeros(512, dtype=torch.uint8).cuda(), torch.zeros(2).cuda()
+    other, zero = torch.zeros(512).cuda(), torch.zeros(512).cuda()
+    opt = AdamW(beta1=0.9, beta2=0.95, epsilon=EPS, state_bits=8)
+    opt.add(w, g.cuda(), m=m, v=v, m_scale=torch.zeros(2).cuda(), v_scale=V)
+    opt.add(other, zero, m=codes, v=torch.zeros(512, dtype=torch.uint8).cuda(), m_scale=scale, v_scale=torch.zeros(2).cuda())
+    opt.build()
+    opt.step()
+    torch.cuda.synchronize()
+    second = (1 - 0.95) * g.double() ** 2
+    scales_close("scale of v", V, second.view(2, 256).amax(1))
+    codes_close("v", v.cpu(), torch.sqrt(second / V.cpu().double().repeat_interleave(256)) * 448)
+    assert torch.all(codes == 126)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_what_is_not_finite_stays_in_its_block(bits):
     gen = torch.Generator().manual_seed(1)
