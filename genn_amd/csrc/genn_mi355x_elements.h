@@ -6,7 +6,9 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
+#include <utility>
 
 #include "genn_mi355x.h"
 
@@ -179,6 +181,92 @@ inline int checkWrittenRows(const char *what, const char *which, const gennmi_ro
     if(const int rc = checkRows(what, which, r, s, width, size)) { return rc; }
     const bool overlap = s.count > 1 && (s.offsets ? r.rowStride < width : r.sequenceStride < width);
     return overlap ? gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": " + which + ": sequences overlap") : GENNMI_OK;
+}
+
+// What a call reads or writes, in bytes: `outer` times `inner` runs of `width`, the larger of the strides outside
+struct Region
+{
+    const char *name;
+    int64_t begin, end;             // of all of it; nothing: both 0
+    int64_t width, inner, innerStride, outer, outerStride;
+};
+inline Region regionOf(const char *name, const void *data, uint64_t width, uint64_t inner = 1, uint64_t innerStride = 0, uint64_t outer = 1, uint64_t outerStride = 0)
+{
+    if(innerStride > outerStride) { std::swap(inner, outer); std::swap(innerStride, outerStride); }
+    if(innerStride == 0) { inner = std::min<uint64_t>(inner, 1); }
+    if(outerStride == 0) { outer = std::min<uint64_t>(outer, 1); }
+    const unsigned __int128 bytes = (unsigned __int128)(inner - 1) * innerStride + (unsigned __int128)(outer - 1) * outerStride + width;
+    // (what no address space holds is none of this check's business)
+    if(!data || !width || !inner || !outer || bytes > (1ull << 60)) { return Region{name, 0, 0, 0, 0, 0, 0, 0}; }
+    return Region{name, (int64_t)(uintptr_t)data, (int64_t)(uintptr_t)data + (int64_t)bytes, (int64_t)width, (int64_t)inner, (int64_t)innerStride, (int64_t)outer, (int64_t)outerStride};
+}
+inline Region regionOf(const char *name, const gennmi_rows_t &r, const gennmi_sequences_t &s, uint64_t width, uint32_t size)
+{
+    if(s.offsets) { return regionOf(name, r.data, width * size, s.rows, r.rowStride * size); }
+    return regionOf(name, r.data, width * size, s.length, r.rowStride * size, s.count, r.sequenceStride * size);
+}
+inline int64_t floorOf(int64_t a, int64_t by) { return a / by - (a % by < 0); }
+// Whether a run of r's lies in part in low .. high - 1
+inline bool meets(const Region &r, int64_t low, int64_t high)
+{
+    const int64_t run = (r.inner - 1) * r.innerStride + r.width;
+    low -= r.begin;
+    high -= r.begin;
+    const int64_t first = r.outerStride ? std::max<int64_t>(0, floorOf(low - run, r.outerStride) + 1) : 0;
+    const int64_t last = r.outerStride ? std::min(r.outer - 1, floorOf(high - 1, r.outerStride)) : 0;
+    for(int64_t o = first; o <= last; o++) {
+        const int64_t from = low - o * r.outerStride, to = high - o * r.outerStride;
+        const int64_t i = r.innerStride ? std::max<int64_t>(0, floorOf(from - r.width, r.innerStride) + 1) : 0;
+        if(i < r.inner && i * r.innerStride < to && i * r.innerStride + r.width > from) { return true; }
+    }
+    return false;
+}
+// The places of r's runs, seen from each other
+inline Region differences(const Region &r, int64_t outerFrom, int64_t outerTo)
+{
+    Region d = r;
+    d.begin = outerFrom * r.outerStride - (r.inner - 1) * r.innerStride;
+    d.inner = 2 * r.inner - 1;
+    d.outer = outerTo - outerFrom + 1;
+    return d;
+}
+inline bool overlap(const Region &a, const Region &b)
+{
+    if(a.begin >= b.end || b.begin >= a.end) { return false; }
+    if(a.inner == b.inner && a.outer == b.outer && a.innerStride == b.innerStride && a.outerStride == b.outerStride) {
+        const Region d = differences(b, 1 - b.outer, b.outer - 1);
+        return meets(d, a.begin - b.begin, a.begin - b.begin + a.width);
+    }
+    // (one array's rows between another's that are not as far apart: looked at one by one)
+    const Region &few = a.inner * a.outer <= b.inner * b.outer ? a : b, &many = &few == &a ? b : a;
+    for(int64_t o = 0; o < few.outer; o++) {
+        for(int64_t i = 0; i < few.inner; i++) {
+            const int64_t at = few.begin + o * few.outerStride + i * few.innerStride;
+            if(meets(many, at, at + few.width)) { return true; }
+        }
+    }
+    return false;
+}
+// Runs of one array that overlap each other
+inline bool overlapsItself(const Region &r)
+{
+    if(r.inner > 1 && r.innerStride < r.width) { return true; }
+    return r.outer > 1 && meets(differences(r, 1, r.outer - 1), 0, r.width);
+}
+// Work-groups do not wait for one another: what a call writes is nothing else that it reads or writes.  `last`: written when everything has been read.
+inline int checkApart(const char *what, std::initializer_list<Region> written, std::initializer_list<Region> last, std::initializer_list<Region> read)
+{
+    const auto refuse = [&](const Region &a, const char *why, const char *other) { return gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": " + a.name + why + other); };
+    for(const Region *w = written.begin(); w != written.end(); w++) {
+        if(overlapsItself(*w)) { return refuse(*w, ": sequences overlap", ""); }
+        for(const Region *x = w + 1; x != written.end(); x++) { if(overlap(*w, *x)) { return refuse(*w, " overlaps ", x->name); } }
+        for(const Region &x : read) { if(overlap(*w, x)) { return refuse(*w, " overlaps ", x.name); } }
+    }
+    for(const Region *l = last.begin(); l != last.end(); l++) {
+        for(const Region *x = l + 1; x != last.end(); x++) { if(overlap(*l, *x)) { return refuse(*l, " overlaps ", x->name); } }
+        for(const Region &x : written) { if(overlap(*l, x)) { return refuse(*l, " overlaps ", x.name); } }
+    }
+    return GENNMI_OK;
 }
 inline void noteRows(const gennmi_rows_t &r, const gennmi_sequences_t &s, uint32_t width, uint32_t size)
 {

@@ -93,6 +93,31 @@ int checkConv(const char *what, const gennmi_causal_conv_t *c, bool gradients)
     if((uintptr_t)c->initialState % size || (uintptr_t)c->finalState % size) { return refuse(GENNMI_EINVAL, ": a state is not aligned to its elements"); }
     return GENNMI_OK;
 }
+Region offsetsOf(const gennmi_sequences_t &s) { return regionOf("offsets", s.offsets, (s.count + 1ull) * 4); }
+Region slotsOf(const gennmi_sequences_t &s) { return regionOf("slots", s.slots, s.count * 4ull); }
+// An array that a call may write in place of the one it reads
+Region unlessSame(const Region &r, const void *written) { return (uintptr_t)written == (uintptr_t)r.begin ? Region{r.name, 0, 0, 0, 0, 0, 0, 0} : r; }
+int convApart(const char *what, const gennmi_causal_conv_t &c)
+{
+    const gennmi_sequences_t &s = c.sequences;
+    const uint32_t size = sizeOf(c.type);
+    const uint64_t states = statesOf(s) * (c.taps - 1) * c.channels * size, channels = c.channels * 4ull;
+    return checkApart(what, {regionOf("out", c.out, s, c.channels, size), regionOf("the final state", c.finalState, states)}, {},
+                      {regionOf("x", c.x, s, c.channels, size), regionOf("weight", c.weight, channels * c.taps), regionOf("bias", c.bias, channels),
+                       unlessSame(regionOf("the initial state", c.initialState, states), c.finalState), offsetsOf(s), slotsOf(s)});
+}
+int convApart(const char *what, const gennmi_causal_conv_t &c, const gennmi_causal_conv_gradient_t &g, const void *workspace, size_t workspaceBytes)
+{
+    const gennmi_sequences_t &s = c.sequences;
+    const uint32_t size = sizeOf(c.type);
+    const uint64_t states = statesOf(s) * (c.taps - 1) * c.channels * size, channels = c.channels * 4ull;
+    return checkApart(what, {regionOf("the gradient of x", g.x, s, c.channels, size), regionOf("the gradient of the initial state", g.initialState, states),
+                             regionOf("the workspace", workspace, workspaceBytes)},
+                      {regionOf("the gradient of weight", g.weight, channels * c.taps), regionOf("the gradient of bias", g.bias, channels)},
+                      {regionOf("x", c.x, s, c.channels, size), regionOf("the gradient of out", g.out, s, c.channels, size), regionOf("weight", c.weight, channels * c.taps),
+                       regionOf("bias", c.bias, channels), unlessSame(regionOf("the initial state", c.initialState, states), g.initialState),
+                       regionOf("the gradient of the final state", g.finalState, states), offsetsOf(s)});
+}
 // Channels of a thread: four, for gradients two, where every row and state of them is one aligned access, else one.  (Gradients keep four rows of
 // taps a channel in registers: with four channels a thread two wavefronts fit a SIMD, and 8 x 2048 rows of 2048 channels take 67 us instead of 60.)
 uint32_t convVector(const gennmi_causal_conv_t &c, const gennmi_causal_conv_gradient_t *g)
@@ -190,6 +215,31 @@ int checkScan(const char *what, const gennmi_scan_t *c, bool gradients)
         if((uintptr_t)p % 4) { return refuse(GENNMI_EINVAL, ": an array of fp32 is not aligned"); }
     }
     return GENNMI_OK;
+}
+
+int scanApart(const char *what, const gennmi_scan_t &c, const void *workspace, size_t workspaceBytes)
+{
+    const gennmi_sequences_t &s = c.sequences;
+    const uint32_t size = sizeOf(c.type), width = c.groups * c.states;
+    const uint64_t channels = c.channels * 4ull, states = statesOf(s) * channels * c.states;
+    return checkApart(what, {regionOf("out", c.out, s, c.channels, size), regionOf("the final state", c.finalState, states), regionOf("the workspace", workspace, workspaceBytes)}, {},
+                      {regionOf("u", c.u, s, c.channels, size), regionOf("delta", c.delta, s, c.channels, size), regionOf("z", c.z, s, c.channels, size), regionOf("B", c.B, s, width, size),
+                       regionOf("C", c.C, s, width, size), regionOf("A", c.A, channels * c.states), regionOf("D", c.D, channels), regionOf("delta's bias", c.deltaBias, channels),
+                       unlessSame(regionOf("the initial state", c.initialState, states), c.finalState), offsetsOf(s), slotsOf(s)});
+}
+int scanApart(const char *what, const gennmi_scan_t &c, const gennmi_scan_gradient_t &g, const void *workspace, size_t workspaceBytes)
+{
+    const gennmi_sequences_t &s = c.sequences;
+    const uint32_t size = sizeOf(c.type), width = c.groups * c.states;
+    const uint64_t channels = c.channels * 4ull, states = statesOf(s) * channels * c.states;
+    return checkApart(what, {regionOf("the gradient of u", g.u, s, c.channels, size), regionOf("the gradient of delta", g.delta, s, c.channels, size),
+                             regionOf("the gradient of z", g.z, s, c.channels, size), regionOf("the gradient of B", g.B, s, width, size), regionOf("the gradient of C", g.C, s, width, size),
+                             regionOf("the gradient of the initial state", g.initialState, states), regionOf("the workspace", workspace, workspaceBytes)},
+                      {regionOf("the gradient of A", g.A, channels * c.states), regionOf("the gradient of D", g.D, channels), regionOf("the gradient of delta's bias", g.deltaBias, channels)},
+                      {regionOf("u", c.u, s, c.channels, size), regionOf("delta", c.delta, s, c.channels, size), regionOf("z", c.z, s, c.channels, size), regionOf("B", c.B, s, width, size),
+                       regionOf("C", c.C, s, width, size), regionOf("the gradient of out", g.out, s, c.channels, size), regionOf("A", c.A, channels * c.states), regionOf("D", c.D, channels),
+                       regionOf("delta's bias", c.deltaBias, channels), unlessSame(regionOf("the initial state", c.initialState, states), g.initialState),
+                       unlessSame(regionOf("the gradient of the final state", g.finalState, states), g.initialState), offsetsOf(s)});
 }
 
 struct ScanPlan { uint32_t slab, slabs, chunk; bool split; };
@@ -360,6 +410,7 @@ int gennmi_causal_conv(const gennmi_causal_conv_t *conv, void *stream)
         if(const int rc = checkConv("causal_conv", conv, false)) { return rc; }
         const uint32_t vector = convVector(*conv, nullptr);
         if(convBlocks(*conv, vector, convChunk(*conv, false)) > mostBlocks(256)) { return tooMany("causal_conv"); }
+        if(const int rc = convApart("causal_conv", *conv)) { return rc; }
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, conv->sequences.device)) { return rc; }
         if(const int rc = runConv("causal_conv", *conv, vector, nullptr, (hipStream_t)stream)) { return rc; }
         const uint32_t size = sizeOf(conv->type);
@@ -400,7 +451,9 @@ int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_c
         const bool sums = g.weight || g.bias;
         const uint32_t vector = convVector(*conv, gradient);
         if(convBlocks(*conv, vector, convChunk(*conv, true)) > mostBlocks(256) || (sums && chunkSumBlocks(conv->taps + 1, conv->channels) > mostBlocks(1024))) { return tooMany(what); }
-        if(const int rc = checkWorkspace(what, workspace, workspaceBytes, sums ? convWorkspace(*conv) : 0)) { return rc; }
+        const size_t need = sums ? convWorkspace(*conv) : 0;
+        if(const int rc = checkWorkspace(what, workspace, workspaceBytes, need)) { return rc; }
+        if(const int rc = convApart(what, *conv, g, workspace, need)) { return rc; }
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, conv->sequences.device)) { return rc; }
         ConvGradientArgs a{};
         a.out = g.out;
@@ -442,6 +495,7 @@ int gennmi_selective_scan(const gennmi_scan_t *scan, void *workspace, size_t wor
         if(!scanFits(*scan, p, false)) { return tooMany(what); }
         const ScanSpace space = scanSpace(*scan, p, false);
         if(const int rc = checkWorkspace(what, workspace, workspaceBytes, space.bytes)) { return rc; }
+        if(const int rc = scanApart(what, *scan, workspace, space.bytes)) { return rc; }
         ScanArgs a = scanArgs(*scan, p);
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, scan->sequences.device)) { return rc; }
         if(!scan->sequences.count) { return (int)GENNMI_OK; }
@@ -514,6 +568,7 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
         if(!scanFits(*scan, p, true) || rowSumBlocks > mostBlocks(256) || sumBlocks > mostBlocks(1024)) { return tooMany(what); }
         const ScanSpace space = scanSpace(*scan, p, true);
         if(const int rc = checkWorkspace(what, workspace, workspaceBytes, space.bytes)) { return rc; }
+        if(const int rc = scanApart(what, *scan, in, workspace, space.bytes)) { return rc; }
         ScanArgs a = scanArgs(*scan, p);
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, scan->sequences.device)) { return rc; }
         auto at = [&](size_t offset) { return (float*)((char*)workspace + offset); };

@@ -582,6 +582,8 @@ int gennmi_program_get_info(gennmi_program *program, unsigned long long info[4])
  * runner make the call fail with GENNMI_ESTATE (run gennmi_flush before); the runners do not hear of what a replay wrote
  * (call gennmi_note_device_write).  A workspace belongs to the call until the call has finished on its stream: calls that may
  * run at the same time, and captured graphs that may, need a workspace each.  No result is a sum of atomics: the same call gives the same bits.
+ * What a call writes shares no memory with anything else that it reads or writes (GENNMI_EINVAL, also where arrays overlap in part; rows of several arrays
+ * may lie side by side, and sums for weights may be written over the weights), but for states: see finalState and the gradients' initialState.
  * A launch has fewer than 2^32 threads: what would take more (2^30 channels of tokens in all at 16 states, say) is refused with GENNMI_EINVAL before
  * anything runs.
  * ------------------------------------------------------------------------------------------- */
@@ -624,7 +626,7 @@ typedef struct gennmi_causal_conv_t {
 typedef struct gennmi_causal_conv_gradient_t {      /* `out` and `finalState` come in, the others go out (any may be NULL) and are overwritten */
     gennmi_rows_t out, x;
     const void *finalState;               /* gradient of the final state, or NULL: zero */
-    void *initialState;                   /* (not the array of finalState) */
+    void *initialState;                   /* (not the array of finalState; may be the convolution's initialState itself) */
     float *weight, *bias;
 } gennmi_causal_conv_gradient_t;
 int gennmi_causal_conv(const gennmi_causal_conv_t *conv, void *stream);
@@ -655,7 +657,7 @@ typedef struct gennmi_scan_t {
 typedef struct gennmi_scan_gradient_t {             /* `out` and `finalState` come in, the others go out (any may be NULL) and are overwritten */
     gennmi_rows_t out, u, delta, z, B, C;
     const float *finalState;              /* gradient of the final state, or NULL: zero */
-    float *initialState, *A, *D, *deltaBias;
+    float *initialState, *A, *D, *deltaBias;    /* initialState may be the array of finalState, or the scan's initialState itself */
 } gennmi_scan_gradient_t;
 int gennmi_selective_scan_workspace(const gennmi_scan_t *scan, size_t *bytes);
 int gennmi_selective_scan(const gennmi_scan_t *scan, void *workspace, size_t workspaceBytes, void *stream);

@@ -3,6 +3,7 @@ entry points refuse before they touch the device.  Also the 64-bit restatements 
 import ctypes as C
 import json
 import os
+import random
 import subprocess
 import sys
 
@@ -154,10 +155,12 @@ def reaches_the_device(rc):
 
 
 WIDE = 1 << 24          # channels
+FAR = 1 << 50           # between the addresses of arrays of that size
 
 
 def wide(make, count, length, channels=WIDE, states=None, **changes):
-    rows = {f"{r}__{k}": v for r in (("x", "out") if states is None else ("u", "delta", "z", "out")) for k, v in (("rowStride", channels), ("sequenceStride", channels * length))}
+    rows = {f"{r}__{k}": v for n, r in enumerate(("x", "out") if states is None else ("u", "delta", "z", "out"))
+            for k, v in (("rowStride", channels), ("sequenceStride", channels * length), ("data", (n + 1) * FAR))}
     if states is not None:
         rows.update({f"{r}__{k}": v for r in "BC" for k, v in (("rowStride", states), ("sequenceStride", states * length))}, states=states, groups=1)
     return make(**rows, channels=channels, sequences__count=count, sequences__length=length, sequences__device=78, **changes)
@@ -165,12 +168,12 @@ def wide(make, count, length, channels=WIDE, states=None, **changes):
 
 def test_launches_of_2_to_the_32_threads_are_refused_before_anything_runs():
     """The last size that every launch of a call covers, and the first that one of them does not."""
-    lib, size, space = _abi.load(), C.c_size_t(), (C.c_void_p(AT), 1 << 62)
+    lib, size, space = _abi.load(), C.c_size_t(), (C.c_void_p(60 * FAR), 1 << 62)
     many = "more rows than one launch covers"
     # convolution: four channels a thread, 16 rows; gradients: two, 64 rows
     reaches_the_device(lib.gennmi_causal_conv(C.byref(wide(conv, 1, 1023 * 16)), None))
     refused(lib.gennmi_causal_conv(C.byref(wide(conv, 1, 1023 * 16 + 1)), None), -2, many)
-    g = _abi.CausalConvGradient(out=_abi.Rows(AT + 8192, WIDE, 0))
+    g = _abi.CausalConvGradient(out=_abi.Rows(20 * FAR, WIDE, 0))
     reaches_the_device(lib.gennmi_causal_conv_backward(C.byref(wide(conv, 1, 511 * 64)), C.byref(g), None, 0, None))
     refused(lib.gennmi_causal_conv_backward(C.byref(wide(conv, 1, 511 * 64 + 1)), C.byref(g), None, 0, None), -2, many)
     # scan: a wavefront for 64 channels of a sequence and 16 states; a token: a lane for four states
@@ -183,9 +186,9 @@ def test_launches_of_2_to_the_32_threads_are_refused_before_anything_runs():
             refused(rc, -2, many) if more else None
             assert more or rc == 0
     # gradients: the walk over chunks, a wavefront for a state of a sequence; then the sums of B and C, and those over chunks
-    for count, length, channels, states, gradients in (((1 << 22) - 1, 33, 1, 16, {}), (1, 134217720, 1, 16, dict(B=_abi.Rows(AT + (1 << 20), 16, 0))),
-                                                       (1, 2, 64 * 32767, 126, dict(A=AT + (1 << 20)))):
-        g = _abi.ScanGradient(out=_abi.Rows(AT + 4096 * 7, channels, channels * length), **gradients)
+    for count, length, channels, states, gradients in (((1 << 22) - 1, 33, 1, 16, {}), (1, 134217720, 1, 16, dict(B=_abi.Rows(30 * FAR, 16, 0))),
+                                                       (1, 2, 64 * 32767, 126, dict(A=30 * FAR))):
+        g = _abi.ScanGradient(out=_abi.Rows(20 * FAR, channels, channels * length), **gradients)
         for more in (0, 1):
             at = dict(count=count + (more if count > 1 else 0), length=length + (more if length > 100 else 0), channels=channels + (more if channels > 1 else 0), states=states)
             g.out.rowStride, g.out.sequenceStride = at["channels"], at["channels"] * at["length"]
@@ -248,6 +251,85 @@ def test_optimiser_refuses_settings_order_and_overlaps():
     refused(lib.gennmi_optimiser_get_step(o, C.byref(n)), -4, "not finalised")
     refused(lib.gennmi_optimiser_set_step(o, 3), -4, "not finalised")
     assert lib.gennmi_optimiser_destroy(o) == 0 and lib.gennmi_optimiser_destroy(None) == 0
+
+
+def places(rows, count, length, width):
+    """Elements that an array of 16 bits holds, one set a row."""
+    return [set(range(rows.data // 2 + s * rows.sequenceStride + t * rows.rowStride, rows.data // 2 + s * rows.sequenceStride + t * rows.rowStride + width))
+            for s in range(count) for t in range(length)]
+
+
+def test_arrays_that_overlap_in_part_are_refused():
+    """Any two layouts of rows, against their elements one by one: accepted are those of which no two rows that are written, and none that is written
+    and another that is read, share an element."""
+    rng, lib, said = random.Random(5), _abi.load(), {True: 0, False: 0}
+    for k in range(4000):
+        count, length, width = rng.randint(1, 4), rng.randint(1, 5), rng.randint(1, 4)
+        stride = lambda: rng.choice([width, 2 * width, 3 * width, count * width, length * width, (length + 1) * width, rng.randint(width, 40)])
+        a = _abi.Rows(AT, stride(), stride())
+        b = _abi.Rows(AT + 2 * rng.choice([width, length * width, count * length * width, rng.randint(0, 120)]), *((a.rowStride, a.sequenceStride) if k % 2 else (stride(), stride())))
+        x, out = (a, b) if k % 3 else (b, a)
+        held, written = places(x, count, length, width), places(out, count, length, width)
+        apart = sum(map(len, written)) == len(set().union(*written)) and not set().union(*written) & set().union(*held)
+        c = conv(channels=width, taps=1, silu=0, weight=FAR, bias=None, x=x, out=out, sequences__count=count, sequences__length=length, sequences__device=78)
+        rc = lib.gennmi_causal_conv(C.byref(c), None)
+        if apart:
+            reaches_the_device(rc)
+        else:
+            assert rc == -2 and any(t in lib.gennmi_last_error().decode() for t in ("overlap", "same array")), (lib.gennmi_last_error(), count, length, width, x, out)
+        said[apart] += 1
+    assert min(said.values()) > 500
+
+
+def test_states_gradients_and_workspaces_that_overlap_are_refused():
+    lib, size = _abi.load(), C.c_size_t()
+    far = dict(weight=FAR, bias=2 * FAR, sequences__device=78)
+    state = 2 * 3 * 24 * 2              # bytes of the convolution's states
+    at = AT + (1 << 16)
+    for change, text in ((dict(finalState=at, initialState=at), None), (dict(finalState=at, initialState=at + 2), "the final state overlaps the initial state"),
+                         (dict(finalState=at, initialState=at + state), None), (dict(finalState=AT + 470), "the final state overlaps x"), (dict(finalState=AT + 4096 + 470), "out overlaps the final state"),
+                         (dict(finalState=FAR + 380), "the final state overlaps weight"), (dict(out__data=AT + 48), "out overlaps x"),
+                         (dict(sequences__slots=AT + 4096, sequences__numSlots=2, finalState=at), "out overlaps slots")):
+        rc = lib.gennmi_causal_conv(C.byref(conv(**far, **change)), None)
+        refused(rc, -2, text) if text else reaches_the_device(rc)
+    c = conv(**far, initialState=at)
+    assert lib.gennmi_causal_conv_backward_workspace(C.byref(c), C.byref(size)) == 0
+    for change, text in ((dict(), None), (dict(initialState=at), None), (dict(initialState=at + 4), "the gradient of the initial state overlaps the initial state"),
+                         (dict(x__data=AT + 8192 + 24 * 2), "the gradient of x overlaps the gradient of out"), (dict(weight=AT + 16384), "the gradient of weight overlaps the gradient of x"),
+                         (dict(weight=4 * FAR, bias=4 * FAR + 380), "the gradient of weight overlaps the gradient of bias"), (dict(weight=FAR), None),
+                         (dict(bias=3 * FAR + 16), "the gradient of bias overlaps the workspace"), (dict(x__data=3 * FAR + 16), "the gradient of x overlaps the workspace")):
+        g = changed(_abi.CausalConvGradient(out=_abi.Rows(AT + 8192, 24, 120), x=_abi.Rows(AT + 16384, 24, 120), weight=4 * FAR), change)
+        rc = lib.gennmi_causal_conv_backward(C.byref(c), C.byref(g), 3 * FAR, size.value, None)
+        refused(rc, -2, text) if text else reaches_the_device(rc)
+    far = dict(A=FAR, D=2 * FAR, deltaBias=3 * FAR, sequences__device=78)
+    state = 2 * 24 * 16 * 4
+    space = 4 * FAR
+    for change, text in ((dict(), None), (dict(finalState=at, initialState=at), None), (dict(finalState=at, initialState=at + state - 4), "the final state overlaps the initial state"),
+                         (dict(out__data=AT + 4096 * 5 + 2), "out overlaps B"), (dict(out__data=FAR + 1024), "out overlaps A"), (dict(finalState=AT + 4096 * 6), "the final state overlaps C"),
+                         # rows of one wide array, side by side, and one element too near
+                         (dict(u__rowStride=48, u__sequenceStride=240, out__data=AT + 48, out__rowStride=48, out__sequenceStride=240), None),
+                         (dict(u__rowStride=48, u__sequenceStride=240, out__data=AT + 46, out__rowStride=48, out__sequenceStride=240), "out overlaps u"),
+                         # time outside, sequences inside
+                         (dict(u__rowStride=96, u__sequenceStride=48, out__data=AT + 48, out__rowStride=96, out__sequenceStride=48), None),
+                         # sequences that hold all rows of one array, then all of another's, which are not as far apart
+                         (dict(u__rowStride=24, u__sequenceStride=400, out__data=AT + 240, out__rowStride=30, out__sequenceStride=400), None),
+                         (dict(u__rowStride=24, u__sequenceStride=400, out__data=AT + 238, out__rowStride=30, out__sequenceStride=400), "out overlaps u"),
+                         (dict(out__rowStride=24, out__sequenceStride=60), "out: sequences overlap"), (dict(out__rowStride=24, out__sequenceStride=24), "out: sequences overlap")):
+        rc = lib.gennmi_selective_scan(C.byref(scan(**far, **change)), space, 1 << 20, None)
+        refused(rc, -2, text) if text else reaches_the_device(rc)
+    c = scan(**far, sequences__length=100, **{f"{n}__{k}": v for n, w, p in (("u", 24, 10), ("delta", 24, 11), ("z", 24, 12), ("out", 24, 13), ("B", 32, 14), ("C", 32, 15))
+                                              for k, v in (("data", p * FAR), ("sequenceStride", 100 * w))})
+    assert lib.gennmi_selective_scan_backward_workspace(C.byref(c), C.byref(size)) == 0
+    rows = lambda data, width=24, wide=None: _abi.Rows(data, wide or width, 100 * (wide or width))
+    for gradients, text in ((dict(u=rows(21 * FAR)), None), (dict(u=rows(10 * FAR + 24)), "the gradient of u overlaps u"), (dict(delta=rows(space + 48)), "the gradient of delta overlaps the workspace"),
+                            (dict(u=rows(21 * FAR), delta=rows(21 * FAR + 24)), "the gradient of u overlaps the gradient of delta"),
+                            (dict(B=rows(21 * FAR, 32, 64), C=rows(21 * FAR + 64, 32, 64)), None), (dict(B=rows(21 * FAR, 32, 64), C=rows(21 * FAR + 62, 32, 64)), "the gradient of B overlaps the gradient of C"),
+                            (dict(A=21 * FAR, D=21 * FAR + 4 * 24 * 16 - 4), "the gradient of A overlaps the gradient of D"), (dict(A=21 * FAR, D=21 * FAR + 4 * 24 * 16), None),
+                            (dict(A=FAR, D=2 * FAR, deltaBias=3 * FAR), None), (dict(deltaBias=space + 64), "the gradient of delta's bias overlaps the workspace"),
+                            (dict(initialState=21 * FAR, finalState=21 * FAR), None), (dict(initialState=21 * FAR, finalState=21 * FAR + 4), "the gradient of the initial state overlaps the gradient of the final state")):
+        g = _abi.ScanGradient(out=rows(20 * FAR), **gradients)
+        rc = lib.gennmi_selective_scan_backward(C.byref(c), C.byref(g), space, size.value, None)
+        refused(rc, -2, text) if text else reaches_the_device(rc)
 
 
 # The runtime's calls that an optimiser's table takes, on host memory: copy number `failing` (counted from 1) fails
