@@ -27,7 +27,7 @@ class _SequenceOperator:
         self._lib = _abi.load()
         _abi.check(self._lib.gennmi_init(device))
         self._bound = self._gradients = None        # operands (kept alive) of the descriptors
-        self._packed = None
+        self._packed = self._bound_packed = None    # rows of packed arrays: of a call of bind(), and of the one that held
         self._workspaces = {}           # (stream, which pass): one each, as calls on different streams may overlap
 
     def _operand(self, array, name, shape=None):
@@ -143,7 +143,7 @@ class CausalConvolution(_SequenceOperator):
                 raise ValueError("initial_state and final_state have different numbers of places")
             c.sequences.numSlots = first or last or 0
         same_device(given, self.device)
-        self._bound, self._descriptor, self._reference, self._gradients = given, c, C.byref(c), None
+        self._bound, self._bound_packed, self._descriptor, self._reference, self._gradients = given, self._packed, c, C.byref(c), None
 
     def run(self, stream=0):
         if self._bound is None:
@@ -155,6 +155,7 @@ class CausalConvolution(_SequenceOperator):
     def bind_gradients(self, out, x=None, weight=None, bias=None, initial_state=None, final_state=None):
         """``out`` and ``final_state``: gradients that come in; the others are written."""
         self._need(self._bound, "bind()")
+        self._packed = self._bound_packed
         given = []
         g = _abi.CausalConvGradient()
         g.out, g.x = self._rows(out, "the gradient of out", self.channels, given), self._rows(x, "the gradient of x", self.channels, given)
@@ -208,12 +209,11 @@ class SelectiveScan(_SequenceOperator):
                 raise ValueError("initial_state and final_state have different numbers of places")
             c.sequences.numSlots = first or last or 0
         same_device(given, self.device)
-        self._bound, self._descriptor, self._reference, self._gradients = given, c, _byref(c), None
-        self.workspace_bytes = 0
+        size = _size_t()
         if out is not None:
-            size = _size_t()
-            _abi.check(self._lib.gennmi_selective_scan_workspace(self._reference, _byref(size)))
-            self.workspace_bytes = size.value
+            _abi.check(self._lib.gennmi_selective_scan_workspace(_byref(c), _byref(size)))
+        self.workspace_bytes = size.value
+        self._bound, self._bound_packed, self._descriptor, self._reference, self._gradients = given, self._packed, c, _byref(c), None
 
     def run(self, stream=0, workspace=None):
         """``workspace``: ``workspace_bytes`` on the device, for a call that is captured into a graph (which keeps using it)."""
@@ -227,6 +227,7 @@ class SelectiveScan(_SequenceOperator):
     def bind_gradients(self, out, u=None, delta=None, A=None, B=None, C=None, D=None, delta_bias=None, z=None, initial_state=None, final_state=None):
         """``out`` and ``final_state``: gradients that come in; the others are written."""
         self._need(self._bound, "bind()")
+        self._packed = self._bound_packed
         given, width = [], self.groups * self.states
         g = _abi.ScanGradient()
         for field, array, n in (("out", out, self.channels), ("u", u, self.channels), ("delta", delta, self.channels), ("z", z, self.channels),

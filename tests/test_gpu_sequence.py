@@ -673,6 +673,40 @@ def test_streams_graphs_and_workspaces():
     assert all(torch.equal(a, b) for a, b in zip(results, got)) and not torch.equal(got[1], want[1])
 
 
+def test_a_bind_that_is_refused_leaves_the_one_before():
+    """Also where the refused arrays were packed and those before are not: gradients are bound to those before."""
+    from genn_amd.sequence import CausalConvolution, SelectiveScan
+    r, S, n, D, N, K = generator(3), 2, 9, 6, 4, 3
+    on = lambda *shape: r(*shape).cuda()
+    offsets = torch.tensor([0, 9, 18], dtype=torch.int32).cuda()
+    args = dict(u=on(S, n, D), delta=on(S, n, D).abs(), A=-torch.rand(D, N).cuda(), B=on(S, n, N), C=on(S, n, N), out=on(S, n, D))
+    flat = {k: v.view(S * n, -1) if v.dim() == 3 else v for k, v in args.items()}
+    dout = on(S, n, D)
+    for op, good, packed, wrong, name, shape in (
+            (SelectiveScan(S, n, D, N), args, flat, dict(A=on(D, N + 1)), "A", (D, N)),
+            (CausalConvolution(S, n, D, K), dict(x=args["u"], weight=on(D, K), out=on(S, n, D)), dict(x=flat["u"], weight=on(D, K)), dict(weight=on(D, K + 1)), "weight", (D, K))):
+        grads = [torch.empty(shape).cuda() for _ in range(2)]
+        for k, g in enumerate(grads):
+            op.bind(**good)
+            if k:
+                with pytest.raises(ValueError, match="shape"):
+                    op.bind(**{**packed, **wrong}, offsets=offsets)
+            op.run()
+            op.bind_gradients(out=dout, **{name: g})
+            op.backward()
+        torch.cuda.synchronize()
+        assert torch.equal(*grads) and grads[0].abs().sum() > 0
+    # ... and where the library refuses it
+    s = SelectiveScan(S, n, D, N)
+    s.bind(**args)
+    with pytest.raises(_abi.GennmiError, match="sequences overlap"):
+        s.bind(**{**args, "out": torch.zeros(n, D).cuda().expand(S, n, D)})
+    args["out"].zero_()
+    s.run()
+    torch.cuda.synchronize()
+    assert args["out"].abs().sum() > 0
+
+
 def test_arrays_of_the_package_and_what_the_layer_refuses():
     from genn_amd.sequence import CausalConvolution, SelectiveScan
     n, D, N, K = 6, 10, 4, 3
