@@ -118,6 +118,58 @@ def test_steps_against_the_formula(weight, gradient, copy, shift, bits):
             assert all(torch.all(r[:shift] == 5.0) and torch.all(r[shift + n:] == 5.0) for r in room)
 
 
+@pytest.mark.parametrize("bits, gradient", [(32, torch.float32), (32, torch.bfloat16), (8, torch.bfloat16)])
+def test_a_step_that_passes_the_caches_by(bits, gradient):
+    """A step of more than 64 MiB takes streaming accesses: the same bits as optimisers of a tensor each, which do not, and the formula's values.  The last tensor
+    begins in the middle of an access."""
+    sizes, rate, decay = [3000001, 2600003, 1027, 5], 1e-2, 0.1
+    step = sum(sizes) * (8 + 4 * bits // 8 + torch.finfo(gradient).bits // 8)
+    most = max(sizes) * (8 + 4 * bits // 8 + torch.finfo(gradient).bits // 8)
+    if bits == 32:
+        sizes, step, most = [s // 2 for s in sizes], step // 2, most // 2
+    assert step > 64 << 20 > most
+    made, again = ([w_g for _, w_g in tensors(sizes, torch.float32, gradient, seed=8)] for _ in range(2))
+    room = torch.zeros(1000 + 3).cuda()
+    first = [w.cpu().double() for w, _ in made]
+    one, several = AdamW(learning_rate=rate, beta1=BETA1, beta2=BETA2, epsilon=EPS, state_bits=bits), []
+    copies = [[torch.zeros(n, dtype=torch.bfloat16).cuda() for n in sizes] for _ in range(2)]
+    for k in range(len(sizes)):
+        one.add(*made[k], copy=copies[0][k], weight_decay=decay)
+        several.append(AdamW(learning_rate=rate, beta1=BETA1, beta2=BETA2, epsilon=EPS, state_bits=bits))
+        several[k].add(*again[k], copy=copies[1][k], weight_decay=decay)
+    odd = [torch.cat([room.clone(), torch.zeros(8).cuda()])[3:][:1000] for _ in range(2)]
+    ones = torch.ones(1000).cuda()
+    one.add(odd[0], ones)
+    several.append(AdamW(learning_rate=rate, beta1=BETA1, beta2=BETA2, epsilon=EPS, state_bits=bits))
+    several[-1].add(odd[1], ones)
+    for o in (one, *several):
+        o.build()
+    for k in range(2):
+        for o in (one, *several):
+            o.step()
+        torch.cuda.synchronize()
+        if k == 0:
+            for n, (w, g) in enumerate(made):
+                want, m, v = ref.adamw(first[n], g.cpu().double(), 0.0, 0.0, 1, rate, BETA1, BETA2, EPS, decay)
+                weights_close(f"weights of {n}", w, first[n], want, decay, rate, torch.float32)
+                got = {s: torch.from_numpy(a.pull_from_device().copy()) for s, a in one.states[n].items()}
+                if bits == 32:
+                    within(f"m of {n}", got["m"], m, 6 * U * m.abs() + 1e-44)
+                    within(f"v of {n}", got["v"], v, 6 * U * v + 1e-44)
+                else:
+                    M, V = (got[s].double().repeat_interleave(256)[:sizes[n]] for s in ("m_scale", "v_scale"))
+                    codes_close(f"m of {n}", got["m"].long() & 127, m.abs() * 448 / M)
+                    codes, root = got["v"].long(), torch.sqrt(v / V) * 448
+                    raised = (v > 0) & (ref.e4m3_codes(root) == 0)
+                    assert torch.all(codes[raised] == 1)
+                    codes_close(f"v of {n}", codes[~raised], root[~raised])
+    assert torch.equal(odd[0], odd[1]) and odd[0].abs().sum() > 0
+    for n in range(len(sizes)):
+        assert torch.equal(made[n][0], again[n][0]) and torch.equal(copies[0][n], copies[1][n])
+        for s in one.states[n]:
+            assert np.array_equal(one.states[n][s].pull_from_device(), several[n].states[0][s].pull_from_device()), (n, s)
+
+
 def test_a_positive_second_moment_never_becomes_zero():
     """A weight whose gradients are 10^-8 of its block's largest keeps a second moment: its next step is no division by epsilon."""
     g = torch.full((256,), 1e-8).cuda()

@@ -205,6 +205,14 @@ def test_selective_scan(lengths, channels, states, groups, dtype, softplus, gate
     assert all(torch.equal(first[n], g) for n, g in grads.items())
 
 
+@pytest.mark.parametrize("lengths, channels, states, groups, dtype, packed", [
+    ([40, 40], 130, 16, 2, "bfloat16", False),          # (65 channels a group: a whole tile and one of a single lane)
+    ([150], 390, 5, 3, "float32", False), ([70, 0, 1, 90], 260, 16, 2, "float32", True), ([33], 260, 20, 2, "float16", False),
+    ([1, 1], 390, 16, 3, "bfloat16", False), ([300], 258, 33, 2, "float32", False)])
+def test_groups_of_several_tiles_of_channels(lengths, channels, states, groups, dtype, packed):
+    test_selective_scan(lengths, channels, states, groups, dtype, True, True, True, True, packed, False, True)
+
+
 @pytest.mark.parametrize("states", [7, 16, 40])
 def test_gradients_asked_for_one_by_one(states):
     """Whichever are asked for, they are the same, and nothing else is written."""
@@ -609,6 +617,58 @@ def test_offsets_beyond_32_bits():
     s.run()
     args = dict(u=x, delta=x, A=A, B=B.view(3, 1, N), C=B.view(3, 1, N))
     close("scan", out, ref.scan(**args)[0], ref.scan(**args, magnitudes=True)[0], 2 * 3 + N + 12, torch.bfloat16)
+
+
+def test_rows_and_sequences_beyond_32_bits_forwards_and_back():
+    """Two sequences of three rows, more than 2^31 elements from row to row and 2^32 from sequence to sequence, all arrays side by side in one."""
+    from genn_amd.sequence import CausalConvolution, SelectiveScan
+    S, n, D, N, K, stride = 2, 3, 64, 16, 3, (1 << 31) + 64
+    room = torch.empty(S * n * stride, dtype=torch.bfloat16, device="cuda")
+    r, used = generator(14), [0]
+
+    def far(width, values=None):
+        at = torch.as_strided(room, (S, n, width), (n * stride, stride, 1), used[0])
+        used[0] += width
+        if values is not None:
+            for k in range(S):
+                at[k].copy_(values[k])
+        return at
+
+    give = {k: r(S, n, w).to(torch.bfloat16) for k, w in (("x", D), ("delta", D), ("B", N), ("C", N), ("z", D), ("dout", D))}
+    on = {k: far(v.shape[-1], v) for k, v in give.items()}
+    weight, A, initial = r(D, K), -torch.rand(D, N), r(S, D, N)
+    back = lambda t: torch.stack([t[k].clone() for k in range(S)]).cpu()
+    c, s = CausalConvolution(S, n, D, K, dtype="bfloat16", silu=True), SelectiveScan(S, n, D, N, dtype="bfloat16", softplus=True)
+    out, dx, dw = far(D), far(D), torch.empty(D, K).cuda()
+    c.bind(x=on["x"], weight=weight.cuda(), out=out)
+    c.bind_gradients(out=on["dout"], x=dx, weight=dw)
+    scanned, final, dA = far(D), torch.empty(S, D, N).cuda(), torch.empty(D, N).cuda()
+    grads = {k: far(w) for k, w in (("u", D), ("delta", D), ("z", D), ("B", N), ("C", N))}
+    s.bind(u=on["x"], delta=on["delta"], A=A.cuda(), B=on["B"], C=on["C"], z=on["z"], out=scanned, initial_state=initial.cuda(), final_state=final)
+    s.bind_gradients(out=on["dout"], A=dA, **grads)
+    for op in (c, s):
+        op.run()
+        op.backward()
+    torch.cuda.synchronize()
+    got = {k: back(v) for k, v in dict(out=out, dx=dx, scanned=scanned, **grads).items()}
+    dws, dAs = [0, 0], [0, 0]
+    for k in range(S):
+        args = (give["x"][k], weight, None, True)
+        close("conv", got["out"][k], ref.causal_conv(*args)[0], ref.causal_conv(*args, magnitudes=True)[0], K + 8, torch.bfloat16)
+        args = (*args, None, give["dout"][k])
+        want, size = (ref.causal_conv(*args, magnitudes=m) for m in (False, True))
+        close("dx", got["dx"][k], want[0], size[0], 2 * K + 16, torch.bfloat16)
+        dws = [dws[0] + want[1], dws[1] + size[1]]
+        args = dict(u=give["x"][k], delta=give["delta"][k], A=A, B=give["B"][k].view(n, 1, N), C=give["C"][k].view(n, 1, N), z=give["z"][k], softplus=True, initial=initial[k])
+        want, size = (ref.scan(**args, magnitudes=m) for m in (False, True))
+        close("scan", got["scanned"][k], want[0], size[0], 2 * n + N + 12, torch.bfloat16)
+        close("final state", final[k], want[1], size[1], 2 * n + N + 12)
+        want, size = (ref.scan(**args, dout=give["dout"][k], magnitudes=m) for m in (False, True))
+        for name in grads:
+            close(f"d{name}", got[name][k], want[name].reshape(n, -1), size[name].reshape(n, -1), 4 * n + N + 47, torch.bfloat16)
+        dAs = [dAs[0] + want["A"], dAs[1] + size["A"]]
+    close("dweight", dw, *dws, K + 16 + 20)
+    close("dA", dA, *dAs, 4 * n + N + 80)
 
 
 def test_streams_graphs_and_workspaces():
