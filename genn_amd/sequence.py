@@ -81,6 +81,8 @@ class _SequenceOperator:
         """``given`` by the caller, or the operator's own for that stream."""
         if given is not None:
             o = Operand(given, "workspace").wants(("uint8", "float32"))
+            o.contiguous(o.shape)
+            same_device([o], self.device)
             size = o.shape[0] if len(o.shape) == 1 else 0
             return o.address, size * (4 if o.dtype == "float32" else 1)
         if not needed:

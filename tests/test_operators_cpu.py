@@ -400,6 +400,32 @@ def test_python_layer_refuses_before_it_touches_the_device():
         Operand([1.0], "x")
 
 
+class Elsewhere:
+    """What a tensor on a device says of itself."""
+    is_cuda, dtype = True, torch.uint8
+
+    def __init__(self, shape, strides, index):
+        self.shape, self.strides, self.device = shape, strides, torch.device("cuda", index)
+
+    def data_ptr(self):
+        return AT
+
+    def stride(self):
+        return self.strides
+
+
+def test_workspaces_are_looked_at_as_other_arrays_are():
+    """On the operator's device, and its bytes one behind another."""
+    from genn_amd.sequence import SelectiveScan
+    op = SelectiveScan.__new__(SelectiveScan)
+    op.device, op._workspaces = 0, {}
+    assert op._workspace("forward", Elsewhere((4096,), (1,), 0), 4096, 0) == (AT, 4096)
+    with pytest.raises(ValueError, match="on device 1"):
+        op._workspace("forward", Elsewhere((4096,), (1,), 1), 4096, 0)
+    with pytest.raises(ValueError, match="workspace is not contiguous"):
+        op._workspace("forward", Elsewhere((4096,), (2,), 0), 4096, 0)
+
+
 def test_gradients_of_the_restatements_are_those_of_differences():
     """Along random directions, by central differences: off by a third derivative times step^2 (1e-10 here) and rounding over step (1e-16 / 1e-5)."""
     gen = torch.Generator().manual_seed(3)
