@@ -188,8 +188,8 @@ void causalConvKernel(ConvArgs a)
 // Gradients.  With ds[t] = dout[t] f'(s[t]):  dx[p] = sum_k w[k] ds[p + (K - 1) - k], which is complete when ds[p + K - 1] is there, so a
 // thread walks K - 1 rows further than its chunk, with the last K inputs and the last K ds in registers, and writes row t - (K - 1)
 // at row t; in front of a sequence's first chunk these are the rows of the initial state.  dw[k] = sum ds[t] x[t - (K - 1) + k] and
-// dbias are summed over the chunk and then over chunks by a kernel of their own, always in the same order.  8 x 2048 rows x 2048 channels x 4 taps in bf16 take 53 us
-// with the sums (5 of them), 3.8 TB/s for what has to be read and written; vector units are busy for 87 % of the time (44 instructions an element).
+// dbias are summed over the chunk and then over chunks by a kernel of their own, always in the same order.  8 x 2048 rows x 2048 channels x 4 taps in bf16 take 54 us
+// with the sums (5 of them), 3.7 TB/s for what has to be read and written; vector units are busy for 87 % of the time (44 instructions an element).
 template<typename T, int K, int VEC>
 __global__ __launch_bounds__(256)
 void causalConvBackwardKernel(ConvArgs a, ConvGradientArgs g)

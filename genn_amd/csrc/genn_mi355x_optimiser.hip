@@ -5,7 +5,7 @@
 // 8 bits the 256 weights that share a scale are one wavefront's four a lane, so their maxima are found in registers and codes are written by the
 // pass that made the states.  The number of the step is the device's: the work-group that ends last counts it, so a captured step counts as well.
 //
-// 80 M weights in 32 bits (fp32 weights, bf16 gradients and copy) take 390 us, 130 M in 8 bits (bf16 gradients) 311: 5.7 and 5.8 TB/s, where a large copy reaches 4.7.
+// 80 M weights in 32 bits (fp32 weights, bf16 gradients and copy) take 382 to 390 us, 130 M in 8 bits (bf16 gradients) 313: 5.7 to 5.9 and 5.8 TB/s, where a large copy reaches 4.7.
 // One access an array and lane, and many short work-groups: without the streaming accesses, and with more arithmetic in 8 bits, CHUNK 1024, 2048, 4096, 8192
 // took 411, 428, 441, 449 us and 369, 373, 410, 409; work-groups that stay and go through the table 466 and more; the next
 // block's loads ahead of the arithmetic 436 and 457 (registers).

@@ -13,8 +13,8 @@
 //
 // Bound by vector instructions, not by memory: a state takes a row a product and an exponential (two slots of a SIMD's issue) for its decay, a product and a sum
 // for what comes in, a sum for y, 6 slots, of which the first kernel of a split scan needs 5 as well.  At 39.3 T lane-slots a second 4096 rows x 2048 channels x 16
-// states are 38 us of these alone, their 68 MB 14 us.  They take 79 us in bf16: 37 the first kernel, 8 the second, 45 the third, with the vector
-// units busy for three quarters of the time (softplus, gate and conversions are a fifth of their instructions).  What there is to gain by matrix instructions is
+// states are 38 us of these alone, their 68 MB 12 us.  They take 77 us in bf16: 36 the first kernel, 8 the second, 42 the third, with the vector
+// units busy for four fifths of the time (softplus, gate and conversions are a fifth of their instructions).  What there is to gain by matrix instructions is
 // nothing: every state of every channel has decays of its own.
 #ifndef GENN_MI355X_SCAN_KERNELS_H
 #define GENN_MI355X_SCAN_KERNELS_H
@@ -586,8 +586,8 @@ void scanTokenKernel(ScanArgs a)
 // A block's walks take PART of the states at a time, so that R * PART of them, and as many decays, fit the registers of two wavefronts a SIMD.
 //
 // Bound by vector instructions: 420 a row and wavefront of 16 states, an eighth of them the sums over channels (all of them in registers: 444 and 690 us), and units
-// busy for three quarters of the time (252 registers, so two wavefronts a SIMD; 20 KiB of LDS each, all that there is for eight).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 670 us, the first 207, the second 57 (memory, 4.8 TB/s), sums
-// over tiles 23 and over chunks 17.  PART 4 spills (813 us), so do three wavefronts a SIMD (1240), without the ties of readAfter it was 9.4 ms.
+// busy for three quarters of the time (252 registers, so two wavefronts a SIMD; 20 KiB of LDS each, all that there is for eight).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 671 us, the first 206, the second 58 (memory, 4.7 TB/s), sums
+// over tiles 23 and over chunks 16.  PART 4 spills (813 us), so do three wavefronts a SIMD (1240), without the ties of readAfter it was 9.4 ms.
 template<typename T, int NP, int R, int BLOCKS, bool SLABS>
 __global__ __launch_bounds__(SLABS ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void scanBackwardKernel(ScanArgs a, ScanGradientArgs g)

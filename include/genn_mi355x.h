@@ -640,7 +640,8 @@ int gennmi_causal_conv_backward(const gennmi_causal_conv_t *conv, const gennmi_c
  *   out[t][d] = (sum_n C[t][g][n] * h[t][d][n] + D[d] * u[t][d]) * z[t][d] * sigmoid(z[t][d])
  * where channels / groups neighbouring channels share the B and C of group g.  States and sums in fp32.  Long sequences
  * are cut into chunks of up to 1024 rows (gradients: 32) whose decay is one factor: where dt A > 0 for long, the growth over a chunk has to stay
- * below 2^128, unless a forward scan's state is zero.  One row per sequence (a token of every
+ * below 2^128, unless a forward scan's state is zero.  What an infinite input or state gives is what the formula gives, as long as no row's decay rounds to zero; of the gradients that it
+ * reaches some may be not a number where the formula has infinity.  One row per sequence (a token of every
  * running sequence) takes a kernel of its own, without a workspace. */
 #define GENNMI_MAX_SCAN_STATES 128
 typedef struct gennmi_scan_t {
