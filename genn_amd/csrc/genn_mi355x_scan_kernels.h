@@ -354,11 +354,10 @@ template<bool BACKWARDS> __device__ inline float walkChunks(float *state, uint64
         for(uint32_t k = 0; k < AHEAD; k++) {
             if(first + k < chunks) {
                 state[chunk(first + k) * stride] = h;
-                // A chunk's decay may be infinite, where A is positive (of nothing, nothing is left all the same), or less than there is in 32 bits: it is
-                // the smallest positive value then, which no finite state can tell from nothing, and which leaves an infinite one as it is
-                // (nothing known of A or dt makes what the chunk adds unknown, if it has a row)
-                const float decay = fmaxf(exp2Of(times[k] * A), 0x1p-149f);
-                h = h == 0.0f ? adds[k] : __builtin_fmaf(decay, h, adds[k]);
+                // (a chunk's decay may be infinite, where A is positive, or round to zero: of nothing, nothing is left all the same, and of what is infinite all)
+                constexpr int ZERO_OR_INFINITE = 0x20 | 0x40 | 0x4 | 0x200;
+                const float sum = h + adds[k], next = __builtin_fmaf(exp2Of(times[k] * A), h, adds[k]);
+                h = __builtin_amdgcn_classf(h, ZERO_OR_INFINITE) ? sum : next;
             }
             adds[k] = nextAdds[k];
             times[k] = nextTimes[k];

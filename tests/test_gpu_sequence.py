@@ -379,6 +379,26 @@ def test_an_infinite_state_outlasts_decays_that_round_to_zero():
     assert torch.isfinite(out).all() and torch.isfinite(final).all()
 
 
+@pytest.mark.parametrize("largest", [1e20, 3e38])
+def test_a_large_state_that_is_forgotten_leaves_nothing(largest):
+    """The decay of the first chunk is none in 32 bits: what was there before is not in the states behind it, however large."""
+    from genn_amd.sequence import SelectiveScan
+    n, D, N = 600, 64, 16
+    r = generator(15)
+    u, B, C, A, delta, initial = r(n, D) * 1e-5, r(n, N), r(n, N), -8 - torch.rand(D, N), torch.full((n, D), 1e-3), torch.full((D, N), largest)
+    delta[:24] = 1.0            # (e^-192 and less, and then hardly any)
+    out, final = torch.empty(1, n, D).cuda(), torch.empty(1, D, N).cuda()
+    s = SelectiveScan(1, n, D, N)
+    s.bind(u=u.cuda(), delta=delta.cuda(), A=A.cuda(), B=B.cuda(), C=C.cuda(), out=out, initial_state=initial.cuda().view(1, D, N), final_state=final)
+    assert s.workspace_bytes > 0
+    s.run()
+    torch.cuda.synchronize()
+    args = dict(u=u, delta=delta, A=A, B=B.view(n, 1, N), C=C.view(n, 1, N), initial=initial)
+    want, size = ref.scan(**args), ref.scan(magnitudes=True, **args)
+    close("final state", final[0], want[1], size[1], 2 * n + N + 12)
+    close("out", out[0], want[0], size[0], 2 * n + N + 12)
+
+
 @pytest.mark.parametrize("lengths", [[5], [0, 13, 0], [0, 500, 3, 0]])
 def test_units_that_forget_everything(lengths):
     """A = -infinity: a row's state is what comes in with it; sequences without rows keep theirs.  Also one whose product with log2(e) is infinite."""
