@@ -237,6 +237,9 @@ inline bool overlap(const Region &a, const Region &b)
         const Region d = differences(b, 1 - b.outer, b.outer - 1);
         return meets(d, a.begin - b.begin, a.begin - b.begin + a.width);
     }
+    // (sequences equally far apart, in which the rows of one array lie behind those of the other)
+    const auto sequencesOf = [](Region r) { r.width += (r.inner - 1) * r.innerStride; r.inner = 1; r.innerStride = 0; return r; };
+    if(a.inner * b.inner > 1 && a.outer == b.outer && a.outerStride == b.outerStride && !overlap(sequencesOf(a), sequencesOf(b))) { return false; }
     // (one array's rows between another's that are not as far apart: looked at one by one)
     const Region &few = a.inner * a.outer <= b.inner * b.outer ? a : b, &many = &few == &a ? b : a;
     for(int64_t o = 0; o < few.outer; o++) {
