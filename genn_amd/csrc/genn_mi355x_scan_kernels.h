@@ -585,7 +585,7 @@ void scanTokenKernel(ScanArgs a)
 // A block's walks take PART of the states at a time, so that R * PART of them, and as many decays, fit the registers of two wavefronts a SIMD.
 //
 // Bound by vector instructions: 420 a row and wavefront of 16 states, an eighth of them the sums over channels (all of them in registers: 444 and 690 us), and units
-// busy for three quarters of the time (252 registers, so two wavefronts a SIMD; 20 KiB of LDS each, all that there is for eight).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 671 us, the first 206, the second 58 (memory, 4.7 TB/s), sums
+// busy for three quarters of the time (252 registers, so two wavefronts a SIMD; 20 KiB of LDS each, all that there is for eight).  8 sequences of 2048 rows x 2048 channels in bf16: this kernel 671 to 676 us, the first 206, the second 57 (memory, 4.8 TB/s), sums
 // over tiles 23 and over chunks 16.  PART 4 spills (813 us), so do three wavefronts a SIMD (1240), without the ties of readAfter it was 9.4 ms.
 template<typename T, int NP, int R, int BLOCKS, bool SLABS>
 __global__ __launch_bounds__(SLABS ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
