@@ -119,6 +119,30 @@ class ScanGradient(C.Structure):
                 ("initialState", p_f32), ("A", p_f32), ("D", p_f32), ("deltaBias", p_f32)]
 
 
+class DeltaRule(C.Structure):
+    _fields_ = [("sequences", Sequences), ("type", C.c_uint32), ("heads", C.c_uint32), ("keyHeads", C.c_uint32), ("keys", C.c_uint32), ("values", C.c_uint32),
+                ("normalise", C.c_uint32), ("scale", C.c_float), ("epsilon", C.c_float), ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("g", Rows),
+                ("beta", Rows), ("initialState", p_f32), ("finalState", p_f32)]
+
+
+class DeltaRuleGradient(C.Structure):
+    _fields_ = [("out", Rows), ("q", Rows), ("k", Rows), ("v", Rows), ("g", Rows), ("beta", Rows), ("finalState", p_f32), ("initialState", p_f32)]
+
+
+class LayerNorm(C.Structure):
+    _fields_ = [("sequences", Sequences), ("type", C.c_uint32), ("channels", C.c_uint32), ("rms", C.c_uint32), ("epsilon", C.c_float), ("x", Rows), ("gate", Rows),
+                ("out", Rows), ("weight", p_f32), ("bias", p_f32)]
+
+
+class LayerNormGradient(C.Structure):
+    _fields_ = [("out", Rows), ("x", Rows), ("gate", Rows), ("weight", p_f32), ("bias", p_f32)]
+
+
+class Dropout(C.Structure):
+    _fields_ = [("sequences", Sequences), ("type", C.c_uint32), ("channels", C.c_uint32), ("probability", C.c_double), ("seed", C.c_uint64), ("call", C.c_uint64),
+                ("callDevice", C.c_void_p), ("x", Rows), ("residual", Rows), ("out", Rows)]
+
+
 class AdamWSettings(C.Structure):
     _fields_ = [("beta1", C.c_double), ("beta2", C.c_double), ("epsilon", C.c_double), ("stateBits", C.c_uint32), ("pad_", C.c_uint32)]
 
@@ -134,6 +158,7 @@ class AdamWStep(C.Structure):
 
 
 OPERATOR_STRUCTS = (Rows, Sequences, CausalConv, CausalConvGradient, Scan, ScanGradient, AdamWSettings, Parameter, AdamWStep)
+LAYER_STRUCTS = (DeltaRule, DeltaRuleGradient, LayerNorm, LayerNormGradient, Dropout)
 
 INIT_SNIPPETS = {"Constant": 0, "Uniform": 1, "Normal": 2, "NormalClipped": 3, "NormalClippedDelay": 4, "Exponential": 5,
                  "Gamma": 6, "Binomial": 7}
@@ -240,6 +265,15 @@ SYMBOLS = {
     "gennmi_selective_scan": (C.c_int, [C.POINTER(Scan), C.c_void_p, C.c_size_t, C.c_void_p]),
     "gennmi_selective_scan_backward_workspace": (C.c_int, [C.POINTER(Scan), C.POINTER(C.c_size_t)]),
     "gennmi_selective_scan_backward": (C.c_int, [C.POINTER(Scan), C.POINTER(ScanGradient), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gennmi_delta_rule_workspace": (C.c_int, [C.POINTER(DeltaRule), C.POINTER(C.c_size_t)]),
+    "gennmi_delta_rule": (C.c_int, [C.POINTER(DeltaRule), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gennmi_delta_rule_backward_workspace": (C.c_int, [C.POINTER(DeltaRule), C.POINTER(C.c_size_t)]),
+    "gennmi_delta_rule_backward": (C.c_int, [C.POINTER(DeltaRule), C.POINTER(DeltaRuleGradient), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gennmi_layer_norm": (C.c_int, [C.POINTER(LayerNorm), C.c_void_p]),
+    "gennmi_layer_norm_backward_workspace": (C.c_int, [C.POINTER(LayerNorm), C.POINTER(C.c_size_t)]),
+    "gennmi_layer_norm_backward": (C.c_int, [C.POINTER(LayerNorm), C.POINTER(LayerNormGradient), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gennmi_dropout": (C.c_int, [C.POINTER(Dropout), C.c_void_p]),
+    "gennmi_abi_layer_sizes": (C.c_int, [C.POINTER(C.c_size_t * 5)]),
     "gennmi_optimiser_create": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(AdamWSettings)]),
     "gennmi_optimiser_destroy": (C.c_int, [C.c_void_p]),
     "gennmi_optimiser_push": (C.c_int, [C.c_void_p, C.POINTER(Parameter), C.POINTER(C.c_uint32)]),

@@ -1,0 +1,1146 @@
+// Part of genn_mi355x_delta.hip: kernels of the gated delta rule.
+//
+// Of one head, with unit keys k^ and queries q^, a[t] = exp(g[t]):
+//   S[t] = a[t] S[t-1] + k^[t] u[t]',   u[t] = beta[t] w[t],   w[t] = v[t] - a[t] S[t-1]' k^[t],   out[t] = scale S[t]' q^[t]
+// Over a chunk of rows that begins with the state S, with G[i] = exp(sum of g up to row i) and D[i][j] = G[i] / G[j] for i >= j:
+//   w[i] = v[i] - G[i] S' k^[i] - sum_{j<i} M[i][j] beta[j] w[j],   M[i][j] = D[i][j] k^[i].k^[j]
+// so that w = (I + M beta)^-1 r with r = v - G k^ S, and the inverse is I - N beta with (I + M beta) N = M.  Then
+//   out = scale G q^ S + P u,   P[i][j] = scale D[i][j] q^[i].k^[j] for i >= j,   S behind the chunk = G[last] S + sum_j D[last][j] k^[j] u[j]'.
+// The transposed inverse of the gradients, (I + beta M')^-1, is I - beta N': N serves both, and no beta is divided by.
+//
+// M, N and P do not need the state: a work-group a chunk and key head finds them (deltaChunkKernel).  Then a state's columns do not need each other:
+// a wavefront owns 16 of them, all rows in registers, and walks the chunks (deltaStateKernel).  Its results become operands of the next product
+// without leaving the registers; what multiplies them (keys, N, P) is shared by the work-group's wavefronts through LDS.  Products have fp32 accuracy (genn_mi355x_planes.h).
+#ifndef GENN_MI355X_DELTA_KERNELS_H
+#define GENN_MI355X_DELTA_KERNELS_H
+
+#include "genn_mi355x_lanes.h"
+#include "genn_mi355x_planes.h"
+
+namespace gennmi_delta
+{
+using namespace gennmi_elements;
+using namespace gennmi_planes;
+using gennmi_lanes::partner;
+
+// What a row of a chunk needs of one head
+struct alignas(32) RowTable
+{
+    float keyState;         // G / |k|: times the key and the state
+    float beta;
+    float keyEnd;           // D[last] / |k|: times the key and u, what the row leaves in the state behind the chunk
+    float queryState;       // scale G / |q|
+    float keyUnit, queryUnit;       // 1 / |k|, 1 / |q|
+    double sum;             // of g, since the chunk's beginning
+};
+struct ChunkTable { float decay; uint32_t bad; };          // G[last]; first row from which nothing is finite, or the chunk's rows
+
+struct DeltaArgs
+{
+    Sequences chunks, segments;
+    gennmi_rows_t q, k, v, out, g, beta;
+    const float *initialState;
+    float *finalState;
+    uint32_t heads, keyHeads, group, keys, values, normalise, wide, columnBlocks;
+    uint32_t padded;                // values, up to a multiple of 32: the width of what is kept of them
+    float scale, epsilon;
+    float *correction, *score;      // of each chunk number and head: -N and P, [C][C]
+    RowTable *rows;                 // [C]
+    ChunkTable *table;
+    float *states, *errors;         // kept for gradients, of each chunk number and head: the state in front of it [DK][padded], w [C][padded]
+};
+
+// Gates below this are as good as minus infinity (exp(-1e6) is 0), and sums of them are finite
+__device__ inline float clampGate(float g) { return g < -1e6f ? -1e6f : g; }
+__device__ inline float decayOver(double sum) { return __builtin_amdgcn_exp2f((float)(sum * 1.4426950408889634)); }
+__device__ inline bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+
+template<typename T> __device__ inline const T *rowAt(const gennmi_rows_t &r, const Sequences &s, const Place &p, uint32_t row) { return rowsOf<const T>(r, s, p) + (uint64_t)row * r.rowStride; }
+
+// ---- what a chunk needs that does not depend on the state
+template<typename T, int C, int DK> constexpr uint32_t chunkLds() { return 2 * planesOf<T> * C * (DK + 8) * 2 + C * (C + 4) * 4 + C * (8 + 3 * 4) + 16; }
+
+template<typename T, int C, int DK>
+__global__ __launch_bounds__(256)
+void deltaChunkKernel(DeltaArgs a)
+{
+    constexpr int NP = planesOf<T>, B = C / 16, PITCH = DK + 8, PLANE = C * PITCH, MP = C + 4, TILES = B * B / 4;
+    extern __shared__ __align__(16) char lds[];
+    uint16_t *const keyPlanes = (uint16_t*)lds, *const queryPlanes = keyPlanes + NP * PLANE;
+    float *const m = (float*)(queryPlanes + NP * PLANE);
+    double *const sums = (double*)(m + C * MP);
+    float *const keyUnit = (float*)(sums + C), *const queryUnit = keyUnit + C, *const beta = queryUnit + C;
+    uint32_t *const bad = (uint32_t*)(beta + C);
+    const uint32_t number = blockIdx.x / a.keyHeads, keyHead = blockIdx.x - number * a.keyHeads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
+    Place p;
+    if(!locate(a.chunks, number, p)) { return; }
+    const uint32_t begin = p.index * C, count = min((uint32_t)C, p.length - min(p.length, begin));
+    if(!count) { return; }
+
+    // keys and queries as planes, and what they are divided by
+    #pragma unroll
+    for(int item = 0; item < C * DK / 8; item += 256) {
+        const uint32_t i = item + tid, row = i / (DK / 8), at = i % (DK / 8) * 8;
+        if(C * DK / 8 < 256 && i >= C * DK / 8) { break; }
+        const uint32_t valid = row < count && at < a.keys ? min(8u, a.keys - at) : 0;
+        #pragma unroll
+        for(int which = 0; which < 2; which++) {
+            const gennmi_rows_t &r = which ? a.q : a.k;
+            T x[8];
+            loadEight(rowAt<T>(r, a.chunks, p, valid ? begin + row : 0) + (valid ? keyHead * a.keys + at : 0), valid, a.wide, x);
+            float sum = 0.0f, first[4], second[4];
+            #pragma unroll
+            for(int e = 0; e < 8; e++) {
+                const float f = widen(x[e]);
+                sum = __builtin_fmaf(f, f, sum);
+                (e < 4 ? first[e] : second[e - 4]) = f;
+            }
+            uint2 low[NP], high[NP];
+            splitFour<NP>(first, low);
+            splitFour<NP>(second, high);
+            uint16_t *const to = (which ? queryPlanes : keyPlanes) + row * PITCH + at;
+            #pragma unroll
+            for(int k = 0; k < NP; k++) { *(uint4*)(to + k * PLANE) = make_uint4(low[k].x, low[k].y, high[k].x, high[k].y); }
+            sum += partner<1>(sum);
+            sum += partner<2>(sum);
+            sum += partner<4>(sum);
+            if(DK == 128) { sum += partner<8>(sum); }
+            if(at == 0) { (which ? queryUnit : keyUnit)[row] = row >= count ? 0.0f : a.normalise ? 1.0f / sqrtf(sum + a.epsilon) : 1.0f; }
+        }
+    }
+    __syncthreads();
+
+    // products of all keys with all keys and queries; tiles above the diagonal are left out
+    f32x4 kk[TILES], qk[TILES];
+    const auto tileRow = [&](int t) { return C == 64 ? wave : wave >> 1; };
+    const auto tileColumn = [&](int t) { return C == 64 ? (uint32_t)t : wave & 1; };
+    #pragma unroll
+    for(int t = 0; t < TILES; t++) {
+        kk[t] = qk[t] = f32x4{0, 0, 0, 0};
+        if(tileColumn(t) > tileRow(t)) { continue; }
+        #pragma unroll
+        for(int s = 0; s < DK / 32; s++) {
+            const uint32_t offset = s * 32 + g * 8, ra = (tileRow(t) * 16 + n16) * PITCH + offset, rb = (tileColumn(t) * 16 + n16) * PITCH + offset;
+            const Planes<NP> kb = fetch<NP>(keyPlanes + rb, PLANE);
+            kk[t] = multiply(fetch<NP>(keyPlanes + ra, PLANE), kb, kk[t]);
+            qk[t] = multiply(fetch<NP>(queryPlanes + ra, PLANE), kb, qk[t]);
+        }
+    }
+
+    for(uint32_t inGroup = 0; inGroup < a.group; inGroup++) {
+        const uint32_t head = keyHead * a.group + inGroup;
+        const uint64_t at = (uint64_t)number * a.heads + head;
+        RowTable *const rows = a.rows + at * C;
+        if(tid == 0) { *bad = C; }
+        float decay = 0.0f;
+        if(wave == 0) {
+            const bool valid = lane < count;
+            const float b = valid ? rowAt<float>(a.beta, a.chunks, p, begin + lane)[head] : 0.0f;
+            double sum = valid ? (double)clampGate(rowAt<float>(a.g, a.chunks, p, begin + lane)[head]) : 0.0;
+            #pragma unroll
+            for(int w = 1; w < C; w *= 2) {
+                const double before = __shfl_up(sum, w);
+                if(lane >= (uint32_t)w) { sum += before; }
+            }
+            const double last = __shfl(sum, C - 1);
+            decay = decayOver(last);
+            if(lane < C) {
+                const float since = decayOver(sum), until = decayOver(last - sum), ku = keyUnit[lane], qu = queryUnit[lane];
+                sums[lane] = sum;
+                beta[lane] = b;
+                rows[lane] = RowTable{since * ku, b, until * ku, a.scale * since * qu, ku, qu, sum};
+                // (sum, b and the key's length: what makes a row's errors no numbers, also in a chunk's first row)
+                if(valid && !(finite(b) && finite(since) && finite(ku))) { atomicMin(bad, lane); }
+            }
+        }
+        __syncthreads();
+        float *const score = a.score + at * C * C, *const correction = a.correction + at * C * C;
+        #pragma unroll
+        for(int t = 0; t < TILES; t++) {
+            const uint32_t column = tileColumn(t) * 16 + n16;
+            const double sum = sums[column];
+            const float ku = keyUnit[column];
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = tileRow(t) * 16 + 4 * g + r;
+                const float d = row >= column ? decayOver(sums[row] - sum) : 0.0f;
+                const float x = row > column ? d * (keyUnit[row] * kk[t][r] * ku) : 0.0f;
+                const float y = row >= column ? d * (a.scale * (queryUnit[row] * qk[t][r] * ku)) : 0.0f;
+                if(!finite(x)) { atomicMin(bad, row); }
+                m[row * MP + column] = x;
+                score[row * C + column] = y;
+            }
+        }
+        __syncthreads();
+        const uint32_t from = *bad;
+        if(from < C) {      // (nothing finite from that row on: the rows before it must not meet it)
+            for(uint32_t i = from * C + tid; i < C * C; i += 256) { m[i / C * MP + i % C] = 0.0f; score[i] = 0.0f; }
+            __syncthreads();
+        }
+        if(tid == 0) { a.table[at] = ChunkTable{decay, from}; }
+        // N's blocks on the diagonal: a lane solves one column, row after row
+        if(wave == 0 && lane < C) {
+            const uint32_t block = lane & ~15u;
+            float x[16];
+            #pragma unroll
+            for(int i = 0; i < 16; i++) {
+                x[i] = m[(block + i) * MP + lane];
+                #pragma unroll
+                for(int j = 0; j < i; j++) { x[i] = __builtin_fmaf(-m[(block + i) * MP + block + j] * beta[block + j], x[j], x[i]); }
+            }
+            #pragma unroll
+            for(int i = 0; i < 16; i++) { m[(block + i) * MP + lane] = x[i]; }
+        }
+        __syncthreads();
+        // Below it: N[r] = Y - N[r][r] beta Y with Y = M[r] - sum_{s<r} M[r][s] beta N[s], a block column a wavefront
+        if(wave < B) {
+            f32x4 found[B];
+            const auto result = [&](uint32_t row) { f32x4 x; for(int r = 0; r < 4; r++) { x[r] = m[(row * 16 + 4 * g + r) * MP + wave * 16 + n16]; } return x; };
+            const auto operand = [&](uint32_t row, uint32_t column) {
+                f32x4 x;
+                #pragma unroll
+                for(int e = 0; e < 4; e++) { x[e] = -m[(row * 16 + n16) * MP + column * 16 + 4 * g + e] * beta[column * 16 + 4 * g + e]; }
+                return x;
+            };
+            #pragma unroll
+            for(int r = 0; r < B; r++) {
+                if((uint32_t)r < wave) { found[r] = f32x4{0, 0, 0, 0}; continue; }
+                found[r] = result(r);
+                if((uint32_t)r == wave) { continue; }
+                #pragma unroll
+                for(int s = 0; s < r; s++) { if((uint32_t)s >= wave) { found[r] = multiply(operand(r, s), found[s], found[r]); } }
+                found[r] = multiply(operand(r, r), found[r], found[r]);
+            }
+            #pragma unroll
+            for(int r = 0; r < B; r++) {
+                #pragma unroll
+                for(int e = 0; e < 4; e++) { correction[(r * 16 + 4 * g + e) * C + wave * 16 + n16] = -found[r][e]; }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- the walk over chunks
+enum { WALK_OUTPUTS, WALK_KEEP };          // writes outputs, or keeps states and errors for gradients
+
+// LDS of a walk, in elements of 16 bits: keys by row and by column, queries by row, -N, P
+template<typename T, int C, int DK, int MODE> struct WalkLayout
+{
+    static constexpr int NP = planesOf<T>, ROW = DK + 8, COLUMN = C + 8;
+    static constexpr uint32_t keyRows = 0, keyColumns = keyRows + NP * C * ROW, queryRows = keyColumns + NP * DK * COLUMN,
+        correction = queryRows + (MODE == WALK_OUTPUTS ? NP * C * ROW : 0), score = correction + 3 * C * COLUMN,
+        table = (score + (MODE == WALK_OUTPUTS ? 3 * C * COLUMN : 0) + 7) / 8 * 8, bytes = table * 2 + C * 16;
+};
+
+// A tile of four rows and eight columns of keys (or queries) on its way to LDS
+template<typename T> struct KeyTile { T x[4][8]; };
+template<typename T, int C, int DK> __device__ inline void loadTile(const DeltaArgs &a, const gennmi_rows_t &r, const Place &p, uint32_t keyHead, uint32_t begin, uint32_t count, uint32_t item, KeyTile<T> &tile)
+{
+    const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
+    const T *const base = rowsOf<const T>(r, a.chunks, p) + (uint64_t)begin * r.rowStride + keyHead * a.keys;
+    #pragma unroll
+    for(int i = 0; i < 4; i++) {
+        const uint32_t valid = row + i < count && at < a.keys ? min(8u, a.keys - at) : 0;
+        loadEight(base + (valid ? (uint64_t)(row + i) * r.rowStride + at : 0), valid, a.wide, tile.x[i]);
+    }
+}
+template<typename T, int NP> __device__ inline void planesOfFour(const T (&x)[4], uint2 (&out)[NP])
+{
+    const float f[4] = {widen(x[0]), widen(x[1]), widen(x[2]), widen(x[3])};
+    splitFour<NP>(f, out);
+}
+template<typename T, int C, int DK> __device__ inline void storeRows(uint16_t *to, uint32_t item, const KeyTile<T> &tile)
+{
+    constexpr int NP = planesOf<T>, PITCH = DK + 8;
+    const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
+    #pragma unroll
+    for(int i = 0; i < 4; i++) {
+        #pragma unroll
+        for(int half = 0; half < 2; half++) {
+            const T x[4] = {tile.x[i][4 * half], tile.x[i][4 * half + 1], tile.x[i][4 * half + 2], tile.x[i][4 * half + 3]};
+            uint2 words[NP];
+            planesOfFour<T, NP>(x, words);
+            #pragma unroll
+            for(int k = 0; k < NP; k++) { *(uint2*)(to + k * C * PITCH + (row + i) * PITCH + place(at + 4 * half)) = words[k]; }
+        }
+    }
+}
+template<typename T, int C, int DK> __device__ inline void storeColumns(uint16_t *to, uint32_t item, const KeyTile<T> &tile)
+{
+    constexpr int NP = planesOf<T>, PITCH = C + 8;
+    const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
+    #pragma unroll
+    for(int e = 0; e < 8; e++) {
+        const T x[4] = {tile.x[0][e], tile.x[1][e], tile.x[2][e], tile.x[3][e]};
+        uint2 words[NP];
+        planesOfFour<T, NP>(x, words);
+        #pragma unroll
+        for(int k = 0; k < NP; k++) { *(uint2*)(to + k * DK * PITCH + (at + e) * PITCH + place(row)) = words[k]; }
+    }
+}
+// [C][C] of floats as three planes, four neighbours an item
+template<int C> __device__ inline void storeSquare(uint16_t *to, uint32_t item, const float4 &x)
+{
+    constexpr int PITCH = C + 8;
+    const uint32_t row = item / (C / 4), at = item % (C / 4) * 4;
+    const float f[4] = {x.x, x.y, x.z, x.w};
+    uint2 words[3];
+    splitFour<3>(f, words);
+    #pragma unroll
+    for(int k = 0; k < 3; k++) { *(uint2*)(to + k * C * PITCH + row * PITCH + place(at)) = words[k]; }
+}
+
+// The first row of a column from which nothing is finite; rows of the chunk, if all are
+template<int C> __device__ inline uint32_t firstBad(const f32x4 (&x)[C / 16], uint32_t g)
+{
+    uint32_t first = C;
+    #pragma unroll
+    for(int t = C / 16 - 1; t >= 0; t--) {
+        #pragma unroll
+        for(int r = 3; r >= 0; r--) { if(!finite(x[t][r])) { first = 16 * t + 4 * g + r; } }
+    }
+    first = min(first, (uint32_t)__shfl_xor((int)first, 16));
+    return min(first, (uint32_t)__shfl_xor((int)first, 32));
+}
+
+// A work-group walks a sequence (or a segment of it) of one head with 16 columns of the state a wavefront.
+template<typename T, int C, int DK, int WAVES, int MODE>
+__global__ __launch_bounds__(64 * WAVES)
+void deltaStateKernel(DeltaArgs a)
+{
+    typedef WalkLayout<T, C, DK, MODE> L;
+    constexpr int NP = planesOf<T>, THREADS = 64 * WAVES, TILES = C / 16, STATE = DK / 16;
+    constexpr bool OUTPUTS = MODE == WALK_OUTPUTS;
+    constexpr int KEYS = C * DK / 32, KEY_ITEMS = KEYS * (OUTPUTS ? 2 : 1), EACH = (KEY_ITEMS + THREADS - 1) / THREADS, SQUARE = C * C / 4, SQUARES = (SQUARE + THREADS - 1) / THREADS;
+    extern __shared__ __align__(16) char lds[];
+    uint16_t *const planes = (uint16_t*)lds;
+    float4 *const table = (float4*)(planes + L::table);
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
+    const uint32_t block = blockIdx.x % a.columnBlocks, rest = blockIdx.x / a.columnBlocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
+    Place p;
+    if(!locate(a.segments, segment, p)) { return; }
+    const uint32_t begin = p.index * a.segments.chunk, end = min(p.length, begin + a.segments.chunk);
+    const uint32_t column = (block * WAVES + wave) * 16 + n16;
+    const bool active = (block * WAVES + wave) * 16 < (OUTPUTS ? a.values : a.padded), inside = column < a.values;
+    const uint32_t chunks = end > begin ? (end - begin + C - 1) / C : 0;
+    const uint64_t firstNumber = firstChunk(a.chunks, p.sequence) + begin / C;
+
+    f32x4 state[STATE];
+    #pragma unroll
+    for(int t = 0; t < STATE; t++) {
+        #pragma unroll
+        for(int r = 0; r < 4; r++) {
+            const uint32_t row = 16 * t + 4 * g + r;
+            state[t][r] = a.initialState && row < a.keys && inside ? a.initialState[(((uint64_t)p.state * a.heads + head) * a.keys + row) * a.values + column] : 0.0f;
+        }
+    }
+
+    KeyTile<T> keyTiles[EACH];
+    float4 corrections[SQUARES], scores[SQUARES];
+    float4 rowTable;
+    const auto prefetch = [&](uint32_t n) {
+        const uint32_t first = begin + n * C, count = min((uint32_t)C, end - first);
+        const uint64_t at = (firstNumber + n) * a.heads + head;
+        #pragma unroll
+        for(int i = 0; i < EACH; i++) {
+            const uint32_t item = tid + i * THREADS;
+            if(KEY_ITEMS % THREADS && item >= KEY_ITEMS) { break; }
+            if(!OUTPUTS || item < KEYS) { loadTile<T, C, DK>(a, a.k, p, keyHead, first, count, item, keyTiles[i]); }
+            else { loadTile<T, C, DK>(a, a.q, p, keyHead, first, count, item - KEYS, keyTiles[i]); }
+        }
+        #pragma unroll
+        for(int i = 0; i < SQUARES; i++) {
+            const uint32_t item = tid + i * THREADS;
+            if(SQUARE % THREADS && item >= SQUARE) { break; }
+            corrections[i] = ((const float4*)(a.correction + at * C * C))[item];
+            if(OUTPUTS) { scores[i] = ((const float4*)(a.score + at * C * C))[item]; }
+        }
+        if(tid < C) { rowTable = *(const float4*)(a.rows + at * C + tid); }
+    };
+    if(chunks) { prefetch(0); }
+    for(uint32_t n = 0; n < chunks; n++) {
+        const uint32_t first = begin + n * C, count = min((uint32_t)C, end - first);
+        const uint64_t at = (firstNumber + n) * a.heads + head;
+        const ChunkTable chunk = a.table[at];
+        __syncthreads();
+        #pragma unroll
+        for(int i = 0; i < EACH; i++) {
+            const uint32_t item = tid + i * THREADS;
+            if(KEY_ITEMS % THREADS && item >= KEY_ITEMS) { break; }
+            if(!OUTPUTS || item < KEYS) {
+                storeRows<T, C, DK>(planes + L::keyRows, item, keyTiles[i]);
+                storeColumns<T, C, DK>(planes + L::keyColumns, item, keyTiles[i]);
+            }
+            else { storeRows<T, C, DK>(planes + L::queryRows, item - KEYS, keyTiles[i]); }
+        }
+        #pragma unroll
+        for(int i = 0; i < SQUARES; i++) {
+            const uint32_t item = tid + i * THREADS;
+            if(SQUARE % THREADS && item >= SQUARE) { break; }
+            storeSquare<C>(planes + L::correction, item, corrections[i]);
+            if(OUTPUTS) { storeSquare<C>(planes + L::score, item, scores[i]); }
+        }
+        if(tid < C) { table[tid] = rowTable; }
+        __syncthreads();
+        if(n + 1 < chunks) { prefetch(n + 1); }
+        if(!active) { continue; }
+
+        // r = v - G k^ S, and the part of the outputs that the state in front has
+        const T *const values = rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)first * a.v.rowStride + head * a.values + column;
+        f32x4 w[TILES], x[TILES], o[TILES];
+        #pragma unroll
+        for(int t = 0; t < TILES; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = 16 * t + 4 * g + r;
+                w[t][r] = inside && row < count ? widen(values[(uint64_t)row * a.v.rowStride]) : 0.0f;
+            }
+            x[t] = o[t] = f32x4{0, 0, 0, 0};
+        }
+        if(!OUTPUTS) {
+            float *const kept = a.states + at * DK * a.padded + column;
+            #pragma unroll
+            for(int t = 0; t < STATE; t++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) { kept[(16 * t + 4 * g + r) * a.padded] = state[t][r]; }
+            }
+        }
+        #pragma unroll
+        for(int s = 0; s < DK / 32; s++) {
+            const Planes<3> b = split<3>(state[2 * s], state[2 * s + 1]);
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) {
+                const uint32_t offset = (16 * t + n16) * L::ROW + 32 * s + 8 * g;
+                x[t] = multiply(fetch<NP>(planes + L::keyRows + offset, C * L::ROW), b, x[t]);
+                if(OUTPUTS) { o[t] = multiply(fetch<NP>(planes + L::queryRows + offset, C * L::ROW), b, o[t]); }
+            }
+        }
+        float notFinite = 0.0f;
+        #pragma unroll
+        for(int t = 0; t < TILES; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const float4 row = table[16 * t + 4 * g + r];
+                w[t][r] = __builtin_fmaf(-row.x, x[t][r], w[t][r]);
+                o[t][r] *= row.w;
+                notFinite = __builtin_fmaf(w[t][r], 0.0f, notFinite);
+            }
+        }
+        uint32_t bad = chunk.bad;
+        if(__builtin_expect(__ballot(notFinite != 0.0f) != 0 || bad < C, 0)) {
+            // (what is not finite must not reach rows before it: 0 times it is not 0)
+            bad = min(bad, firstBad<C>(w, g));
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r >= bad) { w[t][r] = 0.0f; } }
+            }
+        }
+        // w = r - N beta r; tiles above the diagonal are zero
+        {
+            Planes<3> b[TILES / 2];
+            #pragma unroll
+            for(int s = 0; s < TILES / 2; s++) {
+                f32x4 y[2];
+                #pragma unroll
+                for(int h = 0; h < 2; h++) {
+                    #pragma unroll
+                    for(int r = 0; r < 4; r++) { y[h][r] = w[2 * s + h][r] * table[16 * (2 * s + h) + 4 * g + r].y; }
+                }
+                b[s] = split<3>(y[0], y[1]);
+            }
+            #pragma unroll
+            for(int s = 0; s < TILES / 2; s++) {
+                #pragma unroll
+                for(int t = 2 * s; t < TILES; t++) {
+                    w[t] = multiply(fetch<3>(planes + L::correction + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b[s], w[t]);
+                }
+            }
+        }
+        if(!OUTPUTS) {
+            float *const kept = a.errors + at * C * a.padded + column;
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) { kept[(16 * t + 4 * g + r) * a.padded] = 16 * t + 4 * g + r < bad ? w[t][r] : __builtin_nanf(""); }
+            }
+        }
+        // out += P u, and the state behind the chunk
+        #pragma unroll
+        for(int t = 0; t < STATE; t++) { state[t] *= chunk.decay; }
+        #pragma unroll
+        for(int s = 0; s < TILES / 2; s++) {
+            f32x4 u[2], left[2];
+            #pragma unroll
+            for(int h = 0; h < 2; h++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) {
+                    const float4 row = table[16 * (2 * s + h) + 4 * g + r];
+                    u[h][r] = w[2 * s + h][r] * row.y;
+                    left[h][r] = u[h][r] * row.z;
+                }
+            }
+            if(OUTPUTS) {
+                const Planes<3> b = split<3>(u[0], u[1]);
+                #pragma unroll
+                for(int t = 2 * s; t < TILES; t++) { o[t] = multiply(fetch<3>(planes + L::score + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, o[t]); }
+            }
+            const Planes<3> b = split<3>(left[0], left[1]);
+            #pragma unroll
+            for(int t = 0; t < STATE; t++) { state[t] = multiply(fetch<NP>(planes + L::keyColumns + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, DK * L::COLUMN), b, state[t]); }
+        }
+        if(__builtin_expect(bad < C, 0)) {
+            const float no = __builtin_nanf("");
+            #pragma unroll
+            for(int t = 0; t < STATE; t++) { state[t] = f32x4{no, no, no, no}; }
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r >= bad) { o[t][r] = no; } }
+            }
+        }
+        if(OUTPUTS && inside) {
+            T *const out = rowsOf<T>(a.out, a.chunks, p) + (uint64_t)first * a.out.rowStride + head * a.values + column;
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) {
+                    const uint32_t row = 16 * t + 4 * g + r;
+                    if(row < count) { out[(uint64_t)row * a.out.rowStride] = narrow<T>(o[t][r]); }
+                }
+            }
+        }
+    }
+    if(a.finalState && inside && end == p.length) {
+        #pragma unroll
+        for(int t = 0; t < STATE; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = 16 * t + 4 * g + r;
+                if(row < a.keys) { a.finalState[(((uint64_t)p.state * a.heads + head) * a.keys + row) * a.values + column] = state[t][r]; }
+            }
+        }
+    }
+}
+
+// ---- gradients: the same walk from the other end
+// dR = (I - beta N')' of dU, row by row what the loss says of u through everything behind it; v's gradient is beta dR.
+struct DeltaGradientArgs
+{
+    gennmi_rows_t out, q, k, v, g, beta;
+    const float *finalState;
+    float *initialState;
+    float *states, *errors;         // the gradient of the state behind each chunk [DK][padded], dR [C][padded]
+};
+template<typename T, int C, int DK> struct ReverseLayout
+{
+    static constexpr int NP = planesOf<T>, ROW = DK + 8, COLUMN = C + 8;
+    static constexpr uint32_t keyRows = 0, keyColumns = keyRows + NP * C * ROW, queryColumns = keyColumns + NP * DK * COLUMN, correction = queryColumns + NP * DK * COLUMN,
+        score = correction + 3 * C * COLUMN, table = (score + 3 * C * COLUMN + 7) / 8 * 8, bytes = table * 2 + C * 16;
+};
+// Four rows and four columns of a square, stored by column
+struct SquareTile { float4 x[4]; };
+template<int C> __device__ inline void loadSquareTile(const float *from, uint32_t item, SquareTile &tile)
+{
+    const uint32_t row = item / (C / 4) * 4, at = item % (C / 4) * 4;
+    #pragma unroll
+    for(int i = 0; i < 4; i++) { tile.x[i] = *(const float4*)(from + (row + i) * C + at); }
+}
+template<int C> __device__ inline void storeSquareColumns(uint16_t *to, uint32_t item, const SquareTile &tile)
+{
+    constexpr int PITCH = C + 8;
+    const uint32_t row = item / (C / 4) * 4, at = item % (C / 4) * 4;
+    #pragma unroll
+    for(int e = 0; e < 4; e++) {
+        const auto part = [&](const float4 &x) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
+        const float f[4] = {part(tile.x[0]), part(tile.x[1]), part(tile.x[2]), part(tile.x[3])};
+        uint2 words[3];
+        splitFour<3>(f, words);
+        #pragma unroll
+        for(int k = 0; k < 3; k++) { *(uint2*)(to + k * C * PITCH + (at + e) * PITCH + place(row)) = words[k]; }
+    }
+}
+
+template<typename T, int C, int DK, int WAVES>
+__global__ __launch_bounds__(64 * WAVES)
+void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
+{
+    typedef ReverseLayout<T, C, DK> L;
+    constexpr int NP = planesOf<T>, THREADS = 64 * WAVES, TILES = C / 16, STATE = DK / 16;
+    constexpr int KEYS = C * DK / 32, KEY_ITEMS = 2 * KEYS, EACH = (KEY_ITEMS + THREADS - 1) / THREADS, SQUARE = C * C / 16, SQUARE_ITEMS = 2 * SQUARE, SQUARES = (SQUARE_ITEMS + THREADS - 1) / THREADS;
+    extern __shared__ __align__(16) char lds[];
+    uint16_t *const planes = (uint16_t*)lds;
+    float4 *const table = (float4*)(planes + L::table);
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
+    const uint32_t block = blockIdx.x % a.columnBlocks, rest = blockIdx.x / a.columnBlocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
+    Place p;
+    if(!locate(a.segments, segment, p)) { return; }
+    const uint32_t begin = p.index * a.segments.chunk, end = min(p.length, begin + a.segments.chunk);
+    const uint32_t column = (block * WAVES + wave) * 16 + n16;
+    const bool active = (block * WAVES + wave) * 16 < a.padded, inside = column < a.values;
+    const uint32_t chunks = end > begin ? (end - begin + C - 1) / C : 0;
+    const uint64_t firstNumber = firstChunk(a.chunks, p.sequence) + begin / C;
+
+    f32x4 state[STATE];
+    #pragma unroll
+    for(int t = 0; t < STATE; t++) {
+        #pragma unroll
+        for(int r = 0; r < 4; r++) {
+            const uint32_t row = 16 * t + 4 * g + r;
+            state[t][r] = d.finalState && row < a.keys && inside ? d.finalState[(((uint64_t)p.sequence * a.heads + head) * a.keys + row) * a.values + column] : 0.0f;
+        }
+    }
+    KeyTile<T> keyTiles[EACH];
+    SquareTile squares[SQUARES];
+    float4 rowTable;
+    const auto prefetch = [&](uint32_t n) {
+        const uint32_t first = begin + n * C, count = min((uint32_t)C, end - first);
+        const uint64_t at = (firstNumber + n) * a.heads + head;
+        #pragma unroll
+        for(int i = 0; i < EACH; i++) {
+            const uint32_t item = tid + i * THREADS;
+            if(KEY_ITEMS % THREADS && item >= KEY_ITEMS) { break; }
+            if(item < KEYS) { loadTile<T, C, DK>(a, a.k, p, keyHead, first, count, item, keyTiles[i]); }
+            else { loadTile<T, C, DK>(a, a.q, p, keyHead, first, count, item - KEYS, keyTiles[i]); }
+        }
+        #pragma unroll
+        for(int i = 0; i < SQUARES; i++) {
+            const uint32_t item = tid + i * THREADS;
+            if(SQUARE_ITEMS % THREADS && item >= SQUARE_ITEMS) { break; }
+            loadSquareTile<C>((item < SQUARE ? a.correction : a.score) + at * C * C, item < SQUARE ? item : item - SQUARE, squares[i]);
+        }
+        if(tid < C) { rowTable = *(const float4*)(a.rows + at * C + tid); }
+    };
+    if(chunks) { prefetch(chunks - 1); }
+    for(uint32_t left = chunks; left > 0; left--) {
+        const uint32_t n = left - 1, first = begin + n * C, count = min((uint32_t)C, end - first);
+        const uint64_t at = (firstNumber + n) * a.heads + head;
+        const float decay = a.table[at].decay;
+        __syncthreads();
+        #pragma unroll
+        for(int i = 0; i < EACH; i++) {
+            const uint32_t item = tid + i * THREADS;
+            if(KEY_ITEMS % THREADS && item >= KEY_ITEMS) { break; }
+            if(item < KEYS) {
+                storeRows<T, C, DK>(planes + L::keyRows, item, keyTiles[i]);
+                storeColumns<T, C, DK>(planes + L::keyColumns, item, keyTiles[i]);
+            }
+            else { storeColumns<T, C, DK>(planes + L::queryColumns, item - KEYS, keyTiles[i]); }
+        }
+        #pragma unroll
+        for(int i = 0; i < SQUARES; i++) {
+            const uint32_t item = tid + i * THREADS;
+            if(SQUARE_ITEMS % THREADS && item >= SQUARE_ITEMS) { break; }
+            storeSquareColumns<C>(planes + (item < SQUARE ? L::correction : L::score), item < SQUARE ? item : item - SQUARE, squares[i]);
+        }
+        if(tid < C) { table[tid] = rowTable; }
+        __syncthreads();
+        if(n > 0) { prefetch(n - 1); }
+        if(!active) { continue; }
+
+        const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)first * d.out.rowStride + head * a.values + column;
+        f32x4 dout[TILES], du[TILES];
+        #pragma unroll
+        for(int t = 0; t < TILES; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = 16 * t + 4 * g + r;
+                dout[t][r] = inside && row < count ? widen(douts[(uint64_t)row * d.out.rowStride]) : 0.0f;
+            }
+            du[t] = f32x4{0, 0, 0, 0};
+        }
+        float *const keptState = d.states + at * DK * a.padded + column;
+        #pragma unroll
+        for(int t = 0; t < STATE; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { keptState[(16 * t + 4 * g + r) * a.padded] = state[t][r]; }
+        }
+        // dU = D[last] k^ dS + P' dout
+        #pragma unroll
+        for(int s = 0; s < DK / 32; s++) {
+            const Planes<3> b = split<3>(state[2 * s], state[2 * s + 1]);
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) { du[t] = multiply(fetch<NP>(planes + L::keyRows + (16 * t + n16) * L::ROW + 32 * s + 8 * g, C * L::ROW), b, du[t]); }
+        }
+        #pragma unroll
+        for(int t = 0; t < TILES; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { du[t][r] *= table[16 * t + 4 * g + r].z; }
+        }
+        #pragma unroll
+        for(int s = 0; s < TILES / 2; s++) {
+            const Planes<NP> b = split<NP>(dout[2 * s], dout[2 * s + 1]);
+            #pragma unroll
+            for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(fetch<3>(planes + L::score + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, du[t]); }
+        }
+        // dR = dU - N' beta dU
+        {
+            Planes<3> b[TILES / 2];
+            #pragma unroll
+            for(int s = 0; s < TILES / 2; s++) {
+                f32x4 y[2];
+                #pragma unroll
+                for(int h = 0; h < 2; h++) {
+                    #pragma unroll
+                    for(int r = 0; r < 4; r++) { y[h][r] = du[2 * s + h][r] * table[16 * (2 * s + h) + 4 * g + r].y; }
+                }
+                b[s] = split<3>(y[0], y[1]);
+            }
+            #pragma unroll
+            for(int s = 0; s < TILES / 2; s++) {
+                #pragma unroll
+                for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(fetch<3>(planes + L::correction + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b[s], du[t]); }
+            }
+        }
+        float *const keptError = d.errors + at * C * a.padded + column;
+        #pragma unroll
+        for(int t = 0; t < TILES; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { keptError[(16 * t + 4 * g + r) * a.padded] = du[t][r]; }
+        }
+        // dS in front of the chunk = G[last] dS + (scale G q^)' dout - (G k^)' (beta dR)
+        #pragma unroll
+        for(int t = 0; t < STATE; t++) { state[t] *= decay; }
+        #pragma unroll
+        for(int s = 0; s < TILES / 2; s++) {
+            f32x4 x[2], y[2];
+            #pragma unroll
+            for(int h = 0; h < 2; h++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) {
+                    const float4 row = table[16 * (2 * s + h) + 4 * g + r];
+                    x[h][r] = dout[2 * s + h][r] * row.w;
+                    du[2 * s + h][r] *= row.y;
+                    y[h][r] = -row.x * du[2 * s + h][r];
+                }
+            }
+            const Planes<3> bx = split<3>(x[0], x[1]), by = split<3>(y[0], y[1]);
+            #pragma unroll
+            for(int t = 0; t < STATE; t++) {
+                const uint32_t offset = (16 * t + n16) * L::COLUMN + 32 * s + 8 * g;
+                state[t] = multiply(fetch<NP>(planes + L::queryColumns + offset, DK * L::COLUMN), bx, state[t]);
+                state[t] = multiply(fetch<NP>(planes + L::keyColumns + offset, DK * L::COLUMN), by, state[t]);
+            }
+        }
+        if(d.v.data && inside) {
+            T *const dv = rowsOf<T>(d.v, a.chunks, p) + (uint64_t)first * d.v.rowStride + head * a.values + column;
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) {
+                    const uint32_t row = 16 * t + 4 * g + r;
+                    if(row < count) { dv[(uint64_t)row * d.v.rowStride] = narrow<T>(du[t][r]); }
+                }
+            }
+        }
+    }
+    if(d.initialState && inside && begin == 0) {
+        #pragma unroll
+        for(int t = 0; t < STATE; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = 16 * t + 4 * g + r;
+                if(row < a.keys) { d.initialState[(((uint64_t)p.sequence * a.heads + head) * a.keys + row) * a.values + column] = state[t][r]; }
+            }
+        }
+    }
+}
+
+// ---- gradients of a chunk, once the state in front of it, w, the gradient of the state behind it and dR are known
+//   dq^ = scale G (dout S') + sum_j dQK[i][j] k^[j],   dQK[i][j] = scale D[i][j] dout[i].u[j] for i >= j
+//   dk^ = beta (D[last] w dS' - G dR S') + sum_i dQK[i][j] q^[i] + sum_j (dKK + dKK')[i][j] k^[j],   dKK[i][j] = -D[i][j] beta[i] beta[j] dR[i].w[j] for i > j
+//   dbeta[i] = w[i].dR[i]
+// and g's: with states and u in units of the decay so far, outputs grow with it and values shrink, so that what the sum of g up to row i gains the loss
+// is q^[i].dq^[i] - v[i].dv[i], and at the chunk's last row the state behind it times its gradient as well.
+// A work-group has a chunk and a key head and adds up the heads that share it.  Products are summed over the values, 32 at a time, with what multiplies S and dS
+// in LDS; a wavefront has 16 keys' columns of the results, S' and dS' straight from memory.
+template<typename T, int C, int DK> struct GradientLayout
+{
+    static constexpr int NP = planesOf<T>, COLUMN = C + 8, VALUES = 40;
+    static constexpr uint32_t keyColumns = 0, queryColumns = keyColumns + NP * DK * COLUMN, stage = queryColumns + NP * DK * COLUMN,
+        staged = (NP + 6) * C * VALUES, square = 3 * C * COLUMN, floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (6 + 2 * 8 + 1) + 64;
+};
+
+template<typename T, int C, int DK>
+__global__ __launch_bounds__(512)
+void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
+{
+    typedef GradientLayout<T, C, DK> L;
+    constexpr int NP = planesOf<T>, TILES = C / 16, KEY_TILES = DK / 16, SPLIT = 8 / KEY_TILES, MINE = TILES / SPLIT, SQUARES = C == 64 ? 2 : 1, KEYS = C * DK / 32, VP = C * L::VALUES;
+    extern __shared__ __align__(16) char lds[];
+    uint16_t *const planes = (uint16_t*)lds, *const stage = planes + L::stage;
+    uint16_t *const doutPlanes = stage, *const dRPlanes = stage + NP * VP, *const wPlanes = dRPlanes + 3 * VP;
+    double *const sums = (double*)(planes + L::floats);
+    float *const since = (float*)(sums + C), *const until = since + C, *const beta = until + C, *const keyUnit = beta + C, *const queryUnit = keyUnit + C, *const valueDots = queryUnit + C;
+    float *const queryDots = valueDots + C, *const keyDots = queryDots + 8 * C, *const ends = keyDots + 8 * C;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
+    const uint32_t number = blockIdx.x / a.keyHeads, keyHead = blockIdx.x - number * a.keyHeads;
+    Place p;
+    if(!locate(a.chunks, number, p)) { return; }
+    const uint32_t begin = p.index * C, count = min((uint32_t)C, p.length - min(p.length, begin));
+    if(!count) { return; }
+
+    // tiles of this wavefront: 16 keys and every SPLIT-th 16 rows; rows and columns of squares
+    const uint32_t keyTile = wave % KEY_TILES, firstRow = wave / KEY_TILES, key = keyTile * 16 + n16;
+    const auto tileOf = [&](int m) { return firstRow + SPLIT * m; };
+    const auto squareRow = [&](int q) { return C == 64 ? (wave >> 2) + 2 * q : wave >> 1; };
+    const uint32_t squareColumn = C == 64 ? wave & 3 : wave & 1;
+    const bool squares = C == 64 || wave < 4;
+
+    #pragma unroll
+    for(int i = 0; i < (2 * KEYS + 511) / 512; i++) {
+        const uint32_t item = tid + i * 512;
+        if(2 * KEYS % 512 && item >= 2 * KEYS) { break; }
+        KeyTile<T> tile;
+        const bool isKey = item < KEYS;
+        loadTile<T, C, DK>(a, isKey ? a.k : a.q, p, keyHead, begin, count, isKey ? item : item - KEYS, tile);
+        // (rows in their order here)
+        const uint32_t it = isKey ? item : item - KEYS, row = it / (DK / 8) * 4, at = it % (DK / 8) * 8;
+        uint16_t *const to = planes + (isKey ? L::keyColumns : L::queryColumns);
+        #pragma unroll
+        for(int e = 0; e < 8; e++) {
+            const T x[4] = {tile.x[0][e], tile.x[1][e], tile.x[2][e], tile.x[3][e]};
+            uint2 words[NP];
+            planesOfFour<T, NP>(x, words);
+            #pragma unroll
+            for(int k = 0; k < NP; k++) { *(uint2*)(to + k * DK * L::COLUMN + (at + e) * L::COLUMN + row) = words[k]; }
+        }
+    }
+    // the key's (or query's) values at this lane's column, four rows of a tile
+    const auto valuesAt = [&](uint32_t from, uint32_t tile) {
+        f32x4 x = {0, 0, 0, 0};
+        #pragma unroll
+        for(int k = 0; k < NP; k++) {
+            const uint2 w = *(const uint2*)(planes + from + k * DK * L::COLUMN + key * L::COLUMN + tile * 16 + 4 * g);
+            x[0] += __uint_as_float(w.x << 16); x[1] += __uint_as_float(w.x & 0xffff0000u);
+            x[2] += __uint_as_float(w.y << 16); x[3] += __uint_as_float(w.y & 0xffff0000u);
+        }
+        return x;
+    };
+    const auto sumOf16 = [](float x) { x += partner<1>(x); x += partner<2>(x); x += partner<4>(x); return x + partner<8>(x); };
+
+    f32x4 dq[MINE], dk[MINE], dqk[SQUARES], dkk[SQUARES];
+    #pragma unroll
+    for(int m = 0; m < MINE; m++) { dq[m] = dk[m] = f32x4{0, 0, 0, 0}; }
+    #pragma unroll
+    for(int q = 0; q < SQUARES; q++) { dqk[q] = dkk[q] = f32x4{0, 0, 0, 0}; }
+    const bool stages = tid < C * 8;
+    const uint32_t stageRow = tid / 8, stageAt = tid % 8 * 4;
+
+    for(uint32_t inGroup = 0; inGroup < a.group; inGroup++) {
+        const uint32_t head = keyHead * a.group + inGroup;
+        const uint64_t at = (uint64_t)number * a.heads + head;
+        __syncthreads();
+        const float decay = a.table[at].decay;
+        if(tid < C) {
+            const RowTable row = a.rows[at * C + tid];
+            const double last = a.rows[at * C + C - 1].sum;
+            sums[tid] = row.sum;
+            since[tid] = decayOver(row.sum);
+            until[tid] = decayOver(last - row.sum);
+            beta[tid] = row.beta;
+            keyUnit[tid] = row.keyUnit;
+            queryUnit[tid] = row.queryUnit;
+        }
+        f32x4 outS[MINE], rS[MINE], wD[MINE], outW[SQUARES], rW[SQUARES];
+        #pragma unroll
+        for(int m = 0; m < MINE; m++) { outS[m] = rS[m] = wD[m] = f32x4{0, 0, 0, 0}; }
+        #pragma unroll
+        for(int q = 0; q < SQUARES; q++) { outW[q] = rW[q] = f32x4{0, 0, 0, 0}; }
+        float stateDot = 0.0f, valueDot = 0.0f, betaDot = 0.0f;
+        const float *const stateRow = a.states + at * DK * a.padded + (uint64_t)key * a.padded + 8 * g, *const dStateRow = d.states + at * DK * a.padded + (uint64_t)key * a.padded + 8 * g;
+        const uint32_t stageRowUsed = stages && stageRow < count ? stageRow : 0;
+        const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)(begin + stageRowUsed) * d.out.rowStride + head * a.values;
+        const T *const values = rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)(begin + stageRowUsed) * a.v.rowStride + head * a.values;
+        const float *const dRRow = d.errors + (at * C + stageRowUsed) * a.padded, *const wRow = a.errors + (at * C + stageRowUsed) * a.padded;
+        for(uint32_t v = 0; v < a.padded; v += 32) {
+            float4 s0[2], ds[2];
+            #pragma unroll
+            for(int h = 0; h < 2; h++) { s0[h] = *(const float4*)(stateRow + v + 4 * h); ds[h] = *(const float4*)(dStateRow + v + 4 * h); }
+            float dout[4] = {0, 0, 0, 0}, dr[4] = {0, 0, 0, 0}, w[4] = {0, 0, 0, 0};
+            if(stages && stageRow < count) {
+                const float4 x = *(const float4*)(dRRow + v + stageAt), y = *(const float4*)(wRow + v + stageAt);
+                dr[0] = x.x; dr[1] = x.y; dr[2] = x.z; dr[3] = x.w;
+                w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
+                #pragma unroll
+                for(int e = 0; e < 4; e++) {
+                    if(v + stageAt + e < a.values) {
+                        dout[e] = widen(douts[v + stageAt + e]);
+                        valueDot = __builtin_fmaf(widen(values[v + stageAt + e]), dr[e], valueDot);
+                        betaDot = __builtin_fmaf(w[e], dr[e], betaDot);
+                    }
+                }
+            }
+            __syncthreads();
+            if(stages) {
+                uint2 words[3];
+                uint16_t *const to = stage + stageRow * L::VALUES + stageAt;
+                uint2 own[NP];
+                splitFour<NP>(dout, own);
+                #pragma unroll
+                for(int k = 0; k < NP; k++) { *(uint2*)(to + k * VP) = own[k]; }
+                splitFour<3>(dr, words);
+                #pragma unroll
+                for(int k = 0; k < 3; k++) { *(uint2*)(to + (NP + k) * VP) = words[k]; }
+                splitFour<3>(w, words);
+                #pragma unroll
+                for(int k = 0; k < 3; k++) { *(uint2*)(to + (NP + 3 + k) * VP) = words[k]; }
+            }
+            __syncthreads();
+            const f32x4 s0a = {s0[0].x, s0[0].y, s0[0].z, s0[0].w}, s0b = {s0[1].x, s0[1].y, s0[1].z, s0[1].w};
+            const f32x4 dsa = {ds[0].x, ds[0].y, ds[0].z, ds[0].w}, dsb = {ds[1].x, ds[1].y, ds[1].z, ds[1].w};
+            #pragma unroll
+            for(int e = 0; e < 4; e++) { stateDot = __builtin_fmaf(s0a[e], dsa[e], stateDot); stateDot = __builtin_fmaf(s0b[e], dsb[e], stateDot); }
+            const Planes<3> state = split<3>(s0a, s0b), dState = split<3>(dsa, dsb);
+            #pragma unroll
+            for(int m = 0; m < MINE; m++) {
+                const uint32_t offset = (tileOf(m) * 16 + n16) * L::VALUES + 8 * g;
+                outS[m] = multiply(fetch<NP>(doutPlanes + offset, VP), state, outS[m]);
+                rS[m] = multiply(fetch<3>(dRPlanes + offset, VP), state, rS[m]);
+                wD[m] = multiply(fetch<3>(wPlanes + offset, VP), dState, wD[m]);
+            }
+            if(squares) {
+                const Planes<3> other = fetch<3>(wPlanes + (squareColumn * 16 + n16) * L::VALUES + 8 * g, VP);
+                #pragma unroll
+                for(int q = 0; q < SQUARES; q++) {
+                    if(squareRow(q) < squareColumn) { continue; }
+                    const uint32_t offset = (squareRow(q) * 16 + n16) * L::VALUES + 8 * g;
+                    outW[q] = multiply(fetch<NP>(doutPlanes + offset, VP), other, outW[q]);
+                    rW[q] = multiply(fetch<3>(dRPlanes + offset, VP), other, rW[q]);
+                }
+            }
+        }
+        // what this head adds, and its gates' share
+        float endDot = 0.0f;
+        #pragma unroll
+        for(int m = 0; m < MINE; m++) {
+            const f32x4 q = valuesAt(L::queryColumns, tileOf(m)), k = valuesAt(L::keyColumns, tileOf(m));
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = tileOf(m) * 16 + 4 * g + r;
+                const float x = a.scale * since[row] * outS[m][r], y = until[row] * beta[row] * wD[m][r];
+                dq[m][r] += x;
+                dk[m][r] += y - since[row] * beta[row] * rS[m][r];
+                endDot = __builtin_fmaf(k[r] * keyUnit[row], y, endDot);
+                const float dot = sumOf16(q[r] * queryUnit[row] * x);
+                if(n16 == 0) { queryDots[(firstRow * KEY_TILES + keyTile) * C + row] = dot; }
+            }
+        }
+        #pragma unroll
+        for(int q = 0; q < SQUARES; q++) {
+            const uint32_t column = squareColumn * 16 + n16;
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = squareRow(q) * 16 + 4 * g + r;
+                float dot = 0.0f;
+                if(squares && row >= column) {
+                    const float between = decayOver(sums[row] - sums[column]), x = outW[q][r] * beta[column];
+                    dqk[q][r] = __builtin_fmaf(a.scale * between, x, dqk[q][r]);
+                    if(row > column) { dkk[q][r] -= between * (beta[row] * beta[column] * rW[q][r]); }
+                    dot = x * a.score[(at * C + row) * C + column];
+                }
+                dot = sumOf16(dot);
+                if(squares && n16 == 0) { keyDots[squareColumn * C + row] = dot; }
+            }
+        }
+        #pragma unroll
+        for(int w = 1; w < 64; w *= 2) { stateDot += __shfl_xor(stateDot, w); endDot += __shfl_xor(endDot, w); }
+        if(lane == 0) { ends[wave] = wave < KEY_TILES ? decay * stateDot + endDot : endDot; }
+        valueDot += partner<1>(valueDot); valueDot += partner<2>(valueDot); valueDot += partner<4>(valueDot);
+        betaDot += partner<1>(betaDot); betaDot += partner<2>(betaDot); betaDot += partner<4>(betaDot);
+        if(stages && stageAt == 0) {
+            valueDots[stageRow] = valueDot * beta[stageRow];
+            if(d.beta.data && stageRow < count) { (rowsOf<float>(d.beta, a.chunks, p) + (uint64_t)(begin + stageRow) * d.beta.rowStride)[head] = betaDot; }
+        }
+        __syncthreads();
+        if(d.g.data && wave == 0) {
+            double sum = 0.0;
+            if(lane < C) {
+                sum = -(double)valueDots[lane];
+                // (a row's dots lie with the wavefronts that have its tile: all of DK / 16 key tiles)
+                const uint32_t group = (lane / 16) % SPLIT;
+                #pragma unroll
+                for(int w = 0; w < KEY_TILES; w++) { sum += queryDots[(group * KEY_TILES + w) * C + lane]; }
+                #pragma unroll
+                for(int w = 0; w < TILES; w++) { sum += keyDots[w * C + lane]; }
+                if(lane == C - 1) {
+                    #pragma unroll
+                    for(int w = 0; w < 8; w++) { sum += ends[w]; }
+                }
+            }
+            #pragma unroll
+            for(int w = 1; w < C; w *= 2) {
+                const double behind = __shfl_down(sum, w);
+                if(lane + w < C) { sum += behind; }
+            }
+            if(lane < count) { (rowsOf<float>(d.g, a.chunks, p) + (uint64_t)(begin + lane) * d.g.rowStride)[head] = (float)sum; }
+        }
+    }
+
+    // squares times queries and keys
+    const auto storeSquares = [&](bool transposed, auto &&value) {
+        #pragma unroll
+        for(int q = 0; q < SQUARES; q++) {
+            const uint32_t column = squareColumn * 16 + n16, row = squareRow(q) * 16 + 4 * g;
+            float x[4];
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { x[r] = value(q, r, row + r, column); }
+            uint2 words[3];
+            splitFour<3>(x, words);
+            #pragma unroll
+            for(int k = 0; k < 3; k++) {
+                if(transposed) { *(uint2*)(stage + (k * C + column) * L::COLUMN + row) = words[k]; }
+                else {
+                    uint16_t *const to = stage + (k * C + row) * L::COLUMN + column;
+                    to[0] = (uint16_t)words[k].x; to[L::COLUMN] = (uint16_t)(words[k].x >> 16);
+                    to[2 * L::COLUMN] = (uint16_t)words[k].y; to[3 * L::COLUMN] = (uint16_t)(words[k].y >> 16);
+                }
+            }
+        }
+    };
+    const auto timesColumns = [&](uint32_t from, f32x4 (&to)[MINE]) {
+        #pragma unroll
+        for(int s = 0; s < TILES / 2; s++) {
+            const Planes<NP> b = fetch<NP>(planes + from + key * L::COLUMN + 32 * s + 8 * g, DK * L::COLUMN);
+            #pragma unroll
+            for(int m = 0; m < MINE; m++) { to[m] = multiply(fetch<3>(stage + (tileOf(m) * 16 + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, to[m]); }
+        }
+    };
+    __syncthreads();
+    if(squares) { storeSquares(false, [&](int q, int r, uint32_t row, uint32_t column) { return dqk[q][r] * keyUnit[column]; }); }
+    __syncthreads();
+    timesColumns(L::keyColumns, dq);
+    __syncthreads();
+    if(squares) { storeSquares(true, [&](int q, int r, uint32_t row, uint32_t column) { return dqk[q][r] * queryUnit[row]; }); }
+    __syncthreads();
+    timesColumns(L::queryColumns, dk);
+    __syncthreads();
+    if(squares) { storeSquares(false, [&](int q, int r, uint32_t row, uint32_t column) { return dkk[q][r] * keyUnit[column]; }); }
+    __syncthreads();
+    timesColumns(L::keyColumns, dk);
+    __syncthreads();
+    if(squares) { storeSquares(true, [&](int q, int r, uint32_t row, uint32_t column) { return dkk[q][r] * keyUnit[row]; }); }
+    __syncthreads();
+    timesColumns(L::keyColumns, dk);
+
+    // through the lengths of queries and keys
+    if(a.normalise) {
+        #pragma unroll
+        for(int m = 0; m < MINE; m++) {
+            const f32x4 q = valuesAt(L::queryColumns, tileOf(m)), k = valuesAt(L::keyColumns, tileOf(m));
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = tileOf(m) * 16 + 4 * g + r;
+                const float x = sumOf16(q[r] * queryUnit[row] * dq[m][r]), y = sumOf16(k[r] * keyUnit[row] * dk[m][r]);
+                if(n16 == 0) { queryDots[(firstRow * KEY_TILES + keyTile) * C + row] = x; keyDots[(firstRow * KEY_TILES + keyTile) * C + row] = y; }
+            }
+        }
+        __syncthreads();
+    }
+    #pragma unroll
+    for(int m = 0; m < MINE; m++) {
+        const f32x4 q = valuesAt(L::queryColumns, tileOf(m)), k = valuesAt(L::keyColumns, tileOf(m));
+        #pragma unroll
+        for(int r = 0; r < 4; r++) {
+            const uint32_t row = tileOf(m) * 16 + 4 * g + r;
+            float x = dq[m][r], y = dk[m][r];
+            if(a.normalise) {
+                float queryDot = 0.0f, keyDot = 0.0f;
+                #pragma unroll
+                for(int w = 0; w < KEY_TILES; w++) { queryDot += queryDots[(firstRow * KEY_TILES + w) * C + row]; keyDot += keyDots[(firstRow * KEY_TILES + w) * C + row]; }
+                x -= q[r] * queryUnit[row] * queryDot;
+                y -= k[r] * keyUnit[row] * keyDot;
+            }
+            if(row < count && key < a.keys) {
+                if(d.q.data) { (rowsOf<T>(d.q, a.chunks, p) + (uint64_t)(begin + row) * d.q.rowStride)[keyHead * a.keys + key] = narrow<T>(x * queryUnit[row]); }
+                if(d.k.data) { (rowsOf<T>(d.k, a.chunks, p) + (uint64_t)(begin + row) * d.k.rowStride)[keyHead * a.keys + key] = narrow<T>(y * keyUnit[row]); }
+            }
+        }
+    }
+}
+
+// ---- a token of every running sequence
+// Bound by the state, which is read and written once: a work-group has a head's columns of 8 lanes times VEC, a lane the rows with its number (of 32) in them, in registers
+// between reading and writing.  One sum over the rows does for everything: with S' k, S' q, |k|^2, |q|^2 and k.q
+//   u = beta (v - a S' k^),   out = scale (a S' q^ + (k^.q^) u).
+__device__ inline float eightApart(float x) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true)); }      // row_ror:8
+template<typename T, int ROWS, int VEC>
+__global__ __launch_bounds__(256)
+void deltaTokenKernel(DeltaArgs a)
+{
+    constexpr int SUMS = 2 * VEC + 3;
+    __shared__ float sums[4][8][SUMS];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, inRow = tid & 7, part = tid >> 3;
+    const uint32_t block = blockIdx.x % a.columnBlocks, rest = blockIdx.x / a.columnBlocks, head = rest % a.heads, sequence = rest / a.heads, keyHead = head / a.group;
+    const uint32_t column = (block * 8 + inRow) * VEC;
+    const bool inside = column < a.values;
+    Place p;
+    if(!describe(a.chunks, sequence, p)) { return; }
+    const uint64_t stateAt = ((uint64_t)p.state * a.heads + head) * a.keys * a.values + column;
+    typedef Pack<float, VEC> Columns;
+    Columns s[ROWS];
+    #pragma unroll
+    for(int i = 0; i < ROWS; i++) {
+        const uint32_t row = part + 32 * i;
+        s[i] = Columns{};
+        if(a.initialState && row < a.keys && inside) { s[i] = *(const Columns*)(a.initialState + stateAt + (uint64_t)row * a.values); }
+    }
+    if(p.length) {
+        const T *const keys = rowsOf<const T>(a.k, a.chunks, p) + keyHead * a.keys, *const queries = rowsOf<const T>(a.q, a.chunks, p) + keyHead * a.keys;
+        const float beta = rowsOf<const float>(a.beta, a.chunks, p)[head], decay = decayOver(clampGate(rowsOf<const float>(a.g, a.chunks, p)[head]));
+        float v[VEC], k[ROWS], q[ROWS], sum[SUMS] = {};
+        #pragma unroll
+        for(int e = 0; e < VEC; e++) { v[e] = inside && column + e < a.values ? widen((rowsOf<const T>(a.v, a.chunks, p) + head * a.values)[column + e]) : 0.0f; }
+        #pragma unroll
+        for(int i = 0; i < ROWS; i++) {
+            const uint32_t row = part + 32 * i;
+            k[i] = row < a.keys ? widen(keys[row]) : 0.0f;
+            q[i] = row < a.keys ? widen(queries[row]) : 0.0f;
+        }
+        #pragma unroll
+        for(int i = 0; i < ROWS; i++) {
+            #pragma unroll
+            for(int e = 0; e < VEC; e++) { sum[e] = __builtin_fmaf(s[i].v[e], k[i], sum[e]); sum[VEC + e] = __builtin_fmaf(s[i].v[e], q[i], sum[VEC + e]); }
+            sum[2 * VEC] = __builtin_fmaf(k[i], k[i], sum[2 * VEC]);
+            sum[2 * VEC + 1] = __builtin_fmaf(q[i], q[i], sum[2 * VEC + 1]);
+            sum[2 * VEC + 2] = __builtin_fmaf(k[i], q[i], sum[2 * VEC + 2]);
+        }
+        #pragma unroll
+        for(int n = 0; n < SUMS; n++) {
+            // (over the eight parts of the wavefront: lanes 8, 16 and 32 apart)
+            sum[n] += eightApart(sum[n]);
+            sum[n] += partner<16>(sum[n]);
+            sum[n] += partner<32>(sum[n]);
+            if(lane < 8) { sums[wave][inRow][n] = sum[n]; }
+        }
+        __syncthreads();
+        #pragma unroll
+        for(int n = 0; n < SUMS; n++) { sum[n] = (sums[0][inRow][n] + sums[1][inRow][n]) + (sums[2][inRow][n] + sums[3][inRow][n]); }
+        const float keyUnit = a.normalise ? 1.0f / sqrtf(sum[2 * VEC] + a.epsilon) : 1.0f, queryUnit = a.normalise ? 1.0f / sqrtf(sum[2 * VEC + 1] + a.epsilon) : 1.0f;
+        float u[VEC];
+        #pragma unroll
+        for(int e = 0; e < VEC; e++) { u[e] = beta * __builtin_fmaf(-decay * keyUnit, sum[e], v[e]); }
+        if(part == 0 && inside) {
+            T *const out = rowsOf<T>(a.out, a.chunks, p) + head * a.values;
+            const float both = keyUnit * sum[2 * VEC + 2];
+            #pragma unroll
+            for(int e = 0; e < VEC; e++) { if(column + e < a.values) { out[column + e] = narrow<T>(a.scale * queryUnit * __builtin_fmaf(both, u[e], decay * sum[VEC + e])); } }
+        }
+        #pragma unroll
+        for(int i = 0; i < ROWS; i++) {
+            #pragma unroll
+            for(int e = 0; e < VEC; e++) { s[i].v[e] = __builtin_fmaf(k[i] * keyUnit, u[e], decay * s[i].v[e]); }
+        }
+    }
+    if(!a.finalState || !inside) { return; }
+    #pragma unroll
+    for(int i = 0; i < ROWS; i++) {
+        const uint32_t row = part + 32 * i;
+        if(row < a.keys) { *(Columns*)(a.finalState + stateAt + (uint64_t)row * a.values) = s[i]; }
+    }
+}
+}
+
+#endif

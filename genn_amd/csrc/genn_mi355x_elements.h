@@ -179,7 +179,7 @@ inline int checkRows(const char *what, const char *which, const gennmi_rows_t &r
 inline int checkWrittenRows(const char *what, const char *which, const gennmi_rows_t &r, const gennmi_sequences_t &s, uint32_t width, uint32_t size)
 {
     if(const int rc = checkRows(what, which, r, s, width, size)) { return rc; }
-    const bool overlap = s.count > 1 && (s.offsets ? r.rowStride < width : r.sequenceStride < width);
+    const bool overlap = s.count > 1 && (s.offsets ? s.rows : s.length) && (s.offsets ? r.rowStride < width : r.sequenceStride < width);
     return overlap ? gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": " + which + ": sequences overlap") : GENNMI_OK;
 }
 
@@ -279,6 +279,44 @@ inline void noteRows(const gennmi_rows_t &r, const gennmi_sequences_t &s, uint32
     gennmi_detail::noteDeviceWrite(r.data, (last + width) * size);
 }
 inline uint64_t statesOf(const gennmi_sequences_t &s) { return s.slots ? s.numSlots : s.count; }
+
+inline Sequences sequencesOf(const gennmi_sequences_t &s, uint32_t chunk)
+{
+    Sequences d{};
+    d.offsets = s.offsets;
+    d.slots = s.slots;
+    d.rows = s.rows;
+    d.count = s.count;
+    d.length = s.length;
+    d.numSlots = s.numSlots;
+    d.chunk = chunk;
+    d.perSequence = std::max(1u, (s.length + chunk - 1) / chunk);
+    return d;
+}
+// Chunk numbers: see Sequences.  Without sequences none, however many rows packed arrays hold: kernels look for the sequence of a number.
+inline uint64_t chunkNumbers(const gennmi_sequences_t &s, uint32_t chunk)
+{
+    if(!s.count) { return 0; }
+    return s.offsets ? s.rows / chunk + s.count : (uint64_t)s.count * std::max(1u, (s.length + chunk - 1) / chunk);
+}
+inline uint64_t totalRows(const gennmi_sequences_t &s) { return s.offsets ? s.rows : (uint64_t)s.count * s.length; }
+inline Region offsetsOf(const gennmi_sequences_t &s) { return regionOf("offsets", s.offsets, (s.count + 1ull) * 4); }
+inline Region slotsOf(const gennmi_sequences_t &s) { return regionOf("slots", s.slots, s.count * 4ull); }
+// An array that a call may write in place of the one it reads
+inline Region unlessSame(const Region &r, const void *written) { return (uintptr_t)written == (uintptr_t)r.begin ? Region{r.name, 0, 0, 0, 0, 0, 0, 0} : r; }
+inline int checkWorkspace(const char *what, const void *workspace, size_t have, size_t need)
+{
+    if(need && (!workspace || have < need)) { return gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": workspace is missing or too small"); }
+    return (uintptr_t)workspace % 16 ? gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": workspace is not 16-byte aligned") : GENNMI_OK;
+}
+inline int tooMany(const char *what) { return gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers"); }
+
+// Sums over chunks, sums[number][n][channel], in 64 bits: there may be thousands, of either sign.  Row n of the sums goes to out[channel][n] for n < width,
+// behind those to more[0][channel] and more[1][channel].  The 16 wavefronts of a work-group have 64 channels and a sixteenth of the numbers each;
+// what they found is added up in the order of the numbers.
+struct ChunkSums { const float *sums; float *out, *more[2]; uint32_t numbers, channels, width, rows; };
+inline uint64_t chunkSumBlocks(uint32_t rows, uint32_t channels) { return (uint64_t)rows * ((channels + 63) / 64); }
+int launchChunkSum(const char *what, const ChunkSums &a, hipStream_t stream);       // (defined beside the scan)
 }
 
 #endif

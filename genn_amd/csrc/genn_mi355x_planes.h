@@ -1,0 +1,119 @@
+// Part of libgenn_mi355x.so: matrix products of fp32 accuracy on the bf16 matrix instructions.
+//
+// A float is a sum of three bf16 values without a rest, its upper 8 bits of mantissa, the next 8 and the last 8 ("planes").  Of the nine products of
+// two such sums the six whose planes' numbers add up to 2 at most are taken; the others are below 2^-24 of the whole.  A bf16 input is one plane, an fp16
+// input two, so that most products take three to five instructions: 16 x 16 x 32 in 16 cycles each, where the same on the fp32 matrix
+// instructions takes eight of 32.
+#ifndef GENN_MI355X_PLANES_H
+#define GENN_MI355X_PLANES_H
+
+#include "genn_mi355x_elements.h"
+
+namespace gennmi_planes
+{
+using gennmi_elements::bf16;
+using gennmi_elements::f16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template<typename T> constexpr int planesOf = 3;
+template<> constexpr int planesOf<f16> = 2;
+template<> constexpr int planesOf<bf16> = 1;
+
+// Eight values along the axis that is summed over: an operand of one lane
+template<int N> struct Planes { union { uint32_t word[4]; bf16x8 v; } plane[N]; };
+
+// Takes the upper plane of a pair of values off them: its bits, the first value's below
+__device__ inline uint32_t takePlane(float &a, float &b)
+{
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    a -= __uint_as_float(x & 0xffff0000u);
+    b -= __uint_as_float(y & 0xffff0000u);
+    return __builtin_amdgcn_perm(y, x, 0x07060302u);
+}
+// (the last plane: nothing of the values is needed after it)
+__device__ inline uint32_t lastPlane(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
+template<int N> __device__ inline void splitPair(float a, float b, uint32_t (&words)[N])
+{
+    #pragma unroll
+    for(int p = 0; p < N; p++) { words[p] = p + 1 < N ? takePlane(a, b) : lastPlane(a, b); }
+}
+// Four values, N planes of 8 bytes
+template<int N> __device__ inline void splitFour(const float (&x)[4], uint2 (&out)[N])
+{
+    uint32_t low[N], high[N];
+    splitPair<N>(x[0], x[1], low);
+    splitPair<N>(x[2], x[3], high);
+    #pragma unroll
+    for(int p = 0; p < N; p++) { out[p] = make_uint2(low[p], high[p]); }
+}
+// Eight values of one lane: those of two tiles of a result, one below the other, that becomes an operand (see place())
+template<int N> __device__ inline Planes<N> split(const f32x4 &a, const f32x4 &b)
+{
+    Planes<N> out;
+    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    #pragma unroll
+    for(int i = 0; i < 4; i++) {
+        uint32_t words[N];
+        splitPair<N>(x[2 * i], x[2 * i + 1], words);
+        #pragma unroll
+        for(int p = 0; p < N; p++) { out.plane[p].word[i] = words[p]; }
+    }
+    return out;
+}
+// A lane of a result tile has the rows 4 (lane / 16) + 0 .. 3 of the column lane % 16.  As an operand that is summed over those rows, two tiles are taken
+// together, and a lane's eight values are rows 4 g .. 4 g + 3 of either (g = lane / 16).  The other operand lies in memory in that order:
+// element i of 32 at place(i).
+__device__ inline uint32_t place(uint32_t i) { return (i & ~31u) + 8 * ((i >> 2) & 3) + 4 * ((i >> 4) & 1) + (i & 3); }
+
+// From LDS, planes `stride` elements apart; 16-byte aligned
+template<int N> __device__ inline Planes<N> fetch(const uint16_t *at, uint32_t stride)
+{
+    Planes<N> out;
+    #pragma unroll
+    for(int p = 0; p < N; p++) {
+        const uint4 w = *(const uint4*)(at + p * stride);
+        out.plane[p].word[0] = w.x; out.plane[p].word[1] = w.y; out.plane[p].word[2] = w.z; out.plane[p].word[3] = w.w;
+    }
+    return out;
+}
+// sum += a b, the smallest products first
+template<int NA, int NB> __device__ inline f32x4 multiply(const Planes<NA> &a, const Planes<NB> &b, f32x4 sum)
+{
+    #pragma unroll
+    for(int total = 2; total >= 0; total--) {
+        #pragma unroll
+        for(int i = 0; i < NA; i++) {
+            if(total - i >= 0 && total - i < NB) { sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.plane[i].v, b.plane[total - i].v, sum, 0, 0, 0); }
+        }
+    }
+    return sum;
+}
+// sum += a b for 16 x 16 tiles in fp32: a's lane has row lane % 16, its columns 4 (lane / 16) + 0 .. 3; b is a result
+__device__ inline f32x4 multiply(const f32x4 &a, const f32x4 &b, f32x4 sum)
+{
+    #pragma unroll
+    for(int e = 0; e < 4; e++) { sum = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], sum, 0, 0, 0); }
+    return sum;
+}
+// `valid` of eight neighbouring elements, zero behind them; `wide`: they lie on 16 bytes, and there are eight or none
+template<typename T> __device__ inline void loadEight(const T *at, uint32_t valid, bool wide, T (&v)[8])
+{
+    using gennmi_elements::Pack;
+    constexpr int EACH = 16 / sizeof(T);
+    if(wide) {
+        #pragma unroll
+        for(int i = 0; i < 8; i += EACH) {
+            Pack<T, EACH> p{};
+            if(valid) { p = *(const Pack<T, EACH>*)(at + i); }
+            #pragma unroll
+            for(int e = 0; e < EACH; e++) { v[i + e] = p.v[e]; }
+        }
+        return;
+    }
+    #pragma unroll
+    for(int i = 0; i < 8; i++) { v[i] = (uint32_t)i < valid ? at[i] : (T)0.0f; }
+}
+}
+
+#endif

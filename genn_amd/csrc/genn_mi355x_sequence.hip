@@ -10,10 +10,6 @@ using gennmi_detail::fail;
 
 namespace
 {
-// Sums over chunks, sums[number][n][channel], in 64 bits: there may be thousands, of either sign.  Row n of the sums goes to out[channel][n] for n < width,
-// behind those to more[0][channel] and more[1][channel].  The 16 wavefronts of a work-group have 64 channels and a sixteenth of the numbers each;
-// what they found is added up in the order of the numbers.
-struct ChunkSums { const float *sums; float *out, *more[2]; uint32_t numbers, channels, width, rows; };
 __global__ __launch_bounds__(1024)
 void chunkSumKernel(ChunkSums a)
 {
@@ -35,13 +31,11 @@ void chunkSumKernel(ChunkSums a)
     if(n < a.width) { if(a.out) { a.out[(uint64_t)channel * a.width + n] = (float)sum; } }
     else if(a.more[n - a.width]) { a.more[n - a.width][channel] = (float)sum; }
 }
-uint64_t chunkSumBlocks(uint32_t rows, uint32_t channels) { return (uint64_t)rows * ((channels + 63) / 64); }
-int launchChunkSum(const char *what, const ChunkSums &a, hipStream_t stream)
+}
+int gennmi_elements::launchChunkSum(const char *what, const ChunkSums &a, hipStream_t stream)
 {
     chunkSumKernel<<<dim3((uint32_t)chunkSumBlocks(a.rows, a.channels)), dim3(1024), 0, stream>>>(a);
     return gennmi_detail::afterLaunch(what);
-}
-int tooMany(const char *what) { return fail(GENNMI_EINVAL, std::string(what) + ": more rows than one launch covers"); }
 }
 
 #include "genn_mi355x_lanes.h"
@@ -50,27 +44,6 @@ int tooMany(const char *what) { return fail(GENNMI_EINVAL, std::string(what) + "
 
 namespace
 {
-Sequences sequencesOf(const gennmi_sequences_t &s, uint32_t chunk)
-{
-    Sequences d{};
-    d.offsets = s.offsets;
-    d.slots = s.slots;
-    d.rows = s.rows;
-    d.count = s.count;
-    d.length = s.length;
-    d.numSlots = s.numSlots;
-    d.chunk = chunk;
-    d.perSequence = std::max(1u, (s.length + chunk - 1) / chunk);
-    return d;
-}
-// Chunk numbers: see Sequences.  Without sequences none, however many rows packed arrays hold: kernels look for the sequence of a number.
-uint64_t chunkNumbers(const gennmi_sequences_t &s, uint32_t chunk)
-{
-    if(!s.count) { return 0; }
-    return s.offsets ? s.rows / chunk + s.count : (uint64_t)s.count * std::max(1u, (s.length + chunk - 1) / chunk);
-}
-uint64_t totalRows(const gennmi_sequences_t &s) { return s.offsets ? s.rows : (uint64_t)s.count * s.length; }
-
 // ---- causal convolution
 // Rows of a chunk: at least taps - 1, so that only the first chunk reads the initial state
 constexpr uint32_t CONV_ROWS = 16, CONV_GRADIENT_ROWS = 64, CONV_GRADIENT_THREADS = 1u << 17;
@@ -93,10 +66,6 @@ int checkConv(const char *what, const gennmi_causal_conv_t *c, bool gradients)
     if((uintptr_t)c->initialState % size || (uintptr_t)c->finalState % size) { return refuse(GENNMI_EINVAL, ": a state is not aligned to its elements"); }
     return GENNMI_OK;
 }
-Region offsetsOf(const gennmi_sequences_t &s) { return regionOf("offsets", s.offsets, (s.count + 1ull) * 4); }
-Region slotsOf(const gennmi_sequences_t &s) { return regionOf("slots", s.slots, s.count * 4ull); }
-// An array that a call may write in place of the one it reads
-Region unlessSame(const Region &r, const void *written) { return (uintptr_t)written == (uintptr_t)r.begin ? Region{r.name, 0, 0, 0, 0, 0, 0, 0} : r; }
 int convApart(const char *what, const gennmi_causal_conv_t &c)
 {
     const gennmi_sequences_t &s = c.sequences;
@@ -327,12 +296,6 @@ ScanArgs scanArgs(const gennmi_scan_t &c, const ScanPlan &p)
     a.slabs = p.slabs;
     return a;
 }
-int checkWorkspace(const char *what, const void *workspace, size_t have, size_t need)
-{
-    if(need && (!workspace || have < need)) { return fail(GENNMI_EINVAL, std::string(what) + ": workspace is missing or too small"); }
-    return (uintptr_t)workspace % 16 ? fail(GENNMI_EINVAL, std::string(what) + ": workspace is not 16-byte aligned") : GENNMI_OK;
-}
-
 template<typename T, int NP, bool SLABS> int launchScan(const ScanArgs &a, const ScanPlan &p, hipStream_t stream)
 {
     const dim3 grid(a.numbers * a.tiles), threads(64 * p.slabs);

@@ -1,11 +1,13 @@
-"""Operators on sequences over the C ABI in include/genn_mi355x.h: a short causal convolution of every channel and a selective state space
-scan, for whole sequences (with gradients) and for one token of every running sequence.
+"""Operators on sequences over the C ABI in include/genn_mi355x.h: a short causal convolution of every channel, a selective state space
+scan and a gated delta rule, for whole sequences (with gradients) and for one token of every running sequence; and what stands around them: layer norm
+with its gradients, and dropout.
 
 As a model's arrays are handed to its runner once and stepped many times, an operator's arrays are bound once (checked then) and
 ``run()`` / ``backward()`` are single calls of the library.  Arrays are ``Array`` objects of this package or tensors on the device.
 ``stream`` is the address of a HIP stream; 0, the default, is the null stream.  A call while another device than the operator's is current is refused.
 """
 import ctypes as C
+from numbers import Integral
 
 from . import _abi
 from .genn_model import Array
@@ -33,15 +35,15 @@ class _SequenceOperator:
     def _operand(self, array, name, shape=None):
         return None if array is None else Operand(array, name, shape)
 
-    def _rows(self, array, name, width, given):
-        """A ``Rows`` of the operator's element type, or an empty one."""
+    def _rows(self, array, name, width, given, dtype=None):
+        """A ``Rows`` of the operator's element type (or of ``dtype``), or an empty one."""
         if array is None:
             return _abi.Rows()
         shape = None
         if isinstance(array, Array):
             count = self._packed if self._packed is not None else self.sequences * self.length
             shape = (count, width) if array.count == count * width or self._packed is None else (array.count // width, width)
-        o = Operand(array, name, shape).wants(self.dtype)
+        o = Operand(array, name, shape).wants(dtype or self.dtype)
         given.append(o)
         return o.rows(self.sequences, self.length, width, self._packed)
 
@@ -254,6 +256,193 @@ class SelectiveScan(_SequenceOperator):
         rc = self._lib.gennmi_selective_scan_backward(self._reference, self._gradient_reference, address, size, stream)
         if rc:
             _abi.check(rc)
+
+
+class GatedDeltaRule(_SequenceOperator):
+    """S[t] = a S[t-1] + k (x) beta (v - a S[t-1]' k) with a = exp(g),  out[t] = scale S[t]' q; with ``normalise`` q and k divided by sqrt(sum of squares + epsilon).
+
+    ``q, k``: rows of key_heads x keys (heads / key_heads neighbouring heads share a key head); ``v, out``: rows of heads x values; ``g, beta``: rows of heads,
+    float32.  Rows, ``offsets`` and ``slots`` as for ``CausalConvolution``; states [sequences or places, heads, keys, values] are float32.  ``scale``: keys ** -0.5 unless it
+    is given.  ``length=1`` is a token of every running sequence."""
+
+    def __init__(self, sequences, length, heads, keys, values, key_heads=None, dtype="float32", normalise=False, scale=None, epsilon=1e-6, device=0):
+        super().__init__(sequences, length, dtype, device)
+        self.heads, self.keys, self.values = _count(heads, "heads"), _count(keys, "keys"), _count(values, "values")
+        self.key_heads = self.heads if key_heads is None else _count(key_heads, "key_heads")
+        self.normalise, self.epsilon = bool(normalise), float(epsilon)
+        self.scale = max(1, self.keys) ** -0.5 if scale is None else float(scale)
+        self._width = self.key_heads * self.keys
+
+    def _widths(self):
+        return (("q", self._width, None), ("k", self._width, None), ("v", self.heads * self.values, None), ("g", self.heads, "float32"), ("beta", self.heads, "float32"))
+
+    def bind(self, q, k, v, g, beta, out=None, initial_state=None, final_state=None, offsets=None, slots=None):
+        given = []
+        c = _abi.DeltaRule(type=_abi.FLOAT_TYPES[self.dtype], heads=self.heads, keyHeads=self.key_heads, keys=self.keys, values=self.values, normalise=self.normalise,
+                           scale=self.scale, epsilon=self.epsilon)
+        c.sequences = self._sequences(offsets, slots, q, given)
+        for (field, width, dtype), array in zip(self._widths(), (q, k, v, g, beta)):
+            setattr(c, field, self._rows(array, field, width, given, dtype))
+        c.out = self._rows(out, "out", self.heads * self.values, given)
+        shape = (self.heads, self.keys, self.values)
+        c.initialState, first = self._states(initial_state, "initial_state", slots, shape, "float32", given)
+        c.finalState, last = self._states(final_state, "final_state", slots, shape, "float32", given)
+        if slots is not None:
+            if first is not None and last is not None and first != last:
+                raise ValueError("initial_state and final_state have different numbers of places")
+            c.sequences.numSlots = first or last or 0
+        same_device(given, self.device)
+        size = _size_t()
+        if out is not None:
+            _abi.check(self._lib.gennmi_delta_rule_workspace(_byref(c), _byref(size)))
+        self.workspace_bytes = size.value
+        self._bound, self._bound_packed, self._descriptor, self._reference, self._gradients = given, self._packed, c, _byref(c), None
+
+    def run(self, stream=0, workspace=None):
+        """``workspace``: ``workspace_bytes`` on the device, for a call that is captured into a graph (which keeps using it)."""
+        if self._bound is None:
+            raise RuntimeError("bind() must be called first")
+        address, size = self._workspace("forward", workspace, self.workspace_bytes, stream) if self.workspace_bytes else (None, 0)
+        rc = self._lib.gennmi_delta_rule(self._reference, address, size, stream)
+        if rc:
+            _abi.check(rc)
+
+    def bind_gradients(self, out, q=None, k=None, v=None, g=None, beta=None, initial_state=None, final_state=None):
+        """``out`` and ``final_state``: gradients that come in; the others are written."""
+        self._need(self._bound, "bind()")
+        self._packed = self._bound_packed
+        given = []
+        d = _abi.DeltaRuleGradient()
+        d.out = self._rows(out, "the gradient of out", self.heads * self.values, given)
+        for (field, width, dtype), array in zip(self._widths(), (q, k, v, g, beta)):
+            setattr(d, field, self._rows(array, f"the gradient of {field}", width, given, dtype))
+        shape = (self.sequences, self.heads, self.keys, self.values)
+        d.finalState = self._flat(final_state, "the gradient of final_state", shape, "float32", given)
+        d.initialState = self._flat(initial_state, "the gradient of initial_state", shape, "float32", given)
+        same_device(given, self.device)
+        size = _size_t()
+        _abi.check(self._lib.gennmi_delta_rule_backward_workspace(self._reference, _byref(size)))
+        self.backward_workspace_bytes = size.value
+        self._gradients, self._gradient_descriptor, self._gradient_reference = given, d, _byref(d)
+
+    def backward(self, stream=0, workspace=None):
+        """``workspace``: ``backward_workspace_bytes`` on the device, as for ``run``."""
+        self._need(self._gradients, "bind_gradients()")
+        address, size = self._workspace("backward", workspace, self.backward_workspace_bytes, stream)
+        rc = self._lib.gennmi_delta_rule_backward(self._reference, self._gradient_reference, address, size, stream)
+        if rc:
+            _abi.check(rc)
+
+
+class LayerNorm(_SequenceOperator):
+    """out = (x' weight + bias) gate sigmoid(gate) with x' = (x - mean) / sqrt(variance + epsilon) of every row, or with ``rms`` x / sqrt(mean of squares + epsilon).
+
+    ``x, gate, out``: [sequences, length, channels] (or both first axes as one); the heads of a row are such a length.  ``weight, bias``: [channels], float32; without them 1 and 0.
+    ``out`` may be ``x`` or ``gate`` itself."""
+
+    def __init__(self, sequences, length, channels, epsilon=1e-5, rms=False, dtype="float32", device=0):
+        super().__init__(sequences, length, dtype, device)
+        self.channels, self.epsilon, self.rms = _count(channels, "channels"), float(epsilon), bool(rms)
+
+    def bind(self, x, weight=None, bias=None, gate=None, out=None):
+        given = []
+        c = _abi.LayerNorm(type=_abi.FLOAT_TYPES[self.dtype], channels=self.channels, rms=self.rms, epsilon=self.epsilon)
+        c.sequences = self._sequences(None, None, x, given)
+        for field, array in (("x", x), ("gate", gate), ("out", out)):
+            setattr(c, field, self._rows(array, field, self.channels, given))
+        c.weight = self._flat(weight, "weight", (self.channels,), "float32", given)
+        c.bias = self._flat(bias, "bias", (self.channels,), "float32", given)
+        same_device(given, self.device)
+        self._bound, self._descriptor, self._reference, self._gradients = given, c, C.byref(c), None
+
+    def run(self, stream=0):
+        if self._bound is None:
+            raise RuntimeError("bind() must be called first")
+        rc = self._lib.gennmi_layer_norm(self._reference, stream)
+        if rc:
+            _abi.check(rc)
+
+    def bind_gradients(self, out, x=None, weight=None, bias=None, gate=None):
+        """``out``: the gradient that comes in; the others are written."""
+        self._need(self._bound, "bind()")
+        given = []
+        g = _abi.LayerNormGradient()
+        for field, array in (("out", out), ("x", x), ("gate", gate)):
+            setattr(g, field, self._rows(array, f"the gradient of {field}", self.channels, given))
+        g.weight = self._flat(weight, "the gradient of weight", (self.channels,), "float32", given)
+        g.bias = self._flat(bias, "the gradient of bias", (self.channels,), "float32", given)
+        same_device(given, self.device)
+        size = C.c_size_t()
+        _abi.check(self._lib.gennmi_layer_norm_backward_workspace(self._reference, C.byref(size)))
+        self.backward_workspace_bytes = size.value if weight is not None or bias is not None else 0
+        self._gradients, self._gradient_descriptor, self._gradient_reference = given, g, C.byref(g)
+
+    def backward(self, stream=0, workspace=None):
+        """``workspace``: ``backward_workspace_bytes`` on the device, for a call that is captured into a graph (which keeps using it)."""
+        self._need(self._gradients, "bind_gradients()")
+        address, size = self._workspace("backward", workspace, self.backward_workspace_bytes, stream)
+        rc = self._lib.gennmi_layer_norm_backward(self._reference, self._gradient_reference, address, size, stream)
+        if rc:
+            _abi.check(rc)
+
+
+class Dropout(_SequenceOperator):
+    """out = residual + (kept ? x / (1 - probability) : 0), the probability in 65536ths.  No mask is stored: ``backward`` draws it again.
+
+    ``x, residual, out``: [sequences, length, channels] (or both first axes as one).  What is kept depends on ``seed``, on the ``call`` (the number of a step and layer, say)
+    and on the place of an element among rows and channels, not on strides.  ``out`` may be ``x`` or ``residual`` itself."""
+
+    def __init__(self, sequences, length, channels, probability, seed=0, dtype="float32", device=0):
+        super().__init__(sequences, length, dtype, device)
+        self.channels, self.probability, self.seed = _count(channels, "channels"), float(probability), int(seed)
+        if not 0.0 <= self.probability <= 1.0:
+            raise ValueError(f"probability is between 0 and 1, not {probability}")
+        if not 0 <= self.seed < 1 << 64:
+            raise ValueError("seed has 64 bits")
+
+    def _descriptor_of(self, given, x, out, residual, names):
+        d = _abi.Dropout(type=_abi.FLOAT_TYPES[self.dtype], channels=self.channels, probability=self.probability, seed=self.seed)
+        d.sequences = self._sequences(None, None, x, given)
+        for field, array, name in zip(("x", "out", "residual"), (x, out, residual), names):
+            setattr(d, field, self._rows(array, name, self.channels, given))
+        same_device(given, self.device)
+        return d
+
+    def bind(self, x, out, residual=None):
+        given = []
+        self._forward = self._descriptor_of(given, x, out, residual, ("x", "out", "residual"))
+        self._bound = given
+
+    def bind_gradients(self, out, x):
+        """``out``: the gradient that comes in; ``x``: the one that is written (may be the same array).  The residual's gradient is ``out`` itself."""
+        given = []
+        self._backward = self._descriptor_of(given, out, x, None, ("the gradient of out", "the gradient of x", ""))
+        self._gradients = given
+
+    def _call(self, d, call, stream):
+        if isinstance(call, Integral):          # (numpy's numbers are that too)
+            if not 0 <= call < 1 << 64:
+                raise ValueError("call has 64 bits")
+            d.call, d.callDevice, self._value = int(call), None, None
+        else:
+            o = Operand(call, "call").wants(("uint64", "int64"))
+            if any(n != 1 for n in o.shape):
+                raise ValueError("call is one value")
+            same_device([o], self.device)
+            d.call, d.callDevice, self._value = 0, o.address, o          # (kept alive until the next call)
+        rc = self._lib.gennmi_dropout(C.byref(d), stream)
+        if rc:
+            _abi.check(rc)
+
+    def run(self, call, stream=0):
+        """``call``: a number, or an int64 or uint64 array of one element on the device that is read when the call runs (a captured call goes on reading it)."""
+        self._need(self._bound, "bind()")
+        self._call(self._forward, call, stream)
+
+    def backward(self, call, stream=0):
+        """``call``: that of ``run``."""
+        self._need(self._gradients, "bind_gradients()")
+        self._call(self._backward, call, stream)
 
 
 # (`C` names an array of the scan)

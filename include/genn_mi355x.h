@@ -665,6 +665,78 @@ int gennmi_selective_scan(const gennmi_scan_t *scan, void *workspace, size_t wor
 int gennmi_selective_scan_backward_workspace(const gennmi_scan_t *scan, size_t *bytes);
 int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_gradient_t *gradient, void *workspace, size_t workspaceBytes, void *stream);
 
+/* Gated delta rule: every head keeps a matrix that maps keys to values, lets it decay, and corrects it by what it gets wrong for the row's key.
+ * With k' and q' the row's key and query of the head, divided by sqrt(sum of squares + epsilon) each with `normalise`:
+ *   S[t] = a S[t - 1] + k' (x) beta[t] (v[t] - a S[t - 1]^T k'),   a = exp(g[t]),   out[t] = scale * S[t]^T q'
+ * heads / keyHeads neighbouring heads share a key head's keys and queries.  States and sums in fp32 (products as sums of bf16 products that lose nothing of it), one rounding at the end.
+ * Long sequences are taken in chunks of up to 64 rows: where g > 0 for long, the growth over a chunk has to stay below 2^128.  A g below -1e6 counts as that.
+ * What an infinite input or state, one that is not a number, or an overflow gives: outputs before its row are as without it, and its own value's column of outputs and states (keys, g, beta: all of
+ * the head's) is not finite from its row on; in gradients it may reach the whole sequence's head.  One row per sequence (a token of every running
+ * sequence) takes a kernel of its own, without a workspace. */
+#define GENNMI_MAX_DELTA_KEYS 128
+#define GENNMI_MAX_DELTA_VALUES 1024
+typedef struct gennmi_delta_rule_t {
+    gennmi_sequences_t sequences;
+    uint32_t type;                        /* of q, k, v and out: GENNMI_TYPE_F32, _F16 or _BF16 */
+    uint32_t heads, keyHeads;             /* keyHeads divides heads */
+    uint32_t keys, values;                /* of a head: 1 <= keys <= GENNMI_MAX_DELTA_KEYS, 1 <= values <= GENNMI_MAX_DELTA_VALUES */
+    uint32_t normalise;
+    float scale, epsilon;
+    gennmi_rows_t q, k;                   /* [keyHeads][keys] a row */
+    gennmi_rows_t v, out;                 /* [heads][values] a row */
+    gennmi_rows_t g, beta;                /* fp32 [heads] a row */
+    const float *initialState;            /* [states' places][heads][keys][values], or NULL: zero */
+    float *finalState;                    /* after the last row, or NULL; may be initialState itself */
+} gennmi_delta_rule_t;
+typedef struct gennmi_delta_rule_gradient_t {       /* `out` and `finalState` come in, the others go out (any may be NULL) and are overwritten */
+    gennmi_rows_t out, q, k, v, g, beta;
+    const float *finalState;              /* gradient of the final state, or NULL: zero */
+    float *initialState;                  /* may be the array of finalState */
+} gennmi_delta_rule_gradient_t;
+int gennmi_delta_rule_workspace(const gennmi_delta_rule_t *rule, size_t *bytes);
+int gennmi_delta_rule(const gennmi_delta_rule_t *rule, void *workspace, size_t workspaceBytes, void *stream);
+int gennmi_delta_rule_backward_workspace(const gennmi_delta_rule_t *rule, size_t *bytes);
+int gennmi_delta_rule_backward(const gennmi_delta_rule_t *rule, const gennmi_delta_rule_gradient_t *gradient, void *workspace, size_t workspaceBytes, void *stream);
+
+/* Layer norm of every row:  x' = (x - mean) / sqrt(variance + epsilon), or with `rms` x / sqrt(mean of squares + epsilon),
+ *   out = (x' * weight + bias) * gate * sigmoid(gate)
+ * Rows within rows (the heads of a row, say) are sequences of as many rows.  Statistics in fp32, one rounding at the end.  Packed sequences and slots are not for this: rows do not depend on each other. */
+#define GENNMI_MAX_NORM_CHANNELS 16384
+typedef struct gennmi_layer_norm_t {
+    gennmi_sequences_t sequences;         /* count times length rows */
+    uint32_t type;                        /* of x, gate and out: GENNMI_TYPE_F32, _F16 or _BF16 */
+    uint32_t channels;                    /* 1 <= channels <= GENNMI_MAX_NORM_CHANNELS */
+    uint32_t rms;
+    float epsilon;
+    gennmi_rows_t x, gate, out;           /* gate.data NULL: no gate.  `out` may be x or gate itself */
+    const float *weight, *bias;           /* [channels], or NULL: 1 and 0 */
+} gennmi_layer_norm_t;
+typedef struct gennmi_layer_norm_gradient_t {       /* `out` comes in, the others go out (any may be NULL) and are overwritten */
+    gennmi_rows_t out, x, gate;           /* arrays of their own */
+    float *weight, *bias;
+} gennmi_layer_norm_gradient_t;
+int gennmi_layer_norm(const gennmi_layer_norm_t *norm, void *stream);
+int gennmi_layer_norm_backward_workspace(const gennmi_layer_norm_t *norm, size_t *bytes);
+int gennmi_layer_norm_backward(const gennmi_layer_norm_t *norm, const gennmi_layer_norm_gradient_t *gradient, void *workspace, size_t workspaceBytes, void *stream);
+
+/* Dropout:  out = residual + (kept ? x / (1 - p) : 0).  No mask is stored: the gradient of x is the same call on the gradient of out, without residual.
+ * Row r (of count times length), channel c: kept if 16 random bits are at least p * 2^16 rounded, p here and above that many 65536ths.  The bits are the (c % 8)th 16 of
+ * Philox4x32-10 (the lower half of a word before the upper) with key = seed and counter = (r * ceil(channels / 8) + c / 8, call), 64 bits each, lower
+ * words first.  What is dropped leaves nothing, also of infinities. */
+typedef struct gennmi_dropout_t {
+    gennmi_sequences_t sequences;         /* count times length rows; not packed, no slots */
+    uint32_t type;                        /* of x, residual and out: GENNMI_TYPE_F32, _F16 or _BF16 */
+    uint32_t channels;
+    double probability;                   /* of dropping, 0 to 1 */
+    uint64_t seed;
+    uint64_t call;                        /* one for each draw that is to differ: the number of a step and layer, say */
+    const uint64_t *callDevice;           /* device: added to `call` when the operator runs (a captured step), or NULL */
+    gennmi_rows_t x, residual, out;       /* residual.data NULL: none.  `out` may be x or residual itself */
+} gennmi_dropout_t;
+int gennmi_dropout(const gennmi_dropout_t *dropout, void *stream);
+/* sizeof() of gennmi_delta_rule_t, gennmi_delta_rule_gradient_t, gennmi_layer_norm_t, gennmi_layer_norm_gradient_t, gennmi_dropout_t */
+int gennmi_abi_layer_sizes(size_t sizes[5]);
+
 /* AdamW (Loshchilov & Hutter 2019) over many tensors in one launch:
  *   g = gradientScale * gradient,  m = beta1 * m + (1 - beta1) * g,  v = beta2 * v + (1 - beta2) * g^2
  *   weight = weight * (1 - rate * weightDecay) - rate * (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + epsilon)
