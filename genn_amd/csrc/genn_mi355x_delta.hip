@@ -1,4 +1,5 @@
 // The gated delta rule, for whole sequences (with gradients) and for single tokens.  Entry points and their checks; the kernels are in the header included below.
+#include <cstdlib>
 #include <type_traits>
 
 #include "genn_mi355x_delta_kernels.h"
@@ -43,6 +44,9 @@ int checkDelta(const char *what, const gennmi_delta_rule_t *c, bool gradients)
         {"q", &c->q, c->keyHeads * c->keys, size}, {"k", &c->k, c->keyHeads * c->keys, size}, {"v", &c->v, c->heads * c->values, size}, {"g", &c->g, c->heads, 4}, {"beta", &c->beta, c->heads, 4}};
     for(const auto &r : read) { if(const int rc = checkRows(what, r.which, *r.rows, c->sequences, r.width, r.size)) { return rc; } }
     if(!gradients) { if(const int rc = checkWrittenRows(what, "out", c->out, c->sequences, c->heads * c->values, size)) { return rc; } }
+    for(const gennmi_rows_t *r : {&c->v, &c->out}) {
+        if(c->sequences.length > 1 && r->data && r->rowStride >= (1u << 26)) { return refuse(GENNMI_EINVAL, ": stride of v or out out of range"); }
+    }
     if((uintptr_t)c->initialState % 4 || (uintptr_t)c->finalState % 4) { return refuse(GENNMI_EINVAL, ": a state is not aligned"); }
     return GENNMI_OK;
 }
@@ -69,7 +73,23 @@ int deltaApart(const char *what, const gennmi_delta_rule_t &c, const gennmi_delt
                        unlessSame(regionOf("the gradient of the final state", g.finalState, states), g.initialState), offsetsOf(s)});
 }
 
-struct DeltaSpace { size_t correction, score, rows, table, states, errors, gradientStates, gradientErrors, bytes; };
+// Segments that a sequence is cut into, so that there are work-groups for the whole chip: what each does to the state is found for all of them at once (the state's columns and
+// those of a unit matrix), then joined, then outputs are found for all of them at once.
+uint32_t segmentsOf(const gennmi_delta_rule_t &c, uint32_t columns)
+{
+    const uint32_t C = chunkRows(c.type), chunks = (c.sequences.length + C - 1) / C;
+    if(const char *e = getenv("SEG")) { return std::max(1u, std::min(chunks, (uint32_t)atoi(e))); }
+    return 1;
+}
+// Rows of a segment: a multiple of a chunk's
+uint32_t segmentRows(const gennmi_delta_rule_t &c, bool gradients)
+{
+    const uint32_t C = chunkRows(c.type), chunks = std::max(1u, (c.sequences.length + C - 1) / C), segments = gradients ? 1 : segmentsOf(c, c.values);
+    return (chunks + segments - 1) / segments * C;
+}
+bool isCut(const gennmi_delta_rule_t &c, bool gradients) { return c.sequences.length > segmentRows(c, gradients); }
+uint32_t moveBlocks(const gennmi_delta_rule_t &c, uint32_t columns) { const uint32_t each = 16 * wavesFor(columns); return (paddedKeys(c.keys) + each - 1) / each; }
+struct DeltaSpace { size_t correction, score, rows, table, segmentStates, segmentMoves, states, errors, gradientStates, gradientErrors, bytes; };
 DeltaSpace deltaSpace(const gennmi_delta_rule_t &c, bool gradients)
 {
     DeltaSpace s{};
@@ -78,8 +98,13 @@ DeltaSpace deltaSpace(const gennmi_delta_rule_t &c, bool gradients)
     const auto take = [&](uint64_t bytes) { const size_t at = s.bytes; s.bytes += (bytes + 255) / 256 * 256; return at; };
     s.correction = take(numbers * C * C * 4);
     s.score = take(numbers * C * C * 4);
-    s.rows = take(numbers * C * sizeof(RowTable));
+    s.rows = take(numbers * C * 32);
     s.table = take(numbers * sizeof(ChunkTable));
+    if(isCut(c, gradients)) {
+        const uint64_t segments = chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.heads;
+        s.segmentStates = take(segments * paddedKeys(c.keys) * padded * 4);
+        s.segmentMoves = take(segments * paddedKeys(c.keys) * paddedKeys(c.keys) * 4);
+    }
     if(gradients) {
         s.states = take(numbers * paddedKeys(c.keys) * padded * 4);
         s.errors = take(numbers * C * padded * 4);
@@ -88,12 +113,6 @@ DeltaSpace deltaSpace(const gennmi_delta_rule_t &c, bool gradients)
     }
     return s;
 }
-// Rows of a segment: a multiple of a chunk's
-uint32_t segmentRows(const gennmi_delta_rule_t &c)
-{
-    const uint32_t C = chunkRows(c.type);
-    return std::max(1u, (c.sequences.length + C - 1) / C) * C;
-}
 uint32_t tokenVector(const gennmi_delta_rule_t &c) { return c.values % 4 == 0 && (uintptr_t)c.initialState % 16 == 0 && (uintptr_t)c.finalState % 16 == 0 ? 4 : 1; }
 uint64_t tokenBlocks(const gennmi_delta_rule_t &c) { const uint32_t columns = 8 * tokenVector(c); return (uint64_t)c.sequences.count * c.heads * ((c.values + columns - 1) / columns); }
 bool deltaFits(const gennmi_delta_rule_t &c, bool gradients)
@@ -101,13 +120,14 @@ bool deltaFits(const gennmi_delta_rule_t &c, bool gradients)
     if(!gradients && c.sequences.length <= 1) { return tokenBlocks(c) <= mostBlocks(256); }
     const uint32_t columns = gradients ? paddedValues(c.values) : c.values;
     return chunkNumbers(c.sequences, chunkRows(c.type)) * c.keyHeads <= mostBlocks(512) &&
-        chunkNumbers(c.sequences, segmentRows(c)) * c.heads * blocksOf(columns) <= mostBlocks(64 * wavesFor(columns));
+        chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.heads * (blocksOf(columns) + moveBlocks(c, columns)) <= mostBlocks(64 * wavesFor(columns)) &&
+        (uint64_t)c.sequences.count * c.heads * (paddedValues(c.values) / 16) <= mostBlocks(64);
 }
 DeltaArgs deltaArgs(const gennmi_delta_rule_t &c, const DeltaSpace &space, void *workspace, bool gradients)
 {
     DeltaArgs a{};
     a.chunks = sequencesOf(c.sequences, chunkRows(c.type));
-    a.segments = sequencesOf(c.sequences, segmentRows(c));
+    a.segments = sequencesOf(c.sequences, segmentRows(c, gradients));
     a.q = c.q; a.k = c.k; a.v = c.v; a.out = c.out; a.g = c.g; a.beta = c.beta;
     a.initialState = c.initialState;
     a.finalState = gradients ? nullptr : c.finalState;
@@ -121,8 +141,13 @@ DeltaArgs deltaArgs(const gennmi_delta_rule_t &c, const DeltaSpace &space, void 
     const auto at = [&](size_t offset) { return (char*)workspace + offset; };
     a.correction = (float*)at(space.correction);
     a.score = (float*)at(space.score);
-    a.rows = (RowTable*)at(space.rows);
+    a.rows = at(space.rows);
     a.table = (ChunkTable*)at(space.table);
+    if(isCut(c, gradients)) {
+        a.segmentStates = (float*)at(space.segmentStates);
+        a.segmentMoves = (float*)at(space.segmentMoves);
+        a.moveBlocks = moveBlocks(c, gradients ? a.padded : a.values);
+    }
     if(gradients) {
         a.states = (float*)at(space.states);
         a.errors = (float*)at(space.errors);
@@ -137,29 +162,37 @@ template<typename K> int withLds(const char *what, K kernel, size_t bytes)
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     return e == hipSuccess ? (int)GENNMI_OK : fail(GENNMI_EHIP, std::string(what) + ": " + hipGetErrorString(e));
 }
-template<typename T, int C, int DK> int launchChunks(const char *what, const DeltaArgs &a, uint64_t numbers, hipStream_t stream)
+template<typename T, int C, int DK, bool FOLDED> int launchChunks(const char *what, const DeltaArgs &a, uint64_t numbers, hipStream_t stream)
 {
-    const auto kernel = deltaChunkKernel<T, C, DK>;
+    const auto kernel = deltaChunkKernel<T, C, DK, FOLDED>;
     constexpr size_t lds = chunkLds<T, C, DK>();
     if(const int rc = withLds(what, kernel, lds)) { return rc; }
     kernel<<<dim3((uint32_t)(numbers * a.keyHeads)), dim3(256), lds, stream>>>(a);
     return gennmi_detail::afterLaunch(what);
 }
-template<typename T, int C, int DK, int MODE> int launchWalk(const char *what, const DeltaArgs &a, uint64_t segments, hipStream_t stream)
+template<typename T, int C, int DK, int MODE, bool FOLDED> int launchWalk(const char *what, const DeltaArgs &a, uint64_t segments, hipStream_t stream)
 {
-    return withWaves(MODE == WALK_OUTPUTS ? a.values : a.padded, [&](auto waves) {
+    return withWaves(FOLDED ? a.values : a.padded, [&](auto waves) {
         constexpr int WAVES = decltype(waves)::value;
-        const auto kernel = deltaStateKernel<T, C, DK, WAVES, MODE>;
+        const auto kernel = deltaStateKernel<T, C, DK, WAVES, MODE, FOLDED>;
         constexpr size_t lds = WalkLayout<T, C, DK, MODE>::bytes;
         if(const int rc = withLds(what, kernel, lds)) { return rc; }
-        kernel<<<dim3((uint32_t)(segments * a.heads * a.columnBlocks)), dim3(64 * WAVES), lds, stream>>>(a);
+        kernel<<<dim3((uint32_t)(segments * a.heads * (a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0)))), dim3(64 * WAVES), lds, stream>>>(a);
         return gennmi_detail::afterLaunch(what);
     });
 }
+// The state in front of every segment
+template<typename T, int C, int DK, bool FOLDED> int launchSegments(const char *what, const DeltaArgs &a, uint64_t segments, hipStream_t stream)
+{
+    if(!a.segmentStates) { return GENNMI_OK; }
+    if(const int rc = launchWalk<T, C, DK, WALK_SUMMARY, FOLDED>(what, a, segments, stream)) { return rc; }
+    deltaJoinKernel<DK><<<dim3(a.chunks.count * a.heads * (a.padded / 16)), dim3(64), 0, stream>>>(a);
+    return gennmi_detail::afterLaunch(what);
+}
 template<typename T, int C, int DK> int launchGradients(const char *what, const DeltaArgs &a, const DeltaGradientArgs &d, uint64_t numbers, uint64_t segments, hipStream_t stream)
 {
-    if(const int rc = launchChunks<T, C, DK>(what, a, numbers, stream)) { return rc; }
-    if(const int rc = launchWalk<T, C, DK, WALK_KEEP>(what, a, segments, stream)) { return rc; }
+    if(const int rc = launchChunks<T, C, DK, false>(what, a, numbers, stream)) { return rc; }
+    if(const int rc = launchWalk<T, C, DK, WALK_KEEP, false>(what, a, segments, stream)) { return rc; }
     const int rc = withWaves(a.padded, [&](auto waves) {
         constexpr int WAVES = decltype(waves)::value;
         const auto kernel = deltaReverseKernel<T, C, DK, WAVES>;
@@ -224,8 +257,10 @@ int gennmi_delta_rule(const gennmi_delta_rule_t *rule, void *workspace, size_t w
             rc = withSizes(*rule, [&](auto t, auto rows, auto keys) {
                 typedef decltype(t) T;
                 constexpr int C = decltype(rows)::value, DK = decltype(keys)::value;
-                if(const int rcChunks = launchChunks<T, C, DK>(what, a, chunkNumbers(rule->sequences, C), s)) { return rcChunks; }
-                return launchWalk<T, C, DK, WALK_OUTPUTS>(what, a, chunkNumbers(rule->sequences, a.segments.chunk), s);
+                if(const int rcChunks = launchChunks<T, C, DK, true>(what, a, chunkNumbers(rule->sequences, C), s)) { return rcChunks; }
+                const uint64_t segments = chunkNumbers(rule->sequences, a.segments.chunk);
+                if(const int rcSegments = launchSegments<T, C, DK, true>(what, a, segments, s)) { return rcSegments; }
+                return launchWalk<T, C, DK, WALK_OUTPUTS, true>(what, a, segments, s);
             });
         }
         if(rc) { return rc; }
@@ -261,6 +296,9 @@ int gennmi_delta_rule_backward(const gennmi_delta_rule_t *rule, const gennmi_del
         for(const auto &w : written) {
             if(!w.rows->data) { continue; }
             if(const int rc = checkWrittenRows(what, w.which, *w.rows, rule->sequences, w.width, w.size)) { return rc; }
+        }
+        if(rule->sequences.length > 1 && (in.out.rowStride >= (1u << 26) || (in.v.data && in.v.rowStride >= (1u << 26)))) {
+            return fail(GENNMI_EINVAL, "delta_rule_backward: stride of the gradients of v or out out of range");
         }
         if((uintptr_t)in.finalState % 4 || (uintptr_t)in.initialState % 4) { return fail(GENNMI_EINVAL, "delta_rule_backward: a state is not aligned"); }
         if(!deltaFits(*rule, true)) { return tooMany(what); }

@@ -23,15 +23,28 @@ using namespace gennmi_elements;
 using namespace gennmi_planes;
 using gennmi_lanes::partner;
 
-// What a row of a chunk needs of one head
-struct alignas(32) RowTable
+// Keeps the compiler from asking for all of LDS's operands at once, which costs more registers than there are
+__device__ inline void inTurn() { __builtin_amdgcn_sched_barrier(0); }
+
+// What the rows of a chunk need of one head
+template<int C> struct alignas(16) RowTable
 {
-    float keyState;         // G / |k|: times the key and the state
-    float beta;
-    float keyEnd;           // D[last] / |k|: times the key and u, what the row leaves in the state behind the chunk
-    float queryState;       // scale G / |q|
-    float keyUnit, queryUnit;       // 1 / |k|, 1 / |q|
-    double sum;             // of g, since the chunk's beginning
+    float keyState[C];      // G / |k|: times the key and the state
+    float beta[C];
+    float keyEnd[C];        // D[last] / |k|: times the key and u, what the row leaves in the state behind the chunk
+    float queryState[C];    // scale G / |q|
+    float keyUnit[C], queryUnit[C];     // 1 / |k|, 1 / |q|
+    double sum[C];          // of g, since the chunk's beginning
+};
+// The first four of them, in LDS; four rows that are a lane's in a result an access
+template<int C> struct RowFactors
+{
+    float *at;
+    __device__ f32x4 four(int which, uint32_t row) const { const float4 x = *(const float4*)(at + which * C + row); return f32x4{x.x, x.y, x.z, x.w}; }
+    __device__ f32x4 keyState(uint32_t row) const { return four(0, row); }
+    __device__ f32x4 beta(uint32_t row) const { return four(1, row); }
+    __device__ f32x4 keyEnd(uint32_t row) const { return four(2, row); }
+    __device__ f32x4 queryState(uint32_t row) const { return four(3, row); }
 };
 struct ChunkTable { float decay; uint32_t bad; };          // G[last]; first row from which nothing is finite, or the chunk's rows
 
@@ -45,8 +58,10 @@ struct DeltaArgs
     uint32_t padded;                // values, up to a multiple of 32: the width of what is kept of them
     float scale, epsilon;
     float *correction, *score;      // of each chunk number and head: -N and P, [C][C]
-    RowTable *rows;                 // [C]
+    void *rows;                     // RowTable
     ChunkTable *table;
+    uint32_t moveBlocks;            // of the columns of a segment's `move`
+    float *segmentStates, *segmentMoves;        // of each segment and head [DK][padded], [DK][DK]; NULL: sequences are not cut
     float *states, *errors;         // kept for gradients, of each chunk number and head: the state in front of it [DK][padded], w [C][padded]
 };
 
@@ -58,9 +73,10 @@ __device__ inline bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 template<typename T> __device__ inline const T *rowAt(const gennmi_rows_t &r, const Sequences &s, const Place &p, uint32_t row) { return rowsOf<const T>(r, s, p) + (uint64_t)row * r.rowStride; }
 
 // ---- what a chunk needs that does not depend on the state
-template<typename T, int C, int DK> constexpr uint32_t chunkLds() { return 2 * planesOf<T> * C * (DK + 8) * 2 + C * (C + 4) * 4 + C * (8 + 3 * 4) + 16; }
+// FOLDED: for outputs alone, -N beta and P beta (I - N beta) are left, which r is multiplied with at once; else, for gradients, -N and P.
+template<typename T, int C, int DK> constexpr uint32_t chunkLds() { return 2 * planesOf<T> * C * (DK + 8) * 2 + 2 * C * (C + 4) * 4 + C * (8 + 3 * 4) + 16; }
 
-template<typename T, int C, int DK>
+template<typename T, int C, int DK, bool FOLDED>
 __global__ __launch_bounds__(256)
 void deltaChunkKernel(DeltaArgs a)
 {
@@ -68,7 +84,8 @@ void deltaChunkKernel(DeltaArgs a)
     extern __shared__ __align__(16) char lds[];
     uint16_t *const keyPlanes = (uint16_t*)lds, *const queryPlanes = keyPlanes + NP * PLANE;
     float *const m = (float*)(queryPlanes + NP * PLANE);
-    double *const sums = (double*)(m + C * MP);
+    float *const scores = m + C * MP;
+    double *const sums = (double*)(scores + C * MP);
     float *const keyUnit = (float*)(sums + C), *const queryUnit = keyUnit + C, *const beta = queryUnit + C;
     uint32_t *const bad = (uint32_t*)(beta + C);
     const uint32_t number = blockIdx.x / a.keyHeads, keyHead = blockIdx.x - number * a.keyHeads;
@@ -87,12 +104,11 @@ void deltaChunkKernel(DeltaArgs a)
         #pragma unroll
         for(int which = 0; which < 2; which++) {
             const gennmi_rows_t &r = which ? a.q : a.k;
-            T x[8];
-            loadEight(rowAt<T>(r, a.chunks, p, valid ? begin + row : 0) + (valid ? keyHead * a.keys + at : 0), valid, a.wide, x);
+            const Eight<T> x = loadEight(rowAt<T>(r, a.chunks, p, valid ? begin + row : 0) + (valid ? keyHead * a.keys + at : 0), valid, a.wide);
             float sum = 0.0f, first[4], second[4];
             #pragma unroll
             for(int e = 0; e < 8; e++) {
-                const float f = widen(x[e]);
+                const float f = widen(x.at(e));
                 sum = __builtin_fmaf(f, f, sum);
                 (e < 4 ? first[e] : second[e - 4]) = f;
             }
@@ -121,6 +137,7 @@ void deltaChunkKernel(DeltaArgs a)
         if(tileColumn(t) > tileRow(t)) { continue; }
         #pragma unroll
         for(int s = 0; s < DK / 32; s++) {
+            inTurn();
             const uint32_t offset = s * 32 + g * 8, ra = (tileRow(t) * 16 + n16) * PITCH + offset, rb = (tileColumn(t) * 16 + n16) * PITCH + offset;
             const Planes<NP> kb = fetch<NP>(keyPlanes + rb, PLANE);
             kk[t] = multiply(fetch<NP>(keyPlanes + ra, PLANE), kb, kk[t]);
@@ -131,7 +148,7 @@ void deltaChunkKernel(DeltaArgs a)
     for(uint32_t inGroup = 0; inGroup < a.group; inGroup++) {
         const uint32_t head = keyHead * a.group + inGroup;
         const uint64_t at = (uint64_t)number * a.heads + head;
-        RowTable *const rows = a.rows + at * C;
+        RowTable<C> *const rows = (RowTable<C>*)a.rows + at;
         if(tid == 0) { *bad = C; }
         float decay = 0.0f;
         if(wave == 0) {
@@ -149,7 +166,13 @@ void deltaChunkKernel(DeltaArgs a)
                 const float since = decayOver(sum), until = decayOver(last - sum), ku = keyUnit[lane], qu = queryUnit[lane];
                 sums[lane] = sum;
                 beta[lane] = b;
-                rows[lane] = RowTable{since * ku, b, until * ku, a.scale * since * qu, ku, qu, sum};
+                rows->keyState[lane] = since * ku;
+                rows->beta[lane] = b;
+                rows->keyEnd[lane] = until * ku;
+                rows->queryState[lane] = a.scale * since * qu;
+                rows->keyUnit[lane] = ku;
+                rows->queryUnit[lane] = qu;
+                rows->sum[lane] = sum;
                 // (sum, b and the key's length: what makes a row's errors no numbers, also in a chunk's first row)
                 if(valid && !(finite(b) && finite(since) && finite(ku))) { atomicMin(bad, lane); }
             }
@@ -169,13 +192,16 @@ void deltaChunkKernel(DeltaArgs a)
                 const float y = row >= column ? d * (a.scale * (queryUnit[row] * qk[t][r] * ku)) : 0.0f;
                 if(!finite(x)) { atomicMin(bad, row); }
                 m[row * MP + column] = x;
-                score[row * C + column] = y;
+                if(FOLDED) { scores[row * MP + column] = y; } else { score[row * C + column] = y; }
             }
         }
         __syncthreads();
         const uint32_t from = *bad;
         if(from < C) {      // (nothing finite from that row on: the rows before it must not meet it)
-            for(uint32_t i = from * C + tid; i < C * C; i += 256) { m[i / C * MP + i % C] = 0.0f; score[i] = 0.0f; }
+            for(uint32_t i = from * C + tid; i < C * C; i += 256) {
+                m[i / C * MP + i % C] = 0.0f;
+                if(FOLDED) { scores[i / C * MP + i % C] = 0.0f; } else { score[i] = 0.0f; }
+            }
             __syncthreads();
         }
         if(tid == 0) { a.table[at] = ChunkTable{decay, from}; }
@@ -212,10 +238,32 @@ void deltaChunkKernel(DeltaArgs a)
                 for(int s = 0; s < r; s++) { if((uint32_t)s >= wave) { found[r] = multiply(operand(r, s), found[s], found[r]); } }
                 found[r] = multiply(operand(r, r), found[r], found[r]);
             }
+            const float betaColumn = FOLDED ? beta[wave * 16 + n16] : 1.0f;
             #pragma unroll
             for(int r = 0; r < B; r++) {
                 #pragma unroll
-                for(int e = 0; e < 4; e++) { correction[(r * 16 + 4 * g + e) * C + wave * 16 + n16] = -found[r][e]; }
+                for(int e = 0; e < 4; e++) { found[r][e] *= -betaColumn; correction[(r * 16 + 4 * g + e) * C + wave * 16 + n16] = found[r][e]; }
+            }
+            if constexpr(FOLDED) {
+                // P beta (I - N beta), the same block column
+                #pragma unroll
+                for(int r = 0; r < B; r++) {
+                    f32x4 y = {0, 0, 0, 0};
+                    if((uint32_t)r >= wave) {
+                        #pragma unroll
+                        for(int e = 0; e < 4; e++) { y[e] = scores[(r * 16 + 4 * g + e) * MP + wave * 16 + n16] * betaColumn; }
+                        #pragma unroll
+                        for(int t = 0; t <= r; t++) {
+                            if((uint32_t)t < wave) { continue; }
+                            f32x4 x;
+                            #pragma unroll
+                            for(int e = 0; e < 4; e++) { x[e] = scores[(r * 16 + n16) * MP + t * 16 + 4 * g + e] * beta[t * 16 + 4 * g + e]; }
+                            y = multiply(x, found[t], y);
+                        }
+                    }
+                    #pragma unroll
+                    for(int e = 0; e < 4; e++) { score[(r * 16 + 4 * g + e) * C + wave * 16 + n16] = y[e]; }
+                }
             }
         }
         __syncthreads();
@@ -223,7 +271,8 @@ void deltaChunkKernel(DeltaArgs a)
 }
 
 // ---- the walk over chunks
-enum { WALK_OUTPUTS, WALK_KEEP };          // writes outputs, or keeps states and errors for gradients
+// Writes outputs; keeps states and errors for gradients; or finds what a segment of a sequence does to the state in front of it, S behind = move S + its own.
+enum { WALK_OUTPUTS, WALK_KEEP, WALK_SUMMARY };
 
 // LDS of a walk, in elements of 16 bits: keys by row and by column, queries by row, -N, P
 template<typename T, int C, int DK, int MODE> struct WalkLayout
@@ -235,7 +284,7 @@ template<typename T, int C, int DK, int MODE> struct WalkLayout
 };
 
 // A tile of four rows and eight columns of keys (or queries) on its way to LDS
-template<typename T> struct KeyTile { T x[4][8]; };
+template<typename T> struct KeyTile { Eight<T> row[4]; };
 template<typename T, int C, int DK> __device__ inline void loadTile(const DeltaArgs &a, const gennmi_rows_t &r, const Place &p, uint32_t keyHead, uint32_t begin, uint32_t count, uint32_t item, KeyTile<T> &tile)
 {
     const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
@@ -243,7 +292,7 @@ template<typename T, int C, int DK> __device__ inline void loadTile(const DeltaA
     #pragma unroll
     for(int i = 0; i < 4; i++) {
         const uint32_t valid = row + i < count && at < a.keys ? min(8u, a.keys - at) : 0;
-        loadEight(base + (valid ? (uint64_t)(row + i) * r.rowStride + at : 0), valid, a.wide, tile.x[i]);
+        tile.row[i] = loadEight(base + (valid ? (uint64_t)(row + i) * r.rowStride + at : 0), valid, a.wide);
     }
 }
 template<typename T, int NP> __device__ inline void planesOfFour(const T (&x)[4], uint2 (&out)[NP])
@@ -257,14 +306,36 @@ template<typename T, int C, int DK> __device__ inline void storeRows(uint16_t *t
     const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
     #pragma unroll
     for(int i = 0; i < 4; i++) {
+        uint2 words[2][NP];
         #pragma unroll
         for(int half = 0; half < 2; half++) {
-            const T x[4] = {tile.x[i][4 * half], tile.x[i][4 * half + 1], tile.x[i][4 * half + 2], tile.x[i][4 * half + 3]};
-            uint2 words[NP];
-            planesOfFour<T, NP>(x, words);
-            #pragma unroll
-            for(int k = 0; k < NP; k++) { *(uint2*)(to + k * C * PITCH + (row + i) * PITCH + place(at + 4 * half)) = words[k]; }
+            if constexpr(NP == 1) { words[half][0] = half ? make_uint2(tile.row[i].word[0].z, tile.row[i].word[0].w) : make_uint2(tile.row[i].word[0].x, tile.row[i].word[0].y); }
+            else {
+                const T x[4] = {tile.row[i].at(4 * half), tile.row[i].at(4 * half + 1), tile.row[i].at(4 * half + 2), tile.row[i].at(4 * half + 3)};
+                planesOfFour<T, NP>(x, words[half]);
+            }
         }
+        #pragma unroll
+        for(int k = 0; k < NP; k++) {
+            *(uint2*)(to + k * C * PITCH + (row + i) * PITCH + place(at)) = words[0][k];
+            *(uint2*)(to + k * C * PITCH + (row + i) * PITCH + place(at + 4)) = words[1][k];
+        }
+    }
+}
+// Four rows of one column, planes of 8 bytes
+template<typename T> __device__ inline void columnOf(const KeyTile<T> &tile, int e, uint2 (&words)[planesOf<T>])
+{
+    if constexpr(planesOf<T> == 1) {
+        const auto pair = [&](int i) {
+            const uint4 x = tile.row[i].word[0], y = tile.row[i + 1].word[0];
+            const uint32_t low = e / 2 == 0 ? x.x : e / 2 == 1 ? x.y : e / 2 == 2 ? x.z : x.w, high = e / 2 == 0 ? y.x : e / 2 == 1 ? y.y : e / 2 == 2 ? y.z : y.w;
+            return __builtin_amdgcn_perm(high, low, e % 2 ? 0x07060302u : 0x05040100u);
+        };
+        words[0] = make_uint2(pair(0), pair(2));
+    }
+    else {
+        const T x[4] = {tile.row[0].at(e), tile.row[1].at(e), tile.row[2].at(e), tile.row[3].at(e)};
+        planesOfFour<T, planesOf<T>>(x, words);
     }
 }
 template<typename T, int C, int DK> __device__ inline void storeColumns(uint16_t *to, uint32_t item, const KeyTile<T> &tile)
@@ -273,9 +344,8 @@ template<typename T, int C, int DK> __device__ inline void storeColumns(uint16_t
     const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
     #pragma unroll
     for(int e = 0; e < 8; e++) {
-        const T x[4] = {tile.x[0][e], tile.x[1][e], tile.x[2][e], tile.x[3][e]};
         uint2 words[NP];
-        planesOfFour<T, NP>(x, words);
+        columnOf<T>(tile, e, words);
         #pragma unroll
         for(int k = 0; k < NP; k++) { *(uint2*)(to + k * DK * PITCH + (at + e) * PITCH + place(row)) = words[k]; }
     }
@@ -305,8 +375,64 @@ template<int C> __device__ inline uint32_t firstBad(const f32x4 (&x)[C / 16], ui
     return min(first, (uint32_t)__shfl_xor((int)first, 32));
 }
 
+// Rows of values at a lane's column, in the order of a result: row 16 t + 4 g + r.  What differs between lanes is an offset of 32 bits (strides are
+// below 2^26 here), the rest is the scalar unit's.  Behind `count` rows, or the last column: zero.
+template<typename T, int TILES> struct Result { T v[TILES][4]; };
+template<typename T, int TILES> __device__ inline Result<T, TILES> requestResult(const T *rows, uint64_t stride, uint32_t g, uint32_t column, bool inside, uint32_t count)
+{
+    Result<T, TILES> x;
+    const uint32_t offset = 4 * g * (uint32_t)stride + (inside ? column : 0);
+    if(count >= 16 * TILES) {       // (all there: without a branch a row; columns behind the last read the first)
+        #pragma unroll
+        for(int t = 0; t < TILES; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { x.v[t][r] = (rows + (16 * t + r) * stride)[offset]; }
+        }
+        return x;
+    }
+    #pragma unroll
+    for(int t = 0; t < TILES; t++) {
+        #pragma unroll
+        for(int r = 0; r < 4; r++) {
+            x.v[t][r] = (T)0.0f;
+            if(16 * t + 4 * g + r < count) { x.v[t][r] = (rows + (16 * t + r) * stride)[offset]; }
+        }
+    }
+    return x;
+}
+template<typename T, int TILES> __device__ inline void takeResult(const Result<T, TILES> &from, bool inside, f32x4 (&x)[TILES])
+{
+    #pragma unroll
+    for(int t = 0; t < TILES; t++) {
+        #pragma unroll
+        for(int r = 0; r < 4; r++) { x[t][r] = inside ? widen(from.v[t][r]) : 0.0f; }
+    }
+}
+template<typename T, int C> __device__ inline void loadResult(const T *rows, uint64_t stride, uint32_t g, uint32_t column, bool inside, uint32_t count, f32x4 (&x)[C / 16])
+{
+    takeResult(requestResult<T, C / 16>(rows, stride, g, column, inside, count), inside, x);
+}
+template<typename T, int C> __device__ inline void storeResult(T *rows, uint64_t stride, uint32_t g, uint32_t column, bool inside, uint32_t count, const f32x4 (&x)[C / 16])
+{
+    const uint32_t offset = 4 * g * (uint32_t)stride + column;
+    if(!inside) { return; }
+    if(count >= C) {
+        #pragma unroll
+        for(int t = 0; t < C / 16; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { (rows + (16 * t + r) * stride)[offset] = narrow<T>(x[t][r]); }
+        }
+        return;
+    }
+    #pragma unroll
+    for(int t = 0; t < C / 16; t++) {
+        #pragma unroll
+        for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r < count) { (rows + (16 * t + r) * stride)[offset] = narrow<T>(x[t][r]); } }
+    }
+}
+
 // A work-group walks a sequence (or a segment of it) of one head with 16 columns of the state a wavefront.
-template<typename T, int C, int DK, int WAVES, int MODE>
+template<typename T, int C, int DK, int WAVES, int MODE, bool FOLDED>
 __global__ __launch_bounds__(64 * WAVES)
 void deltaStateKernel(DeltaArgs a)
 {
@@ -316,26 +442,35 @@ void deltaStateKernel(DeltaArgs a)
     constexpr int KEYS = C * DK / 32, KEY_ITEMS = KEYS * (OUTPUTS ? 2 : 1), EACH = (KEY_ITEMS + THREADS - 1) / THREADS, SQUARE = C * C / 4, SQUARES = (SQUARE + THREADS - 1) / THREADS;
     extern __shared__ __align__(16) char lds[];
     uint16_t *const planes = (uint16_t*)lds;
-    float4 *const table = (float4*)(planes + L::table);
+    const RowFactors<C> table{(float*)(planes + L::table)};
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
-    const uint32_t block = blockIdx.x % a.columnBlocks, rest = blockIdx.x / a.columnBlocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
+    const uint32_t blocks = a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0);
+    const uint32_t block = blockIdx.x % blocks, rest = blockIdx.x / blocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
     Place p;
     if(!locate(a.segments, segment, p)) { return; }
     const uint32_t begin = p.index * a.segments.chunk, end = min(p.length, begin + a.segments.chunk);
-    const uint32_t column = (block * WAVES + wave) * 16 + n16;
-    const bool active = (block * WAVES + wave) * 16 < (OUTPUTS ? a.values : a.padded), inside = column < a.values;
+    // (what is behind the last segment nobody asks)
+    if(MODE == WALK_SUMMARY && end == p.length) { return; }
+    const bool move = MODE == WALK_SUMMARY && block >= a.columnBlocks;
+    const uint32_t firstColumn = ((move ? block - a.columnBlocks : block) * WAVES + wave) * 16, column = firstColumn + n16;
+    const bool active = firstColumn < (move ? (uint32_t)DK : OUTPUTS ? a.values : a.padded), inside = !move && column < a.values;
     const uint32_t chunks = end > begin ? (end - begin + C - 1) / C : 0;
-    const uint64_t firstNumber = firstChunk(a.chunks, p.sequence) + begin / C;
+    const uint64_t firstNumber = firstChunk(a.chunks, p.sequence) + begin / C, segmentAt = (uint64_t)segment * a.heads + head;
 
     f32x4 state[STATE];
     #pragma unroll
-    for(int t = 0; t < STATE; t++) {
+    for(int t = 0; t < STATE; t++) { state[t] = f32x4{0, 0, 0, 0}; }
+    if(MODE == WALK_SUMMARY) {
         #pragma unroll
-        for(int r = 0; r < 4; r++) {
-            const uint32_t row = 16 * t + 4 * g + r;
-            state[t][r] = a.initialState && row < a.keys && inside ? a.initialState[(((uint64_t)p.state * a.heads + head) * a.keys + row) * a.values + column] : 0.0f;
+        for(int t = 0; t < STATE; t++) {
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { if(move && 16 * t + 4 * g + r == column) { state[t][r] = 1.0f; } }
         }
     }
+    else if(a.segmentStates) {
+        if(active) { loadResult<float, DK>(a.segmentStates + segmentAt * DK * a.padded, a.padded, g, column, true, DK, state); }
+    }
+    else if(a.initialState) { loadResult<float, DK>(a.initialState + ((uint64_t)p.state * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
 
     KeyTile<T> keyTiles[EACH];
     float4 corrections[SQUARES], scores[SQUARES];
@@ -357,13 +492,15 @@ void deltaStateKernel(DeltaArgs a)
             corrections[i] = ((const float4*)(a.correction + at * C * C))[item];
             if(OUTPUTS) { scores[i] = ((const float4*)(a.score + at * C * C))[item]; }
         }
-        if(tid < C) { rowTable = *(const float4*)(a.rows + at * C + tid); }
+        if(tid < C) { rowTable = ((const float4*)((const RowTable<C>*)a.rows + at))[tid]; }
     };
     if(chunks) { prefetch(0); }
     for(uint32_t n = 0; n < chunks; n++) {
         const uint32_t first = begin + n * C, count = min((uint32_t)C, end - first);
         const uint64_t at = (firstNumber + n) * a.heads + head;
         const ChunkTable chunk = a.table[at];
+        Result<T, TILES> values;
+        if(active) { values = requestResult<T, TILES>(rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)first * a.v.rowStride + head * a.values, a.v.rowStride, g, column, inside, move ? 0 : count); }
         __syncthreads();
         #pragma unroll
         for(int i = 0; i < EACH; i++) {
@@ -382,33 +519,20 @@ void deltaStateKernel(DeltaArgs a)
             storeSquare<C>(planes + L::correction, item, corrections[i]);
             if(OUTPUTS) { storeSquare<C>(planes + L::score, item, scores[i]); }
         }
-        if(tid < C) { table[tid] = rowTable; }
+        if(tid < C) { ((float4*)table.at)[tid] = rowTable; }
         __syncthreads();
         if(n + 1 < chunks) { prefetch(n + 1); }
         if(!active) { continue; }
 
         // r = v - G k^ S, and the part of the outputs that the state in front has
-        const T *const values = rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)first * a.v.rowStride + head * a.values + column;
         f32x4 w[TILES], x[TILES], o[TILES];
+        takeResult(values, inside, w);
+        if(MODE == WALK_KEEP) { storeResult<float, DK>(a.states + at * DK * a.padded, a.padded, g, column, true, DK, state); }
         #pragma unroll
-        for(int t = 0; t < TILES; t++) {
-            #pragma unroll
-            for(int r = 0; r < 4; r++) {
-                const uint32_t row = 16 * t + 4 * g + r;
-                w[t][r] = inside && row < count ? widen(values[(uint64_t)row * a.v.rowStride]) : 0.0f;
-            }
-            x[t] = o[t] = f32x4{0, 0, 0, 0};
-        }
-        if(!OUTPUTS) {
-            float *const kept = a.states + at * DK * a.padded + column;
-            #pragma unroll
-            for(int t = 0; t < STATE; t++) {
-                #pragma unroll
-                for(int r = 0; r < 4; r++) { kept[(16 * t + 4 * g + r) * a.padded] = state[t][r]; }
-            }
-        }
+        for(int t = 0; t < TILES; t++) { x[t] = o[t] = f32x4{0, 0, 0, 0}; }
         #pragma unroll
         for(int s = 0; s < DK / 32; s++) {
+            inTurn();
             const Planes<3> b = split<3>(state[2 * s], state[2 * s + 1]);
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
@@ -417,14 +541,15 @@ void deltaStateKernel(DeltaArgs a)
                 if(OUTPUTS) { o[t] = multiply(fetch<NP>(planes + L::queryRows + offset, C * L::ROW), b, o[t]); }
             }
         }
+        inTurn();
         float notFinite = 0.0f;
         #pragma unroll
         for(int t = 0; t < TILES; t++) {
+            const f32x4 keyState = table.keyState(16 * t + 4 * g);
+            if(OUTPUTS) { o[t] *= table.queryState(16 * t + 4 * g); }
             #pragma unroll
             for(int r = 0; r < 4; r++) {
-                const float4 row = table[16 * t + 4 * g + r];
-                w[t][r] = __builtin_fmaf(-row.x, x[t][r], w[t][r]);
-                o[t][r] *= row.w;
+                w[t][r] = __builtin_fmaf(-keyState[r], x[t][r], w[t][r]);
                 notFinite = __builtin_fmaf(w[t][r], 0.0f, notFinite);
             }
         }
@@ -438,55 +563,49 @@ void deltaStateKernel(DeltaArgs a)
                 for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r >= bad) { w[t][r] = 0.0f; } }
             }
         }
-        // w = r - N beta r; tiles above the diagonal are zero
+        // w = r - N beta r and out += P beta w; tiles above the diagonal are zero
         {
             Planes<3> b[TILES / 2];
             #pragma unroll
             for(int s = 0; s < TILES / 2; s++) {
-                f32x4 y[2];
-                #pragma unroll
-                for(int h = 0; h < 2; h++) {
+                f32x4 y[2] = {w[2 * s], w[2 * s + 1]};
+                if(!FOLDED) {
                     #pragma unroll
-                    for(int r = 0; r < 4; r++) { y[h][r] = w[2 * s + h][r] * table[16 * (2 * s + h) + 4 * g + r].y; }
+                    for(int h = 0; h < 2; h++) { y[h] *= table.beta(16 * (2 * s + h) + 4 * g); }
                 }
                 b[s] = split<3>(y[0], y[1]);
             }
             #pragma unroll
             for(int s = 0; s < TILES / 2; s++) {
+                inTurn();
                 #pragma unroll
                 for(int t = 2 * s; t < TILES; t++) {
-                    w[t] = multiply(fetch<3>(planes + L::correction + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b[s], w[t]);
+                    const uint32_t offset = (16 * t + n16) * L::COLUMN + 32 * s + 8 * g;
+                    w[t] = multiply(fetch<3>(planes + L::correction + offset, C * L::COLUMN), b[s], w[t]);
+                    if(OUTPUTS) { o[t] = multiply(fetch<3>(planes + L::score + offset, C * L::COLUMN), b[s], o[t]); }
                 }
             }
         }
-        if(!OUTPUTS) {
-            float *const kept = a.errors + at * C * a.padded + column;
+        inTurn();
+        if(__builtin_expect(bad < C, 0)) {
+            const float no = __builtin_nanf("");
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
                 #pragma unroll
-                for(int r = 0; r < 4; r++) { kept[(16 * t + 4 * g + r) * a.padded] = 16 * t + 4 * g + r < bad ? w[t][r] : __builtin_nanf(""); }
+                for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r >= bad) { w[t][r] = o[t][r] = no; } }
             }
         }
-        // out += P u, and the state behind the chunk
+        if(MODE == WALK_KEEP) { storeResult<float, C>(a.errors + at * C * a.padded, a.padded, g, column, true, C, w); }
+        if(OUTPUTS) { storeResult<T, C>(rowsOf<T>(a.out, a.chunks, p) + (uint64_t)first * a.out.rowStride + head * a.values, a.out.rowStride, g, column, inside, count, o); }
+        // the state behind the chunk
         #pragma unroll
         for(int t = 0; t < STATE; t++) { state[t] *= chunk.decay; }
         #pragma unroll
         for(int s = 0; s < TILES / 2; s++) {
-            f32x4 u[2], left[2];
+            inTurn();
+            f32x4 left[2];
             #pragma unroll
-            for(int h = 0; h < 2; h++) {
-                #pragma unroll
-                for(int r = 0; r < 4; r++) {
-                    const float4 row = table[16 * (2 * s + h) + 4 * g + r];
-                    u[h][r] = w[2 * s + h][r] * row.y;
-                    left[h][r] = u[h][r] * row.z;
-                }
-            }
-            if(OUTPUTS) {
-                const Planes<3> b = split<3>(u[0], u[1]);
-                #pragma unroll
-                for(int t = 2 * s; t < TILES; t++) { o[t] = multiply(fetch<3>(planes + L::score + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, o[t]); }
-            }
+            for(int h = 0; h < 2; h++) { left[h] = w[2 * s + h] * table.beta(16 * (2 * s + h) + 4 * g) * table.keyEnd(16 * (2 * s + h) + 4 * g); }
             const Planes<3> b = split<3>(left[0], left[1]);
             #pragma unroll
             for(int t = 0; t < STATE; t++) { state[t] = multiply(fetch<NP>(planes + L::keyColumns + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, DK * L::COLUMN), b, state[t]); }
@@ -495,33 +614,51 @@ void deltaStateKernel(DeltaArgs a)
             const float no = __builtin_nanf("");
             #pragma unroll
             for(int t = 0; t < STATE; t++) { state[t] = f32x4{no, no, no, no}; }
-            #pragma unroll
-            for(int t = 0; t < TILES; t++) {
-                #pragma unroll
-                for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r >= bad) { o[t][r] = no; } }
-            }
-        }
-        if(OUTPUTS && inside) {
-            T *const out = rowsOf<T>(a.out, a.chunks, p) + (uint64_t)first * a.out.rowStride + head * a.values + column;
-            #pragma unroll
-            for(int t = 0; t < TILES; t++) {
-                #pragma unroll
-                for(int r = 0; r < 4; r++) {
-                    const uint32_t row = 16 * t + 4 * g + r;
-                    if(row < count) { out[(uint64_t)row * a.out.rowStride] = narrow<T>(o[t][r]); }
-                }
-            }
         }
     }
-    if(a.finalState && inside && end == p.length) {
+    if(!active) { return; }
+    if(MODE == WALK_SUMMARY) {
+        float *const to = move ? a.segmentMoves + segmentAt * DK * DK : a.segmentStates + segmentAt * DK * a.padded;
+        storeResult<float, DK>(to, move ? DK : a.padded, g, column, true, DK, state);
+    }
+    if(MODE == WALK_OUTPUTS && a.finalState && end == p.length) {
+        storeResult<float, DK>(a.finalState + ((uint64_t)p.state * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state);
+    }
+}
+
+// From what each segment does: the state in front of each, in place of its own share.  A wavefront has 16 columns; S = move S + own in fp32.
+template<int DK>
+__global__ __launch_bounds__(64)
+void deltaJoinKernel(DeltaArgs a)
+{
+    constexpr int STATE = DK / 16;
+    const uint32_t lane = threadIdx.x, n16 = lane & 15, g = lane >> 4, tiles = a.padded / 16;
+    const uint32_t tile = blockIdx.x % tiles, rest = blockIdx.x / tiles, head = rest % a.heads, sequence = rest / a.heads, column = tile * 16 + n16;
+    Place p;
+    if(!describe(a.segments, sequence, p)) { return; }
+    f32x4 state[STATE];
+    #pragma unroll
+    for(int t = 0; t < STATE; t++) { state[t] = f32x4{0, 0, 0, 0}; }
+    if(a.initialState) { loadResult<float, DK>(a.initialState + ((uint64_t)p.state * a.heads + head) * a.keys * a.values, a.values, g, column, column < a.values, a.keys, state); }
+    const uint32_t segments = max(1u, (p.length + a.segments.chunk - 1) / a.segments.chunk);
+    uint64_t at = firstChunk(a.segments, sequence) * a.heads + head;
+    for(uint32_t n = 0; n < segments; n++, at += a.heads) {
+        float *const own = a.segmentStates + at * DK * a.padded;
+        f32x4 next[STATE];
+        if(n + 1 < segments) { loadResult<float, DK>(own, a.padded, g, column, true, DK, next); }
+        storeResult<float, DK>(own, a.padded, g, column, true, DK, state);
+        if(n + 1 == segments) { break; }
+        const float *const move = a.segmentMoves + at * DK * DK;
         #pragma unroll
-        for(int t = 0; t < STATE; t++) {
+        for(int m = 0; m < STATE; m++) {
             #pragma unroll
-            for(int r = 0; r < 4; r++) {
-                const uint32_t row = 16 * t + 4 * g + r;
-                if(row < a.keys) { a.finalState[(((uint64_t)p.state * a.heads + head) * a.keys + row) * a.values + column] = state[t][r]; }
+            for(int t = 0; t < STATE; t++) {
+                const float4 x = *(const float4*)(move + (16 * m + n16) * DK + 16 * t + 4 * g);
+                next[m] = multiply(f32x4{x.x, x.y, x.z, x.w}, state[t], next[m]);
             }
         }
+        #pragma unroll
+        for(int t = 0; t < STATE; t++) { state[t] = next[t]; }
     }
 }
 
@@ -572,7 +709,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
     constexpr int KEYS = C * DK / 32, KEY_ITEMS = 2 * KEYS, EACH = (KEY_ITEMS + THREADS - 1) / THREADS, SQUARE = C * C / 16, SQUARE_ITEMS = 2 * SQUARE, SQUARES = (SQUARE_ITEMS + THREADS - 1) / THREADS;
     extern __shared__ __align__(16) char lds[];
     uint16_t *const planes = (uint16_t*)lds;
-    float4 *const table = (float4*)(planes + L::table);
+    const RowFactors<C> table{(float*)(planes + L::table)};
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
     const uint32_t block = blockIdx.x % a.columnBlocks, rest = blockIdx.x / a.columnBlocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
     Place p;
@@ -585,13 +722,8 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
 
     f32x4 state[STATE];
     #pragma unroll
-    for(int t = 0; t < STATE; t++) {
-        #pragma unroll
-        for(int r = 0; r < 4; r++) {
-            const uint32_t row = 16 * t + 4 * g + r;
-            state[t][r] = d.finalState && row < a.keys && inside ? d.finalState[(((uint64_t)p.sequence * a.heads + head) * a.keys + row) * a.values + column] : 0.0f;
-        }
-    }
+    for(int t = 0; t < STATE; t++) { state[t] = f32x4{0, 0, 0, 0}; }
+    if(d.finalState) { loadResult<float, DK>(d.finalState + ((uint64_t)p.sequence * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
     KeyTile<T> keyTiles[EACH];
     SquareTile squares[SQUARES];
     float4 rowTable;
@@ -611,13 +743,15 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             if(SQUARE_ITEMS % THREADS && item >= SQUARE_ITEMS) { break; }
             loadSquareTile<C>((item < SQUARE ? a.correction : a.score) + at * C * C, item < SQUARE ? item : item - SQUARE, squares[i]);
         }
-        if(tid < C) { rowTable = *(const float4*)(a.rows + at * C + tid); }
+        if(tid < C) { rowTable = ((const float4*)((const RowTable<C>*)a.rows + at))[tid]; }
     };
     if(chunks) { prefetch(chunks - 1); }
     for(uint32_t left = chunks; left > 0; left--) {
         const uint32_t n = left - 1, first = begin + n * C, count = min((uint32_t)C, end - first);
         const uint64_t at = (firstNumber + n) * a.heads + head;
         const float decay = a.table[at].decay;
+        Result<T, TILES> douts;
+        if(active) { douts = requestResult<T, TILES>(rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)first * d.out.rowStride + head * a.values, d.out.rowStride, g, column, inside, count); }
         __syncthreads();
         #pragma unroll
         for(int i = 0; i < EACH; i++) {
@@ -635,42 +769,31 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             if(SQUARE_ITEMS % THREADS && item >= SQUARE_ITEMS) { break; }
             storeSquareColumns<C>(planes + (item < SQUARE ? L::correction : L::score), item < SQUARE ? item : item - SQUARE, squares[i]);
         }
-        if(tid < C) { table[tid] = rowTable; }
+        if(tid < C) { ((float4*)table.at)[tid] = rowTable; }
         __syncthreads();
         if(n > 0) { prefetch(n - 1); }
         if(!active) { continue; }
 
-        const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)first * d.out.rowStride + head * a.values + column;
         f32x4 dout[TILES], du[TILES];
+        takeResult(douts, inside, dout);
         #pragma unroll
-        for(int t = 0; t < TILES; t++) {
-            #pragma unroll
-            for(int r = 0; r < 4; r++) {
-                const uint32_t row = 16 * t + 4 * g + r;
-                dout[t][r] = inside && row < count ? widen(douts[(uint64_t)row * d.out.rowStride]) : 0.0f;
-            }
-            du[t] = f32x4{0, 0, 0, 0};
-        }
-        float *const keptState = d.states + at * DK * a.padded + column;
-        #pragma unroll
-        for(int t = 0; t < STATE; t++) {
-            #pragma unroll
-            for(int r = 0; r < 4; r++) { keptState[(16 * t + 4 * g + r) * a.padded] = state[t][r]; }
-        }
+        for(int t = 0; t < TILES; t++) { du[t] = f32x4{0, 0, 0, 0}; }
+        storeResult<float, DK>(d.states + at * DK * a.padded, a.padded, g, column, true, DK, state);
         // dU = D[last] k^ dS + P' dout
         #pragma unroll
         for(int s = 0; s < DK / 32; s++) {
+            inTurn();
             const Planes<3> b = split<3>(state[2 * s], state[2 * s + 1]);
             #pragma unroll
             for(int t = 0; t < TILES; t++) { du[t] = multiply(fetch<NP>(planes + L::keyRows + (16 * t + n16) * L::ROW + 32 * s + 8 * g, C * L::ROW), b, du[t]); }
         }
         #pragma unroll
         for(int t = 0; t < TILES; t++) {
-            #pragma unroll
-            for(int r = 0; r < 4; r++) { du[t][r] *= table[16 * t + 4 * g + r].z; }
+            du[t] *= table.keyEnd(16 * t + 4 * g);
         }
         #pragma unroll
         for(int s = 0; s < TILES / 2; s++) {
+            inTurn();
             const Planes<NP> b = split<NP>(dout[2 * s], dout[2 * s + 1]);
             #pragma unroll
             for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(fetch<3>(planes + L::score + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, du[t]); }
@@ -680,41 +803,33 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             Planes<3> b[TILES / 2];
             #pragma unroll
             for(int s = 0; s < TILES / 2; s++) {
+                inTurn();
                 f32x4 y[2];
                 #pragma unroll
-                for(int h = 0; h < 2; h++) {
-                    #pragma unroll
-                    for(int r = 0; r < 4; r++) { y[h][r] = du[2 * s + h][r] * table[16 * (2 * s + h) + 4 * g + r].y; }
-                }
+                for(int h = 0; h < 2; h++) { y[h] = du[2 * s + h] * table.beta(16 * (2 * s + h) + 4 * g); }
                 b[s] = split<3>(y[0], y[1]);
             }
             #pragma unroll
             for(int s = 0; s < TILES / 2; s++) {
+                inTurn();
                 #pragma unroll
                 for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(fetch<3>(planes + L::correction + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b[s], du[t]); }
             }
         }
-        float *const keptError = d.errors + at * C * a.padded + column;
-        #pragma unroll
-        for(int t = 0; t < TILES; t++) {
-            #pragma unroll
-            for(int r = 0; r < 4; r++) { keptError[(16 * t + 4 * g + r) * a.padded] = du[t][r]; }
-        }
+        storeResult<float, C>(d.errors + at * C * a.padded, a.padded, g, column, true, C, du);
         // dS in front of the chunk = G[last] dS + (scale G q^)' dout - (G k^)' (beta dR)
         #pragma unroll
         for(int t = 0; t < STATE; t++) { state[t] *= decay; }
         #pragma unroll
         for(int s = 0; s < TILES / 2; s++) {
+            inTurn();
             f32x4 x[2], y[2];
             #pragma unroll
             for(int h = 0; h < 2; h++) {
-                #pragma unroll
-                for(int r = 0; r < 4; r++) {
-                    const float4 row = table[16 * (2 * s + h) + 4 * g + r];
-                    x[h][r] = dout[2 * s + h][r] * row.w;
-                    du[2 * s + h][r] *= row.y;
-                    y[h][r] = -row.x * du[2 * s + h][r];
-                }
+                const uint32_t row = 16 * (2 * s + h) + 4 * g;
+                x[h] = dout[2 * s + h] * table.queryState(row);
+                du[2 * s + h] *= table.beta(row);
+                y[h] = -table.keyState(row) * du[2 * s + h];
             }
             const Planes<3> bx = split<3>(x[0], x[1]), by = split<3>(y[0], y[1]);
             #pragma unroll
@@ -724,28 +839,9 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
                 state[t] = multiply(fetch<NP>(planes + L::keyColumns + offset, DK * L::COLUMN), by, state[t]);
             }
         }
-        if(d.v.data && inside) {
-            T *const dv = rowsOf<T>(d.v, a.chunks, p) + (uint64_t)first * d.v.rowStride + head * a.values + column;
-            #pragma unroll
-            for(int t = 0; t < TILES; t++) {
-                #pragma unroll
-                for(int r = 0; r < 4; r++) {
-                    const uint32_t row = 16 * t + 4 * g + r;
-                    if(row < count) { dv[(uint64_t)row * d.v.rowStride] = narrow<T>(du[t][r]); }
-                }
-            }
-        }
+        if(d.v.data) { storeResult<T, C>(rowsOf<T>(d.v, a.chunks, p) + (uint64_t)first * d.v.rowStride + head * a.values, d.v.rowStride, g, column, inside, count, du); }
     }
-    if(d.initialState && inside && begin == 0) {
-        #pragma unroll
-        for(int t = 0; t < STATE; t++) {
-            #pragma unroll
-            for(int r = 0; r < 4; r++) {
-                const uint32_t row = 16 * t + 4 * g + r;
-                if(row < a.keys) { d.initialState[(((uint64_t)p.sequence * a.heads + head) * a.keys + row) * a.values + column] = state[t][r]; }
-            }
-        }
-    }
+    if(d.initialState && active && begin == 0) { storeResult<float, DK>(d.initialState + ((uint64_t)p.sequence * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
 }
 
 // ---- gradients of a chunk, once the state in front of it, w, the gradient of the state behind it and dR are known
@@ -801,9 +897,8 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         uint16_t *const to = planes + (isKey ? L::keyColumns : L::queryColumns);
         #pragma unroll
         for(int e = 0; e < 8; e++) {
-            const T x[4] = {tile.x[0][e], tile.x[1][e], tile.x[2][e], tile.x[3][e]};
             uint2 words[NP];
-            planesOfFour<T, NP>(x, words);
+            columnOf<T>(tile, e, words);
             #pragma unroll
             for(int k = 0; k < NP; k++) { *(uint2*)(to + k * DK * L::COLUMN + (at + e) * L::COLUMN + row) = words[k]; }
         }
@@ -835,14 +930,14 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         __syncthreads();
         const float decay = a.table[at].decay;
         if(tid < C) {
-            const RowTable row = a.rows[at * C + tid];
-            const double last = a.rows[at * C + C - 1].sum;
-            sums[tid] = row.sum;
-            since[tid] = decayOver(row.sum);
-            until[tid] = decayOver(last - row.sum);
-            beta[tid] = row.beta;
-            keyUnit[tid] = row.keyUnit;
-            queryUnit[tid] = row.queryUnit;
+            const RowTable<C> &rows = ((const RowTable<C>*)a.rows)[at];
+            const double sum = rows.sum[tid], last = rows.sum[C - 1];
+            sums[tid] = sum;
+            since[tid] = decayOver(sum);
+            until[tid] = decayOver(last - sum);
+            beta[tid] = rows.beta[tid];
+            keyUnit[tid] = rows.keyUnit[tid];
+            queryUnit[tid] = rows.queryUnit[tid];
         }
         f32x4 outS[MINE], rS[MINE], wD[MINE], outW[SQUARES], rW[SQUARES];
         #pragma unroll
@@ -896,6 +991,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             const Planes<3> state = split<3>(s0a, s0b), dState = split<3>(dsa, dsb);
             #pragma unroll
             for(int m = 0; m < MINE; m++) {
+                inTurn();
                 const uint32_t offset = (tileOf(m) * 16 + n16) * L::VALUES + 8 * g;
                 outS[m] = multiply(fetch<NP>(doutPlanes + offset, VP), state, outS[m]);
                 rS[m] = multiply(fetch<3>(dRPlanes + offset, VP), state, rS[m]);
@@ -905,6 +1001,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
                 const Planes<3> other = fetch<3>(wPlanes + (squareColumn * 16 + n16) * L::VALUES + 8 * g, VP);
                 #pragma unroll
                 for(int q = 0; q < SQUARES; q++) {
+                    inTurn();
                     if(squareRow(q) < squareColumn) { continue; }
                     const uint32_t offset = (squareRow(q) * 16 + n16) * L::VALUES + 8 * g;
                     outW[q] = multiply(fetch<NP>(doutPlanes + offset, VP), other, outW[q]);
@@ -1003,9 +1100,10 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     const auto timesColumns = [&](uint32_t from, f32x4 (&to)[MINE]) {
         #pragma unroll
         for(int s = 0; s < TILES / 2; s++) {
+            inTurn();
             const Planes<NP> b = fetch<NP>(planes + from + key * L::COLUMN + 32 * s + 8 * g, DK * L::COLUMN);
             #pragma unroll
-            for(int m = 0; m < MINE; m++) { to[m] = multiply(fetch<3>(stage + (tileOf(m) * 16 + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, to[m]); }
+            for(int m = 0; m < MINE; m++) { inTurn(); to[m] = multiply(fetch<3>(stage + (tileOf(m) * 16 + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, to[m]); }
         }
     };
     __syncthreads();

@@ -96,23 +96,41 @@ __device__ inline f32x4 multiply(const f32x4 &a, const f32x4 &b, f32x4 sum)
     for(int e = 0; e < 4; e++) { sum = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], sum, 0, 0, 0); }
     return sum;
 }
-// `valid` of eight neighbouring elements, zero behind them; `wide`: they lie on 16 bytes, and there are eight or none
-template<typename T> __device__ inline void loadEight(const T *at, uint32_t valid, bool wide, T (&v)[8])
+// Eight neighbouring elements, as they lie in memory
+template<typename T> struct Eight
 {
-    using gennmi_elements::Pack;
-    constexpr int EACH = 16 / sizeof(T);
+    uint4 word[sizeof(T) / 2];
+    __device__ T at(int i) const
+    {
+        const uint32_t w[4] = {word[i * sizeof(T) / 16].x, word[i * sizeof(T) / 16].y, word[i * sizeof(T) / 16].z, word[i * sizeof(T) / 16].w};
+        const int byte = i * sizeof(T) % 16;
+        if constexpr(sizeof(T) == 4) { return __builtin_bit_cast(T, w[byte / 4]); }
+        else { return __builtin_bit_cast(T, (uint16_t)(w[byte / 4] >> (byte % 4 * 8))); }
+    }
+};
+// `valid` of them, zero behind those; `wide`: they lie on 16 bytes, and there are eight or none
+template<typename T> __device__ inline Eight<T> loadEight(const T *at, uint32_t valid, bool wide)
+{
+    Eight<T> out;
+    #pragma unroll
+    for(int h = 0; h < (int)sizeof(T) / 2; h++) { out.word[h] = make_uint4(0, 0, 0, 0); }
     if(wide) {
-        #pragma unroll
-        for(int i = 0; i < 8; i += EACH) {
-            Pack<T, EACH> p{};
-            if(valid) { p = *(const Pack<T, EACH>*)(at + i); }
+        if(valid) {
             #pragma unroll
-            for(int e = 0; e < EACH; e++) { v[i + e] = p.v[e]; }
+            for(int h = 0; h < (int)sizeof(T) / 2; h++) { out.word[h] = ((const uint4*)at)[h]; }
         }
-        return;
+        return out;
+    }
+    uint32_t w[2 * sizeof(T)] = {};
+    #pragma unroll
+    for(int i = 0; i < 8; i++) {
+        if((uint32_t)i >= valid) { continue; }
+        if constexpr(sizeof(T) == 4) { w[i] = __builtin_bit_cast(uint32_t, at[i]); }
+        else { w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, at[i]) << (i % 2 * 16); }
     }
     #pragma unroll
-    for(int i = 0; i < 8; i++) { v[i] = (uint32_t)i < valid ? at[i] : (T)0.0f; }
+    for(int h = 0; h < (int)sizeof(T) / 2; h++) { out.word[h] = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]); }
+    return out;
 }
 }
 
