@@ -14,55 +14,61 @@ using gennmi_lanes::partner;
 namespace
 {
 // ---- layer norm
-// A row lies in the registers of the lanes that share it: 16 or 64 of a wavefront, or a work-group, each with up to 16 elements of it, so that it is read once and its
-// statistics are those of its elements as they are: first the mean, then the squares of what is left.
+// A row lies in the registers of the lanes that share it: 16 or 64 of a wavefront, or several wavefronts, each with 8 or 16 elements of it, so that it is read once and its
+// statistics are those of its elements as they are: first the mean, then the squares of what is left.  Where wavefronts share a row, each finds both for its own part, and the parts are joined
+// (Chan, Golub, LeVeque: sum of squares = sum over parts of their own and of count (mean of the part - mean)^2): one barrier a row instead of two.
 struct NormArgs
 {
     gennmi_rows_t x, gate, out;
     const float *weight, *bias;
-    uint32_t rows, length, channels, rms;
+    uint32_t rows, length, channels, rms, lanes;        // lanes: of a row
     float epsilon, share;           // 1 / channels
     gennmi_rows_t dout, dx, dgate;
     float *sums;                    // of each work-group: weight's and bias's, [2][channels]
 };
 template<typename T> __device__ inline T *normRow(const gennmi_rows_t &r, uint32_t sequence, uint32_t row) { return (T*)r.data + (uint64_t)sequence * r.sequenceStride + (uint64_t)row * r.rowStride; }
 
-// Sums of N values over the lanes of a row.  `LANES` 0: over the work-group, through LDS; two of its places are used in turn, so that one barrier a sum does.
-template<int LANES, int N> __device__ inline void sumOfRow(float (&v)[N], float (*found)[2][16], uint32_t &turn)
+// Where a thread stands: `lane` of the `lanes` of the row of `group`, one of `groups` of the work-group
+struct NormPlace { uint32_t lanes, lane, group, groups; };
+template<int LANES> __device__ inline NormPlace normPlace(const NormArgs &a)
+{
+    constexpr uint32_t OWN = LANES ? LANES : 1;
+    if(LANES) { return NormPlace{OWN, threadIdx.x % OWN, threadIdx.x / OWN, 256u / OWN}; }
+    // (wavefronts have one row each)
+    const uint32_t group = __builtin_amdgcn_readfirstlane(threadIdx.x / a.lanes);
+    return NormPlace{a.lanes, threadIdx.x - group * a.lanes, group, blockDim.x / a.lanes};
+}
+template<int LANES> __device__ inline float sumOfLanes(float x)
+{
+    x += partner<1>(x); x += partner<2>(x); x += partner<4>(x); x += partner<8>(x);
+    if(LANES != 16) { x += partner<16>(x); x += partner<32>(x); }
+    return x;
+}
+// Two sums a row over its wavefronts; two places in LDS are used in turn, so that one barrier does
+struct NormShared { float2 found[2][16]; };
+
+template<typename T, int E, int VEC> struct NormRow { Pack<T, VEC> part[E / VEC]; };
+template<typename T, int E, int VEC> __device__ inline NormRow<T, E, VEC> requestRow(const T *row, const NormPlace &at, uint32_t channels, bool valid)
+{
+    NormRow<T, E, VEC> x;
+    #pragma unroll
+    for(int i = 0; i < E / VEC; i++) {
+        const uint32_t c = (i * at.lanes + at.lane) * VEC;
+        x.part[i] = Pack<T, VEC>{};
+        if(valid && c < channels) { x.part[i] = *(const Pack<T, VEC>*)(row + c); }
+    }
+    return x;
+}
+template<typename T, int E, int VEC> __device__ inline void takeRow(const NormRow<T, E, VEC> &from, float (&x)[E])
 {
     #pragma unroll
-    for(int n = 0; n < N; n++) {
-        v[n] += partner<1>(v[n]); v[n] += partner<2>(v[n]); v[n] += partner<4>(v[n]); v[n] += partner<8>(v[n]);
-        if(LANES != 16) { v[n] += partner<16>(v[n]); v[n] += partner<32>(v[n]); }
-    }
-    if constexpr(LANES == 0) {
-        const uint32_t wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-        if((threadIdx.x & 63) == 0) { for(int n = 0; n < N; n++) { found[turn][n][wave] = v[n]; } }
-        __syncthreads();
-        for(int n = 0; n < N; n++) {
-            float sum = 0.0f;
-            for(uint32_t w = 0; w < waves; w++) { sum += found[turn][n][w]; }
-            v[n] = sum;
-        }
-        turn ^= 1;
-    }
+    for(int e = 0; e < E; e++) { x[e] = widen(from.part[e / VEC].v[e % VEC]); }
 }
-template<typename T, int E, int VEC> __device__ inline void loadRow(const T *row, uint32_t lane, uint32_t lanes, uint32_t channels, float (&x)[E])
+template<typename T, int E, int VEC> __device__ inline void storeRow(T *row, const NormPlace &at, uint32_t channels, const float (&x)[E])
 {
     #pragma unroll
     for(int i = 0; i < E / VEC; i++) {
-        const uint32_t c = (i * lanes + lane) * VEC;
-        Pack<T, VEC> p{};
-        if(c < channels) { p = *(const Pack<T, VEC>*)(row + c); }
-        #pragma unroll
-        for(int e = 0; e < VEC; e++) { x[i * VEC + e] = widen(p.v[e]); }
-    }
-}
-template<typename T, int E, int VEC> __device__ inline void storeRow(T *row, uint32_t lane, uint32_t lanes, uint32_t channels, const float (&x)[E])
-{
-    #pragma unroll
-    for(int i = 0; i < E / VEC; i++) {
-        const uint32_t c = (i * lanes + lane) * VEC;
+        const uint32_t c = (i * at.lanes + at.lane) * VEC;
         if(c >= channels) { continue; }
         Pack<T, VEC> p;
         #pragma unroll
@@ -70,63 +76,117 @@ template<typename T, int E, int VEC> __device__ inline void storeRow(T *row, uin
         *(Pack<T, VEC>*)(row + c) = p;
     }
 }
-template<int E, int VEC> __device__ inline void loadParameters(const float *from, float without, uint32_t lane, uint32_t lanes, uint32_t channels, float (&x)[E])
+template<int E, int VEC> __device__ inline void loadParameters(const float *from, float without, const NormPlace &at, uint32_t channels, float (&x)[E])
 {
+    constexpr int EACH = VEC < 4 ? 1 : 4;
+    const bool wide = (uintptr_t)from % 16 == 0;
     #pragma unroll
-    for(int i = 0; i < E / VEC; i++) {
+    for(int i = 0; i < E; i += EACH) {
+        const uint32_t c = (i / VEC * at.lanes + at.lane) * VEC + i % VEC;
         #pragma unroll
-        for(int e = 0; e < VEC; e++) {
-            const uint32_t c = (i * lanes + lane) * VEC + e;
-            x[i * VEC + e] = c < channels ? from ? from[c] : without : 0.0f;
+        for(int e = 0; e < EACH; e++) { x[i + e] = c < channels ? without : 0.0f; }
+        if(!from || c >= channels) { continue; }
+        if(wide) {
+            const Pack<float, EACH> p = *(const Pack<float, EACH>*)(from + c);
+            #pragma unroll
+            for(int e = 0; e < EACH; e++) { x[i + e] = p.v[e]; }
+        }
+        else {
+            #pragma unroll
+            for(int e = 0; e < EACH; e++) { x[i + e] = from[c + e]; }
         }
     }
 }
-// x becomes x', its length before is returned as a factor
-template<int LANES, int E, int VEC> __device__ inline float normalise(const NormArgs &a, float (&x)[E], uint32_t lane, uint32_t lanes, float (*found)[2][16], uint32_t &turn)
+template<int E, int VEC> __device__ inline bool hasElement(const NormPlace &at, int e, uint32_t channels) { return (e / VEC * at.lanes + at.lane) * VEC + e % VEC < channels; }
+// Elements that a row's wavefront has
+template<int E, int VEC> __device__ inline float elementsOf(const NormPlace &at, uint32_t wave, uint32_t channels)
 {
-    if(!a.rms) {
-        float sum[1] = {0.0f};
-        #pragma unroll
-        for(int e = 0; e < E; e++) { sum[0] += x[e]; }
-        sumOfRow<LANES>(sum, found, turn);
-        const float mean = sum[0] * a.share;
-        #pragma unroll
-        for(int e = 0; e < E; e++) { x[e] = (uint32_t)(((e / VEC) * lanes + lane) * VEC + e % VEC) < a.channels ? x[e] - mean : 0.0f; }
+    uint32_t n = 0;
+    #pragma unroll
+    for(int i = 0; i < E / VEC; i++) {
+        const uint32_t first = (i * at.lanes + 64 * wave) * VEC;
+        n += first < channels ? min(channels - first, 64u * VEC) : 0;
     }
-    float square[1] = {0.0f};
+    return (float)n;
+}
+
+// x becomes x'; what it is divided by is returned as a factor
+template<int LANES, int E, int VEC> __device__ inline float normalise(const NormArgs &a, float (&x)[E], const NormPlace &at, NormShared &shared, uint32_t &turn, float inWave, float inWaveShare)
+{
+    float sum = 0.0f, square = 0.0f, mean = 0.0f;
+    if(!a.rms) {
+        #pragma unroll
+        for(int e = 0; e < E; e++) { sum += x[e]; }
+        sum = sumOfLanes<LANES>(sum);
+        mean = sum * (LANES ? a.share : inWaveShare);
+    }
     #pragma unroll
-    for(int e = 0; e < E; e++) { square[0] = __builtin_fmaf(x[e], x[e], square[0]); }
-    sumOfRow<LANES>(square, found, turn);
-    const float r = 1.0f / sqrtf(__builtin_fmaf(square[0], a.share, a.epsilon));
+    for(int e = 0; e < E; e++) {
+        const float d = hasElement<E, VEC>(at, e, a.channels) ? x[e] - mean : 0.0f;
+        square = __builtin_fmaf(d, d, square);
+    }
+    square = sumOfLanes<LANES>(square);
+    if constexpr(LANES == 0) {
+        const uint32_t waves = at.lanes >> 6, first = at.group * waves, mine = threadIdx.x >> 6;
+        if((threadIdx.x & 63) == 0) { shared.found[turn][mine] = make_float2(sum, square); }
+        __syncthreads();
+        sum = square = 0.0f;
+        for(uint32_t w = 0; w < waves; w++) { const float2 f = shared.found[turn][first + w]; sum += f.x; square += f.y; }
+        if(!a.rms) {
+            mean = sum * a.share;
+            for(uint32_t w = 0; w < waves; w++) {
+                const float n = elementsOf<E, VEC>(at, w, a.channels), off = n > 0.0f ? shared.found[turn][first + w].x / n - mean : 0.0f;
+                square = __builtin_fmaf(n * off, off, square);
+            }
+        }
+        turn ^= 1;
+    }
+    const float r = 1.0f / sqrtf(__builtin_fmaf(square, a.share, a.epsilon));
     #pragma unroll
-    for(int e = 0; e < E; e++) { x[e] *= r; }
+    for(int e = 0; e < E; e++) { x[e] = hasElement<E, VEC>(at, e, a.channels) ? (x[e] - mean) * r : 0.0f; }
     return r;
 }
 __device__ inline float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
 
-// Work-groups of 256 threads where 16 lanes or a wavefront have a row, else of as many as a row takes; each walks rows that are a grid apart, with the parameters in registers.
+// Work-groups of 256 threads where 16 lanes or a wavefront have a row, else of 512 or what one row takes; each walks rows that are a grid apart, with the parameters in registers
+// and the next row asked for while one is worked on.  (4096 x 4096 in bf16: 63 us with a row a work-group, whose parameters are four times the row.)
 template<typename T, int LANES, int E, int VEC>
 __global__ __launch_bounds__(LANES ? 256 : 1024)
 void normKernel(NormArgs a)
 {
-    __shared__ float found[2][2][16];
+    __shared__ NormShared shared;
     uint32_t turn = 0;
-    const uint32_t lanes = LANES ? LANES : blockDim.x, lane = threadIdx.x % lanes, each = LANES ? 256 / LANES : 1;
+    const NormPlace at = normPlace<LANES>(a);
     float weight[E], bias[E];
-    loadParameters<E, VEC>(a.weight, 1.0f, lane, lanes, a.channels, weight);
-    loadParameters<E, VEC>(a.bias, 0.0f, lane, lanes, a.channels, bias);
-    for(uint64_t n = (uint64_t)blockIdx.x * each + threadIdx.x / lanes; n < a.rows; n += (uint64_t)gridDim.x * each) {
-        const uint32_t sequence = (uint32_t)n / a.length, row = (uint32_t)n - sequence * a.length;
+    loadParameters<E, VEC>(a.weight, 1.0f, at, a.channels, weight);
+    loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias);
+    const float inWave = LANES ? 0.0f : elementsOf<E, VEC>(at, at.lane >> 6, a.channels), inWaveShare = inWave > 0.0f ? 1.0f / inWave : 0.0f;
+    const uint64_t step = (uint64_t)gridDim.x * at.groups;
+    NormRow<T, E, VEC> nextX, nextZ{};
+    const auto request = [&](uint64_t n) {
+        const bool valid = n < a.rows;
+        const uint32_t sequence = valid ? (uint32_t)n / a.length : 0, row = valid ? (uint32_t)n - sequence * a.length : 0;
+        nextX = requestRow<T, E, VEC>(normRow<const T>(a.x, sequence, row), at, a.channels, valid);
+        if(a.gate.data) { nextZ = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
+    };
+    uint64_t first = (uint64_t)blockIdx.x * at.groups;
+    request(first + at.group);
+    for(; first < a.rows; first += step) {
+        const uint64_t n = first + at.group;
         float x[E], z[E];
-        loadRow<T, E, VEC>(normRow<const T>(a.x, sequence, row), lane, lanes, a.channels, x);
-        if(a.gate.data) { loadRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), lane, lanes, a.channels, z); }
-        normalise<LANES, E, VEC>(a, x, lane, lanes, found, turn);
+        takeRow(nextX, x);
+        if(a.gate.data) { takeRow(nextZ, z); }
+        request(n + step);
+        normalise<LANES, E, VEC>(a, x, at, shared, turn, inWave, inWaveShare);
         #pragma unroll
         for(int e = 0; e < E; e++) {
             x[e] = __builtin_fmaf(x[e], weight[e], bias[e]);
             if(a.gate.data) { x[e] *= z[e] * logistic(z[e]); }
         }
-        storeRow<T, E, VEC>(normRow<T>(a.out, sequence, row), lane, lanes, a.channels, x);
+        if(n < a.rows) {
+            const uint32_t sequence = (uint32_t)n / a.length, row = (uint32_t)n - sequence * a.length;
+            storeRow<T, E, VEC>(normRow<T>(a.out, sequence, row), at, a.channels, x);
+        }
     }
 }
 
@@ -136,66 +196,90 @@ template<typename T, int LANES, int E, int VEC>
 __global__ __launch_bounds__(LANES ? 256 : 1024)
 void normBackwardKernel(NormArgs a)
 {
-    __shared__ float found[2][2][16];
-    __shared__ float shared[LANES ? 256 * E : 1];
+    __shared__ NormShared shared;
+    extern __shared__ float rows[];
     uint32_t turn = 0;
-    const uint32_t lanes = LANES ? LANES : blockDim.x, lane = threadIdx.x % lanes, each = LANES ? 256 / LANES : 1;
+    const NormPlace at = normPlace<LANES>(a);
     float weight[E], bias[E], dweight[E] = {}, dbias[E] = {};
-    loadParameters<E, VEC>(a.weight, 1.0f, lane, lanes, a.channels, weight);
-    loadParameters<E, VEC>(a.bias, 0.0f, lane, lanes, a.channels, bias);
-    for(uint64_t n = (uint64_t)blockIdx.x * each + threadIdx.x / lanes; n < a.rows; n += (uint64_t)gridDim.x * each) {
-        const uint32_t sequence = (uint32_t)n / a.length, row = (uint32_t)n - sequence * a.length;
+    loadParameters<E, VEC>(a.weight, 1.0f, at, a.channels, weight);
+    loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias);
+    const float inWave = LANES ? 0.0f : elementsOf<E, VEC>(at, at.lane >> 6, a.channels), inWaveShare = inWave > 0.0f ? 1.0f / inWave : 0.0f;
+    const uint64_t step = (uint64_t)gridDim.x * at.groups;
+    NormRow<T, E, VEC> nextX, nextD;
+    const auto request = [&](uint64_t n) {
+        const bool valid = n < a.rows;
+        const uint32_t sequence = valid ? (uint32_t)n / a.length : 0, row = valid ? (uint32_t)n - sequence * a.length : 0;
+        nextX = requestRow<T, E, VEC>(normRow<const T>(a.x, sequence, row), at, a.channels, valid);
+        nextD = requestRow<T, E, VEC>(normRow<const T>(a.dout, sequence, row), at, a.channels, valid);
+    };
+    uint64_t first = (uint64_t)blockIdx.x * at.groups;
+    request(first + at.group);
+    for(; first < a.rows; first += step) {
+        const uint64_t n = first + at.group;
+        const bool valid = n < a.rows;
+        const uint32_t sequence = valid ? (uint32_t)n / a.length : 0, row = valid ? (uint32_t)n - sequence * a.length : 0;
         float x[E], d[E];
-        loadRow<T, E, VEC>(normRow<const T>(a.x, sequence, row), lane, lanes, a.channels, x);
-        loadRow<T, E, VEC>(normRow<const T>(a.dout, sequence, row), lane, lanes, a.channels, d);
-        const float r = normalise<LANES, E, VEC>(a, x, lane, lanes, found, turn);
+        takeRow(nextX, x);
+        takeRow(nextD, d);
+        NormRow<T, E, VEC> gate{};
+        if(a.gate.data) { gate = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
+        request(n + step);
+        const float r = normalise<LANES, E, VEC>(a, x, at, shared, turn, inWave, inWaveShare);
         if(a.gate.data) {
             float z[E];
-            loadRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), lane, lanes, a.channels, z);
+            takeRow(gate, z);
             #pragma unroll
             for(int e = 0; e < E; e++) {
                 const float s = logistic(z[e]), y = __builtin_fmaf(x[e], weight[e], bias[e]), dz = d[e] * y * (s * __builtin_fmaf(z[e], 1.0f - s, 1.0f));
                 d[e] *= z[e] * s;
                 z[e] = dz;
             }
-            if(a.dgate.data) { storeRow<T, E, VEC>(normRow<T>(a.dgate, sequence, row), lane, lanes, a.channels, z); }
+            if(a.dgate.data && valid) { storeRow<T, E, VEC>(normRow<T>(a.dgate, sequence, row), at, a.channels, z); }
         }
-        float means[2] = {0.0f, 0.0f};
+        // (of a row that is not there d is zero)
+        float along = 0.0f, mean = 0.0f;
         #pragma unroll
         for(int e = 0; e < E; e++) {
-            dweight[e] = __builtin_fmaf(d[e], x[e], dweight[e]);
+            if(valid) { dweight[e] = __builtin_fmaf(d[e], x[e], dweight[e]); }
             dbias[e] += d[e];
             d[e] *= weight[e];
-            means[0] = __builtin_fmaf(d[e], x[e], means[0]);
-            means[1] += d[e];
+            along = __builtin_fmaf(d[e], x[e], along);
+            mean += d[e];
         }
         if(!a.dx.data) { continue; }
-        sumOfRow<LANES>(means, found, turn);
-        const float along = means[0] * a.share, mean = a.rms ? 0.0f : means[1] * a.share;
+        along = sumOfLanes<LANES>(along);
+        mean = sumOfLanes<LANES>(mean);
+        if constexpr(LANES == 0) {
+            const uint32_t waves = at.lanes >> 6;
+            if((threadIdx.x & 63) == 0) { shared.found[turn][threadIdx.x >> 6] = make_float2(along, mean); }
+            __syncthreads();
+            along = mean = 0.0f;
+            for(uint32_t w = 0; w < waves; w++) { const float2 f = shared.found[turn][at.group * waves + w]; along += f.x; mean += f.y; }
+            turn ^= 1;
+        }
+        along *= a.share;
+        mean = a.rms ? 0.0f : mean * a.share;
         #pragma unroll
         for(int e = 0; e < E; e++) { x[e] = r * (__builtin_fmaf(-x[e], along, d[e]) - mean); }
-        storeRow<T, E, VEC>(normRow<T>(a.dx, sequence, row), lane, lanes, a.channels, x);
+        if(valid) { storeRow<T, E, VEC>(normRow<T>(a.dx, sequence, row), at, a.channels, x); }
     }
     if(!a.sums) { return; }
     float *const to = a.sums + (uint64_t)blockIdx.x * 2 * a.channels;
     #pragma unroll
     for(int which = 0; which < 2; which++) {
         float (&sum)[E] = which ? dbias : dweight;
-        if constexpr(LANES != 0) {
+        if(at.groups > 1) {
             // (the rows of a work-group one after another)
             __syncthreads();
             #pragma unroll
-            for(int e = 0; e < E; e++) { shared[e * 256 + threadIdx.x] = sum[e]; }
+            for(int e = 0; e < E; e++) { rows[e * blockDim.x + threadIdx.x] = sum[e]; }
             __syncthreads();
-            if(threadIdx.x >= LANES) { continue; }
+            if(at.group) { continue; }
             #pragma unroll
-            for(int e = 0; e < E; e++) { for(uint32_t k = 1; k < each; k++) { sum[e] += shared[e * 256 + k * LANES + lane]; } }
+            for(int e = 0; e < E; e++) { for(uint32_t k = 1; k < at.groups; k++) { sum[e] += rows[e * blockDim.x + k * at.lanes + at.lane]; } }
         }
         #pragma unroll
-        for(int e = 0; e < E; e++) {
-            const uint32_t c = ((e / VEC) * lanes + lane) * VEC + e % VEC;
-            if(c < a.channels) { to[which * a.channels + c] = sum[e]; }
-        }
+        for(int e = 0; e < E; e++) { if(hasElement<E, VEC>(at, e, a.channels)) { to[which * a.channels + (e / VEC * at.lanes + at.lane) * VEC + e % VEC] = sum[e]; } }
     }
 }
 
@@ -285,23 +369,28 @@ uint32_t vectorOf(uint32_t size, uint32_t channels, std::initializer_list<const 
     for(const gennmi_rows_t *r : arrays) { whole = whole && (!r->data || ((uintptr_t)r->data % 16 == 0 && r->rowStride % vector == 0 && r->sequenceStride % vector == 0)); }
     return whole ? vector : 1;
 }
-struct NormPlan { uint32_t lanes, threads, blocks; };       // lanes 0: a work-group a row
+struct NormPlan { uint32_t lanes, rowLanes, groups, threads, blocks; };       // lanes 0: wavefronts share a row, rowLanes of them
 NormPlan normPlan(const gennmi_layer_norm_t &c, bool gradients)
 {
     const uint64_t rows = totalRows(c.sequences);
     NormPlan p;
-    p.lanes = c.channels <= 128 ? 16 : c.channels <= 1024 ? 64 : 0;
-    p.threads = p.lanes ? 256 : ((c.channels + 15) / 16 + 63) / 64 * 64;
-    const uint64_t each = p.lanes ? 256 / p.lanes : 1, most = gradients ? 1024 : 4096;
-    p.blocks = (uint32_t)std::min<uint64_t>((rows + each - 1) / each, most);
+    p.lanes = c.channels <= 128 ? 16 : c.channels <= 512 ? 64 : 0;
+    const uint32_t each = c.channels <= 8192 ? 8 : 16;
+    p.rowLanes = p.lanes ? p.lanes : ((c.channels + each - 1) / each + 63) / 64 * 64;
+    p.groups = p.lanes ? 256 / p.lanes : std::max(1u, 512 / p.rowLanes);
+    p.threads = p.groups * p.rowLanes;
+    // Work-groups: for gradients fewer, with four rows at least, as each leaves a sum for every channel
+    const uint64_t needed = (rows + p.groups - 1) / p.groups;
+    p.blocks = (uint32_t)std::min<uint64_t>(gradients ? (needed + 3) / 4 : needed, gradients ? 1024 : 2048);
     return p;
 }
 template<typename T, int VEC, typename F> int withNormLayout(const NormPlan &p, uint32_t channels, F &&f)
 {
     typedef std::integral_constant<int, VEC> Vec;
-    if(p.lanes == 16) { return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{}, Vec{}); }
-    if(p.lanes == 64 && channels <= 512) { return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{}, Vec{}); }
-    if(p.lanes == 64) { return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{}, Vec{}); }
+    typedef std::integral_constant<int, 8> Eight;
+    if(p.lanes == 16) { return f(std::integral_constant<int, 16>{}, Eight{}, Vec{}); }
+    if(p.lanes == 64) { return f(std::integral_constant<int, 64>{}, Eight{}, Vec{}); }
+    if(channels <= 8192) { return f(std::integral_constant<int, 0>{}, Eight{}, Vec{}); }
     return f(std::integral_constant<int, 0>{}, std::integral_constant<int, 16>{}, Vec{});
 }
 template<typename F> int withNorm(const gennmi_layer_norm_t &c, const NormPlan &p, uint32_t vector, F &&f)
@@ -313,14 +402,14 @@ template<typename F> int withNorm(const gennmi_layer_norm_t &c, const NormPlan &
         return withNormLayout<T, 1>(p, c.channels, g);
     });
 }
-NormArgs normArgs(const gennmi_layer_norm_t &c, bool flat)
+NormArgs normArgs(const gennmi_layer_norm_t &c, const NormPlan &p, bool flat)
 {
     NormArgs a{};
     a.x = c.x; a.gate = c.gate; a.out = c.out;
     a.weight = c.weight; a.bias = c.bias;
     a.rows = (uint32_t)totalRows(c.sequences);
     a.length = flat ? a.rows : c.sequences.length;
-    a.channels = c.channels; a.rms = c.rms;
+    a.channels = c.channels; a.rms = c.rms; a.lanes = p.rowLanes;
     a.epsilon = c.epsilon; a.share = 1.0f / (float)c.channels;
     return a;
 }
@@ -343,7 +432,7 @@ int gennmi_layer_norm(const gennmi_layer_norm_t *norm, void *stream)
         if(!totalRows(s)) { return (int)GENNMI_OK; }
         const NormPlan p = normPlan(*norm, false);
         const auto arrays = {&norm->x, &norm->gate, &norm->out};
-        const NormArgs a = normArgs(*norm, oneBehindAnother(s, arrays));
+        const NormArgs a = normArgs(*norm, p, oneBehindAnother(s, arrays));
         const int rc = withNorm(*norm, p, vectorOf(size, norm->channels, arrays), [&](auto t, auto lanes, auto each, auto vec) {
             normKernel<decltype(t), decltype(lanes)::value, decltype(each)::value, decltype(vec)::value><<<dim3(p.blocks), dim3(p.threads), 0, (hipStream_t)stream>>>(a);
             return gennmi_detail::afterLaunch(what);
@@ -389,12 +478,12 @@ int gennmi_layer_norm_backward(const gennmi_layer_norm_t *norm, const gennmi_lay
                                       regionOf("weight", norm->weight, bytes), regionOf("bias", norm->bias, bytes)})) { return rc; }
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, s.device)) { return rc; }
         const auto arrays = {&norm->x, &norm->gate, &g.out, &g.x, &g.gate};
-        NormArgs a = normArgs(*norm, oneBehindAnother(s, arrays));
+        NormArgs a = normArgs(*norm, p, oneBehindAnother(s, arrays));
         a.dout = g.out; a.dx = g.x; a.dgate = g.gate;
         a.sums = sums ? (float*)workspace : nullptr;
         if(a.rows) {
             const int rc = withNorm(*norm, p, vectorOf(size, channels, arrays), [&](auto t, auto lanes, auto each, auto vec) {
-                normBackwardKernel<decltype(t), decltype(lanes)::value, decltype(each)::value, decltype(vec)::value><<<dim3(p.blocks), dim3(p.threads), 0, (hipStream_t)stream>>>(a);
+                normBackwardKernel<decltype(t), decltype(lanes)::value, decltype(each)::value, decltype(vec)::value><<<dim3(p.blocks), dim3(p.threads), sums && p.groups > 1 ? p.threads * decltype(each)::value * sizeof(float) : 0, (hipStream_t)stream>>>(a);
                 return gennmi_detail::afterLaunch(what);
             });
             if(rc) { return rc; }
