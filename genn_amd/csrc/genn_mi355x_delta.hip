@@ -89,7 +89,7 @@ uint32_t segmentRows(const gennmi_delta_rule_t &c, bool gradients)
 }
 bool isCut(const gennmi_delta_rule_t &c, bool gradients) { return c.sequences.length > segmentRows(c, gradients); }
 uint32_t moveBlocks(const gennmi_delta_rule_t &c, uint32_t columns) { const uint32_t each = 16 * wavesFor(columns); return (paddedKeys(c.keys) + each - 1) / each; }
-struct DeltaSpace { size_t correction, score, rows, table, segmentStates, segmentMoves, states, errors, gradientStates, gradientErrors, bytes; };
+struct DeltaSpace { size_t correction, score, rows, table, segmentStates, segmentMoves, states, errors, gradientStates, gradientErrors, shared, bytes; };
 DeltaSpace deltaSpace(const gennmi_delta_rule_t &c, bool gradients)
 {
     DeltaSpace s{};
@@ -110,6 +110,7 @@ DeltaSpace deltaSpace(const gennmi_delta_rule_t &c, bool gradients)
         s.errors = take(numbers * C * padded * 4);
         s.gradientStates = take(numbers * paddedKeys(c.keys) * padded * 4);
         s.gradientErrors = take(numbers * C * padded * 4);
+        if(c.heads > c.keyHeads) { s.shared = take(numbers * 2 * C * paddedKeys(c.keys) * 4); }
     }
     return s;
 }
@@ -119,7 +120,7 @@ bool deltaFits(const gennmi_delta_rule_t &c, bool gradients)
 {
     if(!gradients && c.sequences.length <= 1) { return tokenBlocks(c) <= mostBlocks(256); }
     const uint32_t columns = gradients ? paddedValues(c.values) : c.values;
-    return chunkNumbers(c.sequences, chunkRows(c.type)) * c.keyHeads <= mostBlocks(512) &&
+    return chunkNumbers(c.sequences, chunkRows(c.type)) * c.heads <= mostBlocks(512) &&
         chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.heads * (blocksOf(columns) + moveBlocks(c, columns)) <= mostBlocks(64 * wavesFor(columns)) &&
         (uint64_t)c.sequences.count * c.heads * (paddedValues(c.values) / 16) <= mostBlocks(64);
 }
@@ -205,7 +206,10 @@ template<typename T, int C, int DK> int launchGradients(const char *what, const 
     const auto kernel = deltaGradientKernel<T, C, DK>;
     constexpr size_t lds = GradientLayout<T, C, DK>::bytes;
     if(const int rcLds = withLds(what, kernel, lds)) { return rcLds; }
-    kernel<<<dim3((uint32_t)(numbers * a.keyHeads)), dim3(512), lds, stream>>>(a, d);
+    kernel<<<dim3((uint32_t)(numbers * a.heads)), dim3(512), lds, stream>>>(a, d);
+    if(const int rcGradient = gennmi_detail::afterLaunch(what)) { return rcGradient; }
+    if(a.group == 1 || !(d.q.data || d.k.data)) { return GENNMI_OK; }
+    deltaSharedKernel<T, C, DK><<<dim3((uint32_t)(numbers * a.keyHeads)), dim3(256), 0, stream>>>(a, d);
     return gennmi_detail::afterLaunch(what);
 }
 template<typename T, int VEC> int launchToken(const char *what, const DeltaArgs &a, uint32_t blocks, hipStream_t stream)
@@ -307,12 +311,15 @@ int gennmi_delta_rule_backward(const gennmi_delta_rule_t *rule, const gennmi_del
         if(const int rc = deltaApart(what, *rule, in, workspace, space.bytes)) { return rc; }
         if(const int rc = gennmi_detail::beforeLaunch((hipStream_t)stream, rule->sequences.device)) { return rc; }
         if(!rule->sequences.count) { return (int)GENNMI_OK; }
-        const DeltaArgs a = deltaArgs(*rule, space, workspace, true);
+        DeltaArgs a = deltaArgs(*rule, space, workspace, true);
+        const auto fours = [&](const gennmi_rows_t &r) { return (uintptr_t)r.data % (4 * size) == 0 && r.rowStride % 4 == 0 && r.sequenceStride % 4 == 0; };
+        a.wideValues = rule->values % 4 == 0 && fours(rule->v) && fours(in.out);
         DeltaGradientArgs d{};
         d.out = in.out; d.q = in.q; d.k = in.k; d.v = in.v; d.g = in.g; d.beta = in.beta;
         d.finalState = in.finalState; d.initialState = in.initialState;
         d.states = (float*)((char*)workspace + space.gradientStates);
         d.errors = (float*)((char*)workspace + space.gradientErrors);
+        d.shared = (float*)((char*)workspace + space.shared);
         const int rc = withSizes(*rule, [&](auto t, auto rows, auto keysRoom) {
             typedef decltype(t) T;
             constexpr int C = decltype(rows)::value, DK = decltype(keysRoom)::value;

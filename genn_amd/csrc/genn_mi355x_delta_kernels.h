@@ -54,7 +54,7 @@ struct DeltaArgs
     gennmi_rows_t q, k, v, out, g, beta;
     const float *initialState;
     float *finalState;
-    uint32_t heads, keyHeads, group, keys, values, normalise, wide, columnBlocks;
+    uint32_t heads, keyHeads, group, keys, values, normalise, wide, wideValues, columnBlocks;
     uint32_t padded;                // values, up to a multiple of 32: the width of what is kept of them
     float scale, epsilon;
     float *correction, *score;      // of each chunk number and head: -N and P, [C][C]
@@ -431,6 +431,16 @@ template<typename T, int C> __device__ inline void storeResult(T *rows, uint64_t
     }
 }
 
+// Some tiles of a result, every SPLIT-th from `first` on, all rows and columns
+template<int TILES, int SPLIT> __device__ inline void storeResultTiles(float *rows, uint32_t stride, uint32_t first, uint32_t g, uint32_t column, const f32x4 (&x)[TILES])
+{
+    #pragma unroll
+    for(int t = 0; t < TILES; t++) {
+        #pragma unroll
+        for(int r = 0; r < 4; r++) { rows[((first + SPLIT * t) * 16 + 4 * g + r) * stride + column] = x[t][r]; }
+    }
+}
+
 // A work-group walks a sequence (or a segment of it) of one head with 16 columns of the state a wavefront.
 template<typename T, int C, int DK, int WAVES, int MODE, bool FOLDED>
 __global__ __launch_bounds__(64 * WAVES)
@@ -670,6 +680,7 @@ struct DeltaGradientArgs
     const float *finalState;
     float *initialState;
     float *states, *errors;         // the gradient of the state behind each chunk [DK][padded], dR [C][padded]
+    float *shared;                  // where heads share keys: each one's gradients of unit queries and keys, [2][C][DK]
 };
 template<typename T, int C, int DK> struct ReverseLayout
 {
@@ -850,13 +861,14 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
 //   dbeta[i] = w[i].dR[i]
 // and g's: with states and u in units of the decay so far, outputs grow with it and values shrink, so that what the sum of g up to row i gains the loss
 // is q^[i].dq^[i] - v[i].dv[i], and at the chunk's last row the state behind it times its gradient as well.
-// A work-group has a chunk and a key head and adds up the heads that share it.  Products are summed over the values, 32 at a time, with what multiplies S and dS
-// in LDS; a wavefront has 16 keys' columns of the results, S' and dS' straight from memory.
+// A work-group has a chunk and a head.  Products are summed over the values, 32 at a time, with what multiplies S and dS
+// in LDS (the next 32 on their way meanwhile); a wavefront has 16 keys' columns of the results, S' and dS' straight from memory.  Where heads share keys, what each finds for them is left for
+// deltaSharedKernel to add up.
 template<typename T, int C, int DK> struct GradientLayout
 {
     static constexpr int NP = planesOf<T>, COLUMN = C + 8, VALUES = 40;
     static constexpr uint32_t keyColumns = 0, queryColumns = keyColumns + NP * DK * COLUMN, stage = queryColumns + NP * DK * COLUMN,
-        staged = (NP + 6) * C * VALUES, square = 3 * C * COLUMN, floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (6 + 2 * 8 + 1) + 64;
+        staged = (NP + 6) * C * VALUES, square = 3 * C * COLUMN, floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (6 + 2 * 8) + 64;
 };
 
 template<typename T, int C, int DK>
@@ -871,8 +883,9 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     double *const sums = (double*)(planes + L::floats);
     float *const since = (float*)(sums + C), *const until = since + C, *const beta = until + C, *const keyUnit = beta + C, *const queryUnit = keyUnit + C, *const valueDots = queryUnit + C;
     float *const queryDots = valueDots + C, *const keyDots = queryDots + 8 * C, *const ends = keyDots + 8 * C;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
-    const uint32_t number = blockIdx.x / a.keyHeads, keyHead = blockIdx.x - number * a.keyHeads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
+    const uint32_t number = blockIdx.x / a.heads, head = blockIdx.x - number * a.heads, keyHead = head / a.group;
+    const uint64_t at = (uint64_t)number * a.heads + head;
     Place p;
     if(!locate(a.chunks, number, p)) { return; }
     const uint32_t begin = p.index * C, count = min((uint32_t)C, p.length - min(p.length, begin));
@@ -885,23 +898,68 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     const uint32_t squareColumn = C == 64 ? wave & 3 : wave & 1;
     const bool squares = C == 64 || wave < 4;
 
+    // what multiplies S and dS: eight threads a row, four values each
+    const bool stages = tid < C * 8;
+    const uint32_t stageRow = stages ? tid / 8 : 0, stageAt = tid % 8 * 4;
+    const bool staged = stages && stageRow < count;
+    const float *const stateRow = a.states + at * DK * a.padded + (uint64_t)key * a.padded + 8 * g, *const dStateRow = d.states + at * DK * a.padded + (uint64_t)key * a.padded + 8 * g;
+    const uint64_t usedRow = begin + (staged ? stageRow : 0);
+    const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + usedRow * d.out.rowStride + head * a.values, *const values = rowsOf<const T>(a.v, a.chunks, p) + usedRow * a.v.rowStride + head * a.values;
+    const float *const dRRow = d.errors + (at * C + stageRow) * a.padded, *const wRow = a.errors + (at * C + stageRow) * a.padded;
+    typedef Pack<T, 4> Four;
+    float4 nextState[2], nextDState[2], nextDR, nextW;
+    Four nextDout, nextValues;
+    const auto four = [&](const T *from, uint32_t v) {
+        Four x{};
+        if(a.wideValues) { if(v < a.values) { x = *(const Four*)(from + v); } }
+        else {
+            #pragma unroll
+            for(int e = 0; e < 4; e++) { if(v + e < a.values) { x.v[e] = from[v + e]; } }
+        }
+        return x;
+    };
+    const auto request = [&](uint32_t v) {
+        #pragma unroll
+        for(int h = 0; h < 2; h++) { nextState[h] = *(const float4*)(stateRow + v + 4 * h); nextDState[h] = *(const float4*)(dStateRow + v + 4 * h); }
+        nextDR = nextW = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        nextDout = nextValues = Four{};
+        if(staged) {
+            nextDR = *(const float4*)(dRRow + v + stageAt);
+            nextW = *(const float4*)(wRow + v + stageAt);
+            nextDout = four(douts, v + stageAt);
+            nextValues = four(values, v + stageAt);
+        }
+    };
+    request(0);
+
     #pragma unroll
     for(int i = 0; i < (2 * KEYS + 511) / 512; i++) {
         const uint32_t item = tid + i * 512;
         if(2 * KEYS % 512 && item >= 2 * KEYS) { break; }
         KeyTile<T> tile;
         const bool isKey = item < KEYS;
-        loadTile<T, C, DK>(a, isKey ? a.k : a.q, p, keyHead, begin, count, isKey ? item : item - KEYS, tile);
+        const uint32_t it = isKey ? item : item - KEYS, row = it / (DK / 8) * 4, column = it % (DK / 8) * 8;
+        loadTile<T, C, DK>(a, isKey ? a.k : a.q, p, keyHead, begin, count, it, tile);
         // (rows in their order here)
-        const uint32_t it = isKey ? item : item - KEYS, row = it / (DK / 8) * 4, at = it % (DK / 8) * 8;
         uint16_t *const to = planes + (isKey ? L::keyColumns : L::queryColumns);
         #pragma unroll
         for(int e = 0; e < 8; e++) {
             uint2 words[NP];
             columnOf<T>(tile, e, words);
             #pragma unroll
-            for(int k = 0; k < NP; k++) { *(uint2*)(to + k * DK * L::COLUMN + (at + e) * L::COLUMN + row) = words[k]; }
+            for(int k = 0; k < NP; k++) { *(uint2*)(to + k * DK * L::COLUMN + (column + e) * L::COLUMN + row) = words[k]; }
         }
+    }
+    const float decay = a.table[at].decay;
+    if(tid < C) {
+        const RowTable<C> &rows = ((const RowTable<C>*)a.rows)[at];
+        const double sum = rows.sum[tid], last = rows.sum[C - 1];
+        sums[tid] = sum;
+        since[tid] = decayOver(sum);
+        until[tid] = decayOver(last - sum);
+        beta[tid] = rows.beta[tid];
+        keyUnit[tid] = rows.keyUnit[tid];
+        queryUnit[tid] = rows.queryUnit[tid];
     }
     // the key's (or query's) values at this lane's column, four rows of a tile
     const auto valuesAt = [&](uint32_t from, uint32_t tile) {
@@ -914,176 +972,149 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         }
         return x;
     };
+    const auto fourRows = [&](const float *from, uint32_t tile) { const float4 x = *(const float4*)(from + tile * 16 + 4 * g); return f32x4{x.x, x.y, x.z, x.w}; };
     const auto sumOf16 = [](float x) { x += partner<1>(x); x += partner<2>(x); x += partner<4>(x); return x + partner<8>(x); };
 
-    f32x4 dq[MINE], dk[MINE], dqk[SQUARES], dkk[SQUARES];
+    f32x4 dq[MINE], rS[MINE], dk[MINE], dqk[SQUARES], dkk[SQUARES];
     #pragma unroll
-    for(int m = 0; m < MINE; m++) { dq[m] = dk[m] = f32x4{0, 0, 0, 0}; }
+    for(int m = 0; m < MINE; m++) { dq[m] = rS[m] = dk[m] = f32x4{0, 0, 0, 0}; }
     #pragma unroll
     for(int q = 0; q < SQUARES; q++) { dqk[q] = dkk[q] = f32x4{0, 0, 0, 0}; }
-    const bool stages = tid < C * 8;
-    const uint32_t stageRow = tid / 8, stageAt = tid % 8 * 4;
-
-    for(uint32_t inGroup = 0; inGroup < a.group; inGroup++) {
-        const uint32_t head = keyHead * a.group + inGroup;
-        const uint64_t at = (uint64_t)number * a.heads + head;
+    float stateDot = 0.0f, valueDot = 0.0f, betaDot = 0.0f;
+    for(uint32_t v = 0; v < a.padded; v += 32) {
+        const f32x4 s0a = {nextState[0].x, nextState[0].y, nextState[0].z, nextState[0].w}, s0b = {nextState[1].x, nextState[1].y, nextState[1].z, nextState[1].w};
+        const f32x4 dsa = {nextDState[0].x, nextDState[0].y, nextDState[0].z, nextDState[0].w}, dsb = {nextDState[1].x, nextDState[1].y, nextDState[1].z, nextDState[1].w};
         __syncthreads();
-        const float decay = a.table[at].decay;
-        if(tid < C) {
-            const RowTable<C> &rows = ((const RowTable<C>*)a.rows)[at];
-            const double sum = rows.sum[tid], last = rows.sum[C - 1];
-            sums[tid] = sum;
-            since[tid] = decayOver(sum);
-            until[tid] = decayOver(last - sum);
-            beta[tid] = rows.beta[tid];
-            keyUnit[tid] = rows.keyUnit[tid];
-            queryUnit[tid] = rows.queryUnit[tid];
+        if(stages) {
+            const float dr[4] = {nextDR.x, nextDR.y, nextDR.z, nextDR.w}, w[4] = {nextW.x, nextW.y, nextW.z, nextW.w};
+            float dout[4];
+            #pragma unroll
+            for(int e = 0; e < 4; e++) {
+                dout[e] = widen(nextDout.v[e]);
+                valueDot = __builtin_fmaf(widen(nextValues.v[e]), dr[e], valueDot);
+                betaDot = __builtin_fmaf(w[e], dr[e], betaDot);
+            }
+            uint2 words[3], own[NP];
+            uint16_t *const to = stage + stageRow * L::VALUES + stageAt;
+            splitFour<NP>(dout, own);
+            #pragma unroll
+            for(int k = 0; k < NP; k++) { *(uint2*)(to + k * VP) = own[k]; }
+            splitFour<3>(dr, words);
+            #pragma unroll
+            for(int k = 0; k < 3; k++) { *(uint2*)(to + (NP + k) * VP) = words[k]; }
+            splitFour<3>(w, words);
+            #pragma unroll
+            for(int k = 0; k < 3; k++) { *(uint2*)(to + (NP + 3 + k) * VP) = words[k]; }
         }
-        f32x4 outS[MINE], rS[MINE], wD[MINE], outW[SQUARES], rW[SQUARES];
+        __syncthreads();
+        if(v + 32 < a.padded) { request(v + 32); }
         #pragma unroll
-        for(int m = 0; m < MINE; m++) { outS[m] = rS[m] = wD[m] = f32x4{0, 0, 0, 0}; }
-        #pragma unroll
-        for(int q = 0; q < SQUARES; q++) { outW[q] = rW[q] = f32x4{0, 0, 0, 0}; }
-        float stateDot = 0.0f, valueDot = 0.0f, betaDot = 0.0f;
-        const float *const stateRow = a.states + at * DK * a.padded + (uint64_t)key * a.padded + 8 * g, *const dStateRow = d.states + at * DK * a.padded + (uint64_t)key * a.padded + 8 * g;
-        const uint32_t stageRowUsed = stages && stageRow < count ? stageRow : 0;
-        const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)(begin + stageRowUsed) * d.out.rowStride + head * a.values;
-        const T *const values = rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)(begin + stageRowUsed) * a.v.rowStride + head * a.values;
-        const float *const dRRow = d.errors + (at * C + stageRowUsed) * a.padded, *const wRow = a.errors + (at * C + stageRowUsed) * a.padded;
-        for(uint32_t v = 0; v < a.padded; v += 32) {
-            float4 s0[2], ds[2];
-            #pragma unroll
-            for(int h = 0; h < 2; h++) { s0[h] = *(const float4*)(stateRow + v + 4 * h); ds[h] = *(const float4*)(dStateRow + v + 4 * h); }
-            float dout[4] = {0, 0, 0, 0}, dr[4] = {0, 0, 0, 0}, w[4] = {0, 0, 0, 0};
-            if(stages && stageRow < count) {
-                const float4 x = *(const float4*)(dRRow + v + stageAt), y = *(const float4*)(wRow + v + stageAt);
-                dr[0] = x.x; dr[1] = x.y; dr[2] = x.z; dr[3] = x.w;
-                w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
-                #pragma unroll
-                for(int e = 0; e < 4; e++) {
-                    if(v + stageAt + e < a.values) {
-                        dout[e] = widen(douts[v + stageAt + e]);
-                        valueDot = __builtin_fmaf(widen(values[v + stageAt + e]), dr[e], valueDot);
-                        betaDot = __builtin_fmaf(w[e], dr[e], betaDot);
-                    }
-                }
-            }
-            __syncthreads();
-            if(stages) {
-                uint2 words[3];
-                uint16_t *const to = stage + stageRow * L::VALUES + stageAt;
-                uint2 own[NP];
-                splitFour<NP>(dout, own);
-                #pragma unroll
-                for(int k = 0; k < NP; k++) { *(uint2*)(to + k * VP) = own[k]; }
-                splitFour<3>(dr, words);
-                #pragma unroll
-                for(int k = 0; k < 3; k++) { *(uint2*)(to + (NP + k) * VP) = words[k]; }
-                splitFour<3>(w, words);
-                #pragma unroll
-                for(int k = 0; k < 3; k++) { *(uint2*)(to + (NP + 3 + k) * VP) = words[k]; }
-            }
-            __syncthreads();
-            const f32x4 s0a = {s0[0].x, s0[0].y, s0[0].z, s0[0].w}, s0b = {s0[1].x, s0[1].y, s0[1].z, s0[1].w};
-            const f32x4 dsa = {ds[0].x, ds[0].y, ds[0].z, ds[0].w}, dsb = {ds[1].x, ds[1].y, ds[1].z, ds[1].w};
-            #pragma unroll
-            for(int e = 0; e < 4; e++) { stateDot = __builtin_fmaf(s0a[e], dsa[e], stateDot); stateDot = __builtin_fmaf(s0b[e], dsb[e], stateDot); }
-            const Planes<3> state = split<3>(s0a, s0b), dState = split<3>(dsa, dsb);
-            #pragma unroll
-            for(int m = 0; m < MINE; m++) {
-                inTurn();
-                const uint32_t offset = (tileOf(m) * 16 + n16) * L::VALUES + 8 * g;
-                outS[m] = multiply(fetch<NP>(doutPlanes + offset, VP), state, outS[m]);
-                rS[m] = multiply(fetch<3>(dRPlanes + offset, VP), state, rS[m]);
-                wD[m] = multiply(fetch<3>(wPlanes + offset, VP), dState, wD[m]);
-            }
-            if(squares) {
-                const Planes<3> other = fetch<3>(wPlanes + (squareColumn * 16 + n16) * L::VALUES + 8 * g, VP);
-                #pragma unroll
-                for(int q = 0; q < SQUARES; q++) {
-                    inTurn();
-                    if(squareRow(q) < squareColumn) { continue; }
-                    const uint32_t offset = (squareRow(q) * 16 + n16) * L::VALUES + 8 * g;
-                    outW[q] = multiply(fetch<NP>(doutPlanes + offset, VP), other, outW[q]);
-                    rW[q] = multiply(fetch<3>(dRPlanes + offset, VP), other, rW[q]);
-                }
-            }
-        }
-        // what this head adds, and its gates' share
-        float endDot = 0.0f;
+        for(int e = 0; e < 4; e++) { stateDot = __builtin_fmaf(s0a[e], dsa[e], stateDot); stateDot = __builtin_fmaf(s0b[e], dsb[e], stateDot); }
+        const Planes<3> state = split<3>(s0a, s0b), dState = split<3>(dsa, dsb);
         #pragma unroll
         for(int m = 0; m < MINE; m++) {
-            const f32x4 q = valuesAt(L::queryColumns, tileOf(m)), k = valuesAt(L::keyColumns, tileOf(m));
+            inTurn();
+            const uint32_t offset = (tileOf(m) * 16 + n16) * L::VALUES + 8 * g;
+            dq[m] = multiply(fetch<NP>(doutPlanes + offset, VP), state, dq[m]);
+            rS[m] = multiply(fetch<3>(dRPlanes + offset, VP), state, rS[m]);
+            dk[m] = multiply(fetch<3>(wPlanes + offset, VP), dState, dk[m]);
+        }
+        if(squares) {
+            const Planes<3> other = fetch<3>(wPlanes + (squareColumn * 16 + n16) * L::VALUES + 8 * g, VP);
             #pragma unroll
-            for(int r = 0; r < 4; r++) {
-                const uint32_t row = tileOf(m) * 16 + 4 * g + r;
-                const float x = a.scale * since[row] * outS[m][r], y = until[row] * beta[row] * wD[m][r];
-                dq[m][r] += x;
-                dk[m][r] += y - since[row] * beta[row] * rS[m][r];
-                endDot = __builtin_fmaf(k[r] * keyUnit[row], y, endDot);
-                const float dot = sumOf16(q[r] * queryUnit[row] * x);
-                if(n16 == 0) { queryDots[(firstRow * KEY_TILES + keyTile) * C + row] = dot; }
+            for(int q = 0; q < SQUARES; q++) {
+                inTurn();
+                if(squareRow(q) < squareColumn) { continue; }
+                const uint32_t offset = (squareRow(q) * 16 + n16) * L::VALUES + 8 * g;
+                dqk[q] = multiply(fetch<NP>(doutPlanes + offset, VP), other, dqk[q]);
+                dkk[q] = multiply(fetch<3>(dRPlanes + offset, VP), other, dkk[q]);
             }
         }
+        inTurn();
+    }
+    // what the rows' factors make of them, and the gates' share
+    float endDot = 0.0f;
+    #pragma unroll
+    for(int m = 0; m < MINE; m++) {
+        const uint32_t tile = tileOf(m);
+        const f32x4 q = valuesAt(L::queryColumns, tile) * fourRows(queryUnit, tile), k = valuesAt(L::keyColumns, tile) * fourRows(keyUnit, tile);
+        const f32x4 grown = fourRows(since, tile), by = fourRows(beta, tile);
+        dq[m] *= a.scale * grown;
+        dk[m] *= fourRows(until, tile) * by;
+        #pragma unroll
+        for(int r = 0; r < 4; r++) {
+            endDot = __builtin_fmaf(k[r], dk[m][r], endDot);
+            const float dot = sumOf16(q[r] * dq[m][r]);
+            if(n16 == 0) { queryDots[wave * C + tile * 16 + 4 * g + r] = dot; }
+        }
+        dk[m] -= grown * by * rS[m];
+    }
+    if(squares) {
+        const uint32_t column = squareColumn * 16 + n16;
+        const float betaColumn = beta[column];
+        const double sumColumn = sums[column];
         #pragma unroll
         for(int q = 0; q < SQUARES; q++) {
-            const uint32_t column = squareColumn * 16 + n16;
+            const f32x4 by = fourRows(beta, squareRow(q));
             #pragma unroll
             for(int r = 0; r < 4; r++) {
                 const uint32_t row = squareRow(q) * 16 + 4 * g + r;
                 float dot = 0.0f;
-                if(squares && row >= column) {
-                    const float between = decayOver(sums[row] - sums[column]), x = outW[q][r] * beta[column];
-                    dqk[q][r] = __builtin_fmaf(a.scale * between, x, dqk[q][r]);
-                    if(row > column) { dkk[q][r] -= between * (beta[row] * beta[column] * rW[q][r]); }
+                if(row >= column) {
+                    const float between = decayOver(sums[row] - sumColumn), x = dqk[q][r] * betaColumn;
                     dot = x * a.score[(at * C + row) * C + column];
+                    dqk[q][r] = a.scale * between * x;
+                    dkk[q][r] = row > column ? -between * (by[r] * betaColumn * dkk[q][r]) : 0.0f;
                 }
+                else { dqk[q][r] = dkk[q][r] = 0.0f; }
                 dot = sumOf16(dot);
-                if(squares && n16 == 0) { keyDots[squareColumn * C + row] = dot; }
+                if(n16 == 0) { keyDots[squareColumn * C + row] = dot; }
+            }
+        }
+    }
+    #pragma unroll
+    for(int w = 1; w < 64; w *= 2) { stateDot += __shfl_xor(stateDot, w); endDot += __shfl_xor(endDot, w); }
+    // (wavefronts that split a key tile's rows have read the same state)
+    if(lane == 0) { ends[wave] = wave < KEY_TILES ? decay * stateDot + endDot : endDot; }
+    valueDot += partner<1>(valueDot); valueDot += partner<2>(valueDot); valueDot += partner<4>(valueDot);
+    betaDot += partner<1>(betaDot); betaDot += partner<2>(betaDot); betaDot += partner<4>(betaDot);
+    if(stages && stageAt == 0) {
+        valueDots[stageRow] = valueDot * beta[stageRow];
+        if(d.beta.data && stageRow < count) { (rowsOf<float>(d.beta, a.chunks, p) + (uint64_t)(begin + stageRow) * d.beta.rowStride)[head] = betaDot; }
+    }
+    __syncthreads();
+    if(d.g.data && wave == 0) {
+        double sum = 0.0;
+        if(lane < C) {
+            sum = -(double)valueDots[lane];
+            // (a row's dots lie with the wavefronts that have its tile)
+            const uint32_t firstWave = (lane / 16) % SPLIT * KEY_TILES;
+            #pragma unroll
+            for(int w = 0; w < KEY_TILES; w++) { sum += queryDots[(firstWave + w) * C + lane]; }
+            #pragma unroll
+            for(int w = 0; w < TILES; w++) { sum += keyDots[w * C + lane]; }
+            if(lane == C - 1) {
+                #pragma unroll
+                for(int w = 0; w < 8; w++) { sum += ends[w]; }
             }
         }
         #pragma unroll
-        for(int w = 1; w < 64; w *= 2) { stateDot += __shfl_xor(stateDot, w); endDot += __shfl_xor(endDot, w); }
-        if(lane == 0) { ends[wave] = wave < KEY_TILES ? decay * stateDot + endDot : endDot; }
-        valueDot += partner<1>(valueDot); valueDot += partner<2>(valueDot); valueDot += partner<4>(valueDot);
-        betaDot += partner<1>(betaDot); betaDot += partner<2>(betaDot); betaDot += partner<4>(betaDot);
-        if(stages && stageAt == 0) {
-            valueDots[stageRow] = valueDot * beta[stageRow];
-            if(d.beta.data && stageRow < count) { (rowsOf<float>(d.beta, a.chunks, p) + (uint64_t)(begin + stageRow) * d.beta.rowStride)[head] = betaDot; }
+        for(int w = 1; w < C; w *= 2) {
+            const double behind = __shfl_down(sum, w);
+            if(lane + w < C) { sum += behind; }
         }
-        __syncthreads();
-        if(d.g.data && wave == 0) {
-            double sum = 0.0;
-            if(lane < C) {
-                sum = -(double)valueDots[lane];
-                // (a row's dots lie with the wavefronts that have its tile: all of DK / 16 key tiles)
-                const uint32_t group = (lane / 16) % SPLIT;
-                #pragma unroll
-                for(int w = 0; w < KEY_TILES; w++) { sum += queryDots[(group * KEY_TILES + w) * C + lane]; }
-                #pragma unroll
-                for(int w = 0; w < TILES; w++) { sum += keyDots[w * C + lane]; }
-                if(lane == C - 1) {
-                    #pragma unroll
-                    for(int w = 0; w < 8; w++) { sum += ends[w]; }
-                }
-            }
-            #pragma unroll
-            for(int w = 1; w < C; w *= 2) {
-                const double behind = __shfl_down(sum, w);
-                if(lane + w < C) { sum += behind; }
-            }
-            if(lane < count) { (rowsOf<float>(d.g, a.chunks, p) + (uint64_t)(begin + lane) * d.g.rowStride)[head] = (float)sum; }
-        }
+        if(lane < count) { (rowsOf<float>(d.g, a.chunks, p) + (uint64_t)(begin + lane) * d.g.rowStride)[head] = (float)sum; }
     }
+    if(!d.q.data && !d.k.data) { return; }
 
     // squares times queries and keys
-    const auto storeSquares = [&](bool transposed, auto &&value) {
+    const auto storeSquares = [&](bool transposed, const f32x4 (&square)[SQUARES], const float *rowFactor, const float *columnFactor) {
+        if(!squares) { return; }
         #pragma unroll
         for(int q = 0; q < SQUARES; q++) {
             const uint32_t column = squareColumn * 16 + n16, row = squareRow(q) * 16 + 4 * g;
-            float x[4];
-            #pragma unroll
-            for(int r = 0; r < 4; r++) { x[r] = value(q, r, row + r, column); }
+            const f32x4 scaled = square[q] * (rowFactor ? fourRows(rowFactor, squareRow(q)) : f32x4{1, 1, 1, 1} * columnFactor[column]);
+            const float x[4] = {scaled[0], scaled[1], scaled[2], scaled[3]};
             uint2 words[3];
             splitFour<3>(x, words);
             #pragma unroll
@@ -1100,61 +1131,114 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     const auto timesColumns = [&](uint32_t from, f32x4 (&to)[MINE]) {
         #pragma unroll
         for(int s = 0; s < TILES / 2; s++) {
-            inTurn();
             const Planes<NP> b = fetch<NP>(planes + from + key * L::COLUMN + 32 * s + 8 * g, DK * L::COLUMN);
             #pragma unroll
             for(int m = 0; m < MINE; m++) { inTurn(); to[m] = multiply(fetch<3>(stage + (tileOf(m) * 16 + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, to[m]); }
         }
     };
-    __syncthreads();
-    if(squares) { storeSquares(false, [&](int q, int r, uint32_t row, uint32_t column) { return dqk[q][r] * keyUnit[column]; }); }
+    storeSquares(false, dqk, nullptr, keyUnit);
     __syncthreads();
     timesColumns(L::keyColumns, dq);
     __syncthreads();
-    if(squares) { storeSquares(true, [&](int q, int r, uint32_t row, uint32_t column) { return dqk[q][r] * queryUnit[row]; }); }
+    storeSquares(true, dqk, queryUnit, nullptr);
     __syncthreads();
     timesColumns(L::queryColumns, dk);
     __syncthreads();
-    if(squares) { storeSquares(false, [&](int q, int r, uint32_t row, uint32_t column) { return dkk[q][r] * keyUnit[column]; }); }
+    storeSquares(false, dkk, nullptr, keyUnit);
     __syncthreads();
     timesColumns(L::keyColumns, dk);
     __syncthreads();
-    if(squares) { storeSquares(true, [&](int q, int r, uint32_t row, uint32_t column) { return dkk[q][r] * keyUnit[row]; }); }
+    storeSquares(true, dkk, keyUnit, nullptr);
     __syncthreads();
     timesColumns(L::keyColumns, dk);
+    if(a.group > 1) {
+        float *const to = d.shared + at * 2 * C * DK;
+        storeResultTiles<MINE, SPLIT>(to, DK, firstRow, g, key, dq);
+        storeResultTiles<MINE, SPLIT>(to + C * DK, DK, firstRow, g, key, dk);
+        return;
+    }
 
     // through the lengths of queries and keys
     if(a.normalise) {
         #pragma unroll
         for(int m = 0; m < MINE; m++) {
-            const f32x4 q = valuesAt(L::queryColumns, tileOf(m)), k = valuesAt(L::keyColumns, tileOf(m));
+            const f32x4 q = valuesAt(L::queryColumns, tileOf(m)) * fourRows(queryUnit, tileOf(m)), k = valuesAt(L::keyColumns, tileOf(m)) * fourRows(keyUnit, tileOf(m));
             #pragma unroll
             for(int r = 0; r < 4; r++) {
-                const uint32_t row = tileOf(m) * 16 + 4 * g + r;
-                const float x = sumOf16(q[r] * queryUnit[row] * dq[m][r]), y = sumOf16(k[r] * keyUnit[row] * dk[m][r]);
-                if(n16 == 0) { queryDots[(firstRow * KEY_TILES + keyTile) * C + row] = x; keyDots[(firstRow * KEY_TILES + keyTile) * C + row] = y; }
+                const float x = sumOf16(q[r] * dq[m][r]), y = sumOf16(k[r] * dk[m][r]);
+                if(n16 == 0) { queryDots[wave * C + tileOf(m) * 16 + 4 * g + r] = x; keyDots[wave * C + tileOf(m) * 16 + 4 * g + r] = y; }
             }
         }
         __syncthreads();
     }
     #pragma unroll
     for(int m = 0; m < MINE; m++) {
-        const f32x4 q = valuesAt(L::queryColumns, tileOf(m)), k = valuesAt(L::keyColumns, tileOf(m));
+        const uint32_t tile = tileOf(m);
+        const f32x4 queryLength = fourRows(queryUnit, tile), keyLength = fourRows(keyUnit, tile);
+        f32x4 x = dq[m], y = dk[m];
+        if(a.normalise) {
+            f32x4 queryDot = {0, 0, 0, 0}, keyDot = {0, 0, 0, 0};
+            #pragma unroll
+            for(int w = 0; w < KEY_TILES; w++) {
+                queryDot += fourRows(queryDots + (firstRow * KEY_TILES + w) * C, tile);
+                keyDot += fourRows(keyDots + (firstRow * KEY_TILES + w) * C, tile);
+            }
+            x -= valuesAt(L::queryColumns, tile) * queryLength * queryDot;
+            y -= valuesAt(L::keyColumns, tile) * keyLength * keyDot;
+        }
+        x *= queryLength;
+        y *= keyLength;
         #pragma unroll
         for(int r = 0; r < 4; r++) {
-            const uint32_t row = tileOf(m) * 16 + 4 * g + r;
-            float x = dq[m][r], y = dk[m][r];
-            if(a.normalise) {
-                float queryDot = 0.0f, keyDot = 0.0f;
-                #pragma unroll
-                for(int w = 0; w < KEY_TILES; w++) { queryDot += queryDots[(firstRow * KEY_TILES + w) * C + row]; keyDot += keyDots[(firstRow * KEY_TILES + w) * C + row]; }
-                x -= q[r] * queryUnit[row] * queryDot;
-                y -= k[r] * keyUnit[row] * keyDot;
-            }
+            const uint32_t row = tile * 16 + 4 * g + r;
             if(row < count && key < a.keys) {
-                if(d.q.data) { (rowsOf<T>(d.q, a.chunks, p) + (uint64_t)(begin + row) * d.q.rowStride)[keyHead * a.keys + key] = narrow<T>(x * queryUnit[row]); }
-                if(d.k.data) { (rowsOf<T>(d.k, a.chunks, p) + (uint64_t)(begin + row) * d.k.rowStride)[keyHead * a.keys + key] = narrow<T>(y * keyUnit[row]); }
+                if(d.q.data) { (rowsOf<T>(d.q, a.chunks, p) + (uint64_t)(begin + row) * d.q.rowStride)[keyHead * a.keys + key] = narrow<T>(x[r]); }
+                if(d.k.data) { (rowsOf<T>(d.k, a.chunks, p) + (uint64_t)(begin + row) * d.k.rowStride)[keyHead * a.keys + key] = narrow<T>(y[r]); }
             }
+        }
+    }
+}
+
+// Gradients of keys and queries that heads share: the heads' one after another, then through the lengths.  A wavefront a row of a key head, lane l its keys l and l + 64.
+template<typename T, int C, int DK>
+__global__ __launch_bounds__(256)
+void deltaSharedKernel(DeltaArgs a, DeltaGradientArgs d)
+{
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t number = blockIdx.x / a.keyHeads, keyHead = blockIdx.x - number * a.keyHeads;
+    Place p;
+    if(!locate(a.chunks, number, p)) { return; }
+    const uint32_t begin = p.index * C, count = min((uint32_t)C, p.length - min(p.length, begin));
+    const float *const from = d.shared + ((uint64_t)number * a.heads + keyHead * a.group) * 2 * C * DK;
+    for(uint32_t row = wave; row < count; row += 4) {
+        #pragma unroll
+        for(int which = 0; which < 2; which++) {
+            const gennmi_rows_t &in = which ? a.k : a.q, &out = which ? d.k : d.q;
+            if(!out.data) { continue; }
+            float x[DK / 64], hat[DK / 64], square = 0.0f, dot = 0.0f;
+            #pragma unroll
+            for(int i = 0; i < DK / 64; i++) {
+                const uint32_t key = lane + 64 * i;
+                x[i] = 0.0f;
+                for(uint32_t h = 0; h < a.group; h++) { x[i] += from[(h * 2 + which) * C * DK + row * DK + key]; }
+                hat[i] = key < a.keys ? widen(rowAt<T>(in, a.chunks, p, begin + row)[keyHead * a.keys + key]) : 0.0f;
+                square = __builtin_fmaf(hat[i], hat[i], square);
+            }
+            float unit = 1.0f;
+            if(a.normalise) {
+                #pragma unroll
+                for(int w = 1; w < 64; w *= 2) { square += __shfl_xor(square, w); }
+                unit = 1.0f / sqrtf(square + a.epsilon);
+                #pragma unroll
+                for(int i = 0; i < DK / 64; i++) { hat[i] *= unit; dot = __builtin_fmaf(hat[i], x[i], dot); }
+                #pragma unroll
+                for(int w = 1; w < 64; w *= 2) { dot += __shfl_xor(dot, w); }
+                #pragma unroll
+                for(int i = 0; i < DK / 64; i++) { x[i] -= hat[i] * dot; }
+            }
+            T *const to = rowsOf<T>(out, a.chunks, p) + (uint64_t)(begin + row) * out.rowStride + keyHead * a.keys;
+            #pragma unroll
+            for(int i = 0; i < DK / 64; i++) { if(lane + 64 * i < a.keys) { to[lane + 64 * i] = narrow<T>(x[i] * unit); } }
         }
     }
 }
