@@ -26,9 +26,8 @@ template<typename F> int withSizes(const gennmi_delta_rule_t &c, F &&f)
     default: return keys(bf16{}, std::integral_constant<int, 64>{});
     }
 }
-template<typename F> int withWaves(uint32_t columns, F &&f) { return columns <= 64 ? f(std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 8>{}); }
-uint32_t wavesFor(uint32_t columns) { return columns <= 64 ? 4 : 8; }
-uint32_t blocksOf(uint32_t columns) { return (columns + 16 * wavesFor(columns) - 1) / (16 * wavesFor(columns)); }
+constexpr uint32_t WALK_COLUMNS = WALK_THREADS / 64 * 16;         // of a work-group of a walk
+uint32_t blocksOf(uint32_t columns) { return (columns + WALK_COLUMNS - 1) / WALK_COLUMNS; }
 
 int checkDelta(const char *what, const gennmi_delta_rule_t *c, bool gradients)
 {
@@ -88,7 +87,7 @@ uint32_t segmentRows(const gennmi_delta_rule_t &c, bool gradients)
     return (chunks + segments - 1) / segments * C;
 }
 bool isCut(const gennmi_delta_rule_t &c, bool gradients) { return c.sequences.length > segmentRows(c, gradients); }
-uint32_t moveBlocks(const gennmi_delta_rule_t &c, uint32_t columns) { const uint32_t each = 16 * wavesFor(columns); return (paddedKeys(c.keys) + each - 1) / each; }
+uint32_t moveBlocks(const gennmi_delta_rule_t &c) { return blocksOf(paddedKeys(c.keys)); }
 struct DeltaSpace { size_t correction, score, rows, table, segmentStates, segmentMoves, states, errors, gradientStates, gradientErrors, shared, bytes; };
 DeltaSpace deltaSpace(const gennmi_delta_rule_t &c, bool gradients)
 {
@@ -121,7 +120,7 @@ bool deltaFits(const gennmi_delta_rule_t &c, bool gradients)
     if(!gradients && c.sequences.length <= 1) { return tokenBlocks(c) <= mostBlocks(256); }
     const uint32_t columns = gradients ? paddedValues(c.values) : c.values;
     return chunkNumbers(c.sequences, chunkRows(c.type)) * c.heads <= mostBlocks(512) &&
-        chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.heads * (blocksOf(columns) + moveBlocks(c, columns)) <= mostBlocks(64 * wavesFor(columns)) &&
+        chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.heads * (blocksOf(columns) + moveBlocks(c)) <= mostBlocks(WALK_THREADS) &&
         (uint64_t)c.sequences.count * c.heads * (paddedValues(c.values) / 16) <= mostBlocks(64);
 }
 DeltaArgs deltaArgs(const gennmi_delta_rule_t &c, const DeltaSpace &space, void *workspace, bool gradients)
@@ -147,7 +146,7 @@ DeltaArgs deltaArgs(const gennmi_delta_rule_t &c, const DeltaSpace &space, void 
     if(isCut(c, gradients)) {
         a.segmentStates = (float*)at(space.segmentStates);
         a.segmentMoves = (float*)at(space.segmentMoves);
-        a.moveBlocks = moveBlocks(c, gradients ? a.padded : a.values);
+        a.moveBlocks = moveBlocks(c);
     }
     if(gradients) {
         a.states = (float*)at(space.states);
@@ -173,14 +172,11 @@ template<typename T, int C, int DK, bool FOLDED> int launchChunks(const char *wh
 }
 template<typename T, int C, int DK, int MODE, bool FOLDED> int launchWalk(const char *what, const DeltaArgs &a, uint64_t segments, hipStream_t stream)
 {
-    return withWaves(FOLDED ? a.values : a.padded, [&](auto waves) {
-        constexpr int WAVES = decltype(waves)::value;
-        const auto kernel = deltaStateKernel<T, C, DK, WAVES, MODE, FOLDED>;
-        constexpr size_t lds = WalkLayout<T, C, DK, MODE>::bytes;
-        if(const int rc = withLds(what, kernel, lds)) { return rc; }
-        kernel<<<dim3((uint32_t)(segments * a.heads * (a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0)))), dim3(64 * WAVES), lds, stream>>>(a);
-        return gennmi_detail::afterLaunch(what);
-    });
+    const auto kernel = deltaStateKernel<T, C, DK, MODE, FOLDED>;
+    constexpr size_t lds = WalkLayout<T, C, DK, MODE == WALK_OUTPUTS>::bytes;
+    if(const int rc = withLds(what, kernel, lds)) { return rc; }
+    kernel<<<dim3((uint32_t)(segments * a.heads * (a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0)))), dim3(WALK_THREADS), lds, stream>>>(a);
+    return gennmi_detail::afterLaunch(what);
 }
 // The state in front of every segment
 template<typename T, int C, int DK, bool FOLDED> int launchSegments(const char *what, const DeltaArgs &a, uint64_t segments, hipStream_t stream)
@@ -194,14 +190,11 @@ template<typename T, int C, int DK> int launchGradients(const char *what, const 
 {
     if(const int rc = launchChunks<T, C, DK, false>(what, a, numbers, stream)) { return rc; }
     if(const int rc = launchWalk<T, C, DK, WALK_KEEP, false>(what, a, segments, stream)) { return rc; }
-    const int rc = withWaves(a.padded, [&](auto waves) {
-        constexpr int WAVES = decltype(waves)::value;
-        const auto kernel = deltaReverseKernel<T, C, DK, WAVES>;
-        constexpr size_t lds = ReverseLayout<T, C, DK>::bytes;
-        if(const int rcLds = withLds(what, kernel, lds)) { return rcLds; }
-        kernel<<<dim3((uint32_t)(segments * a.heads * a.columnBlocks)), dim3(64 * WAVES), lds, stream>>>(a, d);
-        return gennmi_detail::afterLaunch(what);
-    });
+    const auto reverse = deltaReverseKernel<T, C, DK>;
+    constexpr size_t reverseLds = WalkLayout<T, C, DK, true>::bytes;
+    if(const int rc = withLds(what, reverse, reverseLds)) { return rc; }
+    reverse<<<dim3((uint32_t)(segments * a.heads * a.columnBlocks)), dim3(WALK_THREADS), reverseLds, stream>>>(a, d);
+    const int rc = gennmi_detail::afterLaunch(what);
     if(rc || !(d.q.data || d.k.data || d.g.data || d.beta.data)) { return rc; }
     const auto kernel = deltaGradientKernel<T, C, DK>;
     constexpr size_t lds = GradientLayout<T, C, DK>::bytes;

@@ -74,18 +74,19 @@ template<typename T> __device__ inline const T *rowAt(const gennmi_rows_t &r, co
 
 // ---- what a chunk needs that does not depend on the state
 // FOLDED: for outputs alone, -N beta and P beta (I - N beta) are left, which r is multiplied with at once; else, for gradients, -N and P.
-template<typename T, int C, int DK> constexpr uint32_t chunkLds() { return 2 * planesOf<T> * C * (DK + 8) * 2 + 2 * C * (C + 4) * 4 + C * (8 + 3 * 4) + 16; }
+// (M and P lie where the keys and queries were)
+template<typename T, int C, int DK> constexpr uint32_t chunkSquares() { const uint32_t keys = 2 * planesOf<T> * C * DK * 2, squares = 2 * C * (C + 4) * 4; return keys > squares ? keys : squares; }
+template<typename T, int C, int DK> constexpr uint32_t chunkLds() { return chunkSquares<T, C, DK>() + C * (8 + 3 * 4) + 16; }
 
 template<typename T, int C, int DK, bool FOLDED>
 __global__ __launch_bounds__(256)
 void deltaChunkKernel(DeltaArgs a)
 {
-    constexpr int NP = planesOf<T>, B = C / 16, PITCH = DK + 8, PLANE = C * PITCH, MP = C + 4, TILES = B * B / 4;
+    constexpr int NP = planesOf<T>, B = C / 16, PLANE = C * DK, MP = C + 4, TILES = B * B / 4;
     extern __shared__ __align__(16) char lds[];
     uint16_t *const keyPlanes = (uint16_t*)lds, *const queryPlanes = keyPlanes + NP * PLANE;
-    float *const m = (float*)(queryPlanes + NP * PLANE);
-    float *const scores = m + C * MP;
-    double *const sums = (double*)(scores + C * MP);
+    float *const m = (float*)lds, *const scores = m + C * MP;
+    double *const sums = (double*)(lds + chunkSquares<T, C, DK>());
     float *const keyUnit = (float*)(sums + C), *const queryUnit = keyUnit + C, *const beta = queryUnit + C;
     uint32_t *const bad = (uint32_t*)(beta + C);
     const uint32_t number = blockIdx.x / a.keyHeads, keyHead = blockIdx.x - number * a.keyHeads;
@@ -105,19 +106,10 @@ void deltaChunkKernel(DeltaArgs a)
         for(int which = 0; which < 2; which++) {
             const gennmi_rows_t &r = which ? a.q : a.k;
             const Eight<T> x = loadEight(rowAt<T>(r, a.chunks, p, valid ? begin + row : 0) + (valid ? keyHead * a.keys + at : 0), valid, a.wide);
-            float sum = 0.0f, first[4], second[4];
+            float sum = 0.0f;
             #pragma unroll
-            for(int e = 0; e < 8; e++) {
-                const float f = widen(x.at(e));
-                sum = __builtin_fmaf(f, f, sum);
-                (e < 4 ? first[e] : second[e - 4]) = f;
-            }
-            uint2 low[NP], high[NP];
-            splitFour<NP>(first, low);
-            splitFour<NP>(second, high);
-            uint16_t *const to = (which ? queryPlanes : keyPlanes) + row * PITCH + at;
-            #pragma unroll
-            for(int k = 0; k < NP; k++) { *(uint4*)(to + k * PLANE) = make_uint4(low[k].x, low[k].y, high[k].x, high[k].y); }
+            for(int e = 0; e < 8; e++) { const float f = widen(x.at(e)); sum = __builtin_fmaf(f, f, sum); }
+            storeUnit((which ? queryPlanes : keyPlanes) + unitAt<DK>(row, at / 8), PLANE, x);
             sum += partner<1>(sum);
             sum += partner<2>(sum);
             sum += partner<4>(sum);
@@ -138,7 +130,7 @@ void deltaChunkKernel(DeltaArgs a)
         #pragma unroll
         for(int s = 0; s < DK / 32; s++) {
             inTurn();
-            const uint32_t offset = s * 32 + g * 8, ra = (tileRow(t) * 16 + n16) * PITCH + offset, rb = (tileColumn(t) * 16 + n16) * PITCH + offset;
+            const uint32_t ra = unitAt<DK>(tileRow(t) * 16 + n16, 4 * s + g), rb = unitAt<DK>(tileColumn(t) * 16 + n16, 4 * s + g);
             const Planes<NP> kb = fetch<NP>(keyPlanes + rb, PLANE);
             kk[t] = multiply(fetch<NP>(keyPlanes + ra, PLANE), kb, kk[t]);
             qk[t] = multiply(fetch<NP>(queryPlanes + ra, PLANE), kb, qk[t]);
@@ -274,93 +266,95 @@ void deltaChunkKernel(DeltaArgs a)
 // Writes outputs; keeps states and errors for gradients; or finds what a segment of a sequence does to the state in front of it, S behind = move S + its own.
 enum { WALK_OUTPUTS, WALK_KEEP, WALK_SUMMARY };
 
-// LDS of a walk, in elements of 16 bits: keys by row and by column, queries by row, -N, P
-template<typename T, int C, int DK, int MODE> struct WalkLayout
+// A lower triangle of C rows and columns in LDS: blocks of 32 rows, each as wide as it has to be
+template<int C> struct Triangle
 {
-    static constexpr int NP = planesOf<T>, ROW = DK + 8, COLUMN = C + 8;
-    static constexpr uint32_t keyRows = 0, keyColumns = keyRows + NP * C * ROW, queryRows = keyColumns + NP * DK * COLUMN,
-        correction = queryRows + (MODE == WALK_OUTPUTS ? NP * C * ROW : 0), score = correction + 3 * C * COLUMN,
-        table = (score + (MODE == WALK_OUTPUTS ? 3 * C * COLUMN : 0) + 7) / 8 * 8, bytes = table * 2 + C * 16;
+    static constexpr uint32_t elements = C == 64 ? 3 * 1024 : 1024;
+    // unit of a row
+    __device__ static uint32_t at(uint32_t row, uint32_t unit) { return C == 64 && row >= 32 ? 1024 + unitAt<64>(row - 32, unit) : unitAt<32>(row, unit); }
+    // which four neighbours of [C][C] item k is, of 8 of each of the first 32 rows and 16 of the others
+    static constexpr int items = C == 64 ? 768 : 256;
+    __device__ static uint32_t row(uint32_t k) { return k < 256 ? k / 8 : 32 + (k - 256) / 16; }
+    __device__ static uint32_t column(uint32_t k) { return (k < 256 ? k % 8 : (k - 256) % 16) * 4; }
 };
+// LDS of a walk, in elements of 16 bits: keys, queries, -N, P, factors of rows
+template<typename T, int C, int DK, bool QUERIES> struct WalkLayout
+{
+    static constexpr int NP = planesOf<T>;
+    static constexpr uint32_t keys = 0, queries = keys + NP * C * DK, correction = queries + (QUERIES ? NP * C * DK : 0), score = correction + 3 * Triangle<C>::elements,
+        table = score + (QUERIES ? 3 * Triangle<C>::elements : 0), bytes = table * 2 + C * 16;
+};
+constexpr int WALK_THREADS = 256;
+// What the next chunk needs, on its way to LDS
+template<typename T, int C, int DK, bool QUERIES> struct WalkStage
+{
+    typedef WalkLayout<T, C, DK, QUERIES> L;
+    static constexpr int EACH = C * DK / 8 / WALK_THREADS, SQUARES = Triangle<C>::items / WALK_THREADS;
+    Eight<T> keys[EACH], queries[QUERIES ? EACH : 1];
+    float4 corrections[SQUARES], scores[QUERIES ? SQUARES : 1], rows;
 
-// A tile of four rows and eight columns of keys (or queries) on its way to LDS
-template<typename T> struct KeyTile { Eight<T> row[4]; };
-template<typename T, int C, int DK> __device__ inline void loadTile(const DeltaArgs &a, const gennmi_rows_t &r, const Place &p, uint32_t keyHead, uint32_t begin, uint32_t count, uint32_t item, KeyTile<T> &tile)
-{
-    const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
-    const T *const base = rowsOf<const T>(r, a.chunks, p) + (uint64_t)begin * r.rowStride + keyHead * a.keys;
-    #pragma unroll
-    for(int i = 0; i < 4; i++) {
-        const uint32_t valid = row + i < count && at < a.keys ? min(8u, a.keys - at) : 0;
-        tile.row[i] = loadEight(base + (valid ? (uint64_t)(row + i) * r.rowStride + at : 0), valid, a.wide);
-    }
-}
-template<typename T, int NP> __device__ inline void planesOfFour(const T (&x)[4], uint2 (&out)[NP])
-{
-    const float f[4] = {widen(x[0]), widen(x[1]), widen(x[2]), widen(x[3])};
-    splitFour<NP>(f, out);
-}
-template<typename T, int C, int DK> __device__ inline void storeRows(uint16_t *to, uint32_t item, const KeyTile<T> &tile)
-{
-    constexpr int NP = planesOf<T>, PITCH = DK + 8;
-    const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
-    #pragma unroll
-    for(int i = 0; i < 4; i++) {
-        uint2 words[2][NP];
+    __device__ void request(const DeltaArgs &a, const Place &p, uint32_t keyHead, uint32_t first, uint32_t count, uint64_t at)
+    {
+        const T *const key = rowsOf<const T>(a.k, a.chunks, p) + (uint64_t)first * a.k.rowStride + keyHead * a.keys, *const query = rowsOf<const T>(a.q, a.chunks, p) + (uint64_t)first * a.q.rowStride + keyHead * a.keys;
         #pragma unroll
-        for(int half = 0; half < 2; half++) {
-            if constexpr(NP == 1) { words[half][0] = half ? make_uint2(tile.row[i].word[0].z, tile.row[i].word[0].w) : make_uint2(tile.row[i].word[0].x, tile.row[i].word[0].y); }
-            else {
-                const T x[4] = {tile.row[i].at(4 * half), tile.row[i].at(4 * half + 1), tile.row[i].at(4 * half + 2), tile.row[i].at(4 * half + 3)};
-                planesOfFour<T, NP>(x, words[half]);
-            }
+        for(int i = 0; i < EACH; i++) {
+            const uint32_t item = threadIdx.x + i * WALK_THREADS, row = item / (DK / 8), column = item % (DK / 8) * 8, valid = row < count && column < a.keys ? min(8u, a.keys - column) : 0;
+            keys[i] = loadEight(key + (valid ? row * a.k.rowStride + column : 0), valid, a.wide);
+            if(QUERIES) { queries[i] = loadEight(query + (valid ? row * a.q.rowStride + column : 0), valid, a.wide); }
         }
         #pragma unroll
-        for(int k = 0; k < NP; k++) {
-            *(uint2*)(to + k * C * PITCH + (row + i) * PITCH + place(at)) = words[0][k];
-            *(uint2*)(to + k * C * PITCH + (row + i) * PITCH + place(at + 4)) = words[1][k];
+        for(int i = 0; i < SQUARES; i++) {
+            const uint32_t item = threadIdx.x + i * WALK_THREADS, offset = Triangle<C>::row(item) * C + Triangle<C>::column(item);
+            corrections[i] = *(const float4*)(a.correction + at * C * C + offset);
+            if(QUERIES) { scores[i] = *(const float4*)(a.score + at * C * C + offset); }
         }
+        if(threadIdx.x < C) { rows = ((const float4*)((const RowTable<C>*)a.rows + at))[threadIdx.x]; }
     }
-}
-// Four rows of one column, planes of 8 bytes
-template<typename T> __device__ inline void columnOf(const KeyTile<T> &tile, int e, uint2 (&words)[planesOf<T>])
-{
-    if constexpr(planesOf<T> == 1) {
-        const auto pair = [&](int i) {
-            const uint4 x = tile.row[i].word[0], y = tile.row[i + 1].word[0];
-            const uint32_t low = e / 2 == 0 ? x.x : e / 2 == 1 ? x.y : e / 2 == 2 ? x.z : x.w, high = e / 2 == 0 ? y.x : e / 2 == 1 ? y.y : e / 2 == 2 ? y.z : y.w;
-            return __builtin_amdgcn_perm(high, low, e % 2 ? 0x07060302u : 0x05040100u);
-        };
-        words[0] = make_uint2(pair(0), pair(2));
-    }
-    else {
-        const T x[4] = {tile.row[0].at(e), tile.row[1].at(e), tile.row[2].at(e), tile.row[3].at(e)};
-        planesOfFour<T, planesOf<T>>(x, words);
-    }
-}
-template<typename T, int C, int DK> __device__ inline void storeColumns(uint16_t *to, uint32_t item, const KeyTile<T> &tile)
-{
-    constexpr int NP = planesOf<T>, PITCH = C + 8;
-    const uint32_t row = item / (DK / 8) * 4, at = item % (DK / 8) * 8;
-    #pragma unroll
-    for(int e = 0; e < 8; e++) {
-        uint2 words[NP];
-        columnOf<T>(tile, e, words);
+    __device__ static void storeSquare(uint16_t *to, uint32_t item, const float4 &x)
+    {
+        const float f[4] = {x.x, x.y, x.z, x.w};
+        uint2 words[3];
+        splitFour<3>(f, words);
+        const uint32_t column = Triangle<C>::column(item);
+        to += Triangle<C>::at(Triangle<C>::row(item), column / 8) + column % 8;
         #pragma unroll
-        for(int k = 0; k < NP; k++) { *(uint2*)(to + k * DK * PITCH + (at + e) * PITCH + place(row)) = words[k]; }
+        for(int k = 0; k < 3; k++) { *(uint2*)(to + k * Triangle<C>::elements) = words[k]; }
     }
-}
-// [C][C] of floats as three planes, four neighbours an item
-template<int C> __device__ inline void storeSquare(uint16_t *to, uint32_t item, const float4 &x)
+    __device__ void store(uint16_t *planes) const
+    {
+        #pragma unroll
+        for(int i = 0; i < EACH; i++) {
+            const uint32_t item = threadIdx.x + i * WALK_THREADS, to = unitAt<DK>(item / (DK / 8), item % (DK / 8));
+            storeUnit(planes + L::keys + to, C * DK, keys[i]);
+            if(QUERIES) { storeUnit(planes + L::queries + to, C * DK, queries[i]); }
+        }
+        #pragma unroll
+        for(int i = 0; i < SQUARES; i++) {
+            storeSquare(planes + L::correction, threadIdx.x + i * WALK_THREADS, corrections[i]);
+            if(QUERIES) { storeSquare(planes + L::score, threadIdx.x + i * WALK_THREADS, scores[i]); }
+        }
+        if(threadIdx.x < C) { ((float4*)(planes + L::table))[threadIdx.x] = rows; }
+    }
+};
+// Operands of a walk.  Tile t of a result has rows in the order of rowIn(): of keys (or queries, of the chunk's rows), times what is summed over keys 32 s ..; of a triangle, summed over
+// rows 32 s ..; of their transposes, summed over the chunk's rows 32 s ..
+template<typename T, int C, int DK> struct WalkOperands
 {
-    constexpr int PITCH = C + 8;
-    const uint32_t row = item / (C / 4), at = item % (C / 4) * 4;
-    const float f[4] = {x.x, x.y, x.z, x.w};
-    uint2 words[3];
-    splitFour<3>(f, words);
-    #pragma unroll
-    for(int k = 0; k < 3; k++) { *(uint2*)(to + k * C * PITCH + row * PITCH + place(at)) = words[k]; }
-}
+    static constexpr int NP = planesOf<T>;
+    uint32_t n16, g;
+    __device__ Planes<NP> rows(const uint16_t *from, int t, int s) const { return fetch<NP>(from + unitAt<DK>(rowIn(t, n16), 4 * s + g), C * DK); }
+    __device__ Planes<NP> columns(const uint16_t *from, int t, int s) const
+    {
+        const uint32_t row = 32 * s + 8 * g + n16 / 4, unit = 4 * (t / 2) + n16 % 4, half = 4 * (t % 2);
+        return fetchColumn<NP>(from + unitAt<DK>(row, unit) + half, from + unitAt<DK>(row + 4, unit) + half, C * DK);
+    }
+    __device__ Planes<3> triangle(const uint16_t *from, int t, int s) const { return fetch<3>(from + Triangle<C>::at(rowIn(t, n16), 4 * s + g), Triangle<C>::elements); }
+    __device__ Planes<3> triangleColumns(const uint16_t *from, int t, int s) const
+    {
+        const uint32_t row = 32 * s + 8 * g + n16 / 4, unit = 4 * (t / 2) + n16 % 4, half = 4 * (t % 2);
+        return fetchColumn<3>(from + Triangle<C>::at(row, unit) + half, from + Triangle<C>::at(row + 4, unit) + half, Triangle<C>::elements);
+    }
+};
 
 // The first row of a column from which nothing is finite; rows of the chunk, if all are
 template<int C> __device__ inline uint32_t firstBad(const f32x4 (&x)[C / 16], uint32_t g)
@@ -369,24 +363,24 @@ template<int C> __device__ inline uint32_t firstBad(const f32x4 (&x)[C / 16], ui
     #pragma unroll
     for(int t = C / 16 - 1; t >= 0; t--) {
         #pragma unroll
-        for(int r = 3; r >= 0; r--) { if(!finite(x[t][r])) { first = 16 * t + 4 * g + r; } }
+        for(int r = 3; r >= 0; r--) { if(!finite(x[t][r])) { first = min(first, rowIn(t, 4 * g + r)); } }
     }
     first = min(first, (uint32_t)__shfl_xor((int)first, 16));
     return min(first, (uint32_t)__shfl_xor((int)first, 32));
 }
 
-// Rows of values at a lane's column, in the order of a result: row 16 t + 4 g + r.  What differs between lanes is an offset of 32 bits (strides are
+// Rows of values at a lane's column, in the order of a result: row 4 g + r of tile t.  What differs between lanes is an offset of 32 bits (strides are
 // below 2^26 here), the rest is the scalar unit's.  Behind `count` rows, or the last column: zero.
 template<typename T, int TILES> struct Result { T v[TILES][4]; };
 template<typename T, int TILES> __device__ inline Result<T, TILES> requestResult(const T *rows, uint64_t stride, uint32_t g, uint32_t column, bool inside, uint32_t count)
 {
     Result<T, TILES> x;
-    const uint32_t offset = 4 * g * (uint32_t)stride + (inside ? column : 0);
+    const uint32_t offset = 8 * g * (uint32_t)stride + (inside ? column : 0);
     if(count >= 16 * TILES) {       // (all there: without a branch a row; columns behind the last read the first)
         #pragma unroll
         for(int t = 0; t < TILES; t++) {
             #pragma unroll
-            for(int r = 0; r < 4; r++) { x.v[t][r] = (rows + (16 * t + r) * stride)[offset]; }
+            for(int r = 0; r < 4; r++) { x.v[t][r] = (rows + rowIn(t, r) * stride)[offset]; }
         }
         return x;
     }
@@ -395,7 +389,7 @@ template<typename T, int TILES> __device__ inline Result<T, TILES> requestResult
         #pragma unroll
         for(int r = 0; r < 4; r++) {
             x.v[t][r] = (T)0.0f;
-            if(16 * t + 4 * g + r < count) { x.v[t][r] = (rows + (16 * t + r) * stride)[offset]; }
+            if(rowIn(t, 4 * g + r) < count) { x.v[t][r] = (rows + rowIn(t, r) * stride)[offset]; }
         }
     }
     return x;
@@ -414,20 +408,20 @@ template<typename T, int C> __device__ inline void loadResult(const T *rows, uin
 }
 template<typename T, int C> __device__ inline void storeResult(T *rows, uint64_t stride, uint32_t g, uint32_t column, bool inside, uint32_t count, const f32x4 (&x)[C / 16])
 {
-    const uint32_t offset = 4 * g * (uint32_t)stride + column;
+    const uint32_t offset = 8 * g * (uint32_t)stride + column;
     if(!inside) { return; }
     if(count >= C) {
         #pragma unroll
         for(int t = 0; t < C / 16; t++) {
             #pragma unroll
-            for(int r = 0; r < 4; r++) { (rows + (16 * t + r) * stride)[offset] = narrow<T>(x[t][r]); }
+            for(int r = 0; r < 4; r++) { (rows + rowIn(t, r) * stride)[offset] = narrow<T>(x[t][r]); }
         }
         return;
     }
     #pragma unroll
     for(int t = 0; t < C / 16; t++) {
         #pragma unroll
-        for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r < count) { (rows + (16 * t + r) * stride)[offset] = narrow<T>(x[t][r]); } }
+        for(int r = 0; r < 4; r++) { if(rowIn(t, 4 * g + r) < count) { (rows + rowIn(t, r) * stride)[offset] = narrow<T>(x[t][r]); } }
     }
 }
 
@@ -442,18 +436,18 @@ template<int TILES, int SPLIT> __device__ inline void storeResultTiles(float *ro
 }
 
 // A work-group walks a sequence (or a segment of it) of one head with 16 columns of the state a wavefront.
-template<typename T, int C, int DK, int WAVES, int MODE, bool FOLDED>
-__global__ __launch_bounds__(64 * WAVES)
+template<typename T, int C, int DK, int MODE, bool FOLDED>
+__global__ __launch_bounds__(WALK_THREADS, 2)
 void deltaStateKernel(DeltaArgs a)
 {
-    typedef WalkLayout<T, C, DK, MODE> L;
-    constexpr int NP = planesOf<T>, THREADS = 64 * WAVES, TILES = C / 16, STATE = DK / 16;
     constexpr bool OUTPUTS = MODE == WALK_OUTPUTS;
-    constexpr int KEYS = C * DK / 32, KEY_ITEMS = KEYS * (OUTPUTS ? 2 : 1), EACH = (KEY_ITEMS + THREADS - 1) / THREADS, SQUARE = C * C / 4, SQUARES = (SQUARE + THREADS - 1) / THREADS;
+    typedef WalkLayout<T, C, DK, OUTPUTS> L;
+    constexpr int TILES = C / 16, STATE = DK / 16, WAVES = WALK_THREADS / 64;
     extern __shared__ __align__(16) char lds[];
     uint16_t *const planes = (uint16_t*)lds;
     const RowFactors<C> table{(float*)(planes + L::table)};
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
+    const WalkOperands<T, C, DK> operand{n16, g};
     const uint32_t blocks = a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0);
     const uint32_t block = blockIdx.x % blocks, rest = blockIdx.x / blocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
     Place p;
@@ -474,7 +468,7 @@ void deltaStateKernel(DeltaArgs a)
         #pragma unroll
         for(int t = 0; t < STATE; t++) {
             #pragma unroll
-            for(int r = 0; r < 4; r++) { if(move && 16 * t + 4 * g + r == column) { state[t][r] = 1.0f; } }
+            for(int r = 0; r < 4; r++) { if(move && rowIn(t, 4 * g + r) == column) { state[t][r] = 1.0f; } }
         }
     }
     else if(a.segmentStates) {
@@ -482,29 +476,8 @@ void deltaStateKernel(DeltaArgs a)
     }
     else if(a.initialState) { loadResult<float, DK>(a.initialState + ((uint64_t)p.state * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
 
-    KeyTile<T> keyTiles[EACH];
-    float4 corrections[SQUARES], scores[SQUARES];
-    float4 rowTable;
-    const auto prefetch = [&](uint32_t n) {
-        const uint32_t first = begin + n * C, count = min((uint32_t)C, end - first);
-        const uint64_t at = (firstNumber + n) * a.heads + head;
-        #pragma unroll
-        for(int i = 0; i < EACH; i++) {
-            const uint32_t item = tid + i * THREADS;
-            if(KEY_ITEMS % THREADS && item >= KEY_ITEMS) { break; }
-            if(!OUTPUTS || item < KEYS) { loadTile<T, C, DK>(a, a.k, p, keyHead, first, count, item, keyTiles[i]); }
-            else { loadTile<T, C, DK>(a, a.q, p, keyHead, first, count, item - KEYS, keyTiles[i]); }
-        }
-        #pragma unroll
-        for(int i = 0; i < SQUARES; i++) {
-            const uint32_t item = tid + i * THREADS;
-            if(SQUARE % THREADS && item >= SQUARE) { break; }
-            corrections[i] = ((const float4*)(a.correction + at * C * C))[item];
-            if(OUTPUTS) { scores[i] = ((const float4*)(a.score + at * C * C))[item]; }
-        }
-        if(tid < C) { rowTable = ((const float4*)((const RowTable<C>*)a.rows + at))[tid]; }
-    };
-    if(chunks) { prefetch(0); }
+    WalkStage<T, C, DK, OUTPUTS> stage;
+    if(chunks) { stage.request(a, p, keyHead, begin, min((uint32_t)C, end - begin), firstNumber * a.heads + head); }
     for(uint32_t n = 0; n < chunks; n++) {
         const uint32_t first = begin + n * C, count = min((uint32_t)C, end - first);
         const uint64_t at = (firstNumber + n) * a.heads + head;
@@ -512,26 +485,9 @@ void deltaStateKernel(DeltaArgs a)
         Result<T, TILES> values;
         if(active) { values = requestResult<T, TILES>(rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)first * a.v.rowStride + head * a.values, a.v.rowStride, g, column, inside, move ? 0 : count); }
         __syncthreads();
-        #pragma unroll
-        for(int i = 0; i < EACH; i++) {
-            const uint32_t item = tid + i * THREADS;
-            if(KEY_ITEMS % THREADS && item >= KEY_ITEMS) { break; }
-            if(!OUTPUTS || item < KEYS) {
-                storeRows<T, C, DK>(planes + L::keyRows, item, keyTiles[i]);
-                storeColumns<T, C, DK>(planes + L::keyColumns, item, keyTiles[i]);
-            }
-            else { storeRows<T, C, DK>(planes + L::queryRows, item - KEYS, keyTiles[i]); }
-        }
-        #pragma unroll
-        for(int i = 0; i < SQUARES; i++) {
-            const uint32_t item = tid + i * THREADS;
-            if(SQUARE % THREADS && item >= SQUARE) { break; }
-            storeSquare<C>(planes + L::correction, item, corrections[i]);
-            if(OUTPUTS) { storeSquare<C>(planes + L::score, item, scores[i]); }
-        }
-        if(tid < C) { ((float4*)table.at)[tid] = rowTable; }
+        stage.store(planes);
         __syncthreads();
-        if(n + 1 < chunks) { prefetch(n + 1); }
+        if(n + 1 < chunks) { stage.request(a, p, keyHead, first + C, min((uint32_t)C, end - first - C), at + a.heads); }
         if(!active) { continue; }
 
         // r = v - G k^ S, and the part of the outputs that the state in front has
@@ -546,17 +502,16 @@ void deltaStateKernel(DeltaArgs a)
             const Planes<3> b = split<3>(state[2 * s], state[2 * s + 1]);
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
-                const uint32_t offset = (16 * t + n16) * L::ROW + 32 * s + 8 * g;
-                x[t] = multiply(fetch<NP>(planes + L::keyRows + offset, C * L::ROW), b, x[t]);
-                if(OUTPUTS) { o[t] = multiply(fetch<NP>(planes + L::queryRows + offset, C * L::ROW), b, o[t]); }
+                x[t] = multiply(operand.rows(planes + L::keys, t, s), b, x[t]);
+                if(OUTPUTS) { o[t] = multiply(operand.rows(planes + L::queries, t, s), b, o[t]); }
             }
         }
         inTurn();
         float notFinite = 0.0f;
         #pragma unroll
         for(int t = 0; t < TILES; t++) {
-            const f32x4 keyState = table.keyState(16 * t + 4 * g);
-            if(OUTPUTS) { o[t] *= table.queryState(16 * t + 4 * g); }
+            const f32x4 keyState = table.keyState(rowIn(t, 4 * g));
+            if(OUTPUTS) { o[t] *= table.queryState(rowIn(t, 4 * g)); }
             #pragma unroll
             for(int r = 0; r < 4; r++) {
                 w[t][r] = __builtin_fmaf(-keyState[r], x[t][r], w[t][r]);
@@ -570,7 +525,7 @@ void deltaStateKernel(DeltaArgs a)
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
                 #pragma unroll
-                for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r >= bad) { w[t][r] = 0.0f; } }
+                for(int r = 0; r < 4; r++) { if(rowIn(t, 4 * g + r) >= bad) { w[t][r] = 0.0f; } }
             }
         }
         // w = r - N beta r and out += P beta w; tiles above the diagonal are zero
@@ -581,7 +536,7 @@ void deltaStateKernel(DeltaArgs a)
                 f32x4 y[2] = {w[2 * s], w[2 * s + 1]};
                 if(!FOLDED) {
                     #pragma unroll
-                    for(int h = 0; h < 2; h++) { y[h] *= table.beta(16 * (2 * s + h) + 4 * g); }
+                    for(int h = 0; h < 2; h++) { y[h] *= table.beta(rowIn(2 * s + h, 4 * g)); }
                 }
                 b[s] = split<3>(y[0], y[1]);
             }
@@ -590,9 +545,8 @@ void deltaStateKernel(DeltaArgs a)
                 inTurn();
                 #pragma unroll
                 for(int t = 2 * s; t < TILES; t++) {
-                    const uint32_t offset = (16 * t + n16) * L::COLUMN + 32 * s + 8 * g;
-                    w[t] = multiply(fetch<3>(planes + L::correction + offset, C * L::COLUMN), b[s], w[t]);
-                    if(OUTPUTS) { o[t] = multiply(fetch<3>(planes + L::score + offset, C * L::COLUMN), b[s], o[t]); }
+                    w[t] = multiply(operand.triangle(planes + L::correction, t, s), b[s], w[t]);
+                    if(OUTPUTS) { o[t] = multiply(operand.triangle(planes + L::score, t, s), b[s], o[t]); }
                 }
             }
         }
@@ -602,7 +556,7 @@ void deltaStateKernel(DeltaArgs a)
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
                 #pragma unroll
-                for(int r = 0; r < 4; r++) { if(16 * t + 4 * g + r >= bad) { w[t][r] = o[t][r] = no; } }
+                for(int r = 0; r < 4; r++) { if(rowIn(t, 4 * g + r) >= bad) { w[t][r] = o[t][r] = no; } }
             }
         }
         if(MODE == WALK_KEEP) { storeResult<float, C>(a.errors + at * C * a.padded, a.padded, g, column, true, C, w); }
@@ -615,10 +569,10 @@ void deltaStateKernel(DeltaArgs a)
             inTurn();
             f32x4 left[2];
             #pragma unroll
-            for(int h = 0; h < 2; h++) { left[h] = w[2 * s + h] * table.beta(16 * (2 * s + h) + 4 * g) * table.keyEnd(16 * (2 * s + h) + 4 * g); }
+            for(int h = 0; h < 2; h++) { left[h] = w[2 * s + h] * table.beta(rowIn(2 * s + h, 4 * g)) * table.keyEnd(rowIn(2 * s + h, 4 * g)); }
             const Planes<3> b = split<3>(left[0], left[1]);
             #pragma unroll
-            for(int t = 0; t < STATE; t++) { state[t] = multiply(fetch<NP>(planes + L::keyColumns + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, DK * L::COLUMN), b, state[t]); }
+            for(int t = 0; t < STATE; t++) { state[t] = multiply(operand.columns(planes + L::keys, t, s), b, state[t]); }
         }
         if(__builtin_expect(bad < C, 0)) {
             const float no = __builtin_nanf("");
@@ -663,7 +617,7 @@ void deltaJoinKernel(DeltaArgs a)
         for(int m = 0; m < STATE; m++) {
             #pragma unroll
             for(int t = 0; t < STATE; t++) {
-                const float4 x = *(const float4*)(move + (16 * m + n16) * DK + 16 * t + 4 * g);
+                const float4 x = *(const float4*)(move + rowIn(m, n16) * DK + rowIn(t, 4 * g));
                 next[m] = multiply(f32x4{x.x, x.y, x.z, x.w}, state[t], next[m]);
             }
         }
@@ -682,46 +636,17 @@ struct DeltaGradientArgs
     float *states, *errors;         // the gradient of the state behind each chunk [DK][padded], dR [C][padded]
     float *shared;                  // where heads share keys: each one's gradients of unit queries and keys, [2][C][DK]
 };
-template<typename T, int C, int DK> struct ReverseLayout
-{
-    static constexpr int NP = planesOf<T>, ROW = DK + 8, COLUMN = C + 8;
-    static constexpr uint32_t keyRows = 0, keyColumns = keyRows + NP * C * ROW, queryColumns = keyColumns + NP * DK * COLUMN, correction = queryColumns + NP * DK * COLUMN,
-        score = correction + 3 * C * COLUMN, table = (score + 3 * C * COLUMN + 7) / 8 * 8, bytes = table * 2 + C * 16;
-};
-// Four rows and four columns of a square, stored by column
-struct SquareTile { float4 x[4]; };
-template<int C> __device__ inline void loadSquareTile(const float *from, uint32_t item, SquareTile &tile)
-{
-    const uint32_t row = item / (C / 4) * 4, at = item % (C / 4) * 4;
-    #pragma unroll
-    for(int i = 0; i < 4; i++) { tile.x[i] = *(const float4*)(from + (row + i) * C + at); }
-}
-template<int C> __device__ inline void storeSquareColumns(uint16_t *to, uint32_t item, const SquareTile &tile)
-{
-    constexpr int PITCH = C + 8;
-    const uint32_t row = item / (C / 4) * 4, at = item % (C / 4) * 4;
-    #pragma unroll
-    for(int e = 0; e < 4; e++) {
-        const auto part = [&](const float4 &x) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
-        const float f[4] = {part(tile.x[0]), part(tile.x[1]), part(tile.x[2]), part(tile.x[3])};
-        uint2 words[3];
-        splitFour<3>(f, words);
-        #pragma unroll
-        for(int k = 0; k < 3; k++) { *(uint2*)(to + k * C * PITCH + (at + e) * PITCH + place(row)) = words[k]; }
-    }
-}
-
-template<typename T, int C, int DK, int WAVES>
-__global__ __launch_bounds__(64 * WAVES)
+template<typename T, int C, int DK>
+__global__ __launch_bounds__(WALK_THREADS, 2)
 void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
 {
-    typedef ReverseLayout<T, C, DK> L;
-    constexpr int NP = planesOf<T>, THREADS = 64 * WAVES, TILES = C / 16, STATE = DK / 16;
-    constexpr int KEYS = C * DK / 32, KEY_ITEMS = 2 * KEYS, EACH = (KEY_ITEMS + THREADS - 1) / THREADS, SQUARE = C * C / 16, SQUARE_ITEMS = 2 * SQUARE, SQUARES = (SQUARE_ITEMS + THREADS - 1) / THREADS;
+    typedef WalkLayout<T, C, DK, true> L;
+    constexpr int NP = planesOf<T>, TILES = C / 16, STATE = DK / 16, WAVES = WALK_THREADS / 64;
     extern __shared__ __align__(16) char lds[];
     uint16_t *const planes = (uint16_t*)lds;
     const RowFactors<C> table{(float*)(planes + L::table)};
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
+    const WalkOperands<T, C, DK> operand{n16, g};
     const uint32_t block = blockIdx.x % a.columnBlocks, rest = blockIdx.x / a.columnBlocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
     Place p;
     if(!locate(a.segments, segment, p)) { return; }
@@ -735,28 +660,8 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
     #pragma unroll
     for(int t = 0; t < STATE; t++) { state[t] = f32x4{0, 0, 0, 0}; }
     if(d.finalState) { loadResult<float, DK>(d.finalState + ((uint64_t)p.sequence * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
-    KeyTile<T> keyTiles[EACH];
-    SquareTile squares[SQUARES];
-    float4 rowTable;
-    const auto prefetch = [&](uint32_t n) {
-        const uint32_t first = begin + n * C, count = min((uint32_t)C, end - first);
-        const uint64_t at = (firstNumber + n) * a.heads + head;
-        #pragma unroll
-        for(int i = 0; i < EACH; i++) {
-            const uint32_t item = tid + i * THREADS;
-            if(KEY_ITEMS % THREADS && item >= KEY_ITEMS) { break; }
-            if(item < KEYS) { loadTile<T, C, DK>(a, a.k, p, keyHead, first, count, item, keyTiles[i]); }
-            else { loadTile<T, C, DK>(a, a.q, p, keyHead, first, count, item - KEYS, keyTiles[i]); }
-        }
-        #pragma unroll
-        for(int i = 0; i < SQUARES; i++) {
-            const uint32_t item = tid + i * THREADS;
-            if(SQUARE_ITEMS % THREADS && item >= SQUARE_ITEMS) { break; }
-            loadSquareTile<C>((item < SQUARE ? a.correction : a.score) + at * C * C, item < SQUARE ? item : item - SQUARE, squares[i]);
-        }
-        if(tid < C) { rowTable = ((const float4*)((const RowTable<C>*)a.rows + at))[tid]; }
-    };
-    if(chunks) { prefetch(chunks - 1); }
+    WalkStage<T, C, DK, true> stage;
+    if(chunks) { const uint32_t last = begin + (chunks - 1) * C; stage.request(a, p, keyHead, last, end - last, (firstNumber + chunks - 1) * a.heads + head); }
     for(uint32_t left = chunks; left > 0; left--) {
         const uint32_t n = left - 1, first = begin + n * C, count = min((uint32_t)C, end - first);
         const uint64_t at = (firstNumber + n) * a.heads + head;
@@ -764,25 +669,9 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
         Result<T, TILES> douts;
         if(active) { douts = requestResult<T, TILES>(rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)first * d.out.rowStride + head * a.values, d.out.rowStride, g, column, inside, count); }
         __syncthreads();
-        #pragma unroll
-        for(int i = 0; i < EACH; i++) {
-            const uint32_t item = tid + i * THREADS;
-            if(KEY_ITEMS % THREADS && item >= KEY_ITEMS) { break; }
-            if(item < KEYS) {
-                storeRows<T, C, DK>(planes + L::keyRows, item, keyTiles[i]);
-                storeColumns<T, C, DK>(planes + L::keyColumns, item, keyTiles[i]);
-            }
-            else { storeColumns<T, C, DK>(planes + L::queryColumns, item - KEYS, keyTiles[i]); }
-        }
-        #pragma unroll
-        for(int i = 0; i < SQUARES; i++) {
-            const uint32_t item = tid + i * THREADS;
-            if(SQUARE_ITEMS % THREADS && item >= SQUARE_ITEMS) { break; }
-            storeSquareColumns<C>(planes + (item < SQUARE ? L::correction : L::score), item < SQUARE ? item : item - SQUARE, squares[i]);
-        }
-        if(tid < C) { ((float4*)table.at)[tid] = rowTable; }
+        stage.store(planes);
         __syncthreads();
-        if(n > 0) { prefetch(n - 1); }
+        if(n > 0) { stage.request(a, p, keyHead, first - C, C, at - a.heads); }
         if(!active) { continue; }
 
         f32x4 dout[TILES], du[TILES];
@@ -796,18 +685,18 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             inTurn();
             const Planes<3> b = split<3>(state[2 * s], state[2 * s + 1]);
             #pragma unroll
-            for(int t = 0; t < TILES; t++) { du[t] = multiply(fetch<NP>(planes + L::keyRows + (16 * t + n16) * L::ROW + 32 * s + 8 * g, C * L::ROW), b, du[t]); }
+            for(int t = 0; t < TILES; t++) { du[t] = multiply(operand.rows(planes + L::keys, t, s), b, du[t]); }
         }
         #pragma unroll
         for(int t = 0; t < TILES; t++) {
-            du[t] *= table.keyEnd(16 * t + 4 * g);
+            du[t] *= table.keyEnd(rowIn(t, 4 * g));
         }
         #pragma unroll
         for(int s = 0; s < TILES / 2; s++) {
             inTurn();
             const Planes<NP> b = split<NP>(dout[2 * s], dout[2 * s + 1]);
             #pragma unroll
-            for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(fetch<3>(planes + L::score + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, du[t]); }
+            for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(operand.triangleColumns(planes + L::score, t, s), b, du[t]); }
         }
         // dR = dU - N' beta dU
         {
@@ -817,14 +706,14 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
                 inTurn();
                 f32x4 y[2];
                 #pragma unroll
-                for(int h = 0; h < 2; h++) { y[h] = du[2 * s + h] * table.beta(16 * (2 * s + h) + 4 * g); }
+                for(int h = 0; h < 2; h++) { y[h] = du[2 * s + h] * table.beta(rowIn(2 * s + h, 4 * g)); }
                 b[s] = split<3>(y[0], y[1]);
             }
             #pragma unroll
             for(int s = 0; s < TILES / 2; s++) {
                 inTurn();
                 #pragma unroll
-                for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(fetch<3>(planes + L::correction + (16 * t + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b[s], du[t]); }
+                for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(operand.triangleColumns(planes + L::correction, t, s), b[s], du[t]); }
             }
         }
         storeResult<float, C>(d.errors + at * C * a.padded, a.padded, g, column, true, C, du);
@@ -837,7 +726,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             f32x4 x[2], y[2];
             #pragma unroll
             for(int h = 0; h < 2; h++) {
-                const uint32_t row = 16 * (2 * s + h) + 4 * g;
+                const uint32_t row = rowIn(2 * s + h, 4 * g);
                 x[h] = dout[2 * s + h] * table.queryState(row);
                 du[2 * s + h] *= table.beta(row);
                 y[h] = -table.keyState(row) * du[2 * s + h];
@@ -845,9 +734,8 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             const Planes<3> bx = split<3>(x[0], x[1]), by = split<3>(y[0], y[1]);
             #pragma unroll
             for(int t = 0; t < STATE; t++) {
-                const uint32_t offset = (16 * t + n16) * L::COLUMN + 32 * s + 8 * g;
-                state[t] = multiply(fetch<NP>(planes + L::queryColumns + offset, DK * L::COLUMN), bx, state[t]);
-                state[t] = multiply(fetch<NP>(planes + L::keyColumns + offset, DK * L::COLUMN), by, state[t]);
+                state[t] = multiply(operand.columns(planes + L::queries, t, s), bx, state[t]);
+                state[t] = multiply(operand.columns(planes + L::keys, t, s), by, state[t]);
             }
         }
         if(d.v.data) { storeResult<T, C>(rowsOf<T>(d.v, a.chunks, p) + (uint64_t)first * d.v.rowStride + head * a.values, d.v.rowStride, g, column, inside, count, du); }
@@ -866,9 +754,9 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
 // deltaSharedKernel to add up.
 template<typename T, int C, int DK> struct GradientLayout
 {
-    static constexpr int NP = planesOf<T>, COLUMN = C + 8, VALUES = 40;
-    static constexpr uint32_t keyColumns = 0, queryColumns = keyColumns + NP * DK * COLUMN, stage = queryColumns + NP * DK * COLUMN,
-        staged = (NP + 6) * C * VALUES, square = 3 * C * COLUMN, floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (6 + 2 * 8) + 64;
+    static constexpr int NP = planesOf<T>;
+    static constexpr uint32_t keys = 0, queries = keys + NP * C * DK, stage = queries + NP * C * DK, staged = (NP + 6) * C * 32, square = 3 * C * C,
+        floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (6 + 2 * 8) + 64;
 };
 
 template<typename T, int C, int DK>
@@ -876,7 +764,7 @@ __global__ __launch_bounds__(512)
 void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
 {
     typedef GradientLayout<T, C, DK> L;
-    constexpr int NP = planesOf<T>, TILES = C / 16, KEY_TILES = DK / 16, SPLIT = 8 / KEY_TILES, MINE = TILES / SPLIT, SQUARES = C == 64 ? 2 : 1, KEYS = C * DK / 32, VP = C * L::VALUES;
+    constexpr int NP = planesOf<T>, TILES = C / 16, KEY_TILES = DK / 16, SPLIT = 8 / KEY_TILES, MINE = TILES / SPLIT, SQUARES = C == 64 ? 2 : 1, UNITS = C * DK / 8, VP = C * 32;
     extern __shared__ __align__(16) char lds[];
     uint16_t *const planes = (uint16_t*)lds, *const stage = planes + L::stage;
     uint16_t *const doutPlanes = stage, *const dRPlanes = stage + NP * VP, *const wPlanes = dRPlanes + 3 * VP;
@@ -933,22 +821,12 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     request(0);
 
     #pragma unroll
-    for(int i = 0; i < (2 * KEYS + 511) / 512; i++) {
-        const uint32_t item = tid + i * 512;
-        if(2 * KEYS % 512 && item >= 2 * KEYS) { break; }
-        KeyTile<T> tile;
-        const bool isKey = item < KEYS;
-        const uint32_t it = isKey ? item : item - KEYS, row = it / (DK / 8) * 4, column = it % (DK / 8) * 8;
-        loadTile<T, C, DK>(a, isKey ? a.k : a.q, p, keyHead, begin, count, it, tile);
-        // (rows in their order here)
-        uint16_t *const to = planes + (isKey ? L::keyColumns : L::queryColumns);
-        #pragma unroll
-        for(int e = 0; e < 8; e++) {
-            uint2 words[NP];
-            columnOf<T>(tile, e, words);
-            #pragma unroll
-            for(int k = 0; k < NP; k++) { *(uint2*)(to + k * DK * L::COLUMN + (column + e) * L::COLUMN + row) = words[k]; }
-        }
+    for(int i = 0; i < 2 * UNITS / 512; i++) {
+        const uint32_t item = (tid + i * 512) % UNITS, row = item / (DK / 8), column = item % (DK / 8) * 8, valid = row < count && column < a.keys ? min(8u, a.keys - column) : 0;
+        const bool isKey = tid + i * 512 < UNITS;
+        const gennmi_rows_t &r = isKey ? a.k : a.q;
+        const Eight<T> x = loadEight(rowAt<T>(r, a.chunks, p, valid ? begin + row : 0) + (valid ? keyHead * a.keys + column : 0), valid, a.wide);
+        storeUnit(planes + (isKey ? L::keys : L::queries) + unitAt<DK>(row, column / 8), C * DK, x);
     }
     const float decay = a.table[at].decay;
     if(tid < C) {
@@ -966,7 +844,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         f32x4 x = {0, 0, 0, 0};
         #pragma unroll
         for(int k = 0; k < NP; k++) {
-            const uint2 w = *(const uint2*)(planes + from + k * DK * L::COLUMN + key * L::COLUMN + tile * 16 + 4 * g);
+            const uint2 w = readColumn(planes + from + k * C * DK + unitAt<DK>(tile * 16 + 4 * g + n16 / 4, 2 * keyTile + n16 % 4 / 2) + n16 % 2 * 4);
             x[0] += __uint_as_float(w.x << 16); x[1] += __uint_as_float(w.x & 0xffff0000u);
             x[2] += __uint_as_float(w.y << 16); x[3] += __uint_as_float(w.y & 0xffff0000u);
         }
@@ -995,7 +873,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
                 betaDot = __builtin_fmaf(w[e], dr[e], betaDot);
             }
             uint2 words[3], own[NP];
-            uint16_t *const to = stage + stageRow * L::VALUES + stageAt;
+            uint16_t *const to = stage + unitAt<32>(stageRow, stageAt / 8) + stageAt % 8;
             splitFour<NP>(dout, own);
             #pragma unroll
             for(int k = 0; k < NP; k++) { *(uint2*)(to + k * VP) = own[k]; }
@@ -1014,18 +892,18 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         #pragma unroll
         for(int m = 0; m < MINE; m++) {
             inTurn();
-            const uint32_t offset = (tileOf(m) * 16 + n16) * L::VALUES + 8 * g;
+            const uint32_t offset = unitAt<32>(tileOf(m) * 16 + n16, g);
             dq[m] = multiply(fetch<NP>(doutPlanes + offset, VP), state, dq[m]);
             rS[m] = multiply(fetch<3>(dRPlanes + offset, VP), state, rS[m]);
             dk[m] = multiply(fetch<3>(wPlanes + offset, VP), dState, dk[m]);
         }
         if(squares) {
-            const Planes<3> other = fetch<3>(wPlanes + (squareColumn * 16 + n16) * L::VALUES + 8 * g, VP);
+            const Planes<3> other = fetch<3>(wPlanes + unitAt<32>(squareColumn * 16 + n16, g), VP);
             #pragma unroll
             for(int q = 0; q < SQUARES; q++) {
                 inTurn();
                 if(squareRow(q) < squareColumn) { continue; }
-                const uint32_t offset = (squareRow(q) * 16 + n16) * L::VALUES + 8 * g;
+                const uint32_t offset = unitAt<32>(squareRow(q) * 16 + n16, g);
                 dqk[q] = multiply(fetch<NP>(doutPlanes + offset, VP), other, dqk[q]);
                 dkk[q] = multiply(fetch<3>(dRPlanes + offset, VP), other, dkk[q]);
             }
@@ -1037,7 +915,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     #pragma unroll
     for(int m = 0; m < MINE; m++) {
         const uint32_t tile = tileOf(m);
-        const f32x4 q = valuesAt(L::queryColumns, tile) * fourRows(queryUnit, tile), k = valuesAt(L::keyColumns, tile) * fourRows(keyUnit, tile);
+        const f32x4 q = valuesAt(L::queries, tile) * fourRows(queryUnit, tile), k = valuesAt(L::keys, tile) * fourRows(keyUnit, tile);
         const f32x4 grown = fourRows(since, tile), by = fourRows(beta, tile);
         dq[m] *= a.scale * grown;
         dk[m] *= fourRows(until, tile) * by;
@@ -1119,11 +997,13 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             splitFour<3>(x, words);
             #pragma unroll
             for(int k = 0; k < 3; k++) {
-                if(transposed) { *(uint2*)(stage + (k * C + column) * L::COLUMN + row) = words[k]; }
+                uint16_t *const to = stage + k * C * C;
+                if(transposed) { *(uint2*)(to + unitAt<C>(column, row / 8) + row % 8) = words[k]; }
                 else {
-                    uint16_t *const to = stage + (k * C + row) * L::COLUMN + column;
-                    to[0] = (uint16_t)words[k].x; to[L::COLUMN] = (uint16_t)(words[k].x >> 16);
-                    to[2 * L::COLUMN] = (uint16_t)words[k].y; to[3 * L::COLUMN] = (uint16_t)(words[k].y >> 16);
+                    to[unitAt<C>(row, column / 8) + column % 8] = (uint16_t)words[k].x;
+                    to[unitAt<C>(row + 1, column / 8) + column % 8] = (uint16_t)(words[k].x >> 16);
+                    to[unitAt<C>(row + 2, column / 8) + column % 8] = (uint16_t)words[k].y;
+                    to[unitAt<C>(row + 3, column / 8) + column % 8] = (uint16_t)(words[k].y >> 16);
                 }
             }
         }
@@ -1131,26 +1011,27 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     const auto timesColumns = [&](uint32_t from, f32x4 (&to)[MINE]) {
         #pragma unroll
         for(int s = 0; s < TILES / 2; s++) {
-            const Planes<NP> b = fetch<NP>(planes + from + key * L::COLUMN + 32 * s + 8 * g, DK * L::COLUMN);
+            const uint32_t row = 32 * s + 8 * g + n16 / 4, unit = 2 * keyTile + n16 % 4 / 2, half = n16 % 2 * 4;
+            const Planes<NP> b = fetchColumn<NP>(planes + from + unitAt<DK>(row, unit) + half, planes + from + unitAt<DK>(row + 4, unit) + half, C * DK);
             #pragma unroll
-            for(int m = 0; m < MINE; m++) { inTurn(); to[m] = multiply(fetch<3>(stage + (tileOf(m) * 16 + n16) * L::COLUMN + 32 * s + 8 * g, C * L::COLUMN), b, to[m]); }
+            for(int m = 0; m < MINE; m++) { inTurn(); to[m] = multiply(fetch<3>(stage + unitAt<C>(tileOf(m) * 16 + n16, 4 * s + g), C * C), b, to[m]); }
         }
     };
     storeSquares(false, dqk, nullptr, keyUnit);
     __syncthreads();
-    timesColumns(L::keyColumns, dq);
+    timesColumns(L::keys, dq);
     __syncthreads();
     storeSquares(true, dqk, queryUnit, nullptr);
     __syncthreads();
-    timesColumns(L::queryColumns, dk);
+    timesColumns(L::queries, dk);
     __syncthreads();
     storeSquares(false, dkk, nullptr, keyUnit);
     __syncthreads();
-    timesColumns(L::keyColumns, dk);
+    timesColumns(L::keys, dk);
     __syncthreads();
     storeSquares(true, dkk, keyUnit, nullptr);
     __syncthreads();
-    timesColumns(L::keyColumns, dk);
+    timesColumns(L::keys, dk);
     if(a.group > 1) {
         float *const to = d.shared + at * 2 * C * DK;
         storeResultTiles<MINE, SPLIT>(to, DK, firstRow, g, key, dq);
@@ -1162,7 +1043,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     if(a.normalise) {
         #pragma unroll
         for(int m = 0; m < MINE; m++) {
-            const f32x4 q = valuesAt(L::queryColumns, tileOf(m)) * fourRows(queryUnit, tileOf(m)), k = valuesAt(L::keyColumns, tileOf(m)) * fourRows(keyUnit, tileOf(m));
+            const f32x4 q = valuesAt(L::queries, tileOf(m)) * fourRows(queryUnit, tileOf(m)), k = valuesAt(L::keys, tileOf(m)) * fourRows(keyUnit, tileOf(m));
             #pragma unroll
             for(int r = 0; r < 4; r++) {
                 const float x = sumOf16(q[r] * dq[m][r]), y = sumOf16(k[r] * dk[m][r]);
@@ -1183,8 +1064,8 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
                 queryDot += fourRows(queryDots + (firstRow * KEY_TILES + w) * C, tile);
                 keyDot += fourRows(keyDots + (firstRow * KEY_TILES + w) * C, tile);
             }
-            x -= valuesAt(L::queryColumns, tile) * queryLength * queryDot;
-            y -= valuesAt(L::keyColumns, tile) * keyLength * keyDot;
+            x -= valuesAt(L::queries, tile) * queryLength * queryDot;
+            y -= valuesAt(L::keys, tile) * keyLength * keyDot;
         }
         x *= queryLength;
         y *= keyLength;

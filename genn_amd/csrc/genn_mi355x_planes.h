@@ -47,7 +47,7 @@ template<int N> __device__ inline void splitFour(const float (&x)[4], uint2 (&ou
     #pragma unroll
     for(int p = 0; p < N; p++) { out[p] = make_uint2(low[p], high[p]); }
 }
-// Eight values of one lane: those of two tiles of a result, one below the other, that becomes an operand (see place())
+// Eight values of one lane, four of each of two tiles of a result, which become an operand: see rowIn()
 template<int N> __device__ inline Planes<N> split(const f32x4 &a, const f32x4 &b)
 {
     Planes<N> out;
@@ -61,12 +61,21 @@ template<int N> __device__ inline Planes<N> split(const f32x4 &a, const f32x4 &b
     }
     return out;
 }
-// A lane of a result tile has the rows 4 (lane / 16) + 0 .. 3 of the column lane % 16.  As an operand that is summed over those rows, two tiles are taken
-// together, and a lane's eight values are rows 4 g .. 4 g + 3 of either (g = lane / 16).  The other operand lies in memory in that order:
-// element i of 32 at place(i).
-__device__ inline uint32_t place(uint32_t i) { return (i & ~31u) + 8 * ((i >> 2) & 3) + 4 * ((i >> 4) & 1) + (i & 3); }
+// A lane of a result tile has rows 4 (lane / 16) + 0 .. 3 of it, column lane % 16; an operand's lane has eight neighbours (8 (lane / 16) + 0 .. 7) along the axis that
+// is summed over.  So that results become operands where they are, two tiles t, t + 1 (t even) hold 32 rows in this order: row i of tile t is row
+// 8 (i / 4) + 4 (t % 2) + i % 4 of them.  A lane's eight values of both are neighbours then.
+__device__ inline uint32_t rowIn(uint32_t t, uint32_t i) { return 32 * (t / 2) + 8 * (i / 4) + 4 * (t % 2) + i % 4; }
 
-// From LDS, planes `stride` elements apart; 16-byte aligned
+// Rows of WIDTH elements of 16 bits in LDS without a gap, units of 16 bytes in an order that differs from row to row, so that neither reads of a unit from 8 rows
+// in that order, two a row, nor reads of four elements from each of four rows meet in a bank (64 of 4 bytes: 16 units).
+template<int WIDTH> __device__ inline uint32_t unitAt(uint32_t row, uint32_t unit)
+{
+    constexpr int UNITS = WIDTH / 8;
+    static_assert(UNITS == 4 || UNITS == 8 || UNITS == 16, "");
+    const uint32_t turn = (UNITS == 16 ? (row & 3) << 2 : UNITS == 8 ? (row & 2) << 1 : 0) | ((row >> 2) & 2);
+    return row * WIDTH + ((unit ^ turn) << 3);
+}
+// One unit of every plane
 template<int N> __device__ inline Planes<N> fetch(const uint16_t *at, uint32_t stride)
 {
     Planes<N> out;
@@ -74,6 +83,25 @@ template<int N> __device__ inline Planes<N> fetch(const uint16_t *at, uint32_t s
     for(int p = 0; p < N; p++) {
         const uint4 w = *(const uint4*)(at + p * stride);
         out.plane[p].word[0] = w.x; out.plane[p].word[1] = w.y; out.plane[p].word[2] = w.z; out.plane[p].word[3] = w.w;
+    }
+    return out;
+}
+// Four neighbouring rows of one column.  The lanes of a quarter of the wavefront each name four neighbours of a row, lane l those that begin at column 4 (l % 4) of row l / 4; lane l gets
+// column l of the four rows.
+__device__ inline uint2 readColumn(const uint16_t *at)
+{
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+    return __builtin_bit_cast(uint2, x);
+}
+// Eight neighbouring rows of one column of every plane: `first` names rows 0 .. 3 of them, `second` rows 4 .. 7
+template<int N> __device__ inline Planes<N> fetchColumn(const uint16_t *first, const uint16_t *second, uint32_t stride)
+{
+    Planes<N> out;
+    #pragma unroll
+    for(int p = 0; p < N; p++) {
+        const uint2 a = readColumn(first + p * stride), b = readColumn(second + p * stride);
+        out.plane[p].word[0] = a.x; out.plane[p].word[1] = a.y; out.plane[p].word[2] = b.x; out.plane[p].word[3] = b.y;
     }
     return out;
 }
@@ -131,6 +159,22 @@ template<typename T> __device__ inline Eight<T> loadEight(const T *at, uint32_t 
     #pragma unroll
     for(int h = 0; h < (int)sizeof(T) / 2; h++) { out.word[h] = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]); }
     return out;
+}
+// A unit of every plane
+template<typename T> __device__ inline void storeUnit(uint16_t *to, uint32_t stride, const Eight<T> &x)
+{
+    constexpr int N = planesOf<T>;
+    if constexpr(N == 1) { *(uint4*)to = x.word[0]; }
+    else {
+        float low[4], high[4];
+        #pragma unroll
+        for(int e = 0; e < 4; e++) { low[e] = gennmi_elements::widen(x.at(e)); high[e] = gennmi_elements::widen(x.at(4 + e)); }
+        uint2 a[N], b[N];
+        splitFour<N>(low, a);
+        splitFour<N>(high, b);
+        #pragma unroll
+        for(int p = 0; p < N; p++) { *(uint4*)(to + p * stride) = make_uint4(a[p].x, a[p].y, b[p].x, b[p].y); }
+    }
 }
 }
 
