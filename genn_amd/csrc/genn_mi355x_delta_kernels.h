@@ -40,7 +40,7 @@ template<int C> struct alignas(16) RowTable
 template<int C> struct RowFactors
 {
     float *at;
-    __device__ f32x4 four(int which, uint32_t row) const { const float4 x = *(const float4*)(at + which * C + row); return f32x4{x.x, x.y, x.z, x.w}; }
+    __device__ f32x4 four(int which, uint32_t row) const { return *(const f32x4*)(at + which * C + row); }
     __device__ f32x4 keyState(uint32_t row) const { return four(0, row); }
     __device__ f32x4 beta(uint32_t row) const { return four(1, row); }
     __device__ f32x4 keyEnd(uint32_t row) const { return four(2, row); }
@@ -105,7 +105,7 @@ void deltaChunkKernel(DeltaArgs a)
         #pragma unroll
         for(int which = 0; which < 2; which++) {
             const gennmi_rows_t &r = which ? a.q : a.k;
-            const Eight<T> x = loadEight(rowAt<T>(r, a.chunks, p, valid ? begin + row : 0) + (valid ? keyHead * a.keys + at : 0), valid, a.wide);
+            const Eight<T> x = loadUnit(rowAt<T>(r, a.chunks, p, valid ? begin + row : begin) + (valid ? keyHead * a.keys + at : 0), valid, a.wide);
             float sum = 0.0f;
             #pragma unroll
             for(int e = 0; e < 8; e++) { const float f = widen(x.at(e)); sum = __builtin_fmaf(f, f, sum); }
@@ -291,28 +291,41 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
     typedef WalkLayout<T, C, DK, QUERIES> L;
     static constexpr int EACH = C * DK / 8 / WALK_THREADS, SQUARES = Triangle<C>::items / WALK_THREADS;
     Eight<T> keys[EACH], queries[QUERIES ? EACH : 1];
-    float4 corrections[SQUARES], scores[QUERIES ? SQUARES : 1], rows;
+    f32x4 corrections[SQUARES], scores[QUERIES ? SQUARES : 1], rows;
 
+    __device__ static uint32_t rowOf(int i) { return (threadIdx.x + i * WALK_THREADS) / (DK / 8); }
+    __device__ static uint32_t columnOf(int i) { return (threadIdx.x + i * WALK_THREADS) % (DK / 8) * 8; }
+    // Units that are not there are asked for at another place, and become zero in store(): no branch a unit, with which the compiler would wait for each
     __device__ void request(const DeltaArgs &a, const Place &p, uint32_t keyHead, uint32_t first, uint32_t count, uint64_t at)
     {
         const T *const key = rowsOf<const T>(a.k, a.chunks, p) + (uint64_t)first * a.k.rowStride + keyHead * a.keys, *const query = rowsOf<const T>(a.q, a.chunks, p) + (uint64_t)first * a.q.rowStride + keyHead * a.keys;
-        #pragma unroll
-        for(int i = 0; i < EACH; i++) {
-            const uint32_t item = threadIdx.x + i * WALK_THREADS, row = item / (DK / 8), column = item % (DK / 8) * 8, valid = row < count && column < a.keys ? min(8u, a.keys - column) : 0;
-            keys[i] = loadEight(key + (valid ? row * a.k.rowStride + column : 0), valid, a.wide);
-            if(QUERIES) { queries[i] = loadEight(query + (valid ? row * a.q.rowStride + column : 0), valid, a.wide); }
+        if(a.wide) {
+            #pragma unroll
+            for(int i = 0; i < EACH; i++) {
+                const uint32_t row = min(rowOf(i), count - 1), column = columnOf(i) < a.keys ? columnOf(i) : 0;
+                keys[i] = *(const Eight<T>*)(key + row * a.k.rowStride + column);
+                if(QUERIES) { queries[i] = *(const Eight<T>*)(query + row * a.q.rowStride + column); }
+            }
+        }
+        else {
+            #pragma unroll
+            for(int i = 0; i < EACH; i++) {
+                const uint32_t row = min(rowOf(i), count - 1), valid = columnOf(i) < a.keys ? min(8u, a.keys - columnOf(i)) : 0;
+                keys[i] = loadEight(key + row * a.k.rowStride + columnOf(i), valid);
+                if(QUERIES) { queries[i] = loadEight(query + row * a.q.rowStride + columnOf(i), valid); }
+            }
         }
         #pragma unroll
         for(int i = 0; i < SQUARES; i++) {
             const uint32_t item = threadIdx.x + i * WALK_THREADS, offset = Triangle<C>::row(item) * C + Triangle<C>::column(item);
-            corrections[i] = *(const float4*)(a.correction + at * C * C + offset);
-            if(QUERIES) { scores[i] = *(const float4*)(a.score + at * C * C + offset); }
+            corrections[i] = *(const f32x4*)(a.correction + at * C * C + offset);
+            if(QUERIES) { scores[i] = *(const f32x4*)(a.score + at * C * C + offset); }
         }
-        if(threadIdx.x < C) { rows = ((const float4*)((const RowTable<C>*)a.rows + at))[threadIdx.x]; }
+        if(threadIdx.x < C) { rows = ((const f32x4*)((const RowTable<C>*)a.rows + at))[threadIdx.x]; }
     }
-    __device__ static void storeSquare(uint16_t *to, uint32_t item, const float4 &x)
+    __device__ static void storeSquare(uint16_t *to, uint32_t item, const f32x4 &x)
     {
-        const float f[4] = {x.x, x.y, x.z, x.w};
+        const float f[4] = {x[0], x[1], x[2], x[3]};
         uint2 words[3];
         splitFour<3>(f, words);
         const uint32_t column = Triangle<C>::column(item);
@@ -320,11 +333,19 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
         #pragma unroll
         for(int k = 0; k < 3; k++) { *(uint2*)(to + k * Triangle<C>::elements) = words[k]; }
     }
-    __device__ void store(uint16_t *planes) const
+    __device__ void store(const DeltaArgs &a, uint16_t *planes, uint32_t count)
     {
+        if(count < C || a.keys <= DK - 8) {
+            #pragma unroll
+            for(int i = 0; i < EACH; i++) {
+                if(rowOf(i) < count && columnOf(i) < a.keys) { continue; }
+                keys[i] = Eight<T>{};
+                if(QUERIES) { queries[i] = Eight<T>{}; }
+            }
+        }
         #pragma unroll
         for(int i = 0; i < EACH; i++) {
-            const uint32_t item = threadIdx.x + i * WALK_THREADS, to = unitAt<DK>(item / (DK / 8), item % (DK / 8));
+            const uint32_t to = unitAt<DK>(rowOf(i), columnOf(i) / 8);
             storeUnit(planes + L::keys + to, C * DK, keys[i]);
             if(QUERIES) { storeUnit(planes + L::queries + to, C * DK, queries[i]); }
         }
@@ -333,7 +354,7 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
             storeSquare(planes + L::correction, threadIdx.x + i * WALK_THREADS, corrections[i]);
             if(QUERIES) { storeSquare(planes + L::score, threadIdx.x + i * WALK_THREADS, scores[i]); }
         }
-        if(threadIdx.x < C) { ((float4*)(planes + L::table))[threadIdx.x] = rows; }
+        if(threadIdx.x < C) { ((f32x4*)(planes + L::table))[threadIdx.x] = rows; }
     }
 };
 // Operands of a walk.  Tile t of a result has rows in the order of rowIn(): of keys (or queries, of the chunk's rows), times what is summed over keys 32 s ..; of a triangle, summed over
@@ -442,7 +463,7 @@ void deltaStateKernel(DeltaArgs a)
 {
     constexpr bool OUTPUTS = MODE == WALK_OUTPUTS;
     typedef WalkLayout<T, C, DK, OUTPUTS> L;
-    constexpr int TILES = C / 16, STATE = DK / 16, WAVES = WALK_THREADS / 64;
+    constexpr int NP = planesOf<T>, TILES = C / 16, STATE = DK / 16, WAVES = WALK_THREADS / 64;
     extern __shared__ __align__(16) char lds[];
     uint16_t *const planes = (uint16_t*)lds;
     const RowFactors<C> table{(float*)(planes + L::table)};
@@ -485,33 +506,32 @@ void deltaStateKernel(DeltaArgs a)
         Result<T, TILES> values;
         if(active) { values = requestResult<T, TILES>(rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)first * a.v.rowStride + head * a.values, a.v.rowStride, g, column, inside, move ? 0 : count); }
         __syncthreads();
-        stage.store(planes);
+        stage.store(a, planes, count);
         __syncthreads();
         if(n + 1 < chunks) { stage.request(a, p, keyHead, first + C, min((uint32_t)C, end - first - C), at + a.heads); }
         if(!active) { continue; }
 
-        // r = v - G k^ S, and the part of the outputs that the state in front has
-        f32x4 w[TILES], x[TILES], o[TILES];
-        takeResult(values, inside, w);
+        // r = v - G k^ S, and the part of the outputs that the state in front has: x's first tiles and the others
+        constexpr int ROWS = OUTPUTS ? 2 * TILES : TILES;
+        f32x4 w[TILES], x[ROWS];
         if(MODE == WALK_KEEP) { storeResult<float, DK>(a.states + at * DK * a.padded, a.padded, g, column, true, DK, state); }
         #pragma unroll
-        for(int t = 0; t < TILES; t++) { x[t] = o[t] = f32x4{0, 0, 0, 0}; }
+        for(int t = 0; t < ROWS; t++) { x[t] = f32x4{0, 0, 0, 0}; }
         #pragma unroll
         for(int s = 0; s < DK / 32; s++) {
             inTurn();
-            const Planes<3> b = split<3>(state[2 * s], state[2 * s + 1]);
+            Planes<NP> rows[ROWS];
             #pragma unroll
-            for(int t = 0; t < TILES; t++) {
-                x[t] = multiply(operand.rows(planes + L::keys, t, s), b, x[t]);
-                if(OUTPUTS) { o[t] = multiply(operand.rows(planes + L::queries, t, s), b, o[t]); }
-            }
+            for(int t = 0; t < ROWS; t++) { rows[t] = operand.rows(planes + (t < TILES ? L::keys : L::queries), t % TILES, s); }
+            multiplyAll(rows, split<3>(state[2 * s], state[2 * s + 1]), x);
         }
         inTurn();
+        takeResult(values, inside, w);
         float notFinite = 0.0f;
         #pragma unroll
         for(int t = 0; t < TILES; t++) {
             const f32x4 keyState = table.keyState(rowIn(t, 4 * g));
-            if(OUTPUTS) { o[t] *= table.queryState(rowIn(t, 4 * g)); }
+            if(OUTPUTS) { x[TILES + t] *= table.queryState(rowIn(t, 4 * g)); }
             #pragma unroll
             for(int r = 0; r < 4; r++) {
                 w[t][r] = __builtin_fmaf(-keyState[r], x[t][r], w[t][r]);
@@ -542,11 +562,20 @@ void deltaStateKernel(DeltaArgs a)
             }
             #pragma unroll
             for(int s = 0; s < TILES / 2; s++) {
-                inTurn();
                 #pragma unroll
-                for(int t = 2 * s; t < TILES; t++) {
-                    w[t] = multiply(operand.triangle(planes + L::correction, t, s), b[s], w[t]);
-                    if(OUTPUTS) { o[t] = multiply(operand.triangle(planes + L::score, t, s), b[s], o[t]); }
+                for(int t = 2 * s; t < TILES; t += 2) {
+                    inTurn();
+                    constexpr int SQUARES = OUTPUTS ? 4 : 2;
+                    Planes<3> rows[SQUARES];
+                    f32x4 sum[SQUARES];
+                    #pragma unroll
+                    for(int i = 0; i < SQUARES; i++) {
+                        rows[i] = operand.triangle(planes + (i < 2 ? L::correction : L::score), t + i % 2, s);
+                        sum[i] = i < 2 ? w[t + i] : x[TILES + t + i % 2];
+                    }
+                    multiplyAll(rows, b[s], sum);
+                    #pragma unroll
+                    for(int i = 0; i < SQUARES; i++) { (i < 2 ? w[t + i] : x[ROWS - TILES + t + i % 2]) = sum[i]; }
                 }
             }
         }
@@ -556,11 +585,11 @@ void deltaStateKernel(DeltaArgs a)
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
                 #pragma unroll
-                for(int r = 0; r < 4; r++) { if(rowIn(t, 4 * g + r) >= bad) { w[t][r] = o[t][r] = no; } }
+                for(int r = 0; r < 4; r++) { if(rowIn(t, 4 * g + r) >= bad) { w[t][r] = x[ROWS - TILES + t][r] = no; } }
             }
         }
         if(MODE == WALK_KEEP) { storeResult<float, C>(a.errors + at * C * a.padded, a.padded, g, column, true, C, w); }
-        if(OUTPUTS) { storeResult<T, C>(rowsOf<T>(a.out, a.chunks, p) + (uint64_t)first * a.out.rowStride + head * a.values, a.out.rowStride, g, column, inside, count, o); }
+        if(OUTPUTS) { storeResult<T, C>(rowsOf<T>(a.out, a.chunks, p) + (uint64_t)first * a.out.rowStride + head * a.values, a.out.rowStride, g, column, inside, count, *(const f32x4 (*)[TILES])(x + ROWS - TILES)); }
         // the state behind the chunk
         #pragma unroll
         for(int t = 0; t < STATE; t++) { state[t] *= chunk.decay; }
@@ -570,9 +599,10 @@ void deltaStateKernel(DeltaArgs a)
             f32x4 left[2];
             #pragma unroll
             for(int h = 0; h < 2; h++) { left[h] = w[2 * s + h] * table.beta(rowIn(2 * s + h, 4 * g)) * table.keyEnd(rowIn(2 * s + h, 4 * g)); }
-            const Planes<3> b = split<3>(left[0], left[1]);
+            Planes<NP> columns[STATE];
             #pragma unroll
-            for(int t = 0; t < STATE; t++) { state[t] = multiply(operand.columns(planes + L::keys, t, s), b, state[t]); }
+            for(int t = 0; t < STATE; t++) { columns[t] = operand.columns(planes + L::keys, t, s); }
+            multiplyAll(columns, split<3>(left[0], left[1]), state);
         }
         if(__builtin_expect(bad < C, 0)) {
             const float no = __builtin_nanf("");
@@ -617,8 +647,7 @@ void deltaJoinKernel(DeltaArgs a)
         for(int m = 0; m < STATE; m++) {
             #pragma unroll
             for(int t = 0; t < STATE; t++) {
-                const float4 x = *(const float4*)(move + rowIn(m, n16) * DK + rowIn(t, 4 * g));
-                next[m] = multiply(f32x4{x.x, x.y, x.z, x.w}, state[t], next[m]);
+                next[m] = multiply(*(const f32x4*)(move + rowIn(m, n16) * DK + rowIn(t, 4 * g)), state[t], next[m]);
             }
         }
         #pragma unroll
@@ -660,6 +689,15 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
     #pragma unroll
     for(int t = 0; t < STATE; t++) { state[t] = f32x4{0, 0, 0, 0}; }
     if(d.finalState) { loadResult<float, DK>(d.finalState + ((uint64_t)p.sequence * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
+    // two tiles of a triangle's transpose
+    const auto timesTriangle = [&](uint32_t from, int t, int s, const auto &b, f32x4 (&to)[TILES]) {
+        inTurn();
+        const Planes<3> rows[2] = {operand.triangleColumns(planes + from, t, s), operand.triangleColumns(planes + from, t + 1, s)};
+        f32x4 sum[2] = {to[t], to[t + 1]};
+        multiplyAll(rows, b, sum);
+        to[t] = sum[0];
+        to[t + 1] = sum[1];
+    };
     WalkStage<T, C, DK, true> stage;
     if(chunks) { const uint32_t last = begin + (chunks - 1) * C; stage.request(a, p, keyHead, last, end - last, (firstNumber + chunks - 1) * a.heads + head); }
     for(uint32_t left = chunks; left > 0; left--) {
@@ -669,13 +707,12 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
         Result<T, TILES> douts;
         if(active) { douts = requestResult<T, TILES>(rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)first * d.out.rowStride + head * a.values, d.out.rowStride, g, column, inside, count); }
         __syncthreads();
-        stage.store(planes);
+        stage.store(a, planes, count);
         __syncthreads();
         if(n > 0) { stage.request(a, p, keyHead, first - C, C, at - a.heads); }
         if(!active) { continue; }
 
         f32x4 dout[TILES], du[TILES];
-        takeResult(douts, inside, dout);
         #pragma unroll
         for(int t = 0; t < TILES; t++) { du[t] = f32x4{0, 0, 0, 0}; }
         storeResult<float, DK>(d.states + at * DK * a.padded, a.padded, g, column, true, DK, state);
@@ -683,10 +720,13 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
         #pragma unroll
         for(int s = 0; s < DK / 32; s++) {
             inTurn();
-            const Planes<3> b = split<3>(state[2 * s], state[2 * s + 1]);
+            Planes<NP> rows[TILES];
             #pragma unroll
-            for(int t = 0; t < TILES; t++) { du[t] = multiply(operand.rows(planes + L::keys, t, s), b, du[t]); }
+            for(int t = 0; t < TILES; t++) { rows[t] = operand.rows(planes + L::keys, t, s); }
+            multiplyAll(rows, split<3>(state[2 * s], state[2 * s + 1]), du);
         }
+        inTurn();
+        takeResult(douts, inside, dout);
         #pragma unroll
         for(int t = 0; t < TILES; t++) {
             du[t] *= table.keyEnd(rowIn(t, 4 * g));
@@ -696,7 +736,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             inTurn();
             const Planes<NP> b = split<NP>(dout[2 * s], dout[2 * s + 1]);
             #pragma unroll
-            for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(operand.triangleColumns(planes + L::score, t, s), b, du[t]); }
+            for(int t = 0; t < 2 * s + 2; t += 2) { timesTriangle(L::score, t, s, b, du); }
         }
         // dR = dU - N' beta dU
         {
@@ -713,7 +753,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             for(int s = 0; s < TILES / 2; s++) {
                 inTurn();
                 #pragma unroll
-                for(int t = 0; t < 2 * s + 2; t++) { du[t] = multiply(operand.triangleColumns(planes + L::correction, t, s), b[s], du[t]); }
+                for(int t = 0; t < 2 * s + 2; t += 2) { timesTriangle(L::correction, t, s, b[s], du); }
             }
         }
         storeResult<float, C>(d.errors + at * C * a.padded, a.padded, g, column, true, C, du);
@@ -731,11 +771,13 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
                 du[2 * s + h] *= table.beta(row);
                 y[h] = -table.keyState(row) * du[2 * s + h];
             }
-            const Planes<3> bx = split<3>(x[0], x[1]), by = split<3>(y[0], y[1]);
             #pragma unroll
-            for(int t = 0; t < STATE; t++) {
-                state[t] = multiply(operand.columns(planes + L::queries, t, s), bx, state[t]);
-                state[t] = multiply(operand.columns(planes + L::keys, t, s), by, state[t]);
+            for(int which = 0; which < 2; which++) {
+                inTurn();
+                Planes<NP> columns[STATE];
+                #pragma unroll
+                for(int t = 0; t < STATE; t++) { columns[t] = operand.columns(planes + (which ? L::keys : L::queries), t, s); }
+                multiplyAll(columns, which ? split<3>(y[0], y[1]) : split<3>(x[0], x[1]), state);
             }
         }
         if(d.v.data) { storeResult<T, C>(rowsOf<T>(d.v, a.chunks, p) + (uint64_t)first * d.v.rowStride + head * a.values, d.v.rowStride, g, column, inside, count, du); }
@@ -825,7 +867,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         const uint32_t item = (tid + i * 512) % UNITS, row = item / (DK / 8), column = item % (DK / 8) * 8, valid = row < count && column < a.keys ? min(8u, a.keys - column) : 0;
         const bool isKey = tid + i * 512 < UNITS;
         const gennmi_rows_t &r = isKey ? a.k : a.q;
-        const Eight<T> x = loadEight(rowAt<T>(r, a.chunks, p, valid ? begin + row : 0) + (valid ? keyHead * a.keys + column : 0), valid, a.wide);
+        const Eight<T> x = loadUnit(rowAt<T>(r, a.chunks, p, valid ? begin + row : begin) + (valid ? keyHead * a.keys + column : 0), valid, a.wide);
         storeUnit(planes + (isKey ? L::keys : L::queries) + unitAt<DK>(row, column / 8), C * DK, x);
     }
     const float decay = a.table[at].decay;
@@ -850,7 +892,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         }
         return x;
     };
-    const auto fourRows = [&](const float *from, uint32_t tile) { const float4 x = *(const float4*)(from + tile * 16 + 4 * g); return f32x4{x.x, x.y, x.z, x.w}; };
+    const auto fourRows = [&](const float *from, uint32_t tile) { return *(const f32x4*)(from + tile * 16 + 4 * g); };
     const auto sumOf16 = [](float x) { x += partner<1>(x); x += partner<2>(x); x += partner<4>(x); return x + partner<8>(x); };
 
     f32x4 dq[MINE], rS[MINE], dk[MINE], dqk[SQUARES], dkk[SQUARES];
@@ -893,9 +935,9 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         for(int m = 0; m < MINE; m++) {
             inTurn();
             const uint32_t offset = unitAt<32>(tileOf(m) * 16 + n16, g);
-            dq[m] = multiply(fetch<NP>(doutPlanes + offset, VP), state, dq[m]);
-            rS[m] = multiply(fetch<3>(dRPlanes + offset, VP), state, rS[m]);
-            dk[m] = multiply(fetch<3>(wPlanes + offset, VP), dState, dk[m]);
+            const Planes<NP> out = fetch<NP>(doutPlanes + offset, VP);
+            const Planes<3> r = fetch<3>(dRPlanes + offset, VP), w = fetch<3>(wPlanes + offset, VP);
+            multiplyThree(out, state, dq[m], r, state, rS[m], w, dState, dk[m]);
         }
         if(squares) {
             const Planes<3> other = fetch<3>(wPlanes + unitAt<32>(squareColumn * 16 + n16, g), VP);

@@ -15,6 +15,7 @@ using gennmi_elements::bf16;
 using gennmi_elements::f16;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template<typename T> constexpr int planesOf = 3;
 template<> constexpr int planesOf<f16> = 2;
@@ -81,8 +82,7 @@ template<int N> __device__ inline Planes<N> fetch(const uint16_t *at, uint32_t s
     Planes<N> out;
     #pragma unroll
     for(int p = 0; p < N; p++) {
-        const uint4 w = *(const uint4*)(at + p * stride);
-        out.plane[p].word[0] = w.x; out.plane[p].word[1] = w.y; out.plane[p].word[2] = w.z; out.plane[p].word[3] = w.w;
+        out.plane[p].v = *(const bf16x8*)(at + p * stride);
     }
     return out;
 }
@@ -117,6 +117,32 @@ template<int NA, int NB> __device__ inline f32x4 multiply(const Planes<NA> &a, c
     }
     return sum;
 }
+// sum[m] += a[m] b for several tiles: product after product, so that none waits for the one before it (a product takes 16 cycles, its sum is there after more than that)
+template<int NA, int NB, int M> __device__ inline void multiplyAll(const Planes<NA> (&a)[M], const Planes<NB> &b, f32x4 (&sum)[M])
+{
+    #pragma unroll
+    for(int total = 2; total >= 0; total--) {
+        #pragma unroll
+        for(int i = 0; i < NA; i++) {
+            if(total - i < 0 || total - i >= NB) { continue; }
+            #pragma unroll
+            for(int m = 0; m < M; m++) { sum[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].plane[i].v, b.plane[total - i].v, sum[m], 0, 0, 0); }
+        }
+    }
+}
+// Three sums at once, in turn
+template<int NA> __device__ inline void multiplyThree(const Planes<NA> &a, const Planes<3> &b, f32x4 &x, const Planes<3> &c, const Planes<3> &d, f32x4 &y, const Planes<3> &e, const Planes<3> &f, f32x4 &z)
+{
+    #pragma unroll
+    for(int total = 2; total >= 0; total--) {
+        #pragma unroll
+        for(int i = 0; i <= total; i++) {
+            if(i < NA) { x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.plane[i].v, b.plane[total - i].v, x, 0, 0, 0); }
+            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c.plane[i].v, d.plane[total - i].v, y, 0, 0, 0);
+            z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e.plane[i].v, f.plane[total - i].v, z, 0, 0, 0);
+        }
+    }
+}
 // sum += a b for 16 x 16 tiles in fp32: a's lane has row lane % 16, its columns 4 (lane / 16) + 0 .. 3; b is a result
 __device__ inline f32x4 multiply(const f32x4 &a, const f32x4 &b, f32x4 sum)
 {
@@ -127,44 +153,41 @@ __device__ inline f32x4 multiply(const f32x4 &a, const f32x4 &b, f32x4 sum)
 // Eight neighbouring elements, as they lie in memory
 template<typename T> struct Eight
 {
-    uint4 word[sizeof(T) / 2];
+    u32x4 word[sizeof(T) / 2];
     __device__ T at(int i) const
     {
-        const uint32_t w[4] = {word[i * sizeof(T) / 16].x, word[i * sizeof(T) / 16].y, word[i * sizeof(T) / 16].z, word[i * sizeof(T) / 16].w};
-        const int byte = i * sizeof(T) % 16;
-        if constexpr(sizeof(T) == 4) { return __builtin_bit_cast(T, w[byte / 4]); }
-        else { return __builtin_bit_cast(T, (uint16_t)(w[byte / 4] >> (byte % 4 * 8))); }
+        const int byte = i * sizeof(T);
+        const uint32_t w = word[byte / 16][byte % 16 / 4];
+        if constexpr(sizeof(T) == 4) { return __builtin_bit_cast(T, w); }
+        else { return __builtin_bit_cast(T, (uint16_t)(w >> (byte % 4 * 8))); }
     }
 };
-// `valid` of them, zero behind those; `wide`: they lie on 16 bytes, and there are eight or none
-template<typename T> __device__ inline Eight<T> loadEight(const T *at, uint32_t valid, bool wide)
+// `valid` of them, one by one, zero behind those
+template<typename T> __device__ inline Eight<T> loadEight(const T *at, uint32_t valid)
 {
-    Eight<T> out;
-    #pragma unroll
-    for(int h = 0; h < (int)sizeof(T) / 2; h++) { out.word[h] = make_uint4(0, 0, 0, 0); }
-    if(wide) {
-        if(valid) {
-            #pragma unroll
-            for(int h = 0; h < (int)sizeof(T) / 2; h++) { out.word[h] = ((const uint4*)at)[h]; }
-        }
-        return out;
-    }
-    uint32_t w[2 * sizeof(T)] = {};
+    Eight<T> out{};
     #pragma unroll
     for(int i = 0; i < 8; i++) {
         if((uint32_t)i >= valid) { continue; }
-        if constexpr(sizeof(T) == 4) { w[i] = __builtin_bit_cast(uint32_t, at[i]); }
-        else { w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, at[i]) << (i % 2 * 16); }
+        const int byte = i * sizeof(T);
+        if constexpr(sizeof(T) == 4) { out.word[byte / 16][byte % 16 / 4] = __builtin_bit_cast(uint32_t, at[i]); }
+        else { out.word[byte / 16][byte % 16 / 4] |= (uint32_t)__builtin_bit_cast(uint16_t, at[i]) << (byte % 4 * 8); }
     }
-    #pragma unroll
-    for(int h = 0; h < (int)sizeof(T) / 2; h++) { out.word[h] = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]); }
+    return out;
+}
+// All or none, from an address on 16 bytes where something lies; or one by one
+template<typename T> __device__ inline Eight<T> loadUnit(const T *at, uint32_t valid, bool wide)
+{
+    if(!wide) { return loadEight(at, valid); }
+    Eight<T> out = *(const Eight<T>*)at;
+    if(!valid) { out = Eight<T>{}; }
     return out;
 }
 // A unit of every plane
 template<typename T> __device__ inline void storeUnit(uint16_t *to, uint32_t stride, const Eight<T> &x)
 {
     constexpr int N = planesOf<T>;
-    if constexpr(N == 1) { *(uint4*)to = x.word[0]; }
+    if constexpr(N == 1) { *(u32x4*)to = x.word[0]; }
     else {
         float low[4], high[4];
         #pragma unroll
@@ -173,7 +196,7 @@ template<typename T> __device__ inline void storeUnit(uint16_t *to, uint32_t str
         splitFour<N>(low, a);
         splitFour<N>(high, b);
         #pragma unroll
-        for(int p = 0; p < N; p++) { *(uint4*)(to + p * stride) = make_uint4(a[p].x, a[p].y, b[p].x, b[p].y); }
+        for(int p = 0; p < N; p++) { *(u32x4*)(to + p * stride) = u32x4{a[p].x, a[p].y, b[p].x, b[p].y}; }
     }
 }
 }
