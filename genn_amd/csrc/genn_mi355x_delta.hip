@@ -1,5 +1,5 @@
 // The gated delta rule, for whole sequences (with gradients) and for single tokens.  Entry points and their checks; the kernels are in the header included below.
-#include <cstdlib>
+#include <algorithm>
 #include <type_traits>
 
 #include "genn_mi355x_delta_kernels.h"
@@ -29,6 +29,9 @@ template<typename F> int withSizes(const gennmi_delta_rule_t &c, F &&f)
 constexpr uint32_t WALK_COLUMNS = WALK_THREADS / 64 * 16;         // of a work-group of a walk
 uint32_t blocksOf(uint32_t columns) { return (columns + WALK_COLUMNS - 1) / WALK_COLUMNS; }
 
+// Work-groups of a walk: segments and key heads eight at a time, of each so many work-groups
+uint64_t walkGrid(uint64_t outer, uint64_t each) { return (outer + 7) / 8 * 8 * each; }
+
 int checkDelta(const char *what, const gennmi_delta_rule_t *c, bool gradients)
 {
     if(!c) { return fail(GENNMI_EINVAL, std::string(what) + ": null descriptor"); }
@@ -43,8 +46,8 @@ int checkDelta(const char *what, const gennmi_delta_rule_t *c, bool gradients)
         {"q", &c->q, c->keyHeads * c->keys, size}, {"k", &c->k, c->keyHeads * c->keys, size}, {"v", &c->v, c->heads * c->values, size}, {"g", &c->g, c->heads, 4}, {"beta", &c->beta, c->heads, 4}};
     for(const auto &r : read) { if(const int rc = checkRows(what, r.which, *r.rows, c->sequences, r.width, r.size)) { return rc; } }
     if(!gradients) { if(const int rc = checkWrittenRows(what, "out", c->out, c->sequences, c->heads * c->values, size)) { return rc; } }
-    for(const gennmi_rows_t *r : {&c->v, &c->out}) {
-        if(c->sequences.length > 1 && r->data && r->rowStride >= (1u << 26)) { return refuse(GENNMI_EINVAL, ": stride of v or out out of range"); }
+    for(const gennmi_rows_t *r : {&c->q, &c->k, &c->v, &c->out}) {
+        if(c->sequences.length > 1 && r->data && r->rowStride >= GENNMI_MAX_DELTA_STRIDE) { return refuse(GENNMI_EINVAL, ": stride of q, k, v or out out of range"); }
     }
     if((uintptr_t)c->initialState % 4 || (uintptr_t)c->finalState % 4) { return refuse(GENNMI_EINVAL, ": a state is not aligned"); }
     return GENNMI_OK;
@@ -73,12 +76,22 @@ int deltaApart(const char *what, const gennmi_delta_rule_t &c, const gennmi_delt
 }
 
 // Segments that a sequence is cut into, so that there are work-groups for the whole chip: what each does to the state is found for all of them at once (the state's columns and
-// those of a unit matrix), then joined, then outputs are found for all of them at once.
+// those of a unit matrix), then joined, then outputs are found for all of them at once.  The number is the one that should take the shortest, in units of a chunk's step of a walk alone on the chip (5.7 us):
+// two work-groups fit a compute unit, and with all 512 a step takes 1.8 units; what a segment does takes 0.57 of that a step; the join 0.8 units a segment.  One prompt of 64 chunks x 32 heads
+// in 1, 2, 4, 8, 16 segments: 369, 328, 215, 207, 253 us; 33 sequences of 8011 rows in all x 6 heads (fp16) in 1, 2, 4, 8: 234, 226, 163, 181.
 uint32_t segmentsOf(const gennmi_delta_rule_t &c, uint32_t columns)
 {
     const uint32_t C = chunkRows(c.type), chunks = (c.sequences.length + C - 1) / C;
-    if(const char *e = getenv("SEG")) { return std::max(1u, std::min(chunks, (uint32_t)atoi(e))); }
-    return 1;
+    const double all = (double)chunkNumbers(c.sequences, C) / std::max(1u, chunks) * c.heads, room = 512.0, blocks = blocksOf(columns), both = blocks + blocksOf(paddedKeys(c.keys));
+    const auto step = [&](double groups) { return (1.0 + 0.8 * std::min(1.0, groups / room)) * std::max(1.0, groups / room); };
+    uint32_t best = 1;
+    double least = chunks * step(all * blocks);
+    for(uint32_t n = 2; n <= std::min(chunks, 64u); n++) {
+        const uint32_t each = (chunks + n - 1) / n;
+        const double cost = each * (step(all * blocks * n) + 0.57 * step(all * both * (n - 1))) + 0.8 * n + 0.5;
+        if(cost < least) { least = cost; best = n; }
+    }
+    return best;
 }
 // Rows of a segment: a multiple of a chunk's
 uint32_t segmentRows(const gennmi_delta_rule_t &c, bool gradients)
@@ -119,9 +132,9 @@ bool deltaFits(const gennmi_delta_rule_t &c, bool gradients)
 {
     if(!gradients && c.sequences.length <= 1) { return tokenBlocks(c) <= mostBlocks(256); }
     const uint32_t columns = gradients ? paddedValues(c.values) : c.values;
-    return chunkNumbers(c.sequences, chunkRows(c.type)) * c.heads <= mostBlocks(512) &&
-        chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.heads * (blocksOf(columns) + moveBlocks(c)) <= mostBlocks(WALK_THREADS) &&
-        (uint64_t)c.sequences.count * c.heads * (paddedValues(c.values) / 16) <= mostBlocks(64);
+    return chunkNumbers(c.sequences, chunkRows(c.type)) * c.heads * (gradients && c.heads > c.keyHeads ? 8 : 1) <= mostBlocks(512) &&
+        walkGrid(chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.keyHeads, (uint64_t)(c.heads / c.keyHeads) * (blocksOf(columns) + moveBlocks(c))) <= mostBlocks(WALK_THREADS) &&
+        (uint64_t)c.sequences.count * c.heads * (paddedValues(c.values) / 16) <= mostBlocks(256);
 }
 DeltaArgs deltaArgs(const gennmi_delta_rule_t &c, const DeltaSpace &space, void *workspace, bool gradients)
 {
@@ -134,6 +147,7 @@ DeltaArgs deltaArgs(const gennmi_delta_rule_t &c, const DeltaSpace &space, void 
     a.heads = c.heads; a.keyHeads = c.keyHeads; a.group = c.heads / c.keyHeads; a.keys = c.keys; a.values = c.values; a.normalise = c.normalise;
     a.padded = paddedValues(c.values);
     a.columnBlocks = blocksOf(gradients ? a.padded : a.values);
+    a.segmentNumbers = (uint32_t)chunkNumbers(c.sequences, segmentRows(c, gradients));
     a.scale = c.scale; a.epsilon = c.epsilon;
     const uint32_t size = sizeOf(c.type);
     const auto wide = [&](const gennmi_rows_t &r) { return (uintptr_t)r.data % 16 == 0 && r.rowStride * size % 16 == 0 && r.sequenceStride * size % 16 == 0; };
@@ -175,7 +189,7 @@ template<typename T, int C, int DK, int MODE, bool FOLDED> int launchWalk(const 
     const auto kernel = deltaStateKernel<T, C, DK, MODE, FOLDED>;
     constexpr size_t lds = WalkLayout<T, C, DK, MODE == WALK_OUTPUTS>::bytes;
     if(const int rc = withLds(what, kernel, lds)) { return rc; }
-    kernel<<<dim3((uint32_t)(segments * a.heads * (a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0)))), dim3(WALK_THREADS), lds, stream>>>(a);
+    kernel<<<dim3((uint32_t)walkGrid(segments * a.keyHeads, a.group * (a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0)))), dim3(WALK_THREADS), lds, stream>>>(a);
     return gennmi_detail::afterLaunch(what);
 }
 // The state in front of every segment
@@ -183,7 +197,7 @@ template<typename T, int C, int DK, bool FOLDED> int launchSegments(const char *
 {
     if(!a.segmentStates) { return GENNMI_OK; }
     if(const int rc = launchWalk<T, C, DK, WALK_SUMMARY, FOLDED>(what, a, segments, stream)) { return rc; }
-    deltaJoinKernel<DK><<<dim3(a.chunks.count * a.heads * (a.padded / 16)), dim3(64), 0, stream>>>(a);
+    deltaJoinKernel<DK><<<dim3(a.chunks.count * a.heads * (a.padded / 16)), dim3(256), 0, stream>>>(a);
     return gennmi_detail::afterLaunch(what);
 }
 template<typename T, int C, int DK> int launchGradients(const char *what, const DeltaArgs &a, const DeltaGradientArgs &d, uint64_t numbers, uint64_t segments, hipStream_t stream)
@@ -193,7 +207,7 @@ template<typename T, int C, int DK> int launchGradients(const char *what, const 
     const auto reverse = deltaReverseKernel<T, C, DK>;
     constexpr size_t reverseLds = WalkLayout<T, C, DK, true>::bytes;
     if(const int rc = withLds(what, reverse, reverseLds)) { return rc; }
-    reverse<<<dim3((uint32_t)(segments * a.heads * a.columnBlocks)), dim3(WALK_THREADS), reverseLds, stream>>>(a, d);
+    reverse<<<dim3((uint32_t)walkGrid(segments * a.keyHeads, a.group * a.columnBlocks)), dim3(WALK_THREADS), reverseLds, stream>>>(a, d);
     const int rc = gennmi_detail::afterLaunch(what);
     if(rc || !(d.q.data || d.k.data || d.g.data || d.beta.data)) { return rc; }
     const auto kernel = deltaGradientKernel<T, C, DK>;
@@ -202,7 +216,7 @@ template<typename T, int C, int DK> int launchGradients(const char *what, const 
     kernel<<<dim3((uint32_t)(numbers * a.heads)), dim3(512), lds, stream>>>(a, d);
     if(const int rcGradient = gennmi_detail::afterLaunch(what)) { return rcGradient; }
     if(a.group == 1 || !(d.q.data || d.k.data)) { return GENNMI_OK; }
-    deltaSharedKernel<T, C, DK><<<dim3((uint32_t)(numbers * a.keyHeads)), dim3(256), 0, stream>>>(a, d);
+    deltaSharedKernel<T, C, DK><<<dim3((uint32_t)(numbers * a.keyHeads * (C / 4))), dim3(256), 0, stream>>>(a, d);
     return gennmi_detail::afterLaunch(what);
 }
 template<typename T, int VEC> int launchToken(const char *what, const DeltaArgs &a, uint32_t blocks, hipStream_t stream)
@@ -294,7 +308,7 @@ int gennmi_delta_rule_backward(const gennmi_delta_rule_t *rule, const gennmi_del
             if(!w.rows->data) { continue; }
             if(const int rc = checkWrittenRows(what, w.which, *w.rows, rule->sequences, w.width, w.size)) { return rc; }
         }
-        if(rule->sequences.length > 1 && (in.out.rowStride >= (1u << 26) || (in.v.data && in.v.rowStride >= (1u << 26)))) {
+        if(rule->sequences.length > 1 && (in.out.rowStride >= GENNMI_MAX_DELTA_STRIDE || (in.v.data && in.v.rowStride >= GENNMI_MAX_DELTA_STRIDE))) {
             return fail(GENNMI_EINVAL, "delta_rule_backward: stride of the gradients of v or out out of range");
         }
         if((uintptr_t)in.finalState % 4 || (uintptr_t)in.initialState % 4) { return fail(GENNMI_EINVAL, "delta_rule_backward: a state is not aligned"); }

@@ -60,7 +60,7 @@ struct DeltaArgs
     float *correction, *score;      // of each chunk number and head: -N and P, [C][C]
     void *rows;                     // RowTable
     ChunkTable *table;
-    uint32_t moveBlocks;            // of the columns of a segment's `move`
+    uint32_t segmentNumbers, moveBlocks;        // moveBlocks: of the columns of a segment's `move`
     float *segmentStates, *segmentMoves;        // of each segment and head [DK][padded], [DK][DK]; NULL: sequences are not cut
     float *states, *errors;         // kept for gradients, of each chunk number and head: the state in front of it [DK][padded], w [C][padded]
 };
@@ -293,26 +293,29 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
     Eight<T> keys[EACH], queries[QUERIES ? EACH : 1];
     f32x4 corrections[SQUARES], scores[QUERIES ? SQUARES : 1], rows;
 
-    __device__ static uint32_t rowOf(int i) { return (threadIdx.x + i * WALK_THREADS) / (DK / 8); }
-    __device__ static uint32_t columnOf(int i) { return (threadIdx.x + i * WALK_THREADS) % (DK / 8) * 8; }
+    static constexpr uint32_t STEP = WALK_THREADS * 8 / DK;         // rows between a thread's units
+    __device__ static uint32_t rowOf(int i) { return threadIdx.x / (DK / 8) + i * STEP; }
+    __device__ static uint32_t column() { return threadIdx.x % (DK / 8) * 8; }
     // Units that are not there are asked for at another place, and become zero in store(): no branch a unit, with which the compiler would wait for each
     __device__ void request(const DeltaArgs &a, const Place &p, uint32_t keyHead, uint32_t first, uint32_t count, uint64_t at)
     {
         const T *const key = rowsOf<const T>(a.k, a.chunks, p) + (uint64_t)first * a.k.rowStride + keyHead * a.keys, *const query = rowsOf<const T>(a.q, a.chunks, p) + (uint64_t)first * a.q.rowStride + keyHead * a.keys;
-        if(a.wide) {
+        if(a.wide && count == C) {
+            // (an offset of 32 bits a lane, the rest is the scalar unit's)
+            const uint32_t at0 = column() < a.keys ? column() : 0, keyOffset = rowOf(0) * (uint32_t)a.k.rowStride + at0, queryOffset = rowOf(0) * (uint32_t)a.q.rowStride + at0;
             #pragma unroll
             for(int i = 0; i < EACH; i++) {
-                const uint32_t row = min(rowOf(i), count - 1), column = columnOf(i) < a.keys ? columnOf(i) : 0;
-                keys[i] = *(const Eight<T>*)(key + row * a.k.rowStride + column);
-                if(QUERIES) { queries[i] = *(const Eight<T>*)(query + row * a.q.rowStride + column); }
+                keys[i] = *(const Eight<T>*)((key + i * STEP * a.k.rowStride) + keyOffset);
+                if(QUERIES) { queries[i] = *(const Eight<T>*)((query + i * STEP * a.q.rowStride) + queryOffset); }
             }
         }
         else {
+            const uint32_t valid = column() < a.keys ? min(8u, a.keys - column()) : 0, at0 = valid ? column() : 0;
             #pragma unroll
             for(int i = 0; i < EACH; i++) {
-                const uint32_t row = min(rowOf(i), count - 1), valid = columnOf(i) < a.keys ? min(8u, a.keys - columnOf(i)) : 0;
-                keys[i] = loadEight(key + row * a.k.rowStride + columnOf(i), valid);
-                if(QUERIES) { queries[i] = loadEight(query + row * a.q.rowStride + columnOf(i), valid); }
+                const uint64_t row = min(rowOf(i), count - 1);
+                keys[i] = a.wide ? *(const Eight<T>*)(key + row * a.k.rowStride + at0) : loadEight(key + row * a.k.rowStride + at0, valid);
+                if(QUERIES) { queries[i] = a.wide ? *(const Eight<T>*)(query + row * a.q.rowStride + at0) : loadEight(query + row * a.q.rowStride + at0, valid); }
             }
         }
         #pragma unroll
@@ -338,14 +341,14 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
         if(count < C || a.keys <= DK - 8) {
             #pragma unroll
             for(int i = 0; i < EACH; i++) {
-                if(rowOf(i) < count && columnOf(i) < a.keys) { continue; }
+                if(rowOf(i) < count && column() < a.keys) { continue; }
                 keys[i] = Eight<T>{};
                 if(QUERIES) { queries[i] = Eight<T>{}; }
             }
         }
         #pragma unroll
         for(int i = 0; i < EACH; i++) {
-            const uint32_t to = unitAt<DK>(rowOf(i), columnOf(i) / 8);
+            const uint32_t to = unitAt<DK>(rowOf(i), column() / 8);
             storeUnit(planes + L::keys + to, C * DK, keys[i]);
             if(QUERIES) { storeUnit(planes + L::queries + to, C * DK, queries[i]); }
         }
@@ -384,14 +387,14 @@ template<int C> __device__ inline uint32_t firstBad(const f32x4 (&x)[C / 16], ui
     #pragma unroll
     for(int t = C / 16 - 1; t >= 0; t--) {
         #pragma unroll
-        for(int r = 3; r >= 0; r--) { if(!finite(x[t][r])) { first = min(first, rowIn(t, 4 * g + r)); } }
+        for(int r = 3; r >= 0; r--) { if(!finite(x[t][r])) { first = min(first, rowIn(t, r) + 8 * g); } }
     }
     first = min(first, (uint32_t)__shfl_xor((int)first, 16));
     return min(first, (uint32_t)__shfl_xor((int)first, 32));
 }
 
 // Rows of values at a lane's column, in the order of a result: row 4 g + r of tile t.  What differs between lanes is an offset of 32 bits (strides are
-// below 2^26 here), the rest is the scalar unit's.  Behind `count` rows, or the last column: zero.
+// below 2^25 here), the rest is the scalar unit's.  Behind `count` rows, or the last column: zero.
 template<typename T, int TILES> struct Result { T v[TILES][4]; };
 template<typename T, int TILES> __device__ inline Result<T, TILES> requestResult(const T *rows, uint64_t stride, uint32_t g, uint32_t column, bool inside, uint32_t count)
 {
@@ -410,7 +413,7 @@ template<typename T, int TILES> __device__ inline Result<T, TILES> requestResult
         #pragma unroll
         for(int r = 0; r < 4; r++) {
             x.v[t][r] = (T)0.0f;
-            if(rowIn(t, 4 * g + r) < count) { x.v[t][r] = (rows + rowIn(t, r) * stride)[offset]; }
+            if((int)rowIn(t, r) < (int)(count - 8 * g)) { x.v[t][r] = (rows + rowIn(t, r) * stride)[offset]; }
         }
     }
     return x;
@@ -442,7 +445,7 @@ template<typename T, int C> __device__ inline void storeResult(T *rows, uint64_t
     #pragma unroll
     for(int t = 0; t < C / 16; t++) {
         #pragma unroll
-        for(int r = 0; r < 4; r++) { if(rowIn(t, 4 * g + r) < count) { (rows + rowIn(t, r) * stride)[offset] = narrow<T>(x[t][r]); } }
+        for(int r = 0; r < 4; r++) { if((int)rowIn(t, r) < (int)(count - 8 * g)) { (rows + rowIn(t, r) * stride)[offset] = narrow<T>(x[t][r]); } }
     }
 }
 
@@ -454,6 +457,15 @@ template<int TILES, int SPLIT> __device__ inline void storeResultTiles(float *ro
         #pragma unroll
         for(int r = 0; r < 4; r++) { rows[((first + SPLIT * t) * 16 + 4 * g + r) * stride + column] = x[t][r]; }
     }
+}
+
+// Which head, columns and segment a work-group of a walk has.  Those of one segment and key head read the same keys, queries and squares: they go to one of the eight parts of the chip with an L2 of
+// its own, to which the hardware hands work-groups in turn.
+struct WalkPlace { uint32_t segment, head, block; bool valid; };
+__device__ inline WalkPlace walkPlace(const DeltaArgs &a, uint32_t blocks)
+{
+    const uint32_t each = a.group * blocks, slot = blockIdx.x / 8, outer = slot / each * 8 + blockIdx.x % 8, inner = slot % each, segment = outer / a.keyHeads;
+    return WalkPlace{segment, (outer - segment * a.keyHeads) * a.group + inner / blocks, inner % blocks, segment < a.segmentNumbers};
 }
 
 // A work-group walks a sequence (or a segment of it) of one head with 16 columns of the state a wavefront.
@@ -469,10 +481,10 @@ void deltaStateKernel(DeltaArgs a)
     const RowFactors<C> table{(float*)(planes + L::table)};
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
     const WalkOperands<T, C, DK> operand{n16, g};
-    const uint32_t blocks = a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0);
-    const uint32_t block = blockIdx.x % blocks, rest = blockIdx.x / blocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
+    const WalkPlace mine = walkPlace(a, a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0));
+    const uint32_t block = mine.block, head = mine.head, segment = mine.segment, keyHead = head / a.group;
     Place p;
-    if(!locate(a.segments, segment, p)) { return; }
+    if(!mine.valid || !locate(a.segments, segment, p)) { return; }
     const uint32_t begin = p.index * a.segments.chunk, end = min(p.length, begin + a.segments.chunk);
     // (what is behind the last segment nobody asks)
     if(MODE == WALK_SUMMARY && end == p.length) { return; }
@@ -489,7 +501,7 @@ void deltaStateKernel(DeltaArgs a)
         #pragma unroll
         for(int t = 0; t < STATE; t++) {
             #pragma unroll
-            for(int r = 0; r < 4; r++) { if(move && rowIn(t, 4 * g + r) == column) { state[t][r] = 1.0f; } }
+            for(int r = 0; r < 4; r++) { if(move && (int)rowIn(t, r) == (int)(column - 8 * g)) { state[t][r] = 1.0f; } }
         }
     }
     else if(a.segmentStates) {
@@ -508,8 +520,8 @@ void deltaStateKernel(DeltaArgs a)
         __syncthreads();
         stage.store(a, planes, count);
         __syncthreads();
-        if(n + 1 < chunks) { stage.request(a, p, keyHead, first + C, min((uint32_t)C, end - first - C), at + a.heads); }
-        if(!active) { continue; }
+        const auto requestNext = [&] { if(n + 1 < chunks) { stage.request(a, p, keyHead, first + C, min((uint32_t)C, end - first - C), at + a.heads); } };
+        if(!active) { requestNext(); continue; }
 
         // r = v - G k^ S, and the part of the outputs that the state in front has: x's first tiles and the others
         constexpr int ROWS = OUTPUTS ? 2 * TILES : TILES;
@@ -545,7 +557,7 @@ void deltaStateKernel(DeltaArgs a)
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
                 #pragma unroll
-                for(int r = 0; r < 4; r++) { if(rowIn(t, 4 * g + r) >= bad) { w[t][r] = 0.0f; } }
+                for(int r = 0; r < 4; r++) { if((int)rowIn(t, r) >= (int)(bad - 8 * g)) { w[t][r] = 0.0f; } }
             }
         }
         // w = r - N beta r and out += P beta w; tiles above the diagonal are zero
@@ -585,12 +597,13 @@ void deltaStateKernel(DeltaArgs a)
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
                 #pragma unroll
-                for(int r = 0; r < 4; r++) { if(rowIn(t, 4 * g + r) >= bad) { w[t][r] = x[ROWS - TILES + t][r] = no; } }
+                for(int r = 0; r < 4; r++) { if((int)rowIn(t, r) >= (int)(bad - 8 * g)) { w[t][r] = x[ROWS - TILES + t][r] = no; } }
             }
         }
         if(MODE == WALK_KEEP) { storeResult<float, C>(a.errors + at * C * a.padded, a.padded, g, column, true, C, w); }
         if(OUTPUTS) { storeResult<T, C>(rowsOf<T>(a.out, a.chunks, p) + (uint64_t)first * a.out.rowStride + head * a.values, a.out.rowStride, g, column, inside, count, *(const f32x4 (*)[TILES])(x + ROWS - TILES)); }
-        // the state behind the chunk
+        // the state behind the chunk; meanwhile the next one's operands are on their way (asked for before this they cost registers that there are not)
+        requestNext();
         #pragma unroll
         for(int t = 0; t < STATE; t++) { state[t] *= chunk.decay; }
         #pragma unroll
@@ -620,13 +633,15 @@ void deltaStateKernel(DeltaArgs a)
     }
 }
 
-// From what each segment does: the state in front of each, in place of its own share.  A wavefront has 16 columns; S = move S + own in fp32.
+// From what each segment does: the state in front of each, in place of its own share: S = move S + own in fp32.  A work-group has 16 columns; its four wavefronts share the rows of
+// `move`, and hand each other what they found through LDS.
 template<int DK>
-__global__ __launch_bounds__(64)
+__global__ __launch_bounds__(256)
 void deltaJoinKernel(DeltaArgs a)
 {
-    constexpr int STATE = DK / 16;
-    const uint32_t lane = threadIdx.x, n16 = lane & 15, g = lane >> 4, tiles = a.padded / 16;
+    constexpr int STATE = DK / 16, MINE = STATE / 4;
+    __shared__ f32x4 found[STATE][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4, tiles = a.padded / 16;
     const uint32_t tile = blockIdx.x % tiles, rest = blockIdx.x / tiles, head = rest % a.heads, sequence = rest / a.heads, column = tile * 16 + n16;
     Place p;
     if(!describe(a.segments, sequence, p)) { return; }
@@ -635,23 +650,48 @@ void deltaJoinKernel(DeltaArgs a)
     for(int t = 0; t < STATE; t++) { state[t] = f32x4{0, 0, 0, 0}; }
     if(a.initialState) { loadResult<float, DK>(a.initialState + ((uint64_t)p.state * a.heads + head) * a.keys * a.values, a.values, g, column, column < a.values, a.keys, state); }
     const uint32_t segments = max(1u, (p.length + a.segments.chunk - 1) / a.segments.chunk);
-    uint64_t at = firstChunk(a.segments, sequence) * a.heads + head;
-    for(uint32_t n = 0; n < segments; n++, at += a.heads) {
-        float *const own = a.segmentStates + at * DK * a.padded;
-        f32x4 next[STATE];
-        if(n + 1 < segments) { loadResult<float, DK>(own, a.padded, g, column, true, DK, next); }
-        storeResult<float, DK>(own, a.padded, g, column, true, DK, state);
-        if(n + 1 == segments) { break; }
-        const float *const move = a.segmentMoves + at * DK * DK;
+    const uint64_t first = firstChunk(a.segments, sequence) * a.heads + head;
+    // (this wavefront's tiles of `move` and of a segment's own share)
+    f32x4 move[MINE][STATE], own[MINE];
+    const auto request = [&](uint32_t n) {
+        const uint64_t at = first + (uint64_t)n * a.heads;
         #pragma unroll
-        for(int m = 0; m < STATE; m++) {
+        for(int m = 0; m < MINE; m++) {
+            const uint32_t rows = wave * MINE + m;
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { own[m][r] = a.segmentStates[at * DK * a.padded + rowIn(rows, 4 * g + r) * a.padded + column]; }
+            #pragma unroll
+            for(int t = 0; t < STATE; t++) { move[m][t] = *(const f32x4*)(a.segmentMoves + at * DK * DK + rowIn(rows, n16) * DK + rowIn(t, 4 * g)); }
+        }
+    };
+    if(segments > 1) { request(0); }
+    for(uint32_t n = 0; n < segments; n++) {
+        float *const to = a.segmentStates + (first + (uint64_t)n * a.heads) * DK * a.padded + column;
+        f32x4 next[MINE];
+        if(n + 1 < segments) {
+            #pragma unroll
+            for(int m = 0; m < MINE; m++) { next[m] = own[m]; }
             #pragma unroll
             for(int t = 0; t < STATE; t++) {
-                next[m] = multiply(*(const f32x4*)(move + rowIn(m, n16) * DK + rowIn(t, 4 * g)), state[t], next[m]);
+                #pragma unroll
+                for(int m = 0; m < MINE; m++) { next[m] = multiply(move[m][t], state[t], next[m]); }
             }
         }
+        // (own shares have been read: the state goes in their place)
         #pragma unroll
-        for(int t = 0; t < STATE; t++) { state[t] = next[t]; }
+        for(int t = 0; t < STATE; t++) {
+            if((uint32_t)t / MINE != wave) { continue; }
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { to[rowIn(t, 4 * g + r) * a.padded] = state[t][r]; }
+        }
+        if(n + 1 == segments) { break; }
+        if(n + 2 < segments) { request(n + 1); }
+        __syncthreads();
+        #pragma unroll
+        for(int m = 0; m < MINE; m++) { found[wave * MINE + m][lane] = next[m]; }
+        __syncthreads();
+        #pragma unroll
+        for(int t = 0; t < STATE; t++) { state[t] = found[t][lane]; }
     }
 }
 
@@ -676,9 +716,10 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
     const RowFactors<C> table{(float*)(planes + L::table)};
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
     const WalkOperands<T, C, DK> operand{n16, g};
-    const uint32_t block = blockIdx.x % a.columnBlocks, rest = blockIdx.x / a.columnBlocks, head = rest % a.heads, segment = rest / a.heads, keyHead = head / a.group;
+    const WalkPlace mine = walkPlace(a, a.columnBlocks);
+    const uint32_t block = mine.block, head = mine.head, segment = mine.segment, keyHead = head / a.group;
     Place p;
-    if(!locate(a.segments, segment, p)) { return; }
+    if(!mine.valid || !locate(a.segments, segment, p)) { return; }
     const uint32_t begin = p.index * a.segments.chunk, end = min(p.length, begin + a.segments.chunk);
     const uint32_t column = (block * WAVES + wave) * 16 + n16;
     const bool active = (block * WAVES + wave) * 16 < a.padded, inside = column < a.values;
@@ -709,8 +750,8 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
         __syncthreads();
         stage.store(a, planes, count);
         __syncthreads();
-        if(n > 0) { stage.request(a, p, keyHead, first - C, C, at - a.heads); }
-        if(!active) { continue; }
+        const auto requestNext = [&] { if(n > 0) { stage.request(a, p, keyHead, first - C, C, at - a.heads); } };
+        if(!active) { requestNext(); continue; }
 
         f32x4 dout[TILES], du[TILES];
         #pragma unroll
@@ -757,6 +798,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             }
         }
         storeResult<float, C>(d.errors + at * C * a.padded, a.padded, g, column, true, C, du);
+        requestNext();
         // dS in front of the chunk = G[last] dS + (scale G q^)' dout - (G k^)' (beta dR)
         #pragma unroll
         for(int t = 0; t < STATE; t++) { state[t] *= decay; }
@@ -1127,13 +1169,13 @@ template<typename T, int C, int DK>
 __global__ __launch_bounds__(256)
 void deltaSharedKernel(DeltaArgs a, DeltaGradientArgs d)
 {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t number = blockIdx.x / a.keyHeads, keyHead = blockIdx.x - number * a.keyHeads;
+    const uint32_t lane = threadIdx.x & 63, row = blockIdx.x % (C / 4) * 4 + (threadIdx.x >> 6), chunk = blockIdx.x / (C / 4);
+    const uint32_t number = chunk / a.keyHeads, keyHead = chunk - number * a.keyHeads;
     Place p;
     if(!locate(a.chunks, number, p)) { return; }
     const uint32_t begin = p.index * C, count = min((uint32_t)C, p.length - min(p.length, begin));
     const float *const from = d.shared + ((uint64_t)number * a.heads + keyHead * a.group) * 2 * C * DK;
-    for(uint32_t row = wave; row < count; row += 4) {
+    if(row < count) {
         #pragma unroll
         for(int which = 0; which < 2; which++) {
             const gennmi_rows_t &in = which ? a.k : a.q, &out = which ? d.k : d.q;

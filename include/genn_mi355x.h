@@ -675,6 +675,7 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
  * sequence) takes a kernel of its own, without a workspace. */
 #define GENNMI_MAX_DELTA_KEYS 128
 #define GENNMI_MAX_DELTA_VALUES 1024
+#define GENNMI_MAX_DELTA_STRIDE (1u << 25)      /* rows of q, k, v and out (where there is a second one) are less than that many elements apart */
 typedef struct gennmi_delta_rule_t {
     gennmi_sequences_t sequences;
     uint32_t type;                        /* of q, k, v and out: GENNMI_TYPE_F32, _F16 or _BF16 */
