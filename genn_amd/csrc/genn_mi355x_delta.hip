@@ -213,7 +213,7 @@ template<typename T, int C, int DK> int launchGradients(const char *what, const 
     const auto kernel = deltaGradientKernel<T, C, DK>;
     constexpr size_t lds = GradientLayout<T, C, DK>::bytes;
     if(const int rcLds = withLds(what, kernel, lds)) { return rcLds; }
-    kernel<<<dim3((uint32_t)(numbers * a.heads)), dim3(512), lds, stream>>>(a, d);
+    kernel<<<dim3((uint32_t)(numbers * a.heads)), dim3(256), lds, stream>>>(a, d);
     if(const int rcGradient = gennmi_detail::afterLaunch(what)) { return rcGradient; }
     if(a.group == 1 || !(d.q.data || d.k.data)) { return GENNMI_OK; }
     deltaSharedKernel<T, C, DK><<<dim3((uint32_t)(numbers * a.keyHeads * (C / 4))), dim3(256), 0, stream>>>(a, d);

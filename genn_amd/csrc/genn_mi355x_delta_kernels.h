@@ -449,16 +449,6 @@ template<typename T, int C> __device__ inline void storeResult(T *rows, uint64_t
     }
 }
 
-// Some tiles of a result, every SPLIT-th from `first` on, all rows and columns
-template<int TILES, int SPLIT> __device__ inline void storeResultTiles(float *rows, uint32_t stride, uint32_t first, uint32_t g, uint32_t column, const f32x4 (&x)[TILES])
-{
-    #pragma unroll
-    for(int t = 0; t < TILES; t++) {
-        #pragma unroll
-        for(int r = 0; r < 4; r++) { rows[((first + SPLIT * t) * 16 + 4 * g + r) * stride + column] = x[t][r]; }
-    }
-}
-
 // Which head, columns and segment a work-group of a walk has.  Those of one segment and key head read the same keys, queries and squares: they go to one of the eight parts of the chip with an L2 of
 // its own, to which the hardware hands work-groups in turn.
 struct WalkPlace { uint32_t segment, head, block; bool valid; };
@@ -834,27 +824,27 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
 // and g's: with states and u in units of the decay so far, outputs grow with it and values shrink, so that what the sum of g up to row i gains the loss
 // is q^[i].dq^[i] - v[i].dv[i], and at the chunk's last row the state behind it times its gradient as well.
 // A work-group has a chunk and a head.  Products are summed over the values, 32 at a time, with what multiplies S and dS
-// in LDS (the next 32 on their way meanwhile); a wavefront has 16 keys' columns of the results, S' and dS' straight from memory.  Where heads share keys, what each finds for them is left for
-// deltaSharedKernel to add up.
+// in LDS (the next 32 on their way meanwhile); a wavefront has the results' columns of a quarter of the keys, S' and dS' straight from memory.  What bounds it is waiting, for memory and at barriers: two work-groups
+// of four wavefronts fit a compute unit and fill each other's pauses.  Where heads share keys, what each finds for them is left for deltaSharedKernel to add up.
 template<typename T, int C, int DK> struct GradientLayout
 {
     static constexpr int NP = planesOf<T>;
     static constexpr uint32_t keys = 0, queries = keys + NP * C * DK, stage = queries + NP * C * DK, staged = (NP + 6) * C * 32, square = 3 * C * C,
-        floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (6 + 2 * 8) + 64;
+        floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (6 + 2 * 4) + 32;
 };
 
 template<typename T, int C, int DK>
-__global__ __launch_bounds__(512)
+__global__ __launch_bounds__(256, 2)
 void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
 {
     typedef GradientLayout<T, C, DK> L;
-    constexpr int NP = planesOf<T>, TILES = C / 16, KEY_TILES = DK / 16, SPLIT = 8 / KEY_TILES, MINE = TILES / SPLIT, SQUARES = C == 64 ? 2 : 1, UNITS = C * DK / 8, VP = C * 32;
+    constexpr int NP = planesOf<T>, TILES = C / 16, MINE = DK / 64, SQUARES = C == 64 ? 4 : 1, UNITS = C * DK / 8, VP = C * 32, ITEMS = C / 32;
     extern __shared__ __align__(16) char lds[];
     uint16_t *const planes = (uint16_t*)lds, *const stage = planes + L::stage;
     uint16_t *const doutPlanes = stage, *const dRPlanes = stage + NP * VP, *const wPlanes = dRPlanes + 3 * VP;
     double *const sums = (double*)(planes + L::floats);
     float *const since = (float*)(sums + C), *const until = since + C, *const beta = until + C, *const keyUnit = beta + C, *const queryUnit = keyUnit + C, *const valueDots = queryUnit + C;
-    float *const queryDots = valueDots + C, *const keyDots = queryDots + 8 * C, *const ends = keyDots + 8 * C;
+    float *const queryDots = valueDots + C, *const keyDots = queryDots + 4 * C, *const ends = keyDots + 4 * C;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     const uint32_t number = blockIdx.x / a.heads, head = blockIdx.x - number * a.heads, keyHead = head / a.group;
     const uint64_t at = (uint64_t)number * a.heads + head;
@@ -863,24 +853,26 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     const uint32_t begin = p.index * C, count = min((uint32_t)C, p.length - min(p.length, begin));
     if(!count) { return; }
 
-    // tiles of this wavefront: 16 keys and every SPLIT-th 16 rows; rows and columns of squares
-    const uint32_t keyTile = wave % KEY_TILES, firstRow = wave / KEY_TILES, key = keyTile * 16 + n16;
-    const auto tileOf = [&](int m) { return firstRow + SPLIT * m; };
-    const auto squareRow = [&](int q) { return C == 64 ? (wave >> 2) + 2 * q : wave >> 1; };
-    const uint32_t squareColumn = C == 64 ? wave & 3 : wave & 1;
-    const bool squares = C == 64 || wave < 4;
+    // this wavefront's columns of keys; squares: of 64 rows a column of tiles a wavefront, of 32 a tile
+    const auto keyOf = [&](int m) { return (wave * MINE + m) * 16 + n16; };
+    const auto squareRow = [&](int q) { return C == 64 ? (uint32_t)q : wave >> 1; };
+    const uint32_t squareColumn = C == 64 ? wave : wave & 1;
 
+    // keys and queries
+    Eight<T> units[2 * UNITS / 256];
+    #pragma unroll
+    for(int i = 0; i < 2 * UNITS / 256; i++) {
+        const uint32_t item = (tid + i * 256) % UNITS, row = item / (DK / 8), column = item % (DK / 8) * 8, valid = row < count && column < a.keys ? min(8u, a.keys - column) : 0;
+        const gennmi_rows_t &r = i < UNITS / 256 ? a.k : a.q;
+        units[i] = loadUnit(rowAt<T>(r, a.chunks, p, valid ? begin + row : begin) + (valid ? keyHead * a.keys + column : 0), valid, a.wide);
+    }
     // what multiplies S and dS: eight threads a row, four values each
-    const bool stages = tid < C * 8;
-    const uint32_t stageRow = stages ? tid / 8 : 0, stageAt = tid % 8 * 4;
-    const bool staged = stages && stageRow < count;
-    const float *const stateRow = a.states + at * DK * a.padded + (uint64_t)key * a.padded + 8 * g, *const dStateRow = d.states + at * DK * a.padded + (uint64_t)key * a.padded + 8 * g;
-    const uint64_t usedRow = begin + (staged ? stageRow : 0);
-    const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + usedRow * d.out.rowStride + head * a.values, *const values = rowsOf<const T>(a.v, a.chunks, p) + usedRow * a.v.rowStride + head * a.values;
-    const float *const dRRow = d.errors + (at * C + stageRow) * a.padded, *const wRow = a.errors + (at * C + stageRow) * a.padded;
+    const float *const stateRows = a.states + at * DK * a.padded, *const dStateRows = d.states + at * DK * a.padded;
     typedef Pack<T, 4> Four;
-    float4 nextState[2], nextDState[2], nextDR, nextW;
-    Four nextDout, nextValues;
+    f32x4 nextDR[ITEMS], nextW[ITEMS];
+    Four nextDout[ITEMS], nextValues[ITEMS];
+    const auto rowOfItem = [&](int i) { return tid / 8 + 32 * i; };
+    const uint32_t stageAt = tid % 8 * 4;
     const auto four = [&](const T *from, uint32_t v) {
         Four x{};
         if(a.wideValues) { if(v < a.values) { x = *(const Four*)(from + v); } }
@@ -892,25 +884,21 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     };
     const auto request = [&](uint32_t v) {
         #pragma unroll
-        for(int h = 0; h < 2; h++) { nextState[h] = *(const float4*)(stateRow + v + 4 * h); nextDState[h] = *(const float4*)(dStateRow + v + 4 * h); }
-        nextDR = nextW = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        nextDout = nextValues = Four{};
-        if(staged) {
-            nextDR = *(const float4*)(dRRow + v + stageAt);
-            nextW = *(const float4*)(wRow + v + stageAt);
-            nextDout = four(douts, v + stageAt);
-            nextValues = four(values, v + stageAt);
+        for(int i = 0; i < ITEMS; i++) {
+            // (rows that are not there: another's, and nothing of it is used)
+            const uint64_t row = rowOfItem(i);
+            nextDR[i] = *(const f32x4*)(d.errors + (at * C + row) * a.padded + v + stageAt);
+            nextW[i] = *(const f32x4*)(a.errors + (at * C + row) * a.padded + v + stageAt);
+            const uint64_t there = begin + min((uint32_t)row, count - 1);
+            nextDout[i] = four(rowAt<T>(d.out, a.chunks, p, there) + head * a.values, v + stageAt);
+            nextValues[i] = four(rowAt<T>(a.v, a.chunks, p, there) + head * a.values, v + stageAt);
         }
     };
     request(0);
-
     #pragma unroll
-    for(int i = 0; i < 2 * UNITS / 512; i++) {
-        const uint32_t item = (tid + i * 512) % UNITS, row = item / (DK / 8), column = item % (DK / 8) * 8, valid = row < count && column < a.keys ? min(8u, a.keys - column) : 0;
-        const bool isKey = tid + i * 512 < UNITS;
-        const gennmi_rows_t &r = isKey ? a.k : a.q;
-        const Eight<T> x = loadUnit(rowAt<T>(r, a.chunks, p, valid ? begin + row : begin) + (valid ? keyHead * a.keys + column : 0), valid, a.wide);
-        storeUnit(planes + (isKey ? L::keys : L::queries) + unitAt<DK>(row, column / 8), C * DK, x);
+    for(int i = 0; i < 2 * UNITS / 256; i++) {
+        const uint32_t item = (tid + i * 256) % UNITS;
+        storeUnit(planes + (i < UNITS / 256 ? L::keys : L::queries) + unitAt<DK>(item / (DK / 8), item % (DK / 8)), C * DK, units[i]);
     }
     const float decay = a.table[at].decay;
     if(tid < C) {
@@ -923,12 +911,12 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         keyUnit[tid] = rows.keyUnit[tid];
         queryUnit[tid] = rows.queryUnit[tid];
     }
-    // the key's (or query's) values at this lane's column, four rows of a tile
-    const auto valuesAt = [&](uint32_t from, uint32_t tile) {
+    // the keys' (or queries') values at this lane's column, four rows of a tile
+    const auto valuesAt = [&](uint32_t from, uint32_t tile, int m) {
         f32x4 x = {0, 0, 0, 0};
         #pragma unroll
         for(int k = 0; k < NP; k++) {
-            const uint2 w = readColumn(planes + from + k * C * DK + unitAt<DK>(tile * 16 + 4 * g + n16 / 4, 2 * keyTile + n16 % 4 / 2) + n16 % 2 * 4);
+            const uint2 w = readColumn(planes + from + k * C * DK + unitAt<DK>(tile * 16 + 4 * g + n16 / 4, 2 * (wave * MINE + m) + n16 % 4 / 2) + n16 % 2 * 4);
             x[0] += __uint_as_float(w.x << 16); x[1] += __uint_as_float(w.x & 0xffff0000u);
             x[2] += __uint_as_float(w.y << 16); x[3] += __uint_as_float(w.y & 0xffff0000u);
         }
@@ -937,27 +925,41 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     const auto fourRows = [&](const float *from, uint32_t tile) { return *(const f32x4*)(from + tile * 16 + 4 * g); };
     const auto sumOf16 = [](float x) { x += partner<1>(x); x += partner<2>(x); x += partner<4>(x); return x + partner<8>(x); };
 
-    f32x4 dq[MINE], rS[MINE], dk[MINE], dqk[SQUARES], dkk[SQUARES];
+    f32x4 dq[MINE][TILES], rS[MINE][TILES], dk[MINE][TILES], dqk[SQUARES], dkk[SQUARES];
     #pragma unroll
-    for(int m = 0; m < MINE; m++) { dq[m] = rS[m] = dk[m] = f32x4{0, 0, 0, 0}; }
+    for(int m = 0; m < MINE; m++) {
+        #pragma unroll
+        for(int t = 0; t < TILES; t++) { dq[m][t] = rS[m][t] = dk[m][t] = f32x4{0, 0, 0, 0}; }
+    }
     #pragma unroll
     for(int q = 0; q < SQUARES; q++) { dqk[q] = dkk[q] = f32x4{0, 0, 0, 0}; }
-    float stateDot = 0.0f, valueDot = 0.0f, betaDot = 0.0f;
+    float stateDot = 0.0f, valueDot[ITEMS] = {}, betaDot[ITEMS] = {};
     for(uint32_t v = 0; v < a.padded; v += 32) {
-        const f32x4 s0a = {nextState[0].x, nextState[0].y, nextState[0].z, nextState[0].w}, s0b = {nextState[1].x, nextState[1].y, nextState[1].z, nextState[1].w};
-        const f32x4 dsa = {nextDState[0].x, nextDState[0].y, nextDState[0].z, nextDState[0].w}, dsb = {nextDState[1].x, nextDState[1].y, nextDState[1].z, nextDState[1].w};
+        f32x4 s0[MINE][2], ds[MINE][2];
+        #pragma unroll
+        for(int m = 0; m < MINE; m++) {
+            #pragma unroll
+            for(int h = 0; h < 2; h++) {
+                const uint32_t offset = keyOf(m) * a.padded + v + 8 * g + 4 * h;
+                s0[m][h] = *(const f32x4*)(stateRows + offset);
+                ds[m][h] = *(const f32x4*)(dStateRows + offset);
+            }
+        }
         __syncthreads();
-        if(stages) {
-            const float dr[4] = {nextDR.x, nextDR.y, nextDR.z, nextDR.w}, w[4] = {nextW.x, nextW.y, nextW.z, nextW.w};
-            float dout[4];
+        #pragma unroll
+        for(int i = 0; i < ITEMS; i++) {
+            const bool there = rowOfItem(i) < count;
+            float dr[4], w[4], dout[4];
             #pragma unroll
             for(int e = 0; e < 4; e++) {
-                dout[e] = widen(nextDout.v[e]);
-                valueDot = __builtin_fmaf(widen(nextValues.v[e]), dr[e], valueDot);
-                betaDot = __builtin_fmaf(w[e], dr[e], betaDot);
+                dr[e] = there ? nextDR[i][e] : 0.0f;
+                w[e] = there ? nextW[i][e] : 0.0f;
+                dout[e] = there ? widen(nextDout[i].v[e]) : 0.0f;
+                valueDot[i] = __builtin_fmaf(there ? widen(nextValues[i].v[e]) : 0.0f, dr[e], valueDot[i]);
+                betaDot[i] = __builtin_fmaf(w[e], dr[e], betaDot[i]);
             }
             uint2 words[3], own[NP];
-            uint16_t *const to = stage + unitAt<32>(stageRow, stageAt / 8) + stageAt % 8;
+            uint16_t *const to = stage + unitAt<32>(rowOfItem(i), stageAt / 8) + stageAt % 8;
             splitFour<NP>(dout, own);
             #pragma unroll
             for(int k = 0; k < NP; k++) { *(uint2*)(to + k * VP) = own[k]; }
@@ -970,18 +972,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         }
         __syncthreads();
         if(v + 32 < a.padded) { request(v + 32); }
-        #pragma unroll
-        for(int e = 0; e < 4; e++) { stateDot = __builtin_fmaf(s0a[e], dsa[e], stateDot); stateDot = __builtin_fmaf(s0b[e], dsb[e], stateDot); }
-        const Planes<3> state = split<3>(s0a, s0b), dState = split<3>(dsa, dsb);
-        #pragma unroll
-        for(int m = 0; m < MINE; m++) {
-            inTurn();
-            const uint32_t offset = unitAt<32>(tileOf(m) * 16 + n16, g);
-            const Planes<NP> out = fetch<NP>(doutPlanes + offset, VP);
-            const Planes<3> r = fetch<3>(dRPlanes + offset, VP), w = fetch<3>(wPlanes + offset, VP);
-            multiplyThree(out, state, dq[m], r, state, rS[m], w, dState, dk[m]);
-        }
-        if(squares) {
+        {
             const Planes<3> other = fetch<3>(wPlanes + unitAt<32>(squareColumn * 16 + n16, g), VP);
             #pragma unroll
             for(int q = 0; q < SQUARES; q++) {
@@ -992,26 +983,42 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
                 dkk[q] = multiply(fetch<3>(dRPlanes + offset, VP), other, dkk[q]);
             }
         }
+        #pragma unroll
+        for(int m = 0; m < MINE; m++) {
+            inTurn();
+            #pragma unroll
+            for(int h = 0; h < 2; h++) {
+                #pragma unroll
+                for(int e = 0; e < 4; e++) { stateDot = __builtin_fmaf(s0[m][h][e], ds[m][h][e], stateDot); }
+            }
+            const Planes<3> state = split<3>(s0[m][0], s0[m][1]), dState = split<3>(ds[m][0], ds[m][1]);
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) {
+                inTurn();
+                const uint32_t offset = unitAt<32>(t * 16 + n16, g);
+                const Planes<NP> out = fetch<NP>(doutPlanes + offset, VP);
+                const Planes<3> r = fetch<3>(dRPlanes + offset, VP), w = fetch<3>(wPlanes + offset, VP);
+                multiplyThree(out, state, dq[m][t], r, state, rS[m][t], w, dState, dk[m][t]);
+            }
+        }
         inTurn();
     }
-    // what the rows' factors make of them, and the gates' share
+    // what the rows' factors make of them
     float endDot = 0.0f;
     #pragma unroll
-    for(int m = 0; m < MINE; m++) {
-        const uint32_t tile = tileOf(m);
-        const f32x4 q = valuesAt(L::queries, tile) * fourRows(queryUnit, tile), k = valuesAt(L::keys, tile) * fourRows(keyUnit, tile);
-        const f32x4 grown = fourRows(since, tile), by = fourRows(beta, tile);
-        dq[m] *= a.scale * grown;
-        dk[m] *= fourRows(until, tile) * by;
+    for(int t = 0; t < TILES; t++) {
+        const f32x4 grown = fourRows(since, t), by = fourRows(beta, t), last = fourRows(until, t) * by, keyLength = fourRows(keyUnit, t);
         #pragma unroll
-        for(int r = 0; r < 4; r++) {
-            endDot = __builtin_fmaf(k[r], dk[m][r], endDot);
-            const float dot = sumOf16(q[r] * dq[m][r]);
-            if(n16 == 0) { queryDots[wave * C + tile * 16 + 4 * g + r] = dot; }
+        for(int m = 0; m < MINE; m++) {
+            const f32x4 k = valuesAt(L::keys, t, m) * keyLength;
+            dq[m][t] *= a.scale * grown;
+            dk[m][t] *= last;
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { endDot = __builtin_fmaf(k[r], dk[m][t][r], endDot); }
+            dk[m][t] -= grown * by * rS[m][t];
         }
-        dk[m] -= grown * by * rS[m];
     }
-    if(squares) {
+    {
         const uint32_t column = squareColumn * 16 + n16;
         const float betaColumn = beta[column];
         const double sumColumn = sums[column];
@@ -1021,57 +1028,28 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             #pragma unroll
             for(int r = 0; r < 4; r++) {
                 const uint32_t row = squareRow(q) * 16 + 4 * g + r;
-                float dot = 0.0f;
-                if(row >= column) {
-                    const float between = decayOver(sums[row] - sumColumn), x = dqk[q][r] * betaColumn;
-                    dot = x * a.score[(at * C + row) * C + column];
-                    dqk[q][r] = a.scale * between * x;
-                    dkk[q][r] = row > column ? -between * (by[r] * betaColumn * dkk[q][r]) : 0.0f;
-                }
-                else { dqk[q][r] = dkk[q][r] = 0.0f; }
-                dot = sumOf16(dot);
-                if(n16 == 0) { keyDots[squareColumn * C + row] = dot; }
+                const float between = row >= column ? decayOver(sums[row] - sumColumn) : 0.0f;
+                dqk[q][r] = row >= column ? a.scale * between * (dqk[q][r] * betaColumn) : 0.0f;
+                dkk[q][r] = row > column ? -between * (by[r] * betaColumn * dkk[q][r]) : 0.0f;
             }
         }
     }
     #pragma unroll
     for(int w = 1; w < 64; w *= 2) { stateDot += __shfl_xor(stateDot, w); endDot += __shfl_xor(endDot, w); }
-    // (wavefronts that split a key tile's rows have read the same state)
-    if(lane == 0) { ends[wave] = wave < KEY_TILES ? decay * stateDot + endDot : endDot; }
-    valueDot += partner<1>(valueDot); valueDot += partner<2>(valueDot); valueDot += partner<4>(valueDot);
-    betaDot += partner<1>(betaDot); betaDot += partner<2>(betaDot); betaDot += partner<4>(betaDot);
-    if(stages && stageAt == 0) {
-        valueDots[stageRow] = valueDot * beta[stageRow];
-        if(d.beta.data && stageRow < count) { (rowsOf<float>(d.beta, a.chunks, p) + (uint64_t)(begin + stageRow) * d.beta.rowStride)[head] = betaDot; }
-    }
-    __syncthreads();
-    if(d.g.data && wave == 0) {
-        double sum = 0.0;
-        if(lane < C) {
-            sum = -(double)valueDots[lane];
-            // (a row's dots lie with the wavefronts that have its tile)
-            const uint32_t firstWave = (lane / 16) % SPLIT * KEY_TILES;
-            #pragma unroll
-            for(int w = 0; w < KEY_TILES; w++) { sum += queryDots[(firstWave + w) * C + lane]; }
-            #pragma unroll
-            for(int w = 0; w < TILES; w++) { sum += keyDots[w * C + lane]; }
-            if(lane == C - 1) {
-                #pragma unroll
-                for(int w = 0; w < 8; w++) { sum += ends[w]; }
-            }
+    if(lane == 0) { ends[wave] = decay * stateDot + endDot; }
+    #pragma unroll
+    for(int i = 0; i < ITEMS; i++) {
+        const uint32_t row = rowOfItem(i);
+        valueDot[i] += partner<1>(valueDot[i]); valueDot[i] += partner<2>(valueDot[i]); valueDot[i] += partner<4>(valueDot[i]);
+        betaDot[i] += partner<1>(betaDot[i]); betaDot[i] += partner<2>(betaDot[i]); betaDot[i] += partner<4>(betaDot[i]);
+        if(stageAt == 0) {
+            valueDots[row] = valueDot[i] * beta[row];
+            if(d.beta.data && row < count) { (rowsOf<float>(d.beta, a.chunks, p) + (uint64_t)(begin + row) * d.beta.rowStride)[head] = betaDot[i]; }
         }
-        #pragma unroll
-        for(int w = 1; w < C; w *= 2) {
-            const double behind = __shfl_down(sum, w);
-            if(lane + w < C) { sum += behind; }
-        }
-        if(lane < count) { (rowsOf<float>(d.g, a.chunks, p) + (uint64_t)(begin + lane) * d.g.rowStride)[head] = (float)sum; }
     }
-    if(!d.q.data && !d.k.data) { return; }
 
     // squares times queries and keys
     const auto storeSquares = [&](bool transposed, const f32x4 (&square)[SQUARES], const float *rowFactor, const float *columnFactor) {
-        if(!squares) { return; }
         #pragma unroll
         for(int q = 0; q < SQUARES; q++) {
             const uint32_t column = squareColumn * 16 + n16, row = squareRow(q) * 16 + 4 * g;
@@ -1092,73 +1070,123 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             }
         }
     };
-    const auto timesColumns = [&](uint32_t from, f32x4 (&to)[MINE]) {
+    // (`first` and `last`: the blocks of 32 columns that are not zero in rows of block b)
+    const auto timesColumns = [&](uint32_t from, f32x4 (&to)[MINE][TILES], bool lower, bool upper) {
         #pragma unroll
-        for(int s = 0; s < TILES / 2; s++) {
-            const uint32_t row = 32 * s + 8 * g + n16 / 4, unit = 2 * keyTile + n16 % 4 / 2, half = n16 % 2 * 4;
-            const Planes<NP> b = fetchColumn<NP>(planes + from + unitAt<DK>(row, unit) + half, planes + from + unitAt<DK>(row + 4, unit) + half, C * DK);
+        for(int m = 0; m < MINE; m++) {
             #pragma unroll
-            for(int m = 0; m < MINE; m++) { inTurn(); to[m] = multiply(fetch<3>(stage + unitAt<C>(tileOf(m) * 16 + n16, 4 * s + g), C * C), b, to[m]); }
+            for(int s = 0; s < TILES / 2; s++) {
+                inTurn();
+                const uint32_t row = 32 * s + 8 * g + n16 / 4, unit = 2 * (wave * MINE + m) + n16 % 4 / 2, half = n16 % 2 * 4;
+                const Planes<NP> b = fetchColumn<NP>(planes + from + unitAt<DK>(row, unit) + half, planes + from + unitAt<DK>(row + 4, unit) + half, C * DK);
+                #pragma unroll
+                for(int t = 0; t < TILES; t += 2) {
+                    if((t / 2 < s && !upper) || (t / 2 > s && !lower)) { continue; }
+                    const Planes<3> rows[2] = {fetch<3>(stage + unitAt<C>(t * 16 + n16, 4 * s + g), C * C), fetch<3>(stage + unitAt<C>(t * 16 + 16 + n16, 4 * s + g), C * C)};
+                    f32x4 sum[2] = {to[m][t], to[m][t + 1]};
+                    multiplyAll(rows, b, sum);
+                    to[m][t] = sum[0];
+                    to[m][t + 1] = sum[1];
+                }
+            }
         }
     };
+    __syncthreads();
     storeSquares(false, dqk, nullptr, keyUnit);
     __syncthreads();
-    timesColumns(L::keys, dq);
+    timesColumns(L::keys, dq, true, false);
+    // q^.dq^, for the gates and for the queries' lengths
+    #pragma unroll
+    for(int t = 0; t < TILES; t++) {
+        const f32x4 queryLength = fourRows(queryUnit, t);
+        f32x4 dot = {0, 0, 0, 0};
+        #pragma unroll
+        for(int m = 0; m < MINE; m++) { dot += valuesAt(L::queries, t, m) * queryLength * dq[m][t]; }
+        #pragma unroll
+        for(int r = 0; r < 4; r++) { dot[r] = sumOf16(dot[r]); }
+        if(n16 == 0) { *(f32x4*)(queryDots + wave * C + t * 16 + 4 * g) = dot; }
+    }
     __syncthreads();
+    if(d.g.data && wave == 0) {
+        double sum = 0.0;
+        if(lane < C) {
+            sum = -(double)valueDots[lane];
+            #pragma unroll
+            for(int w = 0; w < 4; w++) { sum += queryDots[w * C + lane]; }
+            if(lane == C - 1) {
+                #pragma unroll
+                for(int w = 0; w < 4; w++) { sum += ends[w]; }
+            }
+        }
+        #pragma unroll
+        for(int w = 1; w < C; w *= 2) {
+            const double behind = __shfl_down(sum, w);
+            if(lane + w < C) { sum += behind; }
+        }
+        if(lane < count) { (rowsOf<float>(d.g, a.chunks, p) + (uint64_t)(begin + lane) * d.g.rowStride)[head] = (float)sum; }
+    }
+    if(!d.q.data && !d.k.data) { return; }
     storeSquares(true, dqk, queryUnit, nullptr);
     __syncthreads();
-    timesColumns(L::queries, dk);
+    timesColumns(L::queries, dk, false, true);
+    __syncthreads();
+    // (both triangles of what is symmetric)
+    storeSquares(true, dkk, keyUnit, nullptr);
+    __syncthreads();
+    timesColumns(L::keys, dk, false, true);
     __syncthreads();
     storeSquares(false, dkk, nullptr, keyUnit);
     __syncthreads();
-    timesColumns(L::keys, dk);
-    __syncthreads();
-    storeSquares(true, dkk, keyUnit, nullptr);
-    __syncthreads();
-    timesColumns(L::keys, dk);
+    timesColumns(L::keys, dk, true, false);
     if(a.group > 1) {
         float *const to = d.shared + at * 2 * C * DK;
-        storeResultTiles<MINE, SPLIT>(to, DK, firstRow, g, key, dq);
-        storeResultTiles<MINE, SPLIT>(to + C * DK, DK, firstRow, g, key, dk);
+        #pragma unroll
+        for(int m = 0; m < MINE; m++) {
+            #pragma unroll
+            for(int t = 0; t < TILES; t++) {
+                #pragma unroll
+                for(int r = 0; r < 4; r++) {
+                    to[(t * 16 + 4 * g + r) * DK + keyOf(m)] = dq[m][t][r];
+                    to[(C + t * 16 + 4 * g + r) * DK + keyOf(m)] = dk[m][t][r];
+                }
+            }
+        }
         return;
     }
 
     // through the lengths of queries and keys
     if(a.normalise) {
         #pragma unroll
-        for(int m = 0; m < MINE; m++) {
-            const f32x4 q = valuesAt(L::queries, tileOf(m)) * fourRows(queryUnit, tileOf(m)), k = valuesAt(L::keys, tileOf(m)) * fourRows(keyUnit, tileOf(m));
+        for(int t = 0; t < TILES; t++) {
+            const f32x4 keyLength = fourRows(keyUnit, t);
+            f32x4 dot = {0, 0, 0, 0};
             #pragma unroll
-            for(int r = 0; r < 4; r++) {
-                const float x = sumOf16(q[r] * dq[m][r]), y = sumOf16(k[r] * dk[m][r]);
-                if(n16 == 0) { queryDots[wave * C + tileOf(m) * 16 + 4 * g + r] = x; keyDots[wave * C + tileOf(m) * 16 + 4 * g + r] = y; }
-            }
+            for(int m = 0; m < MINE; m++) { dot += valuesAt(L::keys, t, m) * keyLength * dk[m][t]; }
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { dot[r] = sumOf16(dot[r]); }
+            if(n16 == 0) { *(f32x4*)(keyDots + wave * C + t * 16 + 4 * g) = dot; }
         }
         __syncthreads();
     }
     #pragma unroll
-    for(int m = 0; m < MINE; m++) {
-        const uint32_t tile = tileOf(m);
-        const f32x4 queryLength = fourRows(queryUnit, tile), keyLength = fourRows(keyUnit, tile);
-        f32x4 x = dq[m], y = dk[m];
+    for(int t = 0; t < TILES; t++) {
+        const f32x4 queryLength = fourRows(queryUnit, t), keyLength = fourRows(keyUnit, t);
+        f32x4 queryDot = {0, 0, 0, 0}, keyDot = {0, 0, 0, 0};
         if(a.normalise) {
-            f32x4 queryDot = {0, 0, 0, 0}, keyDot = {0, 0, 0, 0};
             #pragma unroll
-            for(int w = 0; w < KEY_TILES; w++) {
-                queryDot += fourRows(queryDots + (firstRow * KEY_TILES + w) * C, tile);
-                keyDot += fourRows(keyDots + (firstRow * KEY_TILES + w) * C, tile);
-            }
-            x -= valuesAt(L::queries, tile) * queryLength * queryDot;
-            y -= valuesAt(L::keys, tile) * keyLength * keyDot;
+            for(int w = 0; w < 4; w++) { queryDot += fourRows(queryDots + w * C, t); keyDot += fourRows(keyDots + w * C, t); }
         }
-        x *= queryLength;
-        y *= keyLength;
         #pragma unroll
-        for(int r = 0; r < 4; r++) {
-            const uint32_t row = tile * 16 + 4 * g + r;
-            if(row < count && key < a.keys) {
-                if(d.q.data) { (rowsOf<T>(d.q, a.chunks, p) + (uint64_t)(begin + row) * d.q.rowStride)[keyHead * a.keys + key] = narrow<T>(x[r]); }
-                if(d.k.data) { (rowsOf<T>(d.k, a.chunks, p) + (uint64_t)(begin + row) * d.k.rowStride)[keyHead * a.keys + key] = narrow<T>(y[r]); }
+        for(int m = 0; m < MINE; m++) {
+            const f32x4 x = (dq[m][t] - valuesAt(L::queries, t, m) * queryLength * queryDot) * queryLength, y = (dk[m][t] - valuesAt(L::keys, t, m) * keyLength * keyDot) * keyLength;
+            const uint32_t key = keyOf(m);
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = t * 16 + 4 * g + r;
+                if(row < count && key < a.keys) {
+                    if(d.q.data) { (rowsOf<T>(d.q, a.chunks, p) + (uint64_t)(begin + row) * d.q.rowStride)[keyHead * a.keys + key] = narrow<T>(x[r]); }
+                    if(d.k.data) { (rowsOf<T>(d.k, a.chunks, p) + (uint64_t)(begin + row) * d.k.rowStride)[keyHead * a.keys + key] = narrow<T>(y[r]); }
+                }
             }
         }
     }
