@@ -146,11 +146,13 @@ template<int LANES, int E, int VEC> __device__ inline float normalise(const Norm
     for(int e = 0; e < E; e++) { x[e] = hasElement<E, VEC>(at, e, a.channels) ? (x[e] - mean) * r : 0.0f; }
     return r;
 }
-__device__ inline float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
+// (the hardware's exponential and reciprocal: a few steps of fp32; a division and an exponential to the last bit were a third of the instructions of a gated row)
+__device__ inline float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
 
-// Work-groups of 256 threads where 16 lanes or a wavefront have a row, else of 512 or what one row takes; each walks rows that are a grid apart, with the parameters in registers
-// and the next row asked for while one is worked on.  (4096 x 4096 in bf16: 63 us with a row a work-group, whose parameters are four times the row.)
-template<typename T, int LANES, int E, int VEC>
+// Bound by memory: each row is read once and written once.  Work-groups of 256 threads where 16 lanes or a wavefront have a row, else of what rows take; each walks rows that are a grid apart,
+// with the parameters in registers and the next row asked for while one is worked on.  4096 x 4096 in bf16: 62 us with a row a work-group (its parameters are four times the row), 15.7 so (4.3 TB/s);
+// 131,072 heads of 128 with a gate 20.7 (4.9 TB/s).
+template<typename T, int LANES, int E, int VEC, bool GATE>
 __global__ __launch_bounds__(LANES ? 256 : 1024)
 void normKernel(NormArgs a)
 {
@@ -167,7 +169,7 @@ void normKernel(NormArgs a)
         const bool valid = n < a.rows;
         const uint32_t sequence = valid ? (uint32_t)n / a.length : 0, row = valid ? (uint32_t)n - sequence * a.length : 0;
         nextX = requestRow<T, E, VEC>(normRow<const T>(a.x, sequence, row), at, a.channels, valid);
-        if(a.gate.data) { nextZ = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
+        if constexpr(GATE) { nextZ = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
     };
     uint64_t first = (uint64_t)blockIdx.x * at.groups;
     request(first + at.group);
@@ -175,13 +177,13 @@ void normKernel(NormArgs a)
         const uint64_t n = first + at.group;
         float x[E], z[E];
         takeRow(nextX, x);
-        if(a.gate.data) { takeRow(nextZ, z); }
+        if constexpr(GATE) { takeRow(nextZ, z); }
         request(n + step);
         normalise<LANES, E, VEC>(a, x, at, shared, turn, inWave, inWaveShare);
         #pragma unroll
         for(int e = 0; e < E; e++) {
             x[e] = __builtin_fmaf(x[e], weight[e], bias[e]);
-            if(a.gate.data) { x[e] *= z[e] * logistic(z[e]); }
+            if constexpr(GATE) { x[e] *= z[e] * logistic(z[e]); }
         }
         if(n < a.rows) {
             const uint32_t sequence = (uint32_t)n / a.length, row = (uint32_t)n - sequence * a.length;
@@ -191,8 +193,9 @@ void normKernel(NormArgs a)
 }
 
 // With y = x' weight + bias, s the gate's factor z sigmoid(z) and d = dout s:
+// Bound by memory: 16384 x 2048 in bf16 50 us with the closing sums (4.0 TB/s), 134 with a row's sums over its work-group one behind another.
 //   dgate = dout y s',  dweight += d x',  dbias += d,  dx = (v - x' mean(v x') - mean(v)) / length, v = d weight (without the last mean for `rms`)
-template<typename T, int LANES, int E, int VEC>
+template<typename T, int LANES, int E, int VEC, bool GATE>
 __global__ __launch_bounds__(LANES ? 256 : 1024)
 void normBackwardKernel(NormArgs a)
 {
@@ -200,9 +203,9 @@ void normBackwardKernel(NormArgs a)
     extern __shared__ float rows[];
     uint32_t turn = 0;
     const NormPlace at = normPlace<LANES>(a);
-    float weight[E], bias[E], dweight[E] = {}, dbias[E] = {};
+    float weight[E], bias[GATE ? E : 1], dweight[E] = {}, dbias[E] = {};
     loadParameters<E, VEC>(a.weight, 1.0f, at, a.channels, weight);
-    loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias);
+    if constexpr(GATE) { loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias); }
     const float inWave = LANES ? 0.0f : elementsOf<E, VEC>(at, at.lane >> 6, a.channels), inWaveShare = inWave > 0.0f ? 1.0f / inWave : 0.0f;
     const uint64_t step = (uint64_t)gridDim.x * at.groups;
     NormRow<T, E, VEC> nextX, nextD;
@@ -222,10 +225,10 @@ void normBackwardKernel(NormArgs a)
         takeRow(nextX, x);
         takeRow(nextD, d);
         NormRow<T, E, VEC> gate{};
-        if(a.gate.data) { gate = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
+        if constexpr(GATE) { gate = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
         request(n + step);
         const float r = normalise<LANES, E, VEC>(a, x, at, shared, turn, inWave, inWaveShare);
-        if(a.gate.data) {
+        if constexpr(GATE) {
             float z[E];
             takeRow(gate, z);
             #pragma unroll
@@ -275,8 +278,11 @@ void normBackwardKernel(NormArgs a)
             for(int e = 0; e < E; e++) { rows[e * blockDim.x + threadIdx.x] = sum[e]; }
             __syncthreads();
             if(at.group) { continue; }
-            #pragma unroll
-            for(int e = 0; e < E; e++) { for(uint32_t k = 1; k < at.groups; k++) { sum[e] += rows[e * blockDim.x + k * at.lanes + at.lane]; } }
+            #pragma unroll 1
+            for(uint32_t k = 1; k < at.groups; k++) {
+                #pragma unroll
+                for(int e = 0; e < E; e++) { sum[e] += rows[e * blockDim.x + k * at.lanes + at.lane]; }
+            }
         }
         #pragma unroll
         for(int e = 0; e < E; e++) { if(hasElement<E, VEC>(at, e, a.channels)) { to[which * a.channels + (e / VEC * at.lanes + at.lane) * VEC + e % VEC] = sum[e]; } }
@@ -369,37 +375,55 @@ uint32_t vectorOf(uint32_t size, uint32_t channels, std::initializer_list<const 
     for(const gennmi_rows_t *r : arrays) { whole = whole && (!r->data || ((uintptr_t)r->data % 16 == 0 && r->rowStride % vector == 0 && r->sequenceStride % vector == 0)); }
     return whole ? vector : 1;
 }
-struct NormPlan { uint32_t lanes, rowLanes, groups, threads, blocks; };       // lanes 0: wavefronts share a row, rowLanes of them
+struct NormPlan { uint32_t each, lanes, rowLanes, groups, threads, blocks; };       // lanes 0: wavefronts share a row, rowLanes of them
+// Rows of up to 128 channels: 16 lanes with 8 elements each; of up to 512: a wavefront.  Above that wavefronts share a row in the forward pass, 16 elements a lane; gradients of up to 1024 channels
+// (2048 without a gate) stay with one wavefront, whose rows need no barrier, as long as its registers hold four arrays of them.  us in bf16: 16384 x 2048 a wavefront a row
+// and two, forward 32, 28, gradients 50, 62; gradients of 16384 x 1024 29, 35, of 8192 x 2048 with a gate 67, 48.
+// Work-groups: as many as the chip holds at once, or a quarter of the rows where that is less, as each leaves a sum for every channel.
 NormPlan normPlan(const gennmi_layer_norm_t &c, bool gradients)
 {
     const uint64_t rows = totalRows(c.sequences);
+    const bool gate = c.gate.data != nullptr;
     NormPlan p;
-    p.lanes = c.channels <= 128 ? 16 : c.channels <= 512 ? 64 : 0;
-    const uint32_t each = c.channels <= 8192 ? 8 : 16;
-    p.rowLanes = p.lanes ? p.lanes : ((c.channels + each - 1) / each + 63) / 64 * 64;
-    p.groups = p.lanes ? 256 / p.lanes : std::max(1u, 512 / p.rowLanes);
+    p.lanes = c.channels <= 128 ? 16 : c.channels <= 512 || (gradients && c.channels <= (gate ? 1024u : 2048u)) ? 64 : 0;
+    p.each = p.lanes ? (c.channels <= 512 ? 8 : c.channels <= 1024 ? 16 : 32) : gradients && c.channels <= 8192 ? 8 : 16;
+    p.rowLanes = p.lanes ? p.lanes : ((c.channels + p.each - 1) / p.each + 63) / 64 * 64;
+    p.groups = p.lanes ? 256 / p.lanes : std::max(1u, (gradients ? 512 : 256) / p.rowLanes);
     p.threads = p.groups * p.rowLanes;
-    // Work-groups: for gradients fewer, with four rows at least, as each leaves a sum for every channel
-    const uint64_t needed = (rows + p.groups - 1) / p.groups;
-    p.blocks = (uint32_t)std::min<uint64_t>(gradients ? (needed + 3) / 4 : needed, gradients ? 1024 : 2048);
+    const uint64_t needed = (rows + p.groups - 1) / p.groups, most = gradients ? (p.each == 8 && (p.lanes || !gate) ? 768 : 512) : p.lanes ? 2048 : 1024;
+    p.blocks = (uint32_t)std::min<uint64_t>(gradients ? (needed + 3) / 4 : needed, most);
     return p;
 }
-template<typename T, int VEC, typename F> int withNormLayout(const NormPlan &p, uint32_t channels, F &&f)
+template<bool GRADIENTS, int VEC, typename F> int withNormLayout(const NormPlan &p, F &&f)
 {
     typedef std::integral_constant<int, VEC> Vec;
-    typedef std::integral_constant<int, 8> Eight;
-    if(p.lanes == 16) { return f(std::integral_constant<int, 16>{}, Eight{}, Vec{}); }
-    if(p.lanes == 64) { return f(std::integral_constant<int, 64>{}, Eight{}, Vec{}); }
-    if(channels <= 8192) { return f(std::integral_constant<int, 0>{}, Eight{}, Vec{}); }
-    return f(std::integral_constant<int, 0>{}, std::integral_constant<int, 16>{}, Vec{});
+    const std::integral_constant<int, 8> eight;
+    const std::integral_constant<int, 16> sixteen;
+    if(p.lanes == 16) { return f(sixteen, eight, Vec{}); }
+    if(p.lanes == 64) {
+        const std::integral_constant<int, 64> wave;
+        if constexpr(GRADIENTS) {
+            if(p.each == 32) { return f(wave, std::integral_constant<int, 32>{}, Vec{}); }
+            if(p.each == 16) { return f(wave, sixteen, Vec{}); }
+        }
+        return f(wave, eight, Vec{});
+    }
+    const std::integral_constant<int, 0> several;
+    if constexpr(GRADIENTS) { if(p.each == 8) { return f(several, eight, Vec{}); } }
+    return f(several, sixteen, Vec{});
 }
-template<typename F> int withNorm(const gennmi_layer_norm_t &c, const NormPlan &p, uint32_t vector, F &&f)
+template<bool GRADIENTS, typename F> int withNorm(const gennmi_layer_norm_t &c, const NormPlan &p, uint32_t vector, F &&f)
 {
     return withType(c.type, [&](auto t) {
         typedef decltype(t) T;
-        const auto g = [&](auto lanes, auto each, auto vec) { return f(t, lanes, each, vec); };
-        if(vector > 1) { return withNormLayout<T, 16 / sizeof(T)>(p, c.channels, g); }
-        return withNormLayout<T, 1>(p, c.channels, g);
+        const auto g = [&](auto lanes, auto each, auto vec) {
+            if(!c.gate.data) { return f(t, lanes, each, vec, std::false_type{}); }
+            // (with a gate rows of 32 elements a lane are not planned)
+            if constexpr(decltype(each)::value <= 16) { return f(t, lanes, each, vec, std::true_type{}); }
+            else { return (int)GENNMI_EUNSUPPORTED; }
+        };
+        if(vector > 1) { return withNormLayout<GRADIENTS, 16 / sizeof(T)>(p, g); }
+        return withNormLayout<GRADIENTS, 1>(p, g);
     });
 }
 NormArgs normArgs(const gennmi_layer_norm_t &c, const NormPlan &p, bool flat)
@@ -433,8 +457,8 @@ int gennmi_layer_norm(const gennmi_layer_norm_t *norm, void *stream)
         const NormPlan p = normPlan(*norm, false);
         const auto arrays = {&norm->x, &norm->gate, &norm->out};
         const NormArgs a = normArgs(*norm, p, oneBehindAnother(s, arrays));
-        const int rc = withNorm(*norm, p, vectorOf(size, norm->channels, arrays), [&](auto t, auto lanes, auto each, auto vec) {
-            normKernel<decltype(t), decltype(lanes)::value, decltype(each)::value, decltype(vec)::value><<<dim3(p.blocks), dim3(p.threads), 0, (hipStream_t)stream>>>(a);
+        const int rc = withNorm<false>(*norm, p, vectorOf(size, norm->channels, arrays), [&](auto t, auto lanes, auto each, auto vec, auto gate) {
+            normKernel<decltype(t), decltype(lanes)::value, decltype(each)::value, decltype(vec)::value, decltype(gate)::value><<<dim3(p.blocks), dim3(p.threads), 0, (hipStream_t)stream>>>(a);
             return gennmi_detail::afterLaunch(what);
         });
         if(rc) { return rc; }
@@ -482,8 +506,8 @@ int gennmi_layer_norm_backward(const gennmi_layer_norm_t *norm, const gennmi_lay
         a.dout = g.out; a.dx = g.x; a.dgate = g.gate;
         a.sums = sums ? (float*)workspace : nullptr;
         if(a.rows) {
-            const int rc = withNorm(*norm, p, vectorOf(size, channels, arrays), [&](auto t, auto lanes, auto each, auto vec) {
-                normBackwardKernel<decltype(t), decltype(lanes)::value, decltype(each)::value, decltype(vec)::value><<<dim3(p.blocks), dim3(p.threads), sums && p.groups > 1 ? p.threads * decltype(each)::value * sizeof(float) : 0, (hipStream_t)stream>>>(a);
+            const int rc = withNorm<true>(*norm, p, vectorOf(size, channels, arrays), [&](auto t, auto lanes, auto each, auto vec, auto gate) {
+                normBackwardKernel<decltype(t), decltype(lanes)::value, decltype(each)::value, decltype(vec)::value, decltype(gate)::value><<<dim3(p.blocks), dim3(p.threads), sums && p.groups > 1 ? p.threads * decltype(each)::value * sizeof(float) : 0, (hipStream_t)stream>>>(a);
                 return gennmi_detail::afterLaunch(what);
             });
             if(rc) { return rc; }
