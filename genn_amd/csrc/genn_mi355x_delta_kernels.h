@@ -824,7 +824,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
 // and g's: with states and u in units of the decay so far, outputs grow with it and values shrink, so that what the sum of g up to row i gains the loss
 // is q^[i].dq^[i] - v[i].dv[i], and at the chunk's last row the state behind it times its gradient as well.
 // A work-group has a chunk and a head.  Products are summed over the values, 32 at a time, with what multiplies S and dS
-// in LDS (the next 32 on their way meanwhile); a wavefront has the results' columns of a quarter of the keys, S' and dS' straight from memory.  What bounds it is waiting, for memory and at barriers: two work-groups
+// in LDS; a wavefront has the results' columns of a quarter of the keys, S' and dS' straight from memory.  What bounds it is waiting, for memory and at barriers: two work-groups
 // of four wavefronts fit a compute unit and fill each other's pauses.  Where heads share keys, what each finds for them is left for deltaSharedKernel to add up.
 template<typename T, int C, int DK> struct GradientLayout
 {
@@ -869,32 +869,40 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     // what multiplies S and dS: eight threads a row, four values each
     const float *const stateRows = a.states + at * DK * a.padded, *const dStateRows = d.states + at * DK * a.padded;
     typedef Pack<T, 4> Four;
-    f32x4 nextDR[ITEMS], nextW[ITEMS];
-    Four nextDout[ITEMS], nextValues[ITEMS];
+    f32x4 inDR[ITEMS], inW[ITEMS];
+    Four inDout[ITEMS], inValues[ITEMS];
     const auto rowOfItem = [&](int i) { return tid / 8 + 32 * i; };
     const uint32_t stageAt = tid % 8 * 4;
-    const auto four = [&](const T *from, uint32_t v) {
-        Four x{};
-        if(a.wideValues) { if(v < a.values) { x = *(const Four*)(from + v); } }
-        else {
-            #pragma unroll
-            for(int e = 0; e < 4; e++) { if(v + e < a.values) { x.v[e] = from[v + e]; } }
-        }
-        return x;
-    };
+    const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)begin * d.out.rowStride + head * a.values, *const values = rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)begin * a.v.rowStride + head * a.values;
     const auto request = [&](uint32_t v) {
         #pragma unroll
         for(int i = 0; i < ITEMS; i++) {
-            // (rows that are not there: another's, and nothing of it is used)
-            const uint64_t row = rowOfItem(i);
-            nextDR[i] = *(const f32x4*)(d.errors + (at * C + row) * a.padded + v + stageAt);
-            nextW[i] = *(const f32x4*)(a.errors + (at * C + row) * a.padded + v + stageAt);
-            const uint64_t there = begin + min((uint32_t)row, count - 1);
-            nextDout[i] = four(rowAt<T>(d.out, a.chunks, p, there) + head * a.values, v + stageAt);
-            nextValues[i] = four(rowAt<T>(a.v, a.chunks, p, there) + head * a.values, v + stageAt);
+            inDR[i] = *(const f32x4*)(d.errors + (at * C + rowOfItem(i)) * a.padded + v + stageAt);
+            inW[i] = *(const f32x4*)(a.errors + (at * C + rowOfItem(i)) * a.padded + v + stageAt);
+        }
+        // (rows and values that are not there: others, and nothing of them is used; no branch an access, with which the compiler would wait for each)
+        if(a.wideValues) {
+            const uint32_t there = v + stageAt < a.values ? v + stageAt : 0;
+            #pragma unroll
+            for(int i = 0; i < ITEMS; i++) {
+                const uint64_t row = min(rowOfItem(i), count - 1);
+                inDout[i] = *(const Four*)(douts + row * d.out.rowStride + there);
+                inValues[i] = *(const Four*)(values + row * a.v.rowStride + there);
+            }
+        }
+        else {
+            #pragma unroll
+            for(int i = 0; i < ITEMS; i++) {
+                const uint64_t row = min(rowOfItem(i), count - 1);
+                #pragma unroll
+                for(int e = 0; e < 4; e++) {
+                    const uint32_t there = v + stageAt + e < a.values ? v + stageAt + e : 0;
+                    inDout[i].v[e] = douts[row * d.out.rowStride + there];
+                    inValues[i].v[e] = values[row * a.v.rowStride + there];
+                }
+            }
         }
     };
-    request(0);
     #pragma unroll
     for(int i = 0; i < 2 * UNITS / 256; i++) {
         const uint32_t item = (tid + i * 256) % UNITS;
@@ -935,6 +943,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     for(int q = 0; q < SQUARES; q++) { dqk[q] = dkk[q] = f32x4{0, 0, 0, 0}; }
     float stateDot = 0.0f, valueDot[ITEMS] = {}, betaDot[ITEMS] = {};
     for(uint32_t v = 0; v < a.padded; v += 32) {
+        request(v);
         f32x4 s0[MINE][2], ds[MINE][2];
         #pragma unroll
         for(int m = 0; m < MINE; m++) {
@@ -948,14 +957,14 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         __syncthreads();
         #pragma unroll
         for(int i = 0; i < ITEMS; i++) {
-            const bool there = rowOfItem(i) < count;
             float dr[4], w[4], dout[4];
             #pragma unroll
             for(int e = 0; e < 4; e++) {
-                dr[e] = there ? nextDR[i][e] : 0.0f;
-                w[e] = there ? nextW[i][e] : 0.0f;
-                dout[e] = there ? widen(nextDout[i].v[e]) : 0.0f;
-                valueDot[i] = __builtin_fmaf(there ? widen(nextValues[i].v[e]) : 0.0f, dr[e], valueDot[i]);
+                const bool row = rowOfItem(i) < count, there = row && v + stageAt + e < a.values;
+                dr[e] = row ? inDR[i][e] : 0.0f;
+                w[e] = row ? inW[i][e] : 0.0f;
+                dout[e] = there ? widen(inDout[i].v[e]) : 0.0f;
+                valueDot[i] = __builtin_fmaf(there ? widen(inValues[i].v[e]) : 0.0f, dr[e], valueDot[i]);
                 betaDot[i] = __builtin_fmaf(w[e], dr[e], betaDot[i]);
             }
             uint2 words[3], own[NP];
@@ -971,7 +980,6 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             for(int k = 0; k < 3; k++) { *(uint2*)(to + (NP + 3 + k) * VP) = words[k]; }
         }
         __syncthreads();
-        if(v + 32 < a.padded) { request(v + 32); }
         {
             const Planes<3> other = fetch<3>(wPlanes + unitAt<32>(squareColumn * 16 + n16, g), VP);
             #pragma unroll
