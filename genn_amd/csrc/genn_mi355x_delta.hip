@@ -204,10 +204,11 @@ template<typename T, int C, int DK> int launchGradients(const char *what, const 
 {
     if(const int rc = launchChunks<T, C, DK, false>(what, a, numbers, stream)) { return rc; }
     if(const int rc = launchWalk<T, C, DK, WALK_KEEP, false>(what, a, segments, stream)) { return rc; }
-    const auto reverse = deltaReverseKernel<T, C, DK>;
+    const uint64_t reverseGrid = walkGrid(segments * a.keyHeads, a.group * a.columnBlocks);
+    const auto reverse = reverseGrid <= 256 ? deltaReverseKernel<T, C, DK, true> : deltaReverseKernel<T, C, DK, false>;
     constexpr size_t reverseLds = WalkLayout<T, C, DK, true>::bytes;
     if(const int rc = withLds(what, reverse, reverseLds)) { return rc; }
-    reverse<<<dim3((uint32_t)walkGrid(segments * a.keyHeads, a.group * a.columnBlocks)), dim3(WALK_THREADS), reverseLds, stream>>>(a, d);
+    reverse<<<dim3((uint32_t)reverseGrid), dim3(WALK_THREADS), reverseLds, stream>>>(a, d);
     const int rc = gennmi_detail::afterLaunch(what);
     if(rc || !(d.q.data || d.k.data || d.g.data || d.beta.data)) { return rc; }
     const auto kernel = deltaGradientKernel<T, C, DK>;
@@ -219,12 +220,14 @@ template<typename T, int C, int DK> int launchGradients(const char *what, const 
     deltaSharedKernel<T, C, DK><<<dim3((uint32_t)(numbers * a.keyHeads * (C / 4))), dim3(256), 0, stream>>>(a, d);
     return gennmi_detail::afterLaunch(what);
 }
-template<typename T, int VEC> int launchToken(const char *what, const DeltaArgs &a, uint32_t blocks, hipStream_t stream)
+// States of more than the last cache holds (256 MiB) pass the caches by
+bool streams(const gennmi_delta_rule_t &c) { return tokenVector(c) == 4 && c.sequences.count * stateBytes(c) > (256ull << 20); }
+template<typename T, int VEC, bool STREAM> int launchToken(const char *what, const DeltaArgs &a, uint32_t blocks, hipStream_t stream)
 {
     const dim3 grid(blocks), threads(256);
-    if(a.keys <= 32) { deltaTokenKernel<T, 1, VEC><<<grid, threads, 0, stream>>>(a); }
-    else if(a.keys <= 64) { deltaTokenKernel<T, 2, VEC><<<grid, threads, 0, stream>>>(a); }
-    else { deltaTokenKernel<T, 4, VEC><<<grid, threads, 0, stream>>>(a); }
+    if(a.keys <= 32) { deltaTokenKernel<T, 1, VEC, STREAM><<<grid, threads, 0, stream>>>(a); }
+    else if(a.keys <= 64) { deltaTokenKernel<T, 2, VEC, STREAM><<<grid, threads, 0, stream>>>(a); }
+    else { deltaTokenKernel<T, 4, VEC, STREAM><<<grid, threads, 0, stream>>>(a); }
     return gennmi_detail::afterLaunch(what);
 }
 }
@@ -261,7 +264,8 @@ int gennmi_delta_rule(const gennmi_delta_rule_t *rule, void *workspace, size_t w
             a.columnBlocks = (rule->values + 8 * vector - 1) / (8 * vector);
             rc = withType(rule->type, [&](auto t) {
                 typedef decltype(t) T;
-                return vector == 4 ? launchToken<T, 4>(what, a, blocks, s) : launchToken<T, 1>(what, a, blocks, s);
+                if(vector == 1) { return launchToken<T, 1, false>(what, a, blocks, s); }
+                return streams(*rule) ? launchToken<T, 4, true>(what, a, blocks, s) : launchToken<T, 4, false>(what, a, blocks, s);
             });
         }
         else {

@@ -79,7 +79,7 @@ template<typename T, int C, int DK> constexpr uint32_t chunkSquares() { const ui
 template<typename T, int C, int DK> constexpr uint32_t chunkLds() { return chunkSquares<T, C, DK>() + C * (8 + 3 * 4) + 16; }
 
 template<typename T, int C, int DK, bool FOLDED>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(256, 4)
 void deltaChunkKernel(DeltaArgs a)
 {
     constexpr int NP = planesOf<T>, B = C / 16, PLANE = C * DK, MP = C + 4, TILES = B * B / 4;
@@ -297,7 +297,7 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
     __device__ static uint32_t rowOf(int i) { return threadIdx.x / (DK / 8) + i * STEP; }
     __device__ static uint32_t column() { return threadIdx.x % (DK / 8) * 8; }
     // Units that are not there are asked for at another place, and become zero in store(): no branch a unit, with which the compiler would wait for each
-    __device__ void request(const DeltaArgs &a, const Place &p, uint32_t keyHead, uint32_t first, uint32_t count, uint64_t at)
+    __device__ void requestKeys(const DeltaArgs &a, const Place &p, uint32_t keyHead, uint32_t first, uint32_t count)
     {
         const T *const key = rowsOf<const T>(a.k, a.chunks, p) + (uint64_t)first * a.k.rowStride + keyHead * a.keys, *const query = rowsOf<const T>(a.q, a.chunks, p) + (uint64_t)first * a.q.rowStride + keyHead * a.keys;
         if(a.wide && count == C) {
@@ -318,6 +318,9 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
                 if(QUERIES) { queries[i] = a.wide ? *(const Eight<T>*)(query + row * a.q.rowStride + at0) : loadEight(query + row * a.q.rowStride + at0, valid); }
             }
         }
+    }
+    __device__ void requestSquares(const DeltaArgs &a, uint64_t at)
+    {
         #pragma unroll
         for(int i = 0; i < SQUARES; i++) {
             const uint32_t item = threadIdx.x + i * WALK_THREADS, offset = Triangle<C>::row(item) * C + Triangle<C>::column(item);
@@ -360,12 +363,14 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
         if(threadIdx.x < C) { ((f32x4*)(planes + L::table))[threadIdx.x] = rows; }
     }
 };
+// (What a lane's place makes of them is worked out anew for every product: kept over the walk, as the compiler would have it, it costs registers that there are not.)
 // Operands of a walk.  Tile t of a result has rows in the order of rowIn(): of keys (or queries, of the chunk's rows), times what is summed over keys 32 s ..; of a triangle, summed over
 // rows 32 s ..; of their transposes, summed over the chunk's rows 32 s ..
-template<typename T, int C, int DK> struct WalkOperands
+template<typename T, int C, int DK, bool ANEW = true> struct WalkOperands
 {
     static constexpr int NP = planesOf<T>;
     uint32_t n16, g;
+    __device__ WalkOperands(uint32_t lane) { if(ANEW) { asm volatile("" : "+v"(lane)); } n16 = lane & 15; g = lane >> 4; }
     __device__ Planes<NP> rows(const uint16_t *from, int t, int s) const { return fetch<NP>(from + unitAt<DK>(rowIn(t, n16), 4 * s + g), C * DK); }
     __device__ Planes<NP> columns(const uint16_t *from, int t, int s) const
     {
@@ -470,7 +475,6 @@ void deltaStateKernel(DeltaArgs a)
     uint16_t *const planes = (uint16_t*)lds;
     const RowFactors<C> table{(float*)(planes + L::table)};
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
-    const WalkOperands<T, C, DK> operand{n16, g};
     const WalkPlace mine = walkPlace(a, a.columnBlocks + (MODE == WALK_SUMMARY ? a.moveBlocks : 0));
     const uint32_t block = mine.block, head = mine.head, segment = mine.segment, keyHead = head / a.group;
     Place p;
@@ -500,7 +504,7 @@ void deltaStateKernel(DeltaArgs a)
     else if(a.initialState) { loadResult<float, DK>(a.initialState + ((uint64_t)p.state * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
 
     WalkStage<T, C, DK, OUTPUTS> stage;
-    if(chunks) { stage.request(a, p, keyHead, begin, min((uint32_t)C, end - begin), firstNumber * a.heads + head); }
+    if(chunks) { stage.requestKeys(a, p, keyHead, begin, min((uint32_t)C, end - begin)); stage.requestSquares(a, firstNumber * a.heads + head); }
     for(uint32_t n = 0; n < chunks; n++) {
         const uint32_t first = begin + n * C, count = min((uint32_t)C, end - first);
         const uint64_t at = (firstNumber + n) * a.heads + head;
@@ -510,8 +514,9 @@ void deltaStateKernel(DeltaArgs a)
         __syncthreads();
         stage.store(a, planes, count);
         __syncthreads();
-        const auto requestNext = [&] { if(n + 1 < chunks) { stage.request(a, p, keyHead, first + C, min((uint32_t)C, end - first - C), at + a.heads); } };
-        if(!active) { requestNext(); continue; }
+        const auto requestKeys = [&] { if(n + 1 < chunks) { stage.requestKeys(a, p, keyHead, first + C, min((uint32_t)C, end - first - C)); } };
+        const auto requestSquares = [&] { if(n + 1 < chunks) { stage.requestSquares(a, at + a.heads); } };
+        if(!active) { requestKeys(); requestSquares(); continue; }
 
         // r = v - G k^ S, and the part of the outputs that the state in front has: x's first tiles and the others
         constexpr int ROWS = OUTPUTS ? 2 * TILES : TILES;
@@ -522,6 +527,7 @@ void deltaStateKernel(DeltaArgs a)
         #pragma unroll
         for(int s = 0; s < DK / 32; s++) {
             inTurn();
+            const WalkOperands<T, C, DK, OUTPUTS> operand(lane);
             Planes<NP> rows[ROWS];
             #pragma unroll
             for(int t = 0; t < ROWS; t++) { rows[t] = operand.rows(planes + (t < TILES ? L::keys : L::queries), t % TILES, s); }
@@ -567,6 +573,7 @@ void deltaStateKernel(DeltaArgs a)
                 #pragma unroll
                 for(int t = 2 * s; t < TILES; t += 2) {
                     inTurn();
+                    const WalkOperands<T, C, DK, OUTPUTS> operand(lane);
                     constexpr int SQUARES = OUTPUTS ? 4 : 2;
                     Planes<3> rows[SQUARES];
                     f32x4 sum[SQUARES];
@@ -593,7 +600,7 @@ void deltaStateKernel(DeltaArgs a)
         if(MODE == WALK_KEEP) { storeResult<float, C>(a.errors + at * C * a.padded, a.padded, g, column, true, C, w); }
         if(OUTPUTS) { storeResult<T, C>(rowsOf<T>(a.out, a.chunks, p) + (uint64_t)first * a.out.rowStride + head * a.values, a.out.rowStride, g, column, inside, count, *(const f32x4 (*)[TILES])(x + ROWS - TILES)); }
         // the state behind the chunk; meanwhile the next one's operands are on their way (asked for before this they cost registers that there are not)
-        requestNext();
+        requestKeys();
         #pragma unroll
         for(int t = 0; t < STATE; t++) { state[t] *= chunk.decay; }
         #pragma unroll
@@ -602,11 +609,14 @@ void deltaStateKernel(DeltaArgs a)
             f32x4 left[2];
             #pragma unroll
             for(int h = 0; h < 2; h++) { left[h] = w[2 * s + h] * table.beta(rowIn(2 * s + h, 4 * g)) * table.keyEnd(rowIn(2 * s + h, 4 * g)); }
+            const WalkOperands<T, C, DK, OUTPUTS> operand(lane);
             Planes<NP> columns[STATE];
             #pragma unroll
             for(int t = 0; t < STATE; t++) { columns[t] = operand.columns(planes + L::keys, t, s); }
             multiplyAll(columns, split<3>(left[0], left[1]), state);
         }
+        inTurn();
+        requestSquares();
         if(__builtin_expect(bad < C, 0)) {
             const float no = __builtin_nanf("");
             #pragma unroll
@@ -695,8 +705,9 @@ struct DeltaGradientArgs
     float *states, *errors;         // the gradient of the state behind each chunk [DK][padded], dR [C][padded]
     float *shared;                  // where heads share keys: each one's gradients of unit queries and keys, [2][C][DK]
 };
-template<typename T, int C, int DK>
-__global__ __launch_bounds__(WALK_THREADS, 2)
+// ALONE: not more work-groups than compute units; each may have all registers of one.
+template<typename T, int C, int DK, bool ALONE>
+__global__ __launch_bounds__(WALK_THREADS, ALONE ? 1 : 2)
 void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
 {
     typedef WalkLayout<T, C, DK, true> L;
@@ -705,7 +716,6 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
     uint16_t *const planes = (uint16_t*)lds;
     const RowFactors<C> table{(float*)(planes + L::table)};
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
-    const WalkOperands<T, C, DK> operand{n16, g};
     const WalkPlace mine = walkPlace(a, a.columnBlocks);
     const uint32_t block = mine.block, head = mine.head, segment = mine.segment, keyHead = head / a.group;
     Place p;
@@ -723,6 +733,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
     // two tiles of a triangle's transpose
     const auto timesTriangle = [&](uint32_t from, int t, int s, const auto &b, f32x4 (&to)[TILES]) {
         inTurn();
+        const WalkOperands<T, C, DK, !ALONE> operand(lane);
         const Planes<3> rows[2] = {operand.triangleColumns(planes + from, t, s), operand.triangleColumns(planes + from, t + 1, s)};
         f32x4 sum[2] = {to[t], to[t + 1]};
         multiplyAll(rows, b, sum);
@@ -730,7 +741,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
         to[t + 1] = sum[1];
     };
     WalkStage<T, C, DK, true> stage;
-    if(chunks) { const uint32_t last = begin + (chunks - 1) * C; stage.request(a, p, keyHead, last, end - last, (firstNumber + chunks - 1) * a.heads + head); }
+    if(chunks) { const uint32_t last = begin + (chunks - 1) * C; stage.requestKeys(a, p, keyHead, last, end - last); stage.requestSquares(a, (firstNumber + chunks - 1) * a.heads + head); }
     for(uint32_t left = chunks; left > 0; left--) {
         const uint32_t n = left - 1, first = begin + n * C, count = min((uint32_t)C, end - first);
         const uint64_t at = (firstNumber + n) * a.heads + head;
@@ -740,8 +751,9 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
         __syncthreads();
         stage.store(a, planes, count);
         __syncthreads();
-        const auto requestNext = [&] { if(n > 0) { stage.request(a, p, keyHead, first - C, C, at - a.heads); } };
-        if(!active) { requestNext(); continue; }
+        const auto requestKeys = [&] { if(n > 0) { stage.requestKeys(a, p, keyHead, first - C, C); } };
+        const auto requestSquares = [&] { if(n > 0) { stage.requestSquares(a, at - a.heads); } };
+        if(!active) { requestKeys(); requestSquares(); continue; }
 
         f32x4 dout[TILES], du[TILES];
         #pragma unroll
@@ -751,6 +763,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
         #pragma unroll
         for(int s = 0; s < DK / 32; s++) {
             inTurn();
+            const WalkOperands<T, C, DK, !ALONE> operand(lane);
             Planes<NP> rows[TILES];
             #pragma unroll
             for(int t = 0; t < TILES; t++) { rows[t] = operand.rows(planes + L::keys, t, s); }
@@ -788,7 +801,7 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             }
         }
         storeResult<float, C>(d.errors + at * C * a.padded, a.padded, g, column, true, C, du);
-        requestNext();
+        requestKeys();
         // dS in front of the chunk = G[last] dS + (scale G q^)' dout - (G k^)' (beta dR)
         #pragma unroll
         for(int t = 0; t < STATE; t++) { state[t] *= decay; }
@@ -806,12 +819,15 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
             #pragma unroll
             for(int which = 0; which < 2; which++) {
                 inTurn();
+                const WalkOperands<T, C, DK, !ALONE> operand(lane);
                 Planes<NP> columns[STATE];
                 #pragma unroll
                 for(int t = 0; t < STATE; t++) { columns[t] = operand.columns(planes + (which ? L::keys : L::queries), t, s); }
                 multiplyAll(columns, which ? split<3>(y[0], y[1]) : split<3>(x[0], x[1]), state);
             }
         }
+        inTurn();
+        requestSquares();
         if(d.v.data) { storeResult<T, C>(rowsOf<T>(d.v, a.chunks, p) + (uint64_t)first * d.v.rowStride + head * a.values, d.v.rowStride, g, column, inside, count, du); }
     }
     if(d.initialState && active && begin == 0) { storeResult<float, DK>(d.initialState + ((uint64_t)p.sequence * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
@@ -1249,7 +1265,7 @@ void deltaSharedKernel(DeltaArgs a, DeltaGradientArgs d)
 // between reading and writing.  One sum over the rows does for everything: with S' k, S' q, |k|^2, |q|^2 and k.q
 //   u = beta (v - a S' k^),   out = scale (a S' q^ + (k^.q^) u).
 __device__ inline float eightApart(float x) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true)); }      // row_ror:8
-template<typename T, int ROWS, int VEC>
+template<typename T, int ROWS, int VEC, bool STREAM>
 __global__ __launch_bounds__(256)
 void deltaTokenKernel(DeltaArgs a)
 {
@@ -1263,12 +1279,17 @@ void deltaTokenKernel(DeltaArgs a)
     if(!describe(a.chunks, sequence, p)) { return; }
     const uint64_t stateAt = ((uint64_t)p.state * a.heads + head) * a.keys * a.values + column;
     typedef Pack<float, VEC> Columns;
+    typedef float Stream __attribute__((ext_vector_type(VEC)));
     Columns s[ROWS];
     #pragma unroll
     for(int i = 0; i < ROWS; i++) {
         const uint32_t row = part + 32 * i;
         s[i] = Columns{};
-        if(a.initialState && row < a.keys && inside) { s[i] = *(const Columns*)(a.initialState + stateAt + (uint64_t)row * a.values); }
+        if(a.initialState && row < a.keys && inside) {
+            const float *const from = a.initialState + stateAt + (uint64_t)row * a.values;
+            if constexpr(STREAM) { s[i] = __builtin_bit_cast(Columns, __builtin_nontemporal_load((const Stream*)from)); }
+            else { s[i] = *(const Columns*)from; }
+        }
     }
     if(p.length) {
         const T *const keys = rowsOf<const T>(a.k, a.chunks, p) + keyHead * a.keys, *const queries = rowsOf<const T>(a.q, a.chunks, p) + keyHead * a.keys;
@@ -1321,7 +1342,10 @@ void deltaTokenKernel(DeltaArgs a)
     #pragma unroll
     for(int i = 0; i < ROWS; i++) {
         const uint32_t row = part + 32 * i;
-        if(row < a.keys) { *(Columns*)(a.finalState + stateAt + (uint64_t)row * a.values) = s[i]; }
+        if(row >= a.keys) { continue; }
+        float *const to = a.finalState + stateAt + (uint64_t)row * a.values;
+        if constexpr(STREAM) { __builtin_nontemporal_store(__builtin_bit_cast(Stream, s[i]), (Stream*)to); }
+        else { *(Columns*)to = s[i]; }
     }
 }
 }
