@@ -194,6 +194,7 @@ void deltaChunkKernel(DeltaArgs a)
                 m[i / C * MP + i % C] = 0.0f;
                 if(FOLDED) { scores[i / C * MP + i % C] = 0.0f; } else { score[i] = 0.0f; }
             }
+            if(tid >= from && tid < C) { beta[tid] = 0.0f; }
             __syncthreads();
         }
         if(tid == 0) { a.table[at] = ChunkTable{decay, from}; }
