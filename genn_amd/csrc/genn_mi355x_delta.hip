@@ -169,13 +169,6 @@ DeltaArgs deltaArgs(const gennmi_delta_rule_t &c, const DeltaSpace &space, void 
     return a;
 }
 
-// Kernels ask for more LDS than a launch has without being told
-template<typename K> int withLds(const char *what, K kernel, size_t bytes)
-{
-    if(bytes <= 65536) { return GENNMI_OK; }
-    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    return e == hipSuccess ? (int)GENNMI_OK : fail(GENNMI_EHIP, std::string(what) + ": " + hipGetErrorString(e));
-}
 template<typename T, int C, int DK, bool FOLDED> int launchChunks(const char *what, const DeltaArgs &a, uint64_t numbers, hipStream_t stream)
 {
     const auto kernel = deltaChunkKernel<T, C, DK, FOLDED>;

@@ -304,6 +304,13 @@ inline Region offsetsOf(const gennmi_sequences_t &s) { return regionOf("offsets"
 inline Region slotsOf(const gennmi_sequences_t &s) { return regionOf("slots", s.slots, s.count * 4ull); }
 // An array that a call may write in place of the one it reads
 inline Region unlessSame(const Region &r, const void *written) { return (uintptr_t)written == (uintptr_t)r.begin ? Region{r.name, 0, 0, 0, 0, 0, 0, 0} : r; }
+// Kernels ask for more LDS than a launch has without being told
+template<typename K> int withLds(const char *what, K kernel, size_t bytes)
+{
+    if(bytes <= 65536) { return GENNMI_OK; }
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e == hipSuccess ? (int)GENNMI_OK : gennmi_detail::fail(GENNMI_EHIP, std::string(what) + ": " + hipGetErrorString(e));
+}
 inline int checkWorkspace(const char *what, const void *workspace, size_t have, size_t need)
 {
     if(need && (!workspace || have < need)) { return gennmi_detail::fail(GENNMI_EINVAL, std::string(what) + ": workspace is missing or too small"); }

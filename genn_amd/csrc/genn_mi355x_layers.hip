@@ -45,6 +45,7 @@ template<int LANES> __device__ inline float sumOfLanes(float x)
     return x;
 }
 // Two sums a row over its wavefronts; two places in LDS are used in turn, so that one barrier does
+constexpr int NORM_APART = 1024;        // a lane's sums in LDS, in elements: a constant costs no register a place
 struct NormShared { float2 found[2][16]; };
 
 template<typename T, int E, int VEC> struct NormRow { Pack<T, VEC> part[E / VEC]; };
@@ -164,22 +165,25 @@ void normKernel(NormArgs a)
     loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias);
     const float inWave = LANES ? 0.0f : elementsOf<E, VEC>(at, at.lane >> 6, a.channels), inWaveShare = inWave > 0.0f ? 1.0f / inWave : 0.0f;
     const uint64_t step = (uint64_t)gridDim.x * at.groups;
+    // (a gate's elements one by one, with the places of them all, are more than the registers of 16 wavefronts hold ahead of time)
+    constexpr bool AHEAD = LANES || VEC > 1;
     NormRow<T, E, VEC> nextX, nextZ{};
-    const auto request = [&](uint64_t n) {
+    const auto request = [&](uint64_t n, bool x, bool z) {
         const bool valid = n < a.rows;
         const uint32_t sequence = valid ? (uint32_t)n / a.length : 0, row = valid ? (uint32_t)n - sequence * a.length : 0;
-        nextX = requestRow<T, E, VEC>(normRow<const T>(a.x, sequence, row), at, a.channels, valid);
-        if constexpr(GATE) { nextZ = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
+        if(x) { nextX = requestRow<T, E, VEC>(normRow<const T>(a.x, sequence, row), at, a.channels, valid); }
+        if constexpr(GATE) { if(z) { nextZ = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); } }
     };
     uint64_t first = (uint64_t)blockIdx.x * at.groups;
-    request(first + at.group);
+    request(first + at.group, true, AHEAD);
     for(; first < a.rows; first += step) {
         const uint64_t n = first + at.group;
         float x[E], z[E];
         takeRow(nextX, x);
-        if constexpr(GATE) { takeRow(nextZ, z); }
-        request(n + step);
+        if constexpr(GATE && AHEAD) { takeRow(nextZ, z); }
+        request(n + step, true, AHEAD);
         normalise<LANES, E, VEC>(a, x, at, shared, turn, inWave, inWaveShare);
+        if constexpr(GATE && !AHEAD) { request(n, false, true); takeRow(nextZ, z); }
         #pragma unroll
         for(int e = 0; e < E; e++) {
             x[e] = __builtin_fmaf(x[e], weight[e], bias[e]);
@@ -203,9 +207,17 @@ void normBackwardKernel(NormArgs a)
     extern __shared__ float rows[];
     uint32_t turn = 0;
     const NormPlace at = normPlace<LANES>(a);
-    float weight[E], bias[GATE ? E : 1], dweight[E] = {}, dbias[E] = {};
+    // (16 elements a lane, above 8192 channels, leave 16 wavefronts no registers for the sums, which lie in LDS, nor for the next row or a gate's bias)
+    constexpr bool LARGE = LANES == 0 && E == 16, BIAS_AGAIN = LARGE && VEC == 8;
+    float weight[E], bias[GATE ? E : 1], dweight[LARGE ? 1 : E] = {}, dbias[LARGE ? 1 : E] = {};
+    constexpr int APART = NORM_APART;
+    float *const sums[2] = {rows + threadIdx.x, rows + E * APART + threadIdx.x};
+    if constexpr(LARGE) {
+        #pragma unroll
+        for(int e = 0; e < E; e++) { sums[0][e * APART] = sums[1][e * APART] = 0.0f; }
+    }
     loadParameters<E, VEC>(a.weight, 1.0f, at, a.channels, weight);
-    if constexpr(GATE) { loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias); }
+    if constexpr(GATE && !BIAS_AGAIN) { loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias); }
     const float inWave = LANES ? 0.0f : elementsOf<E, VEC>(at, at.lane >> 6, a.channels), inWaveShare = inWave > 0.0f ? 1.0f / inWave : 0.0f;
     const uint64_t step = (uint64_t)gridDim.x * at.groups;
     NormRow<T, E, VEC> nextX, nextD;
@@ -216,23 +228,27 @@ void normBackwardKernel(NormArgs a)
         nextD = requestRow<T, E, VEC>(normRow<const T>(a.dout, sequence, row), at, a.channels, valid);
     };
     uint64_t first = (uint64_t)blockIdx.x * at.groups;
-    request(first + at.group);
+    if(!LARGE) { request(first + at.group); }
     for(; first < a.rows; first += step) {
         const uint64_t n = first + at.group;
         const bool valid = n < a.rows;
+        if(LARGE) { request(n); }
         const uint32_t sequence = valid ? (uint32_t)n / a.length : 0, row = valid ? (uint32_t)n - sequence * a.length : 0;
         float x[E], d[E];
         takeRow(nextX, x);
         takeRow(nextD, d);
         NormRow<T, E, VEC> gate{};
-        if constexpr(GATE) { gate = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
-        request(n + step);
+        if constexpr(GATE && !LARGE) { gate = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
+        if(!LARGE) { request(n + step); }
         const float r = normalise<LANES, E, VEC>(a, x, at, shared, turn, inWave, inWaveShare);
         if constexpr(GATE) {
+            if constexpr(BIAS_AGAIN) { loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias); }
+            if constexpr(LARGE) { gate = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
             float z[E];
             takeRow(gate, z);
             #pragma unroll
             for(int e = 0; e < E; e++) {
+                if(LARGE && e % 4 == 0) { __builtin_amdgcn_sched_barrier(0); }
                 const float s = logistic(z[e]), y = __builtin_fmaf(x[e], weight[e], bias[e]), dz = d[e] * y * (s * __builtin_fmaf(z[e], 1.0f - s, 1.0f));
                 d[e] *= z[e] * s;
                 z[e] = dz;
@@ -243,8 +259,15 @@ void normBackwardKernel(NormArgs a)
         float along = 0.0f, mean = 0.0f;
         #pragma unroll
         for(int e = 0; e < E; e++) {
-            if(valid) { dweight[e] = __builtin_fmaf(d[e], x[e], dweight[e]); }
-            dbias[e] += d[e];
+            if constexpr(LARGE) {
+                if(e % 4 == 0) { __builtin_amdgcn_sched_barrier(0); }
+                sums[0][e * APART] = __builtin_fmaf(d[e], x[e], sums[0][e * APART]);
+                sums[1][e * APART] += d[e];
+            }
+            else {
+                if(valid) { dweight[e] = __builtin_fmaf(d[e], x[e], dweight[e]); }
+                dbias[e] += d[e];
+            }
             d[e] *= weight[e];
             along = __builtin_fmaf(d[e], x[e], along);
             mean += d[e];
@@ -270,8 +293,13 @@ void normBackwardKernel(NormArgs a)
     float *const to = a.sums + (uint64_t)blockIdx.x * 2 * a.channels;
     #pragma unroll
     for(int which = 0; which < 2; which++) {
-        float (&sum)[E] = which ? dbias : dweight;
-        if(at.groups > 1) {
+        float (&sum)[LARGE ? 1 : E] = which ? dbias : dweight;
+        if constexpr(LARGE) {
+            #pragma unroll
+            for(int e = 0; e < E; e++) { if(hasElement<E, VEC>(at, e, a.channels)) { to[which * a.channels + (e / VEC * at.lanes + at.lane) * VEC + e % VEC] = sums[which][e * APART]; } }
+            continue;
+        }
+        else if(at.groups > 1) {
             // (the rows of a work-group one after another)
             __syncthreads();
             #pragma unroll
@@ -284,8 +312,10 @@ void normBackwardKernel(NormArgs a)
                 for(int e = 0; e < E; e++) { sum[e] += rows[e * blockDim.x + k * at.lanes + at.lane]; }
             }
         }
-        #pragma unroll
-        for(int e = 0; e < E; e++) { if(hasElement<E, VEC>(at, e, a.channels)) { to[which * a.channels + (e / VEC * at.lanes + at.lane) * VEC + e % VEC] = sum[e]; } }
+        if constexpr(!LARGE) {
+            #pragma unroll
+            for(int e = 0; e < E; e++) { if(hasElement<E, VEC>(at, e, a.channels)) { to[which * a.channels + (e / VEC * at.lanes + at.lane) * VEC + e % VEC] = sum[e]; } }
+        }
     }
 }
 
@@ -507,7 +537,11 @@ int gennmi_layer_norm_backward(const gennmi_layer_norm_t *norm, const gennmi_lay
         a.sums = sums ? (float*)workspace : nullptr;
         if(a.rows) {
             const int rc = withNorm<true>(*norm, p, vectorOf(size, channels, arrays), [&](auto t, auto lanes, auto each, auto vec, auto gate) {
-                normBackwardKernel<decltype(t), decltype(lanes)::value, decltype(each)::value, decltype(vec)::value, decltype(gate)::value><<<dim3(p.blocks), dim3(p.threads), sums && p.groups > 1 ? p.threads * decltype(each)::value * sizeof(float) : 0, (hipStream_t)stream>>>(a);
+                constexpr int LANES = decltype(lanes)::value, E = decltype(each)::value;
+                const auto kernel = normBackwardKernel<decltype(t), LANES, E, decltype(vec)::value, decltype(gate)::value>;
+                const size_t lds = LANES == 0 && E == 16 ? 2 * E * NORM_APART * sizeof(float) : sums && p.groups > 1 ? p.threads * E * sizeof(float) : 0;
+                if(const int rcLds = withLds(what, kernel, lds)) { return rcLds; }
+                kernel<<<dim3(p.blocks), dim3(p.threads), lds, (hipStream_t)stream>>>(a);
                 return gennmi_detail::afterLaunch(what);
             });
             if(rc) { return rc; }

@@ -218,3 +218,128 @@ def test_arrays_of_the_package_and_what_the_layer_refuses():
         broken = LayerNorm(2, 3, 20000)
         broken.bind(x=torch.zeros(6, 20000).cuda(), out=torch.zeros(6, 20000).cuda())
         broken.run()
+
+
+@pytest.mark.parametrize("channels", [64, 520, 2048, 5000])
+def test_any_alignment_gives_the_same(channels):
+    from genn_amd.sequence import Dropout, LayerNorm
+    r, rows = generator(channels), 9
+    x, z, d = (r(rows, channels).bfloat16() for _ in range(3))
+    w, b = 1 + r(channels) / 8, r(channels) / 8
+    results = []
+    for shift in (0, 1, 3, 4):
+        def placed(t):
+            room = torch.empty(t.numel() + 8, dtype=t.dtype).cuda()
+            view = room[shift:shift + t.numel()].view(t.shape)
+            view.copy_(t)
+            return view
+        out, dx, dz, dw, db, kept = placed(x), placed(x), placed(x), placed(w), placed(w), placed(x)
+        op = LayerNorm(1, rows, channels, dtype="bfloat16")
+        op.bind(x=placed(x), weight=placed(w), bias=placed(b), gate=placed(z), out=out)
+        op.run()
+        op.bind_gradients(out=placed(d), x=dx, gate=dz, weight=dw, bias=db)
+        op.backward()
+        drop = Dropout(1, rows, channels, 0.3, seed=1, dtype="bfloat16")
+        drop.bind(x=placed(x), residual=placed(z), out=kept)
+        drop.run(2)
+        results.append([t.double().cpu() for t in (out, dx, dz, dw, db, kept)])
+    want, size = ref.layer_norm(x, w, b, z)
+    for other in results:
+        close("out", other[0], want, size, torch.bfloat16)
+        assert torch.equal(other[5], results[0][5])
+        # (another alignment may give a row to other lanes: the last bit of a sum)
+        for a, c in zip(other[:5], results[0][:5]):
+            assert float((a - c).norm()) <= 2.0 ** -8 * float(c.norm())
+
+
+def test_rows_and_calls_at_their_ends():
+    """Sequences more than 2^32 elements apart, the largest seed and numbers of calls, a number on the device that is added to none."""
+    from genn_amd.sequence import Dropout, LayerNorm
+    r, far, channels = generator(5), (1 << 32) + 64, 136
+    room = torch.empty(far + 4096, dtype=torch.bfloat16, device="cuda")
+    x = r(2, 3, channels).bfloat16()
+    there = torch.as_strided(room, (2, 3, channels), (far, channels + 8, 1))
+    there.copy_(x)
+    out = torch.zeros(2, 3, channels, dtype=torch.bfloat16).cuda()
+    op = LayerNorm(2, 3, channels, dtype="bfloat16")
+    op.bind(x=there, out=out)
+    op.run()
+    close("out", out.view(6, channels), *ref.layer_norm(x.view(6, channels)), torch.bfloat16)
+    op.bind(x=x.cuda(), out=there)
+    op.run()
+    assert torch.equal(there, out)
+    seed = (1 << 64) - 1
+    drop = Dropout(2, 3, channels, 0.5, seed=seed, dtype="bfloat16")
+    drop.bind(x=x.cuda(), out=there)
+    for call in (0, (1 << 32) - 1, 1 << 32, (1 << 64) - 1):
+        drop.run(call)
+        keep, factor = ref.kept(6, channels, 0.5, seed, call)
+        want = torch.where(keep.view(x.shape), x.double(), 0.0) * factor
+        close("out", there.contiguous(), want, want.abs(), torch.bfloat16, 3)
+    last = torch.tensor([-1], dtype=torch.int64).cuda()         # (all 64 bits)
+    before = there.clone()
+    there.zero_()
+    drop.run(last)
+    assert torch.equal(there, before)
+
+
+@pytest.mark.parametrize("channels, rows", [(48, 700), (1024, 40), (6000, 5)])
+def test_a_row_that_is_no_number_leaves_the_others_gradients_alone(channels, rows):
+    from genn_amd.sequence import LayerNorm
+    r = generator(channels)
+    x, z, d = r(rows, channels), r(rows, channels), r(rows, channels)
+    grads = []
+    for bad in (False, True):
+        if bad:
+            x[rows // 2, 7] = math.nan
+        dx, dz = torch.zeros(rows, channels).cuda(), torch.zeros(rows, channels).cuda()
+        op = LayerNorm(1, rows, channels, rms=True)
+        op.bind(x=x.cuda(), gate=z.cuda())
+        op.bind_gradients(out=d.cuda(), x=dx, gate=dz)
+        op.backward()
+        grads.append((dx.cpu(), dz.cpu()))
+    rest = torch.arange(rows) != rows // 2
+    for a, b in zip(*grads):
+        assert torch.equal(a[rest], b[rest]) and torch.isnan(b[rows // 2]).all()
+
+
+def test_a_bind_that_is_refused_leaves_what_was_bound():
+    from genn_amd.sequence import Dropout, GatedDeltaRule, LayerNorm
+    x = generator(2)(2, 8).cuda()
+    for op, more in ((GatedDeltaRule(1, 2, 1, 8, 8), ("q", "k", "v")), (LayerNorm(1, 2, 8), ("x",)), (Dropout(1, 2, 8, 0.5), ("x",))):
+        def arrays(t):
+            given = {name: t for name in more}
+            return dict(given, g=t[:, :1], beta=t[:, :1]) if len(more) > 1 else given
+        call = (lambda: op.run(3)) if isinstance(op, Dropout) else op.run
+        first, second = torch.zeros_like(x), torch.zeros_like(x)
+        op.bind(out=first, **arrays(x))
+        call()
+        first.zero_()
+        with pytest.raises((ValueError, TypeError)):
+            op.bind(out=second, **arrays(x[:1]))
+        with pytest.raises((ValueError, TypeError)):
+            op.bind(out=second, **arrays(x.cpu()))
+        call()
+        assert float(first.abs().sum()) > 0 and float(second.abs().sum()) == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("channels, gate, rows", [(8200, True, 2100), (8200, False, 700), (8193, True, 60)])
+def test_gradients_of_the_longest_rows(channels, gate, rows, dtype):
+    """Of rows for more work-groups than the chip holds: each adds up several."""
+    from genn_amd.sequence import LayerNorm
+    T, r = TYPES[dtype], generator(channels + rows)
+    x, d, w, b = r(rows, channels).to(T), r(rows, channels).to(T), 1 + r(channels) / 8, r(channels) / 8
+    z = r(rows, channels).to(T) if gate else None
+    dx, dz, dw, db = torch.zeros_like(x).cuda(), torch.zeros_like(x).cuda(), torch.zeros(channels).cuda(), torch.zeros(channels).cuda()
+    op = LayerNorm(1, rows, channels, dtype=dtype)
+    op.bind(x=x.cuda(), weight=w.cuda(), bias=b.cuda(), gate=z.cuda() if gate else None)
+    op.bind_gradients(out=d.cuda(), x=dx, weight=dw, bias=db, gate=dz if gate else None)
+    op.backward()
+    found, size = ref.layer_norm(x, w, b, z, dout=d)
+    close("dx", dx, found["dx"], size["dx"], T, 2 * OPERATIONS)
+    # (a lane adds up rows / 512 rows before the sums in 64 bits)
+    close("dweight", dw, found["dweight"], size["dweight"], operations=2 * OPERATIONS + rows // 512)
+    close("dbias", db, found["dbias"], size["dbias"], operations=2 * OPERATIONS + rows // 512)
+    if gate:
+        close("dgate", dz, found["dgate"], size["dgate"], T, 2 * OPERATIONS)

@@ -121,6 +121,22 @@ def test_gradients_and_workspaces_that_are_refused():
     refused(lib.gennmi_dropout(None, None), -2, "null descriptor")
 
 
+def test_strides_of_the_delta_rule_are_limited():
+    lib, size = _abi.load(), C.c_size_t()
+    most = 1 << 25
+    for name in ("q", "k", "v", "out"):
+        far = {name + "__data": 1 << 40, name + "__rowStride": most, name + "__sequenceStride": 5 * most}
+        refused(lib.gennmi_delta_rule_workspace(C.byref(delta(**far)), C.byref(size)), -2, "stride of q, k, v or out")
+        far.update({name + "__rowStride": most - 1})
+        assert lib.gennmi_delta_rule_workspace(C.byref(delta(**far)), C.byref(size)) == 0
+        far.update({name + "__rowStride": most, "sequences__length": 1})        # (no second row)
+        assert lib.gennmi_delta_rule_workspace(C.byref(delta(**far)), C.byref(size)) == 0
+    g = _abi.DeltaRuleGradient(out=_abi.Rows(1 << 40, most, 5 * most))
+    refused(lib.gennmi_delta_rule_backward(C.byref(delta()), C.byref(g), AT + (1 << 30), 1 << 40, None), -2, "stride of the gradients")
+    g = _abi.DeltaRuleGradient(out=_abi.Rows(1 << 40, 96, 480), v=_abi.Rows(1 << 41, most, 5 * most))
+    refused(lib.gennmi_delta_rule_backward(C.byref(delta()), C.byref(g), AT + (1 << 30), 1 << 40, None), -2, "stride of the gradients")
+
+
 def test_gradients_of_the_restatements_are_those_of_differences():
     gen = torch.Generator().manual_seed(3)
     r = lambda *shape: torch.randn(*shape, generator=gen, dtype=torch.float64)  # noqa: E731
