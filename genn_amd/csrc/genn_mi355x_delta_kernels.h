@@ -1095,7 +1095,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             }
         }
     };
-    // (`first` and `last`: the blocks of 32 columns that are not zero in rows of block b)
+    // (`lower`, `upper`: whether the square has blocks of 32 rows and columns below the diagonal's, and above them)
     const auto timesColumns = [&](uint32_t from, f32x4 (&to)[MINE][TILES], bool lower, bool upper) {
         #pragma unroll
         for(int m = 0; m < MINE; m++) {
