@@ -123,6 +123,8 @@ void deltaChunkKernel(DeltaArgs a)
     f32x4 kk[TILES], qk[TILES];
     const auto tileRow = [&](int t) { return C == 64 ? wave : wave >> 1; };
     const auto tileColumn = [&](int t) { return C == 64 ? (uint32_t)t : wave & 1; };
+    // (a walk has the first 32 rows of a square without the columns behind them)
+    const auto isRead = [](uint32_t tileRow, uint32_t tileColumn) { return tileRow >= 2 || tileColumn < 2; };
     #pragma unroll
     for(int t = 0; t < TILES; t++) {
         kk[t] = qk[t] = f32x4{0, 0, 0, 0};
@@ -184,7 +186,7 @@ void deltaChunkKernel(DeltaArgs a)
                 const float y = row >= column ? d * (a.scale * (queryUnit[row] * qk[t][r] * ku)) : 0.0f;
                 if(!finite(x)) { atomicMin(bad, row); }
                 m[row * MP + column] = x;
-                if(FOLDED) { scores[row * MP + column] = y; } else { score[row * C + column] = y; }
+                if(FOLDED) { scores[row * MP + column] = y; } else if(isRead(row / 16, column / 16)) { score[row * C + column] = y; }
             }
         }
         __syncthreads();
@@ -235,7 +237,10 @@ void deltaChunkKernel(DeltaArgs a)
             #pragma unroll
             for(int r = 0; r < B; r++) {
                 #pragma unroll
-                for(int e = 0; e < 4; e++) { found[r][e] *= -betaColumn; correction[(r * 16 + 4 * g + e) * C + wave * 16 + n16] = found[r][e]; }
+                for(int e = 0; e < 4; e++) {
+                    found[r][e] *= -betaColumn;
+                    if(isRead(r, wave)) { correction[(r * 16 + 4 * g + e) * C + wave * 16 + n16] = found[r][e]; }
+                }
             }
             if constexpr(FOLDED) {
                 // P beta (I - N beta), the same block column
@@ -254,6 +259,7 @@ void deltaChunkKernel(DeltaArgs a)
                             y = multiply(x, found[t], y);
                         }
                     }
+                    if(!isRead(r, wave)) { continue; }
                     #pragma unroll
                     for(int e = 0; e < 4; e++) { score[(r * 16 + 4 * g + e) * C + wave * 16 + n16] = y[e]; }
                 }
