@@ -29,7 +29,7 @@ template<typename F> int withSizes(const gennmi_delta_rule_t &c, F &&f)
 constexpr uint32_t WALK_COLUMNS = WALK_THREADS / 64 * 16;         // of a work-group of a walk
 uint32_t blocksOf(uint32_t columns) { return (columns + WALK_COLUMNS - 1) / WALK_COLUMNS; }
 
-// Work-groups of a walk: segments and key heads eight at a time, of each so many work-groups
+// Work-groups that share what they read go to one of the chip's eight parts: of segments and key heads (of sequences and heads) eight at a time, so many work-groups each
 uint64_t walkGrid(uint64_t outer, uint64_t each) { return (outer + 7) / 8 * 8 * each; }
 
 int checkDelta(const char *what, const gennmi_delta_rule_t *c, bool gradients)
@@ -133,8 +133,8 @@ bool deltaFits(const gennmi_delta_rule_t &c, bool gradients)
     if(!gradients && c.sequences.length <= 1) { return tokenBlocks(c) <= mostBlocks(256); }
     const uint32_t columns = gradients ? paddedValues(c.values) : c.values;
     return chunkNumbers(c.sequences, chunkRows(c.type)) * c.heads * (gradients && c.heads > c.keyHeads ? 8 : 1) <= mostBlocks(512) &&
-        walkGrid(chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.keyHeads, (uint64_t)(c.heads / c.keyHeads) * (blocksOf(columns) + moveBlocks(c))) <= mostBlocks(WALK_THREADS) &&
-        (uint64_t)c.sequences.count * c.heads * (paddedValues(c.values) / 16) <= mostBlocks(256);
+        walkGrid(chunkNumbers(c.sequences, segmentRows(c, gradients)) * c.keyHeads, (uint64_t)(c.heads / c.keyHeads) * (gradients ? 2 * blocksOf(columns) : blocksOf(columns) + moveBlocks(c))) <= mostBlocks(WALK_THREADS) &&
+        walkGrid((uint64_t)c.sequences.count * c.heads, paddedValues(c.values) / 16) <= mostBlocks(256);
 }
 DeltaArgs deltaArgs(const gennmi_delta_rule_t &c, const DeltaSpace &space, void *workspace, bool gradients)
 {
@@ -190,18 +190,17 @@ template<typename T, int C, int DK, bool FOLDED> int launchSegments(const char *
 {
     if(!a.segmentStates) { return GENNMI_OK; }
     if(const int rc = launchWalk<T, C, DK, WALK_SUMMARY, FOLDED>(what, a, segments, stream)) { return rc; }
-    deltaJoinKernel<DK><<<dim3(a.chunks.count * a.heads * (a.padded / 16)), dim3(256), 0, stream>>>(a);
+    deltaJoinKernel<DK><<<dim3((uint32_t)walkGrid((uint64_t)a.chunks.count * a.heads, a.padded / 16)), dim3(256), 0, stream>>>(a);
     return gennmi_detail::afterLaunch(what);
 }
 template<typename T, int C, int DK> int launchGradients(const char *what, const DeltaArgs &a, const DeltaGradientArgs &d, uint64_t numbers, uint64_t segments, hipStream_t stream)
 {
     if(const int rc = launchChunks<T, C, DK, false>(what, a, numbers, stream)) { return rc; }
-    if(const int rc = launchWalk<T, C, DK, WALK_KEEP, false>(what, a, segments, stream)) { return rc; }
-    const uint64_t reverseGrid = walkGrid(segments * a.keyHeads, a.group * a.columnBlocks);
-    const auto reverse = reverseGrid <= 256 ? deltaReverseKernel<T, C, DK, true> : deltaReverseKernel<T, C, DK, false>;
-    constexpr size_t reverseLds = WalkLayout<T, C, DK, true>::bytes;
-    if(const int rc = withLds(what, reverse, reverseLds)) { return rc; }
-    reverse<<<dim3((uint32_t)reverseGrid), dim3(WALK_THREADS), reverseLds, stream>>>(a, d);
+    const uint64_t grid = walkGrid(segments * a.keyHeads, a.group * a.columnBlocks);
+    const auto walks = 2 * grid <= 256 ? deltaWalksKernel<T, C, DK, true> : deltaWalksKernel<T, C, DK, false>;
+    constexpr size_t walksLds = WalkLayout<T, C, DK, true>::bytes;
+    if(const int rc = withLds(what, walks, walksLds)) { return rc; }
+    walks<<<dim3((uint32_t)grid, 2), dim3(WALK_THREADS), walksLds, stream>>>(a, d);
     const int rc = gennmi_detail::afterLaunch(what);
     if(rc || !(d.q.data || d.k.data || d.g.data || d.beta.data)) { return rc; }
     const auto kernel = deltaGradientKernel<T, C, DK>;

@@ -9,7 +9,7 @@
 // The transposed inverse of the gradients, (I + beta M')^-1, is I - beta N': N serves both, and no beta is divided by.
 //
 // M, N and P do not need the state: a work-group a chunk and key head finds them (deltaChunkKernel).  Then a state's columns do not need each other:
-// a wavefront owns 16 of them, all rows in registers, and walks the chunks (deltaStateKernel).  Its results become operands of the next product
+// a wavefront owns 16 of them, all rows in registers, and walks the chunks (walkForwards, walkBackwards).  Its results become operands of the next product
 // without leaving the registers; what multiplies them (keys, N, P) is shared by the work-group's wavefronts through LDS.  Products have fp32 accuracy (genn_mi355x_planes.h).
 #ifndef GENN_MI355X_DELTA_KERNELS_H
 #define GENN_MI355X_DELTA_KERNELS_H
@@ -471,9 +471,7 @@ __device__ inline WalkPlace walkPlace(const DeltaArgs &a, uint32_t blocks)
 }
 
 // A work-group walks a sequence (or a segment of it) of one head with 16 columns of the state a wavefront.
-template<typename T, int C, int DK, int MODE, bool FOLDED>
-__global__ __launch_bounds__(WALK_THREADS, 2)
-void deltaStateKernel(DeltaArgs a)
+template<typename T, int C, int DK, int MODE, bool FOLDED> __device__ __forceinline__ void walkForwards(const DeltaArgs &a)
 {
     constexpr bool OUTPUTS = MODE == WALK_OUTPUTS;
     typedef WalkLayout<T, C, DK, OUTPUTS> L;
@@ -640,65 +638,75 @@ void deltaStateKernel(DeltaArgs a)
     }
 }
 
+template<typename T, int C, int DK, int MODE, bool FOLDED>
+__global__ __launch_bounds__(WALK_THREADS, 2)
+void deltaStateKernel(DeltaArgs a) { walkForwards<T, C, DK, MODE, FOLDED>(a); }
+
 // From what each segment does: the state in front of each, in place of its own share: S = move S + own in fp32.  A work-group has 16 columns; its four wavefronts share the rows of
-// `move`, and hand each other what they found through LDS.
+// `move`, and hand each other what they found through LDS.  32 heads of 128 keys, 8 segments: 38 us with one share in registers, tiles of a head all over the chip; 27 so.
 template<int DK>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(256, 1)
 void deltaJoinKernel(DeltaArgs a)
 {
     constexpr int STATE = DK / 16, MINE = STATE / 4;
     __shared__ f32x4 found[STATE][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4, tiles = a.padded / 16;
-    const uint32_t tile = blockIdx.x % tiles, rest = blockIdx.x / tiles, head = rest % a.heads, sequence = rest / a.heads, column = tile * 16 + n16;
+    // (those that read one `move` on one part of the chip, as in walkPlace)
+    const uint32_t slot = blockIdx.x / 8, tile = slot % tiles, outer = slot / tiles * 8 + blockIdx.x % 8, sequence = outer / a.heads, head = outer - sequence * a.heads, column = tile * 16 + n16;
     Place p;
-    if(!describe(a.segments, sequence, p)) { return; }
+    if(sequence >= a.segments.count || !describe(a.segments, sequence, p)) { return; }
     f32x4 state[STATE];
     #pragma unroll
     for(int t = 0; t < STATE; t++) { state[t] = f32x4{0, 0, 0, 0}; }
     if(a.initialState) { loadResult<float, DK>(a.initialState + ((uint64_t)p.state * a.heads + head) * a.keys * a.values, a.values, g, column, column < a.values, a.keys, state); }
     const uint32_t segments = max(1u, (p.length + a.segments.chunk - 1) / a.segments.chunk);
     const uint64_t first = firstChunk(a.segments, sequence) * a.heads + head;
-    // (this wavefront's tiles of `move` and of a segment's own share)
-    f32x4 move[MINE][STATE], own[MINE];
-    const auto request = [&](uint32_t n) {
+    // (this wavefront's tiles of `move` and of a segment's own share; those of the next segment are on their way while one is joined)
+    struct Share { f32x4 move[MINE][STATE], own[MINE]; } shares[2];
+    const auto request = [&](uint32_t n, Share &to) {
         const uint64_t at = first + (uint64_t)n * a.heads;
         #pragma unroll
         for(int m = 0; m < MINE; m++) {
             const uint32_t rows = wave * MINE + m;
             #pragma unroll
-            for(int r = 0; r < 4; r++) { own[m][r] = a.segmentStates[at * DK * a.padded + rowIn(rows, 4 * g + r) * a.padded + column]; }
+            for(int r = 0; r < 4; r++) { to.own[m][r] = a.segmentStates[at * DK * a.padded + rowIn(rows, 4 * g + r) * a.padded + column]; }
             #pragma unroll
-            for(int t = 0; t < STATE; t++) { move[m][t] = *(const f32x4*)(a.segmentMoves + at * DK * DK + rowIn(rows, n16) * DK + rowIn(t, 4 * g)); }
+            for(int t = 0; t < STATE; t++) { to.move[m][t] = *(const f32x4*)(a.segmentMoves + at * DK * DK + rowIn(rows, n16) * DK + rowIn(t, 4 * g)); }
         }
     };
-    if(segments > 1) { request(0); }
-    for(uint32_t n = 0; n < segments; n++) {
-        float *const to = a.segmentStates + (first + (uint64_t)n * a.heads) * DK * a.padded + column;
+    const auto join = [&](uint32_t n, const Share &share, Share &ahead) {
+        // (behind the last segment but one nobody asks)
+        if(n + 2 < segments) { request(n + 1, ahead); }
         f32x4 next[MINE];
         if(n + 1 < segments) {
             #pragma unroll
-            for(int m = 0; m < MINE; m++) { next[m] = own[m]; }
+            for(int m = 0; m < MINE; m++) { next[m] = share.own[m]; }
             #pragma unroll
             for(int t = 0; t < STATE; t++) {
                 #pragma unroll
-                for(int m = 0; m < MINE; m++) { next[m] = multiply(move[m][t], state[t], next[m]); }
+                for(int m = 0; m < MINE; m++) { next[m] = multiply(share.move[m][t], state[t], next[m]); }
             }
         }
         // (own shares have been read: the state goes in their place)
+        float *const to = a.segmentStates + (first + (uint64_t)n * a.heads) * DK * a.padded + column;
         #pragma unroll
         for(int t = 0; t < STATE; t++) {
             if((uint32_t)t / MINE != wave) { continue; }
             #pragma unroll
             for(int r = 0; r < 4; r++) { to[rowIn(t, 4 * g + r) * a.padded] = state[t][r]; }
         }
-        if(n + 1 == segments) { break; }
-        if(n + 2 < segments) { request(n + 1); }
+        if(n + 1 == segments) { return; }
         __syncthreads();
         #pragma unroll
         for(int m = 0; m < MINE; m++) { found[wave * MINE + m][lane] = next[m]; }
         __syncthreads();
         #pragma unroll
         for(int t = 0; t < STATE; t++) { state[t] = found[t][lane]; }
+    };
+    if(segments > 1) { request(0, shares[0]); }
+    for(uint32_t n = 0; n < segments; n += 2) {
+        join(n, shares[0], shares[1]);
+        if(n + 1 < segments) { join(n + 1, shares[1], shares[0]); }
     }
 }
 
@@ -712,10 +720,7 @@ struct DeltaGradientArgs
     float *states, *errors;         // the gradient of the state behind each chunk [DK][padded], dR [C][padded]
     float *shared;                  // where heads share keys: each one's gradients of unit queries and keys, [2][C][DK]
 };
-// ALONE: not more work-groups than compute units; each may have all registers of one.
-template<typename T, int C, int DK, bool ALONE>
-__global__ __launch_bounds__(WALK_THREADS, ALONE ? 1 : 2)
-void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
+template<typename T, int C, int DK, bool ALONE> __device__ __forceinline__ void walkBackwards(const DeltaArgs &a, const DeltaGradientArgs &d)
 {
     typedef WalkLayout<T, C, DK, true> L;
     constexpr int NP = planesOf<T>, TILES = C / 16, STATE = DK / 16, WAVES = WALK_THREADS / 64;
@@ -838,6 +843,16 @@ void deltaReverseKernel(DeltaArgs a, DeltaGradientArgs d)
         if(d.v.data) { storeResult<T, C>(rowsOf<T>(d.v, a.chunks, p) + (uint64_t)first * d.v.rowStride + head * a.values, d.v.rowStride, g, column, inside, count, du); }
     }
     if(d.initialState && active && begin == 0) { storeResult<float, DK>(d.initialState + ((uint64_t)p.sequence * a.heads + head) * a.keys * a.values, a.values, g, column, inside, a.keys, state); }
+}
+
+// Neither walk of a gradient needs the other: both at once, so that a compute unit has a work-group of each, and one works where the other waits.  8 sequences of 2048 rows x 16 heads of 128 x 128 in bf16:
+// one behind the other 530 us, both at once 396; 3 of 301 rows x 3 heads of 33 x 47 in fp32: 75, 47.  ALONE: not more work-groups in all than compute units; each may have all registers of one.
+template<typename T, int C, int DK, bool ALONE>
+__global__ __launch_bounds__(WALK_THREADS, ALONE ? 1 : 2)
+void deltaWalksKernel(DeltaArgs a, DeltaGradientArgs d)
+{
+    if(blockIdx.y == 0) { walkBackwards<T, C, DK, ALONE>(a, d); }
+    else { walkForwards<T, C, DK, WALK_KEEP, false>(a); }
 }
 
 // ---- gradients of a chunk, once the state in front of it, w, the gradient of the state behind it and dR are known
