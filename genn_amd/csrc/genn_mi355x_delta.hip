@@ -316,7 +316,7 @@ int gennmi_delta_rule_backward(const gennmi_delta_rule_t *rule, const gennmi_del
         if(!rule->sequences.count) { return (int)GENNMI_OK; }
         DeltaArgs a = deltaArgs(*rule, space, workspace, true);
         const auto fours = [&](const gennmi_rows_t &r) { return (uintptr_t)r.data % (4 * size) == 0 && r.rowStride % 4 == 0 && r.sequenceStride % 4 == 0; };
-        a.wideValues = rule->values % 4 == 0 && fours(rule->v) && fours(in.out);
+        a.wideValues = rule->values % 4 == 0 && fours(in.out);
         DeltaGradientArgs d{};
         d.out = in.out; d.q = in.q; d.k = in.k; d.v = in.v; d.g = in.g; d.beta = in.beta;
         d.finalState = in.finalState; d.initialState = in.initialState;

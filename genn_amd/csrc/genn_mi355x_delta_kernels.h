@@ -862,8 +862,9 @@ void deltaWalksKernel(DeltaArgs a, DeltaGradientArgs d)
 //   dq^ = scale G (dout S') + sum_j dQK[i][j] k^[j],   dQK[i][j] = scale D[i][j] dout[i].u[j] for i >= j
 //   dk^ = beta (D[last] w dS' - G dR S') + sum_i dQK[i][j] q^[i] + sum_j (dKK + dKK')[i][j] k^[j],   dKK[i][j] = -D[i][j] beta[i] beta[j] dR[i].w[j] for i > j
 //   dbeta[i] = w[i].dR[i]
-// and g's: with states and u in units of the decay so far, outputs grow with it and values shrink, so that what the sum of g up to row i gains the loss
-// is q^[i].dq^[i] - v[i].dv[i], and at the chunk's last row the state behind it times its gradient as well.
+// and g[t]'s is what of the loss carries the decay of row t, term by term, so that it vanishes with that decay and no two large numbers cancel:
+//   dg[t] = sum_{i>=t} (q^[i].scale G dout S' - k^[i].beta G dR S')[i] + sum_{i>=t>j} (dQK[i][j] q^[i].k^[j] + dKK[i][j] k^[i].k^[j])
+//           + sum_{j<t} k^[j].beta D[last] w dS'[j] + G[last] S.dS
 // A work-group has a chunk and a head.  Products are summed over the values, 32 at a time, with what multiplies S and dS
 // in LDS; a wavefront has the results' columns of a quarter of the keys, S' and dS' straight from memory.  What bounds it is waiting, for memory and at barriers: two work-groups
 // of four wavefronts fit a compute unit and fill each other's pauses.  256 chunks x 16 heads of 128 x 128 in bf16: 400 to 440 us, some 1.2 GB (3 TB/s).  Where heads share keys, what each finds for them is left for deltaSharedKernel to add up.
@@ -871,7 +872,8 @@ template<typename T, int C, int DK> struct GradientLayout
 {
     static constexpr int NP = planesOf<T>;
     static constexpr uint32_t keys = 0, queries = keys + NP * C * DK, stage = queries + NP * C * DK, staged = (NP + 6) * C * 32, square = 3 * C * C,
-        floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (6 + 2 * 4) + 32;
+        floats = stage + (staged > square ? staged : square), bytes = floats * 2 + C * 8 + C * 4 * (5 + 2 * 4) + 4 * 256 + 32;
+    static_assert((staged > square ? staged : square) * 2 >= 4 * (C * (C + 1) + 256), "");          // (the crossings and their columns' sums lie there as well)
 };
 
 template<typename T, int C, int DK>
@@ -884,8 +886,8 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     uint16_t *const planes = (uint16_t*)lds, *const stage = planes + L::stage;
     uint16_t *const doutPlanes = stage, *const dRPlanes = stage + NP * VP, *const wPlanes = dRPlanes + 3 * VP;
     double *const sums = (double*)(planes + L::floats);
-    float *const since = (float*)(sums + C), *const until = since + C, *const beta = until + C, *const keyUnit = beta + C, *const queryUnit = keyUnit + C, *const valueDots = queryUnit + C;
-    float *const queryDots = valueDots + C, *const keyDots = queryDots + 4 * C, *const ends = keyDots + 4 * C;
+    float *const since = (float*)(sums + C), *const until = since + C, *const beta = until + C, *const keyUnit = beta + C, *const queryUnit = keyUnit + C;
+    float *const queryDots = queryUnit + C, *const keyDots = queryDots + 4 * C, *const crossingDots = keyDots + 4 * C, *const ends = crossingDots + 256;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     const uint32_t number = blockIdx.x / a.heads, head = blockIdx.x - number * a.heads, keyHead = head / a.group;
     const uint64_t at = (uint64_t)number * a.heads + head;
@@ -911,10 +913,10 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     const float *const stateRows = a.states + at * DK * a.padded, *const dStateRows = d.states + at * DK * a.padded;
     typedef Pack<T, 4> Four;
     f32x4 inDR[ITEMS], inW[ITEMS];
-    Four inDout[ITEMS], inValues[ITEMS];
+    Four inDout[ITEMS];
     const auto rowOfItem = [&](int i) { return tid / 8 + 32 * i; };
     const uint32_t stageAt = tid % 8 * 4;
-    const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)begin * d.out.rowStride + head * a.values, *const values = rowsOf<const T>(a.v, a.chunks, p) + (uint64_t)begin * a.v.rowStride + head * a.values;
+    const T *const douts = rowsOf<const T>(d.out, a.chunks, p) + (uint64_t)begin * d.out.rowStride + head * a.values;
     const auto request = [&](uint32_t v) {
         #pragma unroll
         for(int i = 0; i < ITEMS; i++) {
@@ -928,7 +930,6 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             for(int i = 0; i < ITEMS; i++) {
                 const uint64_t row = min(rowOfItem(i), count - 1);
                 inDout[i] = *(const Four*)(douts + row * d.out.rowStride + there);
-                inValues[i] = *(const Four*)(values + row * a.v.rowStride + there);
             }
         }
         else {
@@ -939,7 +940,6 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
                 for(int e = 0; e < 4; e++) {
                     const uint32_t there = v + stageAt + e < a.values ? v + stageAt + e : 0;
                     inDout[i].v[e] = douts[row * d.out.rowStride + there];
-                    inValues[i].v[e] = values[row * a.v.rowStride + there];
                 }
             }
         }
@@ -982,7 +982,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
     }
     #pragma unroll
     for(int q = 0; q < SQUARES; q++) { dqk[q] = dkk[q] = f32x4{0, 0, 0, 0}; }
-    float stateDot = 0.0f, valueDot[ITEMS] = {}, betaDot[ITEMS] = {};
+    float stateDot = 0.0f, betaDot[ITEMS] = {};
     for(uint32_t v = 0; v < a.padded; v += 32) {
         request(v);
         f32x4 s0[MINE][2], ds[MINE][2];
@@ -1005,7 +1005,6 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
                 dr[e] = row ? inDR[i][e] : 0.0f;
                 w[e] = row ? inW[i][e] : 0.0f;
                 dout[e] = there ? widen(inDout[i].v[e]) : 0.0f;
-                valueDot[i] = __builtin_fmaf(there ? widen(inValues[i].v[e]) : 0.0f, dr[e], valueDot[i]);
                 betaDot[i] = __builtin_fmaf(w[e], dr[e], betaDot[i]);
             }
             uint2 words[3], own[NP];
@@ -1052,20 +1051,23 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         }
         inTurn();
     }
-    // what the rows' factors make of them
-    float endDot = 0.0f;
+    // what the rows' factors make of them; for the gates, what each row has of the state in front and what it leaves in the state behind (where the lengths' gradients find place afterwards)
     #pragma unroll
     for(int t = 0; t < TILES; t++) {
-        const f32x4 grown = fourRows(since, t), by = fourRows(beta, t), last = fourRows(until, t) * by, keyLength = fourRows(keyUnit, t);
+        const f32x4 grown = fourRows(since, t), by = fourRows(beta, t), last = fourRows(until, t) * by, keyLength = fourRows(keyUnit, t), queryLength = fourRows(queryUnit, t);
+        f32x4 front = {0, 0, 0, 0}, end = {0, 0, 0, 0};
         #pragma unroll
         for(int m = 0; m < MINE; m++) {
-            const f32x4 k = valuesAt(L::keys, t, m) * keyLength;
+            const f32x4 k = valuesAt(L::keys, t, m) * keyLength, back = grown * by * rS[m][t];
             dq[m][t] *= a.scale * grown;
             dk[m][t] *= last;
-            #pragma unroll
-            for(int r = 0; r < 4; r++) { endDot = __builtin_fmaf(k[r], dk[m][t][r], endDot); }
-            dk[m][t] -= grown * by * rS[m][t];
+            front += valuesAt(L::queries, t, m) * queryLength * dq[m][t] - k * back;
+            end += k * dk[m][t];
+            dk[m][t] -= back;
         }
+        #pragma unroll
+        for(int r = 0; r < 4; r++) { front[r] = sumOf16(front[r]); end[r] = sumOf16(end[r]); }
+        if(n16 == 0) { *(f32x4*)(queryDots + wave * C + t * 16 + 4 * g) = front; *(f32x4*)(keyDots + wave * C + t * 16 + 4 * g) = end; }
     }
     {
         const uint32_t column = squareColumn * 16 + n16;
@@ -1084,18 +1086,83 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
         }
     }
     #pragma unroll
-    for(int w = 1; w < 64; w *= 2) { stateDot += __shfl_xor(stateDot, w); endDot += __shfl_xor(endDot, w); }
-    if(lane == 0) { ends[wave] = decay * stateDot + endDot; }
+    for(int w = 1; w < 64; w *= 2) { stateDot += __shfl_xor(stateDot, w); }
+    if(lane == 0) { ends[wave] = decay * stateDot; }
     #pragma unroll
     for(int i = 0; i < ITEMS; i++) {
         const uint32_t row = rowOfItem(i);
-        valueDot[i] += partner<1>(valueDot[i]); valueDot[i] += partner<2>(valueDot[i]); valueDot[i] += partner<4>(valueDot[i]);
         betaDot[i] += partner<1>(betaDot[i]); betaDot[i] += partner<2>(betaDot[i]); betaDot[i] += partner<4>(betaDot[i]);
-        if(stageAt == 0) {
-            valueDots[row] = valueDot[i] * beta[row];
-            if(d.beta.data && row < count) { (rowsOf<float>(d.beta, a.chunks, p) + (uint64_t)(begin + row) * d.beta.rowStride)[head] = betaDot[i]; }
+        if(stageAt == 0 && d.beta.data && row < count) { (rowsOf<float>(d.beta, a.chunks, p) + (uint64_t)(begin + row) * d.beta.rowStride)[head] = betaDot[i]; }
+    }
+
+    __syncthreads();
+    if(d.g.data) {
+        // crossings[i][j], i > j: what goes from row j to row i.  Sums over the rows from t on of each column, first of a part of the rows, then over the columns before t.
+        constexpr int PARTS = 256 / C, EACH = C / PARTS, PITCH = C + 1;
+        float *const crossings = (float*)stage, *const columnSums = crossings + C * PITCH;
+        #pragma unroll
+        for(int q = 0; q < SQUARES; q++) {
+            if(squareRow(q) < squareColumn) { continue; }
+            const uint32_t column = squareColumn * 16 + n16;
+            f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+            #pragma unroll
+            for(int s = 0; s < DK / 32; s++) {
+                inTurn();
+                const uint32_t rows = unitAt<DK>(squareRow(q) * 16 + n16, 4 * s + g);
+                const Planes<NP> columns = fetch<NP>(planes + L::keys + unitAt<DK>(column, 4 * s + g), C * DK);
+                kk = multiply(fetch<NP>(planes + L::keys + rows, C * DK), columns, kk);
+                qk = multiply(fetch<NP>(planes + L::queries + rows, C * DK), columns, qk);
+            }
+            const float length = keyUnit[column];
+            const f32x4 x = (dqk[q] * (fourRows(queryUnit, squareRow(q)) * qk) + dkk[q] * (fourRows(keyUnit, squareRow(q)) * kk)) * length;
+            #pragma unroll
+            for(int r = 0; r < 4; r++) {
+                const uint32_t row = squareRow(q) * 16 + 4 * g + r;
+                crossings[row * PITCH + column] = row > column ? x[r] : 0.0f;
+            }
+        }
+        __syncthreads();
+        const uint32_t of = tid % C, part = tid / C;
+        float below = 0.0f;
+        #pragma unroll
+        for(int i = EACH - 1; i >= 0; i--) {
+            const uint32_t row = part * EACH + i;
+            if(row <= of) { break; }
+            crossings[row * PITCH + of] = below += crossings[row * PITCH + of];
+        }
+        columnSums[part * C + of] = below;
+        __syncthreads();
+        float across = 0.0f;
+        #pragma unroll
+        for(int i = 0; i < EACH; i++) {
+            const uint32_t column = part * EACH + i;
+            if(column >= of) { break; }
+            float sum = crossings[of * PITCH + column];
+            for(uint32_t behind = of / EACH + 1; behind < PARTS; behind++) { sum += columnSums[behind * C + column]; }
+            across += sum;
+        }
+        crossingDots[part * C + of] = across;
+        __syncthreads();
+        if(wave == 0) {
+            double front = 0.0, end = 0.0, sum = 0.0;
+            if(lane < C) {
+                #pragma unroll
+                for(int w = 0; w < 4; w++) { front += queryDots[w * C + lane]; end += keyDots[w * C + lane]; sum += ends[w]; }
+                #pragma unroll
+                for(int w = 0; w < PARTS; w++) { sum += crossingDots[w * C + lane]; }
+            }
+            #pragma unroll
+            for(int w = 1; w < C; w *= 2) {
+                const double behind = __shfl_down(front, w), before = __shfl_up(end, w);
+                if(lane + w < C) { front += behind; }
+                if(lane >= (uint32_t)w) { end += before; }
+            }
+            const double before = __shfl_up(end, 1);
+            if(lane > 0) { sum += before; }
+            if(lane < count) { (rowsOf<float>(d.g, a.chunks, p) + (uint64_t)(begin + lane) * d.g.rowStride)[head] = (float)(sum + front); }
         }
     }
+    if(!d.q.data && !d.k.data) { return; }
 
     // squares times queries and keys
     const auto storeSquares = [&](bool transposed, const f32x4 (&square)[SQUARES], const float *rowFactor, const float *columnFactor) {
@@ -1140,41 +1207,23 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             }
         }
     };
-    __syncthreads();
     storeSquares(false, dqk, nullptr, keyUnit);
     __syncthreads();
     timesColumns(L::keys, dq, true, false);
-    // q^.dq^, for the gates and for the queries' lengths
-    #pragma unroll
-    for(int t = 0; t < TILES; t++) {
-        const f32x4 queryLength = fourRows(queryUnit, t);
-        f32x4 dot = {0, 0, 0, 0};
+    // q^.dq^, for the queries' lengths
+    if(a.normalise && a.group == 1) {
         #pragma unroll
-        for(int m = 0; m < MINE; m++) { dot += valuesAt(L::queries, t, m) * queryLength * dq[m][t]; }
-        #pragma unroll
-        for(int r = 0; r < 4; r++) { dot[r] = sumOf16(dot[r]); }
-        if(n16 == 0) { *(f32x4*)(queryDots + wave * C + t * 16 + 4 * g) = dot; }
+        for(int t = 0; t < TILES; t++) {
+            const f32x4 queryLength = fourRows(queryUnit, t);
+            f32x4 dot = {0, 0, 0, 0};
+            #pragma unroll
+            for(int m = 0; m < MINE; m++) { dot += valuesAt(L::queries, t, m) * queryLength * dq[m][t]; }
+            #pragma unroll
+            for(int r = 0; r < 4; r++) { dot[r] = sumOf16(dot[r]); }
+            if(n16 == 0) { *(f32x4*)(queryDots + wave * C + t * 16 + 4 * g) = dot; }
+        }
     }
     __syncthreads();
-    if(d.g.data && wave == 0) {
-        double sum = 0.0;
-        if(lane < C) {
-            sum = -(double)valueDots[lane];
-            #pragma unroll
-            for(int w = 0; w < 4; w++) { sum += queryDots[w * C + lane]; }
-            if(lane == C - 1) {
-                #pragma unroll
-                for(int w = 0; w < 4; w++) { sum += ends[w]; }
-            }
-        }
-        #pragma unroll
-        for(int w = 1; w < C; w *= 2) {
-            const double behind = __shfl_down(sum, w);
-            if(lane + w < C) { sum += behind; }
-        }
-        if(lane < count) { (rowsOf<float>(d.g, a.chunks, p) + (uint64_t)(begin + lane) * d.g.rowStride)[head] = (float)sum; }
-    }
-    if(!d.q.data && !d.k.data) { return; }
     storeSquares(true, dqk, queryUnit, nullptr);
     __syncthreads();
     timesColumns(L::queries, dk, false, true);
