@@ -15,7 +15,8 @@ namespace
 {
 // ---- layer norm
 // A row lies in the registers of the lanes that share it: 16 or 64 of a wavefront, or several wavefronts, each with 8 or 16 elements of it, so that it is read once and its
-// statistics are those of its elements as they are: first the mean, then the squares of what is left.  Where wavefronts share a row, each finds both for its own part, and the parts are joined
+// statistics are those of its elements as they are: first the mean, then what is left of the elements, its squares and its own mean, which is what the first mean was rounded by: of rows far from zero
+// (1000 and a spread of 0.01, say) steps of a mean in fp32 are as large as what is left.  Where wavefronts share a row, each finds these for its own part, and the parts are joined
 // (Chan, Golub, LeVeque: sum of squares = sum over parts of their own and of count (mean of the part - mean)^2): one barrier a row instead of two.
 struct NormArgs
 {
@@ -44,9 +45,9 @@ template<int LANES> __device__ inline float sumOfLanes(float x)
     if(LANES != 16) { x += partner<16>(x); x += partner<32>(x); }
     return x;
 }
-// Two sums a row over its wavefronts; two places in LDS are used in turn, so that one barrier does
+// What a row's wavefronts found; two places in LDS are used in turn, so that one barrier does
 constexpr int NORM_APART = 1024;        // a lane's sums in LDS, in elements: a constant costs no register a place
-struct NormShared { float2 found[2][16]; };
+struct NormShared { float4 found[2][16]; };
 
 template<typename T, int E, int VEC> struct NormRow { Pack<T, VEC> part[E / VEC]; };
 template<typename T, int E, int VEC> __device__ inline NormRow<T, E, VEC> requestRow(const T *row, const NormPlace &at, uint32_t channels, bool valid)
@@ -114,37 +115,56 @@ template<int E, int VEC> __device__ inline float elementsOf(const NormPlace &at,
 // x becomes x'; what it is divided by is returned as a factor
 template<int LANES, int E, int VEC> __device__ inline float normalise(const NormArgs &a, float (&x)[E], const NormPlace &at, NormShared &shared, uint32_t &turn, float inWave, float inWaveShare)
 {
-    float sum = 0.0f, square = 0.0f, mean = 0.0f;
-    if(!a.rms) {
+    float left = 0.0f, square = 0.0f, mean = 0.0f;
+    const float share = LANES ? a.share : inWaveShare;
+    if(a.rms) {
+        #pragma unroll
+        for(int e = 0; e < E; e++) { square = __builtin_fmaf(x[e], x[e], square); }
+    }
+    else {
+        float sum = 0.0f;
         #pragma unroll
         for(int e = 0; e < E; e++) { sum += x[e]; }
-        sum = sumOfLanes<LANES>(sum);
-        mean = sum * (LANES ? a.share : inWaveShare);
-    }
-    #pragma unroll
-    for(int e = 0; e < E; e++) {
-        const float d = hasElement<E, VEC>(at, e, a.channels) ? x[e] - mean : 0.0f;
-        square = __builtin_fmaf(d, d, square);
+        mean = sumOfLanes<LANES>(sum) * share;
+        #pragma unroll
+        for(int i = 0; i < E; i += VEC) {
+            if(!hasElement<E, VEC>(at, i, a.channels)) { continue; }
+            #pragma unroll
+            for(int e = i; e < i + VEC; e++) {
+                x[e] -= mean;
+                square = __builtin_fmaf(x[e], x[e], square);
+                left += x[e];
+            }
+        }
     }
     square = sumOfLanes<LANES>(square);
-    if constexpr(LANES == 0) {
-        const uint32_t waves = at.lanes >> 6, first = at.group * waves, mine = threadIdx.x >> 6;
-        if((threadIdx.x & 63) == 0) { shared.found[turn][mine] = make_float2(sum, square); }
+    float off = 0.0f;               // of what is left
+    if(!a.rms) {
+        left = sumOfLanes<LANES>(left);
+        off = left * share;
+        square = __builtin_fmaf(-left, off, square);
+    }
+    if(LANES == 0 && at.lanes > 64) {
+        const uint32_t waves = at.lanes >> 6, first = at.group * waves, mine = threadIdx.x >> 6, other = threadIdx.x & 15;
+        if((threadIdx.x & 63) == 0) { shared.found[turn][mine] = make_float4(mean, square, off, inWave); }
         __syncthreads();
-        sum = square = 0.0f;
-        for(uint32_t w = 0; w < waves; w++) { const float2 f = shared.found[turn][first + w]; sum += f.x; square += f.y; }
-        if(!a.rms) {
-            mean = sum * a.share;
-            for(uint32_t w = 0; w < waves; w++) {
-                const float n = elementsOf<E, VEC>(at, w, a.channels), off = n > 0.0f ? shared.found[turn][first + w].x / n - mean : 0.0f;
-                square = __builtin_fmaf(n * off, off, square);
-            }
+        // (a lane of each 16 has one wavefront's)
+        const float4 f = other < waves ? shared.found[turn][first + other] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if(a.rms) { square = sumOfLanes<16>(f.y); }
+        else {
+            const float whole = sumOfLanes<16>(f.w * f.x) * a.share, o = f.x - whole + f.z;
+            const float all = sumOfLanes<16>(f.w * o);
+            square = __builtin_fmaf(-all, all * a.share, sumOfLanes<16>(__builtin_fmaf(f.w * o, o, f.y)));
+            // (x is without this wavefront's mean, not the row's)
+            off = all * a.share - (mean - whole);
         }
         turn ^= 1;
     }
+    if(square < 0.0f) { square = 0.0f; }        // (what was taken off twice is as large as all of it)
     const float r = 1.0f / sqrtf(__builtin_fmaf(square, a.share, a.epsilon));
+    // (of elements behind the last channel something is left: their weights and what comes in for them are zero, and nothing of them is stored)
     #pragma unroll
-    for(int e = 0; e < E; e++) { x[e] = hasElement<E, VEC>(at, e, a.channels) ? (x[e] - mean) * r : 0.0f; }
+    for(int e = 0; e < E; e++) { x[e] = (x[e] - off) * r; }
     return r;
 }
 // (the hardware's exponential and reciprocal: a few steps of fp32; a division and an exponential to the last bit were a third of the instructions of a gated row)
@@ -277,10 +297,10 @@ void normBackwardKernel(NormArgs a)
         mean = sumOfLanes<LANES>(mean);
         if constexpr(LANES == 0) {
             const uint32_t waves = at.lanes >> 6;
-            if((threadIdx.x & 63) == 0) { shared.found[turn][threadIdx.x >> 6] = make_float2(along, mean); }
+            if((threadIdx.x & 63) == 0) { shared.found[turn][threadIdx.x >> 6] = make_float4(along, mean, 0.0f, 0.0f); }
             __syncthreads();
             along = mean = 0.0f;
-            for(uint32_t w = 0; w < waves; w++) { const float2 f = shared.found[turn][at.group * waves + w]; along += f.x; mean += f.y; }
+            for(uint32_t w = 0; w < waves; w++) { const float4 f = shared.found[turn][at.group * waves + w]; along += f.x; mean += f.y; }
             turn ^= 1;
         }
         along *= a.share;
