@@ -342,7 +342,7 @@ template<typename T, int C, int DK, bool QUERIES> struct WalkStage
     {
         const float f[4] = {x[0], x[1], x[2], x[3]};
         uint2 words[3];
-        splitFour<3>(f, words);
+        splitFour<3, (planesOf<T> > 1)>(f, words);
         const uint32_t column = Triangle<C>::column(item);
         to += Triangle<C>::at(Triangle<C>::row(item), column / 8) + column % 8;
         #pragma unroll
@@ -539,7 +539,7 @@ template<typename T, int C, int DK, int MODE, bool FOLDED> __device__ __forceinl
             Planes<NP> rows[ROWS];
             #pragma unroll
             for(int t = 0; t < ROWS; t++) { rows[t] = operand.rows(planes + (t < TILES ? L::keys : L::queries), t % TILES, s); }
-            multiplyAll(rows, split<3>(state[2 * s], state[2 * s + 1]), x);
+            multiplyAll(rows, split<3, (NP > 1)>(state[2 * s], state[2 * s + 1]), x);
         }
         inTurn();
         takeResult(values, inside, w);
@@ -621,7 +621,7 @@ template<typename T, int C, int DK, int MODE, bool FOLDED> __device__ __forceinl
             Planes<NP> columns[STATE];
             #pragma unroll
             for(int t = 0; t < STATE; t++) { columns[t] = operand.columns(planes + L::keys, t, s); }
-            multiplyAll(columns, split<3>(left[0], left[1]), state);
+            multiplyAll(columns, split<3, (NP > 1)>(left[0], left[1]), state);
         }
         inTurn();
         requestSquares();
@@ -641,8 +641,9 @@ template<typename T, int C, int DK, int MODE, bool FOLDED> __device__ __forceinl
     }
 }
 
+// (what segments of two planes do to a state fits the registers of three work-groups a compute unit, with two registers less than the compiler takes by itself: 33 sequences of 8011 rows in fp16 195 us, with two 216)
 template<typename T, int C, int DK, int MODE, bool FOLDED>
-__global__ __launch_bounds__(WALK_THREADS, 2)
+__global__ __launch_bounds__(WALK_THREADS, MODE == WALK_SUMMARY && planesOf<T> == 2 ? 3 : 2)
 void deltaStateKernel(DeltaArgs a) { walkForwards<T, C, DK, MODE, FOLDED>(a); }
 
 // From what each segment does: the state in front of each, in place of its own share: S = move S + own in fp32.  A work-group has 16 columns; its four wavefronts share the rows of
@@ -782,7 +783,7 @@ template<typename T, int C, int DK, bool ALONE> __device__ __forceinline__ void 
             Planes<NP> rows[TILES];
             #pragma unroll
             for(int t = 0; t < TILES; t++) { rows[t] = operand.rows(planes + L::keys, t, s); }
-            multiplyAll(rows, split<3>(state[2 * s], state[2 * s + 1]), du);
+            multiplyAll(rows, split<3, (NP > 1)>(state[2 * s], state[2 * s + 1]), du);
         }
         inTurn();
         takeResult(douts, inside, dout);
@@ -838,7 +839,7 @@ template<typename T, int C, int DK, bool ALONE> __device__ __forceinline__ void 
                 Planes<NP> columns[STATE];
                 #pragma unroll
                 for(int t = 0; t < STATE; t++) { columns[t] = operand.columns(planes + (which ? L::keys : L::queries), t, s); }
-                multiplyAll(columns, which ? split<3>(y[0], y[1]) : split<3>(x[0], x[1]), state);
+                multiplyAll(columns, which ? split<3, (NP > 1)>(y[0], y[1]) : split<3, (NP > 1)>(x[0], x[1]), state);
             }
         }
         inTurn();
@@ -1039,7 +1040,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
                 #pragma unroll
                 for(int e = 0; e < 4; e++) { stateDot = __builtin_fmaf(s0[m][h][e], ds[m][h][e], stateDot); }
             }
-            const Planes<3> state = split<3>(s0[m][0], s0[m][1]), dState = split<3>(ds[m][0], ds[m][1]);
+            const Planes<3> state = split<3, (NP > 1)>(s0[m][0], s0[m][1]), dState = split<3, (NP > 1)>(ds[m][0], ds[m][1]);
             #pragma unroll
             for(int t = 0; t < TILES; t++) {
                 inTurn();
@@ -1172,7 +1173,7 @@ void deltaGradientKernel(DeltaArgs a, DeltaGradientArgs d)
             const f32x4 scaled = square[q] * (rowFactor ? fourRows(rowFactor, squareRow(q)) : f32x4{1, 1, 1, 1} * columnFactor[column]);
             const float x[4] = {scaled[0], scaled[1], scaled[2], scaled[3]};
             uint2 words[3];
-            splitFour<3>(x, words);
+            splitFour<3, (NP > 1)>(x, words);
             #pragma unroll
             for(int k = 0; k < 3; k++) {
                 uint16_t *const to = stage + k * C * C;

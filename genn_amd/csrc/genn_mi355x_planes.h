@@ -1,7 +1,10 @@
 // Part of libgenn_mi355x.so: matrix products of fp32 accuracy on the bf16 matrix instructions.
 //
-// A float is a sum of three bf16 values without a rest, its upper 8 bits of mantissa, the next 8 and the last 8 ("planes").  Of the nine products of
-// two such sums the six whose planes' numbers add up to 2 at most are taken; the others are below 2^-24 of the whole.  A bf16 input is one plane, an fp16
+// A float is a sum of three bf16 values without a rest ("planes").  Of the nine products of two such sums the six whose planes' numbers add up to 2 at most are taken.  What the others are
+// depends on how the planes were cut.  Rounded to the nearest, they leave at most 2^-8 and 2^-17 of the float's power of two, of either sign: the others are together 2^-24 of the product of the powers of two at most.
+// Cut off, they leave up to 2^-7 and 2^-15, of the float's sign: 2^-21, and always too little, which does not average out.  So in every product of three planes by more than one an operand
+// is rounded: 2^-24 if both are (or the other one is an fp16 input), 3 x 2^-24 if the other one is cut off, of either sign.  Where the other one is a single plane nothing is left out, and cutting off takes
+// fewer cycles (prompts of 4096 rows x 32 heads in bf16: 217.5 us so, 223.5 with all rounded).  Rounded floats from 2^128 - 2^119 on count as an overflow.  A bf16 input is one plane, an fp16
 // input two, so that most products take three to five instructions: 16 x 16 x 32 in 16 cycles each, where the same on the fp32 matrix
 // instructions takes eight of 32.
 #ifndef GENN_MI355X_PLANES_H
@@ -25,38 +28,46 @@ template<> constexpr int planesOf<bf16> = 1;
 template<int N> struct Planes { union { uint32_t word[4]; bf16x8 v; } plane[N]; };
 
 // Takes the upper plane of a pair of values off them: its bits, the first value's below
-__device__ inline uint32_t takePlane(float &a, float &b)
+template<bool ROUNDED> __device__ inline uint32_t takePlane(float &a, float &b)
 {
+    if constexpr(ROUNDED) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        const uint32_t plane = __builtin_bit_cast(uint32_t, bf16x2{(bf16)a, (bf16)b});
+        a -= __uint_as_float(plane << 16);
+        b -= __uint_as_float(plane & 0xffff0000u);
+        return plane;
+    }
     const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
     a -= __uint_as_float(x & 0xffff0000u);
     b -= __uint_as_float(y & 0xffff0000u);
     return __builtin_amdgcn_perm(y, x, 0x07060302u);
 }
-// (the last plane: nothing of the values is needed after it)
+// (the last plane: what is left has no more bits than a bf16, and nothing of it is needed afterwards)
 __device__ inline uint32_t lastPlane(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
-template<int N> __device__ inline void splitPair(float a, float b, uint32_t (&words)[N])
+// (two planes hold an fp16 input without a rest, rounded or not)
+template<int N, bool ROUNDED> __device__ inline void splitPair(float a, float b, uint32_t (&words)[N])
 {
     #pragma unroll
-    for(int p = 0; p < N; p++) { words[p] = p + 1 < N ? takePlane(a, b) : lastPlane(a, b); }
+    for(int p = 0; p < N; p++) { words[p] = p + 1 < N ? takePlane<ROUNDED>(a, b) : lastPlane(a, b); }
 }
 // Four values, N planes of 8 bytes
-template<int N> __device__ inline void splitFour(const float (&x)[4], uint2 (&out)[N])
+template<int N, bool ROUNDED = N == 3> __device__ inline void splitFour(const float (&x)[4], uint2 (&out)[N])
 {
     uint32_t low[N], high[N];
-    splitPair<N>(x[0], x[1], low);
-    splitPair<N>(x[2], x[3], high);
+    splitPair<N, ROUNDED>(x[0], x[1], low);
+    splitPair<N, ROUNDED>(x[2], x[3], high);
     #pragma unroll
     for(int p = 0; p < N; p++) { out[p] = make_uint2(low[p], high[p]); }
 }
 // Eight values of one lane, four of each of two tiles of a result, which become an operand: see rowIn()
-template<int N> __device__ inline Planes<N> split(const f32x4 &a, const f32x4 &b)
+template<int N, bool ROUNDED = N == 3> __device__ inline Planes<N> split(const f32x4 &a, const f32x4 &b)
 {
     Planes<N> out;
     const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     #pragma unroll
     for(int i = 0; i < 4; i++) {
         uint32_t words[N];
-        splitPair<N>(x[2 * i], x[2 * i + 1], words);
+        splitPair<N, ROUNDED>(x[2 * i], x[2 * i + 1], words);
         #pragma unroll
         for(int p = 0; p < N; p++) { out.plane[p].word[i] = words[p]; }
     }

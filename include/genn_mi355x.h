@@ -668,9 +668,9 @@ int gennmi_selective_scan_backward(const gennmi_scan_t *scan, const gennmi_scan_
 /* Gated delta rule: every head keeps a matrix that maps keys to values, lets it decay, and corrects it by what it gets wrong for the row's key.
  * With k' and q' the row's key and query of the head, divided by sqrt(sum of squares + epsilon) each with `normalise`:
  *   S[t] = a S[t - 1] + k' (x) beta[t] (v[t] - a S[t - 1]^T k'),   a = exp(g[t]),   out[t] = scale * S[t]^T q'
- * heads / keyHeads neighbouring heads share a key head's keys and queries.  States and sums in fp32 (products as sums of bf16 products that lose nothing of it), one rounding at the end.
+ * heads / keyHeads neighbouring heads share a key head's keys and queries.  States and sums in fp32 (products as sums of bf16 products, less what is below half a step of fp32), one rounding at the end.
  * Long sequences are taken in chunks of up to 64 rows: where g > 0 for long, the growth over a chunk has to stay below 2^128.  A g below -1e6 counts as that.
- * What an infinite input or state, one that is not a number, or an overflow gives: outputs before its row are as without it, and its own value's column of outputs and states (keys, g, beta: all of
+ * What an infinite input or state, one that is not a number, or an overflow (from 2^128 - 2^119 on) gives: outputs before its row are as without it, and its own value's column of outputs and states (keys, g, beta: all of
  * the head's) is not finite from its row on; in gradients it may reach the whole sequence's head.  One row per sequence (a token of every running
  * sequence) takes a kernel of its own, without a workspace. */
 #define GENNMI_MAX_DELTA_KEYS 128
