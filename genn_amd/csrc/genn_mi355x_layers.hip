@@ -167,8 +167,21 @@ template<int LANES, int E, int VEC> __device__ inline float normalise(const Norm
     for(int e = 0; e < E; e++) { x[e] = (x[e] - off) * r; }
     return r;
 }
-// (the hardware's exponential and reciprocal: a few steps of fp32; a division and an exponential to the last bit were a third of the instructions of a gated row)
-__device__ inline float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+// s = sigmoid(z) and 1 - s.  For results in 16 bits the hardware's exponential of a rounded product (off by |z| / 2 half steps of fp32) and its reciprocal are more than enough; a division and an exponential to
+// the last bit were a third of the instructions of a gated row.  For fp32: of u = exp(-|z|) <= 1, a power of two and a rest below one half whose product with log2(e) has two parts, s or 1 - s is 1 / (1 + u) and
+// the other u / (1 + u): both are within a few half steps of themselves.
+struct Logistic { float s, rest; };
+template<typename T> __device__ inline Logistic logistic(float z)
+{
+    if constexpr(sizeof(T) < 4) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+        return Logistic{s, 1.0f - s};
+    }
+    // (from 200 on u is 0; a z that is no number is one in what s is multiplied with)
+    const float m = fminf(fabsf(z), 200.0f), whole = rintf(m * -1.44269502f), part = __builtin_fmaf(m, -1.925963e-8f, __builtin_fmaf(m, -1.44269502f, -whole));
+    const float u = __builtin_ldexpf(__builtin_amdgcn_exp2f(part), (int)whole), large = __builtin_amdgcn_rcpf(1.0f + u), small = u * large;
+    return z < 0.0f ? Logistic{small, large} : Logistic{large, small};
+}
 
 // Bound by memory: each row is read once and written once.  Work-groups of 256 threads where 16 lanes or a wavefront have a row, else of what rows take; each walks rows that are a grid apart,
 // with the parameters in registers and the next row asked for while one is worked on.  4096 x 4096 in bf16: 62 us with a row a work-group (its parameters are four times the row), 15.7 so (4.3 TB/s);
@@ -207,7 +220,7 @@ void normKernel(NormArgs a)
         #pragma unroll
         for(int e = 0; e < E; e++) {
             x[e] = __builtin_fmaf(x[e], weight[e], bias[e]);
-            if constexpr(GATE) { x[e] *= z[e] * logistic(z[e]); }
+            if constexpr(GATE) { x[e] *= z[e] * logistic<T>(z[e]).s; }
         }
         if(n < a.rows) {
             const uint32_t sequence = (uint32_t)n / a.length, row = (uint32_t)n - sequence * a.length;
@@ -263,17 +276,45 @@ void normBackwardKernel(NormArgs a)
         const float r = normalise<LANES, E, VEC>(a, x, at, shared, turn, inWave, inWaveShare);
         if constexpr(GATE) {
             if constexpr(BIAS_AGAIN) { loadParameters<E, VEC>(a.bias, 0.0f, at, a.channels, bias); }
-            if constexpr(LARGE) { gate = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
-            float z[E];
-            takeRow(gate, z);
-            #pragma unroll
-            for(int e = 0; e < E; e++) {
-                if(LARGE && e % 4 == 0) { __builtin_amdgcn_sched_barrier(0); }
-                const float s = logistic(z[e]), y = __builtin_fmaf(x[e], weight[e], bias[e]), dz = d[e] * y * (s * __builtin_fmaf(z[e], 1.0f - s, 1.0f));
-                d[e] *= z[e] * s;
-                z[e] = dz;
+            // the gate's element becomes its gradient
+            const auto pass = [&](int e, float &z) {
+                const Logistic l = logistic<T>(z);
+                const float y = __builtin_fmaf(x[e], weight[e], bias[e]), dz = d[e] * y * (l.s * __builtin_fmaf(z, l.rest, 1.0f));
+                d[e] *= z * l.s;
+                z = dz;
+            };
+            if constexpr(LARGE && sizeof(T) == 4) {
+                // (no registers for a whole row of it and what fp32 takes for each: four elements at a time)
+                const T *const from = normRow<const T>(a.gate, sequence, row);
+                T *const to = normRow<T>(a.dgate, sequence, row);
+                #pragma unroll
+                for(int i = 0; i < E; i += 4) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    Pack<T, VEC> z[4 / VEC];
+                    #pragma unroll
+                    for(int k = 0; k < 4; k += VEC) {
+                        z[k / VEC] = Pack<T, VEC>{};
+                        if(valid && hasElement<E, VEC>(at, i + k, a.channels)) { z[k / VEC] = *(const Pack<T, VEC>*)(from + ((i + k) / VEC * at.lanes + at.lane) * VEC); }
+                    }
+                    #pragma unroll
+                    for(int k = 0; k < 4; k++) { pass(i + k, z[k / VEC].v[k % VEC]); }
+                    #pragma unroll
+                    for(int k = 0; k < 4; k += VEC) {
+                        if(a.dgate.data && valid && hasElement<E, VEC>(at, i + k, a.channels)) { *(Pack<T, VEC>*)(to + ((i + k) / VEC * at.lanes + at.lane) * VEC) = z[k / VEC]; }
+                    }
+                }
             }
-            if(a.dgate.data && valid) { storeRow<T, E, VEC>(normRow<T>(a.dgate, sequence, row), at, a.channels, z); }
+            else {
+                if constexpr(LARGE) { gate = requestRow<T, E, VEC>(normRow<const T>(a.gate, sequence, row), at, a.channels, valid); }
+                float z[E];
+                takeRow(gate, z);
+                #pragma unroll
+                for(int e = 0; e < E; e++) {
+                    if(LARGE && e % 4 == 0) { __builtin_amdgcn_sched_barrier(0); }
+                    pass(e, z[e]);
+                }
+                if(a.dgate.data && valid) { storeRow<T, E, VEC>(normRow<T>(a.dgate, sequence, row), at, a.channels, z); }
+            }
         }
         // (of a row that is not there d is zero)
         float along = 0.0f, mean = 0.0f;

@@ -1,4 +1,4 @@
-"""Layer norm where a row's statistics are hard: rows far from zero, gates at their ends, more rows than work-groups.
+"""Layer norm where a row's statistics are hard: rows far from zero, gates far from it and at their ends, more rows than work-groups.
 
 Tolerances, in half steps of fp32 (2^-24), of operations as test_gpu_layers.py counts them (64 for a row's sum and what follows).  A row's mean is found, then the mean of what is left of it: the first
 is off by at most 64 of them of the mean size of the elements, what is left by half a step of itself, and the second mean by 64 of the mean size of what is left.  So x - mean is off by
@@ -96,6 +96,31 @@ def test_more_rows_than_work_groups_take_at_once(rows, channels, dtype):
         if gate is not None:
             off = (dz.cpu().double() - found["dgate"]).abs() - (torch.finfo(T).eps / 2 * found["dgate"].abs() + 2 * OPERATIONS * STEP * sizes["dgate"] * (1 + torch.finfo(T).eps) + least)
             assert (off <= 0).all()
+
+
+def test_gates_far_from_zero():
+    """Rows of which x' is 1 exactly (all elements 1, rms, no epsilon), so that out is the gate's own z sigmoid(z).
+
+    Steps of fp32 relative to it: the exponential one step (2 x 2^-24) and half a step of its argument, which is below one half; the sum with 1, a reciprocal of one step, and two
+    products: 1 + 2 + 1/2 x 1/2 + 2 + 2, counted as 8 x 2^-24; and one rounding less than that for each of the products of the slope, s (1 + z (1 - s)), that adds up terms of either sign."""
+    from genn_amd.sequence import LayerNorm
+    z = torch.cat([torch.linspace(-80, 80, 4001), torch.linspace(-3, 3, 1000), torch.tensor([0.0, -0.0, -1.2784645])])
+    n = z.numel()
+    z, x = z.repeat_interleave(8).view(n, 8), torch.ones(n, 8)
+    out, dz, dout = torch.zeros(n, 8).cuda(), torch.zeros(n, 8).cuda(), torch.full((n, 8), 0.7)
+    op = LayerNorm(1, n, 8, epsilon=0.0, rms=True)
+    op.bind(x=x.cuda(), gate=z.cuda(), out=out)
+    op.run()
+    op.bind_gradients(out=dout.cuda(), gate=dz)
+    op.backward()
+    z = z.double()
+    s = torch.sigmoid(z)
+    want = z * s
+    off = (out.cpu().double() - want).abs() / (want.abs() + 2.0 ** -126)
+    assert (off <= 8 * STEP).all(), (float(z.reshape(-1)[int(off.argmax())]), float(off.max() / STEP))
+    want, size = dout.double() * s * (1 + z * torch.sigmoid(-z)), dout.double() * s * (1 + z.abs() * torch.sigmoid(-z))
+    off = (dz.cpu().double() - want).abs() / size
+    assert (off <= 16 * STEP).all(), (float(z.reshape(-1)[int(off.argmax())]), float(off.max() / STEP))
 
 
 @pytest.mark.parametrize("gate", [False, True])
