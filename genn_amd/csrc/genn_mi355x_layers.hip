@@ -470,7 +470,8 @@ struct NormPlan { uint32_t each, lanes, rowLanes, groups, threads, blocks; };   
 // Rows of up to 128 channels: 16 lanes with 8 elements each; of up to 512: a wavefront.  Above that wavefronts share a row in the forward pass, 16 elements a lane; gradients of up to 1024 channels
 // (2048 without a gate) stay with one wavefront, whose rows need no barrier, as long as its registers hold four arrays of them.  us in bf16: 16384 x 2048 a wavefront a row
 // and two, forward 32, 28, gradients 50, 62; gradients of 16384 x 1024 29, 35, of 8192 x 2048 with a gate 67, 48.
-// Work-groups: as many as the chip holds at once, or a quarter of the rows where that is less, as each leaves a sum for every channel.
+// Work-groups: as many as the chip holds at once, or a quarter of the rows where that is less, as each leaves a sum for every channel; more, where a lane would add up more than 256 rows in fp32 (and a
+// work-group its up to 16 lanes' behind that; work-groups' sums are added up in 64 bits).
 NormPlan normPlan(const gennmi_layer_norm_t &c, bool gradients)
 {
     const uint64_t rows = totalRows(c.sequences);
@@ -482,7 +483,7 @@ NormPlan normPlan(const gennmi_layer_norm_t &c, bool gradients)
     p.groups = p.lanes ? 256 / p.lanes : std::max(1u, (gradients ? 512 : 256) / p.rowLanes);
     p.threads = p.groups * p.rowLanes;
     const uint64_t needed = (rows + p.groups - 1) / p.groups, most = gradients ? (p.each == 8 && (p.lanes || !gate) ? 768 : 512) : p.lanes ? 2048 : 1024;
-    p.blocks = (uint32_t)std::min<uint64_t>(gradients ? (needed + 3) / 4 : needed, most);
+    p.blocks = (uint32_t)std::min<uint64_t>(gradients ? (needed + 3) / 4 : needed, gradients ? std::max(most, std::min((needed + 255) / 256, mostBlocks(p.threads))) : most);
     return p;
 }
 template<bool GRADIENTS, int VEC, typename F> int withNormLayout(const NormPlan &p, F &&f)

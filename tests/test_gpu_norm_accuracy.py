@@ -1,4 +1,4 @@
-"""Layer norm where a row's statistics are hard: rows far from zero, gates far from it and at their ends, more rows than work-groups.
+"""Layer norm where a row's statistics are hard: rows far from zero, gates far from it and at their ends, more rows than work-groups, very many for one weight.
 
 Tolerances, in half steps of fp32 (2^-24), of operations as test_gpu_layers.py counts them (64 for a row's sum and what follows).  A row's mean is found, then the mean of what is left of it: the first
 is off by at most 64 of them of the mean size of the elements, what is left by half a step of itself, and the second mean by 64 of the mean size of what is left.  So x - mean is off by
@@ -139,3 +139,19 @@ def test_gates_and_rows_at_their_ends(gate):
             assert torch.all(got == 1.0)
             continue
         assert got[0] == math.inf and torch.isnan(got[1]) and torch.isnan(got[2]) and got[3] == float(z.to(T)[3]) and got[4] == 0.0 and got[5] == 200.0 and got[6].abs() < 1e-37 and got[7] == 0.0
+
+
+def test_weights_of_very_many_rows():
+    """A lane adds up at most 256 rows in 32 bits and a work-group 16 lanes' behind that, each addition off by at most half a step of the sum; then 64 bits.  Equal values of one sign lose most."""
+    from genn_amd.sequence import LayerNorm
+    rows = 64_000_000
+    value = 0.901
+    x = torch.zeros(rows, 1, device="cuda")
+    d = torch.full((rows, 1), value, device="cuda")
+    db = torch.zeros(1, device="cuda")
+    op = LayerNorm(1, rows, 1)
+    op.bind(x=x)
+    op.bind_gradients(out=d, bias=db)
+    op.backward()
+    want = rows * float(torch.tensor(value).double())
+    assert abs(float(db.double()) - want) <= want * STEP * (1 + 256 + 16), (float(db), want)
