@@ -395,6 +395,7 @@ class Dropout(_SequenceOperator):
     def __init__(self, sequences, length, channels, probability, seed=0, dtype="float32", device=0):
         super().__init__(sequences, length, dtype, device)
         self.channels, self.probability, self.seed = _count(channels, "channels"), float(probability), int(seed)
+        self._numbers, self._captured = {}, []          # numbers on the device that are kept alive: the last one of each direction and stream, those of captured calls
         if not 0.0 <= self.probability <= 1.0:
             raise ValueError(f"probability is between 0 and 1, not {probability}")
         if not 0 <= self.seed < 1 << 64:
@@ -419,30 +420,39 @@ class Dropout(_SequenceOperator):
         self._backward = self._descriptor_of(given, out, x, None, ("the gradient of out", "the gradient of x", ""))
         self._gradients = given
 
-    def _call(self, d, call, stream):
+    def _call(self, which, call, stream):
+        d = _abi.Dropout.from_buffer_copy(getattr(self, which))         # (of this call alone: other threads may call with other numbers)
         if isinstance(call, Integral):          # (numpy's numbers are that too)
             if not 0 <= call < 1 << 64:
                 raise ValueError("call has 64 bits")
-            d.call, d.callDevice, self._value = int(call), None, None
+            d.call = int(call)
         else:
             o = Operand(call, "call").wants(("uint64", "int64"))
             if any(n != 1 for n in o.shape):
                 raise ValueError("call is one value")
             same_device([o], self.device)
-            d.call, d.callDevice, self._value = 0, o.address, o          # (kept alive until the next call)
-        rc = self._lib.gennmi_dropout(C.byref(d), stream)
+            d.callDevice = o.address
+            capturing = _int()
+            if stream:
+                _abi.check(self._lib.gennmi_stream_is_capturing(stream, _byref(capturing)))
+            if not capturing.value:
+                self._numbers[which, stream] = o
+            elif all(k.address != o.address for k in self._captured):
+                self._captured.append(o)
+        rc = self._lib.gennmi_dropout(_byref(d), stream)
         if rc:
             _abi.check(rc)
 
     def run(self, call, stream=0):
-        """``call``: a number, or an int64 or uint64 array of one element on the device that is read when the call runs (a captured call goes on reading it)."""
+        """``call``: a number, or an int64 or uint64 array of one element on the device that is read when the call runs.  It has to live until then; the object itself keeps
+        those of captured calls, which go on reading them, and the last one of every stream."""
         self._need(self._bound, "bind()")
-        self._call(self._forward, call, stream)
+        self._call("_forward", call, stream)
 
     def backward(self, call, stream=0):
         """``call``: that of ``run``."""
         self._need(self._gradients, "bind_gradients()")
-        self._call(self._backward, call, stream)
+        self._call("_backward", call, stream)
 
 
 # (`C` names an array of the scan)
