@@ -161,15 +161,19 @@ template<int LANES, int E, int VEC> __device__ inline float normalise(const Norm
         turn ^= 1;
     }
     if(square < 0.0f) { square = 0.0f; }        // (what was taken off twice is as large as all of it)
-    const float r = 1.0f / sqrtf(__builtin_fmaf(square, a.share, a.epsilon));
+    // (a root and a division, and what both were rounded by: r is in all elements of the row)
+    const float variance = __builtin_fmaf(square, a.share, a.epsilon);
+    float r = 1.0f / sqrtf(variance);
+    const float one = variance * r, less = __builtin_fmaf(-one, r, 1.0f) - __builtin_fmaf(variance, r, -one) * r;
+    if(fabsf(less) < 1.0f) { r = __builtin_fmaf(0.5f * r, less, r); }
     // (of elements behind the last channel something is left: their weights and what comes in for them are zero, and nothing of them is stored)
     #pragma unroll
     for(int e = 0; e < E; e++) { x[e] = (x[e] - off) * r; }
     return r;
 }
 // s = sigmoid(z) and 1 - s.  For results in 16 bits the hardware's exponential of a rounded product (off by |z| / 2 half steps of fp32) and its reciprocal are more than enough; a division and an exponential to
-// the last bit were a third of the instructions of a gated row.  For fp32: of u = exp(-|z|) <= 1, a power of two and a rest below one half whose product with log2(e) has two parts, s or 1 - s is 1 / (1 + u) and
-// the other u / (1 + u): both are within a few half steps of themselves.
+// the last bit were a third of the instructions of a gated row.  For fp32: of u = exp(-z), a power of two and a rest below one half whose product with log2(e) has two parts, s is 1 / (1 + u) and 1 - s is
+// u / (1 + u): both are within a few half steps of themselves.
 struct Logistic { float s, rest; };
 template<typename T> __device__ inline Logistic logistic(float z)
 {
@@ -177,10 +181,10 @@ template<typename T> __device__ inline Logistic logistic(float z)
         const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
         return Logistic{s, 1.0f - s};
     }
-    // (from 200 on u is 0; a z that is no number is one in what s is multiplied with)
-    const float m = fminf(fabsf(z), 200.0f), whole = rintf(m * -1.44269502f), part = __builtin_fmaf(m, -1.925963e-8f, __builtin_fmaf(m, -1.44269502f, -whole));
-    const float u = __builtin_ldexpf(__builtin_amdgcn_exp2f(part), (int)whole), large = __builtin_amdgcn_rcpf(1.0f + u), small = u * large;
-    return z < 0.0f ? Logistic{small, large} : Logistic{large, small};
+    // (behind 200 u is 0 or infinite; a z that is no number is one in what s is multiplied with)
+    const float m = fmaxf(fminf(z, 200.0f), -200.0f), whole = rintf(m * -1.44269502f), part = __builtin_fmaf(m, -1.925963e-8f, __builtin_fmaf(m, -1.44269502f, -whole));
+    const float u = __builtin_ldexpf(__builtin_amdgcn_exp2f(part), (int)whole), s = __builtin_amdgcn_rcpf(1.0f + u);
+    return Logistic{s, fminf(u * s, 1.0f)};         // (1 where u is infinite)
 }
 
 // Bound by memory: each row is read once and written once.  Work-groups of 256 threads where 16 lanes or a wavefront have a row, else of what rows take; each walks rows that are a grid apart,
@@ -367,11 +371,21 @@ void normBackwardKernel(NormArgs a)
             for(int e = 0; e < E; e++) { rows[e * blockDim.x + threadIdx.x] = sum[e]; }
             __syncthreads();
             if(at.group) { continue; }
+            // (in 64 bits: in 32 their roundings were as much of the result's error as all of the rows')
             #pragma unroll 1
-            for(uint32_t k = 1; k < at.groups; k++) {
+            for(int e = 0; e < E; e += 4) {
+                double whole[4];
                 #pragma unroll
-                for(int e = 0; e < E; e++) { sum[e] += rows[e * blockDim.x + k * at.lanes + at.lane]; }
+                for(int i = 0; i < 4; i++) { whole[i] = rows[(e + i) * blockDim.x + at.lane]; }
+                for(uint32_t k = 1; k < at.groups; k++) {
+                    #pragma unroll
+                    for(int i = 0; i < 4; i++) { whole[i] += rows[(e + i) * blockDim.x + k * at.lanes + at.lane]; }
+                }
+                #pragma unroll
+                for(int i = 0; i < 4; i++) { rows[(e + i) * blockDim.x + at.lane] = (float)whole[i]; }
             }
+            #pragma unroll
+            for(int e = 0; e < E; e++) { sum[e] = rows[e * blockDim.x + at.lane]; }
         }
         if constexpr(!LARGE) {
             #pragma unroll
@@ -470,8 +484,8 @@ struct NormPlan { uint32_t each, lanes, rowLanes, groups, threads, blocks; };   
 // Rows of up to 128 channels: 16 lanes with 8 elements each; of up to 512: a wavefront.  Above that wavefronts share a row in the forward pass, 16 elements a lane; gradients of up to 1024 channels
 // (2048 without a gate) stay with one wavefront, whose rows need no barrier, as long as its registers hold four arrays of them.  us in bf16: 16384 x 2048 a wavefront a row
 // and two, forward 32, 28, gradients 50, 62; gradients of 16384 x 1024 29, 35, of 8192 x 2048 with a gate 67, 48.
-// Work-groups: as many as the chip holds at once, or a quarter of the rows where that is less, as each leaves a sum for every channel; more, where a lane would add up more than 256 rows in fp32 (and a
-// work-group its up to 16 lanes' behind that; work-groups' sums are added up in 64 bits).
+// Work-groups: as many as the chip holds at once, or a quarter of the rows where that is less, as each leaves a sum for every channel; more, where a lane would add up more than 256 rows in fp32 (what its
+// lanes and the work-groups found is added up in 64 bits).
 NormPlan normPlan(const gennmi_layer_norm_t &c, bool gradients)
 {
     const uint64_t rows = totalRows(c.sequences);
