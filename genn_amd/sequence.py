@@ -7,6 +7,7 @@ As a model's arrays are handed to its runner once and stepped many times, an ope
 ``stream`` is the address of a HIP stream; 0, the default, is the null stream.  A call while another device than the operator's is current is refused.
 """
 import ctypes as C
+import threading
 from numbers import Integral
 
 from . import _abi
@@ -30,7 +31,8 @@ class _SequenceOperator:
         _abi.check(self._lib.gennmi_init(device))
         self._bound = self._gradients = None        # operands (kept alive) of the descriptors
         self._packed = self._bound_packed = None    # rows of packed arrays: of a call of bind(), and of the one that held
-        self._workspaces = {}           # (stream, which pass): one each, as calls on different streams may overlap
+        self._workspaces = {}           # (which pass, stream): one each, as calls on different streams may overlap
+        self._lock = threading.Lock()   # of them: two threads may make the first call on a stream at once
 
     def _operand(self, array, name, shape=None):
         return None if array is None else Operand(array, name, shape)
@@ -94,13 +96,14 @@ class _SequenceOperator:
             _abi.check(self._lib.gennmi_stream_is_capturing(stream, _byref(capturing)))
             if capturing.value:
                 raise ValueError("the stream is being captured: give the call a workspace of its own, which the graph then keeps using")
-        own = self._workspaces.get((key, stream))
-        if own is None or own.count < needed:
-            current_device(self._lib, self.device)
-            if own is not None:
-                own.free()
-            own = self._workspaces[key, stream] = Array(needed, "uint8", device_only=True)
-        return own.ptr, own.count
+        with self._lock:
+            own = self._workspaces.get((key, stream))
+            if own is None or own.count < needed:
+                current_device(self._lib, self.device)
+                if own is not None:
+                    own.free()
+                own = self._workspaces[key, stream] = Array(needed, "uint8", device_only=True)
+            return own.ptr, own.count
 
     def free(self):
         """Gives the operator's own workspaces back."""
