@@ -76,9 +76,11 @@ int deltaApart(const char *what, const gennmi_delta_rule_t &c, const gennmi_delt
 }
 
 // Segments that a sequence is cut into, so that there are work-groups for the whole chip: what each does to the state is found for all of them at once (the state's columns and
-// those of a unit matrix), then joined, then outputs are found for all of them at once.  The number is the one that should take the shortest, in units of a chunk's step of a walk alone on the chip (5.7 us):
+// those of a unit matrix), then joined, then outputs are found for all of them at once.  The number is the one that should take the shortest, in units of a chunk's step of a walk alone on the chip (5.7 us for 64 rows in bf16;
+// one unit for all types):
 // two work-groups fit a compute unit, and with all 512 a step takes 1.8 units; what a segment does takes 0.57 of that a step; a segment's join and what else comes with it 0.8 units.  One prompt of 64 chunks x 32 heads
-// in 1, 2, 4, 8, 16 segments: 375, 330, 223, 207, 237 us, x 8 heads 358, 314, 181, 125, 122; 33 sequences of 8011 rows in all x 6 heads (fp16) in 1, 2, 4, 8, 16: 261, 247, 184, 197, 206.
+// in 1, 2, 4, 8, 16 segments: 375, 330, 223, 207, 237 us, x 8 heads 358, 314, 181, 125, 122; 33 sequences of 8011 rows in all x 6 heads (fp16) in 1, 2, 4, 8, 16: 261, 247, 184, 197, 206
+// (the rule takes 5 there, as the steps of 32 rows are shorter than it has them).
 uint32_t segmentsOf(const gennmi_delta_rule_t &c, uint32_t columns)
 {
     const uint32_t C = chunkRows(c.type), chunks = (c.sequences.length + C - 1) / C;

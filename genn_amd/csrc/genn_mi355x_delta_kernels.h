@@ -76,7 +76,7 @@ template<typename T> __device__ inline const T *rowAt(const gennmi_rows_t &r, co
 // FOLDED: for outputs alone, -N beta and P beta (I - N beta) are left, which r is multiplied with at once; else, for gradients, -N and P.
 // (M and P lie where the keys and queries were)
 // What bounds it is waiting (three quarters of a wavefront's cycles): loads, then a triangle solved row by row by one wavefront.  Hence four work-groups a compute unit, whose pauses fill each other, at the price of 18 registers
-// that are spilled: 64 chunks x 32 heads of 128 keys in bf16 37 us, 256 x 16 for gradients 105 (170 MB written).
+// that are spilled: 64 chunks x 32 heads of 128 keys in bf16 39 us, 256 x 16 for gradients 108 (180 MB written).
 template<typename T, int C, int DK> constexpr uint32_t chunkSquares() { const uint32_t keys = 2 * planesOf<T> * C * DK * 2, squares = 2 * C * (C + 4) * 4; return keys > squares ? keys : squares; }
 template<typename T, int C, int DK> constexpr uint32_t chunkLds() { return chunkSquares<T, C, DK>() + C * (8 + 3 * 4) + 16; }
 
@@ -473,7 +473,8 @@ __device__ inline WalkPlace walkPlace(const DeltaArgs &a, uint32_t blocks)
 }
 
 // A work-group walks a sequence (or a segment of it) of one head with 16 columns of the state a wavefront.  What bounds it: a wavefront's five products of a chunk wait for each other (14,000 cycles alone on a SIMD,
-// of which matrix instructions 3,500), so that two work-groups share a compute unit.  One prompt of 64 chunks x 32 heads of 128 x 128 in bf16, in 8 segments: what they do to a state 87 us, outputs 76.
+// of which matrix instructions 3,500), and of as many vector instructions as take the same time (5.4 to 5.9 for each matrix instruction: most of them cut floats into planes, the same squares in every work-group of a head),
+// so that two work-groups share a compute unit.  One prompt of 64 chunks x 32 heads of 128 x 128 in bf16, in 8 segments: what they do to a state 92 us, outputs 79 (all 256 registers, 19 spilled, 65 scalars in lanes).
 template<typename T, int C, int DK, int MODE, bool FOLDED> __device__ __forceinline__ void walkForwards(const DeltaArgs &a)
 {
     constexpr bool OUTPUTS = MODE == WALK_OUTPUTS;
@@ -850,7 +851,8 @@ template<typename T, int C, int DK, bool ALONE> __device__ __forceinline__ void 
 }
 
 // Neither walk of a gradient needs the other: both at once, so that a compute unit has a work-group of each, and one works where the other waits.  8 sequences of 2048 rows x 16 heads of 128 x 128 in bf16:
-// one behind the other 530 us, both at once 396; 3 of 301 rows x 3 heads of 33 x 47 in fp32: 75, 47.  ALONE: not more work-groups in all than compute units; each may have all registers of one.
+// one behind the other 530 us, both at once 393 (1.4 GB moved, 3.6 TB/s: memory counts as much as the wait; over 500 scalars of the two walks' descriptors are kept in lanes: 7.9 vector instructions a matrix instruction);
+// 3 of 301 rows x 3 heads of 33 x 47 in fp32: 75, 48.  ALONE: not more work-groups in all than compute units; each may have all registers of one.
 template<typename T, int C, int DK, bool ALONE>
 __global__ __launch_bounds__(WALK_THREADS, ALONE ? 1 : 2)
 void deltaWalksKernel(DeltaArgs a, DeltaGradientArgs d)
@@ -868,7 +870,7 @@ void deltaWalksKernel(DeltaArgs a, DeltaGradientArgs d)
 //           + sum_{j<t} k^[j].beta D[last] w dS'[j] + G[last] S.dS
 // A work-group has a chunk and a head.  Products are summed over the values, 32 at a time, with what multiplies S and dS
 // in LDS; a wavefront has the results' columns of a quarter of the keys, S' and dS' straight from memory.  What bounds it is waiting, for memory and at barriers: two work-groups
-// of four wavefronts fit a compute unit and fill each other's pauses.  256 chunks x 16 heads of 128 x 128 in bf16: 400 to 440 us, some 1.2 GB (3 TB/s).  Where heads share keys, what each finds for them is left for deltaSharedKernel to add up.
+// of four wavefronts fit a compute unit and fill each other's pauses.  256 chunks x 16 heads of 128 x 128 in bf16: 447 us, some 1.15 GB (2.6 TB/s).  Sums over keys and within a chunk's square are in fp32 (each term of a gate's gradient carries its decay, so nothing is lost with it), over a chunk's rows in 64 bits.  Where heads share keys, what each finds for them is left for deltaSharedKernel to add up.
 template<typename T, int C, int DK> struct GradientLayout
 {
     static constexpr int NP = planesOf<T>;

@@ -188,8 +188,8 @@ template<typename T> __device__ inline Logistic logistic(float z)
 }
 
 // Bound by memory: each row is read once and written once.  Work-groups of 256 threads where 16 lanes or a wavefront have a row, else of what rows take; each walks rows that are a grid apart,
-// with the parameters in registers and the next row asked for while one is worked on.  4096 x 4096 in bf16: 62 us with a row a work-group (its parameters are four times the row), 15.7 so (4.3 TB/s);
-// 131,072 heads of 128 with a gate 20.7 (4.9 TB/s).
+// with the parameters in registers and the next row asked for while one is worked on.  4096 x 4096 in bf16: 62 us with a row a work-group (its parameters are four times the row), 13.9 so (4.8 TB/s);
+// 131,072 heads of 128 with a gate 20.5 (4.9 TB/s).
 template<typename T, int LANES, int E, int VEC, bool GATE>
 __global__ __launch_bounds__(LANES ? 256 : 1024)
 void normKernel(NormArgs a)
@@ -234,7 +234,7 @@ void normKernel(NormArgs a)
 }
 
 // With y = x' weight + bias, s the gate's factor z sigmoid(z) and d = dout s:
-// Bound by memory: 16384 x 2048 in bf16 50 us with the closing sums (4.0 TB/s), 134 with a row's sums over its work-group one behind another.
+// Bound by memory: 16384 x 2048 in bf16 51 us with the closing sums (3.9 TB/s), 134 with a row's sums over its work-group one behind another.
 //   dgate = dout y s',  dweight += d x',  dbias += d,  dx = (v - x' mean(v x') - mean(v)) / length, v = d weight (without the last mean for `rms`)
 template<typename T, int LANES, int E, int VEC, bool GATE>
 __global__ __launch_bounds__(LANES ? 256 : 1024)
@@ -403,8 +403,9 @@ struct DropoutArgs
     uint32_t k0, k1, items, groups, length, channels, dropped;
     float factor;
 };
-// Bound by memory: a thread has eight neighbouring elements and draws once for them, 16 bits each (ten rounds of two wide products and four
-// exclusive ors; a draw for four would take longer than the memory).  16384 x 2048 in bf16 onto a residual: 37.6 us, 5.4 TB/s, vector units 96 % busy.
+// A thread has eight neighbouring elements and draws once for them, 16 bits each (ten rounds of two wide products and four exclusive ors; a draw for four would take longer than the memory).
+// Arrays beyond the caches are bound by memory: 32768 x 16384 in bf16 onto a residual 532 us, 6.06 TB/s, which is what adding the two takes (534).  Of what the last cache holds the draws are the limit, with the
+// vector units 92 to 96 % busy: 16384 x 2048 31.3 us where adding takes 29.3; 38 with the arrays of other calls between.
 template<typename T, bool WIDE>
 __global__ __launch_bounds__(256)
 void dropoutKernel(DropoutArgs a)
@@ -483,7 +484,8 @@ uint32_t vectorOf(uint32_t size, uint32_t channels, std::initializer_list<const 
 struct NormPlan { uint32_t each, lanes, rowLanes, groups, threads, blocks; };       // lanes 0: wavefronts share a row, rowLanes of them
 // Rows of up to 128 channels: 16 lanes with 8 elements each; of up to 512: a wavefront.  Above that wavefronts share a row in the forward pass, 16 elements a lane; gradients of up to 1024 channels
 // (2048 without a gate) stay with one wavefront, whose rows need no barrier, as long as its registers hold four arrays of them.  us in bf16: 16384 x 2048 a wavefront a row
-// and two, forward 32, 28, gradients 50, 62; gradients of 16384 x 1024 29, 35, of 8192 x 2048 with a gate 67, 48.
+// and two, forward 32, 28, gradients 50, 62; gradients of 16384 x 1024 29, 35, of 8192 x 2048 with a gate 67, 48
+// (all of them before what the mean leaves was taken off: now forward 24, gradients 45, 27, 45 from the caches).
 // Work-groups: as many as the chip holds at once, or a quarter of the rows where that is less, as each leaves a sum for every channel; more, where a lane would add up more than 256 rows in fp32 (what its
 // lanes and the work-groups found is added up in 64 bits).
 NormPlan normPlan(const gennmi_layer_norm_t &c, bool gradients)

@@ -701,7 +701,8 @@ int gennmi_delta_rule_backward(const gennmi_delta_rule_t *rule, const gennmi_del
 
 /* Layer norm of every row:  x' = (x - mean) / sqrt(variance + epsilon), or with `rms` x / sqrt(mean of squares + epsilon),
  *   out = (x' * weight + bias) * gate * sigmoid(gate)
- * Rows within rows (the heads of a row, say) are sequences of as many rows.  Statistics in fp32, one rounding at the end.  Packed sequences and slots are not for this: rows do not depend on each other. */
+ * Rows within rows (the heads of a row, say) are sequences of as many rows.  Statistics in fp32 (squares of x - mean, or with `rms` of x, have to stay below 2^128), the mean of what the mean leaves
+ * taken off as well, one rounding at the end.  Sums of gradients of weight and bias: at most 256 rows in fp32, of those in 64 bits.  Packed sequences and slots are not for this: rows do not depend on each other. */
 #define GENNMI_MAX_NORM_CHANNELS 16384
 typedef struct gennmi_layer_norm_t {
     gennmi_sequences_t sequences;         /* count times length rows */
